@@ -26,6 +26,7 @@ enum lb_status : int {
 enum lb_dtype : int {
     LB_F32 = 0,
     LB_BF16 = 1,
+    LB_E4M3 = 2,      // 8-bit floats with one float32 scale a row (products with 4-bit weights and the norm that feeds them)
 };
 
 // Activations fused into a matrix product's epilogue.

@@ -1,0 +1,137 @@
+// 4-bit weights as the products read them (the layout: api.h, lb_weights4) and what their kernels share: nibbles to halves of a register,
+// 8-bit floats, and the epilogue.
+//
+// w[n, k] = q s r with q in -8 .. 7 (at most three significant bits), s in e4m3 (four) and r in 32 bits.  q, and q s as well (at most seven
+// significant bits), are bfloat16 and float16 numbers without rounding, and so are the activations (bfloat16 as they are, e4m3 as float16):
+// the tensor cores multiply exactly, sums are 32-bit, and r and the activations' scale a row meet the finished sum.
+#pragma once
+
+#include "api.h"
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace lb_w4 {
+
+constexpr int kTileRows = 16, kTileK = 128, kTileBytes = kTileRows * kTileK / 2;
+
+// The operand type of the tensor cores: bfloat16 activations go with bfloat16 weights, e4m3 ones with float16.
+struct Bf16 {
+    static constexpr bool kHalf = false;
+    // Nibbles (q + 8) in the low bits of both halves -> q: 0x4300 | u is 128 + u.
+    static __device__ __forceinline__ uint32_t weights(uint32_t u) {
+        const uint32_t v = u | 0x43004300u, c = 0x43084308u;
+        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&c));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
+};
+struct F16 {
+    static constexpr bool kHalf = true;
+    // 0x6400 | u is 1024 + u.
+    static __device__ __forceinline__ uint32_t weights(uint32_t u) {
+        const uint32_t v = u | 0x64006400u, c = 0x64086408u;
+        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
+};
+
+// Weights 2p and 2p + 1 of a word of eight, in the halves of a register.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(uint32_t word, int p) {
+    return T::weights((word >> (4 * p)) & 0x000F000Fu);
+}
+
+// Two e4m3 numbers (16 bits) -> float16.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+    uint32_t out;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(out) : "h"((uint16_t)two));
+    return out;
+}
+__device__ __forceinline__ float e4m3_to_float(uint32_t byte) {
+    const uint32_t v = e4m3x2_to_f16x2(byte & 0xffu);
+    return __low2float(*reinterpret_cast<const __half2*>(&v));
+}
+// Two floats -> e4m3, rounded to the nearest even, values beyond 448 to 448; `lo` in the low byte.
+__device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
+    uint16_t out;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(out) : "f"(hi), "f"(lo));
+    return out;
+}
+
+// The accumulator's 16 x 8 tile += weights (rows) x activations (columns).
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (T::kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight activations of a row from column k on as four registers of two, zeros past K.  `wide`: rows are aligned so that eight come by one load.
+template <typename T>
+__device__ __forceinline__ void load_eight(uint32_t (&v)[4], const void* a, int64_t row_at, int k, int K, bool wide) {
+    if constexpr (T::kHalf) {
+        const uint8_t* p = static_cast<const uint8_t*>(a) + row_at;
+        uint32_t lo = 0, hi = 0;
+        if (wide && k + 8 <= K) {
+            const uint2 two = *reinterpret_cast<const uint2*>(p + k);
+            lo = two.x;
+            hi = two.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (k + i < K) lo |= (uint32_t)p[k + i] << (8 * i);
+                if (k + 4 + i < K) hi |= (uint32_t)p[k + 4 + i] << (8 * i);
+            }
+        }
+        v[0] = e4m3x2_to_f16x2(lo & 0xffffu);
+        v[1] = e4m3x2_to_f16x2(lo >> 16);
+        v[2] = e4m3x2_to_f16x2(hi & 0xffffu);
+        v[3] = e4m3x2_to_f16x2(hi >> 16);
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a) + row_at;
+        if (wide && k + 8 <= K) {
+            const uint4 four = *reinterpret_cast<const uint4*>(p + k);
+            v[0] = four.x;
+            v[1] = four.y;
+            v[2] = four.z;
+            v[3] = four.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = k + 2 * i < K ? p[k + 2 * i] : 0u, hi = k + 2 * i + 1 < K ? p[k + 2 * i + 1] : 0u;
+                v[i] = lo | hi << 16;
+            }
+        }
+    }
+}
+
+// What happens to a finished sum.  Of paired weights a feature's two sums (already times r and the activations' scale) become one value.
+struct Epilogue {
+    const float* a_scale;        // [M] or null
+    const float* bias;           // [n] or null
+    const float* residual;
+    void* out;
+    int64_t ldr, ldo;
+    int M, n;                    // n: columns of out
+    int act, gate;               // gate: only of paired weights
+    float alpha, limit;
+    bool out_f32;
+};
+
+__device__ __forceinline__ void store_out(const Epilogue& e, int m, int col, float v) {
+    if (e.out_f32) static_cast<float*>(e.out)[(int64_t)m * e.ldo + col] = v;
+    else static_cast<__nv_bfloat16*>(e.out)[(int64_t)m * e.ldo + col] = __float2bfloat16_rn(v);
+}
+
+// Order as the other products': bias, activation, residual.
+__device__ __forceinline__ void finish_one(const Epilogue& e, const lb_act_pair& pair, int m, int col, float v) {
+    if (e.bias != nullptr) v += __ldg(e.bias + col);
+    v = lb_activate(v, e.act, pair);
+    if (e.residual != nullptr) v += e.residual[(int64_t)m * e.ldr + col];
+    store_out(e, m, col, v);
+}
+
+}  // namespace lb_w4

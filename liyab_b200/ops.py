@@ -1173,3 +1173,148 @@ def expert_plan(ids: torch.Tensor, n_experts: int):
     place, pair_at = (torch.full((n,), -7, dtype=i32, device=ids.device) for _ in range(2))
     check(lib().lb_expert_plan(_dev(ids, "ids", i32), n, n_experts, _dev(offsets, "offsets"), _dev(place, "place"), _dev(pair_at, "pair_at"), stream_ptr()), "expert_plan")
     return offsets, place, pair_at
+
+
+# ------------------------------------------------------------------ 4-bit weights and the norm that feeds their products
+
+E4M3 = 2
+_ROWS8 = torch.float8_e4m3fn
+
+
+class Weights4Args(ctypes.Structure):
+    _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _i), ("n_padded", _i), ("scale_stride", _i)]
+
+
+for _name, _args in {
+    "lb_weights4_sizes": [_i, _i, _i, _i, _p, _p, _p],
+    "lb_weights4_lay_out": [_p, _l, _p, _l, _p, _p, _p],
+    "lb_weights4_quantise": [_i, _p, _l, _p, _p],
+    "lb_weights4_values": [_p, _p, _l, _p],
+    "lb_linear4": [_p, _i, _p, _l, _p, _p, _p, _l, _i, _p, _l, _i, _i, _p],
+    "lb_gated4": [_p, _i, _p, _l, _p, _i, _p, _l, _i, _i, _f, _f, _p],
+    "lb_rms_add_rows": [_i, _p, _l, _i, _p, _l, _p, _l, _p, _f, _f, _i, _p, _l, _p, _i, _i, _p],
+}.items():
+    _SIGNATURES[_name] = _args
+
+
+class Weights4:
+    """A matrix w[n, k] = q[n, k] s[n, k / group] r[n] in 4 bits (q in -8 .. 7, s in e4m3, r float32) as the products read it.  `paired`: 2 f rows, the f of a gate
+    and the f of its other factor, for gated4.  The memory belongs to this object; made by quantise_weights4 or lay_out_weights4."""
+
+    __slots__ = ("n", "k", "group", "paired", "device", "nibbles", "scales", "rows", "args", "ref")
+
+    def __init__(self, n: int, k: int, group: int, paired: bool, device: torch.device):
+        nibbles, padded, stride = ctypes.c_int64(0), ctypes.c_int(0), ctypes.c_int(0)
+        check(lib().lb_weights4_sizes(n, k, group, int(paired), ctypes.byref(nibbles), ctypes.byref(padded), ctypes.byref(stride)), "weights4")
+        self.n, self.k, self.group, self.paired, self.device = n, k, group, paired, device
+        self.nibbles = torch.empty(nibbles.value, dtype=torch.uint8, device=device)
+        self.scales = torch.empty((padded.value, stride.value), dtype=torch.uint8, device=device)
+        self.rows = torch.empty(padded.value, dtype=torch.float32, device=device)
+        self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired), padded.value, stride.value)
+        self.ref = ctypes.addressof(self.args)
+
+    @property
+    def nbytes(self) -> int:
+        return self.nibbles.numel() + self.scales.numel() + 4 * self.rows.numel()
+
+
+def _matrix4(t: torch.Tensor, name: str, paired: bool) -> None:
+    if not t.is_cuda:
+        raise invalid_argument(f"{name} is on {t.device}; the engine's kernels run on a CUDA device only")
+    if t.dim() != 2 or t.stride(1) != 1 or (paired and t.shape[0] % 2):
+        raise invalid_argument(f"weights4: {name} has to be a matrix, dense within a row, with an even number of rows when paired")
+
+
+def quantise_weights4(w: torch.Tensor, group: int = 128, paired: bool = False) -> Weights4:
+    """The matrix w [n, k] (float32 or bfloat16) rounded to 4 bits: a group's scale is its largest value / 7 (in e4m3, times the row's float32 factor), q the nearest
+    integer.  `paired`: w is [2 f, k], gate rows first.  Returns when the weights are complete."""
+    _matrix4(w, "w", paired)
+    r = Weights4(w.shape[0], w.shape[1], group, paired, w.device)
+    check(lib().lb_weights4_quantise(_code(w.dtype, "w"), w.data_ptr(), w.stride(0), r.ref, stream_ptr()), "quantise_weights4")
+    return r
+
+
+def lay_out_weights4(q: torch.Tensor, scales: torch.Tensor, rows: torch.Tensor, group: int = 128, paired: bool = False) -> Weights4:
+    """Weights that are in 4 bits already: q int8 [n, k] (-8 .. 7), scales e4m3 [n, ceil(k / group)], rows float32 [n].  Returns when they are laid out."""
+    _matrix4(q, "q", paired)
+    n, k = q.shape
+    if q.dtype != torch.int8 or scales.dtype != _ROWS8 or tuple(scales.shape) != (n, -(-k // group)) or scales.stride(1) != 1 or rows.shape != (n,) or not rows.is_contiguous():
+        raise invalid_argument("weights4: q is int8 [n, k], scales e4m3 [n, ceil(k / group)] and rows float32 [n]")
+    r = Weights4(n, k, group, paired, q.device)
+    check(lib().lb_weights4_lay_out(q.data_ptr(), q.stride(0), _dev(scales, "scales"), scales.stride(0), _dev(rows, "rows", torch.float32), r.ref, stream_ptr()),
+          "lay_out_weights4")
+    return r
+
+
+def weights4_values(w: Weights4) -> torch.Tensor:
+    """The matrix [n, k] that the weights stand for, float32."""
+    out = torch.empty((w.n, w.k), dtype=torch.float32, device=w.device)
+    check(lib().lb_weights4_values(w.ref, out.data_ptr(), out.stride(0), stream_ptr()), "weights4_values")
+    return out
+
+
+def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n: int, a_scale: Optional[torch.Tensor]) -> tuple:
+    """What both products check of their rows; (type of a, a_scale's pointer, type of out)."""
+    if a.device != w.device or out.device != w.device:
+        raise invalid_argument(f"{what}: a is on {a.device} and out on {out.device}, the weights on {w.device}")
+    if a.dim() != 2 or out.dim() != 2 or a.shape[1] != w.k or out.shape[1] != n or not 0 <= m <= min(a.shape[0], out.shape[0]) or a.stride(1) != 1 or out.stride(1) != 1:
+        raise invalid_argument(f"{what}: shapes do not fit: a {tuple(a.shape)}, w ({w.n}, {w.k}), out {tuple(out.shape)}, {m} rows")
+    if a.dtype is _ROWS8:
+        if a_scale is None or a_scale.dtype != torch.float32 or a_scale.device != w.device or a_scale.dim() != 1 or a_scale.shape[0] < m or a_scale.stride(0) != 1:
+            raise invalid_argument(f"{what}: e4m3 activations come with a_scale, float32 [rows]")
+        return E4M3, a_scale.data_ptr(), _code(out.dtype, "out")
+    if a.dtype is not torch.bfloat16 or a_scale is not None:
+        raise invalid_argument(f"{what}: activations are bfloat16, or e4m3 with a_scale; a is {a.dtype}")
+    return BF16, None, _code(out.dtype, "out")
+
+
+def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: torch.Tensor, m: int, activation: str = "none",
+            residual: Optional[torch.Tensor] = None, a_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[:m] = act(a[:m] @ w.T + bias) + residual with 4-bit weights: a is bfloat16, or e4m3 with a_scale (a row of a times a_scale[row] is what it stands for);
+    out is bfloat16 or float32, bias and residual float32; out may be the residual."""
+    code, scale, out_code = _rows4("linear4", a, w, out, m, w.n, a_scale)
+    if residual is not None and (residual.dtype != torch.float32 or residual.device != w.device or residual.dim() != 2 or residual.shape[1] != w.n or residual.shape[0] < m or residual.stride(1) != 1):
+        raise invalid_argument("linear4: the residual is float32 rows of the output's width")
+    if bias is not None and (bias.dtype != torch.float32 or bias.device != w.device or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0)):
+        raise invalid_argument("linear4: the bias is float32, one number a feature")
+    check(lib().lb_linear4(w.ref, code, a.data_ptr(), a.stride(0), scale, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                           0 if residual is None else residual.stride(0), out_code, out.data_ptr(), out.stride(0), m, ACTIVATIONS[activation], stream_ptr()), "linear4")
+    return out
+
+
+def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = "silu", a_scale: Optional[torch.Tensor] = None, alpha: float = 0.0,
+           limit: float = 0.0) -> torch.Tensor:
+    """out[:m] = gate(a[:m] @ w_gate.T) * (a[:m] @ w_up.T) with paired 4-bit weights, one launch; activations as for linear4.  Gates: sigmoid, silu, gelu_tanh, relu,
+    capped (with alpha and limit, as gated_act_kind)."""
+    kind = GATE_KINDS.get(gate, 5)
+    if kind > 4:
+        raise invalid_argument(f"gated4: no gate {gate!r}")
+    code, scale, out_code = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
+    check(lib().lb_gated4(w.ref, code, a.data_ptr(), a.stride(0), scale, out_code, out.data_ptr(), out.stride(0), m, kind, alpha, limit, stream_ptr()), "gated4")
+    return out
+
+
+def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch.Tensor], eps: float, out: torch.Tensor, scale: Optional[torch.Tensor] = None,
+            total: Optional[torch.Tensor] = None, gain_offset: float = 0.0) -> torch.Tensor:
+    """t = x + delta (32 bits), left in `total` (x's type; None: back in x where there is a delta); out = t / sqrt(mean(t^2) + eps) * (gain_offset + gain), bfloat16, or e4m3
+    with scale (float32 [rows]): out * scale is the row, scale its largest |value| / 448.  x and delta are float32 or bfloat16."""
+    rows, width = x.shape
+    if total is None and delta is not None:
+        total = x
+    code = E4M3 if out.dtype is _ROWS8 else BF16 if out.dtype is torch.bfloat16 else -1
+    if code < 0 or (code == E4M3) != (scale is not None):
+        raise invalid_argument(f"rms_add: out is bfloat16, or e4m3 with a scale a row; it is {out.dtype}")
+    for t, name in ((x, "x"), (delta, "delta"), (out, "out"), (total, "total")):
+        if t is not None and (t.device != x.device or t.shape != x.shape or t.stride(1) != 1):
+            raise invalid_argument(f"rms_add: {name} has to be rows of x's shape, dense within a row and on x's device")
+    if total is not None and total.dtype != x.dtype:
+        raise invalid_argument(f"rms_add: total is {total.dtype}, x {x.dtype}")
+    if gain is not None and (gain.dtype != torch.float32 or gain.device != x.device or gain.shape != (width,) or not gain.is_contiguous()):
+        raise invalid_argument("rms_add: the gain is float32, one number a column")
+    if scale is not None and (scale.dtype != torch.float32 or scale.device != x.device or scale.shape != (rows,) or not scale.is_contiguous()):
+        raise invalid_argument("rms_add: the scales are float32, one number a row")
+    check(lib().lb_rms_add_rows(_code(x.dtype, "x"), _dev(x, "x"), x.stride(0), F32 if delta is None else _code(delta.dtype, "delta"),
+                           None if delta is None else delta.data_ptr(), 0 if delta is None else delta.stride(0), None if total is None else total.data_ptr(),
+                           0 if total is None else total.stride(0), None if gain is None else gain.data_ptr(), gain_offset, eps, code, out.data_ptr(), out.stride(0),
+                           None if scale is None else scale.data_ptr(), rows, width, stream_ptr()), "rms_add")
+    return out

@@ -1,0 +1,375 @@
+"""4-bit weights: their layout and rounding, the products that read them and the norm that feeds those, against plain forms in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_kernels_gpu import _rand, dev  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+F8 = torch.float8_e4m3fn
+
+
+def _parts(n, k, group, dev, seed=0):
+    """(q, s, r): every value of q and a wide range of scales, among them zeros."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8)
+    s = torch.rand((n, -(-k // group)), generator=g) * 448.0
+    s = torch.where(torch.rand(s.shape, generator=g) < 0.05, torch.zeros(()), s).to(F8)
+    r = torch.exp(torch.randn((n,), generator=g)) * 1e-4
+    return q.to(dev), s.to(dev), r.to(dev)
+
+
+def _matrix(q, s, r, group):
+    """The matrix in 64 bits."""
+    at = torch.arange(q.shape[1], device=q.device) // group
+    return q.double() * s.double()[:, at] * r.double()[:, None]
+
+
+def _rows8(a):
+    scale = a.float().abs().amax(1) / 448.0
+    return (a.float() / scale[:, None]).to(F8), scale
+
+
+def _sum_bound(k):
+    """Relative to the sum of the terms' sizes: the tensor core adds 16 products to a 32-bit sum at a time, each time with an error below 2^-23 of the larger of the two
+    (truncation); a group's scale, the parts' sums, the row's factor and scale, bias and residual add less than 16 further roundings."""
+    return (k / 16 + 16) * 2.0 ** -23
+
+
+SHAPES = [(1, 1, 32), (8, 31, 64), (16, 128, 128), (17, 129, 64), (100, 200, 32), (250, 1000, 128), (1600, 1600, 64), (1000, 4104, 128), (5003, 768, 128), (129, 16384, 32)]
+TOKENS = [1, 2, 7, 8, 9, 16, 17, 31, 64, 65, 130, 300]
+
+
+# ---- the weights -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,k,group", SHAPES)
+@pytest.mark.parametrize("paired", [False, True])
+def test_laid_out_and_back(dev, n, k, group, paired):
+    from liyab_b200 import ops
+    n = 2 * n if paired else n
+    q, s, r = _parts(n, k, group, dev)
+    w = ops.lay_out_weights4(q, s, r, group, paired)
+    at = torch.arange(k, device=dev) // group
+    assert torch.equal(ops.weights4_values(w), q.float() * s.float()[:, at] * r[:, None])       # q s is exact: one rounding on both sides
+
+
+@pytest.mark.parametrize("n,k,group", SHAPES)
+@pytest.mark.parametrize("paired", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rounded_to_four_bits(dev, n, k, group, paired, dtype):
+    """The same weights as the definition gives in 32-bit arithmetic on the CPU (whose divisions are rounded correctly, as the kernel's are)."""
+    from liyab_b200 import ops
+    n = 2 * n if paired else n
+    g = torch.Generator().manual_seed(n + k)
+    m = torch.randn((n, k + 3), generator=g) * torch.exp(torch.randn((n, 1), generator=g)) * 0.02
+    m[0] = 0.0
+    m[-1, : k // 2] *= 1e-7                                     # groups far below their row's largest
+    m = m.to(dtype)[:, :k]
+    groups = -(-k // group)
+    padded = torch.nn.functional.pad(m.float(), (0, groups * group - k)).view(n, groups, group)
+    t = padded.abs().amax(2) / torch.tensor(7.0)
+    r = t.amax(1) / torch.tensor(448.0)
+    s = torch.where(r[:, None] > 0, t / r[:, None], torch.zeros(())).clamp(max=448.0).to(F8)
+    step = s.float() * r[:, None]
+    q = torch.where(step[..., None] > 0, padded / step[..., None], torch.zeros(())).round().clamp(-8, 7)
+    want = (q * s.float()[..., None] * r[:, None, None]).reshape(n, -1)[:, :k]
+    w = ops.quantise_weights4(m.to(dev), group, paired)
+    assert torch.equal(ops.weights4_values(w).cpu(), want)
+
+
+def test_rounding_of_special_rows(dev):
+    """Rows of zeros and of numbers too small for a normal factor become zeros; an infinity or a NaN makes its row NaN and leaves the others alone."""
+    from liyab_b200 import ops
+    m = torch.randn((24, 256), generator=torch.Generator().manual_seed(3))
+    m[1], m[2], m[3, 7], m[4, 200], m[5] = 0.0, 1e-40, float("inf"), float("nan"), 1e30 * m[5]
+    got = ops.weights4_values(ops.quantise_weights4(m.to(dev), 64)).cpu()
+    assert (got[1:3] == 0).all() and got[3:5].isnan().all() and got[[0, *range(5, 24)]].isfinite().all()
+    # The nearest of steps of (largest / 7): half a step off, and a scale in e4m3 is up to 1/16 off and may clamp 7.47 steps to 7.
+    step = m[6:].view(18, 4, 64).abs().amax(2, keepdim=True) / 7.0
+    assert ((got[6:].view(18, 4, 64) - m[6:].view(18, 4, 64)).abs() <= 0.55 * step).all()
+
+
+# ---- the products ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", TOKENS)
+@pytest.mark.parametrize("n,k,group", SHAPES)
+@pytest.mark.parametrize("eight", [False, True])
+def test_linear(dev, m, n, k, group, eight):
+    """float32 results with a residual in place, bfloat16 ones with bias and activation, both against 64 bits; the same bits on a second call."""
+    from liyab_b200 import ops
+    q, s, r = _parts(n, k, group, dev, seed=m)
+    w, ref_w = ops.lay_out_weights4(q, s, r, group), _matrix(q, s, r, group)
+    a, scale = _rand((m, k), 5, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    bias, res = _rand((n,), 6, dev), _rand((m, n + 8), 7, dev)[:, :n]
+    ref = rows @ ref_w.T
+    bound = _sum_bound(k) * (rows.abs() @ ref_w.abs().T + bias.double().abs() + res.double().abs())
+    outs = []
+    for _ in range(2):
+        out = res.clone()
+        ops.linear4(a, w, None, out, m, residual=out, a_scale=scale)
+        assert ops.device_status() == 0
+        assert ((out.double() - ref - res.double()).abs() <= bound).all()
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1])
+    half = torch.full((m, n + 3), float("nan"), dtype=torch.bfloat16, device=dev)
+    ops.linear4(a, w, bias, half[:, :n], m, activation="relu2", a_scale=scale)
+    z = ref + bias.double()
+    want = z.clamp(min=0) ** 2
+    assert ((half[:, :n].double() - want).abs() <= 2.0 ** -8 * want + 2 * (z.abs() + bound) * bound).all()
+    assert half[:, n:].isnan().all()
+
+
+@pytest.mark.parametrize("m", [1, 5, 16, 40, 129])
+@pytest.mark.parametrize("activation", ["gelu_tanh", "gelu_erf", "xielu", "relu2", "none"])
+def test_activations(dev, m, activation):
+    """Beside the product of the 32-bit units on the matrix that the weights stand for."""
+    from liyab_b200 import ops
+    n, k = 328, 640
+    q, s, r = _parts(n, k, 64, dev)
+    w = ops.lay_out_weights4(q, s, r * 0.05, 64)
+    a, bias = _rand((m, k), 8, dev, torch.bfloat16), _rand((n + 2,), 9, dev)
+    bias[n:] = torch.tensor([0.8, 0.4], device=dev)
+    want, out = torch.empty((m, n), device=dev), torch.empty((m, n), device=dev)
+    values = ops.weights4_values(w)
+    ops.gemm_ffma(a.float(), values, bias, want, m, activation)
+    ops.linear4(a, w, bias, out, m, activation=activation)
+    # Both sums are within the bound of the exact one; the activations' slopes stay below 3 here but for the two squares.
+    size = a.double().abs() @ values.double().abs().T + bias[:n].double().abs()
+    slope = 3.0 + 4.0 * (size if activation in ("relu2", "xielu") else 0.0)
+    assert ((out.double() - want.double()).abs() <= 2.0 * _sum_bound(2 * k) * size * slope).all()
+
+
+@pytest.mark.parametrize("m", TOKENS)
+@pytest.mark.parametrize("f,k,group", [(1, 1, 32), (8, 64, 64), (9, 129, 128), (100, 200, 32), (682, 1600, 64), (1000, 4104, 128), (2731, 2048, 64)])
+@pytest.mark.parametrize("eight", [False, True])
+def test_gated(dev, m, f, k, group, eight):
+    from liyab_b200 import ops
+    q, s, r = _parts(2 * f, k, group, dev, seed=m + 1)
+    r = r * 0.05
+    w, ref_w = ops.lay_out_weights4(q, s, r, group, paired=True), _matrix(q, s, r, group)
+    a, scale = _rand((m, k), 10, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    both, size = rows @ ref_w.T, _sum_bound(k) * (rows.abs() @ ref_w.abs().T)
+    g, u, eg, eu = both[:, :f], both[:, f:], size[:, :f], size[:, f:]
+    for gate in ("silu", "relu", "gelu_tanh", "sigmoid", "capped"):
+        if gate == "capped":
+            gg, uu = g.clamp(max=2.0), u.clamp(-2.0, 2.0)
+            want, uu = gg * torch.sigmoid(1.7 * gg) * (uu + 1.0), uu + 1.0
+            slope, act = 1.7, gg * torch.sigmoid(1.7 * gg)
+        else:
+            act = {"silu": lambda: g * torch.sigmoid(g), "relu": lambda: g.clamp(min=0), "sigmoid": lambda: torch.sigmoid(g),
+                   "gelu_tanh": lambda: 0.5 * g * (1 + torch.tanh(0.7978845608028654 * (g + 0.044715 * g ** 3)))}[gate]()
+            want, uu, slope = act * u, u, 1.2
+        for dtype, rounding in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+            out = torch.full((m, f + 1), float("nan"), dtype=dtype, device=dev)
+            ops.gated4(a, w, out[:, :f], m, gate=gate, a_scale=scale, alpha=1.7, limit=2.0)
+            # The product's rule on both sums' errors, and the gate's own 32-bit arithmetic (under 16 roundings).
+            bound = slope * eg * (uu.abs() + eu) + act.abs() * eu + 2.0 ** -19 * (want.abs() + act.abs()) + 1e-30
+            assert ((out[:, :f].double() - want).abs() <= bound + rounding * want.abs()).all(), (gate, dtype)
+            assert out[:, f:].isnan().all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("m", [1, 3, 12, 40, 150])
+@pytest.mark.parametrize("eight", [False, True])
+def test_rows_that_lie_anyhow(dev, m, eight):
+    """Strides and starts that are no multiple of 16 bytes, and rows behind the last that are not read."""
+    from liyab_b200 import ops
+    n, k = 136, 520
+    q, s, r = _parts(n, k, 64, dev)
+    w = ops.lay_out_weights4(q, s, r, 64)
+    for pad, first in ((0, 0), (8, 8), (16, 0), (3, 1), (1, 0), (4, 4)):
+        wide = _rand((m, k + pad), 11, dev)
+        if eight:
+            rows, scale = _rows8(wide)
+        else:
+            rows, scale = wide.to(torch.bfloat16), None
+        a = rows[:, first:first + k] if first + k <= k + pad else rows[:, :k]
+        a64 = a.double() if scale is None else a.double() * scale.double()[:, None]
+        ref_w = _matrix(q, s, r, 64)
+        out = torch.full((m + 2, n + 1), 5.0, device=dev)
+        ops.linear4(a, w, None, out[:, :n], m, a_scale=scale)
+        assert ((out[:m, :n].double() - a64 @ ref_w.T).abs() <= _sum_bound(k) * (a64.abs() @ ref_w.abs().T)).all()
+        assert (out[m:] == 5.0).all() and (out[:, n:] == 5.0).all()
+
+
+@pytest.mark.parametrize("m", [1, 9, 33, 140])
+def test_special_values_stay_in_their_row(dev, m):
+    """An infinity or a NaN in a row of activations makes that row's outputs what 64 bits make of them, and no other row's; so does a NaN factor of a feature."""
+    from liyab_b200 import ops
+    n, k = 200, 384
+    q, s, r = _parts(n, k, 128, dev)
+    r[5] = float("nan")
+    w = ops.lay_out_weights4(q, s, r, 128)
+    a = _rand((m, k), 12, dev, torch.bfloat16)
+    a[0, 17], a[m // 2, 100], a[m - 1, 380] = float("inf"), float("-inf"), float("nan")
+    out = torch.empty((m, n), device=dev)
+    ops.linear4(a, w, None, out, m)
+    want = a.double() @ _matrix(q, s, r, 128).T
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[out.isinf()], want.float()[out.isinf()]) and torch.equal(out.isinf(), want.isinf())
+    a8, scale = _rows8(_rand((m, k), 13, dev))
+    scale[0] = float("nan")
+    ops.linear4(a8, w, None, out, m, a_scale=scale)
+    assert out[0].isnan().all() and out[1:, :5].isfinite().all() and out[:, 5].isnan().all()
+
+
+def test_no_rows(dev):
+    from liyab_b200 import ops
+    q, s, r = _parts(32, 64, 32, dev)
+    out = torch.full((4, 32), 3.0, device=dev)
+    ops.linear4(torch.zeros((4, 64), dtype=torch.bfloat16, device=dev), ops.lay_out_weights4(q, s, r, 32), None, out, 0)
+    ops.gated4(torch.zeros((4, 64), dtype=torch.bfloat16, device=dev), ops.lay_out_weights4(q, s, r, 32, paired=True), out[:, :16], 0)
+    assert (out == 3.0).all()
+
+
+# ---- the norm ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 3, 200])
+@pytest.mark.parametrize("width", [1, 7, 64, 130, 1600, 4096, 5461, 8192, 16384, 57344])
+@pytest.mark.parametrize("x_type,delta_type", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_norm(dev, rows, width, x_type, delta_type):
+    from liyab_b200 import ops
+    x, delta = _rand((rows, width), 20, dev, x_type, 3.0), _rand((rows, width), 21, dev, delta_type)
+    gain = 1.0 + 0.3 * _rand((width,), 22, dev)
+    t = x.double() + delta.double()
+    h = t / (t.square().mean(1, keepdim=True) + 1e-5).sqrt() * (0.5 + gain.double())
+    # t: one rounding in 32 bits (and one to x's type, 2^-8 for bfloat16's eight bits); the mean: errors of a sum of squares, all of one sign, in parts of 32 at least and 64 levels at most: 2^-17 covers it.
+    total_bound = (2.0 ** -24 + (2.0 ** -8 if x_type is torch.bfloat16 else 0.0)) * t.abs()
+    h_bound = 2.0 ** -17 * h.abs() + 2.0 ** -22 * (0.5 + gain.double()).abs()
+    half = torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+    total = torch.empty_like(x)
+    ops.rms_add(x, delta, gain, 1e-5, half, total=total, gain_offset=0.5)
+    assert ((total.double() - t).abs() <= total_bound).all()
+    assert ((half.double() - h).abs() <= 2.0 ** -8 * h.abs() + h_bound).all()
+    out, scale = torch.empty((rows, width), dtype=F8, device=dev), torch.empty(rows, device=dev)
+    moved = x.clone()
+    ops.rms_add(moved, delta, gain, 1e-5, out, scale=scale, gain_offset=0.5)                      # in place
+    assert torch.equal(moved, total)
+    top = h.abs().amax(1)
+    assert ((scale.double() - top / 448.0).abs() <= 2.0 ** -16 * top / 448.0 + 2.0 ** -30).all()
+    # e4m3: half a step is 2^-4 of a normal number, 2^-10 below 2^-6.
+    got = out.double() * scale.double()[:, None]
+    assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2 * h_bound).all()
+    assert (out.float().abs().amax(1) == 448.0).all()
+
+
+def test_norm_alone_and_strided(dev):
+    """Without a delta nothing is written but the result; without a gain it is one; rows that lie apart, at odd places."""
+    from liyab_b200 import ops
+    for width, pad, first in ((96, 7, 3), (1600, 8, 0), (1600, 1, 1), (4096, 4, 4)):
+        wide = _rand((5, width + pad), 23, dev)
+        x = wide[:, first:first + width]
+        keep = wide.clone()
+        out = torch.full((5, width + pad), float("nan"), dtype=torch.bfloat16, device=dev)
+        ops.rms_add(x, None, None, 1e-6, out[:, first:first + width])
+        h = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt()
+        assert ((out[:, first:first + width].double() - h).abs() <= (2.0 ** -8 + 2.0 ** -17) * h.abs()).all()
+        assert torch.equal(wide, keep) and int(out.isnan().sum()) == 5 * pad
+        eight, scale = torch.zeros((5, width + pad), dtype=F8, device=dev), torch.empty(5, device=dev)
+        delta = _rand((5, width + 5), 24, dev)[:, 2:2 + width]
+        ops.rms_add(x, delta, None, 1e-6, eight[:, first:first + width], scale=scale)
+        t = keep[:, first:first + width].double() + delta.double()
+        assert ((x.double() - t).abs() <= 2.0 ** -23 * t.abs()).all()
+        h = t / (t.square().mean(1, keepdim=True) + 1e-6).sqrt()
+        got = eight[:, first:first + width].double() * scale.double()[:, None]
+        assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2.0 ** -16 * h.abs()).all()
+
+
+def test_norm_of_special_rows(dev):
+    from liyab_b200 import ops
+    for width in (40, 1600, 9000):
+        x = _rand((7, width), 25, dev)
+        x[1], x[2, 3], x[3, width - 1], x[4] = 0.0, float("inf"), float("nan"), 1e-38
+        x[5] = 1e-3 * x[5]
+        out, scale, half = torch.ones((7, width), dtype=F8, device=dev), torch.empty(7, device=dev), torch.empty((7, width), dtype=torch.bfloat16, device=dev)
+        ops.rms_add(x, None, None, 0.1, out, scale=scale)
+        assert (out[1:5].float() == 0).all() and (scale[[1, 4]] == 0).all() and not scale[2:4].isfinite().any() and (scale[[0, 5, 6]] > 0).all()
+        ops.rms_add(x, None, None, 0.1, half)
+        assert (half[1] == 0).all() and half[3].isnan().all() and half[[0, 1, 4, 5, 6]].isfinite().all()
+
+
+# ---- together, and refusals --------------------------------------------------------------------------------
+
+def test_a_block_on_its_own_stream_and_in_a_graph(dev):
+    """Norm, gated half and second half as a feed-forward block: on a stream of its own, then captured and replayed on new rows."""
+    from liyab_b200 import ops
+    width, f = 640, 1712
+    up = ops.quantise_weights4(_rand((2 * f, width), 30, dev, scale=0.04), 64, paired=True)
+    down = ops.quantise_weights4(_rand((width, f), 31, dev, torch.bfloat16, 0.03), 128)
+    wu, wd = ops.weights4_values(up).double(), ops.weights4_values(down).double()
+    gain = 1.0 + 0.1 * _rand((width,), 32, dev)
+    for m in (1, 6, 20, 150):
+        x, delta = _rand((m, width), 33, dev), _rand((m, width), 34, dev)
+        out8, scale = torch.empty((m, width), dtype=F8, device=dev), torch.empty(m, device=dev)
+        mid = torch.empty((m, f), dtype=torch.bfloat16, device=dev)
+
+        def block():
+            ops.rms_add(x, delta, gain, 1e-6, out8, scale=scale)
+            ops.gated4(out8, up, mid, m, a_scale=scale)
+            ops.linear4(mid, down, None, x, m, residual=x)
+
+        def check(x0):
+            t = x0.double() + delta.double()
+            h = out8.double() * scale.double()[:, None]
+            z = h @ wu.T
+            inner = z[:, :f] * torch.sigmoid(z[:, :f]) * z[:, f:]
+            assert ((mid.double() - inner).abs() <= 2.0 ** -8 * inner.abs() + 1e-4).all()
+            y = t + mid.double() @ wd.T
+            assert ((x.double() - y).abs() <= _sum_bound(f) * (mid.double().abs() @ wd.abs().T + t.abs())).all()
+
+        start = x.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block()
+        torch.cuda.current_stream().wait_stream(side)
+        check(start)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            block()
+        x.copy_(_rand((m, width), 35, dev))
+        start = x.clone()
+        graph.replay()
+        check(start)
+        assert ops.device_status() == 0
+
+
+def test_refusals(dev):
+    from liyab_b200 import ops
+    from liyab_b200.status import LiyabError
+    q, s, r = _parts(32, 64, 32, dev)
+    w, pw = ops.lay_out_weights4(q, s, r, 32), ops.lay_out_weights4(q, s, r, 32, paired=True)
+    a, out = torch.zeros((4, 64), dtype=torch.bfloat16, device=dev), torch.zeros((4, 32), device=dev)
+    a8, scale = torch.zeros((4, 64), dtype=F8, device=dev), torch.ones(4, device=dev)
+    x = torch.zeros((4, 64), device=dev)
+    for bad in (
+            lambda: ops.lay_out_weights4(q, s, r, 16), lambda: ops.lay_out_weights4(q, s[:, :1], r, 32), lambda: ops.lay_out_weights4(q.float(), s, r, 32),
+            lambda: ops.lay_out_weights4(q[:31], s[:31], r[:31], 32, paired=True), lambda: ops.lay_out_weights4(q.cpu(), s, r, 32), lambda: ops.lay_out_weights4(q, s, r.double(), 32),
+            lambda: ops.quantise_weights4(x.half()), lambda: ops.quantise_weights4(x.t()), lambda: ops.quantise_weights4(x, 48), lambda: ops.quantise_weights4(x[:0]),
+            lambda: ops.linear4(a, pw, None, out, 4), lambda: ops.gated4(a, w, out[:, :16], 4), lambda: ops.linear4(a, w, None, out, 5), lambda: ops.linear4(a, w, None, out, -1),
+            lambda: ops.linear4(a.float(), w, None, out, 4), lambda: ops.linear4(a8, w, None, out, 4), lambda: ops.linear4(a, w, None, out, 4, a_scale=scale),
+            lambda: ops.linear4(a8, w, None, out, 4, a_scale=scale[:3]), lambda: ops.linear4(a[:, :60], w, None, out, 4), lambda: ops.linear4(a, w, None, out.half(), 4),
+            lambda: ops.linear4(a, w, None, out[:, :31], 4), lambda: ops.linear4(a, w, out[0, :31], out, 4), lambda: ops.linear4(a, w, None, out, 4, activation="xielu"),
+            lambda: ops.linear4(a, w, None, out, 4, residual=out[:3]), lambda: ops.linear4(a.t().contiguous().t(), w, None, out, 4), lambda: ops.linear4(a.cpu(), w, None, out, 4),
+            lambda: ops.gated4(a, pw, out, 4), lambda: ops.gated4(a, pw, out[:, :16], 4, gate="relu2"), lambda: ops.gated4(a, pw, out[:, :16], 4, gate="tanh"),
+            lambda: ops.rms_add(x, None, None, 1e-5, a8), lambda: ops.rms_add(x, None, None, 1e-5, a, scale=scale), lambda: ops.rms_add(x, x[:3], None, 1e-5, a),
+            lambda: ops.rms_add(x, None, None, 1e-5, x), lambda: ops.rms_add(x, x, None, 1e-5, a, total=a), lambda: ops.rms_add(x, None, scale, 1e-5, a),
+            lambda: ops.rms_add(x, None, None, 1e-5, a8, scale=scale[:2]), lambda: ops.rms_add(x.half(), None, None, 1e-5, a), lambda: ops.rms_add(x.cpu(), None, None, 1e-5, a.cpu())):
+        with pytest.raises(LiyabError):
+            bad()
+    with pytest.raises(KeyError):
+        ops.linear4(a, w, None, out, 4, activation="tanh")
