@@ -750,9 +750,9 @@ int lb_channel_memory_pieces(int dtype, const lb_channel_memory* memory, const l
  *
  * A matrix w[n, k] = q[n, k] s[n, k / group] r[n]: q an integer in -8 .. 7, s an e4m3 number, r a float32; group is 32, 64 or 128.  The products read
  * it as lb_weights4_sizes and lb_weights4_lay_out (or lb_weights4_quantise) leave it, in memory of the caller's that stays where it is:
- *   nibbles  [row tile of 16][k tile of 128][row][t = 0..3][j = 0..3] words of eight weights k = 32 j + 8 t + i, stored as q + 8; weight i
+ *   nibbles  [row tile of 16][k tile of 128][t = 0..3][row][j = 0..3] words of eight weights k = 32 j + 8 t + i, stored as q + 8; weight i
  *            is nibble i / 2 + 4 (i % 2) of its word, so that a shift and a mask give two neighbours in the halves of a register.  16-byte aligned.
- *   scales   [row][scale_stride] e4m3, padded with zeros; 16-byte aligned.
+ *   scales   [row tile][k tile][row][128 / group] e4m3, padded with zeros; 16-byte aligned.
  *   rows     [row] float32, padded with zeros.
  * Rows are padded to a multiple of 128 and k to one of 128.  `paired`: a matrix of 2 f rows, the f rows of a gate and the f rows of its other factor, whose
  * rows are laid out in turns of eight, so that a feature's two rows lie eight rows apart in one tile. */
@@ -762,10 +762,9 @@ typedef struct {
     float* rows;
     int n, k;               /* of the matrix; n = 2 f when paired */
     int group, paired;
-    int n_padded, scale_stride;
 } lb_weights4;
-/* The bytes of a matrix's nibbles and its padded sizes. */
-int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int* n_padded, int* scale_stride);
+/* The bytes of a matrix's nibbles and of its scales, and its rows with the padding. */
+int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int64_t* scale_bytes, int* n_padded);
 /* q [n, k] int8 (row stride ldq; values outside -8 .. 7 are clamped), s [n, ceil(k / group)] e4m3 (row stride lds) and r [n] into w's memory, padding included. */
 int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, int64_t lds, const float* r, const lb_weights4* w, void* stream);
 /* A float32 or bfloat16 matrix rounded to 4 bits: t = max |w| of a group / 7, r = max t of a row / 448, s = e4m3(t / r), q = w / (s r) rounded to the nearest
@@ -774,12 +773,16 @@ int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, const lb_we
 /* out[n, k] = q s r (float32, row stride ldo), rows in the matrix's own order. */
 int lb_weights4_values(const lb_weights4* w, float* out, int64_t ldo, void* stream);
 /* out[M, n] = act(a w^T + bias) + residual; a is bfloat16, or e4m3 with a_scale[M]; out is LB_BF16 or LB_F32; bias (n floats) and residual (float32) may be null;
- * out may be the residual. */
+ * out may be the residual.  `scratch`: lb_linear4_scratch(..) bytes, 16-byte aligned (null where that is 0). */
 int lb_linear4(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const float* a_scale, const float* bias, const float* residual, int64_t ldr,
-               int out_dtype, void* out, int64_t ldo, int M, int act, void* stream);
+               int out_dtype, void* out, int64_t ldo, int M, int act, void* scratch, void* stream);
+/* The bytes of scratch memory of either product for these activations: 0 for few rows, and for bfloat16 rows that lie 16-byte aligned. */
+int64_t lb_linear4_scratch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M);
+/* Tests: the next launch of the kernel for many rows never announces its sums, so that its bounded waits run out. */
+int lb_linear4_withhold_next(int on);
 /* out[M, f] = gate(a w_gate^T) * (a w_up^T) for paired weights; gates (lb_gate_kind) 0 sigmoid, 1 silu, 2 gelu_tanh, 3 relu, 4 capped (alpha, limit). */
 int lb_gated4(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const float* a_scale, int out_dtype, void* out, int64_t ldo, int M, int gate,
-              float alpha, float limit, void* stream);
+              float alpha, float limit, void* scratch, void* stream);
 /* t = x + delta in 32 bits (delta may be null), total = t in x's type (may be x itself, may be null), h = t / sqrt(mean(t^2) + eps) * (gain_offset + gain) (gain may be
  * null: 1); out = h in bfloat16, or in e4m3 divided by scale[row] = max |h| / 448.  A row whose largest |h| is below 2^-117 has scale 0 and zeros; one with
  * a value that is not finite has a scale that is not finite and zeros. */

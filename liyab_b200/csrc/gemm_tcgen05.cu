@@ -431,6 +431,10 @@ int lb_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, int row
     return LB_OK;
 }
 
+int lb_tensor_map_2d_encode(CUtensorMap* out, const void* base, int elem_bytes, int rows, int cols, int64_t ld, int box_rows) {
+    return make_map(out, base, elem_bytes, rows, cols, ld, box_rows);
+}
+
 int lb_tc_status_word(int** out) {
     static int* addr = nullptr;
     if (addr == nullptr) LB_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&addr), g_status));

@@ -1,0 +1,23 @@
+// What the kernels behind lb_linear4 and lb_gated4 share on the host.
+#pragma once
+
+#include "weights4.cuh"
+
+int linear4_sm_count();
+
+// How few_tokens cuts a product: token tiles of 8, warps a block, blocks a cluster (along k), clusters, k tiles on the way a warp, row tiles a round, bytes of shared memory.
+// warps 0: it does not take it.
+struct FewPlan {
+    int token_tiles, warps, splits, clusters, ahead, round, smem;
+};
+FewPlan few_plan(int M, int rows, int k, int group, int n_sm);
+int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, const FewPlan& p, cudaStream_t stream);
+
+// How many_tokens cuts one: tokens a tile, blocks a cluster (along k), stages, columns of tensor memory for the sums and in all, bytes of shared memory.
+struct ManyPlan {
+    int tokens, splits, stages, d_columns, tmem_columns, smem;
+};
+ManyPlan many_plan(int M, int rows, int k, int n_sm);
+// Activations that TMA does not take as they are (e4m3, rows off the 16 bytes) go through scratch memory.
+int64_t many_scratch_bytes(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M);
+int many_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, void* scratch, cudaStream_t stream);

@@ -1,0 +1,288 @@
+// Products with 4-bit weights for few tokens: out = act(a w^T + bias) + residual, and gate(a w_gate^T) * (a w_up^T) over paired rows.
+//
+// The weights are the rows of mma.sync (16 of them by 16 k), the tokens its columns (8 a tile, NT tiles).  A block owns a stretch of row tiles; its activations
+// lie in shared memory in the order of the operand.  Row tiles by k tiles of 128 are one sequence that the block's warps cut into equal parts, whatever
+// the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, AHEAD tiles on the way), makes a register of two weights of a shift, a mask and a
+// subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
+// After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
+#include "linear4.h"
+#include "tcgen05.cuh"
+
+namespace {
+
+using namespace lb_w4;
+using lb_tc::smem_u32;
+
+constexpr int kRound = 32;               // row tiles between two barriers
+
+__device__ __forceinline__ uint4 load_weights(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// The scales of a row's k tile (1, 2 or 4 of them) in the low bytes.
+template <int GROUP>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
+    if constexpr (GROUP == 128) return __ldg(p);
+    else if constexpr (GROUP == 64) return __ldg(reinterpret_cast<const uint16_t*>(p));
+    else return __ldg(reinterpret_cast<const uint32_t*>(p));
+}
+
+__device__ __forceinline__ float load_remote(uint32_t local, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .u32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}" : "=f"(v) : "r"(local), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ int load_remote_int(uint32_t local, uint32_t rank) { return __float_as_int(load_remote(local, rank)); }
+
+// Shared memory: activations [k tile][token][j ^ (token & 1)][t] of 16 bytes (the exclusive or keeps eight lanes' reads off one another's banks) behind a line of zeros
+// for the columns without a token; the slots [slot][16][8 NT].
+struct Layout {
+    int rows_at, slots_at, total;
+    __host__ __device__ Layout(int M, int token_tiles, int n_kt, int tiles, int warps) {
+        rows_at = 256;
+        slots_at = rows_at + n_kt * M * 256;
+        total = slots_at + 512 * token_tiles * (tiles + warps);
+    }
+};
+
+// AHEAD: k tiles on the way a warp; SPLIT: the cluster's blocks share the reduction.
+template <typename T, int NT, int GROUP, int AHEAD, bool SPLIT>
+__global__ void __launch_bounds__(AHEAD > 2 ? 512 : 1024)
+few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, bool wide, const Epilogue e, int n_tiles, int k_tiles, int splits, int round_tiles) {
+    constexpr int kSlot = 128 * NT, kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile;
+    extern __shared__ __align__(128) uint8_t shared[];
+    __shared__ int parts_of[kRound][2];                                                               // the first and the last warp of a row tile
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_warps = blockDim.x >> 5;
+    const int rank = SPLIT ? (int)blockIdx.x % splits : 0, cluster = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, clusters = SPLIT ? (int)gridDim.x / splits : (int)gridDim.x;
+    const int per_rank = SPLIT ? (k_tiles + splits - 1) / splits : k_tiles, kt0 = rank * per_rank, n_kt = min(k_tiles, kt0 + per_rank) - kt0;   // the host leaves no rank without one
+    const int first = (int)((int64_t)cluster * n_tiles / clusters), last = (int)((int64_t)(cluster + 1) * n_tiles / clusters);
+    const Layout at_of(e.M, NT, per_rank, round_tiles, n_warps);
+    float* slots = reinterpret_cast<float*>(shared + at_of.slots_at);
+
+    // This warp's part of a round: k tiles x0 .. x1 of the round's sequence, in memory one stretch, but for a rank of several, whose stretch of every row tile ends before
+    // that of the next begins.
+    int x0 = 0, x1 = 0, start = 0, kt = 0, left = 0;
+    const uint4* from = nullptr;                 // of the tile that is computed next (SPLIT: of the one that is fetched next)
+    const uint8_t* scales_from = nullptr;
+    uint4 words[AHEAD][2];
+    uint32_t steps[AHEAD][2];
+    auto fetch = [&](int i, int at) {
+        words[i][0] = load_weights(from + at * (kTileBytes / 16));
+        words[i][1] = load_weights(from + at * (kTileBytes / 16) + 8);
+        steps[i][0] = load_scales<GROUP>(scales_from + at * kScaleBytes);
+        steps[i][1] = load_scales<GROUP>(scales_from + at * kScaleBytes + 8 * kPerTile);
+        if (SPLIT) {
+            const int skip = --left == 0 ? k_tiles - n_kt + 1 : 1;
+            if (left == 0) left = n_kt;
+            from += (size_t)skip * (kTileBytes / 16);
+            scales_from += (size_t)skip * kScaleBytes;
+        }
+    };
+    auto begin_round = [&](int base) {
+        const int length = min(round_tiles, last - base) * n_kt, parts = min(n_warps, length);        // no warp between two others is without a k tile
+        x0 = warp < parts ? (int)((int64_t)warp * length / parts) : 0;
+        x1 = warp < parts ? (int)((int64_t)(warp + 1) * length / parts) : 0;
+        start = base + x0 / n_kt;
+        kt = x0 % n_kt;
+        left = n_kt - kt;
+        const size_t tile0 = (size_t)start * k_tiles + kt0 + kt;
+        from = static_cast<const uint4*>(w.nibbles) + tile0 * (kTileBytes / 16) + kTileRows * t + g;
+        scales_from = static_cast<const uint8_t*>(w.scales) + tile0 * kScaleBytes + g * kPerTile;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (x0 + i < x1) fetch(i, SPLIT ? 0 : i);
+    };
+    if (first < last) begin_round(first);
+    const Unpack<T> unpack;
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    if (threadIdx.x < 16) reinterpret_cast<uint4*>(shared)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    for (int c = threadIdx.x; c < n_kt * 16 * e.M; c += blockDim.x) {
+        const int at = c & 3, j = c >> 2 & 3, m = (c >> 4) % e.M, k_tile = (c >> 4) / e.M;
+        uint32_t v[4];
+        load_eight<T>(v, a, (int64_t)m * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
+        reinterpret_cast<uint4*>(shared + at_of.rows_at)[(k_tile * e.M + m) * 16 + (j ^ (m & 1)) * 4 + at] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+
+    // This lane's activations: of a token, or the line of zeros; words of even and of odd j lie `swap` bytes further and nearer.
+    uint32_t columns[NT];
+    int column_step[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const bool there = 8 * n + g < e.M;
+        columns[n] = smem_u32(shared) + (there ? at_of.rows_at + (8 * n + g) * 256 : 0) + 16 * t;
+        column_step[n] = there ? 256 * e.M : 0;
+    }
+    const int swap = (g & 1) * 64;
+    for (int base = first; base < last; base += round_tiles) {
+        __syncthreads();                    // the activations are there; the last round's slots have been read
+        const int tiles = min(round_tiles, last - base);
+        float acc[NT][4];
+        uint32_t column[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+            column[n] = columns[n] + kt * column_step[n];
+        }
+        int here = n_kt - kt, of = start - base;
+        float* slot = slots + (of + warp) * kSlot;
+        if (x0 < x1 && kt == 0) parts_of[of][0] = warp;
+        for (int x = x0; x < x1; x += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (x + i >= x1) break;
+                const uint4 top = words[i][0], low = words[i][1];
+                const uint32_t st = steps[i][0], sl = steps[i][1];
+                const uint32_t wt[4] = {top.x, top.y, top.z, top.w}, wl[4] = {low.x, low.y, low.z, low.w};
+                float part[NT][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 b[NT];
+#pragma unroll
+                    for (int n8 = 0; n8 < NT; ++n8)
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[n8].x), "=r"(b[n8].y), "=r"(b[n8].z), "=r"(b[n8].w)
+                                     : "r"((j & 1 ? column[n8] - swap : column[n8] + swap) + 64 * j));
+                    if ((j * 32) % GROUP == 0)
+#pragma unroll
+                        for (int n8 = 0; n8 < NT; ++n8) part[n8][0] = part[n8][1] = part[n8][2] = part[n8][3] = 0.0f;
+                    {
+                        const uint32_t a0 = unpack(wt[j], 0), a1 = unpack(wl[j], 0), a2 = unpack(wt[j], 1), a3 = unpack(wl[j], 1);
+#pragma unroll
+                        for (int n8 = 0; n8 < NT; ++n8) mma16816<T>(part[n8], a0, a1, a2, a3, b[n8].x, b[n8].y);
+                    }
+                    {
+                        const uint32_t a0 = unpack(wt[j], 2), a1 = unpack(wl[j], 2), a2 = unpack(wt[j], 3), a3 = unpack(wl[j], 3);
+#pragma unroll
+                        for (int n8 = 0; n8 < NT; ++n8) mma16816<T>(part[n8], a0, a1, a2, a3, b[n8].z, b[n8].w);
+                    }
+                    if ((j * 32 + 32) % GROUP == 0) {
+                        const uint32_t both = e4m3x2_to_f16x2(__byte_perm(st, sl, 0x0040 + (j * 32 / GROUP) * 0x11));
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&both));
+#pragma unroll
+                        for (int n8 = 0; n8 < NT; ++n8) {
+                            acc[n8][0] = fmaf(part[n8][0], f.x, acc[n8][0]);
+                            acc[n8][1] = fmaf(part[n8][1], f.x, acc[n8][1]);
+                            acc[n8][2] = fmaf(part[n8][2], f.y, acc[n8][2]);
+                            acc[n8][3] = fmaf(part[n8][3], f.y, acc[n8][3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n8 = 0; n8 < NT; ++n8) column[n8] += column_step[n8];
+                if (x + i + AHEAD < x1) fetch(i, SPLIT ? 0 : i + AHEAD);
+                if (--here == 0 || x + i == x1 - 1) {
+#pragma unroll
+                    for (int n8 = 0; n8 < NT; ++n8) {
+                        *reinterpret_cast<float2*>(slot + g * 8 * NT + 8 * n8 + 2 * t) = make_float2(acc[n8][0], acc[n8][1]);
+                        *reinterpret_cast<float2*>(slot + (g + 8) * 8 * NT + 8 * n8 + 2 * t) = make_float2(acc[n8][2], acc[n8][3]);
+                        acc[n8][0] = acc[n8][1] = acc[n8][2] = acc[n8][3] = 0.0f;
+                        column[n8] = columns[n8];
+                    }
+                    slot += kSlot;
+                    if (here == 0) parts_of[of][1] = warp;
+                    if (x + i != x1 - 1) parts_of[++of][0] = warp;
+                    here = n_kt;
+                }
+            }
+            if (!SPLIT) {
+                from += AHEAD * (kTileBytes / 16);
+                scales_from += AHEAD * kScaleBytes;
+            }
+        }
+        if (base + round_tiles < last) begin_round(base + round_tiles);
+        __syncthreads();
+
+        if (SPLIT) {
+            // Every row tile's sum into its first slot, where the other ranks read it.
+            for (int u = threadIdx.x; u < tiles * kSlot; u += blockDim.x) {
+                const int i = u / kSlot, at_slot = u % kSlot, lo = parts_of[i][0], hi = parts_of[i][1];
+                float v = 0.0f;
+                for (int q = lo; q <= hi; ++q) v += slots[(i + q) * kSlot + at_slot];
+                slots[(i + lo) * kSlot + at_slot] = v;
+            }
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        }
+        const lb_act_pair pair = w.paired ? lb_act_pair{0.0f, 0.0f} : lb_act_load(e.bias, e.n, e.act);
+        for (int u = rank * (int)blockDim.x + (int)threadIdx.x; u < tiles * 8 * e.M; u += splits * (int)blockDim.x) {
+            const int i = (u >> 3) / e.M, token = (u >> 3) - i * e.M, row = u & 7, tile = base + i;
+            const float a_scale = e.a_scale != nullptr ? e.a_scale[token] : 1.0f;
+            const float factor[2] = {w.rows[tile * 16 + row] * a_scale, w.rows[tile * 16 + row + 8] * a_scale};
+            float v[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at_slot = (row + 8 * h) * 8 * NT + token;
+                if (!SPLIT) {
+                    const int hi = parts_of[i][1];
+                    for (int q = parts_of[i][0]; q <= hi; ++q) v[h] += slots[(i + q) * kSlot + at_slot];
+                } else {
+                    for (int r = 0; r < splits; ++r) {
+                        const int lo = load_remote_int(smem_u32(&parts_of[i][0]), r);
+                        v[h] += load_remote(smem_u32(slots + (i + lo) * kSlot + at_slot), r);
+                    }
+                }
+            }
+            if (w.paired) {
+                const int col = tile * 8 + row;
+                if (col < e.n) store_out(e, token, col, lb_gated_pair(v[0] * factor[0], v[1] * factor[1], e.gate, e.alpha, e.limit));
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = tile * 16 + row + 8 * h;
+                    if (col < e.n) finish_one(e, pair, token, col, v[h] * factor[h]);
+                }
+            }
+        }
+        // No slot is written again, and no block leaves, while another may read this round's sums.
+        if (SPLIT) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    }
+}
+
+template <typename T, int NT, int GROUP>
+int launch_group(const lb_weights4* w, const void* a, int64_t lda, bool wide, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
+    auto kernel = p.ahead > 2 ? (p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, 4, true> : few_tokens_kernel<T, NT, GROUP, 4, false>)
+                              : (p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, 2, true> : few_tokens_kernel<T, NT, GROUP, 2, false>);
+    if (p.smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
+    LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, p.splits, kernel, dim3(p.clusters * p.splits), dim3(32 * p.warps), p.smem, s, *w, a, lda, wide, e, n_tiles, k_tiles, p.splits,
+                                               p.round));
+    return LB_OK;
+}
+
+template <typename T, int NT>
+int launch(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
+    const bool wide = lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % (T::kHalf ? 8 : 16) == 0;
+    if (w->group == 32) return launch_group<T, NT, 32>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+    if (w->group == 64) return launch_group<T, NT, 64>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+    return launch_group<T, NT, 128>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+}
+
+}  // namespace
+
+FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
+    FewPlan p{};
+    const int k_tiles = (k + kTileK - 1) / kTileK, n_tiles = (rows + kTileRows - 1) / kTileRows;
+    if (M > 16) return p;
+    p.token_tiles = M <= 8 ? 1 : 2;
+    for (p.splits = 1; p.splits <= 8; p.splits *= 2) {
+        const int per_rank = (k_tiles + p.splits - 1) / p.splits;
+        if (per_rank * (p.splits - 1) >= k_tiles) return p;
+        p.clusters = n_tiles < n_sm / p.splits ? n_tiles : n_sm / p.splits;
+        p.round = (n_tiles + p.clusters - 1) / p.clusters;
+        if (p.round > kRound) p.round = kRound;
+        const int length = p.round * per_rank, warps = length <= 16 ? 8 : length <= 256 || p.token_tiles > 1 ? 16 : 32;
+        p.ahead = warps > 16 ? 2 : 4;
+        p.smem = Layout(M, p.token_tiles, per_rank, p.round, warps).total;
+        if (p.smem <= 224 * 1024) {
+            p.warps = warps;
+            return p;
+        }
+    }
+    return p;
+}
+
+int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const Epilogue& e, const FewPlan& p, cudaStream_t stream) {
+    const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, n_tiles = (rows + kTileRows - 1) / kTileRows;
+    if (a_dtype == LB_E4M3) return p.token_tiles == 1 ? launch<F16, 1>(w, a, lda, e, p, n_tiles, k_tiles, stream) : launch<F16, 2>(w, a, lda, e, p, n_tiles, k_tiles, stream);
+    return p.token_tiles == 1 ? launch<Bf16, 1>(w, a, lda, e, p, n_tiles, k_tiles, stream) : launch<Bf16, 2>(w, a, lda, e, p, n_tiles, k_tiles, stream);
+}

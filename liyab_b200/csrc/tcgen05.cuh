@@ -191,5 +191,7 @@ __device__ __forceinline__ void named_barrier(int id, int count) {
 // A [rows, cols] matrix of `elem_bytes`-wide elements (2: bfloat16, 4: float32) with `ld` elements between rows,
 // moved in boxes of [box_rows, 128 bytes] with the 128-byte swizzle.  Encoded once per distinct description.
 int lb_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, int rows, int cols, int64_t ld, int box_rows);
+// The same, encoded anew.
+int lb_tensor_map_2d_encode(CUtensorMap* out, const void* base, int elem_bytes, int rows, int cols, int64_t ld, int box_rows);
 // Address of the device word in which the kernels' bounded waits record where they gave up.
 int lb_tc_status_word(int** out);

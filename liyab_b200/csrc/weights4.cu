@@ -8,17 +8,15 @@ namespace {
 using namespace lb_w4;
 
 struct Sizes {
-    int rows, padded, k_tiles, groups, stride;
+    int rows, padded, k_tiles;
 };
 
 // Rows as they are laid out: of a paired matrix each half is filled up to a multiple of eight.
-Sizes sizes_of(int n, int k, int group, int paired) {
+Sizes sizes_of(int n, int k, int paired) {
     Sizes s;
     s.rows = paired ? 2 * ((n / 2 + 7) / 8 * 8) : n;
     s.padded = (s.rows + 127) / 128 * 128;
     s.k_tiles = (k + kTileK - 1) / kTileK;
-    s.groups = s.k_tiles * (kTileK / group);
-    s.stride = (s.groups + 15) / 16 * 16;
     return s;
 }
 
@@ -26,8 +24,6 @@ int check_weights(const lb_weights4* w, const char* what) {
     LB_CHECK_ARG(w != nullptr && w->nibbles != nullptr && w->scales != nullptr && w->rows != nullptr, "%s: weights without memory", what);
     LB_CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "%s: group is %d, not 32, 64 or 128", what, w->group);
     LB_CHECK_ARG(w->n > 0 && w->k > 0 && w->n <= (1 << 26) && w->k <= (1 << 26) && (!w->paired || w->n % 2 == 0), "%s: a matrix of %d x %d", what, w->n, w->k);
-    const Sizes s = sizes_of(w->n, w->k, w->group, w->paired);
-    LB_CHECK_ARG(w->n_padded == s.padded && w->scale_stride == s.stride, "%s: the padded sizes are not those of lb_weights4_sizes", what);
     LB_CHECK_ARG(reinterpret_cast<uintptr_t>(w->nibbles) % 16 == 0 && reinterpret_cast<uintptr_t>(w->scales) % 16 == 0, "%s: nibbles and scales are not 16-byte aligned",
                  what);
     return LB_OK;
@@ -44,7 +40,12 @@ __device__ __forceinline__ int source_row(int row, int n, int paired) {
 __device__ __forceinline__ int nibble_shift(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
 
 __device__ __forceinline__ size_t word_at(int row, int kt, int t, int j, int k_tiles) {
-    return ((size_t)(row >> 4) * k_tiles + kt) * (kTileBytes / 4) + (row & 15) * 16 + 4 * t + j;
+    return ((size_t)(row >> 4) * k_tiles + kt) * (kTileBytes / 4) + (t * kTileRows + (row & 15)) * 4 + j;
+}
+
+// A row's scales of a k tile.
+__device__ __forceinline__ uint8_t* scales_at(const lb_weights4& w, int row, int kt, int k_tiles) {
+    return static_cast<uint8_t*>(w.scales) + (((size_t)(row >> 4) * k_tiles + kt) * kTileRows + (row & 15)) * (kTileK / w.group);
 }
 
 // A block a row: its words of eight weights, its scales and its factor.
@@ -62,8 +63,9 @@ __global__ void lay_out_kernel(const int8_t* __restrict__ q, int64_t ldq, const 
         }
         words[word_at(row, kt, t, j, k_tiles)] = word;
     }
-    uint8_t* scales = static_cast<uint8_t*>(w.scales) + (size_t)row * w.scale_stride;
-    for (int g = threadIdx.x; g < w.scale_stride; g += blockDim.x) scales[g] = from >= 0 && g < groups ? s[(int64_t)from * lds + g] : 0;
+    const int per_tile = kTileK / w.group;
+    for (int g = threadIdx.x; g < k_tiles * per_tile; g += blockDim.x)
+        scales_at(w, row, g / per_tile, k_tiles)[g % per_tile] = from >= 0 && g < groups ? s[(int64_t)from * lds + g] : 0;
     if (threadIdx.x == 0) w.rows[row] = from >= 0 ? r[from] : 0.0f;
 }
 
@@ -96,7 +98,6 @@ __global__ void quantise_kernel(const T* __restrict__ matrix, int64_t ldm, const
     if (!some) r = finite ? 0.0f : __int_as_float(0x7fc00000);
 
     uint32_t* words = static_cast<uint32_t*>(w.nibbles);
-    uint8_t* scales = static_cast<uint8_t*>(w.scales) + (size_t)row * w.scale_stride;
     for (int kt = warp; kt < k_tiles; kt += n_warps) {
         float v[4], peak = 0.0f;
 #pragma unroll
@@ -116,9 +117,8 @@ __global__ void quantise_kernel(const T* __restrict__ matrix, int64_t ldm, const
         }
         part |= __shfl_xor_sync(0xffffffffu, part, 1);
         if ((lane & 1) == 0) words[word_at(row, kt, lane >> 1 & 3, lane >> 3, k_tiles)] = part;
-        if (lane % lanes == 0) scales[kt * (kTileK / w.group) + lane / lanes] = (uint8_t)s;
+        if (lane % lanes == 0) scales_at(w, row, kt, k_tiles)[lane / lanes] = (uint8_t)s;
     }
-    for (int g = k_tiles * (kTileK / w.group) + threadIdx.x; g < w.scale_stride; g += blockDim.x) scales[g] = 0;
     if (threadIdx.x == 0) w.rows[row] = r;
 }
 
@@ -126,12 +126,11 @@ __global__ void values_kernel(const lb_weights4 w, float* __restrict__ out, int6
     const int row = blockIdx.x, to = source_row(row, w.n, w.paired);
     if (to < 0) return;
     const uint32_t* words = static_cast<const uint32_t*>(w.nibbles);
-    const uint8_t* scales = static_cast<const uint8_t*>(w.scales) + (size_t)row * w.scale_stride;
     for (int k = threadIdx.x; k < w.k; k += blockDim.x) {
         const int in = k % kTileK;
         const uint32_t word = words[word_at(row, k / kTileK, in >> 3 & 3, in >> 5, k_tiles)];
         const float q = (float)((int)(word >> nibble_shift(in & 7) & 15u) - 8);
-        out[(int64_t)to * ldo + k] = q * e4m3_to_float(scales[k / w.group]) * w.rows[row];
+        out[(int64_t)to * ldo + k] = q * e4m3_to_float(scales_at(w, row, k / kTileK, k_tiles)[in / w.group]) * w.rows[row];
     }
 }
 
@@ -144,21 +143,21 @@ int finished(cudaStream_t stream) {
 
 }  // namespace
 
-extern "C" int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int* n_padded, int* scale_stride) {
-    LB_CHECK_ARG(nibble_bytes != nullptr && n_padded != nullptr && scale_stride != nullptr, "weights4: nowhere to write the sizes");
+extern "C" int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int64_t* scale_bytes, int* n_padded) {
+    LB_CHECK_ARG(nibble_bytes != nullptr && scale_bytes != nullptr && n_padded != nullptr, "weights4: nowhere to write the sizes");
     LB_CHECK_ARG(group == 32 || group == 64 || group == 128, "weights4: group is %d, not 32, 64 or 128", group);
     LB_CHECK_ARG(n > 0 && k > 0 && n <= (1 << 26) && k <= (1 << 26) && (!paired || n % 2 == 0), "weights4: a matrix of %d x %d", n, k);
-    const Sizes s = sizes_of(n, k, group, paired);
+    const Sizes s = sizes_of(n, k, paired);
     *nibble_bytes = (int64_t)(s.padded / kTileRows) * s.k_tiles * kTileBytes;
     *n_padded = s.padded;
-    *scale_stride = s.stride;
+    *scale_bytes = (int64_t)s.padded * s.k_tiles * (kTileK / group);
     return LB_OK;
 }
 
 extern "C" int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, int64_t lds, const float* r, const lb_weights4* w, void* stream) {
     if (int rc = check_weights(w, "weights4_lay_out")) return rc;
     LB_CHECK_ARG(q != nullptr && s != nullptr && r != nullptr && ldq >= w->k && lds >= (w->k + w->group - 1) / w->group, "weights4_lay_out: a part is missing or its rows overlap");
-    const Sizes z = sizes_of(w->n, w->k, w->group, w->paired);
+    const Sizes z = sizes_of(w->n, w->k, w->paired);
     lay_out_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(q, ldq, static_cast<const uint8_t*>(s), lds, r, *w, z.k_tiles);
     return finished(static_cast<cudaStream_t>(stream));
 }
@@ -167,7 +166,7 @@ extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, 
     if (int rc = check_weights(w, "weights4_quantise")) return rc;
     LB_CHECK_ARG(matrix != nullptr && ldm >= w->k, "weights4_quantise: no matrix, or its rows overlap");
     LB_CHECK_ARG(dtype == LB_F32 || dtype == LB_BF16, "weights4_quantise: a matrix is float32 or bfloat16");
-    const Sizes z = sizes_of(w->n, w->k, w->group, w->paired);
+    const Sizes z = sizes_of(w->n, w->k, w->paired);
     if (dtype == LB_F32) quantise_kernel<float><<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const float*>(matrix), ldm, *w, z.k_tiles);
     else quantise_kernel<__nv_bfloat16><<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(matrix), ldm, *w, z.k_tiles);
     return finished(static_cast<cudaStream_t>(stream));
@@ -176,7 +175,7 @@ extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, 
 extern "C" int lb_weights4_values(const lb_weights4* w, float* out, int64_t ldo, void* stream) {
     if (int rc = check_weights(w, "weights4_values")) return rc;
     LB_CHECK_ARG(out != nullptr && ldo >= w->k, "weights4_values: no output, or its rows overlap");
-    const Sizes z = sizes_of(w->n, w->k, w->group, w->paired);
+    const Sizes z = sizes_of(w->n, w->k, w->paired);
     values_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(*w, out, ldo, z.k_tiles);
     LB_CHECK_LAUNCH();
     return LB_OK;

@@ -15,31 +15,41 @@ namespace lb_w4 {
 
 constexpr int kTileRows = 16, kTileK = 128, kTileBytes = kTileRows * kTileK / 2;
 
+// (x & mask) | bits in one instruction: with both numbers as literals it becomes two.
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(x), "r"(mask), "r"(bits));
+    return v;
+}
+
 // The operand type of the tensor cores: bfloat16 activations go with bfloat16 weights, e4m3 ones with float16.
 struct Bf16 {
     static constexpr bool kHalf = false;
-    // Nibbles (q + 8) in the low bits of both halves -> q: 0x4300 | u is 128 + u.
-    static __device__ __forceinline__ uint32_t weights(uint32_t u) {
-        const uint32_t v = u | 0x43004300u, c = 0x43084308u;
+    static constexpr uint32_t kMagic = 0x43004300u;          // 0x4300 | u is 128 + u
+    static __device__ __forceinline__ uint32_t minus(uint32_t v, uint32_t c) {
         const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&c));
         return *reinterpret_cast<const uint32_t*>(&d);
     }
 };
 struct F16 {
     static constexpr bool kHalf = true;
-    // 0x6400 | u is 1024 + u.
-    static __device__ __forceinline__ uint32_t weights(uint32_t u) {
-        const uint32_t v = u | 0x64006400u, c = 0x64086408u;
+    static constexpr uint32_t kMagic = 0x64006400u;          // 0x6400 | u is 1024 + u
+    static __device__ __forceinline__ uint32_t minus(uint32_t v, uint32_t c) {
         const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
         return *reinterpret_cast<const uint32_t*>(&d);
     }
 };
 
-// Weights 2p and 2p + 1 of a word of eight, in the halves of a register.
+// Nibbles q + 8 to q.  The mask and the exponent bits are kept in registers, hidden from constant folding.
 template <typename T>
-__device__ __forceinline__ uint32_t pair_of(uint32_t word, int p) {
-    return T::weights((word >> (4 * p)) & 0x000F000Fu);
-}
+struct Unpack {
+    uint32_t mask, magic;
+    __device__ __forceinline__ Unpack() {
+        asm volatile("mov.b32 %0, 0x000F000F;\n\tmov.b32 %1, %2;" : "=r"(mask), "=r"(magic) : "n"(T::kMagic));
+    }
+    // Weights 2p and 2p + 1 of a word of eight, in the halves of a register.
+    __device__ __forceinline__ uint32_t operator()(uint32_t word, int p) const { return T::minus(masked_or(word >> (4 * p), mask, magic), T::kMagic | 0x00080008u); }
+};
 
 // Two e4m3 numbers (16 bits) -> float16.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {

@@ -93,6 +93,7 @@ def lib():
     if _lib is None:
         l = load_library()
         l.lb_last_error.restype = _c.c_char_p
+        l.lb_linear4_scratch.argtypes, l.lb_linear4_scratch.restype = [_p, _i, _p, _l, _i], _l
         for name, args in _SIGNATURES.items():
             fn = getattr(l, name)
             fn.argtypes = args
@@ -1182,7 +1183,7 @@ _ROWS8 = torch.float8_e4m3fn
 
 
 class Weights4Args(ctypes.Structure):
-    _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _i), ("n_padded", _i), ("scale_stride", _i)]
+    _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _i)]
 
 
 for _name, _args in {
@@ -1190,8 +1191,9 @@ for _name, _args in {
     "lb_weights4_lay_out": [_p, _l, _p, _l, _p, _p, _p],
     "lb_weights4_quantise": [_i, _p, _l, _p, _p],
     "lb_weights4_values": [_p, _p, _l, _p],
-    "lb_linear4": [_p, _i, _p, _l, _p, _p, _p, _l, _i, _p, _l, _i, _i, _p],
-    "lb_gated4": [_p, _i, _p, _l, _p, _i, _p, _l, _i, _i, _f, _f, _p],
+    "lb_linear4": [_p, _i, _p, _l, _p, _p, _p, _l, _i, _p, _l, _i, _i, _p, _p],
+    "lb_linear4_withhold_next": [_i],
+    "lb_gated4": [_p, _i, _p, _l, _p, _i, _p, _l, _i, _i, _f, _f, _p, _p],
     "lb_rms_add_rows": [_i, _p, _l, _i, _p, _l, _p, _l, _p, _f, _f, _i, _p, _l, _p, _i, _i, _p],
 }.items():
     _SIGNATURES[_name] = _args
@@ -1204,13 +1206,13 @@ class Weights4:
     __slots__ = ("n", "k", "group", "paired", "device", "nibbles", "scales", "rows", "args", "ref")
 
     def __init__(self, n: int, k: int, group: int, paired: bool, device: torch.device):
-        nibbles, padded, stride = ctypes.c_int64(0), ctypes.c_int(0), ctypes.c_int(0)
-        check(lib().lb_weights4_sizes(n, k, group, int(paired), ctypes.byref(nibbles), ctypes.byref(padded), ctypes.byref(stride)), "weights4")
+        nibbles, scales, padded = ctypes.c_int64(0), ctypes.c_int64(0), ctypes.c_int(0)
+        check(lib().lb_weights4_sizes(n, k, group, int(paired), ctypes.byref(nibbles), ctypes.byref(scales), ctypes.byref(padded)), "weights4")
         self.n, self.k, self.group, self.paired, self.device = n, k, group, paired, device
         self.nibbles = torch.empty(nibbles.value, dtype=torch.uint8, device=device)
-        self.scales = torch.empty((padded.value, stride.value), dtype=torch.uint8, device=device)
+        self.scales = torch.empty(scales.value, dtype=torch.uint8, device=device)
         self.rows = torch.empty(padded.value, dtype=torch.float32, device=device)
-        self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired), padded.value, stride.value)
+        self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired))
         self.ref = ctypes.addressof(self.args)
 
     @property
@@ -1268,6 +1270,12 @@ def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n
     return BF16, None, _code(out.dtype, "out")
 
 
+def _scratch4(w: Weights4, code: int, a: torch.Tensor, m: int) -> Optional[torch.Tensor]:
+    """Memory for activations that the kernel for many rows does not read as they are."""
+    n = lib().lb_linear4_scratch(w.ref, code, a.data_ptr(), a.stride(0), m) if m > 16 or w.k > 8192 else 0
+    return torch.empty(n, dtype=torch.uint8, device=w.device) if n else None
+
+
 def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: torch.Tensor, m: int, activation: str = "none",
             residual: Optional[torch.Tensor] = None, a_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[:m] = act(a[:m] @ w.T + bias) + residual with 4-bit weights: a is bfloat16, or e4m3 with a_scale (a row of a times a_scale[row] is what it stands for);
@@ -1277,8 +1285,9 @@ def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: tor
         raise invalid_argument("linear4: the residual is float32 rows of the output's width")
     if bias is not None and (bias.dtype != torch.float32 or bias.device != w.device or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0)):
         raise invalid_argument("linear4: the bias is float32, one number a feature")
+    scratch = _scratch4(w, code, a, m)
     check(lib().lb_linear4(w.ref, code, a.data_ptr(), a.stride(0), scale, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
-                           0 if residual is None else residual.stride(0), out_code, out.data_ptr(), out.stride(0), m, ACTIVATIONS[activation], stream_ptr()), "linear4")
+                           0 if residual is None else residual.stride(0), out_code, out.data_ptr(), out.stride(0), m, ACTIVATIONS[activation], None if scratch is None else scratch.data_ptr(), stream_ptr()), "linear4")
     return out
 
 
@@ -1290,7 +1299,9 @@ def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = 
     if kind > 4:
         raise invalid_argument(f"gated4: no gate {gate!r}")
     code, scale, out_code = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
-    check(lib().lb_gated4(w.ref, code, a.data_ptr(), a.stride(0), scale, out_code, out.data_ptr(), out.stride(0), m, kind, alpha, limit, stream_ptr()), "gated4")
+    scratch = _scratch4(w, code, a, m)
+    check(lib().lb_gated4(w.ref, code, a.data_ptr(), a.stride(0), scale, out_code, out.data_ptr(), out.stride(0), m, kind, alpha, limit,
+                          None if scratch is None else scratch.data_ptr(), stream_ptr()), "gated4")
     return out
 
 
