@@ -772,22 +772,47 @@ int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, int64_t lds
 int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, const lb_weights4* w, void* stream);
 /* out[n, k] = q s r (float32, row stride ldo), rows in the matrix's own order. */
 int lb_weights4_values(const lb_weights4* w, float* out, int64_t ldo, void* stream);
-/* out[M, n] = act(a w^T + bias) + residual; a is bfloat16, or e4m3 with a_scale[M]; out is LB_BF16 or LB_F32; bias (n floats) and residual (float32) may be null;
- * out may be the residual.  `scratch`: lb_linear4_scratch(..) bytes, 16-byte aligned (null where that is 0). */
-int lb_linear4(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const float* a_scale, const float* bias, const float* residual, int64_t ldr,
-               int out_dtype, void* out, int64_t ldo, int M, int act, void* scratch, void* stream);
+/* What a product with 4-bit weights is given.  Row strides are in elements. */
+typedef struct {
+    const lb_weights4* w;
+    const void* a;              /* bfloat16, or e4m3 with */
+    const float* a_scale;       /* a float a row, else null */
+    const float* bias;          /* linear4: n floats (xIELU: n + 2), or null */
+    const float* residual;      /* linear4: float32, or null; may be out */
+    void* out;
+    void* scratch;              /* lb_linear4_scratch(..) bytes, 16-byte aligned (null where that is 0) */
+    void* stream;
+    int64_t lda, ldr, ldo;
+    int a_dtype, out_dtype;     /* LB_BF16 or LB_E4M3; LB_BF16 or LB_F32 */
+    int M;
+    int act;                    /* linear4: the products' activations; gated4: lb_gate_kind 0 sigmoid, 1 silu, 2 gelu_tanh, 3 relu, 4 capped with */
+    float alpha, limit;
+} lb_linear4_args;
+/* out[M, n] = act(a w^T + bias) + residual. */
+int lb_linear4(const lb_linear4_args* args);
+/* out[M, f] = gate(a w_gate^T) * (a w_up^T) for paired weights. */
+int lb_gated4(const lb_linear4_args* args);
 /* The bytes of scratch memory of either product for these activations: 0 for few rows, and for bfloat16 rows that lie 16-byte aligned. */
 int64_t lb_linear4_scratch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M);
 /* Tests: the next launch of the kernel for many rows never announces its sums, so that its bounded waits run out. */
 int lb_linear4_withhold_next(int on);
-/* out[M, f] = gate(a w_gate^T) * (a w_up^T) for paired weights; gates (lb_gate_kind) 0 sigmoid, 1 silu, 2 gelu_tanh, 3 relu, 4 capped (alpha, limit). */
-int lb_gated4(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const float* a_scale, int out_dtype, void* out, int64_t ldo, int M, int gate,
-              float alpha, float limit, void* scratch, void* stream);
 /* t = x + delta in 32 bits (delta may be null), total = t in x's type (may be x itself, may be null), h = t / sqrt(mean(t^2) + eps) * (gain_offset + gain) (gain may be
  * null: 1); out = h in bfloat16, or in e4m3 divided by scale[row] = max |h| / 448.  A row whose largest |h| is below 2^-117 has scale 0 and zeros; one with
- * a value that is not finite has a scale that is not finite and zeros. */
-int lb_rms_add_rows(int x_dtype, const void* x, int64_t ldx, int delta_dtype, const void* delta, int64_t ldd, void* total, int64_t ldt, const float* gain, float gain_offset,
-               float eps, int out_dtype, void* out, int64_t ldo, float* scale, int rows, int width, void* stream);
+ * a value that is not finite has a scale that is not finite and zeros.  Row strides are in elements. */
+typedef struct {
+    const void* x;
+    const void* delta;
+    void* total;
+    const float* gain;
+    void* out;
+    float* scale;               /* null with a bfloat16 output */
+    void* stream;
+    int64_t ldx, ldd, ldt, ldo;
+    int x_dtype, delta_dtype, out_dtype;
+    int rows, width;
+    float gain_offset, eps;
+} lb_rms_add_args;
+int lb_rms_add_rows(const lb_rms_add_args* args);
 
 #ifdef __cplusplus
 }

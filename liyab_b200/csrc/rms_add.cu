@@ -1,5 +1,10 @@
 // A sublayer's output joins the residual stream and is normed for the next one: t = x + delta, h = t / sqrt(mean(t^2) + eps) * gain, left in bfloat16 or in
-// e4m3 with a scale a row.  A block a row; the row stays in shared memory between the passes over it (sum of squares, largest value, results).
+// e4m3 with a scale a row.
+//
+// Bound by memory: one pass, x and delta in, the sum and the result out.  A row stays in registers as t (gain_offset + gain), up to 32 values a thread, between its sum of
+// squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor; a warp has a row of up to 1024 values (no barrier), a block a longer one (two
+// barriers).  About ten instructions a value: with the divisions, selections and comparisons of a first version (29) 4096 bfloat16 rows of 8192 took 69 us, not MEASURED.
+// Rows off the 16 bytes, and of more than 16384 values, go through shared memory, a value at a time and neighbours by neighbouring threads.
 #include "weights4.cuh"
 
 namespace {
@@ -8,82 +13,226 @@ using namespace lb_w4;
 
 constexpr int kMaxWidth = 56 * 1024;
 constexpr float kSmallest = 6.018531e-36f;      // 2^-117: 448 / it is still finite
+constexpr uint32_t kInfinity = 0x7f800000u;
 
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-    v = lb_warp_max(v);
-    __syncthreads();
-    if (lane == 0) scratch[warp] = v;
-    __syncthreads();
-    v = scratch[0];
-    for (int i = 1; i < n_warps; ++i) v = fmaxf(v, scratch[i]);
-    return v;
+using Rows = lb_rms_add_args;
+
+// The larger size; a NaN stays.
+__device__ __forceinline__ float largest(float top, float v) {
+    float out;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(out) : "f"(top), "f"(fabsf(v)));
+    return out;
 }
 
-template <typename TX, typename TD>
-__global__ void rms_add_kernel(const TX* x, int64_t ldx, const TD* delta, int64_t ldd, TX* total, int64_t ldt, const float* __restrict__ gain, float gain_offset, float eps,
-                               void* out, int64_t ldo, float* scale, int width) {
-    extern __shared__ float row[];
-    __shared__ float scratch[33];
+// What a row's largest |h| makes of the row: the factor on h (0: the row becomes zeros) and the scale.
+__device__ __forceinline__ float row_factor(float top, float* scale) {
+    const bool some = __float_as_uint(top) < kInfinity && top >= kSmallest;
+    *scale = some ? top * (1.0f / 448.0f) : __float_as_uint(top) < kInfinity ? 0.0f : __int_as_float(0x7fc00000);
+    return some ? __fdividef(448.0f, top) : 0.0f;
+}
+
+// 8 values from 16 or 32 bytes.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+}
+
+// V: eights a thread.  WARP: a warp a row.
+template <typename TX, typename TD, int V, bool WARP>
+__global__ void __launch_bounds__(512, V == 4 ? 2 : 3)
+rms_add_kernel(const Rows p) {
+    __shared__ float sums[32];
+    __shared__ uint32_t tops[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    const int tid = WARP ? lane : (int)threadIdx.x, threads = WARP ? 32 : (int)blockDim.x;
+    const int r = WARP ? (int)blockIdx.x * n_warps + warp : (int)blockIdx.x;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int r = blockIdx.x;
+    if (WARP && r >= p.rows) return;
+    float v[V][8], d[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int at = (j * threads + tid) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = d[j][i] = 0.0f;
+        if (at < p.width) {
+            load8(static_cast<const TX*>(p.x) + (int64_t)r * p.ldx + at, v[j]);
+            if (p.delta != nullptr) load8(static_cast<const TD*>(p.delta) + (int64_t)r * p.ldd + at, d[j]);
+        }
+    }
     float ss = 0.0f;
-    for (int i = threadIdx.x; i < width; i += blockDim.x) {
-        float t = lb_to_float(x[(int64_t)r * ldx + i]);
-        if (delta != nullptr) t += lb_to_float(delta[(int64_t)r * ldd + i]);
-        if (total != nullptr) total[(int64_t)r * ldt + i] = lb_from_float<TX>(t);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[j][i] += d[j][i];
+            ss = fmaf(v[j][i], v[j][i], ss);
+        }
+    ss = lb_warp_sum(ss);
+    if (!WARP && lane == 0) sums[warp] = ss;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int at = (j * threads + tid) * 8;
+        if (at >= p.width) break;
+        if (p.total != nullptr) store8(static_cast<TX*>(p.total) + (int64_t)r * p.ldt + at, v[j]);
+        if (p.gain != nullptr) {
+            float g[8];
+            load8(p.gain + at, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] *= p.gain_offset + g[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = largest(top, v[j][i]);
+    }
+    uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (!WARP) {
+        if (lane == 0) tops[warp] = bits;
+        __syncthreads();
+        ss = lb_warp_sum(lane < n_warps ? sums[lane] : 0.0f);
+        bits = __reduce_max_sync(0xffffffffu, lane < n_warps ? tops[lane] : 0u);
+    }
+    // h = v inv; where the squares overflow, inv is 0 and the finite values' row becomes zeros.
+    const float inv = rsqrtf(__fdividef(ss, (float)p.width) + p.eps);
+    if (p.scale == nullptr) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int at = (j * threads + tid) * 8;
+            if (at >= p.width) break;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] *= inv;
+            store8(static_cast<__nv_bfloat16*>(p.out) + (int64_t)r * p.ldo + at, v[j]);
+        }
+        return;
+    }
+    float scale;
+    float f = row_factor(__uint_as_float(bits) * inv, &scale);
+    if (f != 0.0f) f *= inv;
+    if (tid == 0) p.scale[r] = scale;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int at = (j * threads + tid) * 8;
+        if (at >= p.width) break;
+        uint2 eight = make_uint2(0u, 0u);
+        if (f != 0.0f) {
+            eight.x = floats_to_e4m3x2(v[j][0] * f, v[j][1] * f) | floats_to_e4m3x2(v[j][2] * f, v[j][3] * f) << 16;
+            eight.y = floats_to_e4m3x2(v[j][4] * f, v[j][5] * f) | floats_to_e4m3x2(v[j][6] * f, v[j][7] * f) << 16;
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (int64_t)r * p.ldo + at) = eight;
+    }
+}
+
+// Rows of any place and length.
+template <typename TX, typename TD>
+__global__ void __launch_bounds__(1024)
+rms_add_any_kernel(const Rows p) {
+    extern __shared__ float row[];
+    __shared__ float sums[33];
+    __shared__ uint32_t tops[32];
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    float ss = 0.0f;
+    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
+        float t = lb_to_float(static_cast<const TX*>(p.x)[(int64_t)r * p.ldx + i]);
+        if (p.delta != nullptr) t += lb_to_float(static_cast<const TD*>(p.delta)[(int64_t)r * p.ldd + i]);
+        if (p.total != nullptr) static_cast<TX*>(p.total)[(int64_t)r * p.ldt + i] = lb_from_float<TX>(t);
         row[i] = t;
         ss = fmaf(t, t, ss);
     }
-    const float inv = 1.0f / sqrtf(lb_block_sum(ss, scratch) / (float)width + eps);
+    const float inv = rsqrtf(__fdividef(lb_block_sum(ss, sums), (float)p.width) + p.eps);
     float top = 0.0f;
-    bool finite = true;
-    for (int i = threadIdx.x; i < width; i += blockDim.x) {
-        const float h = row[i] * inv * (gain != nullptr ? gain_offset + gain[i] : 1.0f);
-        row[i] = h;
-        finite &= fabsf(h) <= 3.402823466e38f;
-        top = fmaxf(top, fabsf(h));
+    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
+        const float h = row[i] * inv * (p.gain != nullptr ? p.gain_offset + p.gain[i] : 1.0f);
+        if (p.scale == nullptr) {
+            static_cast<__nv_bfloat16*>(p.out)[(int64_t)r * p.ldo + i] = __float2bfloat16_rn(h);
+        } else {
+            row[i] = h;
+            top = largest(top, h);
+        }
     }
-    if (scale == nullptr) {
-        for (int i = threadIdx.x; i < width; i += blockDim.x) static_cast<__nv_bfloat16*>(out)[(int64_t)r * ldo + i] = __float2bfloat16_rn(row[i]);
-        return;
-    }
-    finite = __syncthreads_and(finite);
-    top = block_max(top, scratch);
-    const bool some = finite && top >= kSmallest;
-    const float f = some ? 448.0f / top : 0.0f;
-    for (int i = threadIdx.x; i < width; i += blockDim.x)
-        static_cast<uint8_t*>(out)[(int64_t)r * ldo + i] = some ? (uint8_t)floats_to_e4m3x2(row[i] * f, 0.0f) : 0;
-    if (threadIdx.x == 0) scale[r] = some ? top / 448.0f : finite ? 0.0f : __int_as_float(0x7fc00000);
+    if (p.scale == nullptr) return;
+    uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (lane == 0) tops[warp] = bits;
+    __syncthreads();
+    bits = __reduce_max_sync(0xffffffffu, lane < n_warps ? tops[lane] : 0u);
+    float scale;
+    const float f = row_factor(__uint_as_float(bits), &scale);
+    for (int i = threadIdx.x; i < p.width; i += blockDim.x)
+        static_cast<uint8_t*>(p.out)[(int64_t)r * p.ldo + i] = f != 0.0f ? (uint8_t)floats_to_e4m3x2(row[i] * f, 0.0f) : 0;
+    if (threadIdx.x == 0) p.scale[r] = scale;
 }
 
 template <typename TX, typename TD>
-int launch(const void* x, int64_t ldx, const void* delta, int64_t ldd, void* total, int64_t ldt, const float* gain, float gain_offset, float eps, void* out, int64_t ldo,
-           float* scale, int rows, int width, cudaStream_t stream) {
-    const size_t smem = sizeof(float) * width;
-    auto kernel = rms_add_kernel<TX, TD>;
-    if (smem > 48 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(rows), dim3(width >= 2048 ? 512 : 256), smem, stream, static_cast<const TX*>(x), ldx, static_cast<const TD*>(delta), ldd,
-                                       static_cast<TX*>(total), ldt, gain, gain_offset, eps, out, ldo, scale, width));
-    return LB_OK;
+int launch(const Rows& p) {
+    const cudaStream_t s = static_cast<cudaStream_t>(p.stream);
+    auto aligned = [](const void* q, int64_t ld, int bytes) { return q == nullptr || (reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * bytes % 16 == 0); };
+    const bool eight = p.scale != nullptr;
+    const bool wide = p.width % 8 == 0 && aligned(p.x, p.ldx, sizeof(TX)) && aligned(p.delta, p.ldd, sizeof(TD)) && aligned(p.total, p.ldt, sizeof(TX)) && aligned(p.gain, 0, 4) &&
+                      (eight ? reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.ldo % 8 == 0 : aligned(p.out, p.ldo, 2));
+    const int eights = (p.width + 7) / 8;
+    if (!wide || eights > 2048) {
+        const size_t smem = sizeof(float) * p.width;
+        if (smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(rms_add_any_kernel<TX, TD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWidth * 4));
+        const int block = p.width <= 1024 ? 128 : p.width <= 4096 ? 256 : p.width <= 16384 ? 512 : 1024;
+        LB_CHECK_CUDA(lb_launch_overlapped(rms_add_any_kernel<TX, TD>, dim3(p.rows), dim3(block), smem, s, p));
+        return LB_OK;
+    }
+#define LB_RMS(V_, WARP_, GRID_, BLOCK_)                                                                                                                \
+    do {                                                                                                                                                \
+        LB_CHECK_CUDA(lb_launch_overlapped(rms_add_kernel<TX, TD, V_, WARP_>, dim3(GRID_), dim3(BLOCK_), 0, s, p));                                     \
+        return LB_OK;                                                                                                                                   \
+    } while (0)
+    const bool many = p.rows >= 296;
+    if (many && eights <= 64) {
+        if (eights <= 32) LB_RMS(1, true, (p.rows + 3) / 4, 128);
+        LB_RMS(2, true, (p.rows + 3) / 4, 128);
+    }
+    const int v = eights > 1024 ? 4 : eights > 512 || (many && eights > 256) ? 2 : 1;
+    const int block = ((eights + v - 1) / v + 31) / 32 * 32;
+    if (v == 1) LB_RMS(1, false, p.rows, block);
+    if (v == 2) LB_RMS(2, false, p.rows, block);
+    LB_RMS(4, false, p.rows, block);
+#undef LB_RMS
 }
 
 }  // namespace
 
-extern "C" int lb_rms_add_rows(int x_dtype, const void* x, int64_t ldx, int delta_dtype, const void* delta, int64_t ldd, void* total, int64_t ldt, const float* gain,
-                          float gain_offset, float eps, int out_dtype, void* out, int64_t ldo, float* scale, int rows, int width, void* stream) {
-    LB_CHECK_ARG(rows >= 0 && (rows == 0 || (x != nullptr && out != nullptr)), "rms_add: %d rows, or no memory for them", rows);
-    LB_CHECK_ARG(width > 0 && width <= kMaxWidth, "rms_add: rows of %d values (1 to %d)", width, kMaxWidth);
-    LB_CHECK_ARG((x_dtype == LB_F32 || x_dtype == LB_BF16) && (delta_dtype == LB_F32 || delta_dtype == LB_BF16), "rms_add: x and delta are float32 or bfloat16");
-    LB_CHECK_ARG(out_dtype == LB_BF16 || out_dtype == LB_E4M3, "rms_add: the output is bfloat16 or e4m3");
-    LB_CHECK_ARG((out_dtype == LB_E4M3) == (scale != nullptr), "rms_add: an e4m3 output has a scale a row, a bfloat16 one has none");
-    LB_CHECK_ARG(ldx >= width && ldo >= width && (delta == nullptr || ldd >= width) && (total == nullptr || ldt >= width), "rms_add: rows overlap");
-    if (rows == 0) return LB_OK;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x_dtype == LB_F32)
-        return delta_dtype == LB_F32 ? launch<float, float>(x, ldx, delta, ldd, total, ldt, gain, gain_offset, eps, out, ldo, scale, rows, width, s)
-                                     : launch<float, __nv_bfloat16>(x, ldx, delta, ldd, total, ldt, gain, gain_offset, eps, out, ldo, scale, rows, width, s);
-    return delta_dtype == LB_F32 ? launch<__nv_bfloat16, float>(x, ldx, delta, ldd, total, ldt, gain, gain_offset, eps, out, ldo, scale, rows, width, s)
-                                 : launch<__nv_bfloat16, __nv_bfloat16>(x, ldx, delta, ldd, total, ldt, gain, gain_offset, eps, out, ldo, scale, rows, width, s);
+extern "C" int lb_rms_add_rows(const lb_rms_add_args* args) {
+    LB_CHECK_ARG(args != nullptr, "rms_add: no arguments");
+    const lb_rms_add_args& p = *args;
+    LB_CHECK_ARG(p.rows >= 0 && (p.rows == 0 || (p.x != nullptr && p.out != nullptr)), "rms_add: %d rows, or no memory for them", p.rows);
+    LB_CHECK_ARG(p.width > 0 && p.width <= kMaxWidth, "rms_add: rows of %d values (1 to %d)", p.width, kMaxWidth);
+    LB_CHECK_ARG((p.x_dtype == LB_F32 || p.x_dtype == LB_BF16) && (p.delta_dtype == LB_F32 || p.delta_dtype == LB_BF16), "rms_add: x and delta are float32 or bfloat16");
+    LB_CHECK_ARG(p.out_dtype == LB_BF16 || p.out_dtype == LB_E4M3, "rms_add: the output is bfloat16 or e4m3");
+    LB_CHECK_ARG((p.out_dtype == LB_E4M3) == (p.scale != nullptr), "rms_add: an e4m3 output has a scale a row, a bfloat16 one has none");
+    LB_CHECK_ARG(p.ldx >= p.width && p.ldo >= p.width && (p.delta == nullptr || p.ldd >= p.width) && (p.total == nullptr || p.ldt >= p.width), "rms_add: rows overlap");
+    if (p.rows == 0) return LB_OK;
+    if (p.x_dtype == LB_F32) return p.delta_dtype == LB_F32 ? launch<float, float>(p) : launch<float, __nv_bfloat16>(p);
+    return p.delta_dtype == LB_F32 ? launch<__nv_bfloat16, float>(p) : launch<__nv_bfloat16, __nv_bfloat16>(p);
 }

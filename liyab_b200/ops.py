@@ -9,6 +9,7 @@ fallback; a tensor that is not on a CUDA device is an error.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -136,6 +137,11 @@ def stream_ptr() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def stream_of(index: int) -> int:
+    """The current CUDA stream of the device with this index as a raw pointer."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _dev(t: torch.Tensor, name: str, dtype: Optional[torch.dtype] = None) -> int:
@@ -1182,6 +1188,11 @@ E4M3 = 2
 _ROWS8 = torch.float8_e4m3fn
 
 
+# The arguments of a call as the library's structs (lb_linear4_args, lb_rms_add_args): packing them costs a fraction of a conversion each.
+_linear4_args = struct.Struct("@8P3q4i2f").pack
+_rms_add_args = struct.Struct("@7P4q5i2f").pack
+
+
 class Weights4Args(ctypes.Structure):
     _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _i)]
 
@@ -1191,10 +1202,10 @@ for _name, _args in {
     "lb_weights4_lay_out": [_p, _l, _p, _l, _p, _p, _p],
     "lb_weights4_quantise": [_i, _p, _l, _p, _p],
     "lb_weights4_values": [_p, _p, _l, _p],
-    "lb_linear4": [_p, _i, _p, _l, _p, _p, _p, _l, _i, _p, _l, _i, _i, _p, _p],
+    "lb_linear4": [_c.c_char_p],
     "lb_linear4_withhold_next": [_i],
-    "lb_gated4": [_p, _i, _p, _l, _p, _i, _p, _l, _i, _i, _f, _f, _p, _p],
-    "lb_rms_add_rows": [_i, _p, _l, _i, _p, _l, _p, _l, _p, _f, _f, _i, _p, _l, _p, _i, _i, _p],
+    "lb_gated4": [_c.c_char_p],
+    "lb_rms_add_rows": [_c.c_char_p],
 }.items():
     _SIGNATURES[_name] = _args
 
@@ -1203,12 +1214,12 @@ class Weights4:
     """A matrix w[n, k] = q[n, k] s[n, k / group] r[n] in 4 bits (q in -8 .. 7, s in e4m3, r float32) as the products read it.  `paired`: 2 f rows, the f of a gate
     and the f of its other factor, for gated4.  The memory belongs to this object; made by quantise_weights4 or lay_out_weights4."""
 
-    __slots__ = ("n", "k", "group", "paired", "device", "nibbles", "scales", "rows", "args", "ref")
+    __slots__ = ("n", "k", "group", "paired", "device", "index", "nibbles", "scales", "rows", "args", "ref")
 
     def __init__(self, n: int, k: int, group: int, paired: bool, device: torch.device):
         nibbles, scales, padded = ctypes.c_int64(0), ctypes.c_int64(0), ctypes.c_int(0)
         check(lib().lb_weights4_sizes(n, k, group, int(paired), ctypes.byref(nibbles), ctypes.byref(scales), ctypes.byref(padded)), "weights4")
-        self.n, self.k, self.group, self.paired, self.device = n, k, group, paired, device
+        self.n, self.k, self.group, self.paired, self.device, self.index = n, k, group, paired, device, device.index
         self.nibbles = torch.empty(nibbles.value, dtype=torch.uint8, device=device)
         self.scales = torch.empty(scales.value, dtype=torch.uint8, device=device)
         self.rows = torch.empty(padded.value, dtype=torch.float32, device=device)
@@ -1256,23 +1267,30 @@ def weights4_values(w: Weights4) -> torch.Tensor:
 
 
 def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n: int, a_scale: Optional[torch.Tensor]) -> tuple:
-    """What both products check of their rows; (type of a, a_scale's pointer, type of out)."""
-    if a.device != w.device or out.device != w.device:
+    """What both products check of their rows; (type of a, a_scale's pointer, type of out, the row strides of a and of out)."""
+    index, in_shape, out_shape = w.index, a.shape, out.shape
+    if a.get_device() != index or out.get_device() != index:
         raise invalid_argument(f"{what}: a is on {a.device} and out on {out.device}, the weights on {w.device}")
-    if a.dim() != 2 or out.dim() != 2 or a.shape[1] != w.k or out.shape[1] != n or not 0 <= m <= min(a.shape[0], out.shape[0]) or a.stride(1) != 1 or out.stride(1) != 1:
-        raise invalid_argument(f"{what}: shapes do not fit: a {tuple(a.shape)}, w ({w.n}, {w.k}), out {tuple(out.shape)}, {m} rows")
+    if len(in_shape) != 2 or len(out_shape) != 2 or in_shape[1] != w.k or out_shape[1] != n or not 0 <= m <= in_shape[0] or m > out_shape[0]:
+        raise invalid_argument(f"{what}: shapes do not fit: a {tuple(in_shape)}, w ({w.n}, {w.k}), out {tuple(out_shape)}, {m} rows")
+    (lda, dense_a), (ldo, dense_out) = a.stride(), out.stride()
+    if dense_a != 1 or dense_out != 1:
+        raise invalid_argument(f"{what}: a and out have to be dense within a row")
+    out_code = _DT.get(out.dtype, -1)
+    if out_code < 0:
+        raise invalid_argument(f"{what}: out is float32 or bfloat16, not {out.dtype}")
     if a.dtype is _ROWS8:
-        if a_scale is None or a_scale.dtype != torch.float32 or a_scale.device != w.device or a_scale.dim() != 1 or a_scale.shape[0] < m or a_scale.stride(0) != 1:
+        if a_scale is None or a_scale.dtype is not torch.float32 or a_scale.get_device() != index or a_scale.dim() != 1 or a_scale.shape[0] < m or not a_scale.is_contiguous():
             raise invalid_argument(f"{what}: e4m3 activations come with a_scale, float32 [rows]")
-        return E4M3, a_scale.data_ptr(), _code(out.dtype, "out")
+        return E4M3, a_scale.data_ptr(), out_code, lda, ldo
     if a.dtype is not torch.bfloat16 or a_scale is not None:
         raise invalid_argument(f"{what}: activations are bfloat16, or e4m3 with a_scale; a is {a.dtype}")
-    return BF16, None, _code(out.dtype, "out")
+    return BF16, 0, out_code, lda, ldo
 
 
-def _scratch4(w: Weights4, code: int, a: torch.Tensor, m: int) -> Optional[torch.Tensor]:
+def _scratch4(w: Weights4, code: int, a: torch.Tensor, lda: int, m: int) -> Optional[torch.Tensor]:
     """Memory for activations that the kernel for many rows does not read as they are."""
-    n = lib().lb_linear4_scratch(w.ref, code, a.data_ptr(), a.stride(0), m) if m > 16 or w.k > 8192 else 0
+    n = lib().lb_linear4_scratch(w.ref, code, a.data_ptr(), lda, m)
     return torch.empty(n, dtype=torch.uint8, device=w.device) if n else None
 
 
@@ -1280,14 +1298,20 @@ def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: tor
             residual: Optional[torch.Tensor] = None, a_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[:m] = act(a[:m] @ w.T + bias) + residual with 4-bit weights: a is bfloat16, or e4m3 with a_scale (a row of a times a_scale[row] is what it stands for);
     out is bfloat16 or float32, bias and residual float32; out may be the residual."""
-    code, scale, out_code = _rows4("linear4", a, w, out, m, w.n, a_scale)
-    if residual is not None and (residual.dtype != torch.float32 or residual.device != w.device or residual.dim() != 2 or residual.shape[1] != w.n or residual.shape[0] < m or residual.stride(1) != 1):
-        raise invalid_argument("linear4: the residual is float32 rows of the output's width")
-    if bias is not None and (bias.dtype != torch.float32 or bias.device != w.device or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0)):
-        raise invalid_argument("linear4: the bias is float32, one number a feature")
-    scratch = _scratch4(w, code, a, m)
-    check(lib().lb_linear4(w.ref, code, a.data_ptr(), a.stride(0), scale, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
-                           0 if residual is None else residual.stride(0), out_code, out.data_ptr(), out.stride(0), m, ACTIVATIONS[activation], None if scratch is None else scratch.data_ptr(), stream_ptr()), "linear4")
+    code, scale, out_code, lda, ldo = _rows4("linear4", a, w, out, m, w.n, a_scale)
+    bias_at = residual_at = ldr = 0
+    if residual is not None:
+        shape = residual.shape
+        if residual.dtype is not torch.float32 or residual.get_device() != w.index or len(shape) != 2 or shape[1] != w.n or shape[0] < m or residual.stride(1) != 1:
+            raise invalid_argument("linear4: the residual is float32 rows of the output's width")
+        residual_at, ldr = residual.data_ptr(), residual.stride(0)
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.get_device() != w.index or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0):
+            raise invalid_argument("linear4: the bias is float32, one number a feature")
+        bias_at = bias.data_ptr()
+    scratch = _scratch4(w, code, a, lda, m) if m > 16 or w.k > 8192 else None
+    check(lib().lb_linear4(_linear4_args(w.ref, a.data_ptr(), scale, bias_at, residual_at, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                                         stream_of(w.index), lda, ldr, ldo, code, out_code, m, ACTIVATIONS[activation], 0.0, 0.0)), "linear4")
     return out
 
 
@@ -1298,10 +1322,10 @@ def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = 
     kind = GATE_KINDS.get(gate, 5)
     if kind > 4:
         raise invalid_argument(f"gated4: no gate {gate!r}")
-    code, scale, out_code = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
-    scratch = _scratch4(w, code, a, m)
-    check(lib().lb_gated4(w.ref, code, a.data_ptr(), a.stride(0), scale, out_code, out.data_ptr(), out.stride(0), m, kind, alpha, limit,
-                          None if scratch is None else scratch.data_ptr(), stream_ptr()), "gated4")
+    code, scale, out_code, lda, ldo = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
+    scratch = _scratch4(w, code, a, lda, m) if m > 16 or w.k > 8192 else None
+    check(lib().lb_gated4(_linear4_args(w.ref, a.data_ptr(), scale, 0, 0, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(), stream_of(w.index), lda, 0, ldo,
+                                        code, out_code, m, kind, alpha, limit)), "gated4")
     return out
 
 
@@ -1309,23 +1333,37 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
             total: Optional[torch.Tensor] = None, gain_offset: float = 0.0) -> torch.Tensor:
     """t = x + delta (32 bits), left in `total` (x's type; None: back in x where there is a delta); out = t / sqrt(mean(t^2) + eps) * (gain_offset + gain), bfloat16, or e4m3
     with scale (float32 [rows]): out * scale is the row, scale its largest |value| / 448.  x and delta are float32 or bfloat16."""
-    rows, width = x.shape
-    if total is None and delta is not None:
-        total = x
-    code = E4M3 if out.dtype is _ROWS8 else BF16 if out.dtype is torch.bfloat16 else -1
+    shape, index, out_type, x_type = x.shape, x.get_device(), out.dtype, x.dtype
+    if len(shape) != 2 or index < 0:
+        raise invalid_argument(f"rms_add: x has to be rows on a CUDA device; it is {tuple(shape)} on {x.device}")
+    rows, width = shape
+    code = E4M3 if out_type is _ROWS8 else BF16 if out_type is torch.bfloat16 else -1
     if code < 0 or (code == E4M3) != (scale is not None):
-        raise invalid_argument(f"rms_add: out is bfloat16, or e4m3 with a scale a row; it is {out.dtype}")
-    for t, name in ((x, "x"), (delta, "delta"), (out, "out"), (total, "total")):
-        if t is not None and (t.device != x.device or t.shape != x.shape or t.stride(1) != 1):
-            raise invalid_argument(f"rms_add: {name} has to be rows of x's shape, dense within a row and on x's device")
-    if total is not None and total.dtype != x.dtype:
-        raise invalid_argument(f"rms_add: total is {total.dtype}, x {x.dtype}")
-    if gain is not None and (gain.dtype != torch.float32 or gain.device != x.device or gain.shape != (width,) or not gain.is_contiguous()):
-        raise invalid_argument("rms_add: the gain is float32, one number a column")
-    if scale is not None and (scale.dtype != torch.float32 or scale.device != x.device or scale.shape != (rows,) or not scale.is_contiguous()):
-        raise invalid_argument("rms_add: the scales are float32, one number a row")
-    check(lib().lb_rms_add_rows(_code(x.dtype, "x"), _dev(x, "x"), x.stride(0), F32 if delta is None else _code(delta.dtype, "delta"),
-                           None if delta is None else delta.data_ptr(), 0 if delta is None else delta.stride(0), None if total is None else total.data_ptr(),
-                           0 if total is None else total.stride(0), None if gain is None else gain.data_ptr(), gain_offset, eps, code, out.data_ptr(), out.stride(0),
-                           None if scale is None else scale.data_ptr(), rows, width, stream_ptr()), "rms_add")
+        raise invalid_argument(f"rms_add: out is bfloat16, or e4m3 with a scale a row; it is {out_type}")
+    delta_at = total_at = gain_at = scale_at = delta_code = ldd = ldt = 0
+    (ldx, dense), (ldo, dense_out) = x.stride(), out.stride() if out.shape == shape else (0, 0)
+    if delta is not None:
+        delta_code, delta_at = _DT.get(delta.dtype, -1), delta.data_ptr()
+        ldd, dense_delta = delta.stride() if delta.shape == shape else (0, 0)
+        if dense_delta != 1 or delta_code < 0 or delta.get_device() != index:
+            raise invalid_argument("rms_add: delta has to be float32 or bfloat16 rows of x's shape, dense within a row and on x's device")
+        if total is None:
+            total = x
+    if total is not None:
+        total_at = total.data_ptr()
+        ldt, dense_total = total.stride() if total.shape == shape else (0, 0)
+        if dense_total != 1 or total.dtype is not x_type or total.get_device() != index:
+            raise invalid_argument("rms_add: total has to be rows of x's shape and type, dense within a row and on x's device")
+    if dense != 1 or dense_out != 1 or out.get_device() != index:
+        raise invalid_argument("rms_add: x and out have to be rows of one shape, dense within a row and on one device")
+    if gain is not None:
+        gain_at = gain.data_ptr()
+        if gain.dtype is not torch.float32 or gain.get_device() != index or gain.shape != (width,) or not gain.is_contiguous():
+            raise invalid_argument("rms_add: the gain is float32, one number a column")
+    if scale is not None:
+        scale_at = scale.data_ptr()
+        if scale.dtype is not torch.float32 or scale.get_device() != index or scale.shape != (rows,) or not scale.is_contiguous():
+            raise invalid_argument("rms_add: the scales are float32, one number a row")
+    check(lib().lb_rms_add_rows(_rms_add_args(x.data_ptr(), delta_at, total_at, gain_at, out.data_ptr(), scale_at, stream_of(index), ldx, ldd, ldt, ldo,
+                                              _code(x_type, "x"), delta_code, code, rows, width, gain_offset, eps)), "rms_add")
     return out
