@@ -13,9 +13,9 @@ struct FewPlan {
 FewPlan few_plan(int M, int rows, int k, int group, int n_sm);
 int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, const FewPlan& p, cudaStream_t stream);
 
-// How many_tokens cuts one: tokens a tile, blocks a cluster (along k), stages, columns of tensor memory for the sums and in all, bytes of shared memory.
+// How many_tokens cuts one: whether a block an SM walks the tiles, tokens a tile, blocks a cluster (along k), stages, columns of tensor memory for the sums and in all, bytes of shared memory.
 struct ManyPlan {
-    int tokens, splits, stages, d_columns, tmem_columns, smem;
+    int walk, tokens, splits, stages, d_columns, tmem_columns, smem;
 };
 ManyPlan many_plan(int M, int rows, int k, int n_sm);
 // Activations that TMA does not take as they are (e4m3, rows off the 16 bytes) go through scratch memory.

@@ -3,14 +3,20 @@
 // 128 rows of weights are the lanes of the accumulator, up to 256 tokens its columns.  The weights never pass through shared memory: a thread owns a row, makes
 // q s of its nibbles in registers (a shift, a mask and one fused multiply-add for two: (16 + u) s - 24 s with u = q + 8, exact) and stores them into tensor memory, where
 // tcgen05.mma reads its first operand; the activations come by TMA.  So the copies through shared memory are those of the tokens alone, and a k tile
-// of 128 x 128 weights costs 860 instructions of a warp beside eight products, which take 512 cycles with 256 tokens.
-// Where a product has too few tiles for the GPU the reduction is cut between the blocks of a cluster, which hand each other the sums of their share of the tokens through
-// distributed shared memory and finish them in rank order.
+// of 128 x 128 weights costs some 900 instructions of a warp beside eight products, which take 1,024 cycles with 256 tokens.
+// Where a product has more tiles than the GPU has SMs, a block of each SM walks them and warps of their own finish a tile's sums under the next tile's products (the
+// accumulator is free again when the last columns are in registers).  Where it has fewer, sixteen warps make weights and finish; the reduction is cut between the blocks of a
+// cluster, which hand each other the sums of their share of the tokens through distributed shared memory and finish them in rank order.
 //
-// Roles: warp 0 copies the activations, warp 1 issues the products, warps 4 to 11 make weights (warp % 4 names the 32 lanes; the two warps of those take alternate k
-// tiles) and finish the sums.  Handshakes and bounded waits as in the other tcgen05 products.
+// Roles: warp 0 copies the activations, warp 1 issues the products, warps 4 and up make weights (warp % 4 names the 32 lanes; the warps of those take k tiles in turn) and,
+// in the same warps or eight further ones, finish the sums.  Handshakes and bounded waits as in the other tcgen05 products:
+//   a_full[s], b_full[s]   weights of stage s in tensor memory, activations in shared memory
+//   empty[s]               the products have read both
+//   acc_full, acc_empty    the sums of a tile are complete, are in registers
 #include "gemm_tile.cuh"
 #include "linear4.h"
+
+#include <cstdlib>
 
 namespace {
 
@@ -18,15 +24,16 @@ using namespace lb_tc;
 using namespace lb_tile;
 using namespace lb_w4;
 
-constexpr int kMakers = 8, kFirstMaker = 4, kThreads = 32 * (kFirstMaker + kMakers), kGroups = kMakers / 4;
+constexpr int kFirstMaker = 4;
 constexpr int kMaxStages = 6, kStageColumns = kTileK / 2;
 constexpr int kLaneRows = 128;
 
 struct Control {
-    uint64_t a_full[kMaxStages];      // weights in tensor memory
-    uint64_t b_full[kMaxStages];      // activations in shared memory
+    uint64_t a_full[kMaxStages];
+    uint64_t b_full[kMaxStages];
     uint64_t empty[kMaxStages];
-    uint64_t acc_ready;
+    uint64_t acc_full;
+    uint64_t acc_empty;
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -56,6 +63,27 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8_ask(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+// The wait for a load, tied to its registers so that nothing is made of them before it.
+__device__ __forceinline__ void tmem_ld8_wait(uint32_t (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]) :: "memory");
+}
+
+// A long wait that leaves the issue slots to others; bounded as mbar_wait is.
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+        __nanosleep(200);
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag != 0 || clock64() - t0 > kWaitLimitCycles) return false;
+    }
 }
 
 // Weights 2p and 2p + 1 of a word times their scale.  bfloat16: u in bits 3 to 6 under the exponent of 16 is 16 + u; float16: in bits 4 to 7 under that of 64 it is 64 + u.
@@ -91,19 +119,140 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
     else return __ldg(reinterpret_cast<const uint32_t*>(p));
 }
 
-// gridDim.x = blocks of 128 rows x splits (a cluster), gridDim.y = tiles of `tokens` tokens (a multiple of 16).
-template <typename T, int GROUP>
-__global__ void __launch_bounds__(kThreads)
-many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 w, const Epilogue e, int k_tiles, int tokens, int splits, int n_stages, int d_columns,
-                   int tmem_columns, int withhold, int* status) {
+// The epilogue's activations on eight sums; results that are rounded to bfloat16 take the fast exponential and division (gemm_tile.cuh).  What is long stays out of line:
+// the makers' loop and this code share the instruction cache.
+__device__ __noinline__ float activate_long(float v, int act, bool exact, float a, float b) {
+    const lb_act_pair pair{a, b};
+    if (exact) return lb_activate(v, act, pair);
+    return act == LB_ACT_XIELU ? activate<LB_ACT_XIELU, true>(v, pair) : activate<LB_ACT_GELU_ERF, true>(v, pair);
+}
+__device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exact, const lb_act_pair& pair) {
+    if (act == LB_ACT_RELU2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = activate<LB_ACT_RELU2, true>(y[i], pair);
+    } else if (act == LB_ACT_GELU_TANH && !exact) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = activate<LB_ACT_GELU_TANH, true>(y[i], pair);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = activate_long(y[i], act, exact, pair.a, pair.b);
+    }
+}
+__device__ __noinline__ float gated_exact(float g, float u, int kind, float alpha, float limit) { return lb_gated_pair(g, u, kind, alpha, limit); }
+// gate(g) u of lb_gated_pair with the fast exponential and division (relative error about 1e-6), for results that are rounded to bfloat16; the gate is told apart once for four.
+__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + __expf(-fmaxf(v, -80.0f))); }        // (the division by an infinity is none)
+__device__ __forceinline__ void gated_four(float (&z)[4], const float (&g)[4], const float (&u)[4], int kind, float alpha, float limit) {
+    auto all = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = f(g[i], u[i]);
+    };
+    if (kind == LB_GATE_SILU) all([](float x, float y) { return x * sigmoid_fast(x) * y; });
+    else if (kind == LB_GATE_GELU_TANH) all([](float x, float y) { return x * sigmoid_fast(x * fmaf(0.07135481282553524f * x, x, 1.5957691216057308f)) * y; });
+    else if (kind == LB_GATE_RELU) all([](float x, float y) { return fmaxf(x, 0.0f) * y; });
+    else if (kind == LB_GATE_SIGMOID) all([](float x, float y) { return sigmoid_fast(x) * y; });
+    else
+        all([&](float x, float y) {
+            x = fminf(x, limit);
+            return x * sigmoid_fast(alpha * x) * (fminf(fmaxf(y, -limit), limit) + 1.0f);
+        });
+}
+
+// What happens to the sums of a row (a lane) and eight tokens.  Of paired rows lanes 8 apart hold a feature's two sums, and each of them finishes one of two tokens.
+struct RowEnd {
+    int col, up;
+    float factor, bias;
+    __device__ __forceinline__ RowEnd(const Epilogue& e, const lb_weights4& w, int row, int lane, bool used) {
+        up = lane >> 3 & 1;
+        col = w.paired ? row / 16 * 8 + (row & 7) : row;
+        factor = used ? w.rows[row] : 0.0f;
+        bias = used && e.bias != nullptr && col < e.n ? __ldg(e.bias + col) : 0.0f;
+    }
+    template <int COUNT, typename O>
+    static __device__ __forceinline__ void put(O* o, int64_t step, const float (&y)[COUNT], int n) {
+        if (n >= COUNT) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i, o += step) *o = lb_from_float<O>(y[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i, o += step)
+                if (i < n) *o = lb_from_float<O>(y[i]);
+        }
+    }
+    __device__ __forceinline__ void finish(const Epilogue& e, bool paired, const lb_act_pair& pair, float (&y)[8], int token) const {
+        const int n = e.M - token;               // at least one
+        if (e.a_scale != nullptr) {
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = __ldg(e.a_scale + token + min(i, n - 1));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] *= factor * s[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] *= factor;
+        }
+        if (paired) {
+            float g[4], u[4], z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float other = __shfl_xor_sync(0xffffffffu, up ? y[2 * i] : y[2 * i + 1], 8);
+                g[i] = up ? other : y[2 * i];
+                u[i] = up ? y[2 * i + 1] : other;
+            }
+            if (!e.out_f32) {
+                gated_four(z, g, u, e.gate, e.alpha, e.limit);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = gated_exact(g[i], u[i], e.gate, e.alpha, e.limit);
+            }
+            if (col >= e.n) return;
+            const int64_t at = (int64_t)(token + up) * e.ldo + col;
+            const int rows = n >= 8 ? 4 : (n - up + 1) / 2;
+            if (e.out_f32) put<4>(static_cast<float*>(e.out) + at, 2 * e.ldo, z, rows);
+            else put<4>(static_cast<__nv_bfloat16*>(e.out) + at, 2 * e.ldo, z, rows);
+            return;
+        }
+        if (col >= e.n) return;
+        if (e.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] += bias;
+        }
+        if (e.act != LB_ACT_NONE) activate_eight(y, e.act, e.out_f32, pair);
+        if (e.residual != nullptr) {
+            const float* r = e.residual + (int64_t)token * e.ldr + col;
+            float add[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add[i] = r[min(i, n - 1) * e.ldr];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] += add[i];
+        }
+        const int64_t at = (int64_t)token * e.ldo + col;
+        if (e.out_f32) put<8>(static_cast<float*>(e.out) + at, e.ldo, y, n);
+        else put<8>(static_cast<__nv_bfloat16*>(e.out) + at, e.ldo, y, n);
+    }
+};
+
+// How the tiles lie: token tiles of a row block one after another.
+struct Tiles {
+    int tokens, token_tiles, total, k_tiles, splits, n_stages, d_columns;
+};
+
+template <int MAKERS, bool WALK>
+constexpr int threads_of() { return 32 * (kFirstMaker + MAKERS + (WALK ? 8 : 0)); }
+
+// WALK: a block walks the tiles blockIdx.x, blockIdx.x + gridDim.x, ..; else gridDim.x = tiles x splits, the splits of a tile a cluster.
+template <typename T, int GROUP, int MAKERS, bool WALK>
+__global__ void __launch_bounds__(threads_of<MAKERS, WALK>())
+many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 w, const Epilogue e, const Tiles tiles, int tmem_columns, int withhold, int* status) {
+    constexpr int kGroups = MAKERS / 4;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int tokens = tiles.tokens, splits = WALK ? 1 : tiles.splits, n_stages = tiles.n_stages, k_tiles = tiles.k_tiles;
     const uint32_t atom_bytes = (uint32_t)tokens * 128u, stage_bytes = 2 * atom_bytes;
     Control* c = reinterpret_cast<Control*>(base + max((uint32_t)n_stages * stage_bytes, splits > 1 ? (uint32_t)tokens * 512u : 0u));
     float* inbox = reinterpret_cast<float*>(base);                     // [rank][share's tokens][128 rows], over the stages when their products are done
     volatile int* abort_flag = &c->abort_flag;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int rank = (int)blockIdx.x % splits, row0 = (int)blockIdx.x / splits * kLaneRows, m0 = (int)blockIdx.y * tokens;
+    const int rank = WALK ? 0 : (int)blockIdx.x % splits, first = WALK ? (int)blockIdx.x : (int)blockIdx.x / splits, stride = WALK ? (int)gridDim.x : tiles.total;
     const int per = (k_tiles + splits - 1) / splits, kt0 = rank * per, n_kt = min(k_tiles, kt0 + per) - kt0;     // the host leaves no rank without one
 
     if (threadIdx.x == 0) {
@@ -113,7 +262,8 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             mbar_init(&c->b_full[i], 1);
             mbar_init(&c->empty[i], 1);
         }
-        mbar_init(&c->acc_ready, 1);
+        mbar_init(&c->acc_full, 1);
+        mbar_init(&c->acc_empty, 8);
         c->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -124,7 +274,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = __shfl_sync(0xffffffffu, c->tmem_base, 0), tmem_a = tmem_base + d_columns;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, c->tmem_base, 0), tmem_a = tmem_base + tiles.d_columns;
     const uint32_t stages_u32 = smem_u32(base), a_full = smem_u32(&c->a_full[0]), b_full = smem_u32(&c->b_full[0]), empty = smem_u32(&c->empty[0]);
     const int quarter = warp & 3, group = (warp - kFirstMaker) >> 2, row = quarter * 32 + lane;
     bool ok = true;
@@ -134,174 +284,246 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         lb_dependents_may_launch();
         int issued = 0, st = 0;
         uint32_t parity = 1;                                           // a stage's first use waits for nothing
-        for (int kt = 0; kt < n_kt; ++kt) {
-            if (!__all_sync(0xffffffffu, wait_u32(empty + 8 * st, parity, abort_flag))) {
-                give_up(c, status, 1, st);
-                break;
-            }
-            if (elect_one()) {
-                expect_tx_u32(b_full + 8 * st, stage_bytes);
-                tma_load_u32(stages_u32 + st * stage_bytes, &map_a, b_full + 8 * st, (kt0 + kt) * kTileK, m0);
-                tma_load_u32(stages_u32 + st * stage_bytes + atom_bytes, &map_a, b_full + 8 * st, (kt0 + kt) * kTileK + kBlockK, m0);
-            }
-            issued = kt + 1;
-            if (++st == n_stages) {
-                st = 0;
-                parity ^= 1;
+        for (int tile = first; tile < tiles.total && ok; tile += stride) {
+            const int m0 = tile % tiles.token_tiles * tokens;
+            for (int kt = 0; kt < n_kt; ++kt) {
+                if (!__all_sync(0xffffffffu, wait_u32(empty + 8 * st, parity, abort_flag))) {
+                    give_up(c, status, 1, st);
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
+                    expect_tx_u32(b_full + 8 * st, stage_bytes);
+                    tma_load_u32(stages_u32 + st * stage_bytes, &map_a, b_full + 8 * st, (kt0 + kt) * kTileK, m0);
+                    tma_load_u32(stages_u32 + st * stage_bytes + atom_bytes, &map_a, b_full + 8 * st, (kt0 + kt) * kTileK + kBlockK, m0);
+                }
+                ++issued;
+                if (++st == n_stages) {
+                    st = 0;
+                    parity ^= 1;
+                }
             }
         }
         // Leave no copy in flight: the barriers of the last loads complete when their bytes landed.
         if (*abort_flag != 0)
-            for (int kt = max(0, issued - n_stages); kt < issued; ++kt) mbar_wait(&c->b_full[kt % n_stages], (kt / n_stages) & 1, nullptr);
+            for (int i = max(0, issued - n_stages); i < issued; ++i) mbar_wait(&c->b_full[i % n_stages], (i / n_stages) & 1, nullptr);
     } else if (warp == 1) {
-        const uint32_t columns = (uint32_t)min(tokens, (e.M - m0 + 15) / 16 * 16);
-        const uint32_t idesc = T::kHalf ? umma_idesc(kLaneRows, (int)columns) & ~((1u << 7) | (1u << 10)) : umma_idesc(kLaneRows, (int)columns);
         const uint32_t desc_hi = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
         const uint32_t lo0 = ((stages_u32 & 0x3FFFFu) >> 4) | (1u << 16);
         int st = 0;
-        uint32_t parity = 0;
-        for (int kt = 0; kt < n_kt; ++kt) {
-            if (!__all_sync(0xffffffffu, wait_u32(b_full + 8 * st, parity, abort_flag) && wait_u32(a_full + 8 * st, parity, abort_flag))) {
-                give_up(c, status, 2, st);
-                ok = false;
-                break;
+        uint32_t parity = 0, acc_parity = 1;
+        for (int tile = first; tile < tiles.total && ok; tile += stride, acc_parity ^= 1) {
+            const int columns = min(tokens, (e.M - tile % tiles.token_tiles * tokens + 15) / 16 * 16);
+            const uint32_t idesc = umma_idesc(kLaneRows, columns) & (T::kHalf ? ~((1u << 7) | (1u << 10)) : ~0u);
+            if (WALK) {
+                if (!__all_sync(0xffffffffu, wait_u32(smem_u32(&c->acc_empty), acc_parity, abort_flag))) {
+                    give_up(c, status, 5, 0);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
             }
-            tc_fence_after();
-            const uint32_t b_lo = lo0 + (uint32_t)st * (stage_bytes >> 4), ta = tmem_a + st * kStageColumns;
-            if (elect_one()) {
+            for (int kt = 0; kt < n_kt; ++kt) {
+                if (!__all_sync(0xffffffffu, wait_u32(b_full + 8 * st, parity, abort_flag) && wait_u32(a_full + 8 * st, parity, abort_flag))) {
+                    give_up(c, status, 2, st);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t b_lo = lo0 + (uint32_t)st * (stage_bytes >> 4), ta = tmem_a + st * kStageColumns;
+                if (elect_one()) {
 #pragma unroll
-                for (uint32_t k = 0; k < kTileK / kUmmaK; ++k)
-                    umma_ts(tmem_base, ta + k * (kUmmaK / 2), b_lo + (k >> 2) * (atom_bytes >> 4) + 2 * (k & 3), desc_hi, idesc, kt + k != 0 ? 1u : 0u);
-                commit_u32(empty + 8 * st);
+                    for (uint32_t k = 0; k < kTileK / kUmmaK; ++k)
+                        umma_ts(tmem_base, ta + k * (kUmmaK / 2), b_lo + (k >> 2) * (atom_bytes >> 4) + 2 * (k & 3), desc_hi, idesc, kt + k != 0 ? 1u : 0u);
+                    commit_u32(empty + 8 * st);
+                }
+                if (++st == n_stages) {
+                    st = 0;
+                    parity ^= 1;
+                }
             }
-            if (++st == n_stages) {
-                st = 0;
-                parity ^= 1;
-            }
+            // (`withhold`: a test's launch, whose epilogues find nothing and give up.)
+            if (ok && withhold == 0 && elect_one()) umma_commit(&c->acc_full);
         }
-        // (`withhold`: a test's launch, whose epilogues find nothing and give up.)
-        if (ok && withhold == 0 && elect_one()) umma_commit(&c->acc_ready);
         lb_wait_for_predecessor();
         lb_dependents_may_launch();
-    } else if (warp >= kFirstMaker) {
+    } else if (warp >= kFirstMaker && group < kGroups) {
         constexpr int kPerTile = kTileK / GROUP;
-        const size_t tile0 = (size_t)((row0 + row) >> 4) * k_tiles + kt0;
-        const uint4* from = static_cast<const uint4*>(w.nibbles) + tile0 * (kTileBytes / 16) + (row & 15);
-        const uint8_t* scales = static_cast<const uint8_t*>(w.scales) + (tile0 * kTileRows + (row & 15)) * kPerTile;
         uint32_t mask, magic;
         asm volatile("mov.b32 %0, %2;\n\tmov.b32 %1, %3;" : "=r"(mask), "=r"(magic) : "n"(T::kHalf ? 0x00F000F0 : 0x00780078), "n"(T::kHalf ? 0x54005400 : 0x41804180));
+        // No more warps take turns than there are stages: one that was a whole round of the stages ahead would take the parity of the round before for its own.
+        const int turns = min(kGroups, n_stages);
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         uint4 words[2][4];
         uint32_t steps[2];
-        auto fetch = [&](int i, int kt) {
-            if (kt < n_kt) {
+        // The k tiles of all of this block's tiles are one sequence, of which this warp takes every turns-th; `ahead` is where the next to be fetched lies.
+        int ahead_tile = first, ahead_kt = group;
+        const uint4* from = nullptr;
+        const uint8_t* scales = nullptr;
+        auto aim = [&]() {
+            while (WALK && ahead_kt >= n_kt && ahead_tile < tiles.total) {
+                ahead_kt -= n_kt;
+                ahead_tile += stride;
+            }
+            const size_t at = (size_t)((ahead_tile / tiles.token_tiles * kLaneRows + row) >> 4) * k_tiles + kt0 + ahead_kt;
+            from = static_cast<const uint4*>(w.nibbles) + at * (kTileBytes / 16) + (row & 15);
+            scales = static_cast<const uint8_t*>(w.scales) + (at * kTileRows + (row & 15)) * kPerTile;
+        };
+        auto fetch = [&](int i) {
+            if (ahead_tile < tiles.total && ahead_kt < n_kt) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) words[i][t] = __ldg(from + kt * (kTileBytes / 16) + 16 * t);
-                steps[i] = load_scales<GROUP>(scales + kt * kTileRows * kPerTile);
+                for (int t = 0; t < 4; ++t) words[i][t] = __ldg(from + 16 * t);
+                if constexpr (GROUP == 128) steps[i] = __ldg(scales);
+                else if constexpr (GROUP == 64) steps[i] = __ldg(reinterpret_cast<const uint16_t*>(scales));
+                else steps[i] = __ldg(reinterpret_cast<const uint32_t*>(scales));
+                ahead_kt += turns;
+                from += turns * (kTileBytes / 16);
+                scales += turns * kTileRows * kPerTile;
+                if (ahead_kt >= n_kt && WALK) aim();
             }
         };
-        fetch(0, group);
-        fetch(1, group + kGroups);
-        int st = group % n_stages;
-        uint32_t parity = (group / n_stages & 1) ^ 1;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        for (int kt = group, i = 0; kt < n_kt; kt += kGroups, i ^= 1) {
+        if (group < turns) {
+            aim();
+            fetch(0);
+            fetch(1);
+        }
+        int st = group, tile = first, kt = group;
+        uint32_t parity = 1;
+        auto make = [&](int i) {
             if (!__all_sync(0xffffffffu, wait_u32(empty + 8 * st, parity, abort_flag))) {
                 give_up(c, status, 4, st);
                 ok = false;
-                break;
+                return;
             }
             tc_fence_after();
-            auto make = [&](int i) {
-                uint32_t s = 0, minus = 0;
+            const uint32_t to = __shfl_sync(0xffffffffu, tmem_a + lanes + st * kStageColumns, 0);       // one number for the warp
+            uint32_t s = 0, minus = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j * 32 % GROUP == 0) scale_pair<T>(steps[i] >> (8 * (j * 32 / GROUP)), s, minus);
-                    uint32_t v[16];
+            for (int j = 0; j < 4; ++j) {
+                if (j * 32 % GROUP == 0) scale_pair<T>(steps[i] >> (8 * (j * 32 / GROUP)), s, minus);
+                uint32_t v[16];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t word = j == 0 ? words[i][t].x : j == 1 ? words[i][t].y : j == 2 ? words[i][t].z : words[i][t].w;
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t word = j == 0 ? words[i][t].x : j == 1 ? words[i][t].y : j == 2 ? words[i][t].z : words[i][t].w;
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) v[4 * t + p] = scaled_pair<T>(word, p, mask, magic, s, minus);
-                    }
-                    tmem_st16(tmem_a + lanes + st * kStageColumns + 16 * j, v);
+                    for (int p = 0; p < 4; ++p) v[4 * t + p] = scaled_pair<T>(word, p, mask, magic, s, minus);
                 }
-                fetch(i, kt + 2 * kGroups);
-            };
-            if (i == 0) make(0);
-            else make(1);
+                tmem_st16(to + 16 * j, v);
+            }
+            fetch(i);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&c->a_full[st]);
-            st += kGroups;
+            st += turns;
             if (st >= n_stages) {
                 st -= n_stages;
                 parity ^= 1;
             }
+            kt += turns;
+            while (WALK && kt >= n_kt && tile < tiles.total) {
+                kt -= n_kt;
+                tile += stride;
+            }
+        };
+        if (WALK)
+            while (kt >= n_kt && tile < tiles.total) {
+                kt -= n_kt;
+                tile += stride;
+            }
+        while (group < turns && ok && tile < tiles.total && kt < n_kt) {
+            make(0);
+            if (!(ok && tile < tiles.total && kt < n_kt)) break;
+            make(1);
         }
-        lb_wait_for_predecessor();           // before scales and residuals are read and anything is written
-        lb_dependents_may_launch();
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&c->acc_ready, 0, abort_flag));
-        if (!ok) give_up(c, status, 3, quarter);
-        tc_fence_after();
     }
     __syncwarp();
-    // A row's factor; of paired rows lanes 8 apart hold a feature's two sums, and each of them finishes one of two tokens.
-    const bool finishes = warp >= kFirstMaker && ok;
-    const float factor = finishes ? w.rows[row0 + row] : 0.0f;
-    const lb_act_pair pair = finishes && !w.paired ? lb_act_load(e.bias, e.n, e.act) : lb_act_pair{0.0f, 0.0f};
-    const int up = lane >> 3 & 1, col = w.paired ? (row0 + row) / 16 * 8 + (row & 7) : row0 + row;
-    auto finish_eight = [&](const float (&y)[8], int token) {
-        if (w.paired) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float v0 = y[i] * factor, v1 = y[i + 1] * factor, other = __shfl_xor_sync(0xffffffffu, up ? v0 : v1, 8);
-                const int m = token + i + up;
-                if (m >= e.M || col >= e.n) continue;
-                const float s = e.a_scale != nullptr ? e.a_scale[m] : 1.0f;
-                store_out(e, m, col, lb_gated_pair((up ? other : v0) * s, (up ? v1 : other) * s, e.gate, e.alpha, e.limit));
-            }
-        } else if (col < e.n) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (token + i < e.M) finish_one(e, pair, token + i, col, y[i] * (factor * (e.a_scale != nullptr ? e.a_scale[token + i] : 1.0f)));
-        }
-    };
+
+    const bool finisher = WALK ? warp >= kFirstMaker + MAKERS : warp >= kFirstMaker;
     const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const int here = min(tokens, e.M - m0);
-    if (splits > 1) {
-        // Every block's products are complete before their stages are written over.
-        const int share = tokens / splits;
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (finishes) {
+    const lb_act_pair pair = finisher && !w.paired ? lb_act_load(e.bias, e.n, e.act) : lb_act_pair{0.0f, 0.0f};
+    if (WALK) {
+        if (finisher) {
+            const int half = (warp - kFirstMaker - MAKERS) >> 2;       // this warp's 32 columns of every 64
+            lb_wait_for_predecessor();           // before scales and residuals are read and anything is written
+            lb_dependents_may_launch();
+            uint32_t parity = 0;
+            for (int tile = first; tile < tiles.total; tile += stride, parity ^= 1) {
+                const int m0 = tile % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
+                const RowEnd end(e, w, tile / tiles.token_tiles * kLaneRows + row, lane, true);
+                if (!__all_sync(0xffffffffu, wait_asleep(&c->acc_full, parity, abort_flag))) {
+                    give_up(c, status, 3, quarter);
+                    break;
+                }
+                tc_fence_after();
+                // Eights of columns in turn, the next one on its way; when the last is there the next tile's products may begin.
+                uint32_t v[8];
+                int at = 8 * half;
+                if (at < here) tmem_ld8_ask(t_row + at, v);
+#pragma unroll 1
+                for (; at < here || at == 8 * half; at += 16) {
+                    tmem_ld8_wait(v);
+                    float y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[k]);
+                    if (at + 16 < here) {
+                        tmem_ld8_ask(t_row + at + 16, v);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&c->acc_empty);
+                    }
+                    if (at < here) end.finish(e, w.paired, pair, y, m0 + at);
+                }
+            }
+        }
+    } else {
+        if (finisher) {
+            lb_wait_for_predecessor();
+            lb_dependents_may_launch();
+            ok = __all_sync(0xffffffffu, ok && (mbar_wait(&c->acc_full, 0, abort_flag)));
+            if (!ok) give_up(c, status, 3, quarter);
+            tc_fence_after();
+        }
+        __syncwarp();
+        const bool finishes = finisher && ok;
+        const int m0 = first % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
+        const RowEnd end(e, w, first / tiles.token_tiles * kLaneRows + row, lane, finishes);
+        if (splits > 1) {
+            // Every block's products are complete before their stages are written over.
+            const int share = tokens / splits;
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (finishes) {
+                for (int at = 8 * group; at < here; at += 8 * kGroups) {
+                    uint32_t v[8];
+                    tmem_ld8(t_row + at, v);
+                    const int to = at / share;
+                    const uint32_t peer = peer_address(smem_u32(inbox + (size_t)(rank * share + at - to * share) * kLaneRows + row), (uint32_t)to);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(peer + i * kLaneRows * 4), "r"(v[i]) : "memory");
+                }
+            }
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (finishes) {
+                for (int at = 8 * group; at < share && rank * share + at < here; at += 8 * kGroups) {
+                    float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    for (int r = 0; r < splits; ++r)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] += inbox[(size_t)(r * share + at + i) * kLaneRows + row];
+                    end.finish(e, w.paired, pair, y, m0 + rank * share + at);
+                }
+            }
+        } else if (finishes) {
+#pragma unroll 1
             for (int at = 8 * group; at < here; at += 8 * kGroups) {
                 uint32_t v[8];
                 tmem_ld8(t_row + at, v);
-                const int to = at / share;
-                uint32_t peer = peer_address(smem_u32(inbox + (size_t)(rank * share + at - to * share) * kLaneRows + row), (uint32_t)to);
+                float y[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(peer + i * kLaneRows * 4), "r"(v[i]) : "memory");
+                for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+                end.finish(e, w.paired, pair, y, m0 + at);
             }
-        }
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (finishes) {
-            for (int at = 8 * group; at < share && rank * share + at < here; at += 8 * kGroups) {
-                float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                for (int r = 0; r < splits; ++r)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] += inbox[(size_t)(r * share + at + i) * kLaneRows + row];
-                finish_eight(y, m0 + rank * share + at);
-            }
-        }
-    } else if (finishes) {
-        for (int at = 8 * group; at < here; at += 8 * kGroups) {
-            uint32_t v[8];
-            tmem_ld8(t_row + at, v);
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
-            finish_eight(y, m0 + at);
         }
     }
     __syncwarp();
@@ -329,41 +551,50 @@ __global__ void spread_rows_kernel(const void* __restrict__ a, int64_t lda, bool
 
 int g_withhold_next = 0;      // the next launch's blocks leave their accumulator-ready barriers unsignalled (tests)
 
-template <typename T, int GROUP>
-int launch(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, int row_blocks, int token_tiles, int k_tiles, cudaStream_t s) {
+template <typename T, int GROUP, int MAKERS, bool WALK>
+int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
+    auto kernel = many_tokens_kernel<T, GROUP, MAKERS, WALK>;
     static bool configured = false;
     if (!configured) {
-        LB_CHECK_CUDA(cudaFuncSetAttribute(many_tokens_kernel<T, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         configured = true;
     }
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
-    LB_CHECK_CUDA(lb_launch_overlapped_cluster(1, p.splits, many_tokens_kernel<T, GROUP>, dim3(row_blocks * p.splits, token_tiles), dim3(kThreads), p.smem, s, map, *w, e,
-                                               k_tiles, p.tokens, p.splits, p.stages, p.d_columns, p.tmem_columns, g_withhold_next, status));
+    const int blocks = WALK ? (tiles.total < n_sm ? tiles.total : n_sm) : tiles.total * p.splits;
+    LB_CHECK_CUDA(lb_launch_overlapped_cluster(1, p.splits, kernel, dim3(blocks), dim3(threads_of<MAKERS, WALK>()), p.smem, s, map, *w, e, tiles, p.tmem_columns, g_withhold_next,
+                                               status));
     g_withhold_next = 0;
     return LB_OK;
 }
 
+template <typename T, int GROUP>
+int launch(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
+    return p.walk ? launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
+}
+
 template <typename T>
 int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, void* scratch, cudaStream_t s) {
-    const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, row_blocks = (rows + kLaneRows - 1) / kLaneRows;
+    const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, row_blocks = (rows + kLaneRows - 1) / kLaneRows, n_sm = linear4_sm_count();
     if (many_scratch_bytes(w, T::kHalf ? LB_E4M3 : LB_BF16, a, lda, e.M) > 0) {
         LB_CHECK_ARG(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "linear4: these activations need scratch memory (lb_linear4_scratch)");
         const bool wide = lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % (T::kHalf ? 8 : 16) == 0;
         const int eights = (w->k + 7) / 8;
         const int64_t all = (int64_t)e.M * eights, blocks = (all + 255) / 256;
-        LB_CHECK_CUDA(lb_launch_overlapped(spread_rows_kernel<T>, dim3((unsigned)(blocks < 2368 ? blocks : 2368)), dim3(256), 0, s, a, lda, wide,
+        LB_CHECK_CUDA(lb_launch_overlapped(spread_rows_kernel<T>, dim3((unsigned)(blocks < 16 * n_sm ? blocks : 16 * n_sm)), dim3(256), 0, s, a, lda, wide,
                                            static_cast<uint4*>(scratch), eights, all, w->k));
         a = scratch;
         lda = 8 * (int64_t)eights;
     }
-    const ManyPlan p = many_plan(e.M, rows, w->k, linear4_sm_count());
+    const ManyPlan p = many_plan(e.M, rows, w->k, n_sm);
     CUtensorMap map;
     if (int rc = lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k, lda, p.tokens)) return rc;
     const int token_tiles = (e.M + p.tokens - 1) / p.tokens;
-    if (w->group == 32) return launch<T, 32>(map, w, e, p, row_blocks, token_tiles, k_tiles, s);
-    if (w->group == 64) return launch<T, 64>(map, w, e, p, row_blocks, token_tiles, k_tiles, s);
-    return launch<T, 128>(map, w, e, p, row_blocks, token_tiles, k_tiles, s);
+    LB_CHECK_ARG((int64_t)token_tiles * row_blocks * p.splits < (1ll << 30), "linear4: %d rows by %d features are too many tiles", e.M, rows);
+    const Tiles tiles{p.tokens, token_tiles, token_tiles * row_blocks, k_tiles, p.splits, p.stages, p.d_columns};
+    if (w->group == 32) return launch<T, 32>(map, w, e, p, tiles, n_sm, s);
+    if (w->group == 64) return launch<T, 64>(map, w, e, p, tiles, n_sm, s);
+    return launch<T, 128>(map, w, e, p, tiles, n_sm, s);
 }
 
 }  // namespace
@@ -375,14 +606,20 @@ ManyPlan many_plan(int M, int rows, int k, int n_sm) {
     p.splits = 1;
     while (p.splits < 8 && tiles * row_blocks * p.splits * 2 <= n_sm && k_tiles >= 4 * p.splits && (k_tiles + 2 * p.splits - 1) / (2 * p.splits) * (2 * p.splits - 1) < k_tiles)
         p.splits *= 2;
+    if (getenv("MANY_S")) p.splits = atoi(getenv("MANY_S"));
+    if (getenv("MANY_N")) p.tokens = atoi(getenv("MANY_N"));
     // The tokens are shared out in eights between the ranks.
     if (p.splits > 1) p.tokens = (p.tokens + 8 * p.splits - 1) / (8 * p.splits) * (8 * p.splits);
     if (p.tokens > 256) p.tokens = 256;
+    const long total = (long)((M + p.tokens - 1) / p.tokens) * row_blocks;
+    p.walk = p.splits == 1 && total > n_sm;
+    if (getenv("MANY_W")) p.walk = atoi(getenv("MANY_W"));
     p.d_columns = p.tokens <= 64 ? 64 : p.tokens <= 128 ? 128 : 256;
-    p.stages = p.d_columns == 128 ? 6 : 3;
-    p.tmem_columns = p.d_columns == 64 ? 256 : 512;
+    p.stages = p.d_columns <= 128 ? 6 : 3;
+    p.tmem_columns = 512;
     // The blocks of a cluster wait for one another while each holds its columns: as large a share of the shared memory as of the columns (see gemm_tcgen05_narrow.cu).
-    const int needed = 1024 + p.stages * p.tokens * 256 + (p.splits > 1 && p.tokens * 512 > p.stages * p.tokens * 256 ? p.tokens * 512 - p.stages * p.tokens * 256 : 0) + (int)sizeof(Control);
+    const int in_stages = p.stages * p.tokens * 256, inbox = p.splits > 1 ? p.tokens * 512 : 0;
+    const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control);
     const int least = p.tmem_columns * (228 * 1024 / 512) - 1024;
     p.smem = needed < least ? least : needed;
     return p;

@@ -127,6 +127,37 @@ def test_linear(dev, m, n, k, group, eight):
     assert half[:, n:].isnan().all()
 
 
+@pytest.mark.parametrize("m,n,k,group", [(20, 19100, 160, 32), (33, 25000, 64, 64), (130, 12900, 333, 128), (600, 7001, 200, 64), (2500, 1600, 1100, 128), (257, 19000, 129, 32)])
+@pytest.mark.parametrize("eight", [False, True])
+def test_many_tiles(dev, m, n, k, group, eight):
+    """More tiles than SMs, with remainders of rows, tokens and k tiles; as a gated product too."""
+    from liyab_b200 import ops
+    q, s, r = _parts(n, k, group, dev, seed=m)
+    w, ref_w = ops.lay_out_weights4(q, s, r, group), _matrix(q, s, r, group)
+    a, scale = _rand((m, k), 14, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    bias = _rand((n,), 15, dev)
+    ref = rows @ ref_w.T
+    size = rows.abs() @ ref_w.abs().T
+    out = torch.full((m, n), float("nan"), device=dev)
+    ops.linear4(a, w, bias, out, m, a_scale=scale)
+    assert ops.device_status() == 0
+    assert ((out.double() - ref - bias.double()).abs() <= _sum_bound(k) * (size + bias.double().abs())).all()
+    if n % 2 == 0:
+        f = n // 2
+        half = torch.full((m, f), float("nan"), dtype=torch.bfloat16, device=dev)
+        ops.gated4(a, ops.lay_out_weights4(q, s, r, group, paired=True), half, m, gate="relu", a_scale=scale)
+        assert ops.device_status() == 0
+        want, eg, eu = ref[:, :f].clamp(min=0) * ref[:, f:], _sum_bound(k) * size[:, :f], _sum_bound(k) * size[:, f:]
+        bound = eg * (ref[:, f:].abs() + eu) + ref[:, :f].abs() * eu
+        assert ((half.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+
+
 @pytest.mark.parametrize("m", [1, 5, 16, 40, 129])
 @pytest.mark.parametrize("activation", ["gelu_tanh", "gelu_erf", "xielu", "relu2", "none"])
 def test_activations(dev, m, activation):
