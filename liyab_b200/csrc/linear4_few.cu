@@ -2,7 +2,7 @@
 //
 // The weights are the rows of mma.sync (16 of them by 16 k), the tokens its columns (8 a tile, NT tiles).  A block owns a stretch of row tiles; its activations
 // lie in shared memory in the order of the operand.  Row tiles by k tiles of 128 are one sequence that the block's warps cut into equal parts, whatever
-// the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, AHEAD tiles on the way), makes a register of two weights of a shift, a mask and a
+// the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, four tiles on the way), makes a register of two weights of a shift, a mask and a
 // subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
 // After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
 #include "linear4.h"
@@ -13,6 +13,8 @@ namespace {
 using namespace lb_w4;
 using lb_tc::smem_u32;
 
+constexpr int kMostWarps = 16;
+constexpr int kAhead = 4;                // k tiles on the way a warp
 constexpr int kRound = 32;               // row tiles between two barriers
 
 __device__ __forceinline__ uint4 load_weights(const uint4* p) {
@@ -47,12 +49,13 @@ struct Layout {
     }
 };
 
-// AHEAD: k tiles on the way a warp; SPLIT: the cluster's blocks share the reduction.
-template <typename T, int NT, int GROUP, int AHEAD, bool SPLIT>
-__global__ void __launch_bounds__(AHEAD > 2 ? 512 : 1024)
+// SPLIT: the cluster's blocks share the reduction.
+template <typename T, int NT, int GROUP, bool SPLIT>
+__global__ void __launch_bounds__(32 * kMostWarps)
 few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, bool wide, const Epilogue e, int n_tiles, int k_tiles, int splits, int round_tiles) {
     constexpr int kSlot = 128 * NT, kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile;
     extern __shared__ __align__(128) uint8_t shared[];
+    __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[8 * NT];                       // of this round's rows, of the tokens
     __shared__ int parts_of[kRound][2];                                                               // the first and the last warp of a row tile
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_warps = blockDim.x >> 5;
     const int rank = SPLIT ? (int)blockIdx.x % splits : 0, cluster = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, clusters = SPLIT ? (int)gridDim.x / splits : (int)gridDim.x;
@@ -66,8 +69,8 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
     int x0 = 0, x1 = 0, start = 0, kt = 0, left = 0;
     const uint4* from = nullptr;                 // of the tile that is computed next (SPLIT: of the one that is fetched next)
     const uint8_t* scales_from = nullptr;
-    uint4 words[AHEAD][2];
-    uint32_t steps[AHEAD][2];
+    uint4 words[kAhead][2];
+    uint32_t steps[kAhead][2];
     auto fetch = [&](int i, int at) {
         words[i][0] = load_weights(from + at * (kTileBytes / 16));
         words[i][1] = load_weights(from + at * (kTileBytes / 16) + 8);
@@ -91,7 +94,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
         from = static_cast<const uint4*>(w.nibbles) + tile0 * (kTileBytes / 16) + kTileRows * t + g;
         scales_from = static_cast<const uint8_t*>(w.scales) + tile0 * kScaleBytes + g * kPerTile;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
+        for (int i = 0; i < kAhead; ++i)
             if (x0 + i < x1) fetch(i, SPLIT ? 0 : i);
     };
     if (first < last) begin_round(first);
@@ -99,12 +102,20 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
     if (threadIdx.x < 16) reinterpret_cast<uint4*>(shared)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
-    for (int c = threadIdx.x; c < n_kt * 16 * e.M; c += blockDim.x) {
-        const int at = c & 3, j = c >> 2 & 3, m = (c >> 4) % e.M, k_tile = (c >> 4) / e.M;
-        uint32_t v[4];
-        load_eight<T>(v, a, (int64_t)m * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
-        reinterpret_cast<uint4*>(shared + at_of.rows_at)[(k_tile * e.M + m) * 16 + (j ^ (m & 1)) * 4 + at] = make_uint4(v[0], v[1], v[2], v[3]);
+    // Pieces of eight k by four tokens, the four on their way together.
+    const int pieces = n_kt * 16;
+    for (int q = threadIdx.x; q < pieces * ((e.M + 3) / 4); q += blockDim.x) {
+        const int m0 = q / pieces * 4, c = q - m0 / 4 * pieces, at = c & 3, j = c >> 2 & 3, k_tile = c >> 4;
+        uint4* to = reinterpret_cast<uint4*>(shared + at_of.rows_at) + (k_tile * e.M + m0) * 16 + at;
+        uint32_t v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (m0 + i < e.M) load_eight<T::kHalf>(v[i], a, (int64_t)(m0 + i) * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (m0 + i < e.M) to[i * 16 + (j ^ (i & 1)) * 4] = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
     }
+    if (threadIdx.x < 8 * NT) a_scales[threadIdx.x] = e.a_scale != nullptr && (int)threadIdx.x < e.M ? e.a_scale[threadIdx.x] : 1.0f;
 
     // This lane's activations: of a token, or the line of zeros; words of even and of odd j lie `swap` bytes further and nearer.
     uint32_t columns[NT];
@@ -119,6 +130,18 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
     for (int base = first; base < last; base += round_tiles) {
         __syncthreads();                    // the activations are there; the last round's slots have been read
         const int tiles = min(round_tiles, last - base);
+        // What the sums will meet is asked for now: the rows' factors and biases, and the residual of this thread's first unit (a token and the rows `row` and `row` + 8).
+        const int unit0 = rank * (int)blockDim.x + (int)threadIdx.x, units = tiles * 8 * e.M;
+        float add[2] = {0.0f, 0.0f};
+        if (e.residual != nullptr && unit0 < units) {
+            const int i = (unit0 >> 3) / e.M, token = (unit0 >> 3) - i * e.M, col = (base + i) * 16 + (unit0 & 7);
+            if (col < e.n) add[0] = e.residual[(int64_t)token * e.ldr + col];
+            if (col + 8 < e.n) add[1] = e.residual[(int64_t)token * e.ldr + col + 8];
+        }
+        for (int i = threadIdx.x; i < tiles * 16; i += blockDim.x) {
+            factors[i] = w.rows[base * 16 + i];
+            biases[i] = e.bias != nullptr && base * 16 + i < e.n ? __ldg(e.bias + base * 16 + i) : 0.0f;
+        }
         float acc[NT][4];
         uint32_t column[NT];
 #pragma unroll
@@ -126,13 +149,15 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
             column[n] = columns[n] + kt * column_step[n];
         }
-        int here = n_kt - kt, of = start - base;
+        const bool ends_tile = (x1 - x0 + kt) % n_kt == 0;                                            // whether this part ends where a row tile does
+        int of = start - base;
         float* slot = slots + (of + warp) * kSlot;
         if (x0 < x1 && kt == 0) parts_of[of][0] = warp;
-        for (int x = x0; x < x1; x += AHEAD) {
+        // Counted from the group of kAhead k tiles that is at hand: those to be computed, those to be fetched, and where the row tile (or this warp's part) ends.
+        int todo = x1 - x0, to_fetch = todo - kAhead, end = min(n_kt - kt, todo);
+        while (todo > 0) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (x + i >= x1) break;
+            for (int i = 0; i < kAhead; ++i) {
                 const uint4 top = words[i][0], low = words[i][1];
                 const uint32_t st = steps[i][0], sl = steps[i][1];
                 const uint32_t wt[4] = {top.x, top.y, top.z, top.w}, wl[4] = {low.x, low.y, low.z, low.w};
@@ -171,8 +196,8 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                 }
 #pragma unroll
                 for (int n8 = 0; n8 < NT; ++n8) column[n8] += column_step[n8];
-                if (x + i + AHEAD < x1) fetch(i, SPLIT ? 0 : i + AHEAD);
-                if (--here == 0 || x + i == x1 - 1) {
+                if (i < to_fetch) fetch(i, SPLIT ? 0 : i + kAhead);
+                if (end == i + 1) {
 #pragma unroll
                     for (int n8 = 0; n8 < NT; ++n8) {
                         *reinterpret_cast<float2*>(slot + g * 8 * NT + 8 * n8 + 2 * t) = make_float2(acc[n8][0], acc[n8][1]);
@@ -181,16 +206,22 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                         column[n8] = columns[n8];
                     }
                     slot += kSlot;
-                    if (here == 0) parts_of[of][1] = warp;
-                    if (x + i != x1 - 1) parts_of[++of][0] = warp;
-                    here = n_kt;
+                    const bool last_tile = todo == i + 1;
+                    if (!last_tile || ends_tile) parts_of[of][1] = warp;
+                    if (last_tile) goto done;
+                    parts_of[++of][0] = warp;
+                    end = i + 1 + min(n_kt, todo - (i + 1));
                 }
             }
+            todo -= kAhead;
+            to_fetch -= kAhead;
+            end -= kAhead;
             if (!SPLIT) {
-                from += AHEAD * (kTileBytes / 16);
-                scales_from += AHEAD * kScaleBytes;
+                from += kAhead * (kTileBytes / 16);
+                scales_from += kAhead * kScaleBytes;
             }
         }
+    done:
         if (base + round_tiles < last) begin_round(base + round_tiles);
         __syncthreads();
 
@@ -205,10 +236,9 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
         const lb_act_pair pair = w.paired ? lb_act_pair{0.0f, 0.0f} : lb_act_load(e.bias, e.n, e.act);
-        for (int u = rank * (int)blockDim.x + (int)threadIdx.x; u < tiles * 8 * e.M; u += splits * (int)blockDim.x) {
+        for (int u = unit0; u < units; u += splits * (int)blockDim.x) {
             const int i = (u >> 3) / e.M, token = (u >> 3) - i * e.M, row = u & 7, tile = base + i;
-            const float a_scale = e.a_scale != nullptr ? e.a_scale[token] : 1.0f;
-            const float factor[2] = {w.rows[tile * 16 + row] * a_scale, w.rows[tile * 16 + row + 8] * a_scale};
+            const float a_scale = a_scales[token], factor[2] = {factors[i * 16 + row] * a_scale, factors[i * 16 + row + 8] * a_scale};
             float v[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -230,7 +260,10 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int col = tile * 16 + row + 8 * h;
-                    if (col < e.n) finish_one(e, pair, token, col, v[h] * factor[h]);
+                    if (col >= e.n) continue;
+                    float y = lb_activate(fmaf(v[h], factor[h], biases[i * 16 + row + 8 * h]), e.act, pair);
+                    if (e.residual != nullptr) y += u == unit0 ? add[h] : e.residual[(int64_t)token * e.ldr + col];
+                    store_out(e, token, col, y);
                 }
             }
         }
@@ -241,9 +274,8 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
 
 template <typename T, int NT, int GROUP>
 int launch_group(const lb_weights4* w, const void* a, int64_t lda, bool wide, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
-    auto kernel = p.ahead > 2 ? (p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, 4, true> : few_tokens_kernel<T, NT, GROUP, 4, false>)
-                              : (p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, 2, true> : few_tokens_kernel<T, NT, GROUP, 2, false>);
-    if (p.smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
+    auto kernel = p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, true> : few_tokens_kernel<T, NT, GROUP, false>;
+    if (p.smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
     LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, p.splits, kernel, dim3(p.clusters * p.splits), dim3(32 * p.warps), p.smem, s, *w, a, lda, wide, e, n_tiles, k_tiles, p.splits,
                                                p.round));
     return LB_OK;
@@ -270,10 +302,9 @@ FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
         p.clusters = n_tiles < n_sm / p.splits ? n_tiles : n_sm / p.splits;
         p.round = (n_tiles + p.clusters - 1) / p.clusters;
         if (p.round > kRound) p.round = kRound;
-        const int length = p.round * per_rank, warps = length <= 16 ? 8 : length <= 256 || p.token_tiles > 1 ? 16 : 32;
-        p.ahead = warps > 16 ? 2 : 4;
+        const int length = p.round * per_rank, warps = length <= 16 ? 8 : 16;
         p.smem = Layout(M, p.token_tiles, per_rank, p.round, warps).total;
-        if (p.smem <= 224 * 1024) {
+        if (p.smem <= 216 * 1024) {
             p.warps = warps;
             return p;
         }

@@ -16,8 +16,6 @@
 #include "gemm_tile.cuh"
 #include "linear4.h"
 
-#include <cstdlib>
-
 namespace {
 
 using namespace lb_tc;
@@ -236,6 +234,9 @@ struct Tiles {
     int tokens, token_tiles, total, k_tiles, splits, n_stages, d_columns;
 };
 
+// Tokens of a tile that a rank of `splits` finishes, but for the last ones.
+__host__ __device__ __forceinline__ int share_of(int tokens, int splits) { return ((tokens + splits - 1) / splits + 7) / 8 * 8; }
+
 template <int MAKERS, bool WALK>
 constexpr int threads_of() { return 32 * (kFirstMaker + MAKERS + (WALK ? 8 : 0)); }
 
@@ -248,8 +249,8 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tokens = tiles.tokens, splits = WALK ? 1 : tiles.splits, n_stages = tiles.n_stages, k_tiles = tiles.k_tiles;
     const uint32_t atom_bytes = (uint32_t)tokens * 128u, stage_bytes = 2 * atom_bytes;
-    Control* c = reinterpret_cast<Control*>(base + max((uint32_t)n_stages * stage_bytes, splits > 1 ? (uint32_t)tokens * 512u : 0u));
-    float* inbox = reinterpret_cast<float*>(base);                     // [rank][share's tokens][128 rows], over the stages when their products are done
+    Control* c = reinterpret_cast<Control*>(base + max((uint32_t)n_stages * stage_bytes, splits > 1 ? (uint32_t)(splits * share_of(tokens, splits)) * 512u : 0u));
+    uint8_t* inbox = base;                                             // the ranks' sums, over the stages when their products are done
     volatile int* abort_flag = &c->abort_flag;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = WALK ? 0 : (int)blockIdx.x % splits, first = WALK ? (int)blockIdx.x : (int)blockIdx.x / splits, stride = WALK ? (int)gridDim.x : tiles.total;
@@ -490,28 +491,31 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         const int m0 = first % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
         const RowEnd end(e, w, first / tiles.token_tiles * kLaneRows + row, lane, finishes);
         if (splits > 1) {
-            // Every block's products are complete before their stages are written over.
-            const int share = tokens / splits;
+            // Every block's products are complete before their stages are written over.  A rank's share is a whole number of eights of tokens, the last ranks' may be none.
+            const int share = share_of(tokens, splits), eights = share / 8;
+            float4* box = reinterpret_cast<float4*>(inbox) + row;      // [rank][eight][half][128 rows] of four tokens: a warp's 16-byte stores lie side by side
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             if (finishes) {
-                for (int at = 8 * group; at < here; at += 8 * kGroups) {
+                for (int piece = group; 8 * piece < here; piece += kGroups) {
                     uint32_t v[8];
-                    tmem_ld8(t_row + at, v);
-                    const int to = at / share;
-                    const uint32_t peer = peer_address(smem_u32(inbox + (size_t)(rank * share + at - to * share) * kLaneRows + row), (uint32_t)to);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(peer + i * kLaneRows * 4), "r"(v[i]) : "memory");
+                    tmem_ld8(t_row + 8 * piece, v);
+                    const int to = piece / eights;
+                    const uint32_t peer = peer_address(smem_u32(box + (rank * eights + piece - to * eights) * 2 * kLaneRows), (uint32_t)to);
+                    store_at_peer(peer, v[0], v[1], v[2], v[3]);
+                    store_at_peer(peer + kLaneRows * 16, v[4], v[5], v[6], v[7]);
                 }
             }
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             if (finishes) {
-                for (int at = 8 * group; at < share && rank * share + at < here; at += 8 * kGroups) {
+                for (int piece = group; piece < eights && rank * share + 8 * piece < here; piece += kGroups) {
                     float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    for (int r = 0; r < splits; ++r)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] += inbox[(size_t)(r * share + at + i) * kLaneRows + row];
-                    end.finish(e, w.paired, pair, y, m0 + rank * share + at);
+                    for (int r = 0; r < splits; ++r) {
+                        const float4 lo = box[(r * eights + piece) * 2 * kLaneRows], hi = box[((r * eights + piece) * 2 + 1) * kLaneRows];
+                        y[0] += lo.x; y[1] += lo.y; y[2] += lo.z; y[3] += lo.w;
+                        y[4] += hi.x; y[5] += hi.y; y[6] += hi.z; y[7] += hi.w;
+                    }
+                    end.finish(e, w.paired, pair, y, m0 + rank * share + 8 * piece);
                 }
             }
         } else if (finishes) {
@@ -544,7 +548,7 @@ __global__ void spread_rows_kernel(const void* __restrict__ a, int64_t lda, bool
         const int64_t m = i / eights;
         const int k = (int)(i - m * eights) * 8;
         uint32_t v[4];
-        load_eight<T>(v, a, m * lda, k, K, wide);
+        load_eight<T::kHalf>(v, a, m * lda, k, K, wide);
         to[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
@@ -570,7 +574,7 @@ int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& 
 
 template <typename T, int GROUP>
 int launch(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
-    return p.walk ? launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
+    return p.walk ? launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s) : p.tmem_columns == 256 ? launch_kernel<T, GROUP, 8, false>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
 }
 
 template <typename T>
@@ -599,30 +603,47 @@ int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, voi
 
 }  // namespace
 
+// The cheapest cut by an estimate in us (a fit to some 150 launches of 24 to 2,048 tokens): 2.8 for the launch and the first weights; a k tile takes what its eight products take, which is no
+// less than it takes the tensor core to load 128 x 128 weights (0.34, up to some 150 tokens; 0.57 for each of two blocks that share an SM); a token's column of sums 0.0115;
+// the exchange of a cluster grows with its ranks and their tokens.
 ManyPlan many_plan(int M, int rows, int k, int n_sm) {
-    ManyPlan p{};
-    const int k_tiles = (k + kTileK - 1) / kTileK, row_blocks = (rows + kLaneRows - 1) / kLaneRows, tiles = (M + 255) / 256;
-    p.tokens = ((M + tiles - 1) / tiles + 15) / 16 * 16;
-    p.splits = 1;
-    while (p.splits < 8 && tiles * row_blocks * p.splits * 2 <= n_sm && k_tiles >= 4 * p.splits && (k_tiles + 2 * p.splits - 1) / (2 * p.splits) * (2 * p.splits - 1) < k_tiles)
-        p.splits *= 2;
-    if (getenv("MANY_S")) p.splits = atoi(getenv("MANY_S"));
-    if (getenv("MANY_N")) p.tokens = atoi(getenv("MANY_N"));
-    // The tokens are shared out in eights between the ranks.
-    if (p.splits > 1) p.tokens = (p.tokens + 8 * p.splits - 1) / (8 * p.splits) * (8 * p.splits);
-    if (p.tokens > 256) p.tokens = 256;
-    const long total = (long)((M + p.tokens - 1) / p.tokens) * row_blocks;
-    p.walk = p.splits == 1 && total > n_sm;
-    if (getenv("MANY_W")) p.walk = atoi(getenv("MANY_W"));
-    p.d_columns = p.tokens <= 64 ? 64 : p.tokens <= 128 ? 128 : 256;
-    p.stages = p.d_columns <= 128 ? 6 : 3;
-    p.tmem_columns = 512;
-    // The blocks of a cluster wait for one another while each holds its columns: as large a share of the shared memory as of the columns (see gemm_tcgen05_narrow.cu).
-    const int in_stages = p.stages * p.tokens * 256, inbox = p.splits > 1 ? p.tokens * 512 : 0;
-    const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control);
-    const int least = p.tmem_columns * (228 * 1024 / 512) - 1024;
-    p.smem = needed < least ? least : needed;
-    return p;
+    ManyPlan best{};
+    const int k_tiles = (k + kTileK - 1) / kTileK, row_blocks = (rows + kLaneRows - 1) / kLaneRows, fewest = (M + 255) / 256;
+    double least_us = 1e30;
+    for (int token_tiles = fewest; token_tiles <= 2 * fewest + 2; ++token_tiles) {
+        const int tokens = ((M + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+        if (token_tiles > fewest && tokens < 32) break;
+        const long total = (long)((M + tokens - 1) / tokens) * row_blocks;
+        const double stage = 0.55 * tokens / 256 > 0.34 ? 0.55 * tokens / 256 : 0.34, sums = 0.0115 * tokens;
+        for (int splits = 1; splits <= 8; ++splits) {
+            ManyPlan p{};
+            const int per = (k_tiles + splits - 1) / splits;
+            if (splits > 1 && (per < 3 || per * (splits - 1) >= k_tiles)) continue;      // short parts, or a rank without one
+            p.tokens = tokens;
+            p.splits = splits;
+            p.d_columns = tokens <= 64 ? 64 : tokens <= 128 ? 128 : 256;
+            const bool two = p.d_columns == 64;                       // two blocks an SM, whose starts and ends hide under one another
+            p.walk = splits == 1 && !two && total > n_sm;
+            p.stages = two || p.d_columns == 256 ? 3 : 6;
+            p.tmem_columns = two ? 256 : 512;
+            // The blocks of a cluster wait for one another while each holds its columns: as large a share of the shared memory as of the columns (see gemm_tcgen05_narrow.cu).
+            const int in_stages = p.stages * tokens * 256, inbox = splits > 1 ? splits * share_of(tokens, splits) * 512 : 0;
+            const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control), least = p.tmem_columns * (228 * 1024 / 512) - 1024;
+            p.smem = needed < least ? least : needed;
+            if (p.smem > 227 * 1024) continue;
+            // Clusters lie within one group of SMs, which those of more than two blocks do not fill; a second wave of blocks is worth no split.
+            const long blocks = total * splits, at_once = (long)n_sm * (splits <= 2 ? 148 : splits == 3 ? 144 : splits == 4 ? 132 : 104) / 148;
+            if (splits > 1 && blocks > (two && splits == 2 ? 2 * at_once : at_once)) continue;
+            double us = 2.8;
+            if (p.walk) us += (double)((total + n_sm - 1) / n_sm) * (per * stage + 0.4 + sums);
+            else us += (double)((blocks + 2 * n_sm - 1) / (2 * n_sm)) * per * (two && blocks > n_sm ? 0.57 : stage) + sums / splits + (splits > 1 ? 0.8 + (0.005 * splits + 0.004) * tokens : 0.0);
+            if (us < least_us) {
+                least_us = us;
+                best = p;
+            }
+        }
+    }
+    return best;
 }
 
 int64_t many_scratch_bytes(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M) {

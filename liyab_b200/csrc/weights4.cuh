@@ -25,30 +25,36 @@ __device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_
 // The operand type of the tensor cores: bfloat16 activations go with bfloat16 weights, e4m3 ones with float16.
 struct Bf16 {
     static constexpr bool kHalf = false;
-    static constexpr uint32_t kMagic = 0x43004300u;          // 0x4300 | u is 128 + u
-    static __device__ __forceinline__ uint32_t minus(uint32_t v, uint32_t c) {
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&c));
-        return *reinterpret_cast<const uint32_t*>(&d);
-    }
 };
 struct F16 {
     static constexpr bool kHalf = true;
-    static constexpr uint32_t kMagic = 0x64006400u;          // 0x6400 | u is 1024 + u
-    static __device__ __forceinline__ uint32_t minus(uint32_t v, uint32_t c) {
-        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&c));
-        return *reinterpret_cast<const uint32_t*>(&d);
-    }
 };
 
-// Nibbles q + 8 to q.  The mask and the exponent bits are kept in registers, hidden from constant folding.
+template <typename V>
+__device__ __forceinline__ uint32_t minus2(uint32_t v, uint32_t c) {
+    const V d = __hsub2(*reinterpret_cast<const V*>(&v), *reinterpret_cast<const V*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// Nibbles q + 8 to q.  bfloat16 has room for a nibble in one place only: 0x4300 | u is 128 + u, three shifts a word.  float16 has two: 0x6400 | u is 1024 + u and 0x5400 | u << 4
+// is 64 + u, and one shift a word does (a product of one token reads 5.1 TB/s of weights so, 4.1 in bfloat16; bfloat16 rows as float16 times a power of two of their
+// own made up 7 % of that and lost more to finding it).  The masks and the exponent bits are kept in registers, hidden from constant folding.
 template <typename T>
 struct Unpack {
-    uint32_t mask, magic;
+    uint32_t mask, bits, mask4, bits4;
     __device__ __forceinline__ Unpack() {
-        asm volatile("mov.b32 %0, 0x000F000F;\n\tmov.b32 %1, %2;" : "=r"(mask), "=r"(magic) : "n"(T::kMagic));
+        asm volatile("mov.b32 %0, 0x000F000F;\n\tmov.b32 %1, %4;\n\tmov.b32 %2, 0x00F000F0;\n\tmov.b32 %3, 0x54005400;"
+                     : "=r"(mask), "=r"(bits), "=r"(mask4), "=r"(bits4) : "n"(T::kHalf ? 0x64006400 : 0x43004300));
     }
     // Weights 2p and 2p + 1 of a word of eight, in the halves of a register.
-    __device__ __forceinline__ uint32_t operator()(uint32_t word, int p) const { return T::minus(masked_or(word >> (4 * p), mask, magic), T::kMagic | 0x00080008u); }
+    __device__ __forceinline__ uint32_t operator()(uint32_t word, int p) const {
+        if constexpr (T::kHalf) {
+            const uint32_t w = p < 2 ? word : word >> 8;
+            return p & 1 ? minus2<__half2>(masked_or(w, mask4, bits4), 0x54805480u) : minus2<__half2>(masked_or(w, mask, bits), 0x64086408u);
+        } else {
+            return minus2<__nv_bfloat162>(masked_or(word >> (4 * p), mask, bits), 0x43084308u);
+        }
+    }
 };
 
 // Two e4m3 numbers (16 bits) -> float16.
@@ -79,10 +85,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight activations of a row from column k on as four registers of two, zeros past K.  `wide`: rows are aligned so that eight come by one load.
-template <typename T>
+// Eight activations of a row from column k on as four registers of two (bfloat16 as they are, e4m3 as float16), zeros past K.  `wide`: rows are aligned so that eight come by one load.
+template <bool EIGHT>
 __device__ __forceinline__ void load_eight(uint32_t (&v)[4], const void* a, int64_t row_at, int k, int K, bool wide) {
-    if constexpr (T::kHalf) {
+    if constexpr (EIGHT) {
         const uint8_t* p = static_cast<const uint8_t*>(a) + row_at;
         uint32_t lo = 0, hi = 0;
         if (wide && k + 8 <= K) {
@@ -134,14 +140,6 @@ struct Epilogue {
 __device__ __forceinline__ void store_out(const Epilogue& e, int m, int col, float v) {
     if (e.out_f32) static_cast<float*>(e.out)[(int64_t)m * e.ldo + col] = v;
     else static_cast<__nv_bfloat16*>(e.out)[(int64_t)m * e.ldo + col] = __float2bfloat16_rn(v);
-}
-
-// Order as the other products': bias, activation, residual.
-__device__ __forceinline__ void finish_one(const Epilogue& e, const lb_act_pair& pair, int m, int col, float v) {
-    if (e.bias != nullptr) v += __ldg(e.bias + col);
-    v = lb_activate(v, e.act, pair);
-    if (e.residual != nullptr) v += e.residual[(int64_t)m * e.ldr + col];
-    store_out(e, m, col, v);
 }
 
 }  // namespace lb_w4
