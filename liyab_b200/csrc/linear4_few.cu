@@ -302,7 +302,7 @@ FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
         p.clusters = n_tiles < n_sm / p.splits ? n_tiles : n_sm / p.splits;
         p.round = (n_tiles + p.clusters - 1) / p.clusters;
         if (p.round > kRound) p.round = kRound;
-        const int length = p.round * per_rank, warps = length <= 16 ? 8 : 16;
+        const int length = p.round * per_rank, warps = length <= (p.token_tiles == 1 ? 96 : 16) ? 8 : 16;      // (1 x 12000 x 2048 6.1 and 6.5 us, 16 x 4800 x 1600 9.5 and 7.5)
         p.smem = Layout(M, p.token_tiles, per_rank, p.round, warps).total;
         if (p.smem <= 216 * 1024) {
             p.warps = warps;
