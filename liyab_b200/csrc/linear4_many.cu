@@ -9,7 +9,7 @@
 // cluster, which hand each other the sums of their share of the tokens through distributed shared memory and finish them in rank order.
 //
 // Roles: warp 0 copies the activations, warp 1 issues the products, warps 4 and up make weights (warp % 4 names the 32 lanes; the warps of those take k tiles in turn) and,
-// in the same warps or eight further ones, finish the sums.  Handshakes and bounded waits as in the other tcgen05 products:
+// in the same warps or in sixteen further ones, finish the sums.  Handshakes and bounded waits as in the other tcgen05 products:
 //   a_full[s], b_full[s]   weights of stage s in tensor memory, activations in shared memory
 //   empty[s]               the products have read both
 //   acc_full, acc_empty    the sums of a tile are complete, are in registers
@@ -237,8 +237,10 @@ struct Tiles {
 // Tokens of a tile that a rank of `splits` finishes, but for the last ones.
 __host__ __device__ __forceinline__ int share_of(int tokens, int splits) { return ((tokens + splits - 1) / splits + 7) / 8 * 8; }
 
+constexpr int kFinishers = 16;           // where a block walks the tiles
+
 template <int MAKERS, bool WALK>
-constexpr int threads_of() { return 32 * (kFirstMaker + MAKERS + (WALK ? 8 : 0)); }
+constexpr int threads_of() { return 32 * (kFirstMaker + MAKERS + (WALK ? kFinishers : 0)); }
 
 // WALK: a block walks the tiles blockIdx.x, blockIdx.x + gridDim.x, ..; else gridDim.x = tiles x splits, the splits of a tile a cluster.
 template <typename T, int GROUP, int MAKERS, bool WALK>
@@ -264,7 +266,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             mbar_init(&c->empty[i], 1);
         }
         mbar_init(&c->acc_full, 1);
-        mbar_init(&c->acc_empty, 8);
+        mbar_init(&c->acc_empty, kFinishers);
         c->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -355,8 +357,9 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         // No more warps take turns than there are stages: one that was a whole round of the stages ahead would take the parity of the round before for its own.
         const int turns = min(kGroups, n_stages);
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        uint4 words[2][4];
-        uint32_t steps[2];
+        constexpr int kDepth = WALK ? 1 : 2;                               // k tiles on the way a warp (one where registers are short: the products take longer than the loads)
+        uint4 words[kDepth][4];
+        uint32_t steps[kDepth];
         // The k tiles of all of this block's tiles are one sequence, of which this warp takes every turns-th; `ahead` is where the next to be fetched lies.
         int ahead_tile = first, ahead_kt = group;
         const uint4* from = nullptr;
@@ -386,7 +389,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         if (group < turns) {
             aim();
             fetch(0);
-            fetch(1);
+            if (kDepth > 1) fetch(1);
         }
         int st = group, tile = first, kt = group;
         uint32_t parity = 1;
@@ -434,8 +437,9 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             }
         while (group < turns && ok && tile < tiles.total && kt < n_kt) {
             make(0);
+            if (kDepth == 1) continue;
             if (!(ok && tile < tiles.total && kt < n_kt)) break;
-            make(1);
+            make(kDepth - 1);
         }
     }
     __syncwarp();
@@ -445,7 +449,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     const lb_act_pair pair = finisher && !w.paired ? lb_act_load(e.bias, e.n, e.act) : lb_act_pair{0.0f, 0.0f};
     if (WALK) {
         if (finisher) {
-            const int half = (warp - kFirstMaker - MAKERS) >> 2;       // this warp's 32 columns of every 64
+            const int fourth = (warp - kFirstMaker - MAKERS) >> 2;      // this warp's eights of columns are every fourth
             lb_wait_for_predecessor();           // before scales and residuals are read and anything is written
             lb_dependents_may_launch();
             uint32_t parity = 0;
@@ -459,16 +463,16 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                 tc_fence_after();
                 // Eights of columns in turn, the next one on its way; when the last is there the next tile's products may begin.
                 uint32_t v[8];
-                int at = 8 * half;
+                int at = 8 * fourth;
                 if (at < here) tmem_ld8_ask(t_row + at, v);
 #pragma unroll 1
-                for (; at < here || at == 8 * half; at += 16) {
+                for (; at < here || at == 8 * fourth; at += 8 * (kFinishers / 4)) {
                     tmem_ld8_wait(v);
                     float y[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[k]);
-                    if (at + 16 < here) {
-                        tmem_ld8_ask(t_row + at + 16, v);
+                    if (at + 8 * (kFinishers / 4) < here) {
+                        tmem_ld8_ask(t_row + at + 8 * (kFinishers / 4), v);
                     } else {
                         tc_fence_before();
                         __syncwarp();
