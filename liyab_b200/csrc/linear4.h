@@ -5,10 +5,10 @@
 
 int linear4_sm_count();
 
-// How few_tokens cuts a product: token tiles of 8, warps a block, blocks a cluster (along k), clusters, row tiles a round, bytes of shared memory.
+// How few_tokens cuts a product: warps a block, blocks a cluster (along k), clusters, row tiles a round, bytes of shared memory.
 // warps 0: it does not take it.
 struct FewPlan {
-    int token_tiles, warps, splits, clusters, round, smem;
+    int warps, splits, clusters, round, smem;
 };
 FewPlan few_plan(int M, int rows, int k, int group, int n_sm);
 int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, const FewPlan& p, cudaStream_t stream);

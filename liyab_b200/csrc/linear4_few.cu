@@ -1,10 +1,13 @@
 // Products with 4-bit weights for few tokens: out = act(a w^T + bias) + residual, and gate(a w_gate^T) * (a w_up^T) over paired rows.
 //
-// The weights are the rows of mma.sync (16 of them by 16 k), the tokens its columns (8 a tile, NT tiles).  A block owns a stretch of row tiles; its activations
+// The weights are the rows of mma.sync (16 of them by 16 k), the tokens, eight at most, its columns.  A block owns a stretch of row tiles; its activations
 // lie in shared memory in the order of the operand.  Row tiles by k tiles of 128 are one sequence that the block's warps cut into equal parts, whatever
 // the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, four tiles on the way), makes a register of two weights of a shift, a mask and a
 // subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
 // After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
+// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 13.2 us, 45 MB; 8 x 3584 x 18944
+// 15.8 us; the weights' bytes alone 6.5 and 5.4), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
+// would cost a second product and its sums for every operand; the tensor core of linear4_many.cu is then faster (16 x 4096 x 4096 6.6 us there, 7.6 here; 8 x 8192 x 8192 16.3 there, 12.9 here).
 #include "linear4.h"
 #include "tcgen05.cuh"
 
@@ -16,6 +19,8 @@ using lb_tc::smem_u32;
 constexpr int kMostWarps = 16;
 constexpr int kAhead = 4;                // k tiles on the way a warp
 constexpr int kRound = 32;               // row tiles between two barriers
+constexpr int kTokens = 8;
+constexpr int kSlot = 16 * kTokens;      // a row tile's sums
 
 __device__ __forceinline__ uint4 load_weights(const uint4* p) {
     uint4 v;
@@ -39,29 +44,29 @@ __device__ __forceinline__ float load_remote(uint32_t local, uint32_t rank) {
 __device__ __forceinline__ int load_remote_int(uint32_t local, uint32_t rank) { return __float_as_int(load_remote(local, rank)); }
 
 // Shared memory: activations [k tile][token][j ^ (token & 1)][t] of 16 bytes (the exclusive or keeps eight lanes' reads off one another's banks) behind a line of zeros
-// for the columns without a token; the slots [slot][16][8 NT].
+// for the columns without a token; the slots [slot][16][8].
 struct Layout {
     int rows_at, slots_at, total;
-    __host__ __device__ Layout(int M, int token_tiles, int n_kt, int tiles, int warps) {
+    __host__ __device__ Layout(int M, int n_kt, int tiles, int warps) {
         rows_at = 256;
         slots_at = rows_at + n_kt * M * 256;
-        total = slots_at + 512 * token_tiles * (tiles + warps);
+        total = slots_at + 4 * kSlot * (tiles + warps);
     }
 };
 
 // SPLIT: the cluster's blocks share the reduction.
-template <typename T, int NT, int GROUP, bool SPLIT>
+template <typename T, int GROUP, bool SPLIT>
 __global__ void __launch_bounds__(32 * kMostWarps)
 few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, bool wide, const Epilogue e, int n_tiles, int k_tiles, int splits, int round_tiles) {
-    constexpr int kSlot = 128 * NT, kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile;
+    constexpr int kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile;
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[8 * NT];                       // of this round's rows, of the tokens
+    __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[kTokens];                       // of this round's rows, of the tokens
     __shared__ int parts_of[kRound][2];                                                               // the first and the last warp of a row tile
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_warps = blockDim.x >> 5;
     const int rank = SPLIT ? (int)blockIdx.x % splits : 0, cluster = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, clusters = SPLIT ? (int)gridDim.x / splits : (int)gridDim.x;
     const int per_rank = SPLIT ? (k_tiles + splits - 1) / splits : k_tiles, kt0 = rank * per_rank, n_kt = min(k_tiles, kt0 + per_rank) - kt0;   // the host leaves no rank without one
     const int first = (int)((int64_t)cluster * n_tiles / clusters), last = (int)((int64_t)(cluster + 1) * n_tiles / clusters);
-    const Layout at_of(e.M, NT, per_rank, round_tiles, n_warps);
+    const Layout at_of(e.M, per_rank, round_tiles, n_warps);
     float* slots = reinterpret_cast<float*>(shared + at_of.slots_at);
 
     // This warp's part of a round: k tiles x0 .. x1 of the round's sequence, in memory one stretch, but for a rank of several, whose stretch of every row tile ends before
@@ -115,17 +120,12 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
         for (int i = 0; i < 4; ++i)
             if (m0 + i < e.M) to[i * 16 + (j ^ (i & 1)) * 4] = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
     }
-    if (threadIdx.x < 8 * NT) a_scales[threadIdx.x] = e.a_scale != nullptr && (int)threadIdx.x < e.M ? e.a_scale[threadIdx.x] : 1.0f;
+    if (threadIdx.x < kTokens) a_scales[threadIdx.x] = e.a_scale != nullptr && (int)threadIdx.x < e.M ? e.a_scale[threadIdx.x] : 1.0f;
 
     // This lane's activations: of a token, or the line of zeros; words of even and of odd j lie `swap` bytes further and nearer.
-    uint32_t columns[NT];
-    int column_step[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const bool there = 8 * n + g < e.M;
-        columns[n] = smem_u32(shared) + (there ? at_of.rows_at + (8 * n + g) * 256 : 0) + 16 * t;
-        column_step[n] = there ? 256 * e.M : 0;
-    }
+    const bool there = g < e.M;
+    const uint32_t columns = smem_u32(shared) + (there ? at_of.rows_at + g * 256 : 0) + 16 * t;
+    const int column_step = there ? 256 * e.M : 0;
     const int swap = (g & 1) * 64;
     for (int base = first; base < last; base += round_tiles) {
         __syncthreads();                    // the activations are there; the last round's slots have been read
@@ -142,13 +142,8 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             factors[i] = w.rows[base * 16 + i];
             biases[i] = e.bias != nullptr && base * 16 + i < e.n ? __ldg(e.bias + base * 16 + i) : 0.0f;
         }
-        float acc[NT][4];
-        uint32_t column[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-            column[n] = columns[n] + kt * column_step[n];
-        }
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t column = columns + kt * column_step;
         const bool ends_tile = (x1 - x0 + kt) % n_kt == 0;                                            // whether this part ends where a row tile does
         int of = start - base;
         float* slot = slots + (of + warp) * kSlot;
@@ -161,50 +156,30 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                 const uint4 top = words[i][0], low = words[i][1];
                 const uint32_t st = steps[i][0], sl = steps[i][1];
                 const uint32_t wt[4] = {top.x, top.y, top.z, top.w}, wl[4] = {low.x, low.y, low.z, low.w};
-                float part[NT][4];
+                float part[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint4 b[NT];
-#pragma unroll
-                    for (int n8 = 0; n8 < NT; ++n8)
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[n8].x), "=r"(b[n8].y), "=r"(b[n8].z), "=r"(b[n8].w)
-                                     : "r"((j & 1 ? column[n8] - swap : column[n8] + swap) + 64 * j));
-                    if ((j * 32) % GROUP == 0)
-#pragma unroll
-                        for (int n8 = 0; n8 < NT; ++n8) part[n8][0] = part[n8][1] = part[n8][2] = part[n8][3] = 0.0f;
-                    {
-                        const uint32_t a0 = unpack(wt[j], 0), a1 = unpack(wl[j], 0), a2 = unpack(wt[j], 1), a3 = unpack(wl[j], 1);
-#pragma unroll
-                        for (int n8 = 0; n8 < NT; ++n8) mma16816<T>(part[n8], a0, a1, a2, a3, b[n8].x, b[n8].y);
-                    }
-                    {
-                        const uint32_t a0 = unpack(wt[j], 2), a1 = unpack(wl[j], 2), a2 = unpack(wt[j], 3), a3 = unpack(wl[j], 3);
-#pragma unroll
-                        for (int n8 = 0; n8 < NT; ++n8) mma16816<T>(part[n8], a0, a1, a2, a3, b[n8].z, b[n8].w);
-                    }
+                    uint4 b;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "r"((j & 1 ? column - swap : column + swap) + 64 * j));
+                    if ((j * 32) % GROUP == 0) part[0] = part[1] = part[2] = part[3] = 0.0f;
+                    mma16816<T>(part, unpack(wt[j], 0), unpack(wl[j], 0), unpack(wt[j], 1), unpack(wl[j], 1), b.x, b.y);
+                    mma16816<T>(part, unpack(wt[j], 2), unpack(wl[j], 2), unpack(wt[j], 3), unpack(wl[j], 3), b.z, b.w);
                     if ((j * 32 + 32) % GROUP == 0) {
                         const uint32_t both = e4m3x2_to_f16x2(__byte_perm(st, sl, 0x0040 + (j * 32 / GROUP) * 0x11));
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&both));
-#pragma unroll
-                        for (int n8 = 0; n8 < NT; ++n8) {
-                            acc[n8][0] = fmaf(part[n8][0], f.x, acc[n8][0]);
-                            acc[n8][1] = fmaf(part[n8][1], f.x, acc[n8][1]);
-                            acc[n8][2] = fmaf(part[n8][2], f.y, acc[n8][2]);
-                            acc[n8][3] = fmaf(part[n8][3], f.y, acc[n8][3]);
-                        }
+                        acc[0] = fmaf(part[0], f.x, acc[0]);
+                        acc[1] = fmaf(part[1], f.x, acc[1]);
+                        acc[2] = fmaf(part[2], f.y, acc[2]);
+                        acc[3] = fmaf(part[3], f.y, acc[3]);
                     }
                 }
-#pragma unroll
-                for (int n8 = 0; n8 < NT; ++n8) column[n8] += column_step[n8];
+                column += column_step;
                 if (i < to_fetch) fetch(i, SPLIT ? 0 : i + kAhead);
                 if (end == i + 1) {
-#pragma unroll
-                    for (int n8 = 0; n8 < NT; ++n8) {
-                        *reinterpret_cast<float2*>(slot + g * 8 * NT + 8 * n8 + 2 * t) = make_float2(acc[n8][0], acc[n8][1]);
-                        *reinterpret_cast<float2*>(slot + (g + 8) * 8 * NT + 8 * n8 + 2 * t) = make_float2(acc[n8][2], acc[n8][3]);
-                        acc[n8][0] = acc[n8][1] = acc[n8][2] = acc[n8][3] = 0.0f;
-                        column[n8] = columns[n8];
-                    }
+                    *reinterpret_cast<float2*>(slot + g * kTokens + 2 * t) = make_float2(acc[0], acc[1]);
+                    *reinterpret_cast<float2*>(slot + (g + 8) * kTokens + 2 * t) = make_float2(acc[2], acc[3]);
+                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                    column = columns;
                     slot += kSlot;
                     const bool last_tile = todo == i + 1;
                     if (!last_tile || ends_tile) parts_of[of][1] = warp;
@@ -242,7 +217,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             float v[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int at_slot = (row + 8 * h) * 8 * NT + token;
+                const int at_slot = (row + 8 * h) * kTokens + token;
                 if (!SPLIT) {
                     const int hi = parts_of[i][1];
                     for (int q = parts_of[i][0]; q <= hi; ++q) v[h] += slots[(i + q) * kSlot + at_slot];
@@ -272,21 +247,21 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
     }
 }
 
-template <typename T, int NT, int GROUP>
+template <typename T, int GROUP>
 int launch_group(const lb_weights4* w, const void* a, int64_t lda, bool wide, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
-    auto kernel = p.splits > 1 ? few_tokens_kernel<T, NT, GROUP, true> : few_tokens_kernel<T, NT, GROUP, false>;
+    auto kernel = p.splits > 1 ? few_tokens_kernel<T, GROUP, true> : few_tokens_kernel<T, GROUP, false>;
     if (p.smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
     LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, p.splits, kernel, dim3(p.clusters * p.splits), dim3(32 * p.warps), p.smem, s, *w, a, lda, wide, e, n_tiles, k_tiles, p.splits,
                                                p.round));
     return LB_OK;
 }
 
-template <typename T, int NT>
+template <typename T>
 int launch(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
     const bool wide = lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % (T::kHalf ? 8 : 16) == 0;
-    if (w->group == 32) return launch_group<T, NT, 32>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
-    if (w->group == 64) return launch_group<T, NT, 64>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
-    return launch_group<T, NT, 128>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+    if (w->group == 32) return launch_group<T, 32>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+    if (w->group == 64) return launch_group<T, 64>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
+    return launch_group<T, 128>(w, a, lda, wide, e, p, n_tiles, k_tiles, s);
 }
 
 }  // namespace
@@ -294,16 +269,15 @@ int launch(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, 
 FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
     FewPlan p{};
     const int k_tiles = (k + kTileK - 1) / kTileK, n_tiles = (rows + kTileRows - 1) / kTileRows;
-    if (M > 16) return p;
-    p.token_tiles = M <= 8 ? 1 : 2;
+    if (M > kTokens) return p;
     for (p.splits = 1; p.splits <= 8; p.splits *= 2) {
         const int per_rank = (k_tiles + p.splits - 1) / p.splits;
         if (per_rank * (p.splits - 1) >= k_tiles) return p;
         p.clusters = n_tiles < n_sm / p.splits ? n_tiles : n_sm / p.splits;
         p.round = (n_tiles + p.clusters - 1) / p.clusters;
         if (p.round > kRound) p.round = kRound;
-        const int length = p.round * per_rank, warps = length <= (p.token_tiles == 1 ? 96 : 16) ? 8 : 16;      // (1 x 12000 x 2048 6.1 and 6.5 us, 16 x 4800 x 1600 9.5 and 7.5)
-        p.smem = Layout(M, p.token_tiles, per_rank, p.round, warps).total;
+        const int length = p.round * per_rank, warps = length <= 96 ? 8 : 16;          // (1 x 12000 x 2048 6.1 and 6.5 us, gated 1 x 10240 x 4096 14.3 and 12.1)
+        p.smem = Layout(M, per_rank, p.round, warps).total;
         if (p.smem <= 216 * 1024) {
             p.warps = warps;
             return p;
@@ -314,6 +288,5 @@ FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
 
 int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const Epilogue& e, const FewPlan& p, cudaStream_t stream) {
     const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, n_tiles = (rows + kTileRows - 1) / kTileRows;
-    if (a_dtype == LB_E4M3) return p.token_tiles == 1 ? launch<F16, 1>(w, a, lda, e, p, n_tiles, k_tiles, stream) : launch<F16, 2>(w, a, lda, e, p, n_tiles, k_tiles, stream);
-    return p.token_tiles == 1 ? launch<Bf16, 1>(w, a, lda, e, p, n_tiles, k_tiles, stream) : launch<Bf16, 2>(w, a, lda, e, p, n_tiles, k_tiles, stream);
+    return a_dtype == LB_E4M3 ? launch<F16>(w, a, lda, e, p, n_tiles, k_tiles, stream) : launch<Bf16>(w, a, lda, e, p, n_tiles, k_tiles, stream);
 }

@@ -25,11 +25,13 @@ using namespace lb_w4;
 constexpr int kFirstMaker = 4;
 constexpr int kMaxStages = 6, kStageColumns = kTileK / 2;
 constexpr int kLaneRows = 128;
+constexpr int kSpreadTokens = 32, kSpreadAhead = 4;      // e4m3 tokens that become float16 on their way: a tile's, k tiles of them in flight
 
 struct Control {
     uint64_t a_full[kMaxStages];
     uint64_t b_full[kMaxStages];
     uint64_t empty[kMaxStages];
+    uint64_t raw_full[kSpreadAhead], raw_empty[kSpreadAhead];
     uint64_t acc_full;
     uint64_t acc_empty;
     uint32_t tmem_base;
@@ -232,6 +234,7 @@ struct RowEnd {
 // How the tiles lie: token tiles of a row block one after another.
 struct Tiles {
     int tokens, token_tiles, total, k_tiles, splits, n_stages, d_columns;
+    int spread;              // e4m3 rows become float16 on their way
 };
 
 // Tokens of a tile that a rank of `splits` finishes, but for the last ones.
@@ -247,6 +250,8 @@ template <typename T, int GROUP, int MAKERS, bool WALK>
 __global__ void __launch_bounds__(threads_of<MAKERS, WALK>())
 many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 w, const Epilogue e, const Tiles tiles, int tmem_columns, int withhold, int* status) {
     constexpr int kGroups = MAKERS / 4;
+    constexpr bool kSpreads = T::kHalf && MAKERS == 8 && !WALK;        // where up to 64 e4m3 tokens are a tile
+    const bool spread = kSpreads && tiles.spread != 0;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tokens = tiles.tokens, splits = WALK ? 1 : tiles.splits, n_stages = tiles.n_stages, k_tiles = tiles.k_tiles;
@@ -262,9 +267,14 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         prefetch_tensormap(&map_a);
         for (int i = 0; i < n_stages; ++i) {
             mbar_init(&c->a_full[i], 4);
-            mbar_init(&c->b_full[i], 1);
+            mbar_init(&c->b_full[i], spread ? 2 : 1);
             mbar_init(&c->empty[i], 1);
         }
+        if (spread)
+            for (int i = 0; i < kSpreadAhead; ++i) {
+                mbar_init(&c->raw_full[i], 1);
+                mbar_init(&c->raw_empty[i], 2);
+            }
         mbar_init(&c->acc_full, 1);
         mbar_init(&c->acc_empty, kFinishers);
         c->abort_flag = 0;
@@ -282,7 +292,25 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     const int quarter = warp & 3, group = (warp - kFirstMaker) >> 2, row = quarter * 32 + lane;
     bool ok = true;
 
-    if (warp == 0) {
+    const uint32_t raw_u32 = (smem_u32(c + 1) + 1023u) & ~1023u, raw_full = smem_u32(&c->raw_full[0]), raw_empty = smem_u32(&c->raw_empty[0]);
+    if (warp == 0 && spread) {
+        lb_wait_for_predecessor();
+        lb_dependents_may_launch();
+        int issued = 0;
+        for (int kt = 0; kt < n_kt; ++kt, ++issued) {
+            const int slot = kt & (kSpreadAhead - 1);
+            if (!__all_sync(0xffffffffu, wait_u32(raw_empty + 8 * slot, (uint32_t)(kt / kSpreadAhead & 1) ^ 1u, abort_flag))) {
+                give_up(c, status, 7, slot);
+                break;
+            }
+            if (elect_one()) {
+                expect_tx_u32(raw_full + 8 * slot, (uint32_t)tokens * kTileK);
+                tma_load_u32(raw_u32 + slot * tokens * kTileK, &map_a, raw_full + 8 * slot, (kt0 + kt) * (kTileK / 2), first % tiles.token_tiles * tokens);
+            }
+        }
+        if (*abort_flag != 0)
+            for (int i = max(0, issued - kSpreadAhead); i < issued; ++i) mbar_wait(&c->raw_full[i & (kSpreadAhead - 1)], (uint32_t)(i / kSpreadAhead & 1), nullptr);
+    } else if (warp == 0) {
         lb_wait_for_predecessor();
         lb_dependents_may_launch();
         int issued = 0, st = 0;
@@ -350,6 +378,44 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         }
         lb_wait_for_predecessor();
         lb_dependents_may_launch();
+    } else if (spread && (warp == 2 || warp == 3)) {
+        // Two warps make float16 of the e4m3 that warp 0 copies: sixteen of a token a lane and piece, from one 128-byte swizzle to the other.  (Loads of their own would be waited
+        // for by the fence that shows the results to the tensor core: 0.7 us a k tile.)
+        lb_wait_for_predecessor();
+        lb_dependents_may_launch();
+        const int pieces = min(tokens, e.M - first % tiles.token_tiles * tokens) * 8, q = (int)threadIdx.x - 64, piece = q & 7;
+        int st = 0;
+        uint32_t parity = 1;
+        for (int kt = 0; kt < n_kt; ++kt) {
+            const int slot = kt & (kSpreadAhead - 1);
+            if (!__all_sync(0xffffffffu, wait_u32(raw_full + 8 * slot, (uint32_t)(kt / kSpreadAhead & 1), abort_flag) && wait_u32(empty + 8 * st, parity, abort_flag))) {
+                give_up(c, status, 6, st);
+                ok = false;
+                break;
+            }
+            const uint32_t raw = raw_u32 + slot * tokens * kTileK, to = stages_u32 + st * stage_bytes + (piece >> 2) * atom_bytes;
+#pragma unroll
+            for (int i = 0; i < kSpreadTokens / 8; ++i)
+                if (64 * i + q < pieces) {
+                    const int r = 8 * i + (q >> 3), x = r & 7;
+                    const float4 f = lds4(raw + r * 128 + ((piece ^ x) << 4));
+                    const uint32_t v[4] = {__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        sts4(to + r * 128 + (((2 * (piece & 3) + h) ^ x) << 4), make_uint4(e4m3x2_to_f16x2(v[2 * h] & 0xffffu), e4m3x2_to_f16x2(v[2 * h] >> 16),
+                                                                                              e4m3x2_to_f16x2(v[2 * h + 1] & 0xffffu), e4m3x2_to_f16x2(v[2 * h + 1] >> 16)));
+                }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&c->b_full[st]);
+                mbar_arrive(&c->raw_empty[slot]);
+            }
+            if (++st == n_stages) {
+                st = 0;
+                parity ^= 1;
+            }
+        }
     } else if (warp >= kFirstMaker && group < kGroups) {
         constexpr int kPerTile = kTileK / GROUP;
         uint32_t mask, magic;
@@ -578,13 +644,23 @@ int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& 
 
 template <typename T, int GROUP>
 int launch(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
-    return p.walk ? launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s) : p.tmem_columns == 256 ? launch_kernel<T, GROUP, 8, false>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
+    if (p.walk) return launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s);
+    if (p.tmem_columns == 256) return launch_kernel<T, GROUP, 8, false>(map, w, e, p, tiles, n_sm, s);
+    return launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
+}
+
+// Whether e4m3 rows become float16 on their way, in a small tile's block: rows that TMA takes (24 x 8000 x 3008 9.5 us).  With more tokens, whose
+// copies the two warps do not keep up with (60 x 8000 x 3008 14.4 us), or other rows a launch of its own comes first (10.3 and 11.8 us for the same).
+bool spreads(const ManyPlan& p, const lb_weights4* w, const void* a, int64_t lda) {
+    return p.tmem_columns == 256 && !p.walk && p.tokens <= kSpreadTokens && w->k % 2 == 0 && lda % 16 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0;
 }
 
 template <typename T>
 int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, void* scratch, cudaStream_t s) {
     const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, row_blocks = (rows + kLaneRows - 1) / kLaneRows, n_sm = linear4_sm_count();
-    if (many_scratch_bytes(w, T::kHalf ? LB_E4M3 : LB_BF16, a, lda, e.M) > 0) {
+    const ManyPlan p = many_plan(e.M, rows, w->k, n_sm);
+    const bool spread = T::kHalf && spreads(p, w, a, lda);
+    if (!spread && many_scratch_bytes(w, T::kHalf ? LB_E4M3 : LB_BF16, a, lda, e.M) > 0) {
         LB_CHECK_ARG(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "linear4: these activations need scratch memory (lb_linear4_scratch)");
         const bool wide = lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % (T::kHalf ? 8 : 16) == 0;
         const int eights = (w->k + 7) / 8;
@@ -594,12 +670,12 @@ int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, voi
         a = scratch;
         lda = 8 * (int64_t)eights;
     }
-    const ManyPlan p = many_plan(e.M, rows, w->k, n_sm);
+    // (Two e4m3 are copied as one value of two bytes.)
     CUtensorMap map;
-    if (int rc = lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k, lda, p.tokens)) return rc;
+    if (int rc = spread ? lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k / 2, lda / 2, p.tokens) : lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k, lda, p.tokens)) return rc;
     const int token_tiles = (e.M + p.tokens - 1) / p.tokens;
     LB_CHECK_ARG((int64_t)token_tiles * row_blocks * p.splits < (1ll << 30), "linear4: %d rows by %d features are too many tiles", e.M, rows);
-    const Tiles tiles{p.tokens, token_tiles, token_tiles * row_blocks, k_tiles, p.splits, p.stages, p.d_columns};
+    const Tiles tiles{p.tokens, token_tiles, token_tiles * row_blocks, k_tiles, p.splits, p.stages, p.d_columns, spread};
     if (w->group == 32) return launch<T, 32>(map, w, e, p, tiles, n_sm, s);
     if (w->group == 64) return launch<T, 64>(map, w, e, p, tiles, n_sm, s);
     return launch<T, 128>(map, w, e, p, tiles, n_sm, s);
@@ -632,7 +708,7 @@ ManyPlan many_plan(int M, int rows, int k, int n_sm) {
             p.tmem_columns = two ? 256 : 512;
             // The blocks of a cluster wait for one another while each holds its columns: as large a share of the shared memory as of the columns (see gemm_tcgen05_narrow.cu).
             const int in_stages = p.stages * tokens * 256, inbox = splits > 1 ? splits * share_of(tokens, splits) * 512 : 0;
-            const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control), least = p.tmem_columns * (228 * 1024 / 512) - 1024;
+            const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control) + (two && tokens <= kSpreadTokens ? 1024 + kSpreadAhead * tokens * kTileK : 0), least = p.tmem_columns * (228 * 1024 / 512) - 1024;
             p.smem = needed < least ? least : needed;
             if (p.smem > 227 * 1024) continue;
             // Clusters lie within one group of SMs, which those of more than two blocks do not fill; a second wave of blocks is worth no split.
@@ -652,6 +728,8 @@ ManyPlan many_plan(int M, int rows, int k, int n_sm) {
 
 int64_t many_scratch_bytes(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M) {
     if (a_dtype == LB_BF16 && lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0) return 0;
+    const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
+    if (a_dtype == LB_E4M3 && spreads(many_plan(M, rows, w->k, linear4_sm_count()), w, a, lda)) return 0;
     return (int64_t)M * ((w->k + 7) / 8) * 16;
 }
 

@@ -3,7 +3,7 @@
 //
 // Bound by memory: one pass, x and delta in, the sum and the result out.  A row stays in registers as t (gain_offset + gain), up to 32 values a thread, between its sum of
 // squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor; a warp has a row of up to 1024 values (no barrier), a block a longer one (two
-// barriers).  About ten instructions a value: with the divisions, selections and comparisons of a first version (29) 4096 bfloat16 rows of 8192 took 69 us, not MEASURED.
+// barriers).  About ten instructions a value: with the divisions, selections and comparisons of a first version (29) 4096 bfloat16 rows of 8192 took 69 us, not 43.
 // Rows off the 16 bytes, and of more than 16384 values, go through shared memory, a value at a time and neighbours by neighbouring threads.
 #include "weights4.cuh"
 

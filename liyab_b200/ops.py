@@ -1309,7 +1309,7 @@ def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: tor
         if bias.dtype is not torch.float32 or bias.get_device() != w.index or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0):
             raise invalid_argument("linear4: the bias is float32, one number a feature")
         bias_at = bias.data_ptr()
-    scratch = _scratch4(w, code, a, lda, m) if m > 16 or w.k > 8192 else None
+    scratch = _scratch4(w, code, a, lda, m) if m > 8 or w.k > 8192 else None
     check(lib().lb_linear4(_linear4_args(w.ref, a.data_ptr(), scale, bias_at, residual_at, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
                                          stream_of(w.index), lda, ldr, ldo, code, out_code, m, ACTIVATIONS[activation], 0.0, 0.0)), "linear4")
     return out
@@ -1323,7 +1323,7 @@ def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = 
     if kind > 4:
         raise invalid_argument(f"gated4: no gate {gate!r}")
     code, scale, out_code, lda, ldo = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
-    scratch = _scratch4(w, code, a, lda, m) if m > 16 or w.k > 8192 else None
+    scratch = _scratch4(w, code, a, lda, m) if m > 8 or w.k > 8192 else None
     check(lib().lb_gated4(_linear4_args(w.ref, a.data_ptr(), scale, 0, 0, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(), stream_of(w.index), lda, 0, ldo,
                                         code, out_code, m, kind, alpha, limit)), "gated4")
     return out
