@@ -250,7 +250,7 @@ template <typename T, int GROUP, int MAKERS, bool WALK>
 __global__ void __launch_bounds__(threads_of<MAKERS, WALK>())
 many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 w, const Epilogue e, const Tiles tiles, int tmem_columns, int withhold, int* status) {
     constexpr int kGroups = MAKERS / 4;
-    constexpr bool kSpreads = T::kHalf && MAKERS == 8 && !WALK;        // where up to 64 e4m3 tokens are a tile
+    constexpr bool kSpreads = T::kHalf && MAKERS == 8 && !WALK;        // where up to 32 e4m3 tokens may be a tile
     const bool spread = kSpreads && tiles.spread != 0;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);

@@ -10,6 +10,7 @@
     python -m liyab_b200.kernel_cases prefill-attention --soft-cap 50 --score-bound 8.2
     python -m liyab_b200.kernel_cases norm-join --rows 2048 --width 768 --experts 16
     python -m liyab_b200.kernel_cases streams --rows 2048 --streams 2 --width 768 --experts 20
+    python -m liyab_b200.kernel_cases weights4 --rows 1 --width 4096 --inner 10240 [--e4m3]
 
 Each prints one line with the CUDA-event time per repetition and the achieved rate.  The cases are what the
 ncu summaries under profiles/ were captured on (one kernel, a few launches, inputs of a few hundred MB at most).
@@ -317,6 +318,50 @@ def case_norm_join(args) -> None:
     print(f"norm-join {T} rows of {W}{', routed results' if args.routed else ''}{', with a router' if router else ''}: {1e3 * ms:.1f} us, {(10 * T * W + read) / ms / 1e6:.0f} GB/s")
 
 
+def case_weights4(args) -> None:
+    """What stands around attention in a decoder's layer, with 4-bit weights: the output product, the stream's sum and norm, a gated feed-forward and its way back into the stream,
+    the sum and norm for the next layer and its joint projection.  Beside it the same with bfloat16 weights, and how far the two streams are apart."""
+    from . import ops
+    dev, T, W, F = torch.device("cuda:0"), args.rows, args.width, args.inner
+    gen = torch.Generator(device=dev).manual_seed(0)
+    r = lambda *shape: torch.randn(*shape, device=dev, generator=gen)
+    full = [r(W, W) * W ** -0.5, r(2 * F, W) * W ** -0.5, r(W, F) * F ** -0.5, r(3 * W, W) * W ** -0.5]
+    w_out, w_gate_up, w_down, w_qkv = (ops.quantise_weights4(w, args.group, paired=i == 1) for i, w in enumerate(full))
+    plain = [w.bfloat16() for w in full]
+    gains, x0, attended, eps = [1.0 + 0.1 * r(W) for _ in range(2)], r(T, W), r(T, W).bfloat16(), 1e-6
+    x, delta, inner, qkv = x0.clone(), torch.empty(T, W, device=dev), torch.empty(T, F, dtype=torch.bfloat16, device=dev), torch.empty(T, 3 * W, dtype=torch.bfloat16, device=dev)
+    h = torch.empty(T, W, dtype=torch.float8_e4m3fn if args.e4m3 else torch.bfloat16, device=dev)
+    scale = torch.empty(T, device=dev) if args.e4m3 else None
+
+    def layer4():
+        ops.linear4(attended, w_out, None, delta, T)
+        ops.rms_add(x, delta, gains[0], eps, h, scale=scale)
+        ops.gated4(h, w_gate_up, inner, T, gate="silu", a_scale=scale)
+        ops.linear4(inner, w_down, None, delta, T)
+        ops.rms_add(x, delta, gains[1], eps, h, scale=scale)
+        ops.linear4(h, w_qkv, None, qkv, T, a_scale=scale)
+
+    y, rounded, gate_up, room = x0.clone(), torch.empty(T, W, dtype=torch.bfloat16, device=dev), torch.empty(T, 2 * F, device=dev), _Scratch(dev)
+
+    def layer16():
+        ops.linear(attended, plain[0], None, y, T, residual=y, workspace=room)
+        ops.rms_offset(y, gains[0], 0.0, eps, rounded)
+        ops.linear(rounded, plain[1], None, gate_up, T, workspace=room)
+        ops.gated_act_kind(gate_up, inner, "silu")
+        ops.linear(inner, plain[2], None, y, T, residual=y, workspace=room)
+        ops.rms_offset(y, gains[1], 0.0, eps, rounded)
+        ops.linear(rounded, plain[3], None, qkv, T, workspace=room)
+
+    layer4()
+    layer16()
+    torch.cuda.synchronize()
+    apart = ((x - y).norm() / (y - x0).norm()).item()
+    us4, us16 = 1e3 * _graph_timed(layer4, args.reps), 1e3 * _graph_timed(layer16, args.reps)
+    held = sum(w.nbytes for w in (w_out, w_gate_up, w_down, w_qkv))
+    print(f"weights4 {T} rows, {W} wide, {F} inner, groups of {args.group}{', e4m3 rows' if args.e4m3 else ''}: {us4:.1f} us, {held / 1e6:.0f} MB of weights; "
+          f"bfloat16 {us16:.1f} us, {sum(2 * w.numel() for w in plain) / 1e6:.0f} MB; what the sublayers add differs by {100 * apart:.1f} %")
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m liyab_b200.kernel_cases")
     sub = ap.add_subparsers(dest="case", required=True)
@@ -396,6 +441,13 @@ def main(argv=None) -> int:
     st.add_argument("--width", type=int, default=768)
     st.add_argument("--experts", type=int, default=0)
     st.add_argument("--reps", type=int, default=20)
+    w4 = sub.add_parser("weights4")
+    w4.add_argument("--rows", type=int, default=1)
+    w4.add_argument("--width", type=int, default=4096)
+    w4.add_argument("--inner", type=int, default=10240)
+    w4.add_argument("--group", type=int, default=128, choices=[32, 64, 128])
+    w4.add_argument("--e4m3", action="store_true", help="the norms leave e4m3 rows with a scale each")
+    w4.add_argument("--reps", type=int, default=200)
     for name in ("decode-step", "prefill-step"):
         p = sub.add_parser(name)
         p.add_argument("--batch", type=int, default=8)
@@ -411,7 +463,7 @@ def main(argv=None) -> int:
         p.add_argument("--stamps", action="store_true", help="decode-step: per-phase times from inside the one-kernel step")
     args = ap.parse_args(argv)
     {"gemm": case_gemm, "generic-attention": case_generic_attention, "gemm-f32": case_gemm_f32, "decode-attention": case_decode_attention, "prefill-attention": case_prefill_attention, "sample": case_sample, "decode-step": case_decode_step,
-     "prefill-step": case_prefill_step, "channel-memory": case_channel_memory, "streams": case_streams, "norm-join": case_norm_join}[args.case](args)
+     "prefill-step": case_prefill_step, "channel-memory": case_channel_memory, "streams": case_streams, "norm-join": case_norm_join, "weights4": case_weights4}[args.case](args)
     return 0
 
 
