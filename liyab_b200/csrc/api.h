@@ -750,7 +750,7 @@ int lb_channel_memory_pieces(int dtype, const lb_channel_memory* memory, const l
  *
  * A matrix w[n, k] = q[n, k] s[n, k / group] r[n]: q an integer in -8 .. 7, s an e4m3 number, r a float32; group is 32, 64 or 128.  The products read
  * it as lb_weights4_sizes and lb_weights4_lay_out (or lb_weights4_quantise) leave it, in memory of the caller's that stays where it is:
- *   nibbles  [row tile of 16][k tile of 128][t = 0..3][row][j = 0..3] words of eight weights k = 32 j + 8 t + i, stored as q + 8; weight i
+ *   nibbles  [row tile of 16][k tile of 128][row / 4][t / 2][row % 4][t % 2][j = 0..3], t = 0..3, words of eight weights k = 32 j + 8 t + i, stored as q + 8; weight i
  *            is nibble i / 2 + 4 (i % 2) of its word, so that a shift and a mask give two neighbours in the halves of a register.  16-byte aligned.
  *   scales   [row tile][k tile][row][128 / group] e4m3, padded with zeros; 16-byte aligned.
  *   rows     [row] float32, padded with zeros.

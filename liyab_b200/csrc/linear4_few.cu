@@ -5,8 +5,8 @@
 // the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, four tiles on the way), makes a register of two weights of a shift, a mask and a
 // subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
 // After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
-// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 13.2 us, 45 MB; 8 x 3584 x 18944
-// 15.8 us; the weights' bytes alone 6.5 and 5.4), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
+// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 12.3 us, 41 MB; 8 x 3584 x 18944
+// 14.9 us; the weights' bytes alone 6.5 and 5.4; with the products and the unpacking left out 1 x 40960 x 8192 takes 27 us, with them 34), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
 // would cost a second product and its sums for every operand; the tensor core of linear4_many.cu is then faster (16 x 4096 x 4096 6.6 us there, 7.6 here; 8 x 8192 x 8192 16.3 there, 12.9 here).
 #include "linear4.h"
 #include "tcgen05.cuh"
@@ -78,7 +78,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
     uint32_t steps[kAhead][2];
     auto fetch = [&](int i, int at) {
         words[i][0] = load_weights(from + at * (kTileBytes / 16));
-        words[i][1] = load_weights(from + at * (kTileBytes / 16) + 8);
+        words[i][1] = load_weights(from + at * (kTileBytes / 16) + kTileBytes / 32);
         steps[i][0] = load_scales<GROUP>(scales_from + at * kScaleBytes);
         steps[i][1] = load_scales<GROUP>(scales_from + at * kScaleBytes + 8 * kPerTile);
         if (SPLIT) {
@@ -96,7 +96,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
         kt = x0 % n_kt;
         left = n_kt - kt;
         const size_t tile0 = (size_t)start * k_tiles + kt0 + kt;
-        from = static_cast<const uint4*>(w.nibbles) + tile0 * (kTileBytes / 16) + kTileRows * t + g;
+        from = static_cast<const uint4*>(w.nibbles) + tile0 * (kTileBytes / 16) + piece_at(g, t);
         scales_from = static_cast<const uint8_t*>(w.scales) + tile0 * kScaleBytes + g * kPerTile;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
@@ -115,10 +115,20 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
         uint32_t v[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (m0 + i < e.M) load_eight<T::kHalf>(v[i], a, (int64_t)(m0 + i) * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
+            if (m0 + i < e.M) {
+                // (e4m3 becomes float16 when all four are there.)
+                if constexpr (T::kHalf) load_eight_bytes(v[i][0], v[i][1], a, (int64_t)(m0 + i) * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
+                else load_eight<false>(v[i], a, (int64_t)(m0 + i) * lda, (kt0 + k_tile) * kTileK + 32 * j + 8 * at, w.k, wide);
+            }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (m0 + i < e.M) to[i * 16 + (j ^ (i & 1)) * 4] = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            if (m0 + i < e.M) {
+                uint4 eight;
+                if constexpr (T::kHalf)
+                    eight = make_uint4(e4m3x2_to_f16x2(v[i][0] & 0xffffu), e4m3x2_to_f16x2(v[i][0] >> 16), e4m3x2_to_f16x2(v[i][1] & 0xffffu), e4m3x2_to_f16x2(v[i][1] >> 16));
+                else eight = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                to[i * 16 + (j ^ (i & 1)) * 4] = eight;
+            }
     }
     if (threadIdx.x < kTokens) a_scales[threadIdx.x] = e.a_scale != nullptr && (int)threadIdx.x < e.M ? e.a_scale[threadIdx.x] : 1.0f;
 

@@ -436,13 +436,13 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                 ahead_tile += stride;
             }
             const size_t at = (size_t)((ahead_tile / tiles.token_tiles * kLaneRows + row) >> 4) * k_tiles + kt0 + ahead_kt;
-            from = static_cast<const uint4*>(w.nibbles) + at * (kTileBytes / 16) + (row & 15);
+            from = static_cast<const uint4*>(w.nibbles) + at * (kTileBytes / 16) + piece_at(row & 15, 0);
             scales = static_cast<const uint8_t*>(w.scales) + (at * kTileRows + (row & 15)) * kPerTile;
         };
         auto fetch = [&](int i) {
             if (ahead_tile < tiles.total && ahead_kt < n_kt) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) words[i][t] = __ldg(from + 16 * t);
+                for (int t = 0; t < 4; ++t) words[i][t] = __ldg(from + piece_at(0, t));
                 if constexpr (GROUP == 128) steps[i] = __ldg(scales);
                 else if constexpr (GROUP == 64) steps[i] = __ldg(reinterpret_cast<const uint16_t*>(scales));
                 else steps[i] = __ldg(reinterpret_cast<const uint32_t*>(scales));

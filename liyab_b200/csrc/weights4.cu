@@ -40,7 +40,7 @@ __device__ __forceinline__ int source_row(int row, int n, int paired) {
 __device__ __forceinline__ int nibble_shift(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
 
 __device__ __forceinline__ size_t word_at(int row, int kt, int t, int j, int k_tiles) {
-    return ((size_t)(row >> 4) * k_tiles + kt) * (kTileBytes / 4) + (t * kTileRows + (row & 15)) * 4 + j;
+    return ((size_t)(row >> 4) * k_tiles + kt) * (kTileBytes / 4) + piece_at(row & 15, t) * 4 + j;
 }
 
 // A row's scales of a k tile.
