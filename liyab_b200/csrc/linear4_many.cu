@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
 __device__ __noinline__ float activate_long(float v, int act, bool exact, float a, float b) {
     const lb_act_pair pair{a, b};
     if (exact) return lb_activate(v, act, pair);
-    return act == LB_ACT_XIELU ? activate<LB_ACT_XIELU, true>(v, pair) : activate<LB_ACT_GELU_ERF, true>(v, pair);
+    return activate<LB_ACT_XIELU, true>(v, pair);
 }
 __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exact, const lb_act_pair& pair) {
     if (act == LB_ACT_RELU2) {
@@ -133,6 +133,10 @@ __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exac
     } else if (act == LB_ACT_GELU_TANH && !exact) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = activate<LB_ACT_GELU_TANH, true>(y[i], pair);
+    } else if (act == LB_ACT_GELU_ERF) {
+        // (Out of line one by one 1776 x 12232 x 96 took 74 us, in fours 51, so 44.)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = lb_gelu_erf(y[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = activate_long(y[i], act, exact, pair.a, pair.b);

@@ -3,7 +3,8 @@
 //
 // Bound by memory: one pass, x and delta in, the sum and the result out.  A row stays in registers as t (gain_offset + gain), up to 32 values a thread, between its sum of
 // squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor; a warp has a row of up to 1024 values (no barrier), a block a longer one (two
-// barriers).  About ten instructions a value: with the divisions, selections and comparisons of a first version (29) 4096 bfloat16 rows of 8192 took 69 us, not 43.
+// barriers).  24 instructions a value at 2.3 a cycle stay below what memory takes: 4096 bfloat16 rows of 8192 43 us, 0.85 of the measured copy bandwidth (69 with the divisions,
+// selections and comparisons of a first version).
 // Rows off the 16 bytes, and of more than 16384 values, go through shared memory, a value at a time and neighbours by neighbouring threads.
 #include "weights4.cuh"
 
@@ -147,7 +148,9 @@ rms_add_kernel(const Rows p) {
     }
 }
 
-// Rows of any place and length.
+// Rows of any place and length, eight values a thread on their way together (one after the other 19 float32 rows of 10925 took 9.8 us, so 7.6).
+constexpr int kBatch = 8;
+
 template <typename TX, typename TD>
 __global__ void __launch_bounds__(1024)
 rms_add_any_kernel(const Rows p) {
@@ -157,23 +160,47 @@ rms_add_any_kernel(const Rows p) {
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
     const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    const TX* x = static_cast<const TX*>(p.x) + (int64_t)r * p.ldx;
+    const TD* delta = static_cast<const TD*>(p.delta) + (int64_t)r * p.ldd;
     float ss = 0.0f;
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
-        float t = lb_to_float(static_cast<const TX*>(p.x)[(int64_t)r * p.ldx + i]);
-        if (p.delta != nullptr) t += lb_to_float(static_cast<const TD*>(p.delta)[(int64_t)r * p.ldd + i]);
-        if (p.total != nullptr) static_cast<TX*>(p.total)[(int64_t)r * p.ldt + i] = lb_from_float<TX>(t);
-        row[i] = t;
-        ss = fmaf(t, t, ss);
+    for (int i0 = threadIdx.x; i0 < p.width; i0 += kBatch * blockDim.x) {
+        float t[kBatch], d[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * (int)blockDim.x;
+            t[u] = i < p.width ? lb_to_float(x[i]) : 0.0f;
+            d[u] = i < p.width && p.delta != nullptr ? lb_to_float(delta[i]) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * (int)blockDim.x;
+            if (i >= p.width) break;
+            t[u] += d[u];
+            if (p.total != nullptr) static_cast<TX*>(p.total)[(int64_t)r * p.ldt + i] = lb_from_float<TX>(t[u]);
+            row[i] = t[u];
+            ss = fmaf(t[u], t[u], ss);
+        }
     }
     const float inv = rsqrtf(__fdividef(lb_block_sum(ss, sums), (float)p.width) + p.eps);
     float top = 0.0f;
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x) {
-        const float h = row[i] * inv * (p.gain != nullptr ? p.gain_offset + p.gain[i] : 1.0f);
-        if (p.scale == nullptr) {
-            static_cast<__nv_bfloat16*>(p.out)[(int64_t)r * p.ldo + i] = __float2bfloat16_rn(h);
-        } else {
-            row[i] = h;
-            top = largest(top, h);
+    for (int i0 = threadIdx.x; i0 < p.width; i0 += kBatch * blockDim.x) {
+        float g[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * (int)blockDim.x;
+            g[u] = p.gain == nullptr ? 1.0f : i < p.width ? p.gain_offset + p.gain[i] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * (int)blockDim.x;
+            if (i >= p.width) break;
+            const float h = row[i] * inv * g[u];
+            if (p.scale == nullptr) {
+                static_cast<__nv_bfloat16*>(p.out)[(int64_t)r * p.ldo + i] = __float2bfloat16_rn(h);
+            } else {
+                row[i] = h;
+                top = largest(top, h);
+            }
         }
     }
     if (p.scale == nullptr) return;
@@ -199,7 +226,7 @@ int launch(const Rows& p) {
     if (!wide || eights > 2048) {
         const size_t smem = sizeof(float) * p.width;
         if (smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(rms_add_any_kernel<TX, TD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWidth * 4));
-        const int block = p.width <= 1024 ? 128 : p.width <= 4096 ? 256 : p.width <= 16384 ? 512 : 1024;
+        const int share = (p.width + 32 * kBatch - 1) / (32 * kBatch) * 32, block = share < 128 ? 128 : share > 1024 ? 1024 : share;
         LB_CHECK_CUDA(lb_launch_overlapped(rms_add_any_kernel<TX, TD>, dim3(p.rows), dim3(block), smem, s, p));
         return LB_OK;
     }
