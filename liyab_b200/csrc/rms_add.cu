@@ -5,7 +5,7 @@
 // squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor; a warp has a row of up to 1024 values (no barrier), a block a longer one (two
 // barriers).  24 instructions a value at 2.3 a cycle stay below what memory takes: 4096 bfloat16 rows of 8192 43 us, 0.85 of the measured copy bandwidth (69 with the divisions,
 // selections and comparisons of a first version).
-// Rows off the 16 bytes, and of more than 16384 values, go through shared memory, a value at a time and neighbours by neighbouring threads.
+// Rows off the 16 bytes, and of more than 16384 values, go through shared memory, one or two values at a time and neighbours by neighbouring threads.
 #include "weights4.cuh"
 
 namespace {
@@ -148,58 +148,92 @@ rms_add_kernel(const Rows p) {
     }
 }
 
-// Rows of any place and length, eight values a thread on their way together (one after the other 19 float32 rows of 10925 took 9.8 us, so 7.6).
+// One value, or two neighbours.
+template <int U, typename T>
+__device__ __forceinline__ void load_unit(const T* p, float (&v)[U]) {
+    if constexpr (U == 1) {
+        v[0] = lb_to_float(*p);
+    } else if constexpr (sizeof(T) == 4) {
+        const float2 two = *reinterpret_cast<const float2*>(p);
+        v[0] = two.x;
+        v[1] = two.y;
+    } else {
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(p);
+        v[0] = __uint_as_float(two << 16);
+        v[1] = __uint_as_float(two & 0xffff0000u);
+    }
+}
+template <int U, typename T>
+__device__ __forceinline__ void store_unit(T* p, const float (&v)[U]) {
+    if constexpr (U == 1) *p = lb_from_float<T>(v[0]);
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    else *reinterpret_cast<uint32_t*>(p) = pack_bf16(v[0], v[1]);
+}
+
+// Rows of any place and length: units of two values where all rows allow it, else of one, eight values a thread on their way together (one after the other 19 float32 rows of
+// 10925 took 9.8 us, so 6.4; 4096 bfloat16 rows of 8190 take 193 us by ones and 93 by twos).
 constexpr int kBatch = 8;
 
-template <typename TX, typename TD>
+template <typename TX, typename TD, int U>
 __global__ void __launch_bounds__(1024)
 rms_add_any_kernel(const Rows p) {
     extern __shared__ float row[];
     __shared__ float sums[33];
     __shared__ uint32_t tops[32];
+    constexpr int kUnits = kBatch / U;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5, step = U * (int)blockDim.x;
     const TX* x = static_cast<const TX*>(p.x) + (int64_t)r * p.ldx;
     const TD* delta = static_cast<const TD*>(p.delta) + (int64_t)r * p.ldd;
+    TX* total = static_cast<TX*>(p.total) + (int64_t)r * p.ldt;
     float ss = 0.0f;
-    for (int i0 = threadIdx.x; i0 < p.width; i0 += kBatch * blockDim.x) {
-        float t[kBatch], d[kBatch];
+    for (int i0 = U * threadIdx.x; i0 < p.width; i0 += kUnits * step) {
+        float t[kUnits][U] = {}, d[kUnits][U] = {};
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u * (int)blockDim.x;
-            t[u] = i < p.width ? lb_to_float(x[i]) : 0.0f;
-            d[u] = i < p.width && p.delta != nullptr ? lb_to_float(delta[i]) : 0.0f;
+        for (int u = 0; u < kUnits; ++u) {
+            const int i = i0 + u * step;
+            if (i < p.width) load_unit<U>(x + i, t[u]);
+            if (i < p.width && p.delta != nullptr) load_unit<U>(delta + i, d[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u * (int)blockDim.x;
+        for (int u = 0; u < kUnits; ++u) {
+            const int i = i0 + u * step;
             if (i >= p.width) break;
-            t[u] += d[u];
-            if (p.total != nullptr) static_cast<TX*>(p.total)[(int64_t)r * p.ldt + i] = lb_from_float<TX>(t[u]);
-            row[i] = t[u];
-            ss = fmaf(t[u], t[u], ss);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                t[u][k] += d[u][k];
+                ss = fmaf(t[u][k], t[u][k], ss);
+            }
+            if (p.total != nullptr) store_unit<U>(total + i, t[u]);
+            store_unit<U>(row + i, t[u]);
         }
     }
     const float inv = rsqrtf(__fdividef(lb_block_sum(ss, sums), (float)p.width) + p.eps);
     float top = 0.0f;
-    for (int i0 = threadIdx.x; i0 < p.width; i0 += kBatch * blockDim.x) {
-        float g[kBatch];
+    for (int i0 = U * threadIdx.x; i0 < p.width; i0 += kUnits * step) {
+        float g[kUnits][U];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u * (int)blockDim.x;
-            g[u] = p.gain == nullptr ? 1.0f : i < p.width ? p.gain_offset + p.gain[i] : 0.0f;
+        for (int u = 0; u < kUnits; ++u) {
+            const int i = i0 + u * step;
+#pragma unroll
+            for (int k = 0; k < U; ++k) g[u][k] = 1.0f - p.gain_offset;
+            if (p.gain != nullptr && i < p.width) load_unit<U>(p.gain + i, g[u]);
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int i = i0 + u * (int)blockDim.x;
+        for (int u = 0; u < kUnits; ++u) {
+            const int i = i0 + u * step;
             if (i >= p.width) break;
-            const float h = row[i] * inv * g[u];
+            float h[U];
+            load_unit<U>(row + i, h);
+#pragma unroll
+            for (int k = 0; k < U; ++k) h[k] *= p.gain != nullptr ? inv * (p.gain_offset + g[u][k]) : inv;
             if (p.scale == nullptr) {
-                static_cast<__nv_bfloat16*>(p.out)[(int64_t)r * p.ldo + i] = __float2bfloat16_rn(h);
+                store_unit<U>(static_cast<__nv_bfloat16*>(p.out) + (int64_t)r * p.ldo + i, h);
             } else {
-                row[i] = h;
-                top = largest(top, h);
+                store_unit<U>(row + i, h);
+#pragma unroll
+                for (int k = 0; k < U; ++k) top = largest(top, h[k]);
             }
         }
     }
@@ -210,8 +244,14 @@ rms_add_any_kernel(const Rows p) {
     bits = __reduce_max_sync(0xffffffffu, lane < n_warps ? tops[lane] : 0u);
     float scale;
     const float f = row_factor(__uint_as_float(bits), &scale);
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x)
-        static_cast<uint8_t*>(p.out)[(int64_t)r * p.ldo + i] = f != 0.0f ? (uint8_t)floats_to_e4m3x2(row[i] * f, 0.0f) : 0;
+    uint8_t* out = static_cast<uint8_t*>(p.out) + (int64_t)r * p.ldo;
+    for (int i = U * threadIdx.x; i < p.width; i += step) {
+        float h[U];
+        load_unit<U>(row + i, h);
+        const uint32_t bytes = f != 0.0f ? floats_to_e4m3x2(h[0] * f, h[U - 1] * f) : 0u;
+        if constexpr (U == 1) out[i] = (uint8_t)bytes;
+        else *reinterpret_cast<uint16_t*>(out + i) = (uint16_t)bytes;
+    }
     if (threadIdx.x == 0) p.scale[r] = scale;
 }
 
@@ -224,10 +264,14 @@ int launch(const Rows& p) {
                       (eight ? reinterpret_cast<uintptr_t>(p.out) % 8 == 0 && p.ldo % 8 == 0 : aligned(p.out, p.ldo, 2));
     const int eights = (p.width + 7) / 8;
     if (!wide || eights > 2048) {
+        auto even = [](const void* q, int64_t ld, int bytes) { return q == nullptr || (reinterpret_cast<uintptr_t>(q) % (2 * bytes) == 0 && ld % 2 == 0); };
+        const bool twos = p.width % 2 == 0 && even(p.x, p.ldx, sizeof(TX)) && even(p.delta, p.ldd, sizeof(TD)) && even(p.total, p.ldt, sizeof(TX)) && even(p.gain, 0, 4) &&
+                          even(p.out, p.ldo, eight ? 1 : 2);
+        auto kernel = twos ? rms_add_any_kernel<TX, TD, 2> : rms_add_any_kernel<TX, TD, 1>;
         const size_t smem = sizeof(float) * p.width;
-        if (smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(rms_add_any_kernel<TX, TD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWidth * 4));
+        if (smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWidth * 4));
         const int share = (p.width + 32 * kBatch - 1) / (32 * kBatch) * 32, block = share < 128 ? 128 : share > 1024 ? 1024 : share;
-        LB_CHECK_CUDA(lb_launch_overlapped(rms_add_any_kernel<TX, TD>, dim3(p.rows), dim3(block), smem, s, p));
+        LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.rows), dim3(block), smem, s, p));
         return LB_OK;
     }
 #define LB_RMS(V_, WARP_, GRID_, BLOCK_)                                                                                                                \

@@ -1349,7 +1349,9 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
             raise invalid_argument("rms_add: delta has to be float32 or bfloat16 rows of x's shape, dense within a row and on x's device")
         if total is None:
             total = x
-    if total is not None:
+    if total is x:
+        total_at, ldt = x.data_ptr(), ldx
+    elif total is not None:
         total_at = total.data_ptr()
         ldt, dense_total = total.stride() if total.shape == shape else (0, 0)
         if dense_total != 1 or total.dtype is not x_type or total.get_device() != index:
