@@ -2,11 +2,11 @@
 //
 // The weights are the rows of mma.sync (16 of them by 16 k), the tokens, eight at most, its columns.  A block owns a stretch of row tiles; its activations
 // lie in shared memory in the order of the operand.  Row tiles by k tiles of 128 are one sequence that the block's warps cut into equal parts, whatever
-// the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, four tiles on the way), makes a register of two weights of a shift, a mask and a
+// the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, three or four tiles on the way), makes a register of two weights of a shift, a mask and a
 // subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
 // After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
-// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 12.3 us, 41 MB; 8 x 4096 x 16384
-// 14.9 us; the weights' bytes alone 6.5 and 5.4; with the products and the unpacking left out 1 x 40960 x 8192 takes 27 us, with them 34), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
+// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 11.5 us, 41 MB; 8 x 4096 x 16384
+// 14.8 us; the weights' bytes alone 6.5 and 5.4; with the products and the unpacking left out 1 x 40960 x 8192 takes 27 us, with them 34), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
 // would cost a second product and its sums for every operand; the tensor core of linear4_many.cu is then faster (16 x 4096 x 4096 6.6 us there, 7.6 here; 8 x 8192 x 8192 16.3 there, 12.9 here).
 #include "linear4.h"
 #include "tcgen05.cuh"
@@ -16,8 +16,8 @@ namespace {
 using namespace lb_w4;
 using lb_tc::smem_u32;
 
-constexpr int kMostWarps = 16;
-constexpr int kAhead = 4;                // k tiles on the way a warp
+constexpr int kMostWarps = 16, kTwoWarps = 12;     // of a block alone on its SM, of one of two
+constexpr int kTwoFrom = 12;             // row tiles an SM from which two blocks share it
 constexpr int kRound = 32;               // row tiles between two barriers
 constexpr int kTokens = 8;
 constexpr int kSlot = 16 * kTokens;      // a row tile's sums
@@ -54,11 +54,12 @@ struct Layout {
     }
 };
 
-// SPLIT: the cluster's blocks share the reduction.
-template <typename T, int GROUP, bool SPLIT>
-__global__ void __launch_bounds__(32 * kMostWarps)
+// SPLIT: the cluster's blocks share the reduction.  TWO: two blocks an SM with fewer registers each, so that one's sums and results hide under the other's products; for many row
+// tiles, whose ends cost what the shorter way ahead loses (4 x 50257 x 1600 12.3 -> 11.5 us, 1 x 32000 x 2048 9.3 -> 9.1, but 1 x 14336 x 4096 9.0 -> 9.2).
+template <typename T, int GROUP, bool SPLIT, bool TWO>
+__global__ void __launch_bounds__(32 * (TWO ? kTwoWarps : kMostWarps), TWO ? 2 : 1)
 few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, bool wide, const Epilogue e, int n_tiles, int k_tiles, int splits, int round_tiles) {
-    constexpr int kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile;
+    constexpr int kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile, kAhead = TWO ? 3 : 4;      // (k tiles on the way a warp)
     extern __shared__ __align__(128) uint8_t shared[];
     __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[kTokens];                       // of this round's rows, of the tokens
     __shared__ int parts_of[kRound][2];                                                               // the first and the last warp of a row tile
@@ -259,7 +260,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
 
 template <typename T, int GROUP>
 int launch_group(const lb_weights4* w, const void* a, int64_t lda, bool wide, const Epilogue& e, const FewPlan& p, int n_tiles, int k_tiles, cudaStream_t s) {
-    auto kernel = p.splits > 1 ? few_tokens_kernel<T, GROUP, true> : few_tokens_kernel<T, GROUP, false>;
+    auto kernel = p.splits > 1 ? few_tokens_kernel<T, GROUP, true, false> : p.warps == kTwoWarps ? few_tokens_kernel<T, GROUP, false, true> : few_tokens_kernel<T, GROUP, false, false>;
     if (p.smem > 40 * 1024) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
     LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, p.splits, kernel, dim3(p.clusters * p.splits), dim3(32 * p.warps), p.smem, s, *w, a, lda, wide, e, n_tiles, k_tiles, p.splits,
                                                p.round));
@@ -280,6 +281,16 @@ FewPlan few_plan(int M, int rows, int k, int group, int n_sm) {
     FewPlan p{};
     const int k_tiles = (k + kTileK - 1) / kTileK, n_tiles = (rows + kTileRows - 1) / kTileRows;
     if (M > kTokens) return p;
+    if (n_tiles >= kTwoFrom * n_sm) {
+        p.warps = kTwoWarps;
+        p.splits = 1;
+        p.clusters = 2 * n_sm;
+        p.round = (n_tiles + p.clusters - 1) / p.clusters;
+        if (p.round > kRound) p.round = kRound;
+        p.smem = Layout(M, k_tiles, p.round, p.warps).total;
+        if (p.smem <= 106 * 1024) return p;
+        p.warps = 0;
+    }
     for (p.splits = 1; p.splits <= 8; p.splits *= 2) {
         const int per_rank = (k_tiles + p.splits - 1) / p.splits;
         if (per_rank * (p.splits - 1) >= k_tiles) return p;

@@ -127,7 +127,26 @@ def test_linear(dev, m, n, k, group, eight):
     assert half[:, n:].isnan().all()
 
 
-@pytest.mark.parametrize("m,n,k,group", [(20, 19100, 160, 32), (33, 25000, 64, 64), (130, 12900, 333, 128), (600, 7001, 200, 64), (2500, 1600, 1100, 128), (257, 19000, 129, 32)])
+@pytest.mark.parametrize("m,n,k", [(8, 76200, 6900), (5, 76200, 700)])
+def test_rounds_of_row_tiles(dev, m, n, k):
+    """More row tiles than a block takes between two barriers, in blocks that share an SM and in ones whose activations leave no room for a second; every eleventh feature is looked at."""
+    from liyab_b200 import ops
+    g = torch.Generator(device=dev).manual_seed(k)
+    q = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8, device=dev)
+    s = (torch.rand((n, -(-k // 128)), generator=g, device=dev) * 448.0).to(F8)
+    r = torch.rand((n,), generator=g, device=dev) * 1e-4
+    a = _rand((m, k), 16, dev).to(torch.bfloat16)
+    out = torch.full((m, n), float("nan"), device=dev)
+    ops.linear4(a, ops.lay_out_weights4(q, s, r, 128), None, out, m)
+    assert ops.device_status() == 0
+    assert out.isfinite().all()
+    some = torch.arange(0, n, 11, device=dev)
+    ref_w = _matrix(q[some], s[some], r[some], 128)
+    assert ((out[:, some].double() - a.double() @ ref_w.T).abs() <= _sum_bound(k) * (a.double().abs() @ ref_w.abs().T)).all()
+
+
+@pytest.mark.parametrize("m,n,k,group", [(20, 19100, 160, 32), (33, 25000, 64, 64), (130, 12900, 333, 128), (600, 7001, 200, 64), (2500, 1600, 1100, 128), (257, 19000, 129, 32),
+                                         (1, 28446, 200, 64), (8, 30010, 97, 32), (3, 40000, 1290, 128), (4, 152000, 130, 128)])
 @pytest.mark.parametrize("eight", [False, True])
 def test_many_tiles(dev, m, n, k, group, eight):
     """More tiles than SMs, with remainders of rows, tokens and k tiles; as a gated product too."""
