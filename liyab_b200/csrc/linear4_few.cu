@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(32 * (TWO ? kTwoWarps : kMostWarps), TWO ? 2 :
 few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, bool wide, const Epilogue e, int n_tiles, int k_tiles, int splits, int round_tiles) {
     constexpr int kPerTile = kTileK / GROUP, kScaleBytes = kTileRows * kPerTile, kAhead = TWO ? 3 : 4;      // (k tiles on the way a warp)
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[kTokens];                       // of this round's rows, of the tokens
+    __shared__ float factors[kRound * 16], biases[kRound * 16], a_scales[kTokens];                       // of the rows between two barriers, of the tokens
     __shared__ int parts_of[kRound][2];                                                               // the first and the last warp of a row tile
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n_warps = blockDim.x >> 5;
     const int rank = SPLIT ? (int)blockIdx.x % splits : 0, cluster = SPLIT ? (int)blockIdx.x / splits : (int)blockIdx.x, clusters = SPLIT ? (int)gridDim.x / splits : (int)gridDim.x;
@@ -253,7 +253,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                 }
             }
         }
-        // No slot is written again, and no block leaves, while another may read this round's sums.
+        // No slot is written again, and no block leaves, while another may read these sums.
         if (SPLIT) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     }
 }

@@ -1,0 +1,74 @@
+"""4-bit weights, what the host decides without a GPU: sizes of the memory they take, scratch that a product asks for, and refusals at the C entries."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from liyab_b200 import ops
+
+
+def _sizes(n, k, group, paired):
+    nibbles, scales, rows = C.c_int64(0), C.c_int64(0), C.c_int(0)
+    status = ops.lib().lb_weights4_sizes(n, k, group, paired, C.byref(nibbles), C.byref(scales), C.byref(rows))
+    return status, nibbles.value, scales.value, rows.value
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (128, 128, 128), (129, 127, 64), (50257, 1600, 128), (5003, 4104, 32), (2 * 5461, 2048, 64), (1 << 20, 16384, 128)])
+@pytest.mark.parametrize("paired", [0, 1])
+def test_sizes(n, k, group, paired):
+    if paired and n % 2:
+        assert _sizes(n, k, group, paired)[0] != 0
+        return
+    rows = 2 * (-(-(n // 2) // 8) * 8) if paired else n
+    padded, wide = -(-rows // 128) * 128, -(-k // 128) * 128
+    assert _sizes(n, k, group, paired) == (0, padded * wide // 2, padded * wide // group, padded)
+
+
+@pytest.mark.parametrize("n,k,group,paired", [(0, 8, 32, 0), (8, 0, 32, 0), (-1, 8, 32, 0), (8, 8, 16, 0), (8, 8, 0, 0), (7, 8, 32, 1), (1 << 27, 8, 32, 0)])
+def test_sizes_refused(n, k, group, paired):
+    assert _sizes(n, k, group, paired)[0] != 0 and ops.lib().lb_last_error()
+
+
+def _weights(n, k, group=128, paired=0, nibbles=1 << 20):
+    w = ops.Weights4Args(nibbles, 1 << 20, 1 << 20, n, k, group, paired)
+    return w, C.addressof(w)
+
+
+def test_scratch_for_rows_that_are_not_read_as_they_are():
+    scratch, at = ops.lib().lb_linear4_scratch, 1 << 20
+    w, ref = _weights(4096, 4096)
+    BF16, E4M3 = ops.BF16, ops.E4M3
+    assert scratch(ref, BF16, at, 4096, 1) == scratch(ref, BF16, at + 2, 4096, 8) == scratch(ref, E4M3, at + 1, 4097, 8) == 0      # up to eight tokens: any rows
+    assert scratch(ref, BF16, at, 4096, 100) == 0                              # rows that TMA takes
+    assert scratch(ref, BF16, at + 2, 4096, 100) == scratch(ref, BF16, at, 4097, 100) == 100 * 4096 * 2
+    assert scratch(ref, E4M3, at, 4096, 16) == 0                               # e4m3 that becomes float16 on its way
+    assert scratch(ref, E4M3, at + 1, 4096, 16) == 16 * 4096 * 2
+    assert scratch(ref, E4M3, at, 4096, 300) == 300 * 4096 * 2
+    w, ref = _weights(64, 131)
+    assert scratch(ref, BF16, at, 131, 9) == 9 * 136 * 2                       # rows filled up to eights
+    assert scratch(ref, BF16, at, 136, 0) == scratch(None, BF16, at, 136, 9) == 0
+
+
+def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=0, m=0, act=0):
+    code = ops.BF16 if code is None else code
+    return getattr(ops.lib(), name)(ops._linear4_args(ref or 0, a, scale, bias, residual, out, 0, 0, lda, ldr, ldo, code, out_code, m, act, 0.0, 0.0))
+
+
+def test_products_refuse_before_they_launch():
+    plain, ref = _weights(64, 256)
+    pairs, pref = _weights(128, 256, paired=1)
+    assert _call("lb_linear4", ref) == 0 and _call("lb_gated4", pref) == 0     # no rows: nothing to do
+    assert _call("lb_linear4", ref, a=0, out=0) == 0
+    bad = [dict(m=-1), dict(m=1, a=0), dict(m=1, out=0), dict(lda=255), dict(ldo=63), dict(residual=1 << 20, ldr=63), dict(code=7), dict(out_code=ops.E4M3), dict(code=ops.E4M3),
+           dict(scale=1 << 20), dict(m=65535 * 16 + 1)]
+    for kw in bad:
+        assert _call("lb_linear4", ref, **kw) != 0, kw
+    for kw in (dict(act=-1), dict(act=99)):
+        assert _call("lb_linear4", ref, **kw) != 0 and _call("lb_gated4", pref, **kw) != 0, kw
+    assert _call("lb_linear4", pref) != 0 and _call("lb_gated4", ref) != 0     # pairs are for the gated product
+    assert _call("lb_gated4", pref, bias=1 << 20) != 0 and _call("lb_gated4", pref, residual=1 << 20, ldr=128) != 0
+    odd, oref = _weights(64, 256, group=48)
+    assert _call("lb_linear4", oref) != 0
+    empty, eref = _weights(64, 256, nibbles=0)
+    assert _call("lb_linear4", eref) != 0 and _call("lb_linear4", None) != 0
