@@ -695,7 +695,8 @@ typedef struct lb_norm_join_args {
     void* h;
     int64_t ldh;
 } lb_norm_join_args;
-/* Bytes of the structs that callers in other languages lay out by hand: 0 lb_output_terms, 1 lb_router, 2 lb_streams_args, 3 lb_norm_join_args. */
+/* Bytes of the structs that callers in other languages lay out by hand: 0 lb_output_terms, 1 lb_router, 2 lb_streams_args, 3 lb_norm_join_args,
+ * 4 lb_linear4_args, 5 lb_rms_add_args, 6 lb_weights4. */
 int lb_struct_bytes(int which);
 int lb_norm_join(int dtype, const lb_norm_join_args* args, const lb_output_terms* terms, const lb_router* router, int n_rows, void* stream);
 int lb_router_choice(int dtype, const lb_router* router, const void* h, int64_t ldh, int n_rows, int width, void* stream);

@@ -267,6 +267,9 @@ extern "C" int lb_struct_bytes(int which) {
         case 1: return (int)sizeof(lb_router);
         case 2: return (int)sizeof(lb_streams_args);
         case 3: return (int)sizeof(lb_norm_join_args);
+        case 4: return (int)sizeof(lb_linear4_args);
+        case 5: return (int)sizeof(lb_rms_add_args);
+        case 6: return (int)sizeof(lb_weights4);
         default: return 0;
     }
 }

@@ -1189,8 +1189,9 @@ _ROWS8 = torch.float8_e4m3fn
 
 
 # The arguments of a call as the library's structs (lb_linear4_args, lb_rms_add_args): packing them costs a fraction of a conversion each.
-_linear4_args = struct.Struct("@8P3q4i2f").pack
-_rms_add_args = struct.Struct("@7P4q5i2f").pack
+# "0P": filled up to the alignment of a pointer, as the library's structs are, which are copied whole.
+_linear4_args = struct.Struct("@8P3q4i2f0P").pack
+_rms_add_args = struct.Struct("@7P4q5i2f0P").pack
 
 
 class Weights4Args(ctypes.Structure):

@@ -30,6 +30,14 @@ def test_sizes_refused(n, k, group, paired):
     assert _sizes(n, k, group, paired)[0] != 0 and ops.lib().lb_last_error()
 
 
+def test_arguments_are_as_long_as_the_library_reads_them():
+    """Both products and the norm copy their arguments as one struct: a shorter one here would be read past its end."""
+    length = ops.lib().lb_struct_bytes
+    assert len(ops._linear4_args(*[0] * 15, 0.0, 0.0)) == length(4)
+    assert len(ops._rms_add_args(*[0] * 16, 0.0, 0.0)) == length(5)
+    assert C.sizeof(ops.Weights4Args) == length(6)
+
+
 def _weights(n, k, group=128, paired=0, nibbles=1 << 20):
     w = ops.Weights4Args(nibbles, 1 << 20, 1 << 20, n, k, group, paired)
     return w, C.addressof(w)
