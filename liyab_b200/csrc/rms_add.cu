@@ -177,7 +177,7 @@ constexpr int kBatch = 8;
 template <typename TX, typename TD, int U>
 __global__ void __launch_bounds__(1024)
 rms_add_any_kernel(const Rows p) {
-    extern __shared__ float row[];
+    extern __shared__ __align__(16) float row[];        // (read and written in twos)
     __shared__ float sums[33];
     __shared__ uint32_t tops[32];
     constexpr int kUnits = kBatch / U;

@@ -339,6 +339,22 @@ def test_norm_alone_and_strided(dev):
         assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2.0 ** -16 * h.abs()).all()
 
 
+@pytest.mark.parametrize("rows,width,place", [(1, 2, 2), (5, 98, 2), (3, 1602, 6), (40, 8190, 2), (2, 40002, 0), (300, 16386, 0)])
+@pytest.mark.parametrize("x_type,delta_type", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_norm_of_rows_in_twos(dev, rows, width, place, x_type, delta_type):
+    """Rows whose places are even but no multiple of 16 bytes: they go through shared memory two values at a time."""
+    from liyab_b200 import ops
+    x, delta = _rand((rows, width + 8), 26, dev, x_type)[:, place:place + width], _rand((rows, width + 2), 27, dev, delta_type)[:, :width]
+    out, scale, total = torch.empty((rows, width), dtype=F8, device=dev), torch.empty(rows, device=dev), torch.empty((rows, width), dtype=x_type, device=dev)
+    ops.rms_add(x, delta, None, 1e-5, out, scale=scale, total=total)
+    t = x.double() + delta.double()
+    h = t / (t.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    # As in test_norm: one rounding of the sum and one to x's type, a mean's error of 2^-17, half a step of e4m3.
+    assert ((total.double() - t).abs() <= (2.0 ** -24 + (2.0 ** -8 if x_type is torch.bfloat16 else 0.0)) * t.abs()).all()
+    got = out.double() * scale.double()[:, None]
+    assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2 * (2.0 ** -17 * h.abs() + 2.0 ** -22)).all()
+
+
 def test_norm_of_special_rows(dev):
     from liyab_b200 import ops
     for width in (40, 1600, 9000):
