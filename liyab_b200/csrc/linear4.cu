@@ -52,6 +52,25 @@ extern "C" int lb_gated4(const lb_linear4_args* p) {
     return launch(p->w, p->a_dtype, p->a, p->lda, e, 2 * ((e.n + 7) / 8 * 8), p->scratch, static_cast<cudaStream_t>(p->stream));
 }
 
+extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {
+    LB_CHECK_ARG(w != nullptr && plan != nullptr && M > 0, "linear4_plan: no weights, rows or place for the answer");
+    const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
+    const FewPlan f = few_plan(M, rows, w->k, w->group, linear4_sm_count());
+    if (f.warps > 0) {
+        plan[0] = 0;
+        plan[1] = M;
+        plan[2] = f.splits;
+        plan[3] = f.clusters;
+        return LB_OK;
+    }
+    const ManyPlan m = many_plan(M, rows, w->k, linear4_sm_count());
+    plan[0] = m.walk ? 2 : 1;
+    plan[1] = m.tokens;
+    plan[2] = m.splits;
+    plan[3] = (M + m.tokens - 1) / m.tokens * ((rows + 127) / 128);
+    return LB_OK;
+}
+
 extern "C" int64_t lb_linear4_scratch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M) {
     if (w == nullptr || M <= 0) return 0;
     const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;

@@ -60,19 +60,10 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32
         ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// Asked for and waited for in one piece: until the wait nothing may touch the registers, and code between the two (calls above all) may move them.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld8_ask(uint32_t taddr, uint32_t (&v)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
-}
-// The wait for a load, tied to its registers so that nothing is made of them before it.
-__device__ __forceinline__ void tmem_ld8_wait(uint32_t (&v)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]) :: "memory");
 }
 
 // A long wait that leaves the issue slots to others; bounded as mbar_wait is.
@@ -531,19 +522,17 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                     break;
                 }
                 tc_fence_after();
-                // Eights of columns in turn, the next one on its way; when the last is there the next tile's products may begin.
-                uint32_t v[8];
-                int at = 8 * fourth;
-                if (at < here) tmem_ld8_ask(t_row + at, v);
+                // Eights of columns in turn; when the last is there the next tile's products may begin.
 #pragma unroll 1
-                for (; at < here || at == 8 * fourth; at += 8 * (kFinishers / 4)) {
-                    tmem_ld8_wait(v);
+                for (int at = 8 * fourth; at < here || at == 8 * fourth; at += 8 * (kFinishers / 4)) {
                     float y[8];
+                    if (at < here) {
+                        uint32_t v[8];
+                        tmem_ld8(t_row + at, v);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[k]);
-                    if (at + 8 * (kFinishers / 4) < here) {
-                        tmem_ld8_ask(t_row + at + 8 * (kFinishers / 4), v);
-                    } else {
+                        for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[k]);
+                    }
+                    if (at + 8 * (kFinishers / 4) >= here) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&c->acc_empty);

@@ -1205,6 +1205,7 @@ for _name, _args in {
     "lb_weights4_values": [_p, _p, _l, _p],
     "lb_linear4": [_c.c_char_p],
     "lb_linear4_withhold_next": [_i],
+    "lb_linear4_plan": [_p, _i, _p],
     "lb_gated4": [_c.c_char_p],
     "lb_rms_add_rows": [_c.c_char_p],
 }.items():
@@ -1287,6 +1288,13 @@ def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n
     if a.dtype is not torch.bfloat16 or a_scale is not None:
         raise invalid_argument(f"{what}: activations are bfloat16, or e4m3 with a_scale; a is {a.dtype}")
     return BF16, 0, out_code, lda, ldo
+
+
+def linear4_plan(w: Weights4, m: int) -> tuple:
+    """How a product of m rows is cut: ("few", m, blocks that share a reduction, clusters), or ("tiles" or "walk", rows a tile, blocks that share a reduction, tiles)."""
+    plan = (_i * 4)()
+    check(lib().lb_linear4_plan(w.ref, m, plan), "linear4_plan")
+    return (("few", "tiles", "walk")[plan[0]], *plan[1:])
 
 
 def _scratch4(w: Weights4, code: int, a: torch.Tensor, lda: int, m: int) -> Optional[torch.Tensor]:

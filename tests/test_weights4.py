@@ -58,6 +58,23 @@ def test_scratch_for_rows_that_are_not_read_as_they_are():
     assert scratch(ref, BF16, at, 136, 0) == scratch(None, BF16, at, 136, 9) == 0
 
 
+def test_how_a_product_is_cut():
+    """One token to many: the kernel for few, tiles with a block each, reductions that blocks share, blocks that walk the tiles."""
+    def plan(n, k, m, paired=0):
+        w, ref = _weights(n, k, paired=paired)
+        out = (C.c_int * 4)()
+        assert ops.lib().lb_linear4_plan(ref, m, out) == 0
+        return tuple(out)
+    assert plan(1600, 1600, 1) == (0, 1, 1, 100) and plan(1600, 1600, 8)[0] == 0 and plan(1600, 1600, 9)[0] == 1
+    assert plan(4096, 16384, 8)[::2] == (0, 2)                                 # activations of a whole reduction do not fit a block
+    for n, k, m, paired in ((8192, 8192, 2048, 0), (7002, 200, 600, 0), (7002, 200, 600, 1)):
+        which, tokens, splits, tiles = plan(n, k, m, paired)
+        assert which == 2 and splits == 1 and tokens % 16 == 0 and 16 <= tokens <= 256 and tiles == -(-m // tokens) * -(-n // 128) > 148
+    assert plan(512, 8192, 24)[2] > 1
+    w, ref = _weights(64, 64)
+    assert ops.lib().lb_linear4_plan(ref, 0, (C.c_int * 4)()) != 0 and ops.lib().lb_linear4_plan(ref, 1, None) != 0
+
+
 def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=0, m=0, act=0):
     code = ops.BF16 if code is None else code
     return getattr(ops.lib(), name)(ops._linear4_args(ref or 0, a, scale, bias, residual, out, 0, 0, lda, ldr, ldo, code, out_code, m, act, 0.0, 0.0))

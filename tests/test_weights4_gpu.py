@@ -233,6 +233,96 @@ def test_gated(dev, m, f, k, group, eight):
     assert ops.device_status() == 0
 
 
+def _activated(z, kind, a=0.8, b=0.4):
+    """(the activation of z in 64 bits, a bound on its slope within e of z as a function of e)"""
+    if kind == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(0.7978845608028654 * (z + 0.044715 * z ** 3))), lambda e: 1.2
+    if kind == "gelu_erf":
+        return 0.5 * z * (1 + torch.erf(z * 0.7071067811865476)), lambda e: 1.2
+    if kind == "xielu":
+        a, b = torch.nn.functional.softplus(torch.tensor([a, b], dtype=torch.float64)).tolist()
+        return torch.where(z > 0, a * z * z + 0.5 * z, (b + 0.5) * (torch.expm1(z.clamp(max=0)) - z) + 0.5 * z), lambda e: 2 * a * (z.abs() + e) + b + 1.0
+    if kind == "relu2":
+        return z.clamp(min=0) ** 2, lambda e: 2 * (z.abs() + e)
+    return z, lambda e: 1.0
+
+
+# Products whose blocks walk the tiles: remainders of rows, tokens and k tiles.
+WALKS = [(600, 7002, 200, 64), (1030, 5006, 72, 32), (700, 8010, 1000, 128)]
+
+
+@pytest.mark.parametrize("m,n,k,group", WALKS)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("activation", ["none", "gelu_tanh", "gelu_erf", "xielu", "relu2"])
+def test_walked_tiles(dev, m, n, k, group, eight, activation):
+    """Blocks that walk the tiles, with a bias, an activation and a residual (float32: in place), in both result types."""
+    from liyab_b200 import ops
+    q, s, r = _parts(n, k, group, dev, seed=m)
+    r = r * 0.02
+    w, ref_w = ops.lay_out_weights4(q, s, r, group), _matrix(q, s, r, group)
+    assert ops.linear4_plan(w, m)[0] == "walk"
+    a, scale = _rand((m, k), 40, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    bias, res = _rand((n + 2,), 41, dev), _rand((m, n), 42, dev)
+    bias[n:] = torch.tensor([0.8, 0.4], device=dev)
+    z = rows @ ref_w.T + bias[:n].double()
+    e = _sum_bound(k) * (rows.abs() @ ref_w.abs().T + bias[:n].double().abs())
+    want, slope = _activated(z, activation)
+    # The sum's error times the slope; the function's own arithmetic (library calls in 32 bits: under 16 roundings of terms no larger than z and the value); the residual's addition.
+    bound = e * slope(e) + 2.0 ** -19 * (want.abs() + z.abs()) + 2.0 ** -23 * res.double().abs()
+    out = res.clone()
+    ops.linear4(a, w, bias, out, m, activation=activation, residual=out, a_scale=scale)
+    assert ops.device_status() == 0
+    assert ((out.double() - want - res.double()).abs() <= bound).all()
+    half = torch.full((m, n + 1), float("nan"), dtype=torch.bfloat16, device=dev)
+    ops.linear4(a, w, bias, half[:, :n], m, activation=activation, a_scale=scale)
+    assert ops.device_status() == 0
+    # Results in bfloat16: the fast exponential (2 + 1.2 |argument| units of 2^-23, arguments to 90) and division, then the rounding.
+    assert ((half[:, :n].double() - want).abs() <= bound + (2.0 ** -8 + 2.0 ** -15) * (want.abs() + bound) + 2.0 ** -19 * z.abs()).all()
+    assert half[:, n:].isnan().all()
+
+
+@pytest.mark.parametrize("m,n,k,group", WALKS)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("gate", ["silu", "relu", "gelu_tanh", "sigmoid", "capped"])
+def test_walked_gates(dev, m, n, k, group, eight, gate):
+    from liyab_b200 import ops
+    f = n // 2
+    q, s, r = _parts(n, k, group, dev, seed=m + 1)
+    r = r * 0.02
+    w, ref_w = ops.lay_out_weights4(q, s, r, group, paired=True), _matrix(q, s, r, group)
+    assert ops.linear4_plan(w, m)[0] == "walk"
+    a, scale = _rand((m, k), 43, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    both, size = rows @ ref_w.T, _sum_bound(k) * (rows.abs() @ ref_w.abs().T)
+    g, u, eg, eu = both[:, :f], both[:, f:], size[:, :f], size[:, f:]
+    slope = 1.2
+    if gate == "capped":
+        g, u, slope = g.clamp(max=2.0), u.clamp(-2.0, 2.0) + 1.0, 1.7
+        act = g * torch.sigmoid(1.7 * g)
+    else:
+        act = {"silu": lambda: g * torch.sigmoid(g), "relu": lambda: g.clamp(min=0), "sigmoid": lambda: torch.sigmoid(g), "gelu_tanh": lambda: _activated(g, "gelu_tanh")[0]}[gate]()
+    want = act * u
+    for dtype, rounding in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8 + 2.0 ** -15)):
+        out = torch.full((m, f + 1), float("nan"), dtype=dtype, device=dev)
+        ops.gated4(a, w, out[:, :f], m, gate=gate, a_scale=scale, alpha=1.7, limit=2.0)
+        assert ops.device_status() == 0
+        # As in test_gated: the product's rule on both sums' errors, and the gate's own 32-bit arithmetic.
+        bound = slope * eg * (u.abs() + eu) + act.abs() * eu + 2.0 ** -19 * (want.abs() + act.abs()) + 1e-30
+        assert ((out[:, :f].double() - want).abs() <= bound + rounding * (want.abs() + bound)).all()
+        assert out[:, f:].isnan().all()
+
+
 @pytest.mark.parametrize("m", [1, 3, 12, 40, 150])
 @pytest.mark.parametrize("eight", [False, True])
 def test_rows_that_lie_anyhow(dev, m, eight):
