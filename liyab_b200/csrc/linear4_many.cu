@@ -507,12 +507,16 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
 
     const bool finisher = WALK ? warp >= kFirstMaker + MAKERS : warp >= kFirstMaker;
     const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const lb_act_pair pair = finisher && !w.paired ? lb_act_load(e.bias, e.n, e.act) : lb_act_pair{0.0f, 0.0f};
+    lb_act_pair pair{0.0f, 0.0f};
+    // Scales, residuals and the learned numbers behind the bias are read, and results written, after this.
+    if (finisher) {
+        lb_wait_for_predecessor();
+        lb_dependents_may_launch();
+        if (!w.paired) pair = lb_act_load(e.bias, e.n, e.act);
+    }
     if (WALK) {
         if (finisher) {
             const int fourth = (warp - kFirstMaker - MAKERS) >> 2;      // this warp's eights of columns are every fourth
-            lb_wait_for_predecessor();           // before scales and residuals are read and anything is written
-            lb_dependents_may_launch();
             uint32_t parity = 0;
             for (int tile = first; tile < tiles.total; tile += stride, parity ^= 1) {
                 const int m0 = tile % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
@@ -543,8 +547,6 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         }
     } else {
         if (finisher) {
-            lb_wait_for_predecessor();
-            lb_dependents_may_launch();
             ok = __all_sync(0xffffffffu, ok && (mbar_wait(&c->acc_full, 0, abort_flag)));
             if (!ok) give_up(c, status, 3, quarter);
             tc_fence_after();

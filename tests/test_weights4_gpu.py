@@ -287,6 +287,28 @@ def test_walked_tiles(dev, m, n, k, group, eight, activation):
     assert half[:, n:].isnan().all()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 264, 320), (8, 264, 4096), (12, 264, 320), (40, 264, 320), (100, 264, 320), (24, 512, 8192), (600, 7002, 200)])
+def test_bias_that_the_launch_before_wrote(dev, m, n, k):
+    """The bias, xIELU's two numbers behind it among them, comes from a product right before, which the launch overlaps; other numbers every time."""
+    from liyab_b200 import ops
+    q, s, r = _parts(n, k, 64, dev)
+    w, ref_w = ops.lay_out_weights4(q, s, r * 0.02, 64), _matrix(q, s, r * 0.02, 64)
+    makes = ops.quantise_weights4(_rand((n + 2, 2048), 50, dev, scale=0.02), 128)
+    a = _rand((m, k), 51, dev, torch.bfloat16)
+    sources, biases, outs = _rand((6, 2048), 52, dev, torch.bfloat16), torch.zeros((1, n + 2), device=dev), torch.empty((6, m, n), device=dev)
+    seen = torch.empty((6, n + 2), device=dev)
+    for i in range(6):
+        ops.linear4(sources[i:i + 1], makes, None, biases, 1)
+        ops.linear4(a, w, biases[0], outs[i], m, activation="xielu")
+        seen[i].copy_(biases[0])
+    assert ops.device_status() == 0 and len({tuple(b.tolist()) for b in seen[:, n:]}) == 6
+    for i in range(6):
+        z = a.double() @ ref_w.T + seen[i, :n].double()
+        e = _sum_bound(k) * (a.double().abs() @ ref_w.abs().T + seen[i, :n].double().abs())
+        want, slope = _activated(z, "xielu", seen[i, n].item(), seen[i, n + 1].item())
+        assert ((outs[i].double() - want).abs() <= e * slope(e) + 2.0 ** -19 * (want.abs() + z.abs())).all()
+
+
 @pytest.mark.parametrize("m,n,k,group", WALKS)
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("gate", ["silu", "relu", "gelu_tanh", "sigmoid", "capped"])
