@@ -219,6 +219,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                 for (int q = lo; q <= hi; ++q) v += slots[(i + q) * kSlot + at_slot];
                 slots[(i + lo) * kSlot + at_slot] = v;
             }
+            __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
         const lb_act_pair pair = w.paired ? lb_act_pair{0.0f, 0.0f} : lb_act_load(e.bias, e.n, e.act);
@@ -254,7 +255,10 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             }
         }
         // No slot is written again, and no block leaves, while another may read these sums.
-        if (SPLIT) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        if (SPLIT) {
+            __syncwarp();                       // (lanes without a feature went past the others)
+            asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        }
     }
 }
 

@@ -530,6 +530,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
 #pragma unroll 1
                 for (int at = 8 * fourth; at < here || at == 8 * fourth; at += 8 * (kFinishers / 4)) {
                     float y[8];
+                    __syncwarp();                                       // (the results' code parts lanes; a warp loads as one)
                     if (at < here) {
                         uint32_t v[8];
                         tmem_ld8(t_row + at, v);
@@ -559,6 +560,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             // Every block's products are complete before their stages are written over.  A rank's share is a whole number of eights of tokens, the last ranks' may be none.
             const int share = share_of(tokens, splits), eights = share / 8;
             float4* box = reinterpret_cast<float4*>(inbox) + row;      // [rank][eight][half][128 rows] of four tokens: a warp's 16-byte stores lie side by side
+            __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             if (finishes) {
                 for (int piece = group; 8 * piece < here; piece += kGroups) {
@@ -587,6 +589,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
 #pragma unroll 1
             for (int at = 8 * group; at < here; at += 8 * kGroups) {
                 uint32_t v[8];
+                __syncwarp();
                 tmem_ld8(t_row + at, v);
                 float y[8];
 #pragma unroll

@@ -145,6 +145,27 @@ def test_rounds_of_row_tiles(dev, m, n, k):
     assert ((out[:, some].double() - a.double() @ ref_w.T).abs() <= _sum_bound(k) * (a.double().abs() @ ref_w.abs().T)).all()
 
 
+@pytest.mark.parametrize("m,n,k,splits", [(8, 38505, 14500, 2), (8, 20003, 30000, 4), (5, 10007, 90000, 8)])
+def test_shared_reductions_in_rounds(dev, m, n, k, splits):
+    """Blocks that share a reduction take more row tiles than fit between two barriers, and the features end inside a warp's; every 37th feature and the last ones are looked at."""
+    from liyab_b200 import ops
+    g = torch.Generator(device=dev).manual_seed(k)
+    q = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8, device=dev)
+    s = (torch.rand((n, -(-k // 128)), generator=g, device=dev) * 448.0).to(F8)
+    r = torch.rand((n,), generator=g, device=dev) * 1e-4
+    w = ops.lay_out_weights4(q, s, r, 128)
+    assert ops.linear4_plan(w, m)[0] == "few" and ops.linear4_plan(w, m)[2] == splits
+    a, res = _rand((m, k), 17, dev).to(torch.bfloat16), _rand((m, n), 18, dev)
+    out = res.clone()
+    ops.linear4(a, w, None, out, m, residual=out)
+    assert ops.device_status() == 0
+    assert out.isfinite().all()
+    some = torch.cat([torch.arange(0, n, 37, device=dev), torch.arange(n - 20, n, device=dev)])
+    ref_w = _matrix(q[some], s[some], r[some], 128)
+    size = a.double().abs() @ ref_w.abs().T + res[:, some].double().abs()
+    assert ((out[:, some].double() - a.double() @ ref_w.T - res[:, some].double()).abs() <= _sum_bound(k) * size).all()
+
+
 @pytest.mark.parametrize("m,n,k,group", [(20, 19100, 160, 32), (33, 25000, 64, 64), (130, 12900, 333, 128), (600, 7001, 200, 64), (2500, 1600, 1100, 128), (257, 19000, 129, 32),
                                          (1, 28446, 200, 64), (8, 30010, 97, 32), (3, 40000, 1290, 128), (4, 152000, 130, 128)])
 @pytest.mark.parametrize("eight", [False, True])
