@@ -21,8 +21,7 @@ int launch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const 
 int check(const char* what, const lb_linear4_args* p, bool paired) {
     LB_CHECK_ARG(p != nullptr, "%s: no arguments", what);
     const lb_weights4* w = p->w;
-    LB_CHECK_ARG(w != nullptr && w->nibbles != nullptr && w->scales != nullptr && w->rows != nullptr, "%s: weights without memory", what);
-    LB_CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "%s: group is %d, not 32, 64 or 128", what, w->group);
+    if (int rc = weights4_check(w, what)) return rc;
     LB_CHECK_ARG((w->paired != 0) == paired, "%s: the weights are %slaid out in pairs", what, paired ? "not " : "");
     LB_CHECK_ARG(p->M >= 0 && (p->M == 0 || (p->a != nullptr && p->out != nullptr)), "%s: %d rows, or no memory for them", what, p->M);
     LB_CHECK_ARG(p->M <= 65535 * 16, "%s: %d rows are more than %d", what, p->M, 65535 * 16);
@@ -30,6 +29,9 @@ int check(const char* what, const lb_linear4_args* p, bool paired) {
     LB_CHECK_ARG(p->a_dtype == LB_BF16 || p->a_dtype == LB_E4M3, "%s: activations are bfloat16 or e4m3", what);
     LB_CHECK_ARG((p->a_dtype == LB_E4M3) == (p->a_scale != nullptr), "%s: e4m3 activations have a scale a row, bfloat16 ones have none", what);
     LB_CHECK_ARG(p->out_dtype == LB_BF16 || p->out_dtype == LB_F32, "%s: the output is bfloat16 or float32", what);
+    auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+    LB_CHECK_ARG((at(p->a) % (p->a_dtype == LB_BF16 ? 2 : 1) | at(p->out) % (p->out_dtype == LB_BF16 ? 2 : 4) | (at(p->a_scale) | at(p->bias) | at(p->residual)) % 4) == 0,
+                 "%s: a pointer is not aligned to its type", what);
     return LB_OK;
 }
 
@@ -53,7 +55,8 @@ extern "C" int lb_gated4(const lb_linear4_args* p) {
 }
 
 extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {
-    LB_CHECK_ARG(w != nullptr && plan != nullptr && M > 0, "linear4_plan: no weights, rows or place for the answer");
+    if (int rc = weights4_check(w, "linear4_plan")) return rc;
+    LB_CHECK_ARG(plan != nullptr && M > 0, "linear4_plan: no rows, or no place for the answer");
     const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
     const FewPlan f = few_plan(M, rows, w->k, w->group, linear4_sm_count());
     if (f.warps > 0) {
@@ -72,7 +75,7 @@ extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {
 }
 
 extern "C" int64_t lb_linear4_scratch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M) {
-    if (w == nullptr || M <= 0) return 0;
+    if (M <= 0 || weights4_check(w, "linear4_scratch") != LB_OK) return 0;      // (the product refuses such weights)
     const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
     return few_plan(M, rows, w->k, w->group, linear4_sm_count()).warps > 0 ? 0 : many_scratch_bytes(w, a_dtype, a, lda, M);
 }

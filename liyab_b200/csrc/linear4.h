@@ -5,6 +5,9 @@
 
 int linear4_sm_count();
 
+// Whether a kernel can read these weights: memory, alignment, sizes (every entry point that is given weights asks first).
+int weights4_check(const lb_weights4* w, const char* what);
+
 // How few_tokens cuts a product: warps a block, blocks a cluster (along k), clusters, row tiles a round, bytes of shared memory.
 // warps 0: it does not take it.
 struct FewPlan {

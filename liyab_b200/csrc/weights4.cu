@@ -1,7 +1,5 @@
 // 4-bit weights: laying a matrix out, rounding one to 4 bits, reading one back.  Done once when a model is set up; the products are elsewhere.
-#include "weights4.cuh"
-
-
+#include "linear4.h"
 
 namespace {
 
@@ -18,15 +16,6 @@ Sizes sizes_of(int n, int k, int paired) {
     s.padded = (s.rows + 127) / 128 * 128;
     s.k_tiles = (k + kTileK - 1) / kTileK;
     return s;
-}
-
-int check_weights(const lb_weights4* w, const char* what) {
-    LB_CHECK_ARG(w != nullptr && w->nibbles != nullptr && w->scales != nullptr && w->rows != nullptr, "%s: weights without memory", what);
-    LB_CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "%s: group is %d, not 32, 64 or 128", what, w->group);
-    LB_CHECK_ARG(w->n > 0 && w->k > 0 && w->n <= (1 << 26) && w->k <= (1 << 26) && (!w->paired || w->n % 2 == 0), "%s: a matrix of %d x %d", what, w->n, w->k);
-    LB_CHECK_ARG(reinterpret_cast<uintptr_t>(w->nibbles) % 16 == 0 && reinterpret_cast<uintptr_t>(w->scales) % 16 == 0, "%s: nibbles and scales are not 16-byte aligned",
-                 what);
-    return LB_OK;
 }
 
 // The matrix's row that lies at `row`, -1 where it is padding.
@@ -143,6 +132,15 @@ int finished(cudaStream_t stream) {
 
 }  // namespace
 
+int weights4_check(const lb_weights4* w, const char* what) {
+    LB_CHECK_ARG(w != nullptr && w->nibbles != nullptr && w->scales != nullptr && w->rows != nullptr, "%s: weights without memory", what);
+    LB_CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "%s: group is %d, not 32, 64 or 128", what, w->group);
+    LB_CHECK_ARG(w->n > 0 && w->k > 0 && w->n <= (1 << 26) && w->k <= (1 << 26) && (!w->paired || w->n % 2 == 0), "%s: a matrix of %d x %d", what, w->n, w->k);
+    LB_CHECK_ARG(((reinterpret_cast<uintptr_t>(w->nibbles) | reinterpret_cast<uintptr_t>(w->scales)) % 16 | reinterpret_cast<uintptr_t>(w->rows) % 4) == 0,
+                 "%s: nibbles and scales are not 16-byte aligned, or rows not as floats are", what);
+    return LB_OK;
+}
+
 extern "C" int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int64_t* scale_bytes, int* n_padded) {
     LB_CHECK_ARG(nibble_bytes != nullptr && scale_bytes != nullptr && n_padded != nullptr, "weights4: nowhere to write the sizes");
     LB_CHECK_ARG(group == 32 || group == 64 || group == 128, "weights4: group is %d, not 32, 64 or 128", group);
@@ -155,7 +153,7 @@ extern "C" int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* n
 }
 
 extern "C" int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, int64_t lds, const float* r, const lb_weights4* w, void* stream) {
-    if (int rc = check_weights(w, "weights4_lay_out")) return rc;
+    if (int rc = weights4_check(w, "weights4_lay_out")) return rc;
     LB_CHECK_ARG(q != nullptr && s != nullptr && r != nullptr && ldq >= w->k && lds >= (w->k + w->group - 1) / w->group, "weights4_lay_out: a part is missing or its rows overlap");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
     lay_out_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(q, ldq, static_cast<const uint8_t*>(s), lds, r, *w, z.k_tiles);
@@ -163,7 +161,7 @@ extern "C" int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, 
 }
 
 extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, const lb_weights4* w, void* stream) {
-    if (int rc = check_weights(w, "weights4_quantise")) return rc;
+    if (int rc = weights4_check(w, "weights4_quantise")) return rc;
     LB_CHECK_ARG(matrix != nullptr && ldm >= w->k, "weights4_quantise: no matrix, or its rows overlap");
     LB_CHECK_ARG(dtype == LB_F32 || dtype == LB_BF16, "weights4_quantise: a matrix is float32 or bfloat16");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
@@ -173,7 +171,7 @@ extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, 
 }
 
 extern "C" int lb_weights4_values(const lb_weights4* w, float* out, int64_t ldo, void* stream) {
-    if (int rc = check_weights(w, "weights4_values")) return rc;
+    if (int rc = weights4_check(w, "weights4_values")) return rc;
     LB_CHECK_ARG(out != nullptr && ldo >= w->k, "weights4_values: no output, or its rows overlap");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
     values_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(*w, out, ldo, z.k_tiles);

@@ -75,7 +75,7 @@ def test_how_a_product_is_cut():
     assert ops.lib().lb_linear4_plan(ref, 0, (C.c_int * 4)()) != 0 and ops.lib().lb_linear4_plan(ref, 1, None) != 0
 
 
-def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=0, m=0, act=0):
+def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=ops.BF16, m=0, act=0):
     code = ops.BF16 if code is None else code
     return getattr(ops.lib(), name)(ops._linear4_args(ref or 0, a, scale, bias, residual, out, 0, 0, lda, ldr, ldo, code, out_code, m, act, 0.0, 0.0))
 
@@ -97,3 +97,22 @@ def test_products_refuse_before_they_launch():
     assert _call("lb_linear4", oref) != 0
     empty, eref = _weights(64, 256, nibbles=0)
     assert _call("lb_linear4", eref) != 0 and _call("lb_linear4", None) != 0
+
+
+@pytest.mark.parametrize("change", [dict(n=0), dict(k=0), dict(n=-16), dict(k=-128), dict(n=1 << 27), dict(n=127, paired=1), dict(group=0), dict(nibbles=(1 << 20) + 8), dict(scales=(1 << 20) + 4),
+                                    dict(rows=(1 << 20) + 2), dict(scales=0), dict(rows=0)])
+def test_weights_that_no_kernel_can_read_are_refused(change):
+    """As an invalid argument (1), by whichever entry is given them, with an error and not by a division by zero or a fault in a kernel."""
+    w = ops.Weights4Args(**{**dict(nibbles=1 << 20, scales=1 << 20, rows=1 << 20, n=128, k=256, group=128, paired=0), **change})
+    ref = C.addressof(w)
+    for m in (1, 9):
+        assert _call("lb_linear4", ref, m=m, lda=1 << 27, ldo=1 << 27) == 1 and _call("lb_gated4", ref, m=m, lda=1 << 27, ldo=1 << 27) == 1
+        assert ops.lib().lb_linear4_scratch(ref, ops.BF16, 1 << 20, 1 << 27, m) == 0 and ops.lib().lb_linear4_plan(ref, m, (C.c_int * 4)()) == 1
+    assert ops.lib().lb_weights4_values(ref, 1 << 20, 1 << 27, None) == 1
+
+
+def test_pointers_off_their_type_are_refused():
+    plain, ref = _weights(64, 256)
+    at = 1 << 20
+    for kw in (dict(a=at + 1), dict(out=at + 1), dict(out=at + 2, out_code=ops.F32), dict(bias=at + 2), dict(residual=at + 1, ldr=64), dict(code=ops.E4M3, scale=at + 2)):
+        assert _call("lb_linear4", ref, m=1, **kw) == 1, kw
