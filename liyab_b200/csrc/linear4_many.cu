@@ -135,7 +135,12 @@ __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exac
 }
 __device__ __noinline__ float gated_exact(float g, float u, int kind, float alpha, float limit) { return lb_gated_pair(g, u, kind, alpha, limit); }
 // gate(g) u of lb_gated_pair with the fast exponential and division (relative error about 1e-6), for results that are rounded to bfloat16; the gate is told apart once for four.
-__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.0f, 1.0f + __expf(-fmaxf(v, -80.0f))); }        // (the division by an infinity is none)
+// An exponential that overflows makes 1 / infinity = 0 (what is below 2^-126 is 0), and a NaN stays one.
+__device__ __forceinline__ float sigmoid_fast(float v) {
+    float s;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + __expf(-v)));
+    return s;
+}
 __device__ __forceinline__ void gated_four(float (&z)[4], const float (&g)[4], const float (&u)[4], int kind, float alpha, float limit) {
     auto all = [&](auto f) {
 #pragma unroll

@@ -410,6 +410,61 @@ def test_special_values_stay_in_their_row(dev, m):
     assert out[0].isnan().all() and out[1:, :5].isfinite().all() and out[:, 5].isnan().all()
 
 
+# Sums of gates: the ends of the range, values whose exponentials overflow, and ordinary ones.  (Not between -745 and -88: there the sigmoid is a number in 64 bits and 0 in 32.)
+GATE_SUMS = [float("inf"), -float("inf"), float("nan"), 0.0, 3e38, -3e38, 1e30, -1e30, 1e20, -1e20, 1e4, -1e4, 87.0, -87.0, 3.0, -3.0, 1e-30, -1e-30]
+OTHER_SUMS = [1.5, -2.0, 0.0, 3e38, float("inf"), -float("inf"), float("nan")]
+
+
+def _special_sums(m, k, sums, eight, paired, dev):
+    """(a, a_scale, weights, the sums in 64 bits [m, len(sums)]): a feature's only product is +-1, and its factor the sum."""
+    from liyab_b200 import ops
+    n = len(sums)
+    q, s, r = torch.zeros((n, k), dtype=torch.int8), torch.ones((n, -(-k // 64))).to(F8), torch.tensor(sums)
+    q[:, 5] = 1
+    sign = torch.where(torch.arange(m) % 3 == 2, -1.0, 1.0)
+    a = torch.zeros((m, k))
+    a[:, 5] = sign
+    a = a.to(F8 if eight else torch.bfloat16).to(dev)
+    return a, torch.ones(m, device=dev) if eight else None, ops.lay_out_weights4(q.to(dev), s.to(dev), r.to(dev), 64, paired), sign.to(dev).double()[:, None] * r.to(dev).double()
+
+
+def _gate64(g, kind, alpha, limit):
+    if kind == "gelu_tanh":
+        return g * torch.sigmoid(1.5957691216057308 * (g + 0.044715 * g ** 3))
+    return {"sigmoid": lambda: torch.sigmoid(g), "silu": lambda: g * torch.sigmoid(g), "relu": lambda: g.clamp(min=0), "capped": lambda: g.clamp(max=limit) * torch.sigmoid(alpha * g.clamp(max=limit))}[kind]()
+
+
+def _same_specials(out, want, bound):
+    """NaN and infinities (numbers past float32's range are) where 64 bits have them, the others within the bound."""
+    expected = want.float().to(out.dtype)
+    finite = expected.isfinite()
+    return torch.equal(out.isnan(), expected.isnan()) and torch.equal(out[expected.isinf()], expected[expected.isinf()]) and bool(((out.double() - want).abs() <= bound)[finite].all())
+
+
+@pytest.mark.parametrize("m,repeats", [(1, 1), (8, 1), (9, 1), (33, 1), (140, 1), (600, 30)])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("gate", ["sigmoid", "silu", "gelu_tanh"])
+def test_gates_of_special_sums(dev, m, repeats, eight, gate):
+    """On both sides of eight tokens, in small tiles, whole ones and walked ones, in both result types: what the definition makes of them in 64 bits."""
+    from liyab_b200 import ops
+    gates = [g for g in GATE_SUMS for _ in OTHER_SUMS] * repeats
+    others = [u for _ in GATE_SUMS for u in OTHER_SUMS] * repeats
+    a, scale, w, sums = _special_sums(m, 192, gates + others, eight, True, dev)
+    assert ops.linear4_plan(w, m)[0] == ("few" if m <= 8 else "walk" if m == 600 else "tiles")
+    f = len(gates)
+    g, u = sums[:, :f], sums[:, f:]
+    act = _gate64(g, gate, 1.7, 2.0)
+    if gate == "capped":
+        u = u.clamp(-2.0, 2.0) + 1.0
+    # The gate in 32 bits: the fast exponential's 2^-15 at arguments to 90, nothing below 2^-126 (times a gate of up to 88), and where 1 + tanh cancels 2^-22 of the argument.
+    off = 2.0 ** -15 * act.abs() + 1e-35 + (2.0 ** -22 * g.abs().clamp(max=20.0) if gate == "gelu_tanh" else 0.0)
+    for dtype, rounding in ((torch.float32, 2.0 ** -22), (torch.bfloat16, 2.0 ** -8)):
+        out = torch.zeros((m, f), dtype=dtype, device=dev)
+        ops.gated4(a, w, out, m, gate=gate, a_scale=scale, alpha=1.7, limit=2.0)
+        assert _same_specials(out, act * u, off * u.abs() + rounding * (act * u).abs() + 1e-37), dtype
+    assert ops.device_status() == 0
+
+
 def test_no_rows(dev):
     from liyab_b200 import ops
     q, s, r = _parts(32, 64, 32, dev)
