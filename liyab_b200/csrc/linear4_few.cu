@@ -242,7 +242,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
             }
             if (w.paired) {
                 const int col = tile * 8 + row;
-                if (col < e.n) store_out(e, token, col, lb_gated_pair(v[0] * factor[0], v[1] * factor[1], e.gate, e.alpha, e.limit));
+                if (col < e.n) store_out(e, token, col, gated_pair(v[0] * factor[0], v[1] * factor[1], e.gate, e.alpha, e.limit));
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

@@ -133,8 +133,8 @@ __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exac
         for (int i = 0; i < 8; ++i) y[i] = activate_long(y[i], act, exact, pair.a, pair.b);
     }
 }
-__device__ __noinline__ float gated_exact(float g, float u, int kind, float alpha, float limit) { return lb_gated_pair(g, u, kind, alpha, limit); }
-// gate(g) u of lb_gated_pair with the fast exponential and division (relative error about 1e-6), for results that are rounded to bfloat16; the gate is told apart once for four.
+__device__ __noinline__ float gated_exact(float g, float u, int kind, float alpha, float limit) { return gated_pair(g, u, kind, alpha, limit); }
+// gated_pair with the fast exponential and division (relative error about 1e-6), for results that are rounded to bfloat16; the gate is told apart once for four.
 // An exponential that overflows makes 1 / infinity = 0 (what is below 2^-126 is 0), and a NaN stays one.
 __device__ __forceinline__ float sigmoid_fast(float v) {
     float s;
@@ -148,12 +148,12 @@ __device__ __forceinline__ void gated_four(float (&z)[4], const float (&g)[4], c
     };
     if (kind == LB_GATE_SILU) all([](float x, float y) { return x * sigmoid_fast(x) * y; });
     else if (kind == LB_GATE_GELU_TANH) all([](float x, float y) { return x * sigmoid_fast(x * fmaf(0.07135481282553524f * x, x, 1.5957691216057308f)) * y; });
-    else if (kind == LB_GATE_RELU) all([](float x, float y) { return fmaxf(x, 0.0f) * y; });
+    else if (kind == LB_GATE_RELU) all([](float x, float y) { return at_least(x, 0.0f) * y; });
     else if (kind == LB_GATE_SIGMOID) all([](float x, float y) { return sigmoid_fast(x) * y; });
     else
         all([&](float x, float y) {
-            x = fminf(x, limit);
-            return x * sigmoid_fast(alpha * x) * (fminf(fmaxf(y, -limit), limit) + 1.0f);
+            x = at_most(x, limit);
+            return x * sigmoid_fast(alpha * x) * (at_most(at_least(y, -limit), limit) + 1.0f);
         });
 }
 

@@ -147,6 +147,29 @@ struct Epilogue {
     bool out_f32;
 };
 
+// The larger and the smaller of two numbers; a NaN stays, which fmaxf and fminf would drop.
+__device__ __forceinline__ float at_least(float v, float least) {
+    float out;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(out) : "f"(v), "f"(least));
+    return out;
+}
+__device__ __forceinline__ float at_most(float v, float most) {
+    float out;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(out) : "f"(v), "f"(most));
+    return out;
+}
+
+// lb_gated_pair, but a NaN in either half makes the result one under every gate.
+__device__ __forceinline__ float gated_pair(float g, float u, int kind, float alpha, float limit) {
+    if (kind == LB_GATE_RELU) return at_least(g, 0.0f) * u;
+    if (kind == LB_GATE_CAPPED) {
+        g = at_most(g, limit);
+        u = at_most(at_least(u, -limit), limit);
+        return g * (1.0f / (1.0f + expf(-alpha * g))) * (u + 1.0f);
+    }
+    return lb_gated_pair(g, u, kind, alpha, limit);
+}
+
 __device__ __forceinline__ void store_out(const Epilogue& e, int m, int col, float v) {
     if (e.out_f32) static_cast<float*>(e.out)[(int64_t)m * e.ldo + col] = v;
     else static_cast<__nv_bfloat16*>(e.out)[(int64_t)m * e.ldo + col] = __float2bfloat16_rn(v);

@@ -443,7 +443,7 @@ def _same_specials(out, want, bound):
 
 @pytest.mark.parametrize("m,repeats", [(1, 1), (8, 1), (9, 1), (33, 1), (140, 1), (600, 30)])
 @pytest.mark.parametrize("eight", [False, True])
-@pytest.mark.parametrize("gate", ["sigmoid", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("gate", ["sigmoid", "silu", "gelu_tanh", "relu", "capped"])
 def test_gates_of_special_sums(dev, m, repeats, eight, gate):
     """On both sides of eight tokens, in small tiles, whole ones and walked ones, in both result types: what the definition makes of them in 64 bits."""
     from liyab_b200 import ops
