@@ -248,7 +248,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                 for (int h = 0; h < 2; ++h) {
                     const int col = tile * 16 + row + 8 * h;
                     if (col >= e.n) continue;
-                    float y = lb_activate(fmaf(v[h], factor[h], biases[i * 16 + row + 8 * h]), e.act, pair);
+                    float y = activated(fmaf(v[h], factor[h], biases[i * 16 + row + 8 * h]), e.act, pair);
                     if (e.residual != nullptr) y += u == unit0 ? add[h] : e.residual[(int64_t)token * e.ldr + col];
                     store_out(e, token, col, y);
                 }

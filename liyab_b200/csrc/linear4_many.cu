@@ -114,13 +114,13 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
 // the makers' loop and this code share the instruction cache.
 __device__ __noinline__ float activate_long(float v, int act, bool exact, float a, float b) {
     const lb_act_pair pair{a, b};
-    if (exact) return lb_activate(v, act, pair);
+    if (exact) return activated(v, act, pair);
     return activate<LB_ACT_XIELU, true>(v, pair);
 }
 __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exact, const lb_act_pair& pair) {
     if (act == LB_ACT_RELU2) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = activate<LB_ACT_RELU2, true>(y[i], pair);
+        for (int i = 0; i < 8; ++i) y[i] = relu2(y[i]);
     } else if (act == LB_ACT_GELU_TANH && !exact) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = activate<LB_ACT_GELU_TANH, true>(y[i], pair);

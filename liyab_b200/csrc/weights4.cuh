@@ -159,6 +159,13 @@ __device__ __forceinline__ float at_most(float v, float most) {
     return out;
 }
 
+// lb_activate, but relu2 keeps a NaN as the others do.
+__device__ __forceinline__ float relu2(float v) {
+    const float some = at_least(v, 0.0f);
+    return some * some;
+}
+__device__ __forceinline__ float activated(float v, int act, const lb_act_pair& pair) { return act == LB_ACT_RELU2 ? relu2(v) : lb_activate(v, act, pair); }
+
 // lb_gated_pair, but a NaN in either half makes the result one under every gate.
 __device__ __forceinline__ float gated_pair(float g, float u, int kind, float alpha, float limit) {
     if (kind == LB_GATE_RELU) return at_least(g, 0.0f) * u;

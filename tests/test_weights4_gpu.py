@@ -465,6 +465,28 @@ def test_gates_of_special_sums(dev, m, repeats, eight, gate):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("m,repeats", [(1, 1), (8, 1), (9, 1), (33, 1), (140, 1), (600, 350)])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("activation", ["none", "gelu_tanh", "gelu_erf", "relu2"])
+def test_activations_of_special_sums(dev, m, repeats, eight, activation):
+    """As the gates': with xIELU's numbers behind a bias of zeros, the others with and without a bias."""
+    from liyab_b200 import ops
+    a, scale, w, z = _special_sums(m, 192, GATE_SUMS * repeats, eight, False, dev)
+    assert ops.linear4_plan(w, m)[0] == ("few" if m <= 8 else "walk" if m == 600 else "tiles")
+    n = len(GATE_SUMS) * repeats
+    bias = torch.zeros(n + 2, device=dev)
+    bias[n:] = torch.tensor([0.8, 0.4], device=dev)
+    want = _gate64(z, "gelu_tanh", 0.0, 0.0) if activation == "gelu_tanh" else z * torch.special.ndtr(z) if activation == "gelu_erf" else _activated(z, activation)[0]
+    # As for the gates; where 1 + tanh or 1 + erf cancels, and in xIELU's exponential less 1, 2^-22 of the argument.
+    off = 2.0 ** -15 * want.abs() + 1e-35 + 2.0 ** -22 * z.abs().clamp(max=20.0)
+    for dtype, rounding in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+        for b in (bias,) if activation == "xielu" else (bias, None):
+            out = torch.zeros((m, n), dtype=dtype, device=dev)
+            ops.linear4(a, w, b, out, m, activation=activation, a_scale=scale)
+            assert _same_specials(out, want, off + rounding * want.abs()), (dtype, b is None)
+    assert ops.device_status() == 0
+
+
 def test_no_rows(dev):
     from liyab_b200 import ops
     q, s, r = _parts(32, 64, 32, dev)
