@@ -112,10 +112,16 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
 
 // The epilogue's activations on eight sums; results that are rounded to bfloat16 take the fast exponential and division (gemm_tile.cuh).  What is long stays out of line:
 // the makers' loop and this code share the instruction cache.
+// xIELU without a branch: the positive part feeds the square, the negative part exp(n) - 1 - n, which near 0 is the head of its series (the next term is below 5e-6 of it; the
+// difference would keep nothing of numbers below 1e-7).
+__device__ __forceinline__ float xielu_fast(float v, float a, float b) {
+    const float pos = fmaxf(v, 0.0f), neg = fminf(v, 0.0f);
+    const float series = neg * neg * fmaf(neg, fmaf(neg, 1.0f / 24.0f, 1.0f / 6.0f), 0.5f);
+    return fmaf(a * pos, pos, fmaf(b, neg > -0.0625f ? series : __expf(neg) - 1.0f - neg, 0.5f * v));        // (a NaN comes through the last term)
+}
 __device__ __noinline__ float activate_long(float v, int act, bool exact, float a, float b) {
-    const lb_act_pair pair{a, b};
-    if (exact) return activated(v, act, pair);
-    return activate<LB_ACT_XIELU, true>(v, pair);
+    if (exact) return activated(v, act, lb_act_pair{a, b});
+    return xielu_fast(v, a, b);
 }
 __device__ __forceinline__ void activate_eight(float (&y)[8], int act, bool exact, const lb_act_pair& pair) {
     if (act == LB_ACT_RELU2) {

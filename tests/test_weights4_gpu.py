@@ -467,7 +467,7 @@ def test_gates_of_special_sums(dev, m, repeats, eight, gate):
 
 @pytest.mark.parametrize("m,repeats", [(1, 1), (8, 1), (9, 1), (33, 1), (140, 1), (600, 350)])
 @pytest.mark.parametrize("eight", [False, True])
-@pytest.mark.parametrize("activation", ["none", "gelu_tanh", "gelu_erf", "relu2"])
+@pytest.mark.parametrize("activation", ["none", "gelu_tanh", "gelu_erf", "xielu", "relu2"])
 def test_activations_of_special_sums(dev, m, repeats, eight, activation):
     """As the gates': with xIELU's numbers behind a bias of zeros, the others with and without a bias."""
     from liyab_b200 import ops
@@ -484,6 +484,24 @@ def test_activations_of_special_sums(dev, m, repeats, eight, activation):
             out = torch.zeros((m, n), dtype=dtype, device=dev)
             ops.linear4(a, w, b, out, m, activation=activation, a_scale=scale)
             assert _same_specials(out, want, off + rounding * want.abs()), (dtype, b is None)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("m,repeats", [(1, 1), (9, 1), (140, 1), (600, 70)])
+def test_xielu_of_small_sums(dev, m, repeats):
+    """exp(v) - 1 - v of small v, in both result types: to the results' own rounding, not to that of 1."""
+    from liyab_b200 import ops
+    sums = [s * d * 10.0 ** -p for p in range(30) for s in (1.0, -1.0) for d in (1.0, 2.7)] * repeats
+    a, scale, w, z = _special_sums(m, 192, sums, False, False, dev)
+    assert ops.linear4_plan(w, m)[0] == ("few" if m <= 8 else "walk" if m == 600 else "tiles")
+    bias = torch.zeros(len(sums) + 2, device=dev)
+    bias[-2:] = torch.tensor([0.8, 0.4], device=dev)
+    want, size = _activated(z, "xielu")[0], z.abs()
+    for dtype, rounding in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+        out = torch.zeros((m, len(sums)), dtype=dtype, device=dev)
+        ops.linear4(a, w, bias, out, m, activation="xielu")
+        # Terms no larger than twice the argument, each with the fast exponential's 2^-15 (argument below 3) of its own size at the worst where it is not cancelled.
+        assert ((out.double() - want).abs() <= rounding * want.abs() + 2.0 ** -14 * size.clamp(max=1.0) + 2.0 ** -15 * want.abs()).all(), dtype
     assert ops.device_status() == 0
 
 
