@@ -29,7 +29,7 @@ __device__ __forceinline__ float largest(float top, float v) {
 __device__ __forceinline__ float row_factor(float top, float* scale) {
     const bool some = __float_as_uint(top) < kInfinity && top >= kSmallest;
     *scale = some ? top * (1.0f / 448.0f) : __float_as_uint(top) < kInfinity ? 0.0f : __int_as_float(0x7fc00000);
-    return some ? __fdividef(448.0f, top) : 0.0f;
+    return some ? __fdividef(448.0f / 256.0f, top * (1.0f / 256.0f)) : 0.0f;         // (the fast division makes 0 of divisors above 2^126)
 }
 
 // 8 values from 16 or 32 bytes.

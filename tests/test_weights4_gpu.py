@@ -596,6 +596,34 @@ def test_norm_of_special_rows(dev):
         assert (half[1] == 0).all() and half[3].isnan().all() and half[[0, 1, 4, 5, 6]].isfinite().all()
 
 
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("width", [40, 41, 42, 512, 1600, 9000, 9001])
+@pytest.mark.parametrize("x_type", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ends", ["large"])
+def test_norm_at_the_ends_of_the_range(dev, rows, width, x_type, ends):
+    """Rows whose largest |h| lies above 2^126 (gains of 1.5e38), and rows so small that 448 / |t| is no float32 number, zeros among their values."""
+    from liyab_b200 import ops
+    g = torch.Generator().manual_seed(width)
+    x = (0.5 + 0.5 * torch.rand((rows, width), generator=g)) * (torch.randint(0, 2, (rows, width), generator=g) * 2.0 - 1.0)
+    gain = None
+    if ends == "large":
+        gain = torch.full((width,), 1.5e38, device=dev)
+    else:
+        x = torch.where(torch.rand((rows, width), generator=g) < 0.2, torch.zeros(()), x * 1e-37)
+        x[:, 0] = 1e-37
+    x = x.to(x_type).to(dev)
+    h = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt() * (1.0 if gain is None else gain.double())
+    top = h.abs().amax(1)
+    out, scale, half = torch.empty((rows, width), dtype=F8, device=dev), torch.empty(rows, device=dev), torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+    ops.rms_add(x, None, gain, 1e-6, out, scale=scale)
+    ops.rms_add(x, None, gain, 1e-6, half)
+    # The bounds of test_norm.
+    assert ((scale.double() - top / 448.0).abs() <= 2.0 ** -16 * top / 448.0).all()
+    got = out.double() * scale.double()[:, None]
+    assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2.0 ** -16 * h.abs()).all()
+    assert ((half.double() - h).abs() <= (2.0 ** -8 + 2.0 ** -17) * h.abs()).all()
+
+
 # ---- together, and refusals --------------------------------------------------------------------------------
 
 def test_a_block_on_its_own_stream_and_in_a_graph(dev):
