@@ -133,7 +133,15 @@ rms_add_kernel(const Rows p) {
     }
     float scale;
     float f = row_factor(__uint_as_float(bits) * inv, &scale);
-    if (f != 0.0f) f *= inv;
+    if (f * inv < __uint_as_float(kInfinity)) {
+        f *= inv;
+    } else if (f != 0.0f) {
+        // Values so small that one factor for both would be an infinity: the root meets them first.
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] *= inv;
+    }
     if (tid == 0) p.scale[r] = scale;
 #pragma unroll
     for (int j = 0; j < V; ++j) {

@@ -599,7 +599,7 @@ def test_norm_of_special_rows(dev):
 @pytest.mark.parametrize("rows", [5, 300])
 @pytest.mark.parametrize("width", [40, 41, 42, 512, 1600, 9000, 9001])
 @pytest.mark.parametrize("x_type", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("ends", ["large"])
+@pytest.mark.parametrize("ends", ["large", "small"])
 def test_norm_at_the_ends_of_the_range(dev, rows, width, x_type, ends):
     """Rows whose largest |h| lies above 2^126 (gains of 1.5e38), and rows so small that 448 / |t| is no float32 number, zeros among their values."""
     from liyab_b200 import ops
