@@ -25,7 +25,7 @@ int check(const char* what, const lb_linear4_args* p, bool paired) {
     LB_CHECK_ARG((w->paired != 0) == paired, "%s: the weights are %slaid out in pairs", what, paired ? "not " : "");
     LB_CHECK_ARG(p->M >= 0 && (p->M == 0 || (p->a != nullptr && p->out != nullptr)), "%s: %d rows, or no memory for them", what, p->M);
     LB_CHECK_ARG(p->M <= 65535 * 16, "%s: %d rows are more than %d", what, p->M, 65535 * 16);
-    LB_CHECK_ARG(p->lda >= w->k && p->ldo >= (paired ? w->n / 2 : w->n) && (p->residual == nullptr || p->ldr >= w->n), "%s: rows overlap", what);
+    LB_CHECK_ARG(p->M == 1 || (p->lda >= w->k && p->ldo >= (paired ? w->n / 2 : w->n) && (p->residual == nullptr || p->ldr >= w->n)), "%s: rows overlap", what);
     LB_CHECK_ARG(p->a_dtype == LB_BF16 || p->a_dtype == LB_E4M3, "%s: activations are bfloat16 or e4m3", what);
     LB_CHECK_ARG((p->a_dtype == LB_E4M3) == (p->a_scale != nullptr), "%s: e4m3 activations have a scale a row, bfloat16 ones have none", what);
     LB_CHECK_ARG(p->out_dtype == LB_BF16 || p->out_dtype == LB_F32, "%s: the output is bfloat16 or float32", what);
@@ -35,6 +35,9 @@ int check(const char* what, const lb_linear4_args* p, bool paired) {
     return LB_OK;
 }
 
+// A single row has no stride.
+int64_t stride_of(const lb_linear4_args* p) { return p->M > 1 ? p->lda : 0; }
+
 }  // namespace
 
 extern "C" int lb_linear4(const lb_linear4_args* p) {
@@ -42,7 +45,7 @@ extern "C" int lb_linear4(const lb_linear4_args* p) {
     LB_CHECK_ARG(p->act >= LB_ACT_NONE && p->act <= LB_ACT_RELU2 && (p->act != LB_ACT_XIELU || p->bias != nullptr), "linear4: activation %d", p->act);
     if (p->M == 0) return LB_OK;
     const Epilogue e{p->a_scale, p->bias, p->residual, p->out, p->ldr, p->ldo, p->M, p->w->n, p->act, 0, 0.0f, 0.0f, p->out_dtype == LB_F32};
-    return launch(p->w, p->a_dtype, p->a, p->lda, e, p->w->n, p->scratch, static_cast<cudaStream_t>(p->stream));
+    return launch(p->w, p->a_dtype, p->a, stride_of(p), e, p->w->n, p->scratch, static_cast<cudaStream_t>(p->stream));
 }
 
 extern "C" int lb_gated4(const lb_linear4_args* p) {
@@ -51,7 +54,7 @@ extern "C" int lb_gated4(const lb_linear4_args* p) {
     LB_CHECK_ARG(p->bias == nullptr && p->residual == nullptr, "gated4: neither a bias nor a residual is added");
     if (p->M == 0) return LB_OK;
     const Epilogue e{p->a_scale, nullptr, nullptr, p->out, 0, p->ldo, p->M, p->w->n / 2, LB_ACT_NONE, p->act, p->alpha, p->limit, p->out_dtype == LB_F32};
-    return launch(p->w, p->a_dtype, p->a, p->lda, e, 2 * ((e.n + 7) / 8 * 8), p->scratch, static_cast<cudaStream_t>(p->stream));
+    return launch(p->w, p->a_dtype, p->a, stride_of(p), e, 2 * ((e.n + 7) / 8 * 8), p->scratch, static_cast<cudaStream_t>(p->stream));
 }
 
 extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {

@@ -304,12 +304,13 @@ int launch(const Rows& p) {
 
 extern "C" int lb_rms_add_rows(const lb_rms_add_args* args) {
     LB_CHECK_ARG(args != nullptr, "rms_add: no arguments");
-    const lb_rms_add_args& p = *args;
+    lb_rms_add_args p = *args;
     LB_CHECK_ARG(p.rows >= 0 && (p.rows == 0 || (p.x != nullptr && p.out != nullptr)), "rms_add: %d rows, or no memory for them", p.rows);
     LB_CHECK_ARG(p.width > 0 && p.width <= kMaxWidth, "rms_add: rows of %d values (1 to %d)", p.width, kMaxWidth);
     LB_CHECK_ARG((p.x_dtype == LB_F32 || p.x_dtype == LB_BF16) && (p.delta_dtype == LB_F32 || p.delta_dtype == LB_BF16), "rms_add: x and delta are float32 or bfloat16");
     LB_CHECK_ARG(p.out_dtype == LB_BF16 || p.out_dtype == LB_E4M3, "rms_add: the output is bfloat16 or e4m3");
     LB_CHECK_ARG((p.out_dtype == LB_E4M3) == (p.scale != nullptr), "rms_add: an e4m3 output has a scale a row, a bfloat16 one has none");
+    if (p.rows == 1) p.ldx = p.ldd = p.ldt = p.ldo = p.width;         // a single row has no stride
     LB_CHECK_ARG(p.ldx >= p.width && p.ldo >= p.width && (p.delta == nullptr || p.ldd >= p.width) && (p.total == nullptr || p.ldt >= p.width), "rms_add: rows overlap");
     if (p.rows == 0) return LB_OK;
     if (p.x_dtype == LB_F32) return p.delta_dtype == LB_F32 ? launch<float, float>(p) : launch<float, __nv_bfloat16>(p);

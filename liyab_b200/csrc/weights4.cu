@@ -154,7 +154,7 @@ extern "C" int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* n
 
 extern "C" int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, int64_t lds, const float* r, const lb_weights4* w, void* stream) {
     if (int rc = weights4_check(w, "weights4_lay_out")) return rc;
-    LB_CHECK_ARG(q != nullptr && s != nullptr && r != nullptr && ldq >= w->k && lds >= (w->k + w->group - 1) / w->group, "weights4_lay_out: a part is missing or its rows overlap");
+    LB_CHECK_ARG(q != nullptr && s != nullptr && r != nullptr && (w->n == 1 || (ldq >= w->k && lds >= (w->k + w->group - 1) / w->group)), "weights4_lay_out: a part is missing or its rows overlap");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
     lay_out_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(q, ldq, static_cast<const uint8_t*>(s), lds, r, *w, z.k_tiles);
     return finished(static_cast<cudaStream_t>(stream));
@@ -162,7 +162,7 @@ extern "C" int lb_weights4_lay_out(const int8_t* q, int64_t ldq, const void* s, 
 
 extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, const lb_weights4* w, void* stream) {
     if (int rc = weights4_check(w, "weights4_quantise")) return rc;
-    LB_CHECK_ARG(matrix != nullptr && ldm >= w->k, "weights4_quantise: no matrix, or its rows overlap");
+    LB_CHECK_ARG(matrix != nullptr && (w->n == 1 || ldm >= w->k), "weights4_quantise: no matrix, or its rows overlap");
     LB_CHECK_ARG(dtype == LB_F32 || dtype == LB_BF16, "weights4_quantise: a matrix is float32 or bfloat16");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
     if (dtype == LB_F32) quantise_kernel<float><<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const float*>(matrix), ldm, *w, z.k_tiles);
@@ -172,7 +172,7 @@ extern "C" int lb_weights4_quantise(int dtype, const void* matrix, int64_t ldm, 
 
 extern "C" int lb_weights4_values(const lb_weights4* w, float* out, int64_t ldo, void* stream) {
     if (int rc = weights4_check(w, "weights4_values")) return rc;
-    LB_CHECK_ARG(out != nullptr && ldo >= w->k, "weights4_values: no output, or its rows overlap");
+    LB_CHECK_ARG(out != nullptr && (w->n == 1 || ldo >= w->k), "weights4_values: no output, or its rows overlap");
     const Sizes z = sizes_of(w->n, w->k, w->paired);
     values_kernel<<<z.padded, 256, 0, static_cast<cudaStream_t>(stream)>>>(*w, out, ldo, z.k_tiles);
     LB_CHECK_LAUNCH();

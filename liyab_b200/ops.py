@@ -1236,7 +1236,7 @@ class Weights4:
 def _matrix4(t: torch.Tensor, name: str, paired: bool) -> None:
     if not t.is_cuda:
         raise invalid_argument(f"{name} is on {t.device}; the engine's kernels run on a CUDA device only")
-    if t.dim() != 2 or t.stride(1) != 1 or (paired and t.shape[0] % 2):
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (paired and t.shape[0] % 2):
         raise invalid_argument(f"weights4: {name} has to be a matrix, dense within a row, with an even number of rows when paired")
 
 
@@ -1253,7 +1253,7 @@ def lay_out_weights4(q: torch.Tensor, scales: torch.Tensor, rows: torch.Tensor, 
     """Weights that are in 4 bits already: q int8 [n, k] (-8 .. 7), scales e4m3 [n, ceil(k / group)], rows float32 [n].  Returns when they are laid out."""
     _matrix4(q, "q", paired)
     n, k = q.shape
-    if q.dtype != torch.int8 or scales.dtype != _ROWS8 or tuple(scales.shape) != (n, -(-k // group)) or scales.stride(1) != 1 or rows.shape != (n,) or not rows.is_contiguous():
+    if q.dtype != torch.int8 or scales.dtype != _ROWS8 or tuple(scales.shape) != (n, -(-k // group)) or (scales.stride(1) != 1 and k > group) or rows.shape != (n,) or not rows.is_contiguous():
         raise invalid_argument("weights4: q is int8 [n, k], scales e4m3 [n, ceil(k / group)] and rows float32 [n]")
     r = Weights4(n, k, group, paired, q.device)
     check(lib().lb_weights4_lay_out(q.data_ptr(), q.stride(0), _dev(scales, "scales"), scales.stride(0), _dev(rows, "rows", torch.float32), r.ref, stream_ptr()),
@@ -1276,7 +1276,7 @@ def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n
     if len(in_shape) != 2 or len(out_shape) != 2 or in_shape[1] != w.k or out_shape[1] != n or not 0 <= m <= in_shape[0] or m > out_shape[0]:
         raise invalid_argument(f"{what}: shapes do not fit: a {tuple(in_shape)}, w ({w.n}, {w.k}), out {tuple(out_shape)}, {m} rows")
     (lda, dense_a), (ldo, dense_out) = a.stride(), out.stride()
-    if dense_a != 1 or dense_out != 1:
+    if (dense_a != 1 and w.k != 1) or (dense_out != 1 and n != 1):
         raise invalid_argument(f"{what}: a and out have to be dense within a row")
     out_code = _DT.get(out.dtype, -1)
     if out_code < 0:
@@ -1311,7 +1311,7 @@ def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: tor
     bias_at = residual_at = ldr = 0
     if residual is not None:
         shape = residual.shape
-        if residual.dtype is not torch.float32 or residual.get_device() != w.index or len(shape) != 2 or shape[1] != w.n or shape[0] < m or residual.stride(1) != 1:
+        if residual.dtype is not torch.float32 or residual.get_device() != w.index or len(shape) != 2 or shape[1] != w.n or shape[0] < m or (residual.stride(1) != 1 and w.n != 1):
             raise invalid_argument("linear4: the residual is float32 rows of the output's width")
         residual_at, ldr = residual.data_ptr(), residual.stride(0)
     if bias is not None:
@@ -1350,11 +1350,12 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
     if code < 0 or (code == E4M3) != (scale is not None):
         raise invalid_argument(f"rms_add: out is bfloat16, or e4m3 with a scale a row; it is {out_type}")
     delta_at = total_at = gain_at = scale_at = delta_code = ldd = ldt = 0
-    (ldx, dense), (ldo, dense_out) = x.stride(), out.stride() if out.shape == shape else (0, 0)
+    no_rows = (0, -1)           # of a tensor of another shape
+    (ldx, dense), (ldo, dense_out) = x.stride(), out.stride() if out.shape == shape else no_rows
     if delta is not None:
         delta_code, delta_at = _DT.get(delta.dtype, -1), delta.data_ptr()
-        ldd, dense_delta = delta.stride() if delta.shape == shape else (0, 0)
-        if dense_delta != 1 or delta_code < 0 or delta.get_device() != index:
+        ldd, dense_delta = delta.stride() if delta.shape == shape else no_rows
+        if (dense_delta != 1 and (width != 1 or dense_delta < 0)) or delta_code < 0 or delta.get_device() != index:
             raise invalid_argument("rms_add: delta has to be float32 or bfloat16 rows of x's shape, dense within a row and on x's device")
         if total is None:
             total = x
@@ -1362,10 +1363,10 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
         total_at, ldt = x.data_ptr(), ldx
     elif total is not None:
         total_at = total.data_ptr()
-        ldt, dense_total = total.stride() if total.shape == shape else (0, 0)
-        if dense_total != 1 or total.dtype is not x_type or total.get_device() != index:
+        ldt, dense_total = total.stride() if total.shape == shape else no_rows
+        if (dense_total != 1 and (width != 1 or dense_total < 0)) or total.dtype is not x_type or total.get_device() != index:
             raise invalid_argument("rms_add: total has to be rows of x's shape and type, dense within a row and on x's device")
-    if dense != 1 or dense_out != 1 or out.get_device() != index:
+    if ((dense != 1 or dense_out != 1) and (width != 1 or dense_out < 0)) or out.get_device() != index:
         raise invalid_argument("rms_add: x and out have to be rows of one shape, dense within a row and on one device")
     if gain is not None:
         gain_at = gain.data_ptr()

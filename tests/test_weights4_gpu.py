@@ -624,6 +624,55 @@ def test_norm_at_the_ends_of_the_range(dev, rows, width, x_type, ends):
     assert ((half.double() - h).abs() <= (2.0 ** -8 + 2.0 ** -17) * h.abs()).all()
 
 
+def test_single_rows_and_columns_of_any_stride(dev):
+    """A dimension of one has no stride: a column turned over, a broadcast row and columns of one value are rows like any other."""
+    from liyab_b200 import ops
+    from liyab_b200.status import LiyabError
+    n, k = 72, 640
+    q, s, r = _parts(n, k, 64, dev)
+    ref_w, gate_w = _matrix(q, s, r, 64), _matrix(q, s, r * 0.05, 64)
+    w, pairs = ops.lay_out_weights4(q, s, r, 64), ops.lay_out_weights4(q, s, r * 0.05, 64, paired=True)
+    a = _rand((k, 1), 60, dev, torch.bfloat16)
+    want = a.t().double() @ ref_w.T
+    bound = _sum_bound(k) * (a.t().double().abs() @ ref_w.abs().T)
+    for row in (a.t(), a[:, 0].expand(1, k)):
+        out, res = torch.empty((n, 1), device=dev), _rand((n, 1), 61, dev)
+        ops.linear4(row, w, None, out.t(), 1, residual=res.t())
+        assert ((out.t().double() - want - res.t().double()).abs() <= bound + 2.0 ** -23 * res.t().abs()).all()
+        half = torch.empty((n // 2, 1), device=dev)
+        ops.gated4(row, pairs, half.t(), 1, gate="relu")
+        both = row.double() @ gate_w.T
+        size = _sum_bound(k) * (row.double().abs() @ gate_w.abs().T)
+        g, u, eg, eu = both[:, :n // 2].clamp(min=0), both[:, n // 2:], size[:, :n // 2], size[:, n // 2:]
+        assert ((half.t().double() - g * u).abs() <= eg * (u.abs() + eu) + g * eu + 2.0 ** -23 * (g * u).abs()).all()
+        normed, scale = torch.empty((k, 1), dtype=F8, device=dev), torch.empty(1, device=dev)
+        ops.rms_add(row, row.t().t(), None, 1e-6, normed.t(), scale=scale, total=torch.empty((k, 1), dtype=torch.bfloat16, device=dev).t())
+        t = 2.0 * row.double()
+        h = t / (t.square().mean() + 1e-6).sqrt()
+        assert ((normed.t().double() * scale.double() - h).abs() <= 2.0 ** -4 * h.abs() + 2.0 ** -10 * scale.double() + 2.0 ** -16 * h.abs()).all()
+    # One column: a product over k = 1, one feature, and norms of one value.
+    one, by = _rand((1, 30), 62, dev, torch.bfloat16), ops.lay_out_weights4(q[:, :1], s[:, :1].clone().view(1, n).t(), r, 64)
+    out = torch.empty((30, n), device=dev)
+    ops.linear4(one.t(), by, None, out, 30)
+    want = one.t().double() @ _matrix(q[:, :1], s[:, :1], r, 64).T
+    assert ((out.double() - want).abs() <= 2.0 ** -20 * want.abs()).all()
+    single = ops.lay_out_weights4(q[:1, :], s[:1], r[:1], 64)
+    rows, out = _rand((30, k), 63, dev, torch.bfloat16), torch.empty((1, 30), device=dev)
+    ops.linear4(rows, single, None, out.t(), 30)
+    assert ((out.t().double() - rows.double() @ ref_w[:1].T).abs() <= _sum_bound(k) * (rows.double().abs() @ ref_w[:1].abs().T)).all()
+    assert torch.equal(ops.weights4_values(ops.quantise_weights4(a.t())), ops.weights4_values(ops.quantise_weights4(a.t().clone(memory_format=torch.contiguous_format).view(1, k))))
+    out = torch.empty((1, 30), dtype=torch.bfloat16, device=dev)
+    ops.rms_add(one.t(), None, None, 1e-6, out.t())
+    want = one.double() / (one.double().square() + 1e-6).sqrt()
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -17 * want.abs()).all()
+    # Other shapes are refused for one value a row too.
+    x = torch.zeros((1, 1), device=dev)
+    for bad in (lambda: ops.rms_add(x, None, None, 1e-6, out), lambda: ops.rms_add(x, out, None, 1e-6, out[:, :1]), lambda: ops.rms_add(x, x, None, 1e-6, out[:, :1], total=x[0]),
+                lambda: ops.rms_add(x.expand(3, 1), None, None, 1e-6, torch.empty((3, 1), dtype=torch.bfloat16, device=dev))):
+        with pytest.raises(LiyabError):
+            bad()
+
+
 # ---- together, and refusals --------------------------------------------------------------------------------
 
 def test_a_block_on_its_own_stream_and_in_a_graph(dev):
