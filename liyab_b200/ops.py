@@ -1216,7 +1216,7 @@ class Weights4:
     """A matrix w[n, k] = q[n, k] s[n, k / group] r[n] in 4 bits (q in -8 .. 7, s in e4m3, r float32) as the products read it.  `paired`: 2 f rows, the f of a gate
     and the f of its other factor, for gated4.  The memory belongs to this object; made by quantise_weights4 or lay_out_weights4."""
 
-    __slots__ = ("n", "k", "group", "paired", "device", "index", "nibbles", "scales", "rows", "args", "ref")
+    __slots__ = ("n", "k", "group", "paired", "device", "index", "nibbles", "scales", "rows", "args", "ref", "few")
 
     def __init__(self, n: int, k: int, group: int, paired: bool, device: torch.device):
         nibbles, scales, padded = ctypes.c_int64(0), ctypes.c_int64(0), ctypes.c_int(0)
@@ -1227,6 +1227,10 @@ class Weights4:
         self.rows = torch.empty(padded.value, dtype=torch.float32, device=device)
         self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired))
         self.ref = ctypes.addressof(self.args)
+        # Products of up to `few` rows are read as they are, wherever the rows lie: the library is asked once, with rows that no copy takes.
+        self.few = 0
+        while self.few < 64 and lib().lb_linear4_scratch(self.ref, BF16, 2, 2 * k + 1, self.few + 1) == 0:
+            self.few += 1
 
     @property
     def nbytes(self) -> int:
@@ -1318,7 +1322,7 @@ def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: tor
         if bias.dtype is not torch.float32 or bias.get_device() != w.index or not bias.is_contiguous() or bias.numel() < w.n + (2 if activation == "xielu" else 0):
             raise invalid_argument("linear4: the bias is float32, one number a feature")
         bias_at = bias.data_ptr()
-    scratch = _scratch4(w, code, a, lda, m) if m > 8 or w.k > 8192 else None
+    scratch = _scratch4(w, code, a, lda, m) if m > w.few else None
     check(lib().lb_linear4(_linear4_args(w.ref, a.data_ptr(), scale, bias_at, residual_at, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
                                          stream_of(w.index), lda, ldr, ldo, code, out_code, m, ACTIVATIONS[activation], 0.0, 0.0)), "linear4")
     return out
@@ -1332,7 +1336,7 @@ def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = 
     if kind > 4:
         raise invalid_argument(f"gated4: no gate {gate!r}")
     code, scale, out_code, lda, ldo = _rows4("gated4", a, w, out, m, w.n // 2, a_scale)
-    scratch = _scratch4(w, code, a, lda, m) if m > 8 or w.k > 8192 else None
+    scratch = _scratch4(w, code, a, lda, m) if m > w.few else None
     check(lib().lb_gated4(_linear4_args(w.ref, a.data_ptr(), scale, 0, 0, out.data_ptr(), 0 if scratch is None else scratch.data_ptr(), stream_of(w.index), lda, 0, ldo,
                                         code, out_code, m, kind, alpha, limit)), "gated4")
     return out

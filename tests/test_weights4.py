@@ -75,6 +75,19 @@ def test_how_a_product_is_cut():
     assert ops.lib().lb_linear4_plan(ref, 0, (C.c_int * 4)()) != 0 and ops.lib().lb_linear4_plan(ref, 1, None) != 0
 
 
+@pytest.mark.parametrize("n,k,paired", [(64, 1, False), (1600, 1600, False), (4096, 8192, True), (512, 16384, False), (16, 90000, False), (16, 250000, False), (16, 2000000, False)])
+def test_which_products_never_need_scratch(n, k, paired):
+    """The number that calls compare their rows with is the library's: as many rows as the kernel for few takes."""
+    import torch
+    w = ops.Weights4(n, k, 128, paired, torch.device("cpu"))
+    kinds = []
+    for m in range(1, 12):
+        out = (C.c_int * 4)()
+        assert ops.lib().lb_linear4_plan(w.ref, m, out) == 0
+        kinds.append(out[0])
+    assert w.few == (kinds + [1]).index(1) and all(kind != 0 for kind in kinds[w.few:])
+
+
 def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=ops.BF16, m=0, act=0):
     code = ops.BF16 if code is None else code
     return getattr(ops.lib(), name)(ops._linear4_args(ref or 0, a, scale, bias, residual, out, 0, 0, lda, ldr, ldo, code, out_code, m, act, 0.0, 0.0))
