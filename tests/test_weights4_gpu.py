@@ -268,6 +268,42 @@ def _activated(z, kind, a=0.8, b=0.4):
     return z, lambda e: 1.0
 
 
+@pytest.mark.parametrize("m,n,k,group", [(1, 328, 640, 64), (7, 1001, 333, 32), (9, 328, 640, 64), (30, 1001, 333, 32), (64, 2000, 1000, 128), (100, 6400, 200, 64), (140, 328, 640, 64),
+                                         (24, 512, 8192, 128), (250, 1003, 2000, 64), (600, 3610, 200, 64), (1000, 1001, 4096, 32)])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("activation", ["none", "gelu_tanh", "gelu_erf", "xielu", "relu2"])
+def test_activations_in_both_results(dev, m, n, k, group, eight, activation):
+    """Few tokens, small tiles, whole tiles and reductions that blocks share: float32 with a residual, bfloat16 (whose exponentials are the fast ones) with and without one."""
+    from liyab_b200 import ops
+    q, s, r = _parts(n, k, group, dev, seed=m + 2)
+    r = r * 0.02
+    w, ref_w = ops.lay_out_weights4(q, s, r, group), _matrix(q, s, r, group)
+    assert ops.linear4_plan(w, m)[0] == ("few" if m <= 8 else "tiles")
+    a, scale = _rand((m, k), 44, dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    bias, res = _rand((n + 2,), 45, dev), _rand((m, n), 46, dev)
+    bias[n:] = torch.tensor([0.8, 0.4], device=dev)
+    z = rows @ ref_w.T + bias[:n].double()
+    e = _sum_bound(k) * (rows.abs() @ ref_w.abs().T + bias[:n].double().abs())
+    want, slope = _activated(z, activation)
+    # The bounds of test_walked_tiles.
+    bound = e * slope(e) + 2.0 ** -19 * (want.abs() + z.abs()) + 2.0 ** -23 * res.double().abs()
+    out = res.clone()
+    ops.linear4(a, w, bias, out, m, activation=activation, residual=out, a_scale=scale)
+    assert ((out.double() - want - res.double()).abs() <= bound).all()
+    half = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+    for residual in (None, res):
+        ops.linear4(a, w, bias, half, m, activation=activation, residual=residual, a_scale=scale)
+        total = want if residual is None else want + res.double()
+        assert ((half.double() - total).abs() <= bound + 2.0 ** -15 * (want.abs() + bound) + 2.0 ** -8 * (total.abs() + bound) + 2.0 ** -19 * z.abs()).all()
+    assert ops.device_status() == 0
+
+
 # Products whose blocks walk the tiles: remainders of rows, tokens and k tiles.
 WALKS = [(600, 7002, 200, 64), (1030, 5006, 72, 32), (700, 8010, 1000, 128)]
 
@@ -622,6 +658,41 @@ def test_norm_at_the_ends_of_the_range(dev, rows, width, x_type, ends):
     got = out.double() * scale.double()[:, None]
     assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2.0 ** -16 * h.abs()).all()
     assert ((half.double() - h).abs() <= (2.0 ** -8 + 2.0 ** -17) * h.abs()).all()
+
+
+@pytest.mark.parametrize("rows", [295, 296, 297, 1001])
+@pytest.mark.parametrize("width", [8, 40, 256, 264, 512, 520, 2048, 2056, 4096, 4104])
+@pytest.mark.parametrize("x_type,delta_type", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_norm_of_many_rows(dev, rows, width, x_type, delta_type):
+    """Enough rows for a warp a row and for more values a thread, on both sides of where those begin; the sum in place and apart, both outputs; zeros, an infinity and a NaN."""
+    from liyab_b200 import ops
+    x, delta = _rand((rows, width), 28, dev, x_type, 3.0), _rand((rows, width), 29, dev, delta_type)
+    gain = 1.0 + 0.3 * _rand((width,), 30, dev)
+    x[7], delta[7] = 0.0, 0.0
+    x[rows - 2, width - 1], delta[294, 0] = float("inf"), float("nan")
+    odd = torch.zeros(rows, dtype=torch.bool, device=dev)
+    odd[rows - 2] = odd[294] = True
+    t = x.double() + delta.double()
+    h = t / (t.square().mean(1, keepdim=True) + 1e-5).sqrt() * (0.5 + gain.double())
+    # The bounds of test_norm.
+    total_bound = (2.0 ** -24 + (2.0 ** -8 if x_type is torch.bfloat16 else 0.0)) * t.abs()
+    h_bound = 2.0 ** -17 * h.abs() + 2.0 ** -22 * (0.5 + gain.double()).abs()
+    half, total = torch.empty((rows, width), dtype=torch.bfloat16, device=dev), torch.empty_like(x)
+    ops.rms_add(x, delta, gain, 1e-5, half, total=total, gain_offset=0.5)
+    assert torch.equal(total.isnan(), t.isnan()) and torch.equal(total.isinf(), t.isinf())
+    assert ((total.double() - t).abs() <= total_bound)[t.isfinite()].all()
+    assert ((half.double() - h).abs() <= 2.0 ** -8 * h.abs() + h_bound)[~odd].all()
+    out, scale = torch.ones((rows, width), dtype=F8, device=dev), torch.ones(rows, device=dev)
+    moved = x.clone()
+    ops.rms_add(moved, delta, gain, 1e-5, out, scale=scale, gain_offset=0.5)                      # in place
+    assert torch.equal(moved.nan_to_num(7.0), total.nan_to_num(7.0))
+    assert not scale[odd].isfinite().any() and (out[odd].float() == 0).all() and scale[7] == 0 and (out[7].float() == 0).all()
+    top, fine = h.abs().amax(1), ~odd
+    assert ((scale.double() - top / 448.0).abs() <= 2.0 ** -16 * top / 448.0 + 2.0 ** -30)[fine].all()
+    got = out.double() * scale.double()[:, None]
+    assert ((got - h).abs() <= torch.maximum(2.0 ** -4 * h.abs(), 2.0 ** -10 * scale.double()[:, None]) + 2 * h_bound)[fine].all()
+    fine[7] = False
+    assert (out.float().abs().amax(1) == 448.0)[fine].all()
 
 
 def test_single_rows_and_columns_of_any_stride(dev):
