@@ -762,7 +762,9 @@ typedef struct {
     void* scales;
     float* rows;
     int n, k;               /* of the matrix; n = 2 f when paired */
-    int group, paired;
+    int group;
+    int16_t paired;
+    int16_t device;         /* the number of the device that the memory is on, plus 1: products are refused when another is current.  0: not checked */
 } lb_weights4;
 /* The bytes of a matrix's nibbles and of its scales, and its rows with the padding. */
 int lb_weights4_sizes(int n, int k, int group, int paired, int64_t* nibble_bytes, int64_t* scale_bytes, int* n_padded);
@@ -814,6 +816,7 @@ typedef struct {
     int64_t ldx, ldd, ldt, ldo;
     int x_dtype, delta_dtype, out_dtype;
     int rows, width;
+    int device;                 /* as in lb_weights4 */
     float gain_offset, eps;
 } lb_rms_add_args;
 int lb_rms_add_rows(const lb_rms_add_args* args);

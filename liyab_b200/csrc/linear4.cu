@@ -9,6 +9,14 @@ int linear4_sm_count() {
     return count;
 }
 
+int device_check(const char* what, int device) {
+    if (device <= 0) return LB_OK;
+    int current = 0;
+    LB_CHECK_CUDA(cudaGetDevice(&current));
+    LB_CHECK_ARG(current == device - 1, "%s: the tensors are on cuda:%d, the current device is cuda:%d", what, device - 1, current);
+    return LB_OK;
+}
+
 namespace {
 
 using namespace lb_w4;
@@ -32,7 +40,7 @@ int check(const char* what, const lb_linear4_args* p, bool paired) {
     auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
     LB_CHECK_ARG((at(p->a) % (p->a_dtype == LB_BF16 ? 2 : 1) | at(p->out) % (p->out_dtype == LB_BF16 ? 2 : 4) | (at(p->a_scale) | at(p->bias) | at(p->residual)) % 4) == 0,
                  "%s: a pointer is not aligned to its type", what);
-    return LB_OK;
+    return p->M > 0 ? device_check(what, w->device) : LB_OK;
 }
 
 // A single row has no stride.

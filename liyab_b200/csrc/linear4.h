@@ -8,6 +8,9 @@ int linear4_sm_count();
 // Whether a kernel can read these weights: memory, alignment, sizes (every entry point that is given weights asks first).
 int weights4_check(const lb_weights4* w, const char* what);
 
+// Whether the device with this number, less 1, is the current one (0: anyone): kernels run there.
+int device_check(const char* what, int device);
+
 // How few_tokens cuts a product: warps a block, blocks a cluster (along k), clusters, row tiles a round, bytes of shared memory.
 // warps 0: it does not take it.
 struct FewPlan {

@@ -6,7 +6,7 @@
 // barriers).  24 instructions a value at 2.3 a cycle stay below what memory takes: 4096 bfloat16 rows of 8192 43 us, 0.85 of the measured copy bandwidth (69 with the divisions,
 // selections and comparisons of a first version).
 // Rows off the 16 bytes, and of more than 16384 values, go through shared memory, one or two values at a time and neighbours by neighbouring threads.
-#include "weights4.cuh"
+#include "linear4.h"
 
 namespace {
 
@@ -313,6 +313,7 @@ extern "C" int lb_rms_add_rows(const lb_rms_add_args* args) {
     if (p.rows == 1) p.ldx = p.ldd = p.ldt = p.ldo = p.width;         // a single row has no stride
     LB_CHECK_ARG(p.ldx >= p.width && p.ldo >= p.width && (p.delta == nullptr || p.ldd >= p.width) && (p.total == nullptr || p.ldt >= p.width), "rms_add: rows overlap");
     if (p.rows == 0) return LB_OK;
+    if (int rc = device_check("rms_add", p.device)) return rc;
     if (p.x_dtype == LB_F32) return p.delta_dtype == LB_F32 ? launch<float, float>(p) : launch<float, __nv_bfloat16>(p);
     return p.delta_dtype == LB_F32 ? launch<__nv_bfloat16, float>(p) : launch<__nv_bfloat16, __nv_bfloat16>(p);
 }

@@ -1191,11 +1191,19 @@ _ROWS8 = torch.float8_e4m3fn
 # The arguments of a call as the library's structs (lb_linear4_args, lb_rms_add_args): packing them costs a fraction of a conversion each.
 # "0P": filled up to the alignment of a pointer, as the library's structs are, which are copied whole.
 _linear4_args = struct.Struct("@8P3q4i2f0P").pack
-_rms_add_args = struct.Struct("@7P4q5i2f0P").pack
+_rms_add_args = struct.Struct("@7P4q6i2f0P").pack
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _elsewhere(what: str, index: int):
+    """The error of a call whose memory is another device's than the current one: its kernels would run here and read there."""
+    return invalid_argument(f"{what}: the tensors are on cuda:{index}, the current device is cuda:{_current_device()}")
 
 
 class Weights4Args(ctypes.Structure):
-    _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _i)]
+    _fields_ = [("nibbles", _p), ("scales", _p), ("rows", _p), ("n", _i), ("k", _i), ("group", _i), ("paired", _c.c_int16), ("device", _c.c_int16)]
 
 
 for _name, _args in {
@@ -1225,7 +1233,7 @@ class Weights4:
         self.nibbles = torch.empty(nibbles.value, dtype=torch.uint8, device=device)
         self.scales = torch.empty(scales.value, dtype=torch.uint8, device=device)
         self.rows = torch.empty(padded.value, dtype=torch.float32, device=device)
-        self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired))
+        self.args = Weights4Args(self.nibbles.data_ptr(), self.scales.data_ptr(), self.rows.data_ptr(), n, k, group, int(paired), 0 if device.index is None else device.index + 1)
         self.ref = ctypes.addressof(self.args)
         # Products of up to `few` rows are read as they are, wherever the rows lie: the library is asked once, with rows that no copy takes.
         self.few = 0
@@ -1240,6 +1248,8 @@ class Weights4:
 def _matrix4(t: torch.Tensor, name: str, paired: bool) -> None:
     if not t.is_cuda:
         raise invalid_argument(f"{name} is on {t.device}; the engine's kernels run on a CUDA device only")
+    if t.get_device() != _current_device():
+        raise _elsewhere("weights4", t.get_device())
     if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (paired and t.shape[0] % 2):
         raise invalid_argument(f"weights4: {name} has to be a matrix, dense within a row, with an even number of rows when paired")
 
@@ -1259,6 +1269,8 @@ def lay_out_weights4(q: torch.Tensor, scales: torch.Tensor, rows: torch.Tensor, 
     n, k = q.shape
     if q.dtype != torch.int8 or scales.dtype != _ROWS8 or tuple(scales.shape) != (n, -(-k // group)) or (scales.stride(1) != 1 and k > group) or rows.shape != (n,) or not rows.is_contiguous():
         raise invalid_argument("weights4: q is int8 [n, k], scales e4m3 [n, ceil(k / group)] and rows float32 [n]")
+    if scales.device != q.device or rows.device != q.device:
+        raise invalid_argument(f"weights4: q is on {q.device}, the scales on {scales.device} and the rows on {rows.device}")
     r = Weights4(n, k, group, paired, q.device)
     check(lib().lb_weights4_lay_out(q.data_ptr(), q.stride(0), _dev(scales, "scales"), scales.stride(0), _dev(rows, "rows", torch.float32), r.ref, stream_ptr()),
           "lay_out_weights4")
@@ -1267,6 +1279,8 @@ def lay_out_weights4(q: torch.Tensor, scales: torch.Tensor, rows: torch.Tensor, 
 
 def weights4_values(w: Weights4) -> torch.Tensor:
     """The matrix [n, k] that the weights stand for, float32."""
+    if w.index != _current_device():
+        raise _elsewhere("weights4_values", w.index)
     out = torch.empty((w.n, w.k), dtype=torch.float32, device=w.device)
     check(lib().lb_weights4_values(w.ref, out.data_ptr(), out.stride(0), stream_ptr()), "weights4_values")
     return out
@@ -1381,5 +1395,5 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
         if scale.dtype is not torch.float32 or scale.get_device() != index or scale.shape != (rows,) or not scale.is_contiguous():
             raise invalid_argument("rms_add: the scales are float32, one number a row")
     check(lib().lb_rms_add_rows(_rms_add_args(x.data_ptr(), delta_at, total_at, gain_at, out.data_ptr(), scale_at, stream_of(index), ldx, ldd, ldt, ldo,
-                                              _code(x_type, "x"), delta_code, code, rows, width, gain_offset, eps)), "rms_add")
+                                              _code(x_type, "x"), delta_code, code, rows, width, index + 1, gain_offset, eps)), "rms_add")
     return out

@@ -34,7 +34,7 @@ def test_arguments_are_as_long_as_the_library_reads_them():
     """Both products and the norm copy their arguments as one struct: a shorter one here would be read past its end."""
     length = ops.lib().lb_struct_bytes
     assert len(ops._linear4_args(*[0] * 15, 0.0, 0.0)) == length(4)
-    assert len(ops._rms_add_args(*[0] * 16, 0.0, 0.0)) == length(5)
+    assert len(ops._rms_add_args(*[0] * 17, 0.0, 0.0)) == length(5)
     assert C.sizeof(ops.Weights4Args) == length(6)
 
 

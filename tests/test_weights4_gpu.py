@@ -815,3 +815,31 @@ def test_refusals(dev):
             bad()
     with pytest.raises(KeyError):
         ops.linear4(a, w, None, out, 4, activation="tanh")
+
+
+def test_memory_of_another_device_is_refused(dev, monkeypatch):
+    """Kernels run on the current device: tensors of another one are refused before a launch (the test says that theirs is another)."""
+    from liyab_b200 import ops
+    from liyab_b200.status import LiyabError
+    q, s, r = _parts(32, 64, 32, dev)
+    w, pw = ops.lay_out_weights4(q, s, r, 32), ops.lay_out_weights4(q, s, r, 32, paired=True)
+    a, out, x = torch.zeros((4, 64), dtype=torch.bfloat16, device=dev), torch.zeros((4, 32), device=dev), torch.zeros((4, 64), device=dev)
+    set_up = (lambda: ops.weights4_values(w), lambda: ops.quantise_weights4(x, 32), lambda: ops.lay_out_weights4(q, s, r, 32))
+    products = (lambda: ops.linear4(a, w, None, out, 4), lambda: ops.gated4(a, pw, out[:, :16], 4))
+    for call in set_up + products:
+        call()
+    monkeypatch.setattr(ops, "_current_device", lambda: dev.index + 1)
+    for call in set_up:
+        with pytest.raises(LiyabError, match="current device"):
+            call()
+    w.args.device = pw.args.device = dev.index + 2
+    for call in products:
+        with pytest.raises(LiyabError, match="current device"):
+            call()
+    norm = lambda device: ops.lib().lb_rms_add_rows(ops._rms_add_args(x.data_ptr(), 0, 0, 0, a.data_ptr(), 0, ops.stream_ptr(), 64, 0, 0, 64, ops.F32, 0, ops.BF16, 4, 64, device, 0.0, 1e-6))
+    assert norm(dev.index + 1) == norm(0) == 0 and norm(dev.index + 2) == 1
+    monkeypatch.undo()
+    with pytest.raises(LiyabError):
+        ops.lay_out_weights4(q, s.cpu(), r, 32)
+    with pytest.raises(LiyabError):
+        ops.lay_out_weights4(q, s, r.cpu(), 32)
