@@ -225,7 +225,7 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
         const lb_act_pair pair = w.paired ? lb_act_pair{0.0f, 0.0f} : lb_act_load(e.bias, e.n, e.act);
         for (int u = unit0; u < units; u += splits * (int)blockDim.x) {
             const int i = (u >> 3) / e.M, token = (u >> 3) - i * e.M, row = u & 7, tile = base + i;
-            const float a_scale = a_scales[token], factor[2] = {factors[i * 16 + row] * a_scale, factors[i * 16 + row + 8] * a_scale};
+            float factor[2] = {factors[i * 16 + row], factors[i * 16 + row + 8]};
             float v[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -238,6 +238,15 @@ few_tokens_kernel(const lb_weights4 w, const void* __restrict__ a, int64_t lda, 
                         const int lo = load_remote_int(smem_u32(&parts_of[i][0]), r);
                         v[h] += load_remote(smem_u32(slots + (i + lo) * kSlot + at_slot), r);
                     }
+                }
+            }
+            if constexpr (T::kHalf) {
+                const float a_scale = a_scales[token];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float rest = split_factor(factor[h]);
+                    v[h] *= factor[h];
+                    factor[h] = rest * a_scale;
                 }
             }
             if (w.paired) {

@@ -166,11 +166,15 @@ __device__ __forceinline__ void gated_four(float (&z)[4], const float (&g)[4], c
 // What happens to the sums of a row (a lane) and eight tokens.  Of paired rows lanes 8 apart hold a feature's two sums, and each of them finishes one of two tokens.
 struct RowEnd {
     int col, up;
-    float factor, bias;
+    float factor, rest, bias;            // the row's factor: of moderate size, times a power of two (see split_factor)
+    bool extreme;                        // some row of the warp's has one
     __device__ __forceinline__ RowEnd(const Epilogue& e, const lb_weights4& w, int row, int lane, bool used) {
         up = lane >> 3 & 1;
         col = w.paired ? row / 16 * 8 + (row & 7) : row;
         factor = used ? w.rows[row] : 0.0f;
+        rest = 1.0f;
+        if (e.a_scale != nullptr) rest = split_factor(factor);
+        extreme = __any_sync(0xffffffffu, rest != 1.0f);
         bias = used && e.bias != nullptr && col < e.n ? __ldg(e.bias + col) : 0.0f;
     }
     template <int COUNT, typename O>
@@ -190,8 +194,12 @@ struct RowEnd {
             float s[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] = __ldg(e.a_scale + token + min(i, n - 1));
+            if (extreme) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] *= factor * s[i];
+                for (int i = 0; i < 8; ++i) s[i] *= rest;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = y[i] * factor * s[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] *= factor;

@@ -147,6 +147,15 @@ struct Epilogue {
     bool out_f32;
 };
 
+// The weights' factor of a row as one between 2^-60 and 2^60 (left in `factor`) and a power of two, for sums that meet a scale of the activations too: the sum is multiplied by the
+// first and then by the second times the scale, of which no product leaves float32's range before the result does (the product of two small factors would).
+__device__ __forceinline__ float split_factor(float& factor) {
+    const float size = fabsf(factor);
+    const float rest = size < 8.6736174e-19f ? 5.4210109e-20f : size > 1.1529215e18f && size < __int_as_float(0x7f800000) ? 1.8446744e19f : 1.0f;        // 2^-64, 2^64
+    factor *= size < 8.6736174e-19f ? 1.8446744e19f : rest > 1.0f ? 5.4210109e-20f : 1.0f;
+    return rest;
+}
+
 // The larger and the smaller of two numbers; a NaN stays, which fmaxf and fminf would drop.
 __device__ __forceinline__ float at_least(float v, float least) {
     float out;

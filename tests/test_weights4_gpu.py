@@ -541,6 +541,31 @@ def test_xielu_of_small_sums(dev, m, repeats):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("m,n", [(1, 264), (8, 264), (9, 264), (33, 264), (100, 264), (600, 7002)])
+def test_small_scales(dev, m, n):
+    """Rows that the norm scales by its smallest factors: the row's factor and the weights' meet the sum one after the other (their product is below the smallest normal number)."""
+    from liyab_b200 import ops
+    k = 256
+    q, s, r = _parts(n, k, 64, dev, seed=m)
+    a8, _ = _rows8(_rand((m, k), 70, dev))
+    scale = torch.full((m,), 1.5e-38, device=dev)
+    rows = a8.double() * scale.double()[:, None]
+    ref_w = _matrix(q, s, r, 64)
+    want, bound = rows @ ref_w.T, _sum_bound(k) * (rows.abs() @ ref_w.abs().T) + 2.0 ** -149
+    out = torch.empty((m, n), device=dev)
+    ops.linear4(a8, ops.lay_out_weights4(q, s, r, 64), None, out, m, a_scale=scale)
+    assert ((out.double() - want).abs() <= bound).all()
+    # The gated product: the other half's weights are as large as the row's scale is small.
+    r[n // 2:] *= 1e38
+    ref_w = _matrix(q, s, r, 64)
+    both, size = rows @ ref_w.T, _sum_bound(k) * (rows.abs() @ ref_w.abs().T) + 2.0 ** -149
+    g, u, eg, eu = both[:, :n // 2].clamp(min=0), both[:, n // 2:], size[:, :n // 2], size[:, n // 2:]
+    half = torch.empty((m, n // 2), device=dev)
+    ops.gated4(a8, ops.lay_out_weights4(q, s, r, 64, paired=True), half, m, gate="relu", a_scale=scale)
+    assert ((half.double() - g * u).abs() <= eg * (u.abs() + eu) + g * eu + 2.0 ** -23 * (g * u).abs() + 2.0 ** -149).all()
+    assert ops.device_status() == 0
+
+
 def test_no_rows(dev):
     from liyab_b200 import ops
     q, s, r = _parts(32, 64, 32, dev)
