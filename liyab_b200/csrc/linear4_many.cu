@@ -163,7 +163,8 @@ __device__ __forceinline__ void gated_four(float (&z)[4], const float (&g)[4], c
         });
 }
 
-// What happens to the sums of a row (a lane) and eight tokens.  Of paired rows lanes 8 apart hold a feature's two sums, and each of them finishes one of two tokens.
+// What happens to the sums of a row (a lane) and eight tokens.  SCALED: the activations have a scale a row (and nothing waits for the row's factor before a sum meets it where they have not).  Of paired rows lanes 8 apart hold a feature's two sums, and each of them finishes one of two tokens.
+template <bool SCALED>
 struct RowEnd {
     int col, up;
     float factor, rest, bias;            // the row's factor: of moderate size, times a power of two (see split_factor)
@@ -173,8 +174,11 @@ struct RowEnd {
         col = w.paired ? row / 16 * 8 + (row & 7) : row;
         factor = used ? w.rows[row] : 0.0f;
         rest = 1.0f;
-        if (e.a_scale != nullptr) rest = split_factor(factor);
-        extreme = __any_sync(0xffffffffu, rest != 1.0f);
+        extreme = false;
+        if (SCALED) {
+            rest = split_factor(factor);
+            extreme = __any_sync(0xffffffffu, rest != 1.0f);
+        }
         bias = used && e.bias != nullptr && col < e.n ? __ldg(e.bias + col) : 0.0f;
     }
     template <int COUNT, typename O>
@@ -190,7 +194,7 @@ struct RowEnd {
     }
     __device__ __forceinline__ void finish(const Epilogue& e, bool paired, const lb_act_pair& pair, float (&y)[8], int token) const {
         const int n = e.M - token;               // at least one
-        if (e.a_scale != nullptr) {
+        if (SCALED) {
             float s[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] = __ldg(e.a_scale + token + min(i, n - 1));
@@ -539,7 +543,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             uint32_t parity = 0;
             for (int tile = first; tile < tiles.total; tile += stride, parity ^= 1) {
                 const int m0 = tile % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
-                const RowEnd end(e, w, tile / tiles.token_tiles * kLaneRows + row, lane, true);
+                const RowEnd<T::kHalf> end(e, w, tile / tiles.token_tiles * kLaneRows + row, lane, true);
                 if (!__all_sync(0xffffffffu, wait_asleep(&c->acc_full, parity, abort_flag))) {
                     give_up(c, status, 3, quarter);
                     break;
@@ -574,7 +578,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         __syncwarp();
         const bool finishes = finisher && ok;
         const int m0 = first % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
-        const RowEnd end(e, w, first / tiles.token_tiles * kLaneRows + row, lane, finishes);
+        const RowEnd<T::kHalf> end(e, w, first / tiles.token_tiles * kLaneRows + row, lane, finishes);
         if (splits > 1) {
             // Every block's products are complete before their stages are written over.  A rank's share is a whole number of eights of tokens, the last ranks' may be none.
             const int share = share_of(tokens, splits), eights = share / 8;
