@@ -799,7 +799,7 @@ int lb_gated4(const lb_linear4_args* args);
 int64_t lb_linear4_scratch(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M);
 /* How a product of M rows is cut: plan[0] 0 by the kernel for few rows, 1 by blocks of a tile each, 2 by blocks that walk the tiles; plan[1] rows a tile; plan[2] blocks
  * that share a reduction; plan[3] clusters (0) or tiles (1, 2). */
-int lb_linear4_plan(const lb_weights4* w, int M, int* plan);
+int lb_linear4_plan(const lb_weights4* w, int M, int out_dtype, int* plan);
 /* Tests: the next launch of the kernel for many rows never announces its sums, so that its bounded waits run out. */
 int lb_linear4_withhold_next(int on);
 /* t = x + delta in 32 bits (delta may be null), total = t in x's type (may be x itself, may be null), h = t / sqrt(mean(t^2) + eps) * (gain_offset + gain) (gain may be

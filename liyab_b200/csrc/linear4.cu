@@ -65,9 +65,9 @@ extern "C" int lb_gated4(const lb_linear4_args* p) {
     return launch(p->w, p->a_dtype, p->a, stride_of(p), e, 2 * ((e.n + 7) / 8 * 8), p->scratch, static_cast<cudaStream_t>(p->stream));
 }
 
-extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {
+extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int out_dtype, int* plan) {
     if (int rc = weights4_check(w, "linear4_plan")) return rc;
-    LB_CHECK_ARG(plan != nullptr && M > 0, "linear4_plan: no rows, or no place for the answer");
+    LB_CHECK_ARG(plan != nullptr && M > 0 && (out_dtype == LB_BF16 || out_dtype == LB_F32), "linear4_plan: no rows, no such result, or no place for the answer");
     const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
     const FewPlan f = few_plan(M, rows, w->k, w->group, linear4_sm_count());
     if (f.warps > 0) {
@@ -77,7 +77,7 @@ extern "C" int lb_linear4_plan(const lb_weights4* w, int M, int* plan) {
         plan[3] = f.clusters;
         return LB_OK;
     }
-    const ManyPlan m = many_plan(M, rows, w->k, linear4_sm_count());
+    const ManyPlan m = many_plan(M, rows, w->k, out_dtype == LB_F32, linear4_sm_count());
     plan[0] = m.walk ? 2 : 1;
     plan[1] = m.tokens;
     plan[2] = m.splits;

@@ -19,11 +19,12 @@ struct FewPlan {
 FewPlan few_plan(int M, int rows, int k, int group, int n_sm);
 int few_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, const FewPlan& p, cudaStream_t stream);
 
-// How many_tokens cuts one: whether a block an SM walks the tiles, tokens a tile, blocks a cluster (along k), stages, columns of tensor memory for the sums and in all, bytes of shared memory.
+// How many_tokens cuts one: whether a block an SM walks the tiles, tokens a tile, blocks a cluster (along k), stages, columns of tensor memory for the sums and in all, bytes of shared memory; k tiles a
+// chain of the accumulator's additions, chains of a block, columns between accumulators, whether the chains take turns between two; warps that make weights.
 struct ManyPlan {
-    int walk, tokens, splits, stages, d_columns, tmem_columns, smem;
+    int walk, tokens, splits, stages, d_columns, tmem_columns, smem, chain, chains, chain_columns, turn, makers;
 };
-ManyPlan many_plan(int M, int rows, int k, int n_sm);
+ManyPlan many_plan(int M, int rows, int k, bool out_f32, int n_sm);
 // Activations that TMA does not take as they are (e4m3, rows off the 16 bytes) go through scratch memory.
 int64_t many_scratch_bytes(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M);
 int many_tokens(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, const lb_w4::Epilogue& e, void* scratch, cudaStream_t stream);

@@ -32,8 +32,8 @@ struct Control {
     uint64_t b_full[kMaxStages];
     uint64_t empty[kMaxStages];
     uint64_t raw_full[kSpreadAhead], raw_empty[kSpreadAhead];
-    uint64_t acc_full;
-    uint64_t acc_empty;
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -253,21 +253,20 @@ struct RowEnd {
 struct Tiles {
     int tokens, token_tiles, total, k_tiles, splits, n_stages, d_columns;
     int spread;              // e4m3 rows become float16 on their way
+    int chain, chain_columns;              // k tiles that one accumulator adds up; columns between accumulators
 };
 
 // Tokens of a tile that a rank of `splits` finishes, but for the last ones.
 __host__ __device__ __forceinline__ int share_of(int tokens, int splits) { return ((tokens + splits - 1) / splits + 7) / 8 * 8; }
 
-constexpr int kFinishers = 16;           // where a block walks the tiles
-
-template <int MAKERS, bool WALK>
-constexpr int threads_of() { return 32 * (kFirstMaker + MAKERS + (WALK ? kFinishers : 0)); }
-
-// WALK: a block walks the tiles blockIdx.x, blockIdx.x + gridDim.x, ..; else gridDim.x = tiles x splits, the splits of a tile a cluster.
-template <typename T, int GROUP, int MAKERS, bool WALK>
-__global__ void __launch_bounds__(threads_of<MAKERS, WALK>())
+// WALK: a block walks the tiles blockIdx.x, blockIdx.x + gridDim.x, ..; else gridDim.x = tiles x splits, the splits of a tile a cluster.  FINISHERS: warps of their own that read the sums and
+// finish; with none the makers do.  CHAINED: a tile's reduction is several chains of additions, which take turns between two accumulators (with finishing warps) or have one each.
+template <typename T, int GROUP, int MAKERS, int FINISHERS, bool WALK, bool CHAINED>
+__global__ void __launch_bounds__(32 * (kFirstMaker + MAKERS + FINISHERS))
 many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 w, const Epilogue e, const Tiles tiles, int tmem_columns, int withhold, int* status) {
     constexpr int kGroups = MAKERS / 4;
+    constexpr int kTurn = CHAINED && FINISHERS > 0 ? 1 : 0;
+    constexpr int kEnds = (FINISHERS > 0 ? FINISHERS : MAKERS) / 4;      // warps that share a quarter's sums
     constexpr bool kSpreads = T::kHalf && MAKERS == 8 && !WALK;        // where up to 32 e4m3 tokens may be a tile
     const bool spread = kSpreads && tiles.spread != 0;
     extern __shared__ uint8_t smem_raw[];
@@ -280,6 +279,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = WALK ? 0 : (int)blockIdx.x % splits, first = WALK ? (int)blockIdx.x : (int)blockIdx.x / splits, stride = WALK ? (int)gridDim.x : tiles.total;
     const int per = (k_tiles + splits - 1) / splits, kt0 = rank * per, n_kt = min(k_tiles, kt0 + per) - kt0;     // the host leaves no rank without one
+    const int chains = CHAINED ? (n_kt + tiles.chain - 1) / tiles.chain : 1;
 
     if (threadIdx.x == 0) {
         prefetch_tensormap(&map_a);
@@ -293,8 +293,10 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                 mbar_init(&c->raw_full[i], 1);
                 mbar_init(&c->raw_empty[i], 2);
             }
-        mbar_init(&c->acc_full, 1);
-        mbar_init(&c->acc_empty, kFinishers);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&c->acc_full[i], 1);
+            mbar_init(&c->acc_empty[i], FINISHERS > 0 ? FINISHERS : 1);
+        }
         c->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -360,19 +362,34 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         const uint32_t desc_hi = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
         const uint32_t lo0 = ((stages_u32 & 0x3FFFFu) >> 4) | (1u << 16);
         int st = 0;
-        uint32_t parity = 0, acc_parity = 1;
-        for (int tile = first; tile < tiles.total && ok; tile += stride, acc_parity ^= 1) {
+        uint32_t parity = 0, unit = 0;                                 // chains so far
+        for (int tile = first; tile < tiles.total && ok; tile += stride) {
             const int columns = min(tokens, (e.M - tile % tiles.token_tiles * tokens + 15) / 16 * 16);
             const uint32_t idesc = umma_idesc(kLaneRows, columns) & (T::kHalf ? ~((1u << 7) | (1u << 10)) : ~0u);
-            if (WALK) {
-                if (!__all_sync(0xffffffffu, wait_u32(smem_u32(&c->acc_empty), acc_parity, abort_flag))) {
-                    give_up(c, status, 5, 0);
-                    ok = false;
-                    break;
-                }
+            // The sums of a tile, or of a chain, begin when the finishing warps have those that were there.
+            auto begin = [&]() {
+                if (FINISHERS == 0) return true;
+                const bool free = __all_sync(0xffffffffu, wait_u32(smem_u32(&c->acc_empty[unit & kTurn]), (unit >> kTurn & 1) ^ 1, abort_flag));
+                if (!free) give_up(c, status, 5, 0);
                 tc_fence_after();
-            }
-            for (int kt = 0; kt < n_kt; ++kt) {
+                return free;
+            };
+            uint32_t sums = tmem_base + (unit & kTurn) * tiles.chain_columns;
+            int left = tiles.chain;
+            ok = begin();
+            for (int kt = 0; kt < n_kt && ok; ++kt) {
+                if (CHAINED && left-- == 0) {
+                    left = tiles.chain - 1;
+                    if (FINISHERS > 0) {
+                        if (withhold == 0 && elect_one()) umma_commit(&c->acc_full[unit & kTurn]);
+                        ++unit;
+                        sums = tmem_base + (unit & kTurn) * tiles.chain_columns;
+                        ok = begin();
+                        if (!ok) break;
+                    } else {
+                        sums += tiles.chain_columns;
+                    }
+                }
                 if (!__all_sync(0xffffffffu, wait_u32(b_full + 8 * st, parity, abort_flag) && wait_u32(a_full + 8 * st, parity, abort_flag))) {
                     give_up(c, status, 2, st);
                     ok = false;
@@ -383,7 +400,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                 if (elect_one()) {
 #pragma unroll
                     for (uint32_t k = 0; k < kTileK / kUmmaK; ++k)
-                        umma_ts(tmem_base, ta + k * (kUmmaK / 2), b_lo + (k >> 2) * (atom_bytes >> 4) + 2 * (k & 3), desc_hi, idesc, kt + k != 0 ? 1u : 0u);
+                        umma_ts(sums, ta + k * (kUmmaK / 2), b_lo + (k >> 2) * (atom_bytes >> 4) + 2 * (k & 3), desc_hi, idesc, (CHAINED ? left + 1 != tiles.chain : kt != 0) || k != 0 ? 1u : 0u);
                     commit_u32(empty + 8 * st);
                 }
                 if (++st == n_stages) {
@@ -392,7 +409,8 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
                 }
             }
             // (`withhold`: a test's launch, whose epilogues find nothing and give up.)
-            if (ok && withhold == 0 && elect_one()) umma_commit(&c->acc_full);
+            if (ok && withhold == 0 && elect_one()) umma_commit(&c->acc_full[unit & kTurn]);
+            ++unit;
         }
         lb_wait_for_predecessor();
         lb_dependents_may_launch();
@@ -441,7 +459,7 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         // No more warps take turns than there are stages: one that was a whole round of the stages ahead would take the parity of the round before for its own.
         const int turns = min(kGroups, n_stages);
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        constexpr int kDepth = WALK ? 1 : 2;                               // k tiles on the way a warp (one where registers are short: the products take longer than the loads)
+        constexpr int kDepth = FINISHERS > 0 ? 1 : 2;                               // k tiles on the way a warp (one where registers are short: the products take longer than the loads)
         uint4 words[kDepth][4];
         uint32_t steps[kDepth];
         // The k tiles of all of this block's tiles are one sequence, of which this warp takes every turns-th; `ahead` is where the next to be fetched lies.
@@ -528,7 +546,8 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
     }
     __syncwarp();
 
-    const bool finisher = WALK ? warp >= kFirstMaker + MAKERS : warp >= kFirstMaker;
+    const bool finisher = warp >= kFirstMaker + (FINISHERS > 0 ? MAKERS : 0);
+    const int part = (warp - kFirstMaker - (FINISHERS > 0 ? MAKERS : 0)) >> 2;        // this warp's eights of columns are every kEnds-th from here
     const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16);
     lb_act_pair pair{0.0f, 0.0f};
     // Scales, residuals and the learned numbers behind the bias are read, and results written, after this.
@@ -537,48 +556,96 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
         lb_dependents_may_launch();
         if (!w.paired) pair = lb_act_load(e.bias, e.n, e.act);
     }
+    // A thread's sums of the chains before wait in its own words of shared memory, [token][row].
+    float* before = reinterpret_cast<float*>(c + 1) + row;
+    uint32_t unit = 0;                           // chains that the finishing warps have seen
+    auto wait_for_sums = [&]() {
+        const bool there = __all_sync(0xffffffffu, WALK ? wait_asleep(&c->acc_full[unit & kTurn], unit >> kTurn & 1, abort_flag)
+                                                                : mbar_wait(&c->acc_full[unit & kTurn], unit >> kTurn & 1, abort_flag));
+        if (!there) give_up(c, status, 3, quarter);
+        tc_fence_after();
+        return there;
+    };
+    auto sums_read = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c->acc_empty[unit & kTurn]);
+    };
+    // Eight tokens' sums from column `at` on, the chains' added in order.
+    auto sums_at = [&](int at, float (&y)[8]) {
+        uint32_t v[8];
+        __syncwarp();                                                   // (the results' code parts lanes; a warp loads as one)
+        tmem_ld8(t_row + (unit & kTurn) * tiles.chain_columns + at, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+    };
+    auto add_before = [&](int at, float (&y)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] += before[(at + i) * kLaneRows];
+    };
+    // All chains of a tile but the last: their sums to shared memory, under the next one's products.
+    auto earlier_chains = [&](int here) {
+#pragma unroll 1
+        for (int chain = 1; chain < chains; ++chain, ++unit) {
+            if (!wait_for_sums()) return false;
+#pragma unroll 1
+            for (int at = 8 * part; at < here; at += 8 * kEnds) {
+                float y[8];
+                sums_at(at, y);
+                if (chain > 1) add_before(at, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) before[(at + i) * kLaneRows] = y[i];
+            }
+            sums_read();
+        }
+        return true;
+    };
     if (WALK) {
         if (finisher) {
-            const int fourth = (warp - kFirstMaker - MAKERS) >> 2;      // this warp's eights of columns are every fourth
-            uint32_t parity = 0;
-            for (int tile = first; tile < tiles.total; tile += stride, parity ^= 1) {
+            for (int tile = first; tile < tiles.total; tile += stride, ++unit) {
                 const int m0 = tile % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
                 const RowEnd<T::kHalf> end(e, w, tile / tiles.token_tiles * kLaneRows + row, lane, true);
-                if (!__all_sync(0xffffffffu, wait_asleep(&c->acc_full, parity, abort_flag))) {
-                    give_up(c, status, 3, quarter);
-                    break;
-                }
-                tc_fence_after();
-                // Eights of columns in turn; when the last is there the next tile's products may begin.
+                if ((CHAINED && !earlier_chains(here)) || !wait_for_sums()) break;
+                // When the last eight is there the next tile's products may begin.
 #pragma unroll 1
-                for (int at = 8 * fourth; at < here || at == 8 * fourth; at += 8 * (kFinishers / 4)) {
+                for (int at = 8 * part; at < here || at == 8 * part; at += 8 * kEnds) {
                     float y[8];
-                    __syncwarp();                                       // (the results' code parts lanes; a warp loads as one)
-                    if (at < here) {
-                        uint32_t v[8];
-                        tmem_ld8(t_row + at, v);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[k]);
-                    }
-                    if (at + 8 * (kFinishers / 4) >= here) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&c->acc_empty);
-                    }
-                    if (at < here) end.finish(e, w.paired, pair, y, m0 + at);
+                    if (at < here) sums_at(at, y);
+                    if (at + 8 * kEnds >= here) sums_read();
+                    if (at >= here) break;
+                    if (CHAINED && chains > 1) add_before(at, y);
+                    end.finish(e, w.paired, pair, y, m0 + at);
                 }
             }
         }
     } else {
+        const int m0 = first % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
         if (finisher) {
-            ok = __all_sync(0xffffffffu, ok && (mbar_wait(&c->acc_full, 0, abort_flag)));
-            if (!ok) give_up(c, status, 3, quarter);
-            tc_fence_after();
+            if (FINISHERS > 0) {
+                ok = (!CHAINED || earlier_chains(here)) && wait_for_sums();
+            } else {
+                ok = __all_sync(0xffffffffu, ok && (mbar_wait(&c->acc_full[0], 0, abort_flag)));
+                if (!ok) give_up(c, status, 3, quarter);
+                tc_fence_after();
+            }
         }
         __syncwarp();
         const bool finishes = finisher && ok;
-        const int m0 = first % tiles.token_tiles * tokens, here = min(tokens, e.M - m0);
         const RowEnd<T::kHalf> end(e, w, first / tiles.token_tiles * kLaneRows + row, lane, finishes);
+        auto all_sums_at = [&](int at, float (&y)[8]) {
+            sums_at(at, y);
+            if (FINISHERS > 0) {
+                if (CHAINED && chains > 1) add_before(at, y);
+            } else if (CHAINED) {
+#pragma unroll 1
+                for (int chain = 1; chain < chains; ++chain) {
+                    uint32_t v[8];
+                    tmem_ld8(t_row + chain * tiles.chain_columns + at, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += __uint_as_float(v[i]);
+                }
+            }
+        };
         if (splits > 1) {
             // Every block's products are complete before their stages are written over.  A rank's share is a whole number of eights of tokens, the last ranks' may be none.
             const int share = share_of(tokens, splits), eights = share / 8;
@@ -586,19 +653,19 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             if (finishes) {
-                for (int piece = group; 8 * piece < here; piece += kGroups) {
-                    uint32_t v[8];
-                    tmem_ld8(t_row + 8 * piece, v);
+                for (int piece = part; 8 * piece < here; piece += kEnds) {
+                    float y[8];
+                    all_sums_at(8 * piece, y);
                     const int to = piece / eights;
                     const uint32_t peer = peer_address(smem_u32(box + (rank * eights + piece - to * eights) * 2 * kLaneRows), (uint32_t)to);
-                    store_at_peer(peer, v[0], v[1], v[2], v[3]);
-                    store_at_peer(peer + kLaneRows * 16, v[4], v[5], v[6], v[7]);
+                    store_at_peer(peer, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+                    store_at_peer(peer + kLaneRows * 16, __float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7]));
                 }
             }
             __syncwarp();
             asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             if (finishes) {
-                for (int piece = group; piece < eights && rank * share + 8 * piece < here; piece += kGroups) {
+                for (int piece = part; piece < eights && rank * share + 8 * piece < here; piece += kEnds) {
                     float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                     for (int r = 0; r < splits; ++r) {
                         const float4 lo = box[(r * eights + piece) * 2 * kLaneRows], hi = box[((r * eights + piece) * 2 + 1) * kLaneRows];
@@ -610,13 +677,9 @@ many_tokens_kernel(const __grid_constant__ CUtensorMap map_a, const lb_weights4 
             }
         } else if (finishes) {
 #pragma unroll 1
-            for (int at = 8 * group; at < here; at += 8 * kGroups) {
-                uint32_t v[8];
-                __syncwarp();
-                tmem_ld8(t_row + at, v);
+            for (int at = 8 * part; at < here; at += 8 * kEnds) {
                 float y[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(v[i]);
+                all_sums_at(at, y);
                 end.finish(e, w.paired, pair, y, m0 + at);
             }
         }
@@ -646,9 +709,9 @@ __global__ void spread_rows_kernel(const void* __restrict__ a, int64_t lda, bool
 
 int g_withhold_next = 0;      // the next launch's blocks leave their accumulator-ready barriers unsignalled (tests)
 
-template <typename T, int GROUP, int MAKERS, bool WALK>
+template <typename T, int GROUP, int MAKERS, int FINISHERS, bool WALK, bool CHAINED>
 int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
-    auto kernel = many_tokens_kernel<T, GROUP, MAKERS, WALK>;
+    auto kernel = many_tokens_kernel<T, GROUP, MAKERS, FINISHERS, WALK, CHAINED>;
     static bool configured = false;
     if (!configured) {
         LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
@@ -657,7 +720,7 @@ int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& 
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
     const int blocks = WALK ? (tiles.total < n_sm ? tiles.total : n_sm) : tiles.total * p.splits;
-    LB_CHECK_CUDA(lb_launch_overlapped_cluster(1, p.splits, kernel, dim3(blocks), dim3(threads_of<MAKERS, WALK>()), p.smem, s, map, *w, e, tiles, p.tmem_columns, g_withhold_next,
+    LB_CHECK_CUDA(lb_launch_overlapped_cluster(1, p.splits, kernel, dim3(blocks), dim3(32 * (kFirstMaker + MAKERS + FINISHERS)), p.smem, s, map, *w, e, tiles, p.tmem_columns, g_withhold_next,
                                                status));
     g_withhold_next = 0;
     return LB_OK;
@@ -665,9 +728,12 @@ int launch_kernel(const CUtensorMap& map, const lb_weights4* w, const Epilogue& 
 
 template <typename T, int GROUP>
 int launch(const CUtensorMap& map, const lb_weights4* w, const Epilogue& e, const ManyPlan& p, const Tiles& tiles, int n_sm, cudaStream_t s) {
-    if (p.walk) return launch_kernel<T, GROUP, 8, true>(map, w, e, p, tiles, n_sm, s);
-    if (p.tmem_columns == 256) return launch_kernel<T, GROUP, 8, false>(map, w, e, p, tiles, n_sm, s);
-    return launch_kernel<T, GROUP, 16, false>(map, w, e, p, tiles, n_sm, s);
+    if (p.makers == 12)
+        return p.walk ? launch_kernel<T, GROUP, 12, 12, true, true>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 12, 12, false, true>(map, w, e, p, tiles, n_sm, s);
+    if (p.walk) return launch_kernel<T, GROUP, 8, 16, true, false>(map, w, e, p, tiles, n_sm, s);
+    if (p.makers == 8)
+        return p.chains > 1 ? launch_kernel<T, GROUP, 8, 0, false, true>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 8, 0, false, false>(map, w, e, p, tiles, n_sm, s);
+    return p.chains > 1 ? launch_kernel<T, GROUP, 16, 0, false, true>(map, w, e, p, tiles, n_sm, s) : launch_kernel<T, GROUP, 16, 0, false, false>(map, w, e, p, tiles, n_sm, s);
 }
 
 // Whether e4m3 rows become float16 on their way, in a small tile's block: rows that TMA takes (24 x 8000 x 3008 9.5 us).  With more tokens, whose
@@ -676,12 +742,14 @@ bool spreads(const ManyPlan& p, const lb_weights4* w, const void* a, int64_t lda
     return p.tmem_columns == 256 && !p.walk && p.tokens <= kSpreadTokens && w->k % 2 == 0 && lda % 16 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0;
 }
 
+bool copied_as_they_are(const void* a, int64_t lda) { return lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0; }       // bfloat16 rows that TMA takes
+
 template <typename T>
 int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, void* scratch, cudaStream_t s) {
     const int k_tiles = (w->k + kTileK - 1) / kTileK, rows = w->paired ? 2 * ((e.n + 7) / 8 * 8) : e.n, row_blocks = (rows + kLaneRows - 1) / kLaneRows, n_sm = linear4_sm_count();
-    const ManyPlan p = many_plan(e.M, rows, w->k, n_sm);
+    const ManyPlan p = many_plan(e.M, rows, w->k, e.out_f32, n_sm);
     const bool spread = T::kHalf && spreads(p, w, a, lda);
-    if (!spread && many_scratch_bytes(w, T::kHalf ? LB_E4M3 : LB_BF16, a, lda, e.M) > 0) {
+    if (!spread && (T::kHalf || !copied_as_they_are(a, lda))) {
         LB_CHECK_ARG(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "linear4: these activations need scratch memory (lb_linear4_scratch)");
         const bool wide = lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % (T::kHalf ? 8 : 16) == 0;
         const int eights = (w->k + 7) / 8;
@@ -696,7 +764,7 @@ int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, voi
     if (int rc = spread ? lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k / 2, lda / 2, p.tokens) : lb_tensor_map_2d_encode(&map, a, 2, e.M, w->k, lda, p.tokens)) return rc;
     const int token_tiles = (e.M + p.tokens - 1) / p.tokens;
     LB_CHECK_ARG((int64_t)token_tiles * row_blocks * p.splits < (1ll << 30), "linear4: %d rows by %d features are too many tiles", e.M, rows);
-    const Tiles tiles{p.tokens, token_tiles, token_tiles * row_blocks, k_tiles, p.splits, p.stages, p.d_columns, spread};
+    const Tiles tiles{p.tokens, token_tiles, token_tiles * row_blocks, k_tiles, p.splits, p.stages, p.d_columns, spread, p.chain, p.chain_columns};
     if (w->group == 32) return launch<T, 32>(map, w, e, p, tiles, n_sm, s);
     if (w->group == 64) return launch<T, 64>(map, w, e, p, tiles, n_sm, s);
     return launch<T, 128>(map, w, e, p, tiles, n_sm, s);
@@ -707,37 +775,61 @@ int run(const lb_weights4* w, const void* a, int64_t lda, const Epilogue& e, voi
 // The cheapest cut by an estimate in us (a fit to some 150 launches of 24 to 2,048 tokens): 2.8 for the launch and the first weights; a k tile takes what its eight products take, which is no
 // less than it takes the tensor core to load 128 x 128 weights (0.34, up to some 150 tokens; 0.57 for each of two blocks that share an SM); a token's column of sums 0.0115;
 // the exchange of a cluster grows with its ranks and their tokens.
-ManyPlan many_plan(int M, int rows, int k, int n_sm) {
+// The tensor core truncates the sum at each of its additions, which adds up along a chain: 3.4e-7 of the results at 2,048 values of k, 8e-7 at 4,096, 2.0e-6 at 8,192, 5.1e-6 at 16,384 (the
+// additions of a product in 32 bits 1.1e-7 to 4.4e-7).  So float32 results have chains of kChain k tiles, whose sums are added in 32 bits; bfloat16's rounding hides either.  Where there are
+// columns, a chain has an accumulator of its own in tensor memory; else twelve warps move its sums to shared memory under the products of the next, which has another accumulator.
+ManyPlan many_plan(int M, int rows, int k, bool out_f32, int n_sm) {
+    constexpr int kChain = 12;
     ManyPlan best{};
     const int k_tiles = (k + kTileK - 1) / kTileK, row_blocks = (rows + kLaneRows - 1) / kLaneRows, fewest = (M + 255) / 256;
+    const bool deep = out_f32 && k_tiles > kChain;
     double least_us = 1e30;
     for (int token_tiles = fewest; token_tiles <= 2 * fewest + 2; ++token_tiles) {
         const int tokens = ((M + token_tiles - 1) / token_tiles + 15) / 16 * 16;
         if (token_tiles > fewest && tokens < 32) break;
         const long total = (long)((M + tokens - 1) / tokens) * row_blocks;
         const double stage = 0.55 * tokens / 256 > 0.34 ? 0.55 * tokens / 256 : 0.34, sums = 0.0115 * tokens;
-        for (int splits = 1; splits <= 8; ++splits) {
+        // (Each cut once, but for deep products that no cluster shares: by blocks of a tile each and by blocks that walk.)
+        for (int way = 1; way <= (deep ? 9 : 8); ++way) {
+            const int splits = way < 9 ? way : 1;
             ManyPlan p{};
             const int per = (k_tiles + splits - 1) / splits;
             if (splits > 1 && (per < 3 || per * (splits - 1) >= k_tiles)) continue;      // short parts, or a rank without one
             p.tokens = tokens;
             p.splits = splits;
-            p.d_columns = tokens <= 64 ? 64 : tokens <= 128 ? 128 : 256;
-            const bool two = p.d_columns == 64;                       // two blocks an SM, whose starts and ends hide under one another
-            p.walk = splits == 1 && !two && total > n_sm;
-            p.stages = two || p.d_columns == 256 ? 3 : 6;
+            p.chains = deep ? (per + kChain - 1) / kChain : 1;
+            p.chain = (per + p.chains - 1) / p.chains;
+            p.chain_columns = (tokens + 31) / 32 * 32;
+            p.turn = p.chains > 1 && (way == 9 || p.chains * p.chain_columns > 320);
+            const int columns = p.chains == 1 ? tokens : p.chain_columns * (p.turn ? 2 : p.chains);
+            if (columns > 320) continue;
+            const bool two = way < 9 && !p.turn && columns <= 64;     // two blocks an SM, whose starts and ends hide under one another
+            p.walk = deep ? way == 9 : splits == 1 && !two && total > n_sm;
+            p.makers = p.turn ? 12 : two || p.walk ? 8 : 16;
+            p.d_columns = two ? 64 : columns <= 128 ? 128 : columns <= 256 ? 256 : 320;
+            p.stages = two || p.d_columns >= 256 ? 3 : 6;
             p.tmem_columns = two ? 256 : 512;
+            const int before = p.turn ? tokens * kLaneRows * 4 : 0;                      // the sums of the chains before
+            while (p.stages > 3 && 1024 + p.stages * tokens * 256 + (int)sizeof(Control) + before > 227 * 1024) --p.stages;
             // The blocks of a cluster wait for one another while each holds its columns: as large a share of the shared memory as of the columns (see gemm_tcgen05_narrow.cu).
             const int in_stages = p.stages * tokens * 256, inbox = splits > 1 ? splits * share_of(tokens, splits) * 512 : 0;
-            const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control) + (two && tokens <= kSpreadTokens ? 1024 + kSpreadAhead * tokens * kTileK : 0), least = p.tmem_columns * (228 * 1024 / 512) - 1024;
+            const int needed = 1024 + (in_stages > inbox ? in_stages : inbox) + (int)sizeof(Control) + before + (two && tokens <= kSpreadTokens ? 1024 + kSpreadAhead * tokens * kTileK : 0);
+            const int least = p.tmem_columns * (228 * 1024 / 512) - 1024;
             p.smem = needed < least ? least : needed;
             if (p.smem > 227 * 1024) continue;
-            // Clusters lie within one group of SMs, which those of more than two blocks do not fill; a second wave of blocks is worth no split.
+            // Clusters lie within one group of SMs, which those of more than two blocks do not fill; a second wave of blocks is worth no split, unless for the chains' sake.
             const long blocks = total * splits, at_once = (long)n_sm * (splits <= 2 ? 148 : splits == 3 ? 144 : splits == 4 ? 132 : 104) / 148;
-            if (splits > 1 && blocks > (two && splits == 2 ? 2 * at_once : at_once)) continue;
+            if (!deep && splits > 1 && blocks > (two && splits == 2 ? 2 * at_once : at_once)) continue;
+            const double exchange = splits > 1 ? 0.8 + (0.005 * splits + 0.004) * tokens : 0.0;
             double us = 2.8;
-            if (p.walk) us += (double)((total + n_sm - 1) / n_sm) * (per * stage + 0.4 + sums);
-            else us += (double)((blocks + 2 * n_sm - 1) / (2 * n_sm)) * per * (two && blocks > n_sm ? 0.57 : stage) + sums / splits + (splits > 1 ? 0.8 + (0.005 * splits + 0.004) * tokens : 0.0);
+            if (p.walk) {
+                us += (double)((total + n_sm - 1) / n_sm) * (per * (p.turn && stage < 0.4 ? 0.4 : stage) + 0.4 + sums);
+            } else if (deep) {
+                const long fit = two ? 2 * at_once : at_once, waves = (blocks + fit - 1) / fit;
+                us += waves * (per * (two && blocks > at_once ? 0.57 : p.turn && stage < 0.4 ? 0.4 : stage) + sums / splits + exchange) + (waves - 1) * 4.0;
+            } else {
+                us += (double)((blocks + 2 * n_sm - 1) / (2 * n_sm)) * per * (two && blocks > n_sm ? 0.57 : stage) + sums / splits + exchange;
+            }
             if (us < least_us) {
                 least_us = us;
                 best = p;
@@ -748,9 +840,12 @@ ManyPlan many_plan(int M, int rows, int k, int n_sm) {
 }
 
 int64_t many_scratch_bytes(const lb_weights4* w, int a_dtype, const void* a, int64_t lda, int M) {
-    if (a_dtype == LB_BF16 && lda % 8 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0) return 0;
+    if (a_dtype == LB_BF16 && copied_as_they_are(a, lda)) return 0;
     const int rows = w->paired ? 2 * ((w->n / 2 + 7) / 8 * 8) : w->n;
-    if (a_dtype == LB_E4M3 && spreads(many_plan(M, rows, w->k, linear4_sm_count()), w, a, lda)) return 0;
+    // (Enough for either type of result.  Of more rows than this no tile is small enough.)
+    if (a_dtype == LB_E4M3 && M <= 4 * kSpreadTokens && spreads(many_plan(M, rows, w->k, false, linear4_sm_count()), w, a, lda) &&
+        spreads(many_plan(M, rows, w->k, true, linear4_sm_count()), w, a, lda))
+        return 0;
     return (int64_t)M * ((w->k + 7) / 8) * 16;
 }
 

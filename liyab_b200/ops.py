@@ -1213,7 +1213,7 @@ for _name, _args in {
     "lb_weights4_values": [_p, _p, _l, _p],
     "lb_linear4": [_c.c_char_p],
     "lb_linear4_withhold_next": [_i],
-    "lb_linear4_plan": [_p, _i, _p],
+    "lb_linear4_plan": [_p, _i, _i, _p],
     "lb_gated4": [_c.c_char_p],
     "lb_rms_add_rows": [_c.c_char_p],
 }.items():
@@ -1308,10 +1308,10 @@ def _rows4(what: str, a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, n
     return BF16, 0, out_code, lda, ldo
 
 
-def linear4_plan(w: Weights4, m: int) -> tuple:
-    """How a product of m rows is cut: ("few", m, blocks that share a reduction, clusters), or ("tiles" or "walk", rows a tile, blocks that share a reduction, tiles)."""
+def linear4_plan(w: Weights4, m: int, out_dtype: torch.dtype = torch.bfloat16) -> tuple:
+    """How a product of m rows with results of this type is cut: ("few", m, blocks that share a reduction, clusters), or ("tiles" or "walk", rows a tile, blocks that share a reduction, tiles)."""
     plan = (_i * 4)()
-    check(lib().lb_linear4_plan(w.ref, m, plan), "linear4_plan")
+    check(lib().lb_linear4_plan(w.ref, m, _code(out_dtype, "out_dtype"), plan), "linear4_plan")
     return (("few", "tiles", "walk")[plan[0]], *plan[1:])
 
 

@@ -60,11 +60,11 @@ def test_scratch_for_rows_that_are_not_read_as_they_are():
 
 def test_how_a_product_is_cut():
     """One token to many: the kernel for few, tiles with a block each, reductions that blocks share, blocks that walk the tiles."""
-    def plan(n, k, m, paired=0):
+    def plan(n, k, m, paired=0, out=ops.BF16):
         w, ref = _weights(n, k, paired=paired)
-        out = (C.c_int * 4)()
-        assert ops.lib().lb_linear4_plan(ref, m, out) == 0
-        return tuple(out)
+        got = (C.c_int * 4)()
+        assert ops.lib().lb_linear4_plan(ref, m, out, got) == 0
+        return tuple(got)
     assert plan(1600, 1600, 1) == (0, 1, 1, 100) and plan(1600, 1600, 8)[0] == 0 and plan(1600, 1600, 9)[0] == 1
     assert plan(4096, 16384, 8)[::2] == (0, 2)                                 # activations of a whole reduction do not fit a block
     for n, k, m, paired in ((8192, 8192, 2048, 0), (7002, 200, 600, 0), (7002, 200, 600, 1)):
@@ -72,7 +72,7 @@ def test_how_a_product_is_cut():
         assert which == 2 and splits == 1 and tokens % 16 == 0 and 16 <= tokens <= 256 and tiles == -(-m // tokens) * -(-n // 128) > 148
     assert plan(512, 8192, 24)[2] > 1
     w, ref = _weights(64, 64)
-    assert ops.lib().lb_linear4_plan(ref, 0, (C.c_int * 4)()) != 0 and ops.lib().lb_linear4_plan(ref, 1, None) != 0
+    assert ops.lib().lb_linear4_plan(ref, 0, ops.BF16, (C.c_int * 4)()) != 0 and ops.lib().lb_linear4_plan(ref, 1, ops.F32, None) != 0 and ops.lib().lb_linear4_plan(ref, 1, 5, (C.c_int * 4)()) != 0
 
 
 @pytest.mark.parametrize("n,k,paired", [(64, 1, False), (1600, 1600, False), (4096, 8192, True), (512, 16384, False), (16, 90000, False), (16, 250000, False), (16, 2000000, False)])
@@ -83,9 +83,9 @@ def test_which_products_never_need_scratch(n, k, paired):
     kinds = []
     for m in range(1, 12):
         out = (C.c_int * 4)()
-        assert ops.lib().lb_linear4_plan(w.ref, m, out) == 0
-        kinds.append(out[0])
-    assert w.few == (kinds + [1]).index(1) and all(kind != 0 for kind in kinds[w.few:])
+        assert ops.lib().lb_linear4_plan(w.ref, m, ops.F32, out) == 0
+        kinds.append(out[0] != 0)
+    assert w.few == (kinds + [True]).index(True) and all(kinds[w.few:])
 
 
 def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=ops.BF16, m=0, act=0):
@@ -120,7 +120,7 @@ def test_weights_that_no_kernel_can_read_are_refused(change):
     ref = C.addressof(w)
     for m in (1, 9):
         assert _call("lb_linear4", ref, m=m, lda=1 << 27, ldo=1 << 27) == 1 and _call("lb_gated4", ref, m=m, lda=1 << 27, ldo=1 << 27) == 1
-        assert ops.lib().lb_linear4_scratch(ref, ops.BF16, 1 << 20, 1 << 27, m) == 0 and ops.lib().lb_linear4_plan(ref, m, (C.c_int * 4)()) == 1
+        assert ops.lib().lb_linear4_scratch(ref, ops.BF16, 1 << 20, 1 << 27, m) == 0 and ops.lib().lb_linear4_plan(ref, m, ops.F32, (C.c_int * 4)()) == 1
     assert ops.lib().lb_weights4_values(ref, 1 << 20, 1 << 27, None) == 1
 
 

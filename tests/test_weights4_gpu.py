@@ -198,6 +198,44 @@ def test_many_tiles(dev, m, n, k, group, eight):
         assert ((half.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
 
 
+LONG = [(9, 2048, 16384, 64), (24, 512, 9000, 32), (64, 300, 16384, 128), (100, 6400, 16384, 64), (130, 1000, 2177, 64), (300, 2048, 11456, 128), (1711, 2673, 11456, 32), (2048, 4096, 5000, 64),
+        (700, 20000, 2300, 128), (250, 136, 16300, 64), (5, 64, 300000, 128)]
+
+
+@pytest.mark.parametrize("m,n,k,group", LONG)
+@pytest.mark.parametrize("eight", [False, True])
+def test_long_reductions_keep_float32_results(dev, m, n, k, group, eight):
+    """The tensor core truncates every addition: chains of up to 2,048 values, which measure 3.4e-7 of the results (norms), a row's factors and scales a few 2^-24 and the chains' sums less: below 6e-7
+    at every length.  One chain over these lengths has 1e-6 to 5e-6."""
+    from liyab_b200 import ops
+    g = torch.Generator(device=dev).manual_seed(k)
+    q = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8, device=dev)
+    s = (torch.rand((n, -(-k // group)), generator=g, device=dev) * 448.0).to(F8)
+    r = torch.rand((n,), generator=g, device=dev) * 1e-4 + 1e-5
+    ref_w, w = _matrix(q, s, r, group), ops.lay_out_weights4(q, s, r, group)
+    a, scale = torch.randn((m, k), generator=g, device=dev), None
+    if eight:
+        a, scale = _rows8(a)
+        rows = a.double() * scale.double()[:, None]
+    else:
+        a = a.to(torch.bfloat16)
+        rows = a.double()
+    want, out, res = rows @ ref_w.T, torch.full((m, n), float("nan"), device=dev), torch.randn((m, n), generator=g, device=dev)
+    ops.linear4(a, w, None, out, m, a_scale=scale)
+    assert ops.device_status() == 0
+    assert ((out.double() - want).norm() / want.norm()).item() <= 6e-7
+    assert ((out.double() - want).abs() <= _sum_bound(k) * (rows.abs() @ ref_w.abs().T)).all()
+    again = res.clone()
+    ops.linear4(a, w, None, again, m, residual=again, a_scale=scale)
+    assert torch.equal(again, out + res)                          # the same sums, then one addition
+    f = n // 2
+    half, both = torch.empty((m, f), device=dev), rows @ ref_w[:2 * f].T
+    ops.gated4(a, ops.lay_out_weights4(q[:2 * f], s[:2 * f], r[:2 * f], group, paired=True), half, m, gate="relu", a_scale=scale)
+    assert ops.device_status() == 0
+    want = both[:, :f].clamp(min=0) * both[:, f:]
+    assert ((half.double() - want).norm() / want.norm()).item() <= 1.2e-6                             # two factors
+
+
 @pytest.mark.parametrize("m", [1, 5, 16, 40, 129])
 @pytest.mark.parametrize("activation", ["gelu_tanh", "gelu_erf", "xielu", "relu2", "none"])
 def test_activations(dev, m, activation):
