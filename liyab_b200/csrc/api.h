@@ -791,7 +791,7 @@ typedef struct {
     int act;                    /* linear4: the products' activations; gated4: lb_gate_kind 0 sigmoid, 1 silu, 2 gelu_tanh, 3 relu, 4 capped with */
     float alpha, limit;
 } lb_linear4_args;
-/* out[M, n] = act(a w^T + bias) + residual. */
+/* out[M, n] = act(a w^T + bias) + residual.  A NaN stays one under every activation and gate.  A single row may have any stride. */
 int lb_linear4(const lb_linear4_args* args);
 /* out[M, f] = gate(a w_gate^T) * (a w_up^T) for paired weights. */
 int lb_gated4(const lb_linear4_args* args);
@@ -804,7 +804,8 @@ int lb_linear4_plan(const lb_weights4* w, int M, int out_dtype, int* plan);
 int lb_linear4_withhold_next(int on);
 /* t = x + delta in 32 bits (delta may be null), total = t in x's type (may be x itself, may be null), h = t / sqrt(mean(t^2) + eps) * (gain_offset + gain) (gain may be
  * null: 1); out = h in bfloat16, or in e4m3 divided by scale[row] = max |h| / 448.  A row whose largest |h| is below 2^-117 has scale 0 and zeros; one with
- * a value that is not finite has a scale that is not finite and zeros.  Row strides are in elements. */
+ * a value that is not finite has a scale that is not finite and zeros.  Sums and products are 32-bit: a row whose mean square overflows (values beyond some 1e19) is normed to zeros, and a value
+ * whose t (gain_offset + gain) is past float32's range counts as not finite.  Rows of up to 57,344 values.  Row strides are in elements; a single row may have any. */
 typedef struct {
     const void* x;
     const void* delta;

@@ -5,9 +5,10 @@
 // the two sizes are: a warp streams its part (a kilobyte a k tile, 16 bytes a lane twice, three or four tiles on the way), makes a register of two weights of a shift, a mask and a
 // subtraction, and a group's sum of the integers, which meets its scale in 32 bits, and leaves the sum of every row tile that it touched in a slot of shared memory.
 // After one barrier the slots of a row tile (neighbouring warps) are added in order.  The blocks of a cluster share a long reduction and read one another's sums, in order.
-// Bound by the instructions that make operands of nibbles, some 190 a warp and k tile of 16 x 128 weights, at 2.9 to 3.1 a cycle and SM (4 x 50257 x 1600 11.5 us, 41 MB; 8 x 4096 x 16384
-// 14.8 us; the weights' bytes alone 6.5 and 5.4; with the products and the unpacking left out 1 x 40960 x 8192 takes 27 us, with them 34), and under some 5 us by the launch, the first weights' way and the barrier (1 x 1600 x 1600 2.9 us).  More than eight tokens
-// would cost a second product and its sums for every operand; the tensor core of linear4_many.cu is then faster (16 x 4096 x 4096 6.6 us there, 7.6 here; 8 x 8192 x 8192 16.3 there, 12.9 here).
+// Between two bounds: the weights' bytes (4 x 50257 x 1600 6.5 us of 11.5; 8 x 4096 x 16384 5.4 of 14.8) and the instructions that make operands of nibbles (165 a warp and k tile of 16 x 128 weights, 180 with
+// the ends, at 2.2 and 1.6 a cycle and SM; a form with a fifth fewer took the same time), with some 4 us of launch, first weights and barrier (1 x 1600 x 1600 3.0 us).  With the products and the unpacking left out
+// 1 x 40960 x 8192 takes 27 us, with them 34.  More than eight tokens
+// would cost a second product and its sums for every operand; the tensor core of linear4_many.cu is then faster (16 x 4096 x 4096 6.6 us there, 7.6 here; 8 x 8192 x 8192 16.3 there, 12.1 here).
 #include "linear4.h"
 #include "tcgen05.cuh"
 

@@ -8,11 +8,15 @@
 // accumulator is free again when the last columns are in registers).  Where it has fewer, sixteen warps make weights and finish; the reduction is cut between the blocks of a
 // cluster, which hand each other the sums of their share of the tokens through distributed shared memory and finish them in rank order.
 //
+// float32 results over more than 1,536 values of k are added up in several chains (many_plan says why): in accumulators of their own where tensor memory has the columns, else in two in turn, whose sums
+// warps of their own add up in shared memory under the next chain's products.  Their tiles have 160 tokens at most, which cost more weights to make a product: 2048 x 8192 x 8192 218 us with float32 results,
+// 186 with bfloat16 ones; 1024 x 4096 x 10240 84 and 62; up to some 300 tokens a few per cent.
+//
 // Roles: warp 0 copies the activations, warp 1 issues the products, warps 4 and up make weights (warp % 4 names the 32 lanes; the warps of those take k tiles in turn) and,
-// in the same warps or in sixteen further ones, finish the sums.  Handshakes and bounded waits as in the other tcgen05 products:
+// in the same warps or in further ones, finish the sums.  Handshakes and bounded waits as in the other tcgen05 products:
 //   a_full[s], b_full[s]   weights of stage s in tensor memory, activations in shared memory
 //   empty[s]               the products have read both
-//   acc_full, acc_empty    the sums of a tile are complete, are in registers
+//   acc_full, acc_empty    the sums of a tile, or of a chain, are complete, are in registers
 #include "gemm_tile.cuh"
 #include "linear4.h"
 

@@ -2,9 +2,10 @@
 // e4m3 with a scale a row.
 //
 // Bound by memory: one pass, x and delta in, the sum and the result out.  A row stays in registers as t (gain_offset + gain), up to 32 values a thread, between its sum of
-// squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor; a warp has a row of up to 1024 values (no barrier), a block a longer one (two
-// barriers).  24 instructions a value at 2.3 a cycle stay below what memory takes: 4096 bfloat16 rows of 8192 43 us, 0.85 of the measured copy bandwidth (69 with the divisions,
-// selections and comparisons of a first version).
+// squares, its largest value and its results, which 1 / sqrt and the scale meet as one factor (a value whose t (gain_offset + gain) is past float32's range counts as not finite).  From 296 rows
+// on a warp has a row of up to 512 values (no barrier); else a block has a row (one barrier).  24 instructions a value at 2.3 a cycle stay below what memory takes: 4096 bfloat16 rows of 8192
+// 44 us, 0.83 of the measured copy bandwidth (69 with the divisions, selections and comparisons of a first version).  Rows of more than 8192 values have 32 a thread, of which the 64 registers of
+// two blocks an SM spill 8 to 24 (2048 bfloat16 rows of 16384 58 us, 0.63 of the copy bandwidth).
 // Rows off the 16 bytes, and of more than 16384 values, go through shared memory, one or two values at a time and neighbours by neighbouring threads.
 #include "linear4.h"
 

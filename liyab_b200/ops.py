@@ -1222,7 +1222,8 @@ for _name, _args in {
 
 class Weights4:
     """A matrix w[n, k] = q[n, k] s[n, k / group] r[n] in 4 bits (q in -8 .. 7, s in e4m3, r float32) as the products read it.  `paired`: 2 f rows, the f of a gate
-    and the f of its other factor, for gated4.  The memory belongs to this object; made by quantise_weights4 or lay_out_weights4."""
+    and the f of its other factor, for gated4.  The memory belongs to this object; made by quantise_weights4 or lay_out_weights4, on the device that is current.  Products ask for it
+    before the kernel ahead of them has ended: a program that writes it itself synchronises before the first product."""
 
     __slots__ = ("n", "k", "group", "paired", "device", "index", "nibbles", "scales", "rows", "args", "ref", "few")
 
@@ -1324,7 +1325,7 @@ def _scratch4(w: Weights4, code: int, a: torch.Tensor, lda: int, m: int) -> Opti
 def linear4(a: torch.Tensor, w: Weights4, bias: Optional[torch.Tensor], out: torch.Tensor, m: int, activation: str = "none",
             residual: Optional[torch.Tensor] = None, a_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[:m] = act(a[:m] @ w.T + bias) + residual with 4-bit weights: a is bfloat16, or e4m3 with a_scale (a row of a times a_scale[row] is what it stands for);
-    out is bfloat16 or float32, bias and residual float32; out may be the residual."""
+    out is bfloat16 or float32, bias and residual float32; out may be the residual.  Activations: none, gelu_tanh, gelu_erf, xielu (whose two numbers stand behind the bias), relu2."""
     code, scale, out_code, lda, ldo = _rows4("linear4", a, w, out, m, w.n, a_scale)
     bias_at = residual_at = ldr = 0
     if residual is not None:
@@ -1359,7 +1360,8 @@ def gated4(a: torch.Tensor, w: Weights4, out: torch.Tensor, m: int, gate: str = 
 def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch.Tensor], eps: float, out: torch.Tensor, scale: Optional[torch.Tensor] = None,
             total: Optional[torch.Tensor] = None, gain_offset: float = 0.0) -> torch.Tensor:
     """t = x + delta (32 bits), left in `total` (x's type; None: back in x where there is a delta); out = t / sqrt(mean(t^2) + eps) * (gain_offset + gain), bfloat16, or e4m3
-    with scale (float32 [rows]): out * scale is the row, scale its largest |value| / 448.  x and delta are float32 or bfloat16."""
+    with scale (float32 [rows]): out * scale is the row, scale its largest |value| / 448.  x and delta are float32 or bfloat16, rows of up to 57,344 values; what is past float32's
+    range in t (gain_offset + gain) counts as not finite."""
     shape, index, out_type, x_type = x.shape, x.get_device(), out.dtype, x.dtype
     if len(shape) != 2 or index < 0:
         raise invalid_argument(f"rms_add: x has to be rows on a CUDA device; it is {tuple(shape)} on {x.device}")
