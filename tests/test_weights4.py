@@ -88,7 +88,7 @@ def test_which_products_never_need_scratch(n, k, paired):
     assert w.few == (kinds + [True]).index(True) and all(kinds[w.few:])
 
 
-def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=ops.BF16, m=0, act=0):
+def _call(name, ref, a=1 << 20, scale=0, bias=0, residual=0, out=1 << 20, lda=256, ldr=0, ldo=64, code=None, out_code=0, m=0, act=0):
     code = ops.BF16 if code is None else code
     return getattr(ops.lib(), name)(ops._linear4_args(ref or 0, a, scale, bias, residual, out, 0, 0, lda, ldr, ldo, code, out_code, m, act, 0.0, 0.0))
 
