@@ -822,6 +822,76 @@ typedef struct {
 } lb_rms_add_args;
 int lb_rms_add_rows(const lb_rms_add_args* args);
 
+/* ---- 4-bit cache ----
+ *
+ * Pages of keys and values x[slot, d] = n[slot, d] s[slot, d / group]: n an integer in -8 .. 7 (stored as n + 8), s a bfloat16 number; group is 32, 64 or 128 and divides
+ * head_dim (64 or 128).  Slot = page * page_size + place; page_size is a power of two, 16 or more.  The memory is [page][key/value head][page_size / 16] blocks of sixteen
+ * keys, lb_cache4_bytes(..) in all, 16-byte aligned; cache4.cuh has the order inside a block.
+ * A page number outside 0 .. n_pages - 1 in a block table stands for keys that are not there; such a slot is skipped. */
+typedef struct {
+    void* memory;
+    int n_pages, n_kv_head, head_dim, page_size, group;
+    int device;             /* the number of the device that the memory is on, plus 1: calls are refused when another is current.  0: not checked */
+} lb_cache4;
+/* The bytes of the memory of a cache of these sizes. */
+int lb_cache4_bytes(int n_pages, int n_kv_head, int head_dim, int page_size, int group, int64_t* bytes);
+/* Rounds the rows k[t], v[t] (float32 or bfloat16, n_kv_head * head_dim values, row strides ldk and ldv) to 4 bits at slot_mapping[t] (negative: skipped; the slots of a call
+ * differ): s = bfloat16(max |x| of a group / 7), n = x / s rounded to the nearest even and clamped to -8 .. 7; a group that holds an infinity or a NaN gets s = NaN. */
+int lb_append4(int dtype, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot_mapping, const lb_cache4* cache, int n_tokens, void* stream);
+/* The rows at slots[i] as float32 or bfloat16 values (negative slots: the row is left alone). */
+int lb_cache4_values(int dtype, const lb_cache4* cache, const int32_t* slots, int n, void* k, int64_t ldk, void* v, int64_t ldv, void* stream);
+/* Attention over a 4-bit cache.  Decode (q_start null): token i is request i's, its newest key at place last[i] (-1: no keys; the output row is zeros).  Portions: request s
+ * has the tokens q_start[s] .. q_start[s + 1] - 1, the first at place last[s].  A token sees the keys up to its own place under `window` (as in lb_paged_attention_generic); one that sees
+ * none has an output of zeros.  Query head h reads key/value head h / (n_head / n_kv_head).
+ * total (or null): total[r][kv head][key] = mass[r][kv head][key] + the sum, over the request's tokens and the heads of the key/value head, of the softmax weights of that key,
+ * for the keys up to the newest; r = mass_rows[s], or s.  total may be mass.  Portions of up to 64 tokens. */
+typedef struct {
+    const lb_cache4* cache;
+    const void* q;              /* bfloat16 [tokens, n_head * head_dim] */
+    const int32_t* q_start;
+    const int32_t* last;
+    const int32_t* block_table;
+    void* out;                  /* bfloat16 */
+    const float* mass;
+    float* total;
+    const int32_t* mass_rows;
+    const float* distance;      /* as for lb_paged_attention_generic_biased, or null */
+    const float* sink;          /* a number a head, or null */
+    void* scratch;              /* lb_attention4_scratch(..) bytes, 16-byte aligned (null where that is 0) */
+    void* stream;
+    int64_t q_stride, out_stride;
+    int64_t mass_stride, mass_head_stride, total_stride, total_head_stride;   /* of a row r, of a head */
+    int table_stride, n_seq, n_tokens, n_head, max_q_len;
+    int max_keys;               /* no key past this many is read */
+    int n_mass;                 /* rows r of mass and of total */
+    int window;
+    float scale, soft_cap;
+} lb_attention4_args;
+int lb_attention4(const lb_attention4_args* args);
+int64_t lb_attention4_scratch(const lb_attention4_args* args);
+/* How a call is cut: plan[0] 0 by the kernel for few rows, 1 by the one for many; plan[1] query rows a block; plan[2] blocks that share a request's keys; plan[3] warps a block. */
+int lb_attention4_plan(const lb_attention4_args* args, int* plan);
+/* Eviction: of request s's n_keys[s] keys, key/value head h keeps the `recent` newest and, of the others, those with the largest mass[s][h][key] (equal ones: the lowest
+ * places; a NaN counts as the largest), `keep` in all, or all where there are no more.  They are copied, in their order, to the places 0, 1, .. of the pages that
+ * dest_table[s] names (pages that no source table of the call names), kept[s][h][i] is the place that the i-th came from (-1 past the last) and
+ * dest_mass[s][h][i] its mass (0 past the last), i < keep.  mass and dest_mass have rows r = mass_rows[s], or s. */
+typedef struct {
+    const lb_cache4* cache;
+    const float* mass;
+    const int32_t* mass_rows;
+    const int32_t* block_table;
+    const int32_t* n_keys;
+    const int32_t* dest_table;
+    int32_t* kept;              /* [n_seq, n_kv_head, keep] */
+    float* dest_mass;           /* or null */
+    void* stream;
+    int64_t mass_stride, mass_head_stride, dest_stride, dest_head_stride;
+    int table_stride, dest_table_stride, n_seq, keep, recent;
+    int max_keys;               /* no key past this many is read */
+    int n_mass, n_dest_mass;
+} lb_evict4_args;
+int lb_evict4(const lb_evict4_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,151 @@
+// Attention over a 4-bit cache: the checks of a call, the choice of the kernel, and what each key gained in weight.
+#include "attention4.h"
+#include "linear4.h"
+
+#include <algorithm>
+
+namespace {
+
+using namespace lb_a4;
+
+struct Mass {
+    const float* mass;
+    float* total;
+    const int32_t* rows;
+    int64_t mass_stride, mass_head_stride, total_stride, total_head_stride;
+    int n_mass;
+};
+
+// total = mass + the sum over a request's rows of 2^(score - log_sum), a thread a key.  The rows come in their order, so the sum does not depend on the launch.
+__global__ void __launch_bounds__(256)
+attention4_mass_kernel(const Call c, const Mass w) {
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    const int seq = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+    const Portion part = portion_of(c, seq);
+    const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1, newest = min(part.place + part.count - 1, limit);
+    if (part.count <= 0 || key > newest) return;
+    const int r = w.rows != nullptr ? w.rows[seq] : seq;
+    if ((unsigned)r >= (unsigned)w.n_mass) return;
+    const int64_t unit = ((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows;
+    const float* scores = c.scores + unit * c.score_keys + key;
+    const float* log_sums = c.log_sums + unit;
+    float sum = 0.0f;
+    for (int token = 0; token < part.count; ++token) {
+        const int place = min(part.place + token, limit);
+        if (key > place || key < lb_first_visible(max(place, 0), c.window)) continue;
+        for (int h = 0; h < c.per; ++h) {
+            const int row = token * c.per + h;
+            sum += exp2f(scores[(int64_t)row * c.score_keys] - log_sums[row]);
+        }
+    }
+    const int64_t at = (int64_t)r * w.mass_stride + (int64_t)kvh * w.mass_head_stride + key;
+    w.total[(int64_t)r * w.total_stride + (int64_t)kvh * w.total_head_stride + key] = w.mass[at] + sum;
+}
+
+constexpr int kMostMassTokens = 64;
+
+struct Scratch {
+    int64_t scores, log_sums, partial, bytes;       // offsets
+};
+Scratch scratch_of(const lb_attention4_args& a, const RowsPlan& p, int max_rows, int score_keys) {
+    auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+    Scratch s = {};
+    const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
+    if (a.total != nullptr) {
+        s.log_sums = up(units * max_rows * score_keys * 4);
+        s.bytes = s.log_sums + up(units * max_rows * 4);
+    }
+    s.partial = s.bytes;
+    if (p.splits > 1 && !p.cluster) s.bytes += up(units * p.tiles * p.splits * p.rows * (a.cache->head_dim + 2) * 4);
+    return s;
+}
+
+int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch) {
+    LB_CHECK_ARG(args != nullptr, "attention4: no arguments");
+    const lb_attention4_args& a = *args;
+    if (int rc = lb_c4::pages_of(a.cache, "attention4", &c->pages)) return rc;
+    LB_CHECK_ARG(a.n_head > 0 && a.n_head % a.cache->n_kv_head == 0, "attention4: %d heads over %d key/value heads", a.n_head, a.cache->n_kv_head);
+    LB_CHECK_ARG(a.n_seq >= 0 && a.n_seq <= 65535 && a.n_tokens >= 0, "attention4: %d requests (up to 65535), %d tokens", a.n_seq, a.n_tokens);
+    LB_CHECK_ARG(a.q_start != nullptr || a.n_tokens >= a.n_seq, "attention4: %d requests, %d tokens", a.n_seq, a.n_tokens);
+    LB_CHECK_ARG(a.max_q_len > 0 && (a.q_start != nullptr || a.max_q_len == 1), "attention4: portions of up to %d tokens", a.max_q_len);
+    LB_CHECK_ARG(a.max_keys > 0 && a.table_stride > 0 && (int64_t)a.table_stride * a.cache->page_size <= INT32_MAX, "attention4: up to %d keys, tables of %d pages", a.max_keys,
+                 a.table_stride);
+    const int64_t rows = (int64_t)a.max_q_len * (a.n_head / a.cache->n_kv_head);
+    LB_CHECK_ARG(rows <= 1 << 22 && (rows + 7) / 8 * a.cache->n_kv_head <= 65535, "attention4: %d tokens of %d heads are more than one launch takes", a.max_q_len, a.n_head);
+    LB_CHECK_ARG(a.total == nullptr || (a.mass != nullptr && a.max_q_len <= kMostMassTokens), "attention4: the keys' weights come from portions of up to %d tokens", kMostMassTokens);
+    LB_CHECK_ARG(a.total == nullptr || (a.n_mass >= 0 && a.mass_stride >= 0 && a.mass_head_stride >= 0 && a.total_stride >= 0 && a.total_head_stride >= 0),
+                 "attention4: weights of no size");
+    const int score_keys = std::min(a.max_keys, a.table_stride * a.cache->page_size);
+    c->q = static_cast<const __nv_bfloat16*>(a.q);
+    c->q_start = a.q_start;
+    c->last = a.last;
+    c->table = a.block_table;
+    c->out = static_cast<__nv_bfloat16*>(a.out);
+    c->distance = a.distance;
+    c->sink = a.sink;
+    c->q_stride = a.q_stride;
+    c->out_stride = a.out_stride;
+    c->table_stride = a.table_stride;
+    c->n_seq = a.n_seq;
+    c->n_tokens = a.n_tokens;
+    c->n_head = a.n_head;
+    c->per = a.n_head / a.cache->n_kv_head;
+    c->max_rows = (int)rows;
+    c->score_keys = score_keys;
+    c->max_keys = a.max_keys;
+    c->window = a.window;
+    c->scale = a.scale;
+    c->soft_cap = a.soft_cap;
+    *p = rows_plan(std::max(1, a.n_seq), a.cache->n_kv_head, (int)rows, score_keys, a.cache->head_dim, linear4_sm_count());
+    *scratch = scratch_of(a, *p, (int)rows, score_keys);
+    uint8_t* at = static_cast<uint8_t*>(a.scratch);
+    c->scores = a.total != nullptr ? reinterpret_cast<float*>(at) : nullptr;
+    c->log_sums = a.total != nullptr ? reinterpret_cast<float*>(at + scratch->log_sums) : nullptr;
+    c->partial = reinterpret_cast<float*>(at + scratch->partial);
+    return LB_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t lb_attention4_scratch(const lb_attention4_args* args) {
+    Call c;
+    RowsPlan p;
+    Scratch s;
+    return check(args, &c, &p, &s) == LB_OK ? s.bytes : 0;
+}
+
+extern "C" int lb_attention4_plan(const lb_attention4_args* args, int* plan) {
+    Call c;
+    RowsPlan p;
+    Scratch s;
+    LB_CHECK_ARG(plan != nullptr, "attention4: no place for the plan");
+    if (int rc = check(args, &c, &p, &s)) return rc;
+    plan[0] = 0;
+    plan[1] = p.rows;
+    plan[2] = p.splits;
+    plan[3] = p.warps;
+    return LB_OK;
+}
+
+extern "C" int lb_attention4(const lb_attention4_args* args) {
+    Call c;
+    RowsPlan p;
+    Scratch s;
+    if (int rc = check(args, &c, &p, &s)) return rc;
+    const lb_attention4_args& a = *args;
+    if (a.n_seq == 0 || a.n_tokens == 0) return LB_OK;
+    LB_CHECK_ARG(a.q != nullptr && a.last != nullptr && a.block_table != nullptr && a.out != nullptr, "attention4: a pointer is missing");
+    LB_CHECK_ARG(reinterpret_cast<uintptr_t>(a.q) % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % 2 == 0, "attention4: pointers off their type's alignment");
+    const int64_t width = (int64_t)a.n_head * a.cache->head_dim;
+    LB_CHECK_ARG(a.n_tokens < 2 || (a.q_stride >= width && a.out_stride >= width), "attention4: rows overlap");
+    LB_CHECK_ARG(s.bytes == 0 || (a.scratch != nullptr && reinterpret_cast<uintptr_t>(a.scratch) % 16 == 0), "attention4: scratch memory is missing or not 16-byte aligned");
+    if (int rc = device_check("attention4", a.cache->device)) return rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
+    if (int rc = few_rows(c, a.cache->head_dim, p, stream)) return rc;
+    if (a.total != nullptr) {
+        const Mass w = {a.mass, a.total, a.mass_rows, a.mass_stride, a.mass_head_stride, a.total_stride, a.total_head_stride, a.n_mass};
+        LB_CHECK_CUDA(lb_launch_overlapped(attention4_mass_kernel, dim3((c.score_keys + 255) / 256, a.cache->n_kv_head, a.n_seq), dim3(256), 0, stream, c, w));
+    }
+    return LB_OK;
+}

@@ -1,0 +1,51 @@
+// What the kernels behind lb_attention4 share.
+#pragma once
+
+#include "cache4.cuh"
+
+namespace lb_a4 {
+
+// A call, checked (host) and as the kernels get it.
+struct Call {
+    lb_c4::Pages pages;
+    const __nv_bfloat16* q;
+    const int32_t* q_start;
+    const int32_t* last;
+    const int32_t* table;
+    __nv_bfloat16* out;
+    const float* distance;
+    const float* sink;
+    float* scores;                  // [request][key/value head][row][score_keys]: scores (base 2) for the keys' weights, or null
+    float* log_sums;                // [request][key/value head][row]: base-2 logarithm of the softmax's divisor, or null
+    float* partial;                 // [request][key/value head][row tile][range][row][maximum, sum, values] where ranges meet in memory
+    int64_t q_stride, out_stride;
+    int table_stride, n_seq, n_tokens, n_head, per, max_rows, score_keys, max_keys, window;
+    float scale, soft_cap;
+};
+
+// The tokens of request s, [first, first + count), and the place of its first: decode calls have a token a request.
+struct Portion {
+    int first, count, place;
+};
+__device__ __forceinline__ Portion portion_of(const Call& c, int s) {
+    Portion p;
+    if (c.q_start == nullptr) {
+        p.first = s;
+        p.count = 1;
+    } else {
+        p.first = max(c.q_start[s], 0);
+        p.count = min(min(c.q_start[s + 1], c.n_tokens) - p.first, c.max_rows / c.per);       // no more than the call names
+    }
+    p.place = c.last[s];
+    return p;
+}
+
+// How the kernel for few rows cuts a call: rows a block (8 or 16), row tiles a request and key/value head, ranges of the keys, whether the ranges' blocks are one cluster
+// (else their states meet in memory), warps a block.
+struct RowsPlan {
+    int rows, tiles, splits, cluster, warps;
+};
+RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t stream);
+
+}  // namespace lb_a4

@@ -270,6 +270,9 @@ extern "C" int lb_struct_bytes(int which) {
         case 4: return (int)sizeof(lb_linear4_args);
         case 5: return (int)sizeof(lb_rms_add_args);
         case 6: return (int)sizeof(lb_weights4);
+        case 7: return (int)sizeof(lb_attention4_args);
+        case 8: return (int)sizeof(lb_evict4_args);
+        case 9: return (int)sizeof(lb_cache4);
         default: return 0;
     }
 }

@@ -95,6 +95,7 @@ def lib():
         l = load_library()
         l.lb_last_error.restype = _c.c_char_p
         l.lb_linear4_scratch.argtypes, l.lb_linear4_scratch.restype = [_p, _i, _p, _l, _i], _l
+        l.lb_attention4_scratch.argtypes, l.lb_attention4_scratch.restype = [_c.c_char_p], _l
         for name, args in _SIGNATURES.items():
             fn = getattr(l, name)
             fn.argtypes = args
@@ -1399,3 +1400,182 @@ def rms_add(x: torch.Tensor, delta: Optional[torch.Tensor], gain: Optional[torch
     check(lib().lb_rms_add_rows(_rms_add_args(x.data_ptr(), delta_at, total_at, gain_at, out.data_ptr(), scale_at, stream_of(index), ldx, ldd, ldt, ldo,
                                               _code(x_type, "x"), delta_code, code, rows, width, index + 1, gain_offset, eps)), "rms_add")
     return out
+
+
+# ------------------------------------------------------------------ a cache in 4 bits
+
+# lb_attention4_args and lb_evict4_args.
+_attention4_args = struct.Struct("@13P6q8i2f0P").pack
+_evict4_args = struct.Struct("@9P4q8i0P").pack
+
+
+class Cache4Args(ctypes.Structure):
+    _fields_ = [("memory", _p), ("n_pages", _i), ("n_kv_head", _i), ("head_dim", _i), ("page_size", _i), ("group", _i), ("device", _i)]
+
+
+for _name, _args in {
+    "lb_cache4_bytes": [_i, _i, _i, _i, _i, _p],
+    "lb_append4": [_i, _p, _l, _p, _l, _p, _p, _i, _p],
+    "lb_cache4_values": [_i, _p, _p, _i, _p, _l, _p, _l, _p],
+    "lb_attention4": [_c.c_char_p],
+    "lb_attention4_plan": [_c.c_char_p, _p],
+    "lb_evict4": [_c.c_char_p],
+}.items():
+    _SIGNATURES[_name] = _args
+
+
+class Cache4:
+    """Pages of keys and values in 4 bits: x[slot, d] = n s[d / group], n in -8 .. 7, s bfloat16, a slot being page * page_size + place.  Heads of 64 or 128 values, groups of 32, 64 or
+    128, pages of a power of two keys, 16 or more.  The memory belongs to this object; what no append4 or evict4 has written is undefined, and no attention reads it."""
+
+    __slots__ = ("n_pages", "n_kv_head", "head_dim", "page_size", "group", "device", "index", "memory", "args", "ref")
+
+    def __init__(self, n_pages: int, n_kv_head: int, head_dim: int, page_size: int = 16, group: int = 64, device="cuda"):
+        size = ctypes.c_int64(0)
+        check(lib().lb_cache4_bytes(n_pages, n_kv_head, head_dim, page_size, group, ctypes.byref(size)), "cache4")
+        self.n_pages, self.n_kv_head, self.head_dim, self.page_size, self.group = n_pages, n_kv_head, head_dim, page_size, group
+        self.memory = torch.empty(size.value, dtype=torch.uint8, device=device)
+        if not self.memory.is_cuda:
+            raise invalid_argument(f"cache4: the cache is on {self.memory.device}; the engine's kernels run on a CUDA device only")
+        self.device, self.index = self.memory.device, self.memory.get_device()
+        self.args = Cache4Args(self.memory.data_ptr(), n_pages, n_kv_head, head_dim, page_size, group, self.index + 1)
+        self.ref = ctypes.addressof(self.args)
+
+    @property
+    def nbytes(self) -> int:
+        return self.memory.numel()
+
+
+def _rows_of4(what: str, cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, n: int) -> int:
+    """What append4 and cache4_values check of their rows; their type."""
+    width = cache.n_kv_head * cache.head_dim
+    code = _DT.get(k.dtype, -1)
+    if code < 0 or v.dtype is not k.dtype:
+        raise invalid_argument(f"{what}: keys and values are both float32 or both bfloat16, not {k.dtype} and {v.dtype}")
+    if k.dim() != 2 or v.dim() != 2 or k.shape[1] != width or v.shape[1] != width or k.stride(1) != 1 or v.stride(1) != 1 or not 0 <= n <= min(k.shape[0], v.shape[0]):
+        raise invalid_argument(f"{what}: {n} rows of {width} values, dense within a row, from {tuple(k.shape)} and {tuple(v.shape)}")
+    if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.shape[0] < n:
+        raise invalid_argument(f"{what}: the slots are int32, one a row")
+    if k.get_device() != cache.index or v.get_device() != cache.index or slots.get_device() != cache.index:
+        raise invalid_argument(f"{what}: keys are on {k.device}, values on {v.device} and slots on {slots.device}, the cache on {cache.device}")
+    return code
+
+
+def append4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, cache: Cache4, n_tokens: int) -> None:
+    """Rounds the step's key and value rows ([tokens, n_kv_head * head_dim], float32 or bfloat16, any row strides) into the cache's slots (int32, negative: skipped; no slot twice in a call):
+    a group's scale is its largest |x| / 7 in bfloat16, each value the nearest multiple of it.  A group that is not finite reads back as NaN."""
+    code = _rows_of4("append4", cache, k, v, slot_mapping, n_tokens)
+    check(lib().lb_append4(code, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot_mapping.data_ptr(), cache.ref, n_tokens, stream_of(cache.index)), "append4")
+
+
+def cache4_values(cache: Cache4, slots: torch.Tensor, n: int, k: torch.Tensor, v: torch.Tensor) -> tuple:
+    """The first n slots' keys and values as rows of float32 or bfloat16 (rows of negative slots are left as they were); (k, v)."""
+    code = _rows_of4("cache4_values", cache, k, v, slots, n)
+    check(lib().lb_cache4_values(code, cache.ref, slots.data_ptr(), n, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), stream_of(cache.index)), "cache4_values")
+    return k, v
+
+
+def _ints4(what: str, name: str, t: torch.Tensor, index: int, shape: tuple) -> int:
+    """An int32 tensor of at least this shape, dense within a row."""
+    if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != len(shape) or any(a < b for a, b in zip(t.shape, shape)) or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise invalid_argument(f"{what}: {name} has to be int32 of at least {shape}, dense within a row, on the cache's device; it is {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _weights_of4(what: str, name: str, t: torch.Tensor, cache: Cache4, keys: int) -> int:
+    """Accumulated weights [rows, n_kv_head, keys], dense within a row."""
+    if (t.dtype is not torch.float32 or t.get_device() != cache.index or t.dim() != 3 or t.shape[1] != cache.n_kv_head or t.shape[2] < keys or (t.stride(2) != 1 and t.shape[2] > 1)):
+        raise invalid_argument(f"{what}: {name} has to be float32 [rows, {cache.n_kv_head}, at least {keys}], dense within a row, on the cache's device; it is {t.dtype} {tuple(t.shape)} "
+                               f"on {t.device}")
+    return t.data_ptr()
+
+
+def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[torch.Tensor], last: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, n_seq: int,
+                max_q_len: int, n_head: int, scale: float, window: int, mass: Optional[torch.Tensor], total: Optional[torch.Tensor], mass_rows: Optional[torch.Tensor],
+                distance: Optional[torch.Tensor], sink: Optional[torch.Tensor], soft_cap: float, max_keys: int, plan=None):
+    index, width = cache.index, n_head * cache.head_dim
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or q.get_device() != index or out.get_device() != index:
+        raise invalid_argument(f"{what}: q and out are bfloat16 on the cache's device; they are {q.dtype} on {q.device} and {out.dtype} on {out.device}")
+    if q.dim() != 2 or out.dim() != 2 or q.shape[1] != width or out.shape[1] != width or out.shape[0] < q.shape[0] or q.stride(1) != 1 or out.stride(1) != 1:
+        raise invalid_argument(f"{what}: q and out are rows of {width} values, dense within a row; they are {tuple(q.shape)} and {tuple(out.shape)}")
+    last_at = _ints4(what, "positions" if q_start is None else "n_past", last, index, (n_seq,))
+    table_at = _ints4(what, "block_table", block_table, index, (n_seq, 1))
+    start_at = 0 if q_start is None else _ints4(what, "q_start", q_start, index, (n_seq + 1,))
+    keys = min(max_keys, block_table.shape[1] * cache.page_size) if max_keys > 0 else block_table.shape[1] * cache.page_size
+    mass_at = total_at = rows_at = n_mass = 0
+    strides = (0, 0, 0, 0)
+    if mass is not None:
+        total = mass if total is None else total
+        mass_at, total_at = _weights_of4(what, "mass", mass, cache, keys), _weights_of4(what, "total", total, cache, keys)
+        n_mass = min(mass.shape[0], total.shape[0])
+        strides = (mass.stride(0), mass.stride(1), total.stride(0), total.stride(1))
+        if mass_rows is not None:
+            rows_at = _ints4(what, "mass_rows", mass_rows, index, (n_seq,))
+        elif n_mass < n_seq:
+            raise invalid_argument(f"{what}: {n_seq} requests, weights of {n_mass}")
+    elif total is not None or mass_rows is not None:
+        raise invalid_argument(f"{what}: total and mass_rows come with mass")
+    for name, t, n in (("distance", distance, 2 * n_head), ("sink", sink, n_head)):
+        if t is not None and (t.dtype is not torch.float32 or t.get_device() != index or t.numel() != n or not t.is_contiguous()):
+            raise invalid_argument(f"{what}: {name} has to be {n} float32 numbers on the cache's device")
+    parts = (cache.ref, q.data_ptr(), start_at, last_at, table_at, out.data_ptr(), mass_at, total_at, rows_at, 0 if distance is None else distance.data_ptr(),
+             0 if sink is None else sink.data_ptr())
+    rest = (stream_of(index), q.stride(0), out.stride(0), *strides, block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], n_seq, q.shape[0], n_head, max_q_len, keys, n_mass,
+            window, scale, soft_cap)
+    packed = _attention4_args(*parts, 0, *rest)
+    l = lib()
+    if plan is not None:
+        return check(l.lb_attention4_plan(packed, plan), what)
+    size = l.lb_attention4_scratch(packed)
+    if size:
+        scratch = torch.empty(size, dtype=torch.uint8, device=cache.device)
+        packed = _attention4_args(*parts, scratch.data_ptr(), *rest)
+    check(l.lb_attention4(packed), what)
+    return out
+
+
+def decode_attention4(q: torch.Tensor, cache: Cache4, positions: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, n_seq: int, n_head: int, scale: float, window: int = 0,
+                      mass: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None, distance: Optional[torch.Tensor] = None,
+                      sink: Optional[torch.Tensor] = None, soft_cap: float = 0.0, max_keys: int = 0) -> torch.Tensor:
+    """Attention of one new token per request (row i of q is request i's, its newest key at positions[i]; -1: no keys, a row of zeros) over the pages of a 4-bit cache.  `window`,
+    `distance`, `sink`, `soft_cap`: as for paged_attention_generic.  `max_keys`: the most keys a request has (0: what the block table holds); none past it is read.
+    `mass` (float32 [rows, n_kv_head, keys]): total[r, h, key] = mass[r, h, key] + the softmax weights that the key got from the query heads of h, for the keys up to the newest; r is
+    the request's number or mass_rows[request] (no row twice in a call); `total` None: back into mass."""
+    if q.dim() == 2 and not 0 <= n_seq <= q.shape[0]:
+        raise invalid_argument(f"decode_attention4: {n_seq} requests, {q.shape[0]} rows of q")
+    return _attention4("decode_attention4", q, cache, None, positions, block_table, out, n_seq, 1, n_head, scale, window, mass, total, mass_rows, distance, sink, soft_cap, max_keys)
+
+
+def prefill_attention4(q: torch.Tensor, cache: Cache4, q_start: torch.Tensor, n_past: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, n_seq: int, max_q_len: int, n_head: int,
+                       scale: float, window: int = 0, mass: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None,
+                       distance: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None, soft_cap: float = 0.0, max_keys: int = 0) -> torch.Tensor:
+    """Causal attention of portions of up to `max_q_len` tokens per request over the pages of a 4-bit cache, which holds the portions' own keys already: request s has the rows
+    q_start[s] .. q_start[s + 1] - 1 of q, the first at place n_past[s].  The other arguments as for decode_attention4; with `mass` portions of up to 64 tokens (the weights of all of
+    a portion's tokens are added up)."""
+    return _attention4("prefill_attention4", q, cache, q_start, n_past, block_table, out, n_seq, max_q_len, n_head, scale, window, mass, total, mass_rows, distance, sink, soft_cap, max_keys)
+
+
+def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys: torch.Tensor, n_seq: int, keep: int, recent: int, dest_table: torch.Tensor, kept: torch.Tensor,
+           dest_mass: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Leaves each request and key/value head `keep` of its n_keys[s] keys: the `recent` newest and, of the others, those with the largest `mass` (as decode_attention4 adds it up; equal ones:
+    the lowest places).  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
+    they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (memory of its own, not mass)."""
+    index, page = cache.index, cache.page_size
+    table_at, dest_at = _ints4("evict4", "block_table", block_table, index, (n_seq, 1)), _ints4("evict4", "dest_table", dest_table, index, (n_seq, -(-keep // page)))
+    keys = min(block_table.shape[1] * page, mass.shape[2] if mass.dim() == 3 else 0)
+    mass_at, n_keys_at = _weights_of4("evict4", "mass", mass, cache, 1), _ints4("evict4", "n_keys", n_keys, index, (n_seq,))
+    kept_at = _ints4("evict4", "kept", kept, index, (n_seq, cache.n_kv_head, keep))
+    if tuple(kept.shape[1:]) != (cache.n_kv_head, keep) or not kept.is_contiguous():
+        raise invalid_argument(f"evict4: kept has to be contiguous [requests, {cache.n_kv_head}, {keep}]; it is {tuple(kept.shape)}")
+    rows_at = dest_mass_at = n_dest = 0
+    strides = (0, 0)
+    if dest_mass is not None:
+        dest_mass_at, n_dest, strides = _weights_of4("evict4", "dest_mass", dest_mass, cache, keep), dest_mass.shape[0], (dest_mass.stride(0), dest_mass.stride(1))
+    if mass_rows is not None:
+        rows_at = _ints4("evict4", "mass_rows", mass_rows, index, (n_seq,))
+    elif mass.shape[0] < n_seq or (dest_mass is not None and n_dest < n_seq):
+        raise invalid_argument(f"evict4: {n_seq} requests, weights of {mass.shape[0]}{'' if dest_mass is None else f' and {n_dest}'}")
+    check(lib().lb_evict4(_evict4_args(cache.ref, mass_at, rows_at, table_at, n_keys_at, dest_at, kept_at, dest_mass_at, stream_of(index), mass.stride(0), mass.stride(1), *strides,
+                                       block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], dest_table.stride(0) if dest_table.shape[0] > 1 else dest_table.shape[1],
+                                       n_seq, keep, recent, keys, mass.shape[0], n_dest)), "evict4")
+    return kept
