@@ -46,7 +46,7 @@ attention4_mass_kernel(const Call c, const Mass w) {
 constexpr int kMostMassTokens = 64;
 
 struct Scratch {
-    int64_t scores, log_sums, partial, bytes;       // offsets
+    int64_t scores, log_sums, partial, starts, bytes;       // offsets
 };
 Scratch scratch_of(const lb_attention4_args& a, const RowsPlan& p, int max_rows, int score_keys) {
     auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
@@ -57,7 +57,8 @@ Scratch scratch_of(const lb_attention4_args& a, const RowsPlan& p, int max_rows,
         s.bytes = s.log_sums + up(units * max_rows * 4);
     }
     s.partial = s.bytes;
-    if (p.splits > 1 && !p.cluster) s.bytes += up(units * p.tiles * p.splits * p.rows * (a.cache->head_dim + 2) * 4);
+    s.starts = s.partial + up(p.states);
+    s.bytes = s.starts + up(p.starts);
     return s;
 }
 
@@ -97,12 +98,13 @@ int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch
     c->window = a.window;
     c->scale = a.scale;
     c->soft_cap = a.soft_cap;
-    *p = rows_plan(std::max(1, a.n_seq), a.cache->n_kv_head, (int)rows, score_keys, a.cache->head_dim, linear4_sm_count());
+    if (int rc = rows_plan(p, a.n_seq, a.cache->n_kv_head, (int)rows, score_keys, a.cache->head_dim, linear4_sm_count())) return rc;
     *scratch = scratch_of(a, *p, (int)rows, score_keys);
     uint8_t* at = static_cast<uint8_t*>(a.scratch);
     c->scores = a.total != nullptr ? reinterpret_cast<float*>(at) : nullptr;
     c->log_sums = a.total != nullptr ? reinterpret_cast<float*>(at + scratch->log_sums) : nullptr;
     c->partial = reinterpret_cast<float*>(at + scratch->partial);
+    c->starts = reinterpret_cast<int*>(at + scratch->starts);
     return LB_OK;
 }
 
@@ -123,8 +125,8 @@ extern "C" int lb_attention4_plan(const lb_attention4_args* args, int* plan) {
     if (int rc = check(args, &c, &p, &s)) return rc;
     plan[0] = 0;
     plan[1] = p.rows;
-    plan[2] = p.splits;
-    plan[3] = p.warps;
+    plan[2] = p.blocks;
+    plan[3] = p.per_row;
     return LB_OK;
 }
 

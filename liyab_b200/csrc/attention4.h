@@ -17,7 +17,8 @@ struct Call {
     const float* sink;
     float* scores;                  // [request][key/value head][row][score_keys]: scores (base 2) for the keys' weights, or null
     float* log_sums;                // [request][key/value head][row]: base-2 logarithm of the softmax's divisor, or null
-    float* partial;                 // [request][key/value head][row tile][range][row][maximum, sum, values] where ranges meet in memory
+    float* partial;                 // states of runs: [launch row][warp + unit][row][reference, sum, values]
+    int* starts;                    // [launch row][request + 1]: where a request's tiles start in the row's order
     int64_t q_stride, out_stride;
     int table_stride, n_seq, n_tokens, n_head, per, max_rows, score_keys, max_keys, window;
     float scale, soft_cap;
@@ -40,12 +41,13 @@ __device__ __forceinline__ Portion portion_of(const Call& c, int s) {
     return p;
 }
 
-// How the kernel for few rows cuts a call: rows a block (8 or 16), row tiles a request and key/value head, ranges of the keys, whether the ranges' blocks are one cluster
-// (else their states meet in memory), warps a block.
+// How the kernel for few rows cuts a call: rows a tile (8 or 16), row tiles a request and key/value head, requests a launch row, blocks of a row, groups of threads that join a row's
+// states, bytes of the states and of the requests' starts.
 struct RowsPlan {
-    int rows, tiles, splits, cluster, warps;
+    int rows, tiles, per_row, blocks, join_groups;
+    int64_t states, starts;
 };
-RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t stream);
 
 }  // namespace lb_a4

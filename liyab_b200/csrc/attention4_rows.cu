@@ -56,6 +56,19 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Sums of products of bytes, n + 8 by a query's digit.  kMagicBits: the bits of 1.5 2^23, after which integers up to 2^22 either way are the bits of that number plus themselves.
+constexpr int kMagicBits = 0x4b400000;
+constexpr float kMagic = 12582912.0f;
+__device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, int c0, int c1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
+}
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t turned(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -80,494 +93,532 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
 // bfloat16 number i of a run of words.
 __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
 
-template <int HD, int NT, int W>
-struct Shared {
-    static constexpr int kRows = 8 * NT, kState = HD + 2;
-    // The warps' rings; at the end the same bytes hold [warp][row][values], then the block's own state.
-    __host__ __device__ static constexpr int rings(int block) { return W * kStages * block; }
-    static constexpr int kStates = (int)sizeof(float) * (W * kRows * kState + kRows * kState);
-    __host__ __device__ static constexpr int bytes(int block) { return rings(block) > kStates ? rings(block) : kStates; }
-};
+constexpr int kWarps = 4;                      // a block's; they share nothing but the list of requests
+constexpr int kMostRequests = 1024;            // of a launch row (grid.y)
+constexpr int kLeastTiles = 4;                 // of a warp
 
-// NG groups of scales a head, NT tiles of 8 query rows, W warps.  PLAIN: no soft cap, no penalty by distance, no scores written.
-template <int HD, int NG, int NT, int W, bool PLAIN>
-__global__ void __launch_bounds__(W * 32, NT == 1 ? 16 / W : 8 / W)
-attention4_rows_kernel(const Call c, int n_splits, int cluster, int tiles, int* status) {
+// Blocks an SM.
+__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return nt == 1 ? (hd == 64 ? 5 : 4) : nt == 2 ? (hd == 64 ? 4 : 3) : 2; }
+
+// The blocks of keys of a request that any of its rows sees: the first and how many.
+__device__ __forceinline__ void tiles_of(const Call& c, const Portion& p, int* first, int* count) {
+    const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;
+    const int lo = min(p.place, limit), hi = p.count > 0 ? min(p.place + p.count - 1, limit) : -1;
+    *first = lo < 0 ? 0 : lb_first_visible(lo, c.window) / kBlockKeys;
+    *count = hi < 0 ? 0 : hi / kBlockKeys + 1 - *first;
+}
+
+// How many tiles a warp takes, of `total` in its launch row.
+__host__ __device__ __forceinline__ int share_of(int total, int n_warps) {
+    const int even = (total + n_warps - 1) / n_warps;
+    return even > kLeastTiles ? even : kLeastTiles;
+}
+
+// NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.
+template <int HD, int NG, int NT, bool PLAIN>
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD, NT))
+attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
-    using S = Shared<HD, NT, W>;
-    constexpr int kRows = S::kRows, kState = S::kState, kThreads = W * 32;
+    constexpr int kRows = 4 * NT, kState = HD + 2;
     constexpr int JK = HD / 32, JV = HD / 64;             // words of a lane: of a key, of a value row
     constexpr int kBlock = block_bytes(HD, NG);
+    // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
+    constexpr int VT = NT == 1 ? 1 : NT / 2, VG = NT == 1 ? (NG + 1) / 2 : NG;
+    // The warps' rings, then the list of requests: where their tiles start in the row's order, and in their keys.
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[W][kStages];
-    __shared__ float factor[W][kRows];
-    __shared__ float block_m[kRows], block_l[kRows];
+    __shared__ uint64_t bars[kWarps][kStages];
+    __shared__ int found[kWarps][64];                      // the cache's blocks of the tiles to come; -1: on no page
+    int* starts = reinterpret_cast<int*>(smem + kWarps * kStages * kBlock);
+    int* firsts = starts + per_row + 1;
 
-    const int split = blockIdx.x, seq = blockIdx.z, kvh = blockIdx.y / tiles, row_tile = blockIdx.y - kvh * tiles;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int seq0 = blockIdx.y * per_row, n_seq = min(per_row, c.n_seq - seq0), kv = c.pages.n_kv_head;
     if (lane < kStages) lb_tc::mbar_init(&bars[warp][lane], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-
-    const Portion part = portion_of(c, seq);
-    const int n_rows = part.count * c.per, row0 = row_tile * kRows;
-    if (row0 >= n_rows) return;                            // the same for all blocks of a cluster
-    const int rows_here = min(kRows, n_rows - row0);
-    const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;          // no key past this place is read
-    auto place_of = [&](int row) { return min(part.place + min(row, n_rows - 1) / c.per, limit); };
-    const int p_lo = place_of(row0), p_hi = place_of(row0 + rows_here - 1);
-    const int first_lo = p_lo < 0 ? 0 : lb_first_visible(p_lo, c.window), first_hi = p_hi < 0 ? 0 : lb_first_visible(p_hi, c.window);
-    // The range's blocks of keys: all that any row sees, in equal parts.
-    const int tile_lo = first_lo / kBlockKeys, all_tiles = p_hi >= 0 ? p_hi / kBlockKeys + 1 - tile_lo : 0;
-    const int share = (all_tiles + n_splits - 1) / n_splits;
-    const int tile0 = tile_lo + split * share, n_tiles = max(0, min(share, all_tiles - split * share));
-    const int my_tiles = n_tiles > warp ? (n_tiles - warp + W - 1) / W : 0;
-    const int32_t* table = c.table + (int64_t)seq * c.table_stride;
+    if (warp == 0) {
+        int sum = 0;
+        for (int s0 = 0; s0 < n_seq; s0 += 32) {
+            const int s = s0 + lane;
+            int first = 0, mine = 0;
+            if (s < n_seq) {
+                const Portion p = portion_of(c, seq0 + s);
+                tiles_of(c, p, &first, &mine);
+                mine *= kv * (c.q_start == nullptr ? tiles : p.count > 0 ? (p.count * c.per + kRows - 1) / kRows : 0);
+            }
+            int before = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
+            }
+            if (s < n_seq) {
+                starts[s] = sum + before - mine;
+                firsts[s] = first;
+            }
+            sum += __shfl_sync(0xffffffffu, before, 31);
+        }
+        if (lane == 0) starts[n_seq] = sum;
+    }
+    __syncthreads();
+    const int total = starts[n_seq], n_warps = gridDim.x * kWarps, me = blockIdx.x * kWarps + warp;
+    const int share = share_of(total, n_warps);
+    if (blockIdx.x == 0)                                    // for the launch that joins the states
+        for (int s = threadIdx.x; s <= n_seq; s += kWarps * 32) c.starts[(int64_t)blockIdx.y * (per_row + 1) + s] = starts[s];
+    const int begin = min((int64_t)me * share, (int64_t)total), end = min((int64_t)(me + 1) * share, (int64_t)total);
+    if (begin >= end) return;
+    // The request that tile x of the row belongs to.
+    auto request_of = [&](int x) {
+        int lo = 0, hi = n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (starts[mid] <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    auto row_tiles_of = [&](const Portion& p) { return c.q_start == nullptr ? tiles : (p.count * c.per + kRows - 1) / kRows; };
 
     uint8_t* ring = smem + warp * kStages * kBlock;
-    int page_reg = 0;
+    const int n_tiles = end - begin;
+    int listed = 0, asked = 0;                             // tiles whose blocks are found, tiles asked for
     uint32_t missing = 0;                                  // a bit a stage: its keys are on no page
-    auto tile_at = [&](int i) { return tile0 + warp + W * i; };
-    auto fetch = [&](int i) {
-        if ((i & 31) == 0) page_reg = i + lane < my_tiles ? table[tile_at(i + lane) * kBlockKeys >> c.pages.page_shift] : 0;
-        const int64_t at = c.pages.at(__shfl_sync(0xffffffffu, page_reg, i & 31), kvh, tile_at(i) * kBlockKeys);
-        const int stage = i % kStages;
-        missing = (missing & ~(1u << stage)) | (at < 0 ? 1u << stage : 0u);
-        if (at >= 0 && lane == 0) {
+    // Asks for the next n tiles (up to a ring), a lane each.
+    auto fetch = [&](int n) {
+        n = min(n, n_tiles - asked);
+        if (n <= 0) return;
+        if (asked + n > listed) {
+            const int x = begin + listed + lane;
+            int at = -1;
+            if (x < end) {
+                const int s = request_of(x), in_row = row_tiles_of(portion_of(c, seq0 + s)), count = (starts[s + 1] - starts[s]) / (kv * in_row);
+                const int unit = (x - starts[s]) / count, tile = firsts[s] + x - starts[s] - unit * count, kvh = unit / in_row;
+                const int page = c.table[(int64_t)(seq0 + s) * c.table_stride + (tile * kBlockKeys >> c.pages.page_shift)];
+                if ((unsigned)page < (unsigned)c.pages.n_pages) at = ((page * kv + kvh) << (c.pages.page_shift - 4)) + (tile & ((1 << (c.pages.page_shift - 4)) - 1));
+            }
+            found[warp][(listed + lane) & 63] = at;
+            listed += 32;
+            __syncwarp();
+        }
+        const int mine = asked + lane, stage = mine % kStages, at = found[warp][mine & 63];
+        const bool here = lane < n;
+        if (here && at >= 0) {
             lb_tc::mbar_expect_tx(&bars[warp][stage], kBlock);
-            copy_block(ring + stage * kBlock, c.pages.memory + at, kBlock, &bars[warp][stage]);
-        } else if (lane == 0) {
+            copy_block(ring + stage * kBlock, c.pages.memory + (int64_t)at * kBlock, kBlock, &bars[warp][stage]);
+        } else if (here) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lb_tc::smem_u32(&bars[warp][stage])) : "memory");
         }
+        uint32_t bits = __ballot_sync(0xffffffffu, here && at < 0);              // of lanes: tiles asked, asked + 1, ..
+        missing &= ~(((((1u << n) - 1u) << (asked % kStages)) | (((1u << n) - 1u) << (asked % kStages) >> kStages)) & ((1u << kStages) - 1u));
+        bits <<= asked % kStages;
+        missing |= (bits | bits >> kStages) & ((1u << kStages) - 1u);
+        asked += n;
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
-        if (i < my_tiles) fetch(i);
+    fetch(kStages);
 
-    // The queries as the second operand: lane (g, t) has the dims 32 j + 8 t .. + 7 of row g, times a power of two that puts the row's largest at 2^14.
-    uint32_t qf[NT][JK][4];
-    float row_scale[NT][2];                                // of the rows 2 t and 2 t + 1, the accumulators' columns
-    const bool q_wide = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.q_stride % 8 == 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int row = row0 + 8 * n + g;
-        const bool there = row < n_rows;
-        const __nv_bfloat16* from = c.q + (int64_t)(part.first + (there ? row / c.per : 0)) * c.q_stride + (int64_t)(kvh * c.per + (there ? row % c.per : 0)) * HD + 8 * t;
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < JK; ++j) {
-            uint32_t u[4] = {0, 0, 0, 0};
-            if (there && q_wide) {
-                load_words<16>(reinterpret_cast<const uint8_t*>(from + 32 * j), u);
-            } else if (there) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = __bfloat16_as_ushort(from[32 * j + 2 * e]) | (uint32_t)__bfloat16_as_ushort(from[32 * j + 2 * e + 1]) << 16;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                qf[n][j][e] = u[e];
-                top = max(top, max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
-            }
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^shift times the row; a row of zeros, or with values that are not finite, stays as it is.
-        const int shift = top == 0 || top >= 0x7f80u ? 0 : 14 - (max((int)(top >> 7), 1) - 127);
-        const float up = pow2(shift / 2), up2 = pow2(shift - shift / 2);
-#pragma unroll
-        for (int j = 0; j < JK; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                qf[n][j][e] = h2(__floats2half2_rn(__uint_as_float(qf[n][j][e] << 16) * up * up2, __uint_as_float(qf[n][j][e] & 0xffff0000u) * up * up2));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int s = __shfl_sync(0xffffffffu, shift, (2 * t + e) * 4);
-            row_scale[n][e] = c.scale * kLbLog2e * pow2(-s / 2) * pow2(-s - -s / 2);
-        }
-    }
-    float m[NT][2], l[NT][2], o[NT][JV * 4][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) m[n][e] = kLowest, l[n][e] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < JV * 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-    }
-    float f = kLeastScale - kRoom;
-    uint32_t f_bits = (uint32_t)(127 + (int)kLeastScale) << 7;              // 2^(f + kRoom) as bfloat16: no scale seen is larger
     const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.0f);
     const bool biased = !PLAIN && c.distance != nullptr;
-    float r1[NT][2], r2[NT][2];
-    int place[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int row = row0 + 8 * n + 2 * t + e;
-            place[n][e] = place_of(row);
-            r1[n][e] = r2[n][e] = 0.0f;
-            if (biased && row < n_rows) {
-                r1[n][e] = c.distance[kvh * c.per + row % c.per];
-                r2[n][e] = c.distance[c.n_head + kvh * c.per + row % c.per];
-            }
-        }
-    float* scores = PLAIN || c.scores == nullptr ? nullptr : c.scores + (((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + row0) * c.score_keys;
-
+    const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;          // no key past this place is read
+    const bool q_wide = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.q_stride % 8 == 0;
     bool gave_up = false;
     int done = 0;
-    for (int i = 0; i < my_tiles; ++i) {
-        const int stage = i % kStages;
-        if (i + kStages - 1 < my_tiles) fetch(i + kStages - 1);
-        // Bounded; one answer for the warp.
-        if (!__all_sync(0xffffffffu, lb_tc::mbar_wait(&bars[warp][stage], (uint32_t)(i / kStages) & 1u, nullptr))) {
-            gave_up = true;
-            done = i;
-            break;
-        }
-        const uint8_t* block = ring + stage * kBlock;
-        const int key0 = tile_at(i) * kBlockKeys;
-        // S^T of sixteen keys: a[0], a[1] key g and the columns 2 t and 2 t + 1, a[2], a[3] key g + 8.
-        float z[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[n][e] = 0.0f;
-        {
-            uint32_t lo[JK], hi[JK], sc[NG];                    // scales: NG of key g, then NG of key g + 8
-            load_words<L::kPiece>(block + lane * L::kPiece, lo);
-            load_words<L::kPiece>(block + 32 * L::kPiece + lane * L::kPiece, hi);
-            load_words<4 * NG>(block + L::kScales + g * 4 * NG, sc);
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                float a[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a[n][e] = 0.0f;
-#pragma unroll
-                for (int j = gr * JK / NG; j < (gr + 1) * JK / NG; ++j) {
-                    uint32_t x[4], y[4];
-                    pairs_of(lo[j], x);
-                    pairs_of(hi[j], y);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_f16(a[n], x[0], y[0], x[1], y[1], qf[n][j][0], qf[n][j][1]);
-                        mma_f16(a[n], x[2], y[2], x[3], y[3], qf[n][j][2], qf[n][j][3]);
-                    }
-                }
-                const float s0 = number(sc, gr), s1 = number(sc, NG + gr);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    z[n][0] = fmaf(a[n][0], s0, z[n][0]);
-                    z[n][1] = fmaf(a[n][1], s0, z[n][1]);
-                    z[n][2] = fmaf(a[n][2], s1, z[n][2]);
-                    z[n][3] = fmaf(a[n][3], s1, z[n][3]);
-                }
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[n][e] *= row_scale[n][e & 1];
-        if constexpr (!PLAIN) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + g + 8 * (e >> 1);
-                    if (capped.on) z[n][e] = capped(z[n][e]);
-                    if (biased) z[n][e] -= lb_distance_penalty_log2(r1[n][e & 1], r2[n][e & 1], max(place[n][e & 1] - key, 0));
-                }
-        }
-        uint32_t vs[NG];
-        load_words<4 * NG>(block + L::kScales + 32 * NG + g * 4 * NG, vs);
-        const bool absent = (missing >> stage & 1u) != 0;
-        if (key0 + kBlockKeys - 1 > p_lo || key0 < first_hi || absent) {
-            // Keys that some row does not see: their scores are -inf, and the scales of those past every row (whatever the memory holds) 0.
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + g + 8 * (e >> 1), p = place[n][e & 1];
-                    if (absent || key > p || key < lb_first_visible(max(p, 0), c.window)) z[n][e] = -CUDART_INF_F;
-                }
-#pragma unroll
-            for (int i2 = 0; i2 < 2; ++i2) {
-                const int key = key0 + g + 8 * i2;
-                if (absent || key > p_hi || key < first_lo) {
-                    if constexpr (NG == 1) {
-                        vs[0] &= i2 == 0 ? 0xffff0000u : 0x0000ffffu;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < NG / 2; ++e) vs[i2 * NG / 2 + e] = 0;
-                    }
-                }
-            }
-        }
-        if constexpr (!PLAIN) {
-            if (scores != nullptr) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = 8 * n + 2 * t + (e & 1), key = key0 + g + 8 * (e >> 1);
-                        if (row < rows_here && key < c.score_keys) scores[(int64_t)row * c.score_keys + key] = z[n][e];
-                    }
-            }
-        }
-        // Does a score pass its row's reference, or a scale f?
-        uint32_t top = vs[0];
-#pragma unroll
-        for (int e = 1; e < NG; ++e) top = __vmaxu2(top, vs[e]);
-        top = max(top & 0xffffu, top >> 16);
-        bool moved = top > f_bits;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) moved = moved || z[n][e] > m[n][e & 1] + kSlack;
-        if (__any_sync(0xffffffffu, moved)) {
-            top = __reduce_max_sync(0xffffffffu, top);
-            float f_new = f;
-            if (top > f_bits) {
-                f_bits = (min(top, 0x7f00u) + 0x7fu) & 0x7f80u;         // the next power of two (2^127 at most; a NaN stays one whatever it is divided by)
-                f_new = (float)((int)(f_bits >> 7) - 127) - kRoom;
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float high = fmaxf(z[n][e], z[n][e + 2]);
-#pragma unroll
-                    for (int d = 4; d < 32; d *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
-                    high = fmaxf(high, m[n][e]);
-                    const float corr = ex2((m[n][e] - high) + (f - f_new));
-                    m[n][e] = high;
-                    l[n][e] *= corr;
-#pragma unroll
-                    for (int k = 0; k < JV * 4; ++k) {
-                        o[n][k][e] *= corr;
-                        o[n][k][e + 2] *= corr;
-                    }
-                }
-            f = f_new;
-        }
-        uint32_t pf[NT][NG][2];                                          // p s of the groups, as the second operand
+    // A run: the tiles of one request, key/value head and row tile.
+    while (done < n_tiles && !gave_up) {
+        const int s = request_of(begin + done), seq = seq0 + s;
+        const Portion part = portion_of(c, seq);
+        const int in_row = row_tiles_of(part), count = (starts[s + 1] - starts[s]) / (kv * in_row);
+        const int unit = (begin + done - starts[s]) / count, kvh = unit / in_row, row_tile = unit - kvh * in_row;
+        const int tile0 = firsts[s] + begin + done - starts[s] - unit * count;
+        const int run_end = min(n_tiles, starts[s] + (unit + 1) * count - begin), run_begin = done;
+        const int n_rows = part.count * c.per, row0 = row_tile * kRows, rows_here = min(kRows, n_rows - row0);
+        auto token_of = [&](int row) { return part.count == 1 ? 0 : row / c.per; };
+        auto place_of = [&](int row) { return min(part.place + token_of(min(row, n_rows - 1)), limit); };
+        const int p_lo = place_of(row0), p_hi = place_of(row0 + rows_here - 1);
+        const int first_lo = p_lo < 0 ? 0 : lb_first_visible(p_lo, c.window), first_hi = p_hi < 0 ? 0 : lb_first_visible(p_hi, c.window);
+
+        // The queries as the second operand: columns are (row, digit).  A row times a power of two, so that its largest is in 2^14 .. 2^15, is rounded to 16 bits, 256 high + low, both
+        // -128 .. 127; lane (g, t) has digit g % 2 of the dims 32 j + 8 t .. + 7 of row g / 2, in the order of the nibbles of a key's word.  An operand's keys are n + 8, so the sums start
+        // at -8 times the digits' sum, and at the bits of 1.5 2^23: what they come to is a float's bits.
+        uint32_t qd[NT][JK][2];
+        int base[NT][NG][2];                                   // of columns 2 t and 2 t + 1: high and low digit of row t
+        float row_scale[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float ref0 = m[n][0] + f, ref1 = m[n][1] + f;
-            float p[4];
-            p[0] = ex2(z[n][0] - ref0);
-            p[1] = ex2(z[n][1] - ref1);
-            p[2] = ex2(z[n][2] - ref0);
-            p[3] = ex2(z[n][3] - ref1);
-            l[n][0] += p[0] + p[2];
-            l[n][1] += p[1] + p[3];
+            const int row = row0 + 4 * n + (g >> 1);
+            const bool there = row < n_rows;
+            const int token = there ? token_of(row) : 0, head = there ? row - token * c.per : 0;
+            const __nv_bfloat16* from = c.q + (int64_t)(part.first + token) * c.q_stride + (int64_t)(kvh * c.per + head) * HD + 8 * t;
+            uint32_t top = 0, u[JK][4];
+#pragma unroll
+            for (int j = 0; j < JK; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[j][e] = 0;
+                if (there && q_wide) {
+                    load_words<16>(reinterpret_cast<const uint8_t*>(from + 32 * j), u[j]);
+                } else if (there) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[j][e] = __bfloat16_as_ushort(from[32 * j + 2 * e]) | (uint32_t)__bfloat16_as_ushort(from[32 * j + 2 * e + 1]) << 16;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, max(u[j][e] & 0x7fffu, u[j][e] >> 16 & 0x7fffu));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // (A largest value of eight ones, 32,640 of 2^15, would have a high digit of 128: it goes a bit lower.)  A row that is not finite has NaN for a factor.
+            const int shift = top == 0 || top >= 0x7f80u ? 0 : 14 - (max((int)(top >> 7), 1) - 127) - ((top & 0x7fu) == 0x7fu);
+            const float up = pow2(shift / 2), up2 = pow2(shift - shift / 2);
+            int sums[JK];
+#pragma unroll
+            for (int j = 0; j < JK; ++j) {
+                int digit[8];
+                sums[j] = 0;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const float x = __uint_as_float((d & 1) != 0 ? u[j][d / 2] & 0xffff0000u : u[j][d / 2] << 16);
+                    const int v = top >= 0x7f80u ? 0 : __float2int_rn(x * up * up2), low = (int)(int8_t)v;
+                    digit[d] = (g & 1) != 0 ? low : (v - low) >> 8;
+                    sums[j] += digit[d];
+                }
+                auto four = [&](int a, int b, int cc, int dd) { return (digit[a] & 255) | (digit[b] & 255) << 8 | (digit[cc] & 255) << 16 | (uint32_t)(digit[dd] & 255) << 24; };
+                qd[n][j][0] = four(0, 4, 1, 5);                 // nibbles 0, 2, 4, 6
+                qd[n][j][1] = four(2, 6, 3, 7);                 // nibbles 1, 3, 5, 7
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
+            }
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const float s0 = number(vs, gr), s1 = number(vs, NG + gr);
-                pf[n][gr][0] = turned(h2(__floats2half2_rn(p[0] * s0, p[1] * s0)));
-                pf[n][gr][1] = turned(h2(__floats2half2_rn(p[2] * s1, p[3] * s1)));
+                int sum = 0;
+#pragma unroll
+                for (int j = gr * JK / NG; j < (gr + 1) * JK / NG; ++j) sum += sums[j];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) base[n][gr][e] = kMagicBits - 8 * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+            }
+            const int sh = __shfl_sync(0xffffffffu, shift, 8 * t);
+            const uint32_t row_top = __shfl_sync(0xffffffffu, top, 8 * t);
+            row_scale[n] = row_top >= 0x7f80u ? CUDART_NAN_F : c.scale * kLbLog2e * pow2(-sh / 2) * pow2(-sh - -sh / 2);
+        }
+        // m: a row's largest score, or near it; ref: m + f, what scores are taken relative to; passes: m and the slack.
+        float m[NT], l[NT], ref[NT], passes[NT], o[VT][JV * 4][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) m[n] = ref[n] = passes[n] = kLowest, l[n] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < VT; ++n)
+#pragma unroll
+            for (int i = 0; i < JV * 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+        float f = kLeastScale - kRoom;
+        uint32_t f_bits = (uint32_t)(127 + (int)kLeastScale) << 7;              // 2^(f + kRoom) as bfloat16: no scale seen is larger
+        float r1[NT], r2[NT];
+        int place[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = row0 + 4 * n + t;
+            place[n] = place_of(row);
+            r1[n] = r2[n] = 0.0f;
+            if (biased && row < n_rows) {
+                const int head = kvh * c.per + row - token_of(row) * c.per;
+                r1[n] = c.distance[head];
+                r2[n] = c.distance[c.n_head + head];
             }
         }
-        // O^T: lane (g, t) has the words of the keys 2 t, 2 t + 1 (x) and of those plus 8 (y).
-        {
-            uint32_t x[2 * JV], y[2 * JV];
-            const int at = (t * 8 + L::v_turn(g, t)) * L::kPiece;
-            load_words<L::kPiece>(block + L::kV + at, x);
-            load_words<L::kPiece>(block + L::kV + 32 * L::kPiece + at, y);
+        float* scores = PLAIN || c.scores == nullptr ? nullptr : c.scores + (((int64_t)seq * kv + kvh) * c.max_rows + row0) * c.score_keys;
+
+        while (done < run_end) {
+            // Two tiles at a time; where a run has one left, it stands for both and the second is masked.
+            const int pair = min(2, run_end - done);
+            bool there = lb_tc::mbar_wait(&bars[warp][done % kStages], (uint32_t)(done / kStages) & 1u, nullptr);
+            if (pair == 2) there = there && lb_tc::mbar_wait(&bars[warp][(done + 1) % kStages], (uint32_t)((done + 1) / kStages) & 1u, nullptr);
+            if (!__all_sync(0xffffffffu, there)) {                 // bounded; one answer for the warp
+                gave_up = true;
+                break;
+            }
+            const int key0 = (tile0 + done - run_begin) * kBlockKeys;
+            const uint8_t* block[2];
 #pragma unroll
-            for (int j = 0; j < JV; ++j) {
-                uint32_t a0[4], a1[4], a2[4], a3[4];
-                pairs_of(__byte_perm(x[j], x[JV + j], 0x5410), a0);
-                pairs_of(__byte_perm(x[j], x[JV + j], 0x7632), a1);
-                pairs_of(__byte_perm(y[j], y[JV + j], 0x5410), a2);
-                pairs_of(__byte_perm(y[j], y[JV + j], 0x7632), a3);
+            for (int u = 0; u < 2; ++u) block[u] = ring + (done + (u < pair ? u : 0)) % kStages * kBlock;
+            float z[NT][2][2];                                     // [tile][key g, key g + 8] of row t
+            uint32_t vs[2][NG];                                    // the values' scales: NG of key g, then NG of key g + 8
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int gr = (64 * j + 32 * (k >> 1)) / (HD / NG);
+            for (int u = 0; u < 2; ++u) {
+                uint32_t lo[JK], hi[JK], sc[NG];
+                load_words<L::kPiece>(block[u] + lane * L::kPiece, lo);
+                load_words<L::kPiece>(block[u] + 32 * L::kPiece + lane * L::kPiece, hi);
+                load_words<4 * NG>(block[u] + L::kScales + g * 4 * NG, sc);
+                load_words<4 * NG>(block[u] + L::kScales + 32 * NG + g * 4 * NG, vs[u]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(o[n][j * 4 + k], a0[k], a1[k], a2[k], a3[k], pf[n][gr][0], pf[n][gr][1]);
+                for (int gr = 0; gr < NG; ++gr) {
+                    int a[NT][4];
+#pragma unroll
+                    for (int j = gr * JK / NG; j < (gr + 1) * JK / NG; ++j) {
+                        const uint32_t a0 = lo[j] & 0x0f0f0f0fu, a1 = hi[j] & 0x0f0f0f0fu, a2 = lo[j] >> 4 & 0x0f0f0f0fu, a3 = hi[j] >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if (j == gr * JK / NG) mma_u8s8_first(a[n], a0, a1, a2, a3, qd[n][j][0], qd[n][j][1], base[n][gr][0], base[n][gr][1]);
+                            else mma_u8s8(a[n], a0, a1, a2, a3, qd[n][j][0], qd[n][j][1]);
+                        }
+                    }
+                    const float s0 = number(sc, gr), s1 = number(sc, NG + gr);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float k0 = fmaf(__int_as_float(a[n][0]) - kMagic, 256.0f, __int_as_float(a[n][1]) - kMagic);
+                        const float k1 = fmaf(__int_as_float(a[n][2]) - kMagic, 256.0f, __int_as_float(a[n][3]) - kMagic);
+                        z[n][u][0] = gr == 0 ? k0 * s0 : fmaf(k0, s0, z[n][u][0]);
+                        z[n][u][1] = gr == 0 ? k1 * s1 : fmaf(k1, s1, z[n][u][1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        z[n][u][e] *= row_scale[n];
+                        if constexpr (!PLAIN) {
+                            if (capped.on) z[n][u][e] = capped(z[n][u][e]);
+                            if (biased) z[n][u][e] -= lb_distance_penalty_log2(r1[n], r2[n], max(place[n] - (key0 + 16 * u + g + 8 * e), 0));
+                        }
+                    }
+            }
+            const uint32_t gone = (missing >> (done % kStages) & 1u) | (missing >> ((done + 1) % kStages) & 1u) << 1;
+            if (key0 + 2 * kBlockKeys - 1 > p_lo || key0 < first_hi || gone != 0 || pair == 1) {
+                // Keys that some row does not see: their scores are -inf, and the scales of those past every row (whatever the memory holds) 0.
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = key0 + 16 * u + g + 8 * e;
+                        const bool absent = u >= pair || (gone >> u & 1u) != 0;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            if (absent || key > place[n] || key < lb_first_visible(max(place[n], 0), c.window)) z[n][u][e] = -CUDART_INF_F;
+                        if (absent || key > p_hi || key < first_lo) {
+                            if constexpr (NG == 1) {
+                                vs[u][0] &= e == 0 ? 0xffff0000u : 0x0000ffffu;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < NG / 2; ++i) vs[u][e * NG / 2 + i] = 0;
+                            }
+                        }
+                    }
+            }
+            if constexpr (!PLAIN) {
+                if (scores != nullptr) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int row = 4 * n + t, key = key0 + 16 * u + g + 8 * e;
+                                if (row < rows_here && u < pair && key < c.score_keys) scores[(int64_t)row * c.score_keys + key] = z[n][u][e];
+                            }
                 }
             }
+            // Does a score pass its row's reference, or a scale f?
+            uint32_t top = __vmaxu2(vs[0][0], vs[1][0]);
+#pragma unroll
+            for (int i = 1; i < NG; ++i) top = __vmaxu2(top, __vmaxu2(vs[0][i], vs[1][i]));
+            bool moved = (top >> 16) > f_bits || (top & 0xffffu) > f_bits;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) moved = moved || fmaxf(fmaxf(z[n][0][0], z[n][0][1]), fmaxf(z[n][1][0], z[n][1][1])) > passes[n];
+            if (__any_sync(0xffffffffu, moved)) {
+                top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+                float f_new = f;
+                if (top > f_bits) {
+                    f_bits = (min(top, 0x7f00u) + 0x7fu) & 0x7f80u;         // the next power of two (2^127 at most; a NaN stays one whatever it is divided by)
+                    f_new = (float)((int)(f_bits >> 7) - 127) - kRoom;
+                }
+                float corr[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float high = fmaxf(fmaxf(z[n][0][0], z[n][0][1]), fmaxf(z[n][1][0], z[n][1][1]));
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                    high = fmaxf(high, m[n]);
+                    corr[n] = ex2((m[n] - high) + (f - f_new));
+                    m[n] = high;
+                    ref[n] = high + f_new;
+                    passes[n] = high + kSlack;
+                    l[n] *= corr[n];
+                }
+#pragma unroll
+                for (int v = 0; v < VT; ++v)
+#pragma unroll
+                    for (int k = 0; k < JV * 4; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[v][k][e] *= NT == 1 ? corr[0] : corr[(2 * v + (e & 1)) % NT];
+                f = f_new;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t pf[VT][VG][2];                                          // p s, as the second operand
+                float p[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    p[n][0] = ex2(z[n][u][0] - ref[n]);
+                    p[n][1] = ex2(z[n][u][1] - ref[n]);
+                    l[n] += p[n][0] + p[n][1];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float sv[NG];
+#pragma unroll
+                    for (int gr = 0; gr < NG; ++gr) sv[gr] = number(vs[u], e * NG + gr);
+#pragma unroll
+                    for (int v = 0; v < VT; ++v)
+#pragma unroll
+                        for (int x = 0; x < VG; ++x)
+                            pf[v][x][e] = turned(h2(NT == 1 ? __floats2half2_rn(p[0][e] * sv[2 * x], p[0][e] * sv[(2 * x + 1) % NG])
+                                                            : __floats2half2_rn(p[2 * v][e] * sv[x % NG], p[(2 * v + 1) % NT][e] * sv[x % NG])));
+                }
+                // V^T p^T: lane (g, t) has the words of the keys 2 t, 2 t + 1 (x) and of those plus 8 (y).
+                uint32_t x[2 * JV], y[2 * JV];
+                const int at = (t * 8 + L::v_turn(g, t)) * L::kPiece;
+                load_words<L::kPiece>(block[u] + L::kV + at, x);
+                load_words<L::kPiece>(block[u] + L::kV + 32 * L::kPiece + at, y);
+#pragma unroll
+                for (int j = 0; j < JV; ++j) {
+                    uint32_t a0[4], a1[4], a2[4], a3[4];
+                    pairs_of(__byte_perm(x[j], x[JV + j], 0x5410), a0);
+                    pairs_of(__byte_perm(x[j], x[JV + j], 0x7632), a1);
+                    pairs_of(__byte_perm(y[j], y[JV + j], 0x5410), a2);
+                    pairs_of(__byte_perm(y[j], y[JV + j], 0x7632), a3);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int gr = (64 * j + 32 * (k >> 1)) / (HD / NG), x2 = NT == 1 ? gr / 2 : gr;
+#pragma unroll
+                        for (int v = 0; v < VT; ++v) mma_f16(o[v][j * 4 + k], a0[k], a1[k], a2[k], a3[k], pf[v][x2][0], pf[v][x2][1]);
+                    }
+                }
+            }
+            __syncwarp();                                   // the stages are overwritten by the copies asked for next
+            done += pair;
+            fetch(pair);
         }
-        __syncwarp();                                   // the stage is overwritten by the copy issued in the next trip
+        if (gave_up) break;
+
+        // The run's state, for the launch that joins them: m + f, the sum and the values of its rows.
+        float* state = c.partial + ((int64_t)blockIdx.y * (n_warps + (int64_t)per_row * kv * tiles) + me + ((int64_t)s * kv + kvh) * tiles + row_tile) * (kRows * kState);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) l[n] += __shfl_xor_sync(0xffffffffu, l[n], d);
+            const int row = 4 * n + t;
+            if (row >= rows_here) continue;
+            float* to = state + row * kState;
+            if (g == 0) *reinterpret_cast<float2*>(to) = make_float2(ref[n], l[n]);
+#pragma unroll
+            for (int j = 0; j < JV; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int gr = (64 * j + 32 * (k >> 1)) / (HD / NG), e = NT == 1 ? gr & 1 : n & 1;
+                    *reinterpret_cast<float2*>(to + 2 + 64 * j + 32 * (k >> 1) + 4 * g + 2 * (k & 1)) = make_float2(o[n / 2][j * 4 + k][e], o[n / 2][j * 4 + k][e + 2]);
+                }
+        }
     }
     if (gave_up) {
         // The copies still in flight land before the block may leave (bounded as well); the result is wrong and the status word says so.
         if (lane == 0) atomicCAS(status, 0, (0xC << 12) | 1);
-        for (int i = done; i < my_tiles && i < done + kStages; ++i) lb_tc::mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u, nullptr);
+        for (int i = done; i < asked; ++i) lb_tc::mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u, nullptr);
     }
-
-    // The warps' states: m + f, the sum and the values of a row.
-    float* states = reinterpret_cast<float*>(smem);                 // [warp][row][kState]
-    float* own = states + W * kRows * kState;                       // [row][kState]: the block's
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int d = 4; d < 32; d *= 2) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-    __syncthreads();                                                // the rings have been read
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float* st = states + (warp * kRows + 8 * n + 2 * t + e) * kState;
-            if (g == 0) {
-                st[0] = m[n][e] + f;
-                st[1] = l[n][e];
-            }
-#pragma unroll
-            for (int j = 0; j < JV; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    *reinterpret_cast<float2*>(st + 2 + 64 * j + 32 * (k >> 1) + 4 * g + 2 * (k & 1)) = make_float2(o[n][j * 4 + k][e], o[n][j * 4 + k][e + 2]);
-        }
-    __syncthreads();
-    if (threadIdx.x < kRows) {
-        const int row = threadIdx.x;
-        float mm = kLowest, ll = 0.0f;
-        for (int w = 0; w < W; ++w) mm = fmaxf(mm, states[(w * kRows + row) * kState]);
-        for (int w = 0; w < W; ++w) {
-            const float* st = states + (w * kRows + row) * kState;
-            factor[w][row] = st[1] == 0.0f ? 0.0f : exp2f(st[0] - mm);
-            ll += st[1] * factor[w][row];
-        }
-        block_m[row] = mm;
-        block_l[row] = ll;
-        own[row * kState] = mm;
-        own[row * kState + 1] = ll;
-    }
-    __syncthreads();
-    const bool alone = n_splits == 1;
-    const int64_t unit = ((int64_t)seq * c.pages.n_kv_head + kvh) * tiles + row_tile;
-    // A row's result from its divisor's reference and sum (the sink joined) and a sum of values.
-    auto finish = [&](int row, int d, float mm, float ll, float v) {
-        const int r = row0 + row, head = kvh * c.per + r % c.per;
-        if (c.sink != nullptr) v *= lb_sink_join_exp2(c.sink[head] * kLbLog2e, mm, ll);
-        c.out[(int64_t)(part.first + r / c.per) * c.out_stride + head * HD + d] = __float2bfloat16_rn(ll == 0.0f ? 0.0f : v / ll);
-        if (d == 0 && c.log_sums != nullptr) {
-            const float top = c.sink != nullptr ? fmaxf(mm, c.sink[head] * kLbLog2e) : mm;
-            c.log_sums[((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + r] = ll == 0.0f ? CUDART_INF_F : top + log2f(ll);
-        }
-    };
-    for (int i = threadIdx.x; i < rows_here * HD; i += kThreads) {
-        const int row = i / HD, d = i - row * HD;
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) v = fmaf(factor[w][row], states[(w * kRows + row) * kState + 2 + d], v);
-        if (alone) finish(row, d, block_m[row], block_l[row], v);
-        else if (cluster) own[row * kState + 2 + d] = v;
-        else c.partial[((unit * n_splits + split) * kRows + row) * kState + 2 + d] = v;
-    }
-    if (alone) return;
-    if (!cluster) {
-        if (threadIdx.x < rows_here) {
-            float* to = c.partial + ((unit * n_splits + split) * kRows + threadIdx.x) * kState;
-            to[0] = block_m[threadIdx.x];
-            to[1] = block_l[threadIdx.x];
-        }
-        return;
-    }
-    // The ranges' states meet: every block makes its share of the values from all blocks' shared memory.
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const uint32_t own_at = lb_tc::smem_u32(own);
-    auto remote = [&](int rank, int index) {
-        uint32_t at;
-        float v;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(own_at + 4u * (uint32_t)index), "r"(rank));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-        return v;
-    };
-    const int share_of = (rows_here * HD + n_splits - 1) / n_splits;
-    for (int i = split * share_of + threadIdx.x; i < min((split + 1) * share_of, rows_here * HD); i += kThreads) {
-        const int row = i / HD, d = i - row * HD;
-        float mm = kLowest, ll = 0.0f, v = 0.0f;
-        for (int s = 0; s < n_splits; ++s) mm = fmaxf(mm, remote(s, row * kState));
-        for (int s = 0; s < n_splits; ++s) {
-            const float sum = remote(s, row * kState + 1), w = sum == 0.0f ? 0.0f : exp2f(remote(s, row * kState) - mm);
-            ll = fmaf(sum, w, ll);
-            v = fmaf(remote(s, row * kState + 2 + d), w, v);
-        }
-        finish(row, d, mm, ll, v);
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The ranges' states of a row tile, where more blocks share a request's keys than a cluster has.
+// Joins the states of a row's runs, in their order within each of the block's groups of HD threads, the groups' in theirs.
 template <int HD>
-__global__ void __launch_bounds__(256)
-attention4_meet_kernel(const Call c, int n_splits, int tiles, int tile_rows) {
+__global__ void __launch_bounds__(1024)
+attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int tile_rows) {
     constexpr int kState = HD + 2;
+    __shared__ float joined[1024 / HD][kState];
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int seq = blockIdx.z, kvh = blockIdx.y / tiles, row_tile = blockIdx.y - kvh * tiles;
+    const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq / per_row, s = seq - row_of * per_row;
+    const int r = blockIdx.x, d = threadIdx.x % HD, group = threadIdx.x / HD, n_groups = blockDim.x / HD;
     const Portion part = portion_of(c, seq);
-    const int n_rows = part.count * c.per, r = row_tile * tile_rows + blockIdx.x, d = threadIdx.x;
-    if (r >= n_rows || (int)blockIdx.x >= tile_rows || d >= HD) return;
-    const int64_t unit = ((int64_t)seq * c.pages.n_kv_head + kvh) * tiles + row_tile;
-    const float* from = c.partial + (unit * n_splits * tile_rows + blockIdx.x) * kState;
+    if (r >= part.count * c.per) return;
+    const int row_tile = r / tile_rows, in_row = c.q_start == nullptr ? tiles : (part.count * c.per + tile_rows - 1) / tile_rows;
+    const int* starts = c.starts + (int64_t)row_of * (per_row + 1);
+    const int start = starts[s], count = (starts[s + 1] - start) / (kv * in_row), n_seq = min(per_row, c.n_seq - row_of * per_row);
+    const int from = start + (kvh * in_row + row_tile) * count, share = share_of(starts[n_seq], n_warps);
+    const int first = count > 0 ? from / share : 0, runs = count > 0 ? (from + count - 1) / share - first + 1 : 0;
+    const float* state = c.partial + (((int64_t)row_of * (n_warps + (int64_t)per_row * kv * tiles) + first + ((int64_t)s * kv + kvh) * tiles + row_tile) * tile_rows + r - row_tile * tile_rows) *
+                                         kState;
     const int64_t step = (int64_t)tile_rows * kState;
-    float mm = kLowest, ll = 0.0f, v = 0.0f;
-    for (int s = 0; s < n_splits; ++s) mm = fmaxf(mm, from[s * step]);
-    for (int s = 0; s < n_splits; ++s) {
-        const float sum = from[s * step + 1], w = sum == 0.0f ? 0.0f : exp2f(from[s * step] - mm);
-        ll = fmaf(sum, w, ll);
-        v = fmaf(from[s * step + 2 + d], w, v);
+    float m = kLowest, l = 0.0f, v = 0.0f;
+#pragma unroll 4
+    for (int i = group; i < runs; i += n_groups) {
+        const float2 ml = *reinterpret_cast<const float2*>(state + i * step);
+        const float o = state[i * step + 2 + d];
+        const float top = ml.y == 0.0f ? m : fmaxf(m, ml.x), w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top), keep = exp2f(m - top);
+        l = fmaf(l, keep, ml.y * w);
+        v = fmaf(v, keep, o * w);
+        m = top;
+    }
+    if (n_groups > 1) {
+        joined[group][2 + d] = v;
+        if (d == 0) {
+            joined[group][0] = m;
+            joined[group][1] = l;
+        }
+        __syncthreads();
+        if (group > 0) return;
+        for (int i = 1; i < n_groups; ++i) {
+            const float mi = joined[i][0], li = joined[i][1], top = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : exp2f(mi - top), keep = exp2f(m - top);
+            l = fmaf(l, keep, li * w);
+            v = fmaf(v, keep, joined[i][2 + d] * w);
+            m = top;
+        }
     }
     const int head = kvh * c.per + r % c.per;
-    float top = mm;
+    float top = m;
     if (c.sink != nullptr) {
-        top = fmaxf(mm, c.sink[head] * kLbLog2e);
-        v *= lb_sink_join_exp2(c.sink[head] * kLbLog2e, mm, ll);
+        const float sink = c.sink[head] * kLbLog2e;
+        top = fmaxf(m, sink);
+        v *= lb_sink_join_exp2(sink, m, l);
     }
-    c.out[(int64_t)(part.first + r / c.per) * c.out_stride + head * HD + d] = __float2bfloat16_rn(ll == 0.0f ? 0.0f : v / ll);
-    if (d == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + r] = ll == 0.0f ? CUDART_INF_F : top + log2f(ll);
+    c.out[(int64_t)(part.first + r / c.per) * c.out_stride + head * HD + d] = __float2bfloat16_rn(l == 0.0f ? 0.0f : v / l);
+    if (d == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * kv + kvh) * c.max_rows + r] = l == 0.0f ? CUDART_INF_F : top + log2f(l);
 }
 
-template <int HD, int NG, int NT, int W, bool PLAIN>
+template <int HD, int NG, int NT, bool PLAIN>
 int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
-    using S = Shared<HD, NT, W>;
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
-    auto kernel = attention4_rows_kernel<HD, NG, NT, W, PLAIN>;
-    const int smem = S::bytes(block_bytes(HD, NG));
-    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (p.cluster && p.splits > 8) LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    const dim3 grid(p.splits, c.pages.n_kv_head * p.tiles, c.n_seq);
-    LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, p.cluster ? p.splits : 1, kernel, grid, dim3(W * 32), smem, s, c, p.splits, p.cluster, p.tiles, status));
-    if (p.splits > 1 && !p.cluster) {
-        const dim3 rows(p.rows, c.pages.n_kv_head * p.tiles, c.n_seq);
-        LB_CHECK_CUDA(lb_launch_overlapped(attention4_meet_kernel<HD>, rows, dim3(HD), 0, s, c, p.splits, p.tiles, p.rows));
-    }
+    auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN>;
+    const int smem = kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
+    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1)));
+    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.blocks, (c.n_seq + p.per_row - 1) / p.per_row), dim3(kWarps * 32), smem, s, c, p.per_row, p.tiles, status));
+    LB_CHECK_CUDA(lb_launch_overlapped(attention4_join_kernel<HD>, dim3(c.max_rows, c.pages.n_kv_head, c.n_seq), dim3(HD * p.join_groups), 0, s, c, p.per_row, p.blocks * kWarps, p.tiles, p.rows));
     return LB_OK;
 }
 
 template <int HD, int NG>
 int launch_for(const Call& c, const RowsPlan& p, cudaStream_t s) {
     const bool plain = c.distance == nullptr && c.soft_cap <= 0.0f && c.scores == nullptr;
-    if (p.rows == 8) return plain ? launch<HD, NG, 1, 8, true>(c, p, s) : launch<HD, NG, 1, 8, false>(c, p, s);
-    return plain ? launch<HD, NG, 2, 8, true>(c, p, s) : launch<HD, NG, 2, 8, false>(c, p, s);
+    if (p.rows == 4) return plain ? launch<HD, NG, 1, true>(c, p, s) : launch<HD, NG, 1, false>(c, p, s);
+    if (p.rows == 8) return plain ? launch<HD, NG, 2, true>(c, p, s) : launch<HD, NG, 2, false>(c, p, s);
+    return plain ? launch<HD, NG, 4, true>(c, p, s) : launch<HD, NG, 4, false>(c, p, s);
 }
 
 }  // namespace
 
-RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
-    (void)head_dim;
-    RowsPlan p;
-    p.rows = max_rows > 8 ? 16 : 8;
+int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
+    RowsPlan& p = *plan;
+    p.rows = max_rows > 8 ? 16 : max_rows > 4 ? 8 : 4;
     p.tiles = (max_rows + p.rows - 1) / p.rows;
-    p.warps = 8;
-    // Two blocks an SM; a range of fewer than 128 keys has no work for eight warps.
-    const int64_t work = std::max<int64_t>(1, (int64_t)n_seq * n_kv_head * p.tiles);
-    const int64_t want = std::min<int64_t>((2 * n_sm + work - 1) / work, std::max(1, max_keys / 128));
-    p.splits = want > 16 ? (int)std::min<int64_t>(want, 64) : want > 8 ? 16 : (int)std::max<int64_t>(1, want);
-    p.cluster = p.splits > 1 && p.splits <= 16;
-    return p;
+    // A launch row numbers its tiles in 32 bits.
+    const int64_t units = (int64_t)n_kv_head * p.tiles, most = units * ((max_keys + kBlockKeys - 1) / kBlockKeys);
+    LB_CHECK_ARG(most <= 1 << 30, "attention4: a request of %d rows and %d keys is more than one launch takes", max_rows, max_keys);
+    p.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)std::max(1, n_seq), (int64_t)kMostRequests, ((int64_t)1 << 30) / std::max<int64_t>(1, most)}));
+    const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
+    p.blocks = (int)std::max<int64_t>(1, (warps + kWarps - 1) / kWarps);
+    // Runs that a request's row has at most, about; a group of threads takes some eight of them.
+    const int64_t runs = p.blocks * kWarps / (units * p.per_row) + 2;
+    p.join_groups = 1;
+    while (p.join_groups < 1024 / head_dim && p.join_groups * 8 < runs) p.join_groups *= 2;
+    const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
+    p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 2) * 4;
+    p.starts = rows * (p.per_row + 1) * 4;
+    return LB_OK;
 }
 
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t s) {

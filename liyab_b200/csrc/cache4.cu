@@ -18,6 +18,7 @@ int pages_of(const lb_cache4* c, const char* what, Pages* p) {
     LB_CHECK_ARG(c->page_size >= 16 && c->page_size <= (1 << 20) && (c->page_size & (c->page_size - 1)) == 0, "%s: pages of %d keys (a power of two, 16 or more)", what, c->page_size);
     LB_CHECK_ARG(c->n_pages >= 0 && c->n_kv_head > 0 && c->n_kv_head <= 65535, "%s: %d pages of %d heads", what, c->n_pages, c->n_kv_head);
     LB_CHECK_ARG((int64_t)c->n_pages * c->page_size <= INT32_MAX, "%s: %d pages of %d keys have slots past 32 bits", what, c->n_pages, c->page_size);
+    LB_CHECK_ARG((int64_t)c->n_pages * c->n_kv_head * (c->page_size / 16) <= INT32_MAX, "%s: %d pages of %d heads are more than 2^31 blocks of keys", what, c->n_pages, c->n_kv_head);
     LB_CHECK_ARG((c->memory != nullptr || c->n_pages == 0) && reinterpret_cast<uintptr_t>(c->memory) % 16 == 0, "%s: the cache's memory is missing or not 16-byte aligned", what);
     p->memory = static_cast<uint8_t*>(c->memory);
     p->n_pages = c->n_pages;

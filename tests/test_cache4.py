@@ -17,13 +17,13 @@ def _bytes(*sizes):
     return ops.lib().lb_cache4_bytes(*sizes, C.byref(n)), n.value
 
 
-@pytest.mark.parametrize("pages,kv,dim,page,group", [(1, 1, 64, 16, 32), (7, 25, 64, 16, 64), (100, 8, 128, 128, 32), (100000, 8, 128, 64, 128), (0, 1, 64, 16, 64), (1 << 20, 32, 128, 1024, 64)])
+@pytest.mark.parametrize("pages,kv,dim,page,group", [(1, 1, 64, 16, 32), (7, 25, 64, 16, 64), (100, 8, 128, 128, 32), (100000, 8, 128, 64, 128), (0, 1, 64, 16, 64), (1 << 19, 32, 128, 1024, 64)])
 def test_sizes(pages, kv, dim, page, group):
     assert _bytes(pages, kv, dim, page, group) == (0, pages * kv * page * (dim + 4 * dim // group))
 
 
 @pytest.mark.parametrize("sizes", [(-1, 1, 64, 16, 32), (1, 0, 64, 16, 32), (1, 1, 96, 16, 32), (1, 1, 64, 8, 32), (1, 1, 64, 48, 32), (1, 1, 64, 0, 32), (1, 1, 64, 16, 16), (1, 1, 64, 16, 128),
-                                   (1, 1, 64, 16, 0), (1 << 27, 1, 64, 16, 32), (1, 70000, 64, 16, 32)])
+                                   (1, 1, 64, 16, 0), (1 << 27, 1, 64, 16, 32), (1 << 20, 32, 128, 1024, 64), (1, 70000, 64, 16, 32)])
 def test_sizes_refused(sizes):
     assert _bytes(*sizes)[0] != 0 and ops.lib().lb_last_error()
 
@@ -96,33 +96,35 @@ def test_eviction_refused(change):
     assert ops.lib().lb_evict4(_evict(ref, **change)) != 0 and ops.lib().lb_last_error()
 
 
+def _plan(kv, heads, n_seq, keys, q_len=1, dim=64):
+    c, ref = _cache(kv=kv, dim=dim)
+    got = (C.c_int * 4)()
+    more = dict(q_start=AT, max_q_len=q_len) if q_len > 1 else {}
+    call = _call(ref, n_head=heads, n_seq=n_seq, n_tokens=n_seq * q_len, max_keys=keys, table_stride=-(-keys // 16), q_stride=heads * dim, out_stride=heads * dim, **more)
+    assert ops.lib().lb_attention4_plan(call, got) == 0
+    return tuple(got), ops.lib().lb_attention4_scratch(call)
+
+
 def test_how_attention_is_cut():
-    """Rows a block, and blocks that share a request's keys, by the requests, heads, tokens and keys alone."""
-    def plan(kv, heads, n_seq, keys, q_len=1):
-        c, ref = _cache(kv=kv)
-        got = (C.c_int * 4)()
-        more = dict(q_start=AT, max_q_len=q_len) if q_len > 1 else {}
-        assert ops.lib().lb_attention4_plan(_call(ref, n_head=heads, n_seq=n_seq, n_tokens=n_seq * q_len, max_keys=keys, table_stride=keys // 16, **more), got) == 0
-        return tuple(got)
-    assert plan(25, 25, 64, 1024)[:3] == (0, 8, 1) and plan(8, 128, 64, 1024)[:3] == (0, 16, 1)
-    assert plan(8, 32, 1, 16)[2] == 1                          # no keys to share
-    assert 1 < plan(8, 32, 8, 16384)[2] <= 8 and plan(8, 32, 1, 131072)[2] > 8
-    assert plan(1, 8, 1, 131072)[2] > 16                       # more than a cluster has
+    """Rows a tile, blocks, and requests that share them, by the requests, heads, tokens and keys alone."""
+    assert _plan(25, 25, 64, 1024)[0] == (0, 4, 5 * 148, 64) and _plan(8, 128, 64, 1024, dim=128)[0] == (0, 16, 2 * 148, 64)
+    assert _plan(8, 32, 1, 16)[0][2] == 1                      # eight tiles of keys, two warps' work
+    assert _plan(1, 1, 65535, 1024)[0][3] == 1024              # requests in rows of the launch
+    assert _plan(32, 32, 100, 1 << 27)[0][3] == 4              # a row numbers its tiles in 30 bits
     c, ref = _cache()
     assert ops.lib().lb_attention4_plan(_call(ref), None) != 0
+    assert ops.lib().lb_attention4(_call(ref, n_head=8, max_keys=1 << 30, table_stride=1 << 26, q_start=AT, max_q_len=1 << 14)) != 0
 
 
 def test_scratch():
-    """None but for ranges that meet in memory, and for the keys' weights."""
-    scratch = ops.lib().lb_attention4_scratch
+    """States of all runs (a run more than warps and units together has), where requests' tiles start, and the keys' weights."""
+    (_, rows, blocks, per), got = _plan(8, 32, 4, 1024, dim=128)
+    states, starts = (4 * blocks + 4 * 8) * rows * 130 * 4, 5 * 4
+    assert got == states + -(-starts // 16) * 16
     c, ref = _cache(kv=8, dim=128)
-    assert scratch(_call(ref, n_head=32)) == scratch(_call(ref, n_head=32, table_stride=8192, max_keys=131072)) == 0
-    assert scratch(_call(ref, n_head=32, mass=AT, total=AT)) == 4 * 32 * 1024 * 4 + 4 * 32 * 4
+    scratch = ops.lib().lb_attention4_scratch
+    assert scratch(_call(ref, n_head=32, mass=AT, total=AT)) - scratch(_call(ref, n_head=32)) == 4 * 32 * 1024 * 4 + 4 * 32 * 4
     assert scratch(_call(ref, n_head=7)) == 0                  # a call that is refused
-    c, ref = _cache(kv=1, dim=128)
-    got = (C.c_int * 4)()
-    call = _call(ref, n_head=8, n_seq=1, n_tokens=1, table_stride=8192, max_keys=131072)
-    assert ops.lib().lb_attention4_plan(call, got) == 0 and scratch(call) == got[2] * got[1] * 130 * 4
 
 
 def test_ops_refuse_memory_that_is_not_on_a_gpu():

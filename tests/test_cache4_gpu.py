@@ -83,6 +83,10 @@ def _attention(q, k, v, places, scale, window=0, distance=None, sink=None, cap=0
         # Sums of 16 products at a time, each with an error below 2^-23 of the sum of the terms' sizes; the scales, the cap and the penalty add a few roundings of their own terms.
         size = (q[:, h].double().abs() @ kh.abs().T * abs(scale)).amax(1) if keys else torch.zeros(tokens, dtype=F64, device=q.device)
         error = (dim / 16 + 16) * 2.0 ** -23 * size
+        # A row of queries is rounded to 16 bits in steps of at most 2^-14 of its largest value: what has more of bfloat16's eight bits below that is off by up to half a step.
+        if keys:
+            large = q[:, h].double().abs().amax(1, keepdim=True)
+            error = error + ((q[:, h].double().abs() < large * 2.0 ** -6).double() * large * 2.0 ** -15 @ kh.abs().T * abs(scale)).amax(1)
         if cap > 0:
             z = cap * torch.tanh(z / cap)
             error = error + 16 * 2.0 ** -23 * cap
