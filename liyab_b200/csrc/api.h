@@ -836,7 +836,7 @@ typedef struct {
 /* The bytes of the memory of a cache of these sizes. */
 int lb_cache4_bytes(int n_pages, int n_kv_head, int head_dim, int page_size, int group, int64_t* bytes);
 /* Rounds the rows k[t], v[t] (float32 or bfloat16, n_kv_head * head_dim values, row strides ldk and ldv) to 4 bits at slot_mapping[t] (negative: skipped; the slots of a call
- * differ): s = bfloat16(max |x| of a group / 7), n = x / s rounded to the nearest even and clamped to -8 .. 7; a group that holds an infinity or a NaN gets s = NaN. */
+ * differ): s = bfloat16(max |x| of a group / 7), n = x / s (in 32 bits) rounded to the nearest even and clamped to -8 .. 7; a group that holds an infinity or a NaN gets s = NaN. */
 int lb_append4(int dtype, const void* k, int64_t ldk, const void* v, int64_t ldv, const int32_t* slot_mapping, const lb_cache4* cache, int n_tokens, void* stream);
 /* The rows at slots[i] as float32 or bfloat16 values (negative slots: the row is left alone). */
 int lb_cache4_values(int dtype, const lb_cache4* cache, const int32_t* slots, int n, void* k, int64_t ldk, void* v, int64_t ldv, void* stream);

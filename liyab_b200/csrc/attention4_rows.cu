@@ -119,7 +119,7 @@ template <int HD, int NG, int NT, bool PLAIN>
 __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD, NT))
 attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
-    constexpr int kRows = 4 * NT, kState = HD + 2;
+    constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, two places, the values
     constexpr int JK = HD / 32, JV = HD / 64;             // words of a lane: of a key, of a value row
     constexpr int kBlock = block_bytes(HD, NG);
     // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
@@ -268,21 +268,21 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             // (A largest value of eight ones, 32,640 of 2^15, would have a high digit of 128: it goes a bit lower.)  A row that is not finite has NaN for a factor.
             const int shift = top == 0 || top >= 0x7f80u ? 0 : 14 - (max((int)(top >> 7), 1) - 127) - ((top & 0x7fu) == 0x7fu);
             const float up = pow2(shift / 2), up2 = pow2(shift - shift / 2);
+            // x 2^shift + 1.5 2^23 has the 16 bits below: byte 0 is the low digit, byte 1, with the carry of a negative low one, the high digit.
+            const uint32_t carry = (g & 1) != 0 ? 0u : 0x80u, pick = (g & 1) != 0 ? 0x40u : 0x51u;
             int sums[JK];
 #pragma unroll
             for (int j = 0; j < JK; ++j) {
-                int digit[8];
-                sums[j] = 0;
+                uint32_t v[8];
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     const float x = __uint_as_float((d & 1) != 0 ? u[j][d / 2] & 0xffff0000u : u[j][d / 2] << 16);
-                    const int v = top >= 0x7f80u ? 0 : __float2int_rn(x * up * up2), low = (int)(int8_t)v;
-                    digit[d] = (g & 1) != 0 ? low : (v - low) >> 8;
-                    sums[j] += digit[d];
+                    v[d] = __float_as_uint(fmaf(top >= 0x7f80u ? 0.0f : x * up, up2, kMagic)) + carry;
                 }
-                auto four = [&](int a, int b, int cc, int dd) { return (digit[a] & 255) | (digit[b] & 255) << 8 | (digit[cc] & 255) << 16 | (uint32_t)(digit[dd] & 255) << 24; };
+                auto four = [&](int a, int b, int cc, int dd) { return __byte_perm(__byte_perm(v[a], v[b], pick), __byte_perm(v[cc], v[dd], pick), 0x5410u); };
                 qd[n][j][0] = four(0, 4, 1, 5);                 // nibbles 0, 2, 4, 6
                 qd[n][j][1] = four(2, 6, 3, 7);                 // nibbles 1, 3, 5, 7
+                sums[j] = __dp4a((int)qd[n][j][0], 0x01010101, __dp4a((int)qd[n][j][1], 0x01010101, 0));
                 sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
                 sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
             }
@@ -512,7 +512,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int gr = (64 * j + 32 * (k >> 1)) / (HD / NG), e = NT == 1 ? gr & 1 : n & 1;
-                    *reinterpret_cast<float2*>(to + 2 + 64 * j + 32 * (k >> 1) + 4 * g + 2 * (k & 1)) = make_float2(o[n / 2][j * 4 + k][e], o[n / 2][j * 4 + k][e + 2]);
+                    *reinterpret_cast<float2*>(to + 4 + 64 * j + 32 * (k >> 1) + 4 * g + 2 * (k & 1)) = make_float2(o[n / 2][j * 4 + k][e], o[n / 2][j * 4 + k][e + 2]);
                 }
         }
     }
@@ -523,60 +523,86 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     }
 }
 
-// Joins the states of a row's runs, in their order within each of the block's groups of HD threads, the groups' in theirs.
+// Joins the states of the rows' runs.  A team of warps (1 to 32) has a row, a lane HD / 32 neighbouring values; the warps take the runs in turn, and their sums meet in their order.
 template <int HD>
 __global__ void __launch_bounds__(1024)
-attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int tile_rows) {
-    constexpr int kState = HD + 2;
-    __shared__ float joined[1024 / HD][kState];
+attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int rows_shift, int team_shift) {
+    constexpr int V = HD / 32, kState = HD + 4;
+    __shared__ float joined[32][HD + 2];
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq / per_row, s = seq - row_of * per_row;
-    const int r = blockIdx.x, d = threadIdx.x % HD, group = threadIdx.x / HD, n_groups = blockDim.x / HD;
+    const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row, team = 1 << team_shift;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp & (team - 1), r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (warp >> team_shift);
     const Portion part = portion_of(c, seq);
-    if (r >= part.count * c.per) return;
-    const int row_tile = r / tile_rows, in_row = c.q_start == nullptr ? tiles : (part.count * c.per + tile_rows - 1) / tile_rows;
-    const int* starts = c.starts + (int64_t)row_of * (per_row + 1);
-    const int start = starts[s], count = (starts[s + 1] - start) / (kv * in_row), n_seq = min(per_row, c.n_seq - row_of * per_row);
-    const int from = start + (kvh * in_row + row_tile) * count, share = share_of(starts[n_seq], n_warps);
-    const int first = count > 0 ? from / share : 0, runs = count > 0 ? (from + count - 1) / share - first + 1 : 0;
-    const float* state = c.partial + (((int64_t)row_of * (n_warps + (int64_t)per_row * kv * tiles) + first + ((int64_t)s * kv + kvh) * tiles + row_tile) * tile_rows + r - row_tile * tile_rows) *
-                                         kState;
-    const int64_t step = (int64_t)tile_rows * kState;
-    float m = kLowest, l = 0.0f, v = 0.0f;
+    const bool there = r < part.count * c.per;
+    float m = kLowest, l = 0.0f, v[V] = {};
+    if (there) {
+        const int row_tile = r >> rows_shift, in_row = c.q_start == nullptr ? tiles : ((part.count * c.per - 1) >> rows_shift) + 1;
+        const int* starts = c.starts + (int64_t)row_of * (per_row + 1);
+        const int start = starts[s], units = kv * in_row, n_seq = min(per_row, c.n_seq - row_of * per_row), share = share_of(starts[n_seq], n_warps);
+        const int count = units == 1 ? starts[s + 1] - start : (starts[s + 1] - start) / units;
+        const int from = start + (kvh * in_row + row_tile) * count;
+        const int first = from / share, runs = count > 0 ? (from + count - 1) / share - first + 1 : 0;
+        const float* state = c.partial + (((((int64_t)row_of * (n_warps + (int64_t)per_row * kv * tiles) + first + ((int64_t)s * kv + kvh) * tiles + row_tile) << rows_shift) + r - (row_tile << rows_shift)) *
+                                          kState);
+        const int step = kState << rows_shift;
+        // Thirty-two runs at a time: a lane has a run's reference and sum, and its factor once the largest reference is known.
+        for (int i0 = mine; i0 < runs; i0 += 32 * team) {
+            float2 ml = make_float2(kLowest, 0.0f);
+            if (i0 + lane * team < runs) ml = *reinterpret_cast<const float2*>(state + (int64_t)(i0 + lane * team) * step);
+            const bool some = ml.y != 0.0f;                 // (a NaN is some)
+            float high = some ? ml.x : kLowest;
+#pragma unroll
+            for (int x = 16; x > 0; x /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+            high = fmaxf(high, m);
+            const float w = some ? ex2(ml.x - high) : 0.0f, keep = ex2(m - high);
+            l = fmaf(l, keep, lb_warp_sum(some ? ml.y * w : 0.0f));
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] *= keep;
+            m = high;
+            const int n = min(32, (runs - i0 + team - 1) >> team_shift);
+            const float* at = state + (int64_t)i0 * step + 4 + V * lane;
 #pragma unroll 4
-    for (int i = group; i < runs; i += n_groups) {
-        const float2 ml = *reinterpret_cast<const float2*>(state + i * step);
-        const float o = state[i * step + 2 + d];
-        const float top = ml.y == 0.0f ? m : fmaxf(m, ml.x), w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - top), keep = exp2f(m - top);
-        l = fmaf(l, keep, ml.y * w);
-        v = fmaf(v, keep, o * w);
-        m = top;
+            for (int x = 0; x < n; ++x, at += (int64_t)team * step) {
+                const float f = __shfl_sync(0xffffffffu, w, x);
+                float o[V];
+                if constexpr (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(at);
+                else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(at);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = f == 0.0f ? v[e] : fmaf(o[e], f, v[e]);
+            }
+        }
     }
-    if (n_groups > 1) {
-        joined[group][2 + d] = v;
-        if (d == 0) {
-            joined[group][0] = m;
-            joined[group][1] = l;
+    if (team > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) joined[warp][2 + V * lane + e] = v[e];
+        if (lane == 0) {
+            joined[warp][0] = m;
+            joined[warp][1] = l;
         }
         __syncthreads();
-        if (group > 0) return;
-        for (int i = 1; i < n_groups; ++i) {
-            const float mi = joined[i][0], li = joined[i][1], top = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : exp2f(mi - top), keep = exp2f(m - top);
+        if (mine > 0) return;
+        for (int i = 1; i < team; ++i) {
+            const float mi = joined[warp + i][0], li = joined[warp + i][1], high = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : ex2(mi - high), keep = ex2(m - high);
             l = fmaf(l, keep, li * w);
-            v = fmaf(v, keep, joined[i][2 + d] * w);
-            m = top;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = fmaf(v[e], keep, joined[warp + i][2 + V * lane + e] * w);
+            m = high;
         }
     }
-    const int head = kvh * c.per + r % c.per;
-    float top = m;
+    if (!there) return;
+    const int token = part.count == 1 ? 0 : r / c.per, head = kvh * c.per + r - token * c.per;
+    float top = m, factor = 1.0f;
     if (c.sink != nullptr) {
         const float sink = c.sink[head] * kLbLog2e;
         top = fmaxf(m, sink);
-        v *= lb_sink_join_exp2(sink, m, l);
+        factor = lb_sink_join_exp2(sink, m, l);
     }
-    c.out[(int64_t)(part.first + r / c.per) * c.out_stride + head * HD + d] = __float2bfloat16_rn(l == 0.0f ? 0.0f : v / l);
-    if (d == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * kv + kvh) * c.max_rows + r] = l == 0.0f ? CUDART_INF_F : top + log2f(l);
+    factor = l == 0.0f ? 0.0f : __fdividef(factor, l);
+    __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + head * HD + V * lane;
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = __float2bfloat16_rn(v[e] * factor);
+    if (lane == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * kv + kvh) * c.max_rows + r] = l == 0.0f ? CUDART_INF_F : top + log2f(l);
 }
 
 template <int HD, int NG, int NT, bool PLAIN>
@@ -587,7 +613,12 @@ int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     const int smem = kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
     LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1)));
     LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.blocks, (c.n_seq + p.per_row - 1) / p.per_row), dim3(kWarps * 32), smem, s, c, p.per_row, p.tiles, status));
-    LB_CHECK_CUDA(lb_launch_overlapped(attention4_join_kernel<HD>, dim3(c.max_rows, c.pages.n_kv_head, c.n_seq), dim3(HD * p.join_groups), 0, s, c, p.per_row, p.blocks * kWarps, p.tiles, p.rows));
+    // Blocks of four warps or more, but no warps past the rows.
+    int join_warps = p.join_team;
+    while (join_warps < 4 && join_warps < c.max_rows * p.join_team) join_warps *= 2;
+    const int teams = join_warps / p.join_team;
+    LB_CHECK_CUDA(lb_launch_overlapped(attention4_join_kernel<HD>, dim3((c.max_rows + teams - 1) / teams, c.pages.n_kv_head, c.n_seq), dim3(32 * join_warps), 0, s, c, p.per_row,
+                                       p.blocks * kWarps, p.tiles, __builtin_ctz((unsigned)p.rows), __builtin_ctz((unsigned)p.join_team)));
     return LB_OK;
 }
 
@@ -611,12 +642,12 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     p.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)std::max(1, n_seq), (int64_t)kMostRequests, ((int64_t)1 << 30) / std::max<int64_t>(1, most)}));
     const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
     p.blocks = (int)std::max<int64_t>(1, (warps + kWarps - 1) / kWarps);
-    // Runs that a request's row has at most, about; a group of threads takes some eight of them.
+    // Runs that a row has, about; a warp takes some eight of them.
     const int64_t runs = p.blocks * kWarps / (units * p.per_row) + 2;
-    p.join_groups = 1;
-    while (p.join_groups < 1024 / head_dim && p.join_groups * 8 < runs) p.join_groups *= 2;
+    p.join_team = 1;
+    while (p.join_team < 32 && p.join_team * 8 < runs) p.join_team *= 2;
     const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
-    p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 2) * 4;
+    p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
     return LB_OK;
 }

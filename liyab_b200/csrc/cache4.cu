@@ -1,6 +1,6 @@
 // The 4-bit cache's own work: rows in, values out, and eviction.
 //
-// append4 and cache4_values move each value once and are bound by memory; a thread has a word (eight values) of a row, in the order of cache4.cuh.
+// append4 and cache4_values move each value once; sixteen threads have a row, in the order of cache4.cuh.
 // evict4 is two launches.  The first chooses: a block a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  The
 // second copies: a warp a block of sixteen keys of the destination, whose pieces it gathers.  The destination is never a source, so nothing waits for anything.
@@ -35,7 +35,7 @@ namespace {
 
 using namespace lb_c4;
 
-// `count` (4 or 8) neighbouring values of a row.
+// N (4 or 8) neighbouring values of a row.
 template <typename T, int N>
 __device__ __forceinline__ void load_values(const T* p, bool wide, float* v) {
     if (wide) {
@@ -43,13 +43,13 @@ __device__ __forceinline__ void load_values(const T* p, bool wide, float* v) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(p + i);
         } else {
+            uint32_t u[N / 2];
+            if constexpr (N == 8) *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(p);
+            else *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const uint2 u = *reinterpret_cast<const uint2*>(p + i);
-                v[i] = __uint_as_float(u.x << 16);
-                v[i + 1] = __uint_as_float(u.x & 0xffff0000u);
-                v[i + 2] = __uint_as_float(u.y << 16);
-                v[i + 3] = __uint_as_float(u.y & 0xffff0000u);
+            for (int i = 0; i < N / 2; ++i) {
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         }
     } else {
@@ -59,92 +59,122 @@ __device__ __forceinline__ void load_values(const T* p, bool wide, float* v) {
 }
 
 // max |v| as an integer that orders like it, a NaN above all.
-__device__ __forceinline__ uint32_t size_of(const float* v, int n) {
+template <int N>
+__device__ __forceinline__ uint32_t size_of(const float* v) {
     uint32_t top = 0;
-    for (int i = 0; i < n; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     return top;
 }
 
 // The scale of a group whose largest |x| this is, bfloat16(x / 7); the rounding that follows divides by what was stored.
+template <typename T>
 __device__ __forceinline__ __nv_bfloat16 group_scale(uint32_t top) {
-    return __float2bfloat16_rn(top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 7.0f) : CUDART_NAN_F);
-}
-__device__ __forceinline__ uint32_t nibble(float x, float s) {
-    const float r = s > 0.0f ? rintf(__fdiv_rn(x, s)) : 0.0f;            // a scale of 0 or NaN: 0
-    return (uint32_t)((int)fminf(fmaxf(r, -8.0f), 7.0f) + 8);
+    const float a = __uint_as_float(top);
+    if (top >= 0x7f800000u) return __float2bfloat16_rn(CUDART_NAN_F);
+    // A bfloat16 number over seven is never within 2^-12 of the middle of two bfloat16 numbers (seven times a middle has nine bits or more and is odd), so the product with 1 / 7 rounds alike.
+    if (sizeof(T) == 2 && top >= 0x04000000u) return __float2bfloat16_rn(a * 0.14285715f);
+    return __float2bfloat16_rn(__fdiv_rn(a, 7.0f));
 }
 
-// A thread a word: threads are [token][head][K words, V words].
-template <typename T, int HD>
+// Eight values over their scales (the first four over s0), the quotients rounded to 32 bits and then to the nearest even integer, as nibbles n + 8.  VALUES: nibble n is value
+// 4 (n % 4 / 2) + 2 (n % 2) + n / 4, else 2 (n % 4) + n / 4.  The quotient is x r corrected by its rest times r, r the scale's rounded reciprocal (Markstein's division, correctly rounded): six
+// operations a value with the rounding (adding 1.5 2^23) and the place in the word (four numbers -7 .. 7 in base 16).  |x| is at most 7.03 s as long as s is a normal number.
+template <bool VALUES>
+__device__ __forceinline__ uint32_t eight_nibbles(const float* x, float s0, float s1) {
+    constexpr float kMagic = 12582912.0f;
+    auto value_at = [](int n) { return VALUES ? 4 * ((n & 3) >> 1) + 2 * (n & 1) + (n >> 2) : 2 * (n & 3) + (n >> 2); };
+    if (s0 >= 0x1p-90f && s1 >= 0x1p-90f) {
+        const float r0 = __frcp_rn(s0), r1 = __frcp_rn(s1);
+        float half[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int n = 7; n >= 0; --n) {
+            const int d = value_at(n);
+            const float s = d < 4 ? s0 : s1, r = d < 4 ? r0 : r1, q = x[d] * r;
+            half[n >> 2] = fmaf(half[n >> 2], 16.0f, fmaf(fmaf(-q, s, x[d]), r, q) + kMagic - kMagic);
+        }
+        const uint32_t lo = __float_as_uint(half[0] + (kMagic + 34952.0f)), hi = __float_as_uint(half[1] + (kMagic + 34952.0f));         // 8 added to each: 0x8888
+        return __byte_perm(lo, hi, 0x5410);
+    }
+    uint32_t word = 0;                                     // scales of 0, NaN, or with a reciprocal past float32's range
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const int d = value_at(n);
+        const float s = d < 4 ? s0 : s1, q = s > 0.0f ? rintf(__fdiv_rn(x[d], s)) : 0.0f;
+        word |= (uint32_t)((int)fminf(fmaxf(q, -8.0f), 7.0f) + 8) << (4 * n);
+    }
+    return word;
+}
+
+// Eight threads have a row of keys, the next eight its values: HD / 64 words each.
+template <int HD>
+struct Share {
+    static constexpr int kWords = HD / 64, kRowThreads = 16, kBlockRows = 256 / kRowThreads;
+    // The first dim of word i's first, and of its second four values; r: the thread of the eight.
+    __device__ static int dim(int of, int r, int i, int second) {
+        return of == 0 ? 32 * ((r >> 2) * kWords + i) + 8 * (r & 3) + 4 * second : 64 * i + 32 * second + 4 * r;
+    }
+    __device__ static int place(int of, int key, int r, int i) {
+        return of == 0 ? Layout<HD>::k_word(key, 4 * ((r >> 2) * kWords + i) + (r & 3)) : Layout<HD>::v_word(key, r, i);
+    }
+};
+
+template <typename T, int HD, int NG>
 __global__ void __launch_bounds__(256)
 append4_kernel(const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv, const int32_t* __restrict__ slot_mapping, const Pages pages, int n_tokens, int wide) {
     using L = Layout<HD>;
-    constexpr int W = L::kWords;
+    using S = Share<HD>;
+    constexpr int W = S::kWords, group = HD / NG;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, row = id / (2 * W);
-    const int w = (int)(id % W), of = (int)(id / W & 1);
-    const int head = (int)(row % pages.n_kv_head);
-    const int64_t token = row / pages.n_kv_head;
+    const int row = blockIdx.x * S::kBlockRows + threadIdx.x / S::kRowThreads, of = threadIdx.x >> 3 & 1, r = threadIdx.x & 7;
+    const int token = row / pages.n_kv_head, head = row - token * pages.n_kv_head;
     // The threads of a row are neighbours in one warp; those past the end and those of skipped rows go along with the shuffles.
     const int slot = token < n_tokens ? slot_mapping[token] : -1;
     const bool there = slot >= 0 && slot >> pages.page_shift < pages.n_pages;
-    float x[8] = {};
-    uint32_t a, b;                                     // the largest of its values in the first, and in the second group that it touches
-    const int g = w & 7, j = w >> 3;
-    if (of == 0) {
-        if (there) load_values<T, 8>(k + token * ldk + head * HD + 8 * w, wide, x);
-        a = b = size_of(x, 8);
-    } else {
-        if (there) {
-            load_values<T, 4>(v + token * ldv + head * HD + 64 * j + 4 * g, wide, x);
-            load_values<T, 4>(v + token * ldv + head * HD + 64 * j + 32 + 4 * g, wide, x + 4);
+    float x[W][8] = {};
+    uint32_t top[W][2];                                    // of a word's first, and of its second four values
+    const T* from = (of == 0 ? k + (int64_t)token * ldk : v + (int64_t)token * ldv) + head * HD;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (there) load_values<T, 4>(from + S::dim(of, r, i, e), wide, x[i] + 4 * e);
+            top[i][e] = size_of<4>(x[i] + 4 * e);
         }
-        a = size_of(x, 4);
-        b = size_of(x + 4, 4);
+    // Keys: a word lies in one group of 32, which four threads share; two words of a thread, or those of the other four, make groups of 64.  Values: a word's halves lie in two groups of 32,
+    // which the eight threads share.
+    if (of == 0 || group > 32) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) top[i][0] = top[i][1] = max(top[i][0], top[i][1]);
     }
-    auto meet = [&](int distance) {
-        a = max(a, __shfl_xor_sync(0xffffffffu, a, distance));
-        b = max(b, __shfl_xor_sync(0xffffffffu, b, distance));
-    };
-    const int group = HD / pages.groups;
-    meet(1);
-    meet(2);
-    // Eight threads of values have two groups of 32 between them, of keys one of 64.
-    const uint32_t a4 = a, b4 = b;
-    meet(4);
-    if (of == 0) {
-        if (group == 32) a = b = a4;
-        (void)b4;
-    } else if (group != 32) {
-        a = b = max(a, b);
-    }
-    if constexpr (HD == 128) {
-        const uint32_t far = __shfl_xor_sync(0xffffffffu, a, 8);
-        if (group == 128) a = b = max(a, far);
-    }
+    if (W == 2 && (group == 128 || (group == 64 && of == 0))) top[0][0] = top[0][1] = top[W - 1][0] = top[W - 1][1] = max(top[0][0], top[W - 1][0]);
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (group > 32 && e == 1) {
+                top[i][1] = top[i][0];
+                continue;
+            }
+            uint32_t a = top[i][e];
+            a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+            a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+            const uint32_t far = __shfl_xor_sync(0xffffffffu, a, 4);
+            top[i][e] = of == 1 || group == HD ? max(a, far) : a;
+        }
     if (!there) return;
-    const __nv_bfloat16 sa = group_scale(a), sb = group_scale(b);
-    const float fa = __bfloat162float(sa), fb = __bfloat162float(sb);
     uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
     const int key = slot & 15;
-    uint32_t word = 0;
-    __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(block + L::scale(key, pages.groups, of));
-    if (of == 0) {
+    __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(block + L::scale(key, NG, of));
 #pragma unroll
-        for (int d = 0; d < 8; ++d) word |= nibble(x[d], fa) << (4 * (d / 2 + 4 * (d % 2)));
-        *reinterpret_cast<uint32_t*>(block + L::k_word(key, w)) = word;
-        if (8 * w % group == 0) scales[8 * w / group] = sa;
-    } else {
-        // Nibble n is value 2 (n % 2) + n / 4 of the four in the first (n % 4 < 2) or the second group.
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const int second = (n & 3) >> 1;
-            word |= nibble(x[4 * second + 2 * (n & 1) + (n >> 2)], second != 0 ? fb : fa) << (4 * n);
-        }
-        *reinterpret_cast<uint32_t*>(block + L::v_word(key, g, j)) = word;
-        if (g == 0 && 64 * j % group == 0) scales[64 * j / group] = sa;
-        if (g == 0 && group == 32) scales[2 * j + 1] = sb;
+    for (int i = 0; i < W; ++i) {
+        const __nv_bfloat16 sa = group_scale<T>(top[i][0]), sb = group > 32 ? sa : group_scale<T>(top[i][1]);
+        const float fa = __bfloat162float(sa), fb = __bfloat162float(sb);
+        *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, i)) = of == 0 ? eight_nibbles<false>(x[i], fa, fa) : eight_nibbles<true>(x[i], fa, fb);
+        const int da = S::dim(of, r, i, 0), db = S::dim(of, r, i, 1);
+        if (da % group == 0) scales[da / group] = sa;
+        if (of == 1 && group == 32 && db % group == 0) scales[db / group] = sb;
     }
 }
 
@@ -163,47 +193,42 @@ __device__ __forceinline__ void store4(T* p, bool wide, const float* v) {
     }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int NG>
 __global__ void __launch_bounds__(256)
 cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv, int wide) {
     using L = Layout<HD>;
-    constexpr int W = L::kWords;
+    using S = Share<HD>;
+    constexpr int W = S::kWords, group = HD / NG;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, row = id / (2 * W);
-    const int w = (int)(id % W), of = (int)(id / W & 1), head = (int)(row % pages.n_kv_head);
-    const int64_t i = row / pages.n_kv_head;
+    const int row = blockIdx.x * S::kBlockRows + threadIdx.x / S::kRowThreads, of = threadIdx.x >> 3 & 1, r = threadIdx.x & 7;
+    const int i = row / pages.n_kv_head, head = row - i * pages.n_kv_head;
     if (i >= n) return;
     const int slot = slots[i];
     if (slot < 0 || slot >> pages.page_shift >= pages.n_pages) return;
     const uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
-    const int key = slot & 15, group = HD / pages.groups, g = w & 7, j = w >> 3;
-    const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(block + L::scale(key, pages.groups, of));
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(block + (of == 0 ? L::k_word(key, w) : L::v_word(key, g, j)));
-    float x[8];
-    if (of == 0) {
-        const float s = __bfloat162float(scales[8 * w / group]);
+    const int key = slot & 15;
+    const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(block + L::scale(key, NG, of));
+    T* to = (of == 0 ? k + (int64_t)i * ldk : v + (int64_t)i * ldv) + head * HD;
+    uint32_t word[W];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) x[d] = (float)((int)(word >> (4 * (d / 2 + 4 * (d % 2))) & 15u) - 8) * s;
-        T* to = k + i * ldk + head * HD + 8 * w;
-        store4(to, wide, x);
-        store4(to + 4, wide, x + 4);
-    } else {
-        const float sa = __bfloat162float(scales[64 * j / group]), sb = __bfloat162float(scales[(64 * j + 32) / group]);
+    for (int j = 0; j < W; ++j) word[j] = *reinterpret_cast<const uint32_t*>(block + S::place(of, key, r, j));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int second = e >> 2, d = e & 3, nib = 2 * second + (d >> 1) + 4 * (d & 1);
-            x[e] = (float)((int)(word >> (4 * nib) & 15u) - 8) * (second != 0 ? sb : sa);
-        }
-        T* to = v + i * ldv + head * HD + 64 * j + 4 * g;
-        store4(to, wide, x);
-        store4(to + 32, wide, x + 4);
+    for (int j = 0; j < W; ++j) {
+        const int da = S::dim(of, r, j, 0), db = S::dim(of, r, j, 1);
+        const float sa = __bfloat162float(scales[da / group]), sb = group > 32 ? sa : __bfloat162float(scales[db / group]);
+        // Value d of a word is nibble d / 2 + 4 (d % 2), of keys and of values.  1.5 2^23 + n + 8, less that and 8.
+        float x[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) x[d] = (__uint_as_float((word[j] >> (4 * (d / 2 + 4 * (d % 2))) & 15u) | 0x4b400000u) - 12582920.0f) * (d < 4 ? sa : sb);
+        store4(to + da, wide, x);
+        store4(to + db, wide, x + 4);
     }
 }
 
 // ---- eviction ----
 
-constexpr int kChoiceThreads = 1024, kBins = 2048;
+constexpr int kChoiceThreads = 1024, kBins = 2048, kMostHeld = 49152;
 
 // Floats as integers of the same order; -0 is 0, a NaN the largest.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -223,7 +248,8 @@ struct Choice {
 };
 
 __global__ void __launch_bounds__(kChoiceThreads)
-evict4_choose_kernel(const Choice c) {
+evict4_choose_kernel(const Choice c, int held) {
+    extern __shared__ uint32_t keys_s[];       // the first `held` keys' weights as ordered integers
     __shared__ uint32_t bins[kBins];
     __shared__ uint32_t sums[32];
     __shared__ uint32_t found[2];              // the bin that holds the last key to stay, and how many of it stay
@@ -238,7 +264,18 @@ evict4_choose_kernel(const Choice c) {
     float* dest = c.dest_mass != nullptr && (unsigned)r < (unsigned)c.n_dest_mass ? c.dest_mass + (int64_t)r * c.dest_stride + (int64_t)head * c.dest_head_stride : nullptr;
     const int stay = min(n, c.keep), old = n - min(c.recent, n);
     const int by_weight = stay - (n - old);           // of the `old` first keys; recent <= keep, so never negative
-    auto key_at = [&](int i) { return weighed ? ordered(mass[i]) : 0u; };
+    for (int i0 = threadIdx.x; i0 < min(old, held); i0 += 4 * kChoiceThreads) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = weighed && i0 + j * kChoiceThreads < old ? mass[i0 + j * kChoiceThreads] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j * kChoiceThreads < min(old, held)) keys_s[i0 + j * kChoiceThreads] = ordered(v[j]);
+    }
+    __syncthreads();
+    auto key_at = [&](int i) { return i < held ? keys_s[i] : weighed ? ordered(mass[i]) : 0x80000000u; };
+    // The sum of what the warps before this one left.
+    auto before = [&](const uint32_t* of_warps) { return __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[lane] : 0u); };
     // The by_weight-th largest key among the first `old`: `above` its prefix so far, `left` how many keys with that prefix stay.
     uint32_t threshold = 0, left = (uint32_t)by_weight;
     if (by_weight < old && by_weight > 0) {
@@ -248,9 +285,14 @@ evict4_choose_kernel(const Choice c) {
             low -= bits;
             for (int i = threadIdx.x; i < kBins; i += kChoiceThreads) bins[i] = 0;
             __syncthreads();
-            for (int i = threadIdx.x; i < old; i += kChoiceThreads) {
-                const uint32_t key = key_at(i);
-                if (pass == 0 || key >> high == threshold >> high) atomicAdd(&bins[key >> low & ((1u << bits) - 1u)], 1u);
+            for (int i0 = 0; i0 < old; i0 += kChoiceThreads) {
+                const int i = i0 + threadIdx.x;
+                const uint32_t key = i < old ? key_at(i) : 0u;
+                const bool counts = i < old && (pass == 0 || key >> high == threshold >> high);
+                // Many weights are 0: the warp's enter with one addition.
+                const uint32_t zeros = __ballot_sync(0xffffffffu, counts && key == 0x80000000u);
+                if (counts && key != 0x80000000u) atomicAdd(&bins[key >> low & ((1u << bits) - 1u)], 1u);
+                if (zeros != 0 && lane == 0) atomicAdd(&bins[0x80000000u >> low & ((1u << bits) - 1u)], (uint32_t)__popc(zeros));
             }
             __syncthreads();
             // Two bins a thread, from the largest down: how many keys lie in larger bins.
@@ -258,13 +300,12 @@ evict4_choose_kernel(const Choice c) {
             const uint32_t b0 = bins[top], b1 = bins[top - 1];
             uint32_t sum = b0 + b1;
             for (int o = 1; o < 32; o *= 2) {
-                const uint32_t before = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += before;
+                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
             }
             if (lane == 31) sums[warp] = sum;
             __syncthreads();
-            uint32_t larger = sum - b0 - b1;
-            for (int i = 0; i < warp; ++i) larger += sums[i];
+            const uint32_t larger = sum - b0 - b1 + before(sums);
             if (larger < left && left <= larger + b0) {
                 found[0] = (uint32_t)top;
                 found[1] = left - larger;
@@ -298,11 +339,7 @@ evict4_choose_kernel(const Choice c) {
         bins[32 + warp] = at;
     }
     __syncthreads();
-    uint32_t place = 0, ties = 0;
-    for (int i = 0; i < warp; ++i) {
-        place += bins[i];
-        ties += bins[32 + i];
-    }
+    uint32_t place = before(bins), ties = before(bins + 32);
     place += min(ties, left);
     for (int i0 = from; i0 < to; i0 += 32) {
         const int i = i0 + lane;
@@ -387,18 +424,20 @@ bool wide_rows(const void* p, int64_t ld, int bytes) { return reinterpret_cast<u
 template <typename T>
 int append_rows(const T* k, int64_t ldk, const T* v, int64_t ldv, const int32_t* slots, const Pages& pages, int hd, int n, cudaStream_t s) {
     const int wide = wide_rows(k, ldk, sizeof(T)) && wide_rows(v, ldv, sizeof(T));
-    const int64_t threads = (int64_t)n * pages.n_kv_head * 2 * (hd / 8), blocks = (threads + 255) / 256;
-    LB_CHECK_ARG(blocks <= INT32_MAX, "append4: %d tokens are more than one launch takes", n);
-    LB_CHECK_CUDA(lb_launch_overlapped(hd == 128 ? append4_kernel<T, 128> : append4_kernel<T, 64>, dim3((unsigned)blocks), dim3(256), 0, s, k, ldk, v, ldv, slots, pages, n, wide));
+    LB_CHECK_ARG((int64_t)n * pages.n_kv_head <= INT32_MAX - 256, "append4: %d tokens are more than one launch takes", n);
+    const int blocks = (n * pages.n_kv_head + 15) / 16;                  // a block has sixteen rows
+    LB_CHECK_CUDA(lb_launch_overlapped(hd == 64 ? (pages.groups == 1 ? append4_kernel<T, 64, 1> : append4_kernel<T, 64, 2>)
+                                       : pages.groups == 1 ? append4_kernel<T, 128, 1> : pages.groups == 2 ? append4_kernel<T, 128, 2> : append4_kernel<T, 128, 4>, dim3((unsigned)blocks), dim3(256), 0, s, k, ldk, v, ldv, slots, pages, n, wide));
     return LB_OK;
 }
 
 template <typename T>
 int value_rows(const Pages& pages, const int32_t* slots, int n, T* k, int64_t ldk, T* v, int64_t ldv, int hd, cudaStream_t s) {
     const int wide = wide_rows(k, ldk, sizeof(T)) && wide_rows(v, ldv, sizeof(T));
-    const int64_t threads = (int64_t)n * pages.n_kv_head * 2 * (hd / 8), blocks = (threads + 255) / 256;
-    LB_CHECK_ARG(blocks <= INT32_MAX, "cache4_values: %d rows are more than one launch takes", n);
-    LB_CHECK_CUDA(lb_launch_overlapped(hd == 128 ? cache4_values_kernel<T, 128> : cache4_values_kernel<T, 64>, dim3((unsigned)blocks), dim3(256), 0, s, pages, slots, n, k, ldk, v, ldv,
+    LB_CHECK_ARG((int64_t)n * pages.n_kv_head <= INT32_MAX - 256, "cache4_values: %d rows are more than one launch takes", n);
+    const int blocks = (n * pages.n_kv_head + 15) / 16;                  // a block has sixteen rows
+    LB_CHECK_CUDA(lb_launch_overlapped(hd == 64 ? (pages.groups == 1 ? cache4_values_kernel<T, 64, 1> : cache4_values_kernel<T, 64, 2>)
+                                       : pages.groups == 1 ? cache4_values_kernel<T, 128, 1> : pages.groups == 2 ? cache4_values_kernel<T, 128, 2> : cache4_values_kernel<T, 128, 4>, dim3((unsigned)blocks), dim3(256), 0, s, pages, slots, n, k, ldk, v, ldv,
                                        wide));
     return LB_OK;
 }
@@ -461,7 +500,9 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
                       a.n_mass, a.n_dest_mass};
-    LB_CHECK_CUDA(lb_launch_overlapped(evict4_choose_kernel, dim3(pages.n_kv_head, a.n_seq), dim3(kChoiceThreads), 0, s, c));
+    const int held = a.max_keys < kMostHeld ? a.max_keys : kMostHeld;
+    LB_CHECK_CUDA(cudaFuncSetAttribute(evict4_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostHeld));
+    LB_CHECK_CUDA(lb_launch_overlapped(evict4_choose_kernel, dim3(pages.n_kv_head, a.n_seq), dim3(kChoiceThreads), 4 * held, s, c, held));
     const dim3 grid((a.keep + 63) / 64, pages.n_kv_head, a.n_seq);
     LB_CHECK_CUDA(lb_launch_overlapped(a.cache->head_dim == 128 ? evict4_copy_kernel<128> : evict4_copy_kernel<64>, grid, dim3(128), 0, s, pages, a.block_table, a.table_stride,
                                        a.dest_table, a.dest_table_stride, a.kept, a.keep, a.max_keys));

@@ -119,7 +119,7 @@ def test_how_attention_is_cut():
 def test_scratch():
     """States of all runs (a run more than warps and units together has), where requests' tiles start, and the keys' weights."""
     (_, rows, blocks, per), got = _plan(8, 32, 4, 1024, dim=128)
-    states, starts = (4 * blocks + 4 * 8) * rows * 130 * 4, 5 * 4
+    states, starts = (4 * blocks + 4 * 8) * rows * 132 * 4, 5 * 4
     assert got == states + -(-starts // 16) * 16
     c, ref = _cache(kv=8, dim=128)
     scratch = ops.lib().lb_attention4_scratch

@@ -16,12 +16,12 @@ BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
 # ---- plain forms -------------------------------------------------------------------------------------------
 
 def _rounded(x, kv, dim, group):
-    """(n, s) of rows [rows, kv * dim] by the cache's rule, in 32 bits as the rule has it: n int8 [rows, kv, dim], s bfloat16 [rows, kv, dim / group]."""
+    """(n, s) of rows [rows, kv * dim] by the cache's rule: n int8 [rows, kv, dim], s bfloat16 [rows, kv, dim / group]."""
     g = x.float().view(x.shape[0], kv, dim // group, group)
     top = g.abs().amax(3)
     s = (top / torch.full_like(top, 7.0)).to(BF16)
     s = torch.where(top.isfinite(), s, torch.full_like(s, math.nan))
-    t = s.float()[..., None].expand_as(g)
+    t = s.float()[..., None].expand_as(g)                    # quotients are rounded to 32 bits
     n = torch.where(t > 0, (g / torch.where(t > 0, t, torch.ones_like(t))).round().clamp(-8, 7), torch.zeros_like(g))
     return n.view(-1, kv, dim).to(torch.int8), s
 
