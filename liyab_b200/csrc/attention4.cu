@@ -45,6 +45,9 @@ attention4_mass_kernel(const Call c, const Mass w) {
 
 constexpr int kMostMassTokens = 64;
 
+// Which kernel takes a call.
+bool takes_many(const lb_attention4_args& a, int max_rows) { return a.total == nullptr && max_rows > 64; }
+
 struct Scratch {
     int64_t scores, log_sums, partial, starts, bytes;       // offsets
 };
@@ -56,6 +59,7 @@ Scratch scratch_of(const lb_attention4_args& a, const RowsPlan& p, int max_rows,
         s.log_sums = up(units * max_rows * score_keys * 4);
         s.bytes = s.log_sums + up(units * max_rows * 4);
     }
+    if (takes_many(a, max_rows)) return s;
     s.partial = s.bytes;
     s.starts = s.partial + up(p.states);
     s.bytes = s.starts + up(p.starts);
@@ -123,7 +127,7 @@ extern "C" int lb_attention4_plan(const lb_attention4_args* args, int* plan) {
     Scratch s;
     LB_CHECK_ARG(plan != nullptr, "attention4: no place for the plan");
     if (int rc = check(args, &c, &p, &s)) return rc;
-    plan[0] = 0;
+    plan[0] = takes_many(*args, c.max_rows) ? 1 : 0;
     plan[1] = p.rows;
     plan[2] = p.blocks;
     plan[3] = p.per_row;
@@ -144,6 +148,7 @@ extern "C" int lb_attention4(const lb_attention4_args* args) {
     LB_CHECK_ARG(s.bytes == 0 || (a.scratch != nullptr && reinterpret_cast<uintptr_t>(a.scratch) % 16 == 0), "attention4: scratch memory is missing or not 16-byte aligned");
     if (int rc = device_check("attention4", a.cache->device)) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
+    if (takes_many(a, c.max_rows)) return many_rows(c, a.cache->head_dim, stream);
     if (int rc = few_rows(c, a.cache->head_dim, p, stream)) return rc;
     if (a.total != nullptr) {
         const Mass w = {a.mass, a.total, a.mass_rows, a.mass_stride, a.mass_head_stride, a.total_stride, a.total_head_stride, a.n_mass};

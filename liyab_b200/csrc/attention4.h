@@ -48,6 +48,8 @@ struct RowsPlan {
     int64_t states, starts;
 };
 int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+// Portions of many rows, on tcgen05.
+int many_rows(const Call& c, int head_dim, cudaStream_t stream);
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t stream);
 
 }  // namespace lb_a4

@@ -1,0 +1,656 @@
+// Attention over a 4-bit cache for many query rows: portions of prompts, on the fifth-generation tensor cores.
+//
+// The query rows of a request that share a key/value head (its tokens' heads, in the order of the tokens) are cut into tiles of 256; a block has a tile, as two groups of 128 rows, and walks the
+// keys 128 at a time.  Both groups read the same keys and values, which eight warps make from the cache's nibbles:
+//   warps 0..7    softmax, a thread a row: the row's largest score, p = 2^(S - m), p as float16 back into tensor memory over the scores it came from, and O rescaled where m moved.
+//   warps 8..15   makers: a warp has a block of sixteen keys.  The nibbles of the next tile are on their way while this one's become n s as float16, in the 128-byte swizzle that tcgen05 reads.
+//   warps 16, 17  issue tcgen05.mma, one for each group: S = Q K^T (128 x 128), O += P V (64 values at a time, V as it lies, [key][dim]: the "MN-major" form).
+// Tensor memory: the groups' scores (and p, in the first half of their columns), then the groups' O.  A group's next scores are asked for once its update has read p; meanwhile the other group is at
+// its exponentials, so the two take turns at the tensor cores and at the special-function units (a tile's 2 x 16,384 exponentials take those 2,048 cycles, its products for heads of 128 the tensor
+// cores 2,048).
+// Numbers: a row of queries is float16 after a power of two that puts its largest at 2^14; n s after one for the block of sixteen keys that puts its largest scale at 2^8, which the scores, and p, are
+// multiplied by again (for p relative to the largest block's so far, F, which O is in units of).  So K, V and p are rounded to float16 (2^-12), and bfloat16's range is kept.
+// A value scale that is NaN would meet p = 0 of rows that do not see its key in the products: such groups are made zeros, and the rows that see them take a note (a bit a group) and end as NaN.
+// Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results.
+#include "attention4.h"
+#include "tcgen05.cuh"
+
+#include <cuda_fp16.h>
+#include <float.h>
+#include <math_constants.h>
+
+#include <algorithm>
+
+namespace lb_a4 {
+namespace {
+
+using namespace lb_c4;
+using namespace lb_tc;
+
+constexpr int kGroups = 2, kBM = 128, kBN = 128, kTileRows = kGroups * kBM;
+constexpr int kUnit = 64;                      // keys of a score tile: half of what the makers make at a time
+constexpr int kStages = 2;                     // tiles of keys, and of values, in shared memory
+constexpr int kNotes = 4;                      // what the softmax reads of a tile, longer than a stage holds
+constexpr int kMakers = 8, kIssuer = 16, kManyThreads = 32 * 20;         // (warps 18 and 19 are there because registers are dealt to four warps at a time)
+// Registers a thread after the roles part: 2 x 128 + 2 x 88 + 48, the 5 x 96 that the block starts with.
+constexpr int kSoftmaxRegs = 128, kMakerRegs = 88, kIssuerRegs = 48;
+constexpr int kSub = 128 * 128;                // [128 rows][128 bytes]: 64 values of a tile
+constexpr uint32_t kTmemCols = 512, kOCol = 256;
+constexpr float kLowest = -FLT_MAX, kSlack = 8.0f, kLeastExponent = -100.0f;
+
+struct Control {
+    uint64_t q_full;
+    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups];          // a unit's warps may be a unit apart, so p has two
+    uint32_t tmem_base;
+    int abort_flag;
+    float k_factor[kNotes][kMakers], v_exponent[kNotes][kMakers];          // of a tile's blocks of sixteen keys
+    uint8_t gone[kNotes][kMakers], nans[kNotes][kMakers];                  // on no page; values with scales that are NaN
+    uint8_t nan_groups[kNotes][kBN];                                       // a bit a group
+};
+
+__device__ __forceinline__ void give_up(Control* c, int* status, int site) {
+    atomicCAS(status, 0, (0xC << 12) | site);
+    *(volatile int*)&c->abort_flag = 1;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
+template <int BYTES>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+    if constexpr (BYTES == 16) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else if constexpr (BYTES == 8) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = u.x; w[1] = u.y;
+    } else {
+        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    }
+}
+// A word's values times s as four float16 pairs: nibbles (i, i + 4).
+__device__ __forceinline__ void scaled_pairs(uint32_t w, __half2 s, uint32_t (&r)[4]) {
+    const __half2 offset = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f), offset16 = __float2half2_rn(-72.0f);
+    const uint32_t hi = w >> 8;
+    r[0] = h2(__hmul2(__hadd2(as_h2((w & 0x000f000fu) | 0x64006400u), offset), s));
+    r[1] = h2(__hmul2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, offset16), s));
+    r[2] = h2(__hmul2(__hadd2(as_h2((hi & 0x000f000fu) | 0x64006400u), offset), s));
+    r[3] = h2(__hmul2(__hfma2(as_h2((hi & 0x00f000f0u) | 0x64006400u), sixteenth, offset16), s));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The wait for a load, tied to its registers so that nothing is made of them before it.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+                   "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :: "memory");
+}
+// The product with its first operand in tensor memory (lane = row, two float16 values of K to a column).
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Descriptor of a tile [64 values][key][64 values] as the second operand in its MN-major form: rows of 128 bytes, eight keys to a 1024-byte group (the stride offset), the next 64 values
+// behind all keys (the leading offset).
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(kSub >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Instruction descriptors: float16 operands (0 in both format fields), 32-bit sums; the second with the second operand MN-major (bit 16).
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// The largest finite bfloat16 number among the words' (0 where none is above it), over the warp.
+template <int N>
+__device__ __forceinline__ uint32_t largest(const uint32_t* w) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = __vmaxu2(top, w[i]);
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    if (top < 0x7f80u) return top;
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t lo = w[i] & 0xffffu, hi = w[i] >> 16;
+        top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    }
+    return __reduce_max_sync(0xffffffffu, top);
+}
+
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :: "memory");
+}
+
+// A bounded wait, one answer for the warp.  Most find the phase done: one question then (mbar_wait's loop is 90 cycles of a warp that has the SM for itself, this 30).
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+template <int HD, int NG, bool PLAIN>
+__global__ void __launch_bounds__(kManyThreads, 1)
+attention4_many_kernel(const Call c, int* status) {
+    using L = Layout<HD>;
+    constexpr int SUBS = HD / 64, JK = HD / 32, JV = HD / 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* q_s = base;                                            // [group][64 values][128 rows]
+    uint8_t* k_s = q_s + kGroups * SUBS * kSub;                     // [stage][64 values][128 keys]
+    uint8_t* v_s = k_s + kStages * SUBS * kSub;
+    Control* ctl = reinterpret_cast<Control*>(v_s + kStages * SUBS * kSub);
+    volatile int* abort_flag = &ctl->abort_flag;
+
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    const int seq = blockIdx.z, kvh = blockIdx.y, kv = c.pages.n_kv_head;
+    const Portion part = portion_of(c, seq);
+    // The last tiles first, which see the most keys.
+    const int n_rows = part.count * c.per, row0 = ((n_rows + kTileRows - 1) / kTileRows - 1 - (int)blockIdx.x) * kTileRows;
+    if (row0 < 0 || n_rows <= 0) return;
+    const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;          // no key past this place is read
+    auto place_of = [&](int row) { return min(part.place + min(row, n_rows - 1) / c.per, limit); };
+    auto first_of = [&](int place) { return place < 0 ? 0 : lb_first_visible(place, c.window); };
+    const int p_hi = place_of(row0 + kTileRows - 1), kv_lo = first_of(place_of(row0)) / kBN * kBN;
+    const int n_tiles = p_hi >= 0 ? (p_hi - kv_lo) / kBN + 1 : 0;
+    // Whether rows of group g see keys of unit u.
+    int g_lo[kGroups], g_hi[kGroups];                               // units
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int from = row0 + g * kBM, hi = place_of(from + kBM - 1);
+        const bool some = from < n_rows && hi >= 0;
+        g_lo[g] = some ? (first_of(place_of(from)) - kv_lo) / kUnit : 0;
+        g_hi[g] = some ? (hi - kv_lo) / kUnit + 1 : 0;
+    }
+    auto active = [&](int g, int u) { return u >= g_lo[g] && u < g_hi[g]; };
+
+    if (threadIdx.x == 0) {
+        mbar_init(&ctl->q_full, 2 * 4);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&ctl->k_full[i], kMakers);
+            mbar_init(&ctl->k_empty[i], kGroups);
+            mbar_init(&ctl->v_full[i], kMakers);
+            mbar_init(&ctl->v_empty[i], kGroups);
+        }
+        for (int g = 0; g < kGroups; ++g) {
+            mbar_init(&ctl->s_full[g][0], 1);
+            mbar_init(&ctl->s_full[g][1], 1);
+            mbar_init(&ctl->p_full[g][0], 4);
+            mbar_init(&ctl->p_full[g][1], 4);
+            mbar_init(&ctl->o_done[g], 1);
+        }
+        ctl->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kIssuer) {
+        tmem_alloc(&ctl->tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+
+    if (warp >= kIssuer) registers_down<kIssuerRegs>();
+    else if (warp >= 8) registers_down<kMakerRegs>();
+    else registers_up<kSoftmaxRegs>();
+    if (warp >= kIssuer + kGroups) {
+        // (nothing)
+    } else if (warp >= kIssuer) {
+        // ---- products, a warp a group.  A group's scores of unit u + 1 are asked for ahead of its update of unit u, when its update of unit u - 1, whose p lay where they go, is done.
+        constexpr uint32_t idesc_s = idesc_f16(kBM, kUnit), idesc_o = idesc_f16(kBM, HD) | (1u << 16);
+        const int g = warp - kIssuer, lo = g == 0 ? g_lo[0] : g_lo[1], hi = g == 0 ? g_hi[0] : g_hi[1], n_units = 2 * n_tiles;
+        const uint64_t dq = umma_desc(smem_u32(q_s + g * SUBS * kSub)), dk = umma_desc(smem_u32(k_s)), dv = umma_desc_mn(smem_u32(v_s));
+        const uint32_t s_at = tmem_base + g * kBN, o_at = tmem_base + kOCol + g * HD;
+        bool ok = wait(&ctl->q_full, 0, abort_flag);
+        if (!ok) give_up(ctl, status, 2);
+        auto scores = [&](int u) {
+            const int st = (u >> 1) % kStages;
+            if ((u & 1) == 0) ok = wait(&ctl->k_full[st], (u >> 1) / kStages & 1, abort_flag);
+            if (u >= lo && u < hi) {
+                if (u - 2 >= lo) ok = ok && wait(&ctl->o_done[g], (uint32_t)(u - 2 - lo) & 1u, abort_flag);
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t db = dk + (uint64_t)((st * SUBS * kSub + (u & 1) * kUnit * 128) >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < HD / kUmmaK; ++i)
+                        umma_bf16(s_at + (u & 1) * kUnit, dq + (uint64_t)(((i / 4) * kSub + i % 4 * 32) >> 4), db + (uint64_t)(((i / 4) * kSub + i % 4 * 32) >> 4), idesc_s, i != 0 ? 1u : 0u);
+                    umma_commit(&ctl->s_full[g][u & 1]);
+                }
+                __syncwarp();
+            }
+            if (ok && (u & 1) == 1 && elect_one()) umma_commit(&ctl->k_empty[st]);
+            __syncwarp();
+        };
+        if (ok && n_units > 0) scores(0);
+        for (int u = 0; u < n_units && ok; ++u) {
+            const int st = (u >> 1) % kStages;
+            if (u + 1 < n_units) scores(u + 1);
+            if (!ok) break;
+            if ((u & 1) == 0) ok = wait(&ctl->v_full[st], (u >> 1) / kStages & 1, abort_flag);
+            if (ok && u >= lo && u < hi) {
+                ok = wait(&ctl->p_full[g][u & 1], (uint32_t)((u - lo) >> 1) & 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t db = dv + (uint64_t)((st * SUBS * kSub + (u & 1) * kUnit * 128) >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kUnit / kUmmaK; ++k)              // sixteen keys: eight columns of p, 2048 bytes of values
+                        umma_ts(o_at, s_at + (u & 1) * kUnit + k * 8, db + (uint64_t)((k * 2048) >> 4), idesc_o, u > lo || k != 0 ? 1u : 0u);
+                    umma_commit(&ctl->o_done[g]);           // O holds unit u, and p has been read
+                }
+                __syncwarp();
+            }
+            if (ok && (u & 1) == 1 && elect_one()) umma_commit(&ctl->v_empty[st]);
+            __syncwarp();
+        }
+        if (!ok) give_up(ctl, status, 3);
+    } else if (warp >= 8) {
+        // ---- makers
+        const int b = warp - 8, g = lane >> 2, t = lane & 3;
+        const int32_t* table = c.table + (int64_t)seq * c.table_stride;
+        const int kb = block_bytes(HD, NG);
+        int block_at = -1;                                   // lane i: the cache's block of this warp's keys in tile i of this 32; -1: on no page, -2: past the keys
+        struct Raw {
+            uint32_t k[2][JK], v[2][2 * JV], ks[NG], vs[2][NG];
+        };
+        auto load = [&](int j, Raw& r, int* where) {
+            if ((j & 31) == 0) {
+                const int key = kv_lo + (j + lane) * kBN + b * kBlockKeys;
+                block_at = -2;
+                if (key <= p_hi) {
+                    const int page = table[key >> c.pages.page_shift];
+                    block_at = (unsigned)page < (unsigned)c.pages.n_pages
+                                   ? ((page * kv + kvh) << (c.pages.page_shift - 4)) + ((key & ((1 << c.pages.page_shift) - 1)) >> 4) : -1;
+                }
+            }
+            *where = __shfl_sync(0xffffffffu, block_at, j & 31);
+            if (*where < 0) return;
+            const uint8_t* block = c.pages.memory + (int64_t)*where * kb;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                load_words<L::kPiece>(block + (32 * i + lane) * L::kPiece, r.k[i]);
+                load_words<L::kPiece>(block + L::kV + (32 * i + t * 8 + L::v_turn(g, t)) * L::kPiece, r.v[i]);
+                load_words<4 * NG>(block + L::kScales + 32 * NG + (2 * t + i) * 4 * NG, r.vs[i]);
+            }
+            load_words<4 * NG>(block + L::kScales + g * 4 * NG, r.ks);
+        };
+        Raw raw = {}, next = {};
+        int where = -2, next_where = -2;
+        bool ok = true;
+        if (n_tiles > 0) load(0, raw, &where);
+        for (int j = 0; j < n_tiles; ++j) {
+            const int st = j % kStages, note = j % kNotes, key0 = kv_lo + j * kBN + b * kBlockKeys;
+            const uint32_t empty = ((uint32_t)(j / kStages) & 1u) ^ 1u;
+            if (j + 1 < n_tiles) load(j + 1, next, &next_where);
+            if (where < 0) raw = Raw{};
+            // Keys past the last row's: whatever the memory holds, their scales are 0.
+            if (key0 + kBlockKeys - 1 > p_hi) {
+                auto clear = [&](uint32_t* w, int key, int second) {
+                    if (key <= p_hi) return;
+                    if constexpr (NG == 1) {
+                        w[0] &= second != 0 ? 0x0000ffffu : 0xffff0000u;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NG / 2; ++i) w[second * NG / 2 + i] = 0;
+                    }
+                };
+#pragma unroll
+                for (int second = 0; second < 2; ++second) {
+                    clear(raw.ks, key0 + g + 8 * second, second);
+                    clear(raw.vs[0], key0 + 2 * t + 8 * second, second);
+                    clear(raw.vs[1], key0 + 2 * t + 1 + 8 * second, second);
+                }
+            }
+            ok = wait(&ctl->k_empty[st], empty, abort_flag);
+            if (!ok) break;
+            {
+                const uint32_t top = largest<NG>(raw.ks);
+                const int e = max((int)(top >> 7) - 127, (int)kLeastExponent);
+                const float up = pow2(8 - e);
+                uint8_t* to = k_s + st * SUBS * kSub;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int key = b * kBlockKeys + g + 8 * i;
+#pragma unroll
+                    for (int jj = 0; jj < JK; ++jj) {
+                        const int chunk = 4 * jj + t;
+                        uint4 w;
+                        uint32_t r[4];
+                        scaled_pairs(raw.k[i][jj], __float2half2_rn(number(raw.ks, i * NG + jj * NG / JK) * up), r);
+                        w.x = r[0]; w.y = r[1]; w.z = r[2]; w.w = r[3];
+                        *reinterpret_cast<uint4*>(to + (chunk >> 3) * kSub + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)) = w;
+                    }
+                }
+                if (lane == 0) {
+                    ctl->k_factor[note][b] = pow2(e - 8);
+                    ctl->gone[note][b] = where == -1;
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->k_full[st]);
+            ok = wait(&ctl->v_empty[st], empty, abort_flag);
+            if (!ok) break;
+            {
+                const uint32_t top = max(largest<NG>(raw.vs[0]), largest<NG>(raw.vs[1]));
+                const int e = max((int)(top >> 7) - 127, (int)kLeastExponent);
+                const float up = pow2(8 - e);
+                uint8_t* to = v_s + st * SUBS * kSub;
+                bool nans = false;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)                  // the keys 2 t, 2 t + 1, and those plus 8
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        const int key = b * kBlockKeys + 8 * i + 2 * t + a;
+                        float s[NG];
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int x = 0; x < NG; ++x) {
+                            s[x] = number(raw.vs[a], i * NG + x);
+                            if (!(s[x] < CUDART_INF_F)) {
+                                s[x] = 0.0f;
+                                bits |= 1u << x;
+                            }
+                        }
+                        if (g == 0) ctl->nan_groups[note][key] = (uint8_t)bits;
+                        nans = nans || bits != 0;
+#pragma unroll
+                        for (int jj = 0; jj < JV; ++jj) {
+                            uint32_t r[4], r2[4];
+                            const uint32_t w = raw.v[i][a * JV + jj];
+                            const __half2 s0 = __float2half2_rn(s[64 * jj / (HD / NG)] * up), s1 = __float2half2_rn(s[(64 * jj + 32) / (HD / NG)] * up);
+                            scaled_pairs(w, s0, r);
+                            if (NG * 32 == HD) scaled_pairs(w, s1, r2);
+                            uint8_t* row = to + jj * kSub + key * 128 + (g & 1) * 8;
+                            *reinterpret_cast<uint2*>(row + (((g >> 1) ^ (key & 7)) << 4)) = make_uint2(r[0], r[1]);
+                            *reinterpret_cast<uint2*>(row + (((4 + (g >> 1)) ^ (key & 7)) << 4)) = NG * 32 == HD ? make_uint2(r2[2], r2[3]) : make_uint2(r[2], r[3]);
+                        }
+                    }
+                nans = __any_sync(0xffffffffu, nans);
+                if (lane == 0) {
+                    ctl->v_exponent[note][b] = (float)e;
+                    ctl->nans[note][b] = nans;
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->v_full[st]);
+            raw = next;
+            where = next_where;
+        }
+        if (!ok) give_up(ctl, status, 4);
+    } else {
+        // ---- softmax
+        const int g = warp >> 2, quarter = warp & 3, row = row0 + g * kBM + quarter * 32 + lane;
+        const uint32_t t_s = tmem_base + g * kBN + ((uint32_t)(quarter * 32) << 16), t_o = tmem_base + kOCol + g * HD + ((uint32_t)(quarter * 32) << 16);
+        const bool there = row < n_rows;
+        const int token = min(row, n_rows - 1) / c.per, head = kvh * c.per + min(row, n_rows - 1) - token * c.per;
+        float row_scale;                                    // of the scores, in base 2
+        {
+            // The row as float16 in shared memory.
+            const __nv_bfloat16* from = c.q + (int64_t)(part.first + token) * c.q_stride + (int64_t)head * HD;
+            const bool q_wide = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.q_stride % 8 == 0;
+            auto eight = [&](int i, uint32_t (&u)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = 0;
+                if (there && q_wide) {
+                    load_words<16>(reinterpret_cast<const uint8_t*>(from + 8 * i), u);
+                } else if (there) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = __bfloat16_as_ushort(from[8 * i + 2 * e]) | (uint32_t)__bfloat16_as_ushort(from[8 * i + 2 * e + 1]) << 16;
+                }
+            };
+            uint32_t top = 0;
+#pragma unroll 4
+            for (int i = 0; i < HD / 8; ++i) {
+                uint32_t u[4];
+                eight(i, u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = __vmaxu2(top, u[e] & 0x7fff7fffu);
+            }
+            top = max(top & 0xffffu, top >> 16);
+            const bool finite = top < 0x7f80u;
+            const int shift = top == 0 || !finite ? 0 : 14 - (max((int)(top >> 7), 1) - 127);
+            const float up = copysignf(pow2(shift / 2), c.scale), up2 = pow2(shift - shift / 2);            // the scale's sign is the query's
+            row_scale = !finite ? CUDART_NAN_F : fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2);
+            uint8_t* to = q_s + g * SUBS * kSub + (quarter * 32 + lane) * 128;
+#pragma unroll 4
+            for (int i = 0; i < HD / 8; ++i) {              // read again: the row does not fit the registers
+                uint32_t u[4], w[4];
+                eight(i, u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = finite ? h2(__floats2half2_rn(__uint_as_float(u[e] << 16) * up * up2, __uint_as_float(u[e] & 0xffff0000u) * up * up2)) : 0u;
+                *reinterpret_cast<uint4*>(to + (i >> 3) * kSub + (((i & 7) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->q_full);
+        }
+        const int place = place_of(row), first = first_of(place);
+        const int w_row = row0 + g * kBM + quarter * 32;
+        const int place_lo = place_of(w_row), first_hi = first_of(place_of(w_row + 31));            // of the warp's rows
+        const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.25f * c.soft_cap);          // in its series' form
+        const float exact_in = PLAIN ? 0.0f : 2.0f / c.soft_cap;
+        const float r1 = !PLAIN && c.distance != nullptr ? c.distance[head] : 0.0f, r2 = !PLAIN && c.distance != nullptr ? c.distance[c.n_head + head] : 0.0f;
+        const bool biased = !PLAIN && c.distance != nullptr;
+        float m = kLowest, l = 0.0f, big = kLeastExponent;                    // big: F, the largest exponent of value scales so far
+        uint32_t nan_bits = 0;
+        bool ok = true;
+        for (int u = g_lo[g]; u < g_hi[g]; ++u) {
+            const int j = u >> 1, note = j % kNotes, part_of = (u & 1) * (kUnit / kBlockKeys), key0 = kv_lo + u * kUnit;
+            // A buffer of scores is filled every other unit, the first of the two that the range starts with first.
+            ok = wait(&ctl->s_full[g][u & 1], (uint32_t)((u - g_lo[g]) >> 1) & 1u, abort_flag);
+            // What the values' makers left of this tile is read once they are done.
+            if ((u & 1) == 0 || u == g_lo[g]) ok = ok && wait(&ctl->v_full[j % kStages], (j / kStages) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t t_u = t_s + (u & 1) * kUnit;
+            uint32_t v[2][32];
+            tmem_ld32(t_u, v[0]);
+            tmem_ld32(t_u + 32, v[1]);
+            float factor[4], exponent[4], high_exponent = big;
+            uint32_t gone = 0, nans = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                factor[b] = row_scale * ctl->k_factor[note][part_of + b];
+                exponent[b] = ctl->v_exponent[note][part_of + b];
+                high_exponent = fmaxf(high_exponent, exponent[b]);
+                gone |= ctl->gone[note][part_of + b];
+                nans |= ctl->nans[note][part_of + b];
+            }
+            const bool masked = key0 + kUnit - 1 > place_lo || key0 < first_hi || gone != 0;
+            tmem_ld_wait32(v[0]);
+            tmem_ld_wait32(v[1]);
+            if (!PLAIN || masked) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) * factor[2 * h + i / 16]);
+                    if constexpr (!PLAIN) {
+                        if (c.soft_cap > 0.0f) {
+                            // Where no score of the warp passes a quarter of the cap, the series of tanh (see lb_soft_cap); else 1 - 2 / (1 + e^2x).
+                            float size = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) size = fmaxf(size, fabsf(__uint_as_float(v[h][i])));
+                            if (__all_sync(0xffffffffu, size <= 0.25f * capped.out)) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(capped(__uint_as_float(v[h][i])));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    v[h][i] = __float_as_uint(fmaf(-2.0f * capped.out, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[h][i]) * exact_in)), capped.out));
+                            }
+                        }
+                        if (biased) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) - lb_distance_penalty_log2(r1, r2, max(place - (key0 + 32 * h + i), 0)));
+                        }
+                    }
+                    if (masked) {
+                        // A bit a key that the row sees.
+                        const int from = first - (key0 + 32 * h), to = place - (key0 + 32 * h);
+                        uint32_t seen = (to >= 31 ? 0xffffffffu : to < 0 ? 0u : (2u << to) - 1u) & (from <= 0 ? 0xffffffffu : from > 31 ? 0u : ~((1u << from) - 1u));
+                        if (ctl->gone[note][part_of + 2 * h] != 0) seen &= 0xffff0000u;
+                        if (ctl->gone[note][part_of + 2 * h + 1] != 0) seen &= 0x0000ffffu;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[h][i] = (seen >> i & 1u) != 0 ? v[h][i] : 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) factor[b] = 1.0f;
+            }
+            float high = kLowest;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float h0 = __uint_as_float(v[b / 2][16 * (b & 1)]), h1 = __uint_as_float(v[b / 2][16 * (b & 1) + 1]);
+#pragma unroll
+                for (int i = 2; i < 16; i += 2) {
+                    h0 = fmaxf(h0, __uint_as_float(v[b / 2][16 * (b & 1) + i]));
+                    h1 = fmaxf(h1, __uint_as_float(v[b / 2][16 * (b & 1) + i + 1]));
+                }
+                high = fmaxf(high, fmaxf(h0, h1) * factor[b]);            // (a factor is not negative: a scale's sign is the query's)
+            }
+            // O, the sum and p are relative to m, O in units of 2^big as well; where a score passes m by more than 2^8, or a block's exponent big, they move.
+            if (__any_sync(0xffffffffu, high > m + kSlack || high_exponent > big)) {
+                const float m_new = fmaxf(m, high), corr = ex2(m - m_new), corr_o = corr * ex2(big - high_exponent);
+                l *= corr;
+                m = m_new;
+                big = high_exponent;
+                if (u > g_lo[g]) {
+                    ok = wait(&ctl->o_done[g], (uint32_t)(u - 1 - g_lo[g]) & 1u, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t w[16];
+#pragma unroll 1
+                    for (int x = 0; x < HD / 16; ++x) {
+                        tmem_ld16(t_o + x * 16, w);
+                        tmem_ld_wait16(w);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * corr_o);
+                        tmem_st16(t_o + x * 16, w);
+                    }
+                }
+            }
+            // p times 2^(a block's exponent less big) in one exponential; the sum of a block's is brought back.  (What lies 2^60 below the largest scale's is nothing beside it.)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int b = 2 * h + half;
+                    const float less = fmaxf(exponent[b] - big, -60.0f), ref = less - m;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float p0 = ex2(fmaf(__uint_as_float(v[h][16 * half + i]), factor[b], ref)), p1 = ex2(fmaf(__uint_as_float(v[h][16 * half + i + 1]), factor[b], ref));
+                        sum0 += p0;
+                        sum1 += p1;
+                        pk[8 * half + i / 2] = h2(__floats2half2_rn(p0, p1));
+                    }
+                    l = fmaf(sum0 + sum1, ex2(-less), l);
+                }
+                tmem_st16(t_u + h * 16, pk);               // over scores that have been read
+            }
+            if (nans != 0)
+                for (int i = 0; i < kUnit; ++i)
+                    if (key0 + i <= place && key0 + i >= first) nan_bits |= ctl->nan_groups[note][(u & 1) * kUnit + i];
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[g][u & 1]);
+        }
+        // The last two updates may both be under way; a parity alone does not tell a phase from the one before the last.
+        if (ok && g_hi[g] > g_lo[g] + 1) ok = wait(&ctl->o_done[g], (uint32_t)(g_hi[g] - g_lo[g] - 2) & 1u, abort_flag);
+        if (ok && g_hi[g] > g_lo[g]) ok = wait(&ctl->o_done[g], (uint32_t)(g_hi[g] - g_lo[g] - 1) & 1u, abort_flag);
+        if (!ok) give_up(ctl, status, 5);
+        if (ok && w_row < n_rows) {
+            tc_fence_after();
+            const bool none = l == 0.0f;                          // no key seen: O may be what the memory held
+            float factor = 1.0f;
+            if (c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
+            factor = factor / l * ex2(big * 0.5f);
+            const float factor2 = ex2(big * 0.5f - 8.0f);                 // in two steps: big may be 2^127's exponent
+            __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD;
+            const bool out_wide = reinterpret_cast<uintptr_t>(c.out) % 16 == 0 && c.out_stride % 8 == 0;
+#pragma unroll
+            for (int h = 0; h < HD / 32; ++h) {
+                uint32_t v[32];
+                tmem_ld32(t_o + h * 32, v);
+                tmem_ld_wait32(v);
+                const bool nan = (nan_bits >> (32 * h / (HD / NG)) & 1u) != 0;
+                auto value = [&](int i) { return none ? 0.0f : nan ? CUDART_NAN_F : __uint_as_float(v[i]) * factor * factor2; };
+                if (!there) continue;
+                if (out_wide) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4*>(out + 32 * h + i) =
+                            make_uint4(pack2(value(i), value(i + 1)), pack2(value(i + 2), value(i + 3)), pack2(value(i + 4), value(i + 5)), pack2(value(i + 6), value(i + 7)));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) out[32 * h + i] = __float2bfloat16_rn(value(i));
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kIssuer) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+template <int HD, int NG>
+int launch(const Call& c, cudaStream_t s) {
+    int* status = nullptr;
+    if (int rc = lb_tc_status_word(&status)) return rc;
+    const bool plain = c.distance == nullptr && c.soft_cap <= 0.0f;
+    auto kernel = plain ? attention4_many_kernel<HD, NG, true> : attention4_many_kernel<HD, NG, false>;
+    constexpr int smem = 1024 + (kGroups + 2 * kStages) * (HD / 64) * kSub + (int)sizeof(Control);
+    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, status));
+    return LB_OK;
+}
+
+}  // namespace
+
+int many_rows(const Call& c, int head_dim, cudaStream_t s) {
+    if (head_dim == 64) return c.pages.groups == 1 ? launch<64, 1>(c, s) : launch<64, 2>(c, s);
+    return c.pages.groups == 1 ? launch<128, 1>(c, s) : c.pages.groups == 2 ? launch<128, 2>(c, s) : launch<128, 4>(c, s);
+}
+
+}  // namespace lb_a4
