@@ -2,9 +2,9 @@
 //
 // The query rows of a request that share a key/value head (its tokens' heads, in the order of the tokens) are cut into tiles of 256; a block has a tile, as two groups of 128 rows, and walks the
 // keys 128 at a time.  Both groups read the same keys and values, which eight warps make from the cache's nibbles:
-//   warps 0..7    softmax, a thread a row: the row's largest score, p = 2^(S - m), p as float16 back into tensor memory over the scores it came from, and O rescaled where m moved.
-//   warps 8..15   makers: a warp has a block of sixteen keys.  The nibbles of the next tile are on their way while this one's become n s as float16, in the 128-byte swizzle that tcgen05 reads.
-//   warps 16, 17  issue tcgen05.mma, one for each group: S = Q K^T (128 x 128), O += P V (64 values at a time, V as it lies, [key][dim]: the "MN-major" form).
+//   warps 0..15   softmax, two threads a row: p = 2^(S - m) as float16 back into tensor memory over the scores it came from, and O rescaled where m moved.
+//   warps 16..23  makers: a warp has a block of sixteen keys.  The nibbles of the next tile are on their way while this one's become n s as float16, in the 128-byte swizzle that tcgen05 reads.
+//   warps 24, 25  issue tcgen05.mma, one for each group: S = Q K^T (128 x 128), O += P V (64 values at a time, V as it lies, [key][dim]: the "MN-major" form).
 // Tensor memory: the groups' scores (and p, in the first half of their columns), then the groups' O.  A group's next scores are asked for once its update has read p; meanwhile the other group is at
 // its exponentials, so the two take turns at the tensor cores and at the special-function units (a tile's 2 x 16,384 exponentials take those 2,048 cycles, its products for heads of 128 the tensor
 // cores 2,048).
@@ -31,9 +31,10 @@ constexpr int kGroups = 2, kBM = 128, kBN = 128, kTileRows = kGroups * kBM;
 constexpr int kUnit = 64;                      // keys of a score tile: half of what the makers make at a time
 constexpr int kStages = 2;                     // tiles of keys, and of values, in shared memory
 constexpr int kNotes = 4;                      // what the softmax reads of a tile, longer than a stage holds
-constexpr int kMakers = 8, kIssuer = 16, kManyThreads = 32 * 20;         // (warps 18 and 19 are there because registers are dealt to four warps at a time)
-// Registers a thread after the roles part: 2 x 128 + 2 x 88 + 48, the 5 x 96 that the block starts with.
-constexpr int kSoftmaxRegs = 128, kMakerRegs = 88, kIssuerRegs = 48;
+constexpr int kSoftmaxWarps = 16, kMakers = 8, kMaker = kSoftmaxWarps, kIssuer = kMaker + kMakers;
+constexpr int kManyThreads = 32 * (kIssuer + 4);         // (the last two warps are there because registers are dealt to four warps at a time)
+// Registers a thread after the roles part: 4 x 80 + 2 x 72 + 40, the 7 x 72 that the block starts with.
+constexpr int kSoftmaxRegs = 80, kMakerRegs = 72, kIssuerRegs = 40;
 constexpr int kSub = 128 * 128;                // [128 rows][128 bytes]: 64 values of a tile
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr float kLowest = -FLT_MAX, kSlack = 8.0f, kLeastExponent = -100.0f;
@@ -41,12 +42,15 @@ constexpr float kLowest = -FLT_MAX, kSlack = 8.0f, kLeastExponent = -100.0f;
 struct Control {
     uint64_t q_full;
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups];          // a unit's warps may be a unit apart, so p has two
+    uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups][2];       // of units in turn: what waits may be a unit behind, and a parity tells no more than two phases apart
     uint32_t tmem_base;
     int abort_flag;
     float k_factor[kNotes][kMakers], v_exponent[kNotes][kMakers];          // of a tile's blocks of sixteen keys
     uint8_t gone[kNotes][kMakers], nans[kNotes][kMakers];                  // on no page; values with scales that are NaN
     uint8_t nan_groups[kNotes][kBN];                                       // a bit a group
+    float row_scale[kTileRows];                                            // of the scores, in base 2
+    float row_high[kGroups][2][kBM], row_sum[kGroups][2][kBM];             // what the two threads of a row tell each other
+    uint8_t row_nans[kGroups][2][kBM];
 };
 
 __device__ __forceinline__ void give_up(Control* c, int* status, int site) {
@@ -156,6 +160,18 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
+// Whether any of 64 threads says so; a barrier among them.
+__device__ __forceinline__ bool any_of_pair(int barrier, bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, 64, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any) : "r"(barrier), "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
+
 template <int HD, int NG, bool PLAIN>
 __global__ void __launch_bounds__(kManyThreads, 1)
 attention4_many_kernel(const Call c, int* status) {
@@ -194,19 +210,17 @@ attention4_many_kernel(const Call c, int* status) {
     auto active = [&](int g, int u) { return u >= g_lo[g] && u < g_hi[g]; };
 
     if (threadIdx.x == 0) {
-        mbar_init(&ctl->q_full, 2 * 4);
+        mbar_init(&ctl->q_full, kSoftmaxWarps);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&ctl->k_full[i], kMakers);
             mbar_init(&ctl->k_empty[i], kGroups);
             mbar_init(&ctl->v_full[i], kMakers);
             mbar_init(&ctl->v_empty[i], kGroups);
         }
-        for (int g = 0; g < kGroups; ++g) {
-            mbar_init(&ctl->s_full[g][0], 1);
-            mbar_init(&ctl->s_full[g][1], 1);
-            mbar_init(&ctl->p_full[g][0], 4);
-            mbar_init(&ctl->p_full[g][1], 4);
-            mbar_init(&ctl->o_done[g], 1);
+        for (int i = 0; i < 2 * kGroups; ++i) {
+            mbar_init(&ctl->s_full[i / 2][i % 2], 1);
+            mbar_init(&ctl->p_full[i / 2][i % 2], kSoftmaxWarps / kGroups);
+            mbar_init(&ctl->o_done[i / 2][i % 2], 1);
         }
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -221,7 +235,7 @@ attention4_many_kernel(const Call c, int* status) {
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
 
     if (warp >= kIssuer) registers_down<kIssuerRegs>();
-    else if (warp >= 8) registers_down<kMakerRegs>();
+    else if (warp >= kMaker) registers_down<kMakerRegs>();
     else registers_up<kSoftmaxRegs>();
     if (warp >= kIssuer + kGroups) {
         // (nothing)
@@ -235,9 +249,10 @@ attention4_many_kernel(const Call c, int* status) {
         if (!ok) give_up(ctl, status, 2);
         auto scores = [&](int u) {
             const int st = (u >> 1) % kStages;
-            if ((u & 1) == 0) ok = wait(&ctl->k_full[st], (u >> 1) / kStages & 1, abort_flag);
+            // The values too, which are made a little later: what their makers note is the softmax's by the time it has the scores.
+            if ((u & 1) == 0) ok = wait(&ctl->k_full[st], (u >> 1) / kStages & 1, abort_flag) && wait(&ctl->v_full[st], (u >> 1) / kStages & 1, abort_flag);
             if (u >= lo && u < hi) {
-                if (u - 2 >= lo) ok = ok && wait(&ctl->o_done[g], (uint32_t)(u - 2 - lo) & 1u, abort_flag);
+                if (u - 2 >= lo) ok = ok && wait(&ctl->o_done[g][u & 1], (uint32_t)((u - 2 - lo) >> 1) & 1u, abort_flag);
                 if (!ok) return;
                 tc_fence_after();
                 const uint64_t db = dk + (uint64_t)((st * SUBS * kSub + (u & 1) * kUnit * 128) >> 4);
@@ -257,8 +272,7 @@ attention4_many_kernel(const Call c, int* status) {
             const int st = (u >> 1) % kStages;
             if (u + 1 < n_units) scores(u + 1);
             if (!ok) break;
-            if ((u & 1) == 0) ok = wait(&ctl->v_full[st], (u >> 1) / kStages & 1, abort_flag);
-            if (ok && u >= lo && u < hi) {
+            if (u >= lo && u < hi) {
                 ok = wait(&ctl->p_full[g][u & 1], (uint32_t)((u - lo) >> 1) & 1u, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
@@ -267,7 +281,7 @@ attention4_many_kernel(const Call c, int* status) {
 #pragma unroll
                     for (int k = 0; k < kUnit / kUmmaK; ++k)              // sixteen keys: eight columns of p, 2048 bytes of values
                         umma_ts(o_at, s_at + (u & 1) * kUnit + k * 8, db + (uint64_t)((k * 2048) >> 4), idesc_o, u > lo || k != 0 ? 1u : 0u);
-                    umma_commit(&ctl->o_done[g]);           // O holds unit u, and p has been read
+                    umma_commit(&ctl->o_done[g][u & 1]);           // O holds unit u, and p has been read
                 }
                 __syncwarp();
             }
@@ -275,9 +289,9 @@ attention4_many_kernel(const Call c, int* status) {
             __syncwarp();
         }
         if (!ok) give_up(ctl, status, 3);
-    } else if (warp >= 8) {
+    } else if (warp >= kMaker) {
         // ---- makers
-        const int b = warp - 8, g = lane >> 2, t = lane & 3;
+        const int b = warp - kMaker, g = lane >> 2, t = lane & 3;
         const int32_t* table = c.table + (int64_t)seq * c.table_stride;
         const int kb = block_bytes(HD, NG);
         int block_at = -1;                                   // lane i: the cache's block of this warp's keys in tile i of this 32; -1: on no page, -2: past the keys
@@ -411,191 +425,193 @@ attention4_many_kernel(const Call c, int* status) {
         }
         if (!ok) give_up(ctl, status, 4);
     } else {
-        // ---- softmax
-        const int g = warp >> 2, quarter = warp & 3, row = row0 + g * kBM + quarter * 32 + lane;
-        const uint32_t t_s = tmem_base + g * kBN + ((uint32_t)(quarter * 32) << 16), t_o = tmem_base + kOCol + g * HD + ((uint32_t)(quarter * 32) << 16);
-        const bool there = row < n_rows;
-        const int token = min(row, n_rows - 1) / c.per, head = kvh * c.per + min(row, n_rows - 1) - token * c.per;
-        float row_scale;                                    // of the scores, in base 2
+        // ---- softmax, two threads a row (warps w and w + 4): each has 32 of a unit's keys.
+        const int g = warp >> 3, x = warp >> 2 & 1, quarter = warp & 3, row = row0 + g * kBM + quarter * 32 + lane;
+        const uint32_t t_s = tmem_base + g * kBN + ((uint32_t)(quarter * 32) << 16), t_o = tmem_base + kOCol + g * HD + x * (HD / 2) + ((uint32_t)(quarter * 32) << 16);
+        const int pair_barrier = 1 + g * 4 + quarter, all_barrier = 1 + 4 * kGroups;
         {
-            // The row as float16 in shared memory.
-            const __nv_bfloat16* from = c.q + (int64_t)(part.first + token) * c.q_stride + (int64_t)head * HD;
+            // Sixteen rows a warp as float16 into shared memory, HD / 8 lanes a row, and the factors that bring their scores back.
+            constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, STEPS = 16 / AT_ONCE;
             const bool q_wide = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.q_stride % 8 == 0;
-            auto eight = [&](int i, uint32_t (&u)[4]) {
+            const int chunk = lane % LANES;
+            uint32_t u[STEPS][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = 0;
-                if (there && q_wide) {
-                    load_words<16>(reinterpret_cast<const uint8_t*>(from + 8 * i), u);
-                } else if (there) {
+            for (int i = 0; i < STEPS; ++i) {
+                const int r = row0 + warp * 16 + i * AT_ONCE + lane / LANES, token = r / c.per;
+                const __nv_bfloat16* from = c.q + (int64_t)(part.first + token) * c.q_stride + (int64_t)(kvh * c.per + r - token * c.per) * HD + 8 * chunk;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = __bfloat16_as_ushort(from[8 * i + 2 * e]) | (uint32_t)__bfloat16_as_ushort(from[8 * i + 2 * e + 1]) << 16;
+                for (int e = 0; e < 4; ++e) u[i][e] = 0;
+                if (r < n_rows && q_wide) {
+                    load_words<16>(reinterpret_cast<const uint8_t*>(from), u[i]);
+                } else if (r < n_rows) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[i][e] = __bfloat16_as_ushort(from[2 * e]) | (uint32_t)__bfloat16_as_ushort(from[2 * e + 1]) << 16;
                 }
-            };
-            uint32_t top = 0;
-#pragma unroll 4
-            for (int i = 0; i < HD / 8; ++i) {
-                uint32_t u[4];
-                eight(i, u);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = __vmaxu2(top, u[e] & 0x7fff7fffu);
             }
-            top = max(top & 0xffffu, top >> 16);
-            const bool finite = top < 0x7f80u;
-            const int shift = top == 0 || !finite ? 0 : 14 - (max((int)(top >> 7), 1) - 127);
-            const float up = copysignf(pow2(shift / 2), c.scale), up2 = pow2(shift - shift / 2);            // the scale's sign is the query's
-            row_scale = !finite ? CUDART_NAN_F : fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2);
-            uint8_t* to = q_s + g * SUBS * kSub + (quarter * 32 + lane) * 128;
-#pragma unroll 4
-            for (int i = 0; i < HD / 8; ++i) {              // read again: the row does not fit the registers
-                uint32_t u[4], w[4];
-                eight(i, u);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                const int r = warp * 16 + i * AT_ONCE + lane / LANES;
+                uint32_t top = __vmaxu2(__vmaxu2(u[i][0] & 0x7fff7fffu, u[i][1] & 0x7fff7fffu), __vmaxu2(u[i][2] & 0x7fff7fffu, u[i][3] & 0x7fff7fffu));
+                top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+                for (int d = 1; d < LANES; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const bool finite = top < 0x7f80u;
+                const int shift = top == 0 || !finite ? 0 : 14 - (max((int)(top >> 7), 1) - 127);
+                const float up = copysignf(pow2(shift / 2), c.scale), up2 = pow2(shift - shift / 2);            // the scale's sign is the query's
+                uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    w[e] = finite ? h2(__floats2half2_rn(__uint_as_float(u[e] << 16) * up * up2, __uint_as_float(u[e] & 0xffff0000u) * up * up2)) : 0u;
-                *reinterpret_cast<uint4*>(to + (i >> 3) * kSub + (((i & 7) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    w[e] = finite ? h2(__floats2half2_rn(__uint_as_float(u[i][e] << 16) * up * up2, __uint_as_float(u[i][e] & 0xffff0000u) * up * up2)) : 0u;
+                *reinterpret_cast<uint4*>(q_s + ((r >> 7) * SUBS + (chunk >> 3)) * kSub + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (chunk == 0) ctl->row_scale[r] = !finite ? CUDART_NAN_F : fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2);
             }
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl->q_full);
+            named_barrier(all_barrier, 32 * kSoftmaxWarps);
         }
+        const float row_scale = ctl->row_scale[row - row0];
+        const bool there = row < n_rows;
+        const int token = min(row, n_rows - 1) / c.per, head = kvh * c.per + min(row, n_rows - 1) - token * c.per;
         const int place = place_of(row), first = first_of(place);
         const int w_row = row0 + g * kBM + quarter * 32;
         const int place_lo = place_of(w_row), first_hi = first_of(place_of(w_row + 31));            // of the warp's rows
         const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.25f * c.soft_cap);          // in its series' form
         const float exact_in = PLAIN ? 0.0f : 2.0f / c.soft_cap;
-        const float r1 = !PLAIN && c.distance != nullptr ? c.distance[head] : 0.0f, r2 = !PLAIN && c.distance != nullptr ? c.distance[c.n_head + head] : 0.0f;
         const bool biased = !PLAIN && c.distance != nullptr;
+        const float r1 = biased ? c.distance[head] : 0.0f, r2 = biased ? c.distance[c.n_head + head] : 0.0f;
+        const int lo = g == 0 ? g_lo[0] : g_lo[1], hi = g == 0 ? g_hi[0] : g_hi[1];
         float m = kLowest, l = 0.0f, big = kLeastExponent;                    // big: F, the largest exponent of value scales so far
         uint32_t nan_bits = 0;
-        bool ok = true;
-        for (int u = g_lo[g]; u < g_hi[g]; ++u) {
-            const int j = u >> 1, note = j % kNotes, part_of = (u & 1) * (kUnit / kBlockKeys), key0 = kv_lo + u * kUnit;
-            // A buffer of scores is filled every other unit, the first of the two that the range starts with first.
-            ok = wait(&ctl->s_full[g][u & 1], (uint32_t)((u - g_lo[g]) >> 1) & 1u, abort_flag);
-            // What the values' makers left of this tile is read once they are done.
-            if ((u & 1) == 0 || u == g_lo[g]) ok = ok && wait(&ctl->v_full[j % kStages], (j / kStages) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
+        bool ok = true, bad = false;
+        for (int u = lo; u < hi; ++u) {
+            const int note = (u >> 1) % kNotes, b0 = (u & 1) * (kUnit / kBlockKeys) + 2 * x, key0 = kv_lo + u * kUnit + 32 * x;
             const uint32_t t_u = t_s + (u & 1) * kUnit;
-            uint32_t v[2][32];
-            tmem_ld32(t_u, v[0]);
-            tmem_ld32(t_u + 32, v[1]);
-            float factor[4], exponent[4], high_exponent = big;
-            uint32_t gone = 0, nans = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                factor[b] = row_scale * ctl->k_factor[note][part_of + b];
-                exponent[b] = ctl->v_exponent[note][part_of + b];
-                high_exponent = fmaxf(high_exponent, exponent[b]);
-                gone |= ctl->gone[note][part_of + b];
-                nans |= ctl->nans[note][part_of + b];
-            }
-            const bool masked = key0 + kUnit - 1 > place_lo || key0 < first_hi || gone != 0;
-            tmem_ld_wait32(v[0]);
-            tmem_ld_wait32(v[1]);
+            // Both threads of a row give up, or neither: a wait that ran out is met at the barrier below.
+            ok = wait(&ctl->s_full[g][u & 1], (uint32_t)((u - lo) >> 1) & 1u, abort_flag);
+            tc_fence_after();
+            uint32_t v[32];
+            tmem_ld32(t_u + 32 * x, v);
+            float f0 = row_scale * ctl->k_factor[note][b0], f1 = row_scale * ctl->k_factor[note][b0 + 1];
+            const float e0 = ctl->v_exponent[note][b0], e1 = ctl->v_exponent[note][b0 + 1];
+            const uint32_t gone0 = ctl->gone[note][b0], gone1 = ctl->gone[note][b0 + 1], nans = ctl->nans[note][b0] | ctl->nans[note][b0 + 1];
+            const bool masked = key0 + 31 > place_lo || key0 < first_hi || (gone0 | gone1) != 0;
+            tmem_ld_wait32(v);
             if (!PLAIN || masked) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * (i < 16 ? f0 : f1));
+                f0 = f1 = 1.0f;
+                if constexpr (!PLAIN) {
+                    if (c.soft_cap > 0.0f) {
+                        // Where no score of the warp passes a quarter of the cap, the series of tanh (see lb_soft_cap); else 1 - 2 / (1 + e^2x).
+                        float size = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) * factor[2 * h + i / 16]);
-                    if constexpr (!PLAIN) {
-                        if (c.soft_cap > 0.0f) {
-                            // Where no score of the warp passes a quarter of the cap, the series of tanh (see lb_soft_cap); else 1 - 2 / (1 + e^2x).
-                            float size = 0.0f;
+                        for (int i = 0; i < 32; ++i) size = fmaxf(size, fabsf(__uint_as_float(v[i])));
+                        if (__all_sync(0xffffffffu, size <= 0.25f * capped.out)) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) size = fmaxf(size, fabsf(__uint_as_float(v[h][i])));
-                            if (__all_sync(0xffffffffu, size <= 0.25f * capped.out)) {
+                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(capped(__uint_as_float(v[i])));
+                        } else {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(capped(__uint_as_float(v[h][i])));
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    v[h][i] = __float_as_uint(fmaf(-2.0f * capped.out, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[h][i]) * exact_in)), capped.out));
-                            }
-                        }
-                        if (biased) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) - lb_distance_penalty_log2(r1, r2, max(place - (key0 + 32 * h + i), 0)));
+                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(-2.0f * capped.out, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[i]) * exact_in)), capped.out));
                         }
                     }
-                    if (masked) {
-                        // A bit a key that the row sees.
-                        const int from = first - (key0 + 32 * h), to = place - (key0 + 32 * h);
-                        uint32_t seen = (to >= 31 ? 0xffffffffu : to < 0 ? 0u : (2u << to) - 1u) & (from <= 0 ? 0xffffffffu : from > 31 ? 0u : ~((1u << from) - 1u));
-                        if (ctl->gone[note][part_of + 2 * h] != 0) seen &= 0xffff0000u;
-                        if (ctl->gone[note][part_of + 2 * h + 1] != 0) seen &= 0x0000ffffu;
+                    if (biased) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[h][i] = (seen >> i & 1u) != 0 ? v[h][i] : 0xff800000u;
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) - lb_distance_penalty_log2(r1, r2, max(place - (key0 + i), 0)));
                     }
                 }
+                if (masked) {
+                    // A bit a key that the row sees.
+                    const int from = first - key0, to = place - key0;
+                    uint32_t seen = (to >= 31 ? 0xffffffffu : to < 0 ? 0u : (2u << to) - 1u) & (from <= 0 ? 0xffffffffu : from > 31 ? 0u : ~((1u << from) - 1u));
+                    if (gone0 != 0) seen &= 0xffff0000u;
+                    if (gone1 != 0) seen &= 0x0000ffffu;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) factor[b] = 1.0f;
-            }
-            float high = kLowest;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                float h0 = __uint_as_float(v[b / 2][16 * (b & 1)]), h1 = __uint_as_float(v[b / 2][16 * (b & 1) + 1]);
-#pragma unroll
-                for (int i = 2; i < 16; i += 2) {
-                    h0 = fmaxf(h0, __uint_as_float(v[b / 2][16 * (b & 1) + i]));
-                    h1 = fmaxf(h1, __uint_as_float(v[b / 2][16 * (b & 1) + i + 1]));
+                    for (int i = 0; i < 32; ++i) v[i] = (seen >> i & 1u) != 0 ? v[i] : 0xff800000u;
                 }
-                high = fmaxf(high, fmaxf(h0, h1) * factor[b]);            // (a factor is not negative: a scale's sign is the query's)
             }
-            // O, the sum and p are relative to m, O in units of 2^big as well; where a score passes m by more than 2^8, or a block's exponent big, they move.
-            if (__any_sync(0xffffffffu, high > m + kSlack || high_exponent > big)) {
-                const float m_new = fmaxf(m, high), corr = ex2(m - m_new), corr_o = corr * ex2(big - high_exponent);
+            float h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = __uint_as_float(v[(i >> 1) * 16 + (i & 1)]);
+#pragma unroll
+            for (int i = 2; i < 16; ++i) {
+                h[i & 1] = fmaxf(h[i & 1], __uint_as_float(v[i]));
+                h[2 + (i & 1)] = fmaxf(h[2 + (i & 1)], __uint_as_float(v[16 + i]));
+            }
+            // (A factor is not negative: a scale's sign is the query's.)
+            float high = fmaxf(fmaxf(fmaxf(h[0], h[1]) * f0, fmaxf(h[2], h[3]) * f1), kLowest), high_exponent = fmaxf(fmaxf(e0, e1), big);
+            // O, the sum and p are relative to m, O in units of 2^big as well; where a score passes m by more than 2^8, or a block's exponent big, they move, for both threads of a row: the
+            // two warps ask each other.  By then both have their scores in registers, whose place p takes.
+            tc_fence_before();
+            const bool moved = any_of_pair(pair_barrier, !ok || high > m + kSlack || high_exponent > big);
+            tc_fence_after();
+            if (moved) {
+                ctl->row_high[g][x][quarter * 32 + lane] = ok ? high : CUDART_NAN_F;
+                ctl->row_sum[g][x][quarter * 32 + lane] = high_exponent;
+                named_barrier(pair_barrier, 64);
+                const float other = ctl->row_high[g][x ^ 1][quarter * 32 + lane];
+                high_exponent = fmaxf(high_exponent, ctl->row_sum[g][x ^ 1][quarter * 32 + lane]);
+                if (__any_sync(0xffffffffu, isnan(other)) || !ok) {
+                    ok = false;
+                    break;
+                }
+                const float m_new = fmaxf(fmaxf(m, high), other), corr = ex2(m - m_new), corr_o = corr * ex2(big - high_exponent);
                 l *= corr;
                 m = m_new;
                 big = high_exponent;
-                if (u > g_lo[g]) {
-                    ok = wait(&ctl->o_done[g], (uint32_t)(u - 1 - g_lo[g]) & 1u, abort_flag);
-                    if (!ok) break;
+                if (u > lo) {
+                    if (!wait(&ctl->o_done[g][(u - 1) & 1], (uint32_t)((u - 1 - lo) >> 1) & 1u, abort_flag)) {
+                        give_up(ctl, status, 6);
+                        bad = true;
+                    }
                     tc_fence_after();
                     uint32_t w[16];
 #pragma unroll 1
-                    for (int x = 0; x < HD / 16; ++x) {
-                        tmem_ld16(t_o + x * 16, w);
+                    for (int i = 0; i < HD / 32; ++i) {                  // each thread half of O
+                        tmem_ld16(t_o + i * 16, w);
                         tmem_ld_wait16(w);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * corr_o);
-                        tmem_st16(t_o + x * 16, w);
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * corr_o);
+                        tmem_st16(t_o + i * 16, w);
                     }
                 }
+                named_barrier(pair_barrier, 64);                         // both have read before the next are written
             }
             // p times 2^(a block's exponent less big) in one exponential; the sum of a block's is brought back.  (What lies 2^60 below the largest scale's is nothing beside it.)
+            uint32_t pk[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t pk[16];
+            for (int half = 0; half < 2; ++half) {
+                const float less = fmaxf((half == 0 ? e0 : e1) - big, -60.0f), from = less - m, factor = half == 0 ? f0 : f1;
+                float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int b = 2 * h + half;
-                    const float less = fmaxf(exponent[b] - big, -60.0f), ref = less - m;
-                    float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float p0 = ex2(fmaf(__uint_as_float(v[h][16 * half + i]), factor[b], ref)), p1 = ex2(fmaf(__uint_as_float(v[h][16 * half + i + 1]), factor[b], ref));
-                        sum0 += p0;
-                        sum1 += p1;
-                        pk[8 * half + i / 2] = h2(__floats2half2_rn(p0, p1));
-                    }
-                    l = fmaf(sum0 + sum1, ex2(-less), l);
+                for (int i = 0; i < 16; i += 2) {
+                    const float p0 = ex2(fmaf(__uint_as_float(v[16 * half + i]), factor, from)), p1 = ex2(fmaf(__uint_as_float(v[16 * half + i + 1]), factor, from));
+                    sum0 += p0;
+                    sum1 += p1;
+                    pk[8 * half + i / 2] = h2(__floats2half2_rn(p0, p1));
                 }
-                tmem_st16(t_u + h * 16, pk);               // over scores that have been read
+                l = fmaf(sum0 + sum1, ex2(-less), l);
             }
+            tmem_st16(t_u + x * 16, pk);
             if (nans != 0)
-                for (int i = 0; i < kUnit; ++i)
-                    if (key0 + i <= place && key0 + i >= first) nan_bits |= ctl->nan_groups[note][(u & 1) * kUnit + i];
+                for (int i = 0; i < 32; ++i)
+                    if (key0 + i <= place && key0 + i >= first) nan_bits |= ctl->nan_groups[note][(u & 1) * kUnit + 32 * x + i];
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl->p_full[g][u & 1]);
         }
-        // The last two updates may both be under way; a parity alone does not tell a phase from the one before the last.
-        if (ok && g_hi[g] > g_lo[g] + 1) ok = wait(&ctl->o_done[g], (uint32_t)(g_hi[g] - g_lo[g] - 2) & 1u, abort_flag);
-        if (ok && g_hi[g] > g_lo[g]) ok = wait(&ctl->o_done[g], (uint32_t)(g_hi[g] - g_lo[g] - 1) & 1u, abort_flag);
+        ok = ok && !bad;
+        // The last two updates may both be under way.
+        if (ok && hi > lo + 1) ok = wait(&ctl->o_done[g][hi & 1], (uint32_t)((hi - 2 - lo) >> 1) & 1u, abort_flag);
+        if (ok && hi > lo) ok = wait(&ctl->o_done[g][(hi - 1) & 1], (uint32_t)((hi - 1 - lo) >> 1) & 1u, abort_flag);
         if (!ok) give_up(ctl, status, 5);
+        // The threads' sums meet (a thread that gave up is here too), and each has half of the row's values.
+        ctl->row_sum[g][x][quarter * 32 + lane] = l;
+        ctl->row_nans[g][x][quarter * 32 + lane] = (uint8_t)nan_bits;
+        named_barrier(pair_barrier, 64);
+        l += ctl->row_sum[g][x ^ 1][quarter * 32 + lane];
+        nan_bits |= ctl->row_nans[g][x ^ 1][quarter * 32 + lane];
         if (ok && w_row < n_rows) {
             tc_fence_after();
             const bool none = l == 0.0f;                          // no key seen: O may be what the memory held
@@ -603,14 +619,14 @@ attention4_many_kernel(const Call c, int* status) {
             if (c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
             factor = factor / l * ex2(big * 0.5f);
             const float factor2 = ex2(big * 0.5f - 8.0f);                 // in two steps: big may be 2^127's exponent
-            __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD;
+            __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD + x * (HD / 2);
             const bool out_wide = reinterpret_cast<uintptr_t>(c.out) % 16 == 0 && c.out_stride % 8 == 0;
 #pragma unroll
-            for (int h = 0; h < HD / 32; ++h) {
+            for (int h = 0; h < HD / 64; ++h) {
                 uint32_t v[32];
                 tmem_ld32(t_o + h * 32, v);
                 tmem_ld_wait32(v);
-                const bool nan = (nan_bits >> (32 * h / (HD / NG)) & 1u) != 0;
+                const bool nan = (nan_bits >> ((x * (HD / 2) + 32 * h) / (HD / NG)) & 1u) != 0;
                 auto value = [&](int i) { return none ? 0.0f : nan ? CUDART_NAN_F : __uint_as_float(v[i]) * factor * factor2; };
                 if (!there) continue;
                 if (out_wide) {
