@@ -156,8 +156,54 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
 
 // A bounded wait, one answer for the warp.  Most find the phase done: one question then (mbar_wait's loop is 90 cycles of a warp that has the SM for itself, this 30).
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "vote.sync.all.pred q, p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok != 0) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+// Two multiply-adds, two additions, and the largest of three in one instruction each.
+__device__ __forceinline__ void fma2(float& d0, float& d1, uint32_t a0, uint32_t a1, float b, float c) {
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1) : "r"(a0), "r"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
+    asm("{\n\t.reg .b64 a, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\t"
+        "add.rn.f32x2 d, d, a;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
+// Numbers in twos: the pair, a number twice, products and multiply-adds.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ void of_two(Two a, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(a)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // Whether any of 64 threads says so; a barrier among them.
@@ -431,13 +477,15 @@ attention4_many_kernel(const Call c, int* status) {
         const int pair_barrier = 1 + g * 4 + quarter, all_barrier = 1 + 4 * kGroups;
         {
             // Sixteen rows a warp as float16 into shared memory, HD / 8 lanes a row, and the factors that bring their scores back.
-            constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, STEPS = 16 / AT_ONCE;
+            constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, STEPS = 4;
             const bool q_wide = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.q_stride % 8 == 0;
             const int chunk = lane % LANES;
+#pragma unroll 1
+            for (int from_row = warp * 16; from_row < warp * 16 + 16; from_row += STEPS * AT_ONCE) {         // (code that runs once costs its fetching)
             uint32_t u[STEPS][4];
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                const int r = row0 + warp * 16 + i * AT_ONCE + lane / LANES, token = r / c.per;
+                const int r = row0 + from_row + i * AT_ONCE + lane / LANES, token = r / c.per;
                 const __nv_bfloat16* from = c.q + (int64_t)(part.first + token) * c.q_stride + (int64_t)(kvh * c.per + r - token * c.per) * HD + 8 * chunk;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) u[i][e] = 0;
@@ -450,7 +498,7 @@ attention4_many_kernel(const Call c, int* status) {
             }
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                const int r = warp * 16 + i * AT_ONCE + lane / LANES;
+                const int r = from_row + i * AT_ONCE + lane / LANES;
                 uint32_t top = __vmaxu2(__vmaxu2(u[i][0] & 0x7fff7fffu, u[i][1] & 0x7fff7fffu), __vmaxu2(u[i][2] & 0x7fff7fffu, u[i][3] & 0x7fff7fffu));
                 top = max(top & 0xffffu, top >> 16);
 #pragma unroll
@@ -463,7 +511,9 @@ attention4_many_kernel(const Call c, int* status) {
                 for (int e = 0; e < 4; ++e)
                     w[e] = finite ? h2(__floats2half2_rn(__uint_as_float(u[i][e] << 16) * up * up2, __uint_as_float(u[i][e] & 0xffff0000u) * up * up2)) : 0u;
                 *reinterpret_cast<uint4*>(q_s + ((r >> 7) * SUBS + (chunk >> 3)) * kSub + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                if (chunk == 0) ctl->row_scale[r] = !finite ? CUDART_NAN_F : fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2);
+                // (Not 0, so that -inf stays what it is.)
+                if (chunk == 0) ctl->row_scale[r] = !finite ? CUDART_NAN_F : fmaxf(fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2), 1e-37f);
+            }
             }
             fence_async_shared();
             __syncwarp();
@@ -478,6 +528,7 @@ attention4_many_kernel(const Call c, int* status) {
         const int place_lo = place_of(w_row), first_hi = first_of(place_of(w_row + 31));            // of the warp's rows
         const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.25f * c.soft_cap);          // in its series' form
         const float exact_in = PLAIN ? 0.0f : 2.0f / c.soft_cap;
+        const Two cap_in = two(capped.in, capped.in);
         const bool biased = !PLAIN && c.distance != nullptr;
         const float r1 = biased ? c.distance[head] : 0.0f, r2 = biased ? c.distance[c.n_head + head] : 0.0f;
         const int lo = g == 0 ? g_lo[0] : g_lo[1], hi = g == 0 ? g_hi[0] : g_hi[1];
@@ -498,18 +549,21 @@ attention4_many_kernel(const Call c, int* status) {
             const bool masked = key0 + 31 > place_lo || key0 < first_hi || (gone0 | gone1) != 0;
             tmem_ld_wait32(v);
             if (!PLAIN || masked) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * (i < 16 ? f0 : f1));
-                f0 = f1 = 1.0f;
                 if constexpr (!PLAIN) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) of_two(mul2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), i < 16 ? two(f0, f0) : two(f1, f1)), v[i], v[i + 1]);
+                    f0 = f1 = 1.0f;
                     if (c.soft_cap > 0.0f) {
                         // Where no score of the warp passes a quarter of the cap, the series of tanh (see lb_soft_cap); else 1 - 2 / (1 + e^2x).
                         float size = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) size = fmaxf(size, fabsf(__uint_as_float(v[i])));
+                        for (int i = 0; i < 32; i += 2) size = max3(size, fabsf(__uint_as_float(v[i])), fabsf(__uint_as_float(v[i + 1])));
                         if (__all_sync(0xffffffffu, size <= 0.25f * capped.out)) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(capped(__uint_as_float(v[i])));
+                            for (int i = 0; i < 32; i += 2) {
+                                const Two z = two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), w = mul2(z, cap_in), y = mul2(w, w);
+                                of_two(fma2(mul2(z, y), fma2(y, fma2(y, two(-17.0f / 315.0f, -17.0f / 315.0f), two(2.0f / 15.0f, 2.0f / 15.0f)), two(-1.0f / 3.0f, -1.0f / 3.0f)), z), v[i], v[i + 1]);
+                            }
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(-2.0f * capped.out, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[i]) * exact_in)), capped.out));
@@ -530,16 +584,18 @@ attention4_many_kernel(const Call c, int* status) {
                     for (int i = 0; i < 32; ++i) v[i] = (seen >> i & 1u) != 0 ? v[i] : 0xff800000u;
                 }
             }
-            float h[4];
+            float h[2][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = __uint_as_float(v[(i >> 1) * 16 + (i & 1)]);
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int i = 2; i < 16; ++i) {
-                h[i & 1] = fmaxf(h[i & 1], __uint_as_float(v[i]));
-                h[2 + (i & 1)] = fmaxf(h[2 + (i & 1)], __uint_as_float(v[16 + i]));
-            }
+                for (int e = 0; e < 2; ++e) {
+                    h[half][e] = __uint_as_float(v[16 * half + 8 * e]);
+#pragma unroll
+                    for (int i = 1; i < 7; i += 2) h[half][e] = max3(h[half][e], __uint_as_float(v[16 * half + 8 * e + i]), __uint_as_float(v[16 * half + 8 * e + i + 1]));
+                    h[half][e] = fmaxf(h[half][e], __uint_as_float(v[16 * half + 8 * e + 7]));
+                }
             // (A factor is not negative: a scale's sign is the query's.)
-            float high = fmaxf(fmaxf(fmaxf(h[0], h[1]) * f0, fmaxf(h[2], h[3]) * f1), kLowest), high_exponent = fmaxf(fmaxf(e0, e1), big);
+            float high = max3(fmaxf(h[0][0], h[0][1]) * f0, fmaxf(h[1][0], h[1][1]) * f1, kLowest), high_exponent = fmaxf(fmaxf(e0, e1), big);
             // O, the sum and p are relative to m, O in units of 2^big as well; where a score passes m by more than 2^8, or a block's exponent big, they move, for both threads of a row: the
             // two warps ask each other.  By then both have their scores in registers, whose place p takes.
             tc_fence_before();
@@ -585,9 +641,11 @@ attention4_many_kernel(const Call c, int* status) {
                 float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(v[16 * half + i]), factor, from)), p1 = ex2(fmaf(__uint_as_float(v[16 * half + i + 1]), factor, from));
-                    sum0 += p0;
-                    sum1 += p1;
+                    float p0, p1;
+                    fma2(p0, p1, v[16 * half + i], v[16 * half + i + 1], factor, from);
+                    p0 = ex2(p0);
+                    p1 = ex2(p1);
+                    add2(sum0, sum1, p0, p1);
                     pk[8 * half + i / 2] = h2(__floats2half2_rn(p0, p1));
                 }
                 l = fmaf(sum0 + sum1, ex2(-less), l);
@@ -621,7 +679,7 @@ attention4_many_kernel(const Call c, int* status) {
             const float factor2 = ex2(big * 0.5f - 8.0f);                 // in two steps: big may be 2^127's exponent
             __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD + x * (HD / 2);
             const bool out_wide = reinterpret_cast<uintptr_t>(c.out) % 16 == 0 && c.out_stride % 8 == 0;
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < HD / 64; ++h) {
                 uint32_t v[32];
                 tmem_ld32(t_o + h * 32, v);
