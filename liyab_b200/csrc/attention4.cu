@@ -3,6 +3,7 @@
 #include "linear4.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -45,28 +46,30 @@ attention4_mass_kernel(const Call c, const Mass w) {
 
 constexpr int kMostMassTokens = 64;
 
-// Which kernel takes a call.
-bool takes_many(const lb_attention4_args& a, int max_rows) { return a.total == nullptr && max_rows > 64; }
-
-struct Scratch {
-    int64_t scores, log_sums, partial, starts, bytes;       // offsets
+// How a call runs.
+struct Plan {
+    bool many;
+    RowsPlan rows;
+    TilesPlan tiles;
+    int64_t scores, log_sums, partial, starts, bytes;       // offsets in the scratch memory
 };
-Scratch scratch_of(const lb_attention4_args& a, const RowsPlan& p, int max_rows, int score_keys) {
-    auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
-    Scratch s = {};
-    const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
-    if (a.total != nullptr) {
-        s.log_sums = up(units * max_rows * score_keys * 4);
-        s.bytes = s.log_sums + up(units * max_rows * 4);
-    }
-    if (takes_many(a, max_rows)) return s;
-    s.partial = s.bytes;
-    s.starts = s.partial + up(p.states);
-    s.bytes = s.starts + up(p.starts);
-    return s;
+
+// Whether the tcgen05 kernel takes a call: by an estimate of both in microseconds, from their times on 84 calls of 1 to 128 tokens a request (1 and 8 requests on 256, 2,048 and 16,384 keys, 32 heads over
+// 8 of 128 and 12 over 12 of 64).  The kernel for few rows: a start and an end, and what a warp takes for sixteen keys and a tile of rows, all warps of the GPU side by side.  The other: a start, an
+// end and a join of states, and what a block takes for 128 keys, which is little less where it has 128 rows or fewer.  (8 requests on 2,048 keys, 32 heads over 8: 8 tokens each 34 / 36 us, 16
+// tokens 52 / 36; 1 request on 2,048 keys: 32 tokens 20 / 24, 128 tokens 51 / 32.)
+bool takes_many(const lb_attention4_args& a, int max_rows, int keys, const RowsPlan& few, const TilesPlan& many, int n_sm) {
+    if (a.total != nullptr) return false;
+    const bool wide = a.cache->head_dim == 128;
+    const double units = (double)a.n_seq * a.cache->n_kv_head;
+    const double tile = few.rows == 4 ? (wide ? 0.00043 : 0.00027) : wide ? 0.00068 : 0.0004;
+    const double few_us = 10.0 + units * few.tiles * ((keys + 15) / 16) * tile;
+    const double blocks = units * ((max_rows + 255) / 256) * many.splits, each = ((keys + 127) / 128 + many.splits - 1) / many.splits;
+    const double many_us = (many.splits > 1 ? 12.0 : 9.0) + std::ceil(blocks / n_sm) * each * (max_rows <= 128 ? (wide ? 2.5 : 1.9) : wide ? 2.9 : 2.6);
+    return many_us < few_us;
 }
 
-int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch) {
+int check(const lb_attention4_args* args, Call* c, Plan* p) {
     LB_CHECK_ARG(args != nullptr, "attention4: no arguments");
     const lb_attention4_args& a = *args;
     if (int rc = lb_c4::pages_of(a.cache, "attention4", &c->pages)) return rc;
@@ -77,11 +80,12 @@ int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch
     LB_CHECK_ARG(a.max_keys > 0 && a.table_stride > 0 && (int64_t)a.table_stride * a.cache->page_size <= INT32_MAX, "attention4: up to %d keys, tables of %d pages", a.max_keys,
                  a.table_stride);
     const int64_t rows = (int64_t)a.max_q_len * (a.n_head / a.cache->n_kv_head);
-    LB_CHECK_ARG(rows <= 1 << 22 && (rows + 7) / 8 * a.cache->n_kv_head <= 65535, "attention4: %d tokens of %d heads are more than one launch takes", a.max_q_len, a.n_head);
+    LB_CHECK_ARG(rows <= 1 << 22 && (rows + 7) / 8 * a.cache->n_kv_head <= 1 << 22 && a.cache->n_kv_head <= 65535, "attention4: %d tokens of %d heads are more than one launch takes", a.max_q_len,
+                 a.n_head);
     LB_CHECK_ARG(a.total == nullptr || (a.mass != nullptr && a.max_q_len <= kMostMassTokens), "attention4: the keys' weights come from portions of up to %d tokens", kMostMassTokens);
     LB_CHECK_ARG(a.total == nullptr || (a.n_mass >= 0 && a.mass_stride >= 0 && a.mass_head_stride >= 0 && a.total_stride >= 0 && a.total_head_stride >= 0),
                  "attention4: weights of no size");
-    const int score_keys = std::min(a.max_keys, a.table_stride * a.cache->page_size);
+    const int keys = std::min(a.max_keys, a.table_stride * a.cache->page_size), n_sm = linear4_sm_count();
     c->q = static_cast<const __nv_bfloat16*>(a.q);
     c->q_start = a.q_start;
     c->last = a.last;
@@ -97,18 +101,31 @@ int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch
     c->n_head = a.n_head;
     c->per = a.n_head / a.cache->n_kv_head;
     c->max_rows = (int)rows;
-    c->score_keys = score_keys;
+    c->score_keys = keys;
     c->max_keys = a.max_keys;
     c->window = a.window;
     c->scale = a.scale;
     c->soft_cap = a.soft_cap;
-    if (int rc = rows_plan(p, a.n_seq, a.cache->n_kv_head, (int)rows, score_keys, a.cache->head_dim, linear4_sm_count())) return rc;
-    *scratch = scratch_of(a, *p, (int)rows, score_keys);
+    // What lies in the scratch memory: scores and divisors for the keys' weights, states, where requests' tiles start.
+    auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+    const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
+    if (int rc = rows_plan(&p->rows, a.n_seq, a.cache->n_kv_head, (int)rows, keys, a.cache->head_dim, n_sm)) return rc;
+    p->tiles = tiles_plan(a.n_seq, a.cache->n_kv_head, (int)rows, keys, a.cache->head_dim, n_sm);
+    p->many = takes_many(a, (int)rows, keys, p->rows, p->tiles, n_sm);
+    p->scores = 0;
+    p->log_sums = a.total != nullptr ? up(units * rows * keys * 4) : 0;
+    p->partial = p->log_sums + (a.total != nullptr ? up(units * rows * 4) : 0);
+    if (p->many) {
+        p->starts = p->bytes = p->partial + up(p->tiles.states);
+    } else {
+        p->starts = p->partial + up(p->rows.states);
+        p->bytes = p->starts + up(p->rows.starts);
+    }
     uint8_t* at = static_cast<uint8_t*>(a.scratch);
-    c->scores = a.total != nullptr ? reinterpret_cast<float*>(at) : nullptr;
-    c->log_sums = a.total != nullptr ? reinterpret_cast<float*>(at + scratch->log_sums) : nullptr;
-    c->partial = reinterpret_cast<float*>(at + scratch->partial);
-    c->starts = reinterpret_cast<int*>(at + scratch->starts);
+    c->scores = a.total != nullptr ? reinterpret_cast<float*>(at + p->scores) : nullptr;
+    c->log_sums = a.total != nullptr ? reinterpret_cast<float*>(at + p->log_sums) : nullptr;
+    c->partial = reinterpret_cast<float*>(at + p->partial);
+    c->starts = reinterpret_cast<int*>(at + p->starts);
     return LB_OK;
 }
 
@@ -116,40 +133,37 @@ int check(const lb_attention4_args* args, Call* c, RowsPlan* p, Scratch* scratch
 
 extern "C" int64_t lb_attention4_scratch(const lb_attention4_args* args) {
     Call c;
-    RowsPlan p;
-    Scratch s;
-    return check(args, &c, &p, &s) == LB_OK ? s.bytes : 0;
+    Plan p;
+    return check(args, &c, &p) == LB_OK ? p.bytes : 0;
 }
 
 extern "C" int lb_attention4_plan(const lb_attention4_args* args, int* plan) {
     Call c;
-    RowsPlan p;
-    Scratch s;
+    Plan p;
     LB_CHECK_ARG(plan != nullptr, "attention4: no place for the plan");
-    if (int rc = check(args, &c, &p, &s)) return rc;
-    plan[0] = takes_many(*args, c.max_rows) ? 1 : 0;
-    plan[1] = p.rows;
-    plan[2] = p.blocks;
-    plan[3] = p.per_row;
+    if (int rc = check(args, &c, &p)) return rc;
+    plan[0] = p.many ? 1 : 0;
+    plan[1] = p.many ? 256 : p.rows.rows;
+    plan[2] = p.many ? p.tiles.splits : p.rows.blocks;
+    plan[3] = p.many ? 1 : p.rows.per_row;
     return LB_OK;
 }
 
 extern "C" int lb_attention4(const lb_attention4_args* args) {
     Call c;
-    RowsPlan p;
-    Scratch s;
-    if (int rc = check(args, &c, &p, &s)) return rc;
+    Plan p;
+    if (int rc = check(args, &c, &p)) return rc;
     const lb_attention4_args& a = *args;
     if (a.n_seq == 0 || a.n_tokens == 0) return LB_OK;
     LB_CHECK_ARG(a.q != nullptr && a.last != nullptr && a.block_table != nullptr && a.out != nullptr, "attention4: a pointer is missing");
     LB_CHECK_ARG(reinterpret_cast<uintptr_t>(a.q) % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % 2 == 0, "attention4: pointers off their type's alignment");
     const int64_t width = (int64_t)a.n_head * a.cache->head_dim;
     LB_CHECK_ARG(a.n_tokens < 2 || (a.q_stride >= width && a.out_stride >= width), "attention4: rows overlap");
-    LB_CHECK_ARG(s.bytes == 0 || (a.scratch != nullptr && reinterpret_cast<uintptr_t>(a.scratch) % 16 == 0), "attention4: scratch memory is missing or not 16-byte aligned");
+    LB_CHECK_ARG(p.bytes == 0 || (a.scratch != nullptr && reinterpret_cast<uintptr_t>(a.scratch) % 16 == 0), "attention4: scratch memory is missing or not 16-byte aligned");
     if (int rc = device_check("attention4", a.cache->device)) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-    if (takes_many(a, c.max_rows)) return many_rows(c, a.cache->head_dim, stream);
-    if (int rc = few_rows(c, a.cache->head_dim, p, stream)) return rc;
+    if (p.many) return many_rows(c, a.cache->head_dim, p.tiles, stream);
+    if (int rc = few_rows(c, a.cache->head_dim, p.rows, stream)) return rc;
     if (a.total != nullptr) {
         const Mass w = {a.mass, a.total, a.mass_rows, a.mass_stride, a.mass_head_stride, a.total_stride, a.total_head_stride, a.n_mass};
         LB_CHECK_CUDA(lb_launch_overlapped(attention4_mass_kernel, dim3((c.score_keys + 255) / 256, a.cache->n_kv_head, a.n_seq), dim3(256), 0, stream, c, w));

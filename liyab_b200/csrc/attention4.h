@@ -41,15 +41,20 @@ __device__ __forceinline__ Portion portion_of(const Call& c, int s) {
     return p;
 }
 
-// How the kernel for few rows cuts a call: rows a tile (8 or 16), row tiles a request and key/value head, requests a launch row, blocks of a row, warps that join a row's
+// How the kernel for few rows cuts a call: rows a tile (4 or 8), row tiles a request and key/value head, requests a launch row, blocks of a row, warps that join a row's
 // states, bytes of the states and of the requests' starts.
 struct RowsPlan {
     int rows, tiles, per_row, blocks, join_team;
     int64_t states, starts;
 };
 int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
-// Portions of many rows, on tcgen05.
-int many_rows(const Call& c, int head_dim, cudaStream_t stream);
+// Portions of many rows, on tcgen05: blocks that share a row tile's keys, bytes of their states.
+struct TilesPlan {
+    int splits;
+    int64_t states;
+};
+TilesPlan tiles_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+int many_rows(const Call& c, int head_dim, const TilesPlan& p, cudaStream_t stream);
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t stream);
 
 }  // namespace lb_a4

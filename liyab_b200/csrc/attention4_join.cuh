@@ -1,0 +1,88 @@
+// The states of one query row over parts of its keys become its result: what both attention kernels over a 4-bit cache end with.
+#pragma once
+
+#include "attention4.h"
+
+#include <float.h>
+#include <math_constants.h>
+
+namespace lb_a4 {
+namespace {
+
+constexpr float kLowest = -FLT_MAX;            // a reference before any score; finite, so that differences with it are numbers
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A state: [reference, sum, two places, HD values], the sums relative to 2^reference.  A team of warps (a power of two of the block's, 32 at most) has a row, a lane HD / 32 neighbouring values; the warps
+// take the states in turn, and their sums meet in their order.  All threads of the block call it; state is null for rows that are not there.
+template <int HD>
+__device__ __forceinline__ void join_row(const Call& c, const Portion& part, int seq, int kvh, int r, const float* state, int64_t step, int runs, int team_shift, float (*joined)[HD + 2]) {
+    constexpr int V = HD / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = 1 << team_shift, mine = warp & (team - 1);
+    float m = kLowest, l = 0.0f, v[V] = {};
+    if (state != nullptr) {
+        // Thirty-two at a time: a lane has a state's reference and sum, and its factor once the largest reference is known.
+        for (int i0 = mine; i0 < runs; i0 += 32 * team) {
+            float2 ml = make_float2(kLowest, 0.0f);
+            if (i0 + lane * team < runs) ml = *reinterpret_cast<const float2*>(state + (i0 + lane * team) * step);
+            const bool some = ml.y != 0.0f;                 // (a NaN is some)
+            float high = some ? ml.x : kLowest;
+#pragma unroll
+            for (int x = 16; x > 0; x /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+            high = fmaxf(high, m);
+            const float w = some ? ex2(ml.x - high) : 0.0f, keep = ex2(m - high);
+            l = fmaf(l, keep, lb_warp_sum(some ? ml.y * w : 0.0f));
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] *= keep;
+            m = high;
+            const int n = min(32, (runs - i0 + team - 1) >> team_shift);
+            const float* at = state + i0 * step + 4 + V * lane;
+#pragma unroll 4
+            for (int x = 0; x < n; ++x, at += team * step) {
+                const float f = __shfl_sync(0xffffffffu, w, x);
+                float o[V];
+                if constexpr (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(at);
+                else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(at);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = fmaf(o[e], f, v[e]);
+            }
+        }
+    }
+    if (team > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) joined[warp][2 + V * lane + e] = v[e];
+        if (lane == 0) {
+            joined[warp][0] = m;
+            joined[warp][1] = l;
+        }
+        __syncthreads();
+        if (mine > 0) return;
+        for (int i = 1; i < team; ++i) {
+            const float mi = joined[warp + i][0], li = joined[warp + i][1], high = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : ex2(mi - high), keep = ex2(m - high);
+            l = fmaf(l, keep, li * w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = fmaf(v[e], keep, joined[warp + i][2 + V * lane + e] * w);
+            m = high;
+        }
+    }
+    if (state == nullptr) return;
+    const int token = part.count == 1 ? 0 : r / c.per, head = kvh * c.per + r - token * c.per;
+    float top = m, factor = 1.0f;
+    if (c.sink != nullptr) {
+        const float sink = c.sink[head] * kLbLog2e;
+        top = fmaxf(m, sink);
+        factor = lb_sink_join_exp2(sink, m, l);
+    }
+    factor = l == 0.0f ? 0.0f : __fdividef(factor, l);
+    __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + head * HD + V * lane;
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = __float2bfloat16_rn(v[e] * factor);
+    if (lane == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + r] = l == 0.0f ? CUDART_INF_F : top + log2f(l);
+}
+
+}  // namespace
+}  // namespace lb_a4

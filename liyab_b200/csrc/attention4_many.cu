@@ -13,6 +13,7 @@
 // A value scale that is NaN would meet p = 0 of rows that do not see its key in the products: such groups are made zeros, and the rows that see them take a note (a bit a group) and end as NaN.
 // Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results.
 #include "attention4.h"
+#include "attention4_join.cuh"
 #include "tcgen05.cuh"
 
 #include <cuda_fp16.h>
@@ -37,7 +38,7 @@ constexpr int kManyThreads = 32 * (kIssuer + 4);         // (the last two warps 
 constexpr int kSoftmaxRegs = 80, kMakerRegs = 72, kIssuerRegs = 40;
 constexpr int kSub = 128 * 128;                // [128 rows][128 bytes]: 64 values of a tile
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
-constexpr float kLowest = -FLT_MAX, kSlack = 8.0f, kLeastExponent = -100.0f;
+constexpr float kSlack = 8.0f, kLeastExponent = -100.0f;
 
 struct Control {
     uint64_t q_full;
@@ -56,11 +57,6 @@ struct Control {
 __device__ __forceinline__ void give_up(Control* c, int* status, int site) {
     atomicCAS(status, 0, (0xC << 12) | site);
     *(volatile int*)&c->abort_flag = 1;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 template <int N>
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -220,7 +216,7 @@ __device__ __forceinline__ bool any_of_pair(int barrier, bool mine) {
 
 template <int HD, int NG, bool PLAIN>
 __global__ void __launch_bounds__(kManyThreads, 1)
-attention4_many_kernel(const Call c, int* status) {
+attention4_many_kernel(const Call c, int n_splits, int* status) {
     using L = Layout<HD>;
     constexpr int SUBS = HD / 64, JK = HD / 32, JV = HD / 64;
     extern __shared__ uint8_t smem_raw[];
@@ -236,21 +232,23 @@ attention4_many_kernel(const Call c, int* status) {
     lb_dependents_may_launch();
     const int seq = blockIdx.z, kvh = blockIdx.y, kv = c.pages.n_kv_head;
     const Portion part = portion_of(c, seq);
-    // The last tiles first, which see the most keys.
-    const int n_rows = part.count * c.per, row0 = ((n_rows + kTileRows - 1) / kTileRows - 1 - (int)blockIdx.x) * kTileRows;
+    // The last tiles first, which see the most keys; `n_splits` blocks share a tile's.
+    const int split = (int)blockIdx.x % n_splits;
+    const int n_rows = part.count * c.per, row0 = ((n_rows + kTileRows - 1) / kTileRows - 1 - (int)blockIdx.x / n_splits) * kTileRows;
     if (row0 < 0 || n_rows <= 0) return;
     const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;          // no key past this place is read
     auto place_of = [&](int row) { return min(part.place + min(row, n_rows - 1) / c.per, limit); };
     auto first_of = [&](int place) { return place < 0 ? 0 : lb_first_visible(place, c.window); };
-    const int p_hi = place_of(row0 + kTileRows - 1), kv_lo = first_of(place_of(row0)) / kBN * kBN;
-    const int n_tiles = p_hi >= 0 ? (p_hi - kv_lo) / kBN + 1 : 0;
+    const int last = place_of(row0 + kTileRows - 1), all_lo = first_of(place_of(row0)) / kBN * kBN, all_tiles = last >= 0 ? (last - all_lo) / kBN + 1 : 0;
+    const int share = (all_tiles + n_splits - 1) / n_splits, kv_lo = all_lo + split * share * kBN;
+    const int n_tiles = max(0, min(share, all_tiles - split * share)), p_hi = min(last, kv_lo + n_tiles * kBN - 1);
     // Whether rows of group g see keys of unit u.
     int g_lo[kGroups], g_hi[kGroups];                               // units
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        const int from = row0 + g * kBM, hi = place_of(from + kBM - 1);
-        const bool some = from < n_rows && hi >= 0;
-        g_lo[g] = some ? (first_of(place_of(from)) - kv_lo) / kUnit : 0;
+        const int from = row0 + g * kBM, hi = min(place_of(from + kBM - 1), p_hi), first = max(first_of(place_of(from)), kv_lo);
+        const bool some = from < n_rows && hi >= first && n_tiles > 0;
+        g_lo[g] = some ? (first - kv_lo) / kUnit : 0;
         g_hi[g] = some ? (hi - kv_lo) / kUnit + 1 : 0;
     }
     auto active = [&](int g, int u) { return u >= g_lo[g] && u < g_hi[g]; };
@@ -672,9 +670,12 @@ attention4_many_kernel(const Call c, int* status) {
         nan_bits |= ctl->row_nans[g][x ^ 1][quarter * 32 + lane];
         if (ok && w_row < n_rows) {
             tc_fence_after();
-            const bool none = l == 0.0f;                          // no key seen: O may be what the memory held
+            // A row's result; where blocks share its keys a state, normed so that its sum is 1.
+            const bool none = l == 0.0f, whole = n_splits == 1;                          // no key seen: O may be what the memory held
+            float* state = c.partial + ((((int64_t)seq * kv + kvh) * c.max_rows + row) * n_splits + split) * (HD + 4);
+            if (!whole && there && x == 0) *reinterpret_cast<float2*>(state) = make_float2(none ? kLowest : m + log2f(l), none ? 0.0f : 1.0f);
             float factor = 1.0f;
-            if (c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
+            if (whole && c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
             factor = factor / l * ex2(big * 0.5f);
             const float factor2 = ex2(big * 0.5f - 8.0f);                 // in two steps: big may be 2^127's exponent
             __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD + x * (HD / 2);
@@ -687,7 +688,11 @@ attention4_many_kernel(const Call c, int* status) {
                 const bool nan = (nan_bits >> ((x * (HD / 2) + 32 * h) / (HD / NG)) & 1u) != 0;
                 auto value = [&](int i) { return none ? 0.0f : nan ? CUDART_NAN_F : __uint_as_float(v[i]) * factor * factor2; };
                 if (!there) continue;
-                if (out_wide) {
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(state + 4 + x * (HD / 2) + 32 * h + i) = make_float4(value(i), value(i + 1), value(i + 2), value(i + 3));
+                } else if (out_wide) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8)
                         *reinterpret_cast<uint4*>(out + 32 * h + i) =
@@ -708,23 +713,46 @@ attention4_many_kernel(const Call c, int* status) {
     }
 }
 
+// The states of blocks that share a row's keys.
+template <int HD>
+__global__ void __launch_bounds__(128)
+attention4_many_join_kernel(const Call c, int n_splits) {
+    __shared__ float joined[1][HD + 2];
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    const int seq = blockIdx.z, kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const Portion part = portion_of(c, seq);
+    const float* state = r < part.count * c.per ? c.partial + (((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + r) * n_splits * (HD + 4) : nullptr;
+    join_row<HD>(c, part, seq, kvh, r, state, HD + 4, n_splits, 0, joined);
+}
+
 template <int HD, int NG>
-int launch(const Call& c, cudaStream_t s) {
+int launch(const Call& c, const TilesPlan& p, cudaStream_t s) {
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
     const bool plain = c.distance == nullptr && c.soft_cap <= 0.0f;
     auto kernel = plain ? attention4_many_kernel<HD, NG, true> : attention4_many_kernel<HD, NG, false>;
     constexpr int smem = 1024 + (kGroups + 2 * kStages) * (HD / 64) * kSub + (int)sizeof(Control);
     LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, status));
+    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows * p.splits, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, p.splits, status));
+    if (p.splits > 1) LB_CHECK_CUDA(lb_launch_overlapped(attention4_many_join_kernel<HD>, dim3((c.max_rows + 3) / 4, c.pages.n_kv_head, c.n_seq), dim3(128), 0, s, c, p.splits));
     return LB_OK;
 }
 
 }  // namespace
 
-int many_rows(const Call& c, int head_dim, cudaStream_t s) {
-    if (head_dim == 64) return c.pages.groups == 1 ? launch<64, 1>(c, s) : launch<64, 2>(c, s);
-    return c.pages.groups == 1 ? launch<128, 1>(c, s) : c.pages.groups == 2 ? launch<128, 2>(c, s) : launch<128, 4>(c, s);
+TilesPlan tiles_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
+    // As many blocks as SMs, with two tiles of keys each at least.
+    const int64_t blocks = (int64_t)std::max(1, n_seq) * n_kv_head * ((max_rows + kTileRows - 1) / kTileRows);
+    TilesPlan p;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({n_sm / blocks, (int64_t)(max_keys + 2 * kBN - 1) / (2 * kBN), 32}));
+    p.states = p.splits > 1 ? (int64_t)std::max(1, n_seq) * n_kv_head * max_rows * p.splits * (head_dim + 4) * 4 : 0;
+    return p;
+}
+
+int many_rows(const Call& c, int head_dim, const TilesPlan& p, cudaStream_t s) {
+    if (head_dim == 64) return c.pages.groups == 1 ? launch<64, 1>(c, p, s) : launch<64, 2>(c, p, s);
+    return c.pages.groups == 1 ? launch<128, 1>(c, p, s) : c.pages.groups == 2 ? launch<128, 2>(c, p, s) : launch<128, 4>(c, p, s);
 }
 
 }  // namespace lb_a4

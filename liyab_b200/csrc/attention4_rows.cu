@@ -13,6 +13,7 @@
 // 2^8, or a scale f: the warp votes, which costs a few instructions a tile where searching the maximum cost thirty.
 // The warps' states meet in shared memory in their order, the ranges' in the shared memory of a cluster (up to 16), or in memory in another launch.
 #include "attention4.h"
+#include "attention4_join.cuh"
 #include "tcgen05.cuh"
 
 #include <cuda_fp16.h>
@@ -26,17 +27,11 @@ namespace {
 
 using namespace lb_c4;
 
-constexpr int kStages = 4;
-constexpr float kLowest = -FLT_MAX;            // a reference before any score; finite, so that differences with it are numbers
+constexpr int kStages = 3;                     // pairs of tiles in a warp's ring
 constexpr float kSlack = 8.0f;                 // how far a score may pass its row's reference (base 2)
 constexpr float kLeastScale = -80.0f;          // the exponent of the largest value scale, before any
 constexpr float kRoom = 6.0f;                  // p s reaches 2^(kRoom + kSlack) = 2^14 of float16's 2^16; what lies 2^-30 below the largest scale loses bits
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // 2^n, n in -126 .. 127.
 __device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -98,7 +93,7 @@ constexpr int kMostRequests = 1024;            // of a launch row (grid.y)
 constexpr int kLeastTiles = 4;                 // of a warp
 
 // Blocks an SM.
-__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return nt == 1 ? (hd == 64 ? 5 : 4) : nt == 2 ? (hd == 64 ? 4 : 3) : 2; }
+__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return nt == 1 ? (hd == 64 ? 5 : 4) : hd == 64 ? 4 : 3; }
 
 // The blocks of keys of a request that any of its rows sees: the first and how many.
 __device__ __forceinline__ void tiles_of(const Call& c, const Portion& p, int* first, int* count) {
@@ -112,6 +107,19 @@ __device__ __forceinline__ void tiles_of(const Call& c, const Portion& p, int* f
 __host__ __device__ __forceinline__ int share_of(int total, int n_warps) {
     const int even = (total + n_warps - 1) / n_warps;
     return even > kLeastTiles ? even : kLeastTiles;
+}
+
+// A bounded wait, one answer for the warp; most find the phase done.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "vote.sync.all.pred q, p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok) : "r"(lb_tc::smem_u32(bar)), "r"(parity) : "memory");
+    if (ok != 0) return true;
+    return __all_sync(0xffffffffu, lb_tc::mbar_wait(bar, parity, nullptr));
 }
 
 // NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.
@@ -128,12 +136,12 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ int found[kWarps][64];                      // the cache's blocks of the tiles to come; -1: on no page
-    int* starts = reinterpret_cast<int*>(smem + kWarps * kStages * kBlock);
+    int* starts = reinterpret_cast<int*>(smem + kWarps * kStages * 2 * kBlock);
     int* firsts = starts + per_row + 1;
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int seq0 = blockIdx.y * per_row, n_seq = min(per_row, c.n_seq - seq0), kv = c.pages.n_kv_head;
-    if (lane < kStages) lb_tc::mbar_init(&bars[warp][lane], 1);
+    if (lane < kStages) lb_tc::mbar_init(&bars[warp][lane], 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
@@ -180,15 +188,15 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     };
     auto row_tiles_of = [&](const Portion& p) { return c.q_start == nullptr ? tiles : (p.count * c.per + kRows - 1) / kRows; };
 
-    uint8_t* ring = smem + warp * kStages * kBlock;
+    uint8_t* ring = smem + warp * kStages * 2 * kBlock;
     const int n_tiles = end - begin;
-    int listed = 0, asked = 0;                             // tiles whose blocks are found, tiles asked for
-    uint32_t missing = 0;                                  // a bit a stage: its keys are on no page
-    // Asks for the next n tiles (up to a ring), a lane each.
-    auto fetch = [&](int n) {
-        n = min(n, n_tiles - asked);
-        if (n <= 0) return;
-        if (asked + n > listed) {
+    // Tiles come in pairs, counted from the warp's first: a barrier a pair, on which two lanes arrive with a tile each.
+    const int n_pairs = (n_tiles + 1) >> 1;
+    int listed = 0, asked = 0;                             // tiles whose blocks are found, pairs asked for
+    bool all_there = true;                                 // no tile listed so far is on no page
+    auto fetch = [&]() {
+        if (asked >= n_pairs) return;
+        if (2 * asked + 2 > listed) {
             const int x = begin + listed + lane;
             int at = -1;
             if (x < end) {
@@ -198,24 +206,24 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                 if ((unsigned)page < (unsigned)c.pages.n_pages) at = ((page * kv + kvh) << (c.pages.page_shift - 4)) + (tile & ((1 << (c.pages.page_shift - 4)) - 1));
             }
             found[warp][(listed + lane) & 63] = at;
+            all_there = all_there && __all_sync(0xffffffffu, at >= 0 || x >= end);
             listed += 32;
             __syncwarp();
         }
-        const int mine = asked + lane, stage = mine % kStages, at = found[warp][mine & 63];
-        const bool here = lane < n;
-        if (here && at >= 0) {
-            lb_tc::mbar_expect_tx(&bars[warp][stage], kBlock);
-            copy_block(ring + stage * kBlock, c.pages.memory + (int64_t)at * kBlock, kBlock, &bars[warp][stage]);
-        } else if (here) {
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lb_tc::smem_u32(&bars[warp][stage])) : "memory");
+        if (lane < 2) {
+            const int stage = asked % kStages, at = found[warp][(2 * asked + lane) & 63];
+            if (at >= 0) {
+                lb_tc::mbar_expect_tx(&bars[warp][stage], kBlock);
+                copy_block(ring + (2 * stage + lane) * kBlock, c.pages.memory + (int64_t)at * kBlock, kBlock, &bars[warp][stage]);
+            } else {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lb_tc::smem_u32(&bars[warp][stage])) : "memory");
+            }
         }
-        uint32_t bits = __ballot_sync(0xffffffffu, here && at < 0);              // of lanes: tiles asked, asked + 1, ..
-        missing &= ~(((((1u << n) - 1u) << (asked % kStages)) | (((1u << n) - 1u) << (asked % kStages) >> kStages)) & ((1u << kStages) - 1u));
-        bits <<= asked % kStages;
-        missing |= (bits | bits >> kStages) & ((1u << kStages) - 1u);
-        asked += n;
+        ++asked;
+        __syncwarp();
     };
-    fetch(kStages);
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) fetch();
 
     const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.0f);
     const bool biased = !PLAIN && c.distance != nullptr;
@@ -325,28 +333,27 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         }
         float* scores = PLAIN || c.scores == nullptr ? nullptr : c.scores + (((int64_t)seq * kv + kvh) * c.max_rows + row0) * c.score_keys;
 
+        int stage = (done >> 1) % kStages;
+        uint32_t parity = (uint32_t)((done >> 1) / kStages) & 1u;
         while (done < run_end) {
-            // Two tiles at a time; where a run has one left, it stands for both and the second is masked.
-            const int pair = min(2, run_end - done);
-            bool there = lb_tc::mbar_wait(&bars[warp][done % kStages], (uint32_t)(done / kStages) & 1u, nullptr);
-            if (pair == 2) there = there && lb_tc::mbar_wait(&bars[warp][(done + 1) % kStages], (uint32_t)((done + 1) / kStages) & 1u, nullptr);
-            if (!__all_sync(0xffffffffu, there)) {                 // bounded; one answer for the warp
+            // A pair of tiles; where the run begins or ends within one, the other of its two is masked.
+            const int pair = done >> 1;
+            if (!wait(&bars[warp][stage], parity)) {               // bounded; one answer for the warp
                 gave_up = true;
                 break;
             }
-            const int key0 = (tile0 + done - run_begin) * kBlockKeys;
-            const uint8_t* block[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) block[u] = ring + (done + (u < pair ? u : 0)) % kStages * kBlock;
+            const int key0 = (tile0 + 2 * pair - run_begin) * kBlockKeys;
+            const uint8_t* block = ring + 2 * stage * kBlock;
+            const bool half = 2 * pair < run_begin || 2 * pair + 2 > run_end;
             float z[NT][2][2];                                     // [tile][key g, key g + 8] of row t
             uint32_t vs[2][NG];                                    // the values' scales: NG of key g, then NG of key g + 8
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 uint32_t lo[JK], hi[JK], sc[NG];
-                load_words<L::kPiece>(block[u] + lane * L::kPiece, lo);
-                load_words<L::kPiece>(block[u] + 32 * L::kPiece + lane * L::kPiece, hi);
-                load_words<4 * NG>(block[u] + L::kScales + g * 4 * NG, sc);
-                load_words<4 * NG>(block[u] + L::kScales + 32 * NG + g * 4 * NG, vs[u]);
+                load_words<L::kPiece>(block + u * kBlock + lane * L::kPiece, lo);
+                load_words<L::kPiece>(block + u * kBlock + 32 * L::kPiece + lane * L::kPiece, hi);
+                load_words<4 * NG>(block + u * kBlock + L::kScales + g * 4 * NG, sc);
+                load_words<4 * NG>(block + u * kBlock + L::kScales + 32 * NG + g * 4 * NG, vs[u]);
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr) {
                     int a[NT][4];
@@ -379,15 +386,14 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                         }
                     }
             }
-            const uint32_t gone = (missing >> (done % kStages) & 1u) | (missing >> ((done + 1) % kStages) & 1u) << 1;
-            if (key0 + 2 * kBlockKeys - 1 > p_lo || key0 < first_hi || gone != 0 || pair == 1) {
+            if (key0 + 2 * kBlockKeys - 1 > p_lo || key0 < first_hi || half || !all_there) {
                 // Keys that some row does not see: their scores are -inf, and the scales of those past every row (whatever the memory holds) 0.
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int key = key0 + 16 * u + g + 8 * e;
-                        const bool absent = u >= pair || (gone >> u & 1u) != 0;
+                        const bool absent = 2 * pair + u < run_begin || 2 * pair + u >= run_end || found[warp][(2 * pair + u) & 63] < 0;
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             if (absent || key > place[n] || key < lb_first_visible(max(place[n], 0), c.window)) z[n][u][e] = -CUDART_INF_F;
@@ -410,7 +416,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int row = 4 * n + t, key = key0 + 16 * u + g + 8 * e;
-                                if (row < rows_here && u < pair && key < c.score_keys) scores[(int64_t)row * c.score_keys + key] = z[n][u][e];
+                                if (row < rows_here && 2 * pair + u >= run_begin && 2 * pair + u < run_end && key < c.score_keys) scores[(int64_t)row * c.score_keys + key] = z[n][u][e];
                             }
                 }
             }
@@ -474,8 +480,8 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                 // V^T p^T: lane (g, t) has the words of the keys 2 t, 2 t + 1 (x) and of those plus 8 (y).
                 uint32_t x[2 * JV], y[2 * JV];
                 const int at = (t * 8 + L::v_turn(g, t)) * L::kPiece;
-                load_words<L::kPiece>(block[u] + L::kV + at, x);
-                load_words<L::kPiece>(block[u] + L::kV + 32 * L::kPiece + at, y);
+                load_words<L::kPiece>(block + u * kBlock + L::kV + at, x);
+                load_words<L::kPiece>(block + u * kBlock + L::kV + 32 * L::kPiece + at, y);
 #pragma unroll
                 for (int j = 0; j < JV; ++j) {
                     uint32_t a0[4], a1[4], a2[4], a3[4];
@@ -491,9 +497,13 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                     }
                 }
             }
-            __syncwarp();                                   // the stages are overwritten by the copies asked for next
-            done += pair;
-            fetch(pair);
+            __syncwarp();                                   // the pair is overwritten by the copies asked for next
+            done = min(2 * pair + 2, run_end);
+            if ((done & 1) == 0) {                          // (else the next run has the rest of it)
+                fetch();
+                parity ^= stage == kStages - 1;
+                stage = stage == kStages - 1 ? 0 : stage + 1;
+            }
         }
         if (gave_up) break;
 
@@ -519,90 +529,34 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     if (gave_up) {
         // The copies still in flight land before the block may leave (bounded as well); the result is wrong and the status word says so.
         if (lane == 0) atomicCAS(status, 0, (0xC << 12) | 1);
-        for (int i = done; i < asked; ++i) lb_tc::mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u, nullptr);
+        for (int i = done >> 1; i < asked; ++i) lb_tc::mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u, nullptr);
     }
 }
 
-// Joins the states of the rows' runs.  A team of warps (1 to 32) has a row, a lane HD / 32 neighbouring values; the warps take the runs in turn, and their sums meet in their order.
+// Joins the states of the rows' runs.
 template <int HD>
 __global__ void __launch_bounds__(1024)
 attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int rows_shift, int team_shift) {
-    constexpr int V = HD / 32, kState = HD + 4;
+    constexpr int kState = HD + 4;
     __shared__ float joined[32][HD + 2];
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row, team = 1 << team_shift;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp & (team - 1), r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (warp >> team_shift);
+    const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row;
+    const int r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (threadIdx.x >> 5 >> team_shift);
     const Portion part = portion_of(c, seq);
-    const bool there = r < part.count * c.per;
-    float m = kLowest, l = 0.0f, v[V] = {};
-    if (there) {
+    const float* state = nullptr;
+    int runs = 0;
+    if (r < part.count * c.per) {
         const int row_tile = r >> rows_shift, in_row = c.q_start == nullptr ? tiles : ((part.count * c.per - 1) >> rows_shift) + 1;
         const int* starts = c.starts + (int64_t)row_of * (per_row + 1);
         const int start = starts[s], units = kv * in_row, n_seq = min(per_row, c.n_seq - row_of * per_row), share = share_of(starts[n_seq], n_warps);
         const int count = units == 1 ? starts[s + 1] - start : (starts[s + 1] - start) / units;
-        const int from = start + (kvh * in_row + row_tile) * count;
-        const int first = from / share, runs = count > 0 ? (from + count - 1) / share - first + 1 : 0;
-        const float* state = c.partial + (((((int64_t)row_of * (n_warps + (int64_t)per_row * kv * tiles) + first + ((int64_t)s * kv + kvh) * tiles + row_tile) << rows_shift) + r - (row_tile << rows_shift)) *
-                                          kState);
-        const int step = kState << rows_shift;
-        // Thirty-two runs at a time: a lane has a run's reference and sum, and its factor once the largest reference is known.
-        for (int i0 = mine; i0 < runs; i0 += 32 * team) {
-            float2 ml = make_float2(kLowest, 0.0f);
-            if (i0 + lane * team < runs) ml = *reinterpret_cast<const float2*>(state + (int64_t)(i0 + lane * team) * step);
-            const bool some = ml.y != 0.0f;                 // (a NaN is some)
-            float high = some ? ml.x : kLowest;
-#pragma unroll
-            for (int x = 16; x > 0; x /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
-            high = fmaxf(high, m);
-            const float w = some ? ex2(ml.x - high) : 0.0f, keep = ex2(m - high);
-            l = fmaf(l, keep, lb_warp_sum(some ? ml.y * w : 0.0f));
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= keep;
-            m = high;
-            const int n = min(32, (runs - i0 + team - 1) >> team_shift);
-            const float* at = state + (int64_t)i0 * step + 4 + V * lane;
-#pragma unroll 4
-            for (int x = 0; x < n; ++x, at += (int64_t)team * step) {
-                const float f = __shfl_sync(0xffffffffu, w, x);
-                float o[V];
-                if constexpr (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(at);
-                else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(at);
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = f == 0.0f ? v[e] : fmaf(o[e], f, v[e]);
-            }
-        }
+        const int from = start + (kvh * in_row + row_tile) * count, first = from / share;
+        runs = count > 0 ? (from + count - 1) / share - first + 1 : 0;
+        state = c.partial + (((((int64_t)row_of * (n_warps + (int64_t)per_row * kv * tiles) + first + ((int64_t)s * kv + kvh) * tiles + row_tile) << rows_shift) + r - (row_tile << rows_shift)) *
+                             kState);
     }
-    if (team > 1) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) joined[warp][2 + V * lane + e] = v[e];
-        if (lane == 0) {
-            joined[warp][0] = m;
-            joined[warp][1] = l;
-        }
-        __syncthreads();
-        if (mine > 0) return;
-        for (int i = 1; i < team; ++i) {
-            const float mi = joined[warp + i][0], li = joined[warp + i][1], high = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : ex2(mi - high), keep = ex2(m - high);
-            l = fmaf(l, keep, li * w);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = fmaf(v[e], keep, joined[warp + i][2 + V * lane + e] * w);
-            m = high;
-        }
-    }
-    if (!there) return;
-    const int token = part.count == 1 ? 0 : r / c.per, head = kvh * c.per + r - token * c.per;
-    float top = m, factor = 1.0f;
-    if (c.sink != nullptr) {
-        const float sink = c.sink[head] * kLbLog2e;
-        top = fmaxf(m, sink);
-        factor = lb_sink_join_exp2(sink, m, l);
-    }
-    factor = l == 0.0f ? 0.0f : __fdividef(factor, l);
-    __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + head * HD + V * lane;
-#pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = __float2bfloat16_rn(v[e] * factor);
-    if (lane == 0 && c.log_sums != nullptr) c.log_sums[((int64_t)seq * kv + kvh) * c.max_rows + r] = l == 0.0f ? CUDART_INF_F : top + log2f(l);
+    join_row<HD>(c, part, seq, kvh, r, state, kState << rows_shift, runs, team_shift, joined);
 }
 
 template <int HD, int NG, int NT, bool PLAIN>
@@ -610,8 +564,8 @@ int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
     auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN>;
-    const int smem = kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
-    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kStages * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1)));
+    const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
+    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1)));
     LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.blocks, (c.n_seq + p.per_row - 1) / p.per_row), dim3(kWarps * 32), smem, s, c, p.per_row, p.tiles, status));
     // Blocks of four warps or more, but no warps past the rows.
     int join_warps = p.join_team;
@@ -626,15 +580,14 @@ template <int HD, int NG>
 int launch_for(const Call& c, const RowsPlan& p, cudaStream_t s) {
     const bool plain = c.distance == nullptr && c.soft_cap <= 0.0f && c.scores == nullptr;
     if (p.rows == 4) return plain ? launch<HD, NG, 1, true>(c, p, s) : launch<HD, NG, 1, false>(c, p, s);
-    if (p.rows == 8) return plain ? launch<HD, NG, 2, true>(c, p, s) : launch<HD, NG, 2, false>(c, p, s);
-    return plain ? launch<HD, NG, 4, true>(c, p, s) : launch<HD, NG, 4, false>(c, p, s);
+    return plain ? launch<HD, NG, 2, true>(c, p, s) : launch<HD, NG, 2, false>(c, p, s);
 }
 
 }  // namespace
 
 int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
     RowsPlan& p = *plan;
-    p.rows = max_rows > 8 ? 16 : max_rows > 4 ? 8 : 4;
+    p.rows = max_rows > 4 ? 8 : 4;
     p.tiles = (max_rows + p.rows - 1) / p.rows;
     // A launch row numbers its tiles in 32 bits.
     const int64_t units = (int64_t)n_kv_head * p.tiles, most = units * ((max_keys + kBlockKeys - 1) / kBlockKeys);
@@ -642,10 +595,10 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     p.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)std::max(1, n_seq), (int64_t)kMostRequests, ((int64_t)1 << 30) / std::max<int64_t>(1, most)}));
     const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
     p.blocks = (int)std::max<int64_t>(1, (warps + kWarps - 1) / kWarps);
-    // Runs that a row has, about; a warp takes some eight of them.
+    // Runs that a row has, about; a warp takes some four of them.
     const int64_t runs = p.blocks * kWarps / (units * p.per_row) + 2;
     p.join_team = 1;
-    while (p.join_team < 32 && p.join_team * 8 < runs) p.join_team *= 2;
+    while (p.join_team < 32 && p.join_team * 4 < runs) p.join_team *= 2;
     const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
     p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
