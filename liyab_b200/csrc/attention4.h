@@ -3,6 +3,8 @@
 
 #include "cache4.cuh"
 
+#include <atomic>
+
 namespace lb_a4 {
 
 // A call, checked (host) and as the kernels get it.
@@ -39,6 +41,18 @@ __device__ __forceinline__ Portion portion_of(const Call& c, int s) {
     }
     p.place = c.last[s];
     return p;
+}
+
+// Lets a kernel have this much dynamic shared memory: asked once a device (a question costs as much as half a launch).
+template <typename Kernel>
+int allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
+    int device = 0;
+    LB_CHECK_CUDA(cudaGetDevice(&device));
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if ((asked.load(std::memory_order_relaxed) & bit) != 0) return LB_OK;
+    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return LB_OK;
 }
 
 // How the kernel for few rows cuts a call: rows a tile (4 or 8), row tiles a request and key/value head, requests a launch row, blocks of a row, warps that join a row's

@@ -726,17 +726,22 @@ attention4_many_join_kernel(const Call c, int n_splits) {
     join_row<HD>(c, part, seq, kvh, r, state, HD + 4, n_splits, 0, joined);
 }
 
-template <int HD, int NG>
+template <int HD, int NG, bool PLAIN>
 int launch(const Call& c, const TilesPlan& p, cudaStream_t s) {
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
-    const bool plain = c.distance == nullptr && c.soft_cap <= 0.0f;
-    auto kernel = plain ? attention4_many_kernel<HD, NG, true> : attention4_many_kernel<HD, NG, false>;
+    auto kernel = attention4_many_kernel<HD, NG, PLAIN>;
     constexpr int smem = 1024 + (kGroups + 2 * kStages) * (HD / 64) * kSub + (int)sizeof(Control);
-    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> asked{0};
+    if (int rc = allow_shared(kernel, smem, asked)) return rc;
     LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows * p.splits, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, p.splits, status));
     if (p.splits > 1) LB_CHECK_CUDA(lb_launch_overlapped(attention4_many_join_kernel<HD>, dim3((c.max_rows + 3) / 4, c.pages.n_kv_head, c.n_seq), dim3(128), 0, s, c, p.splits));
     return LB_OK;
+}
+
+template <int HD, int NG>
+int launch_for(const Call& c, const TilesPlan& p, cudaStream_t s) {
+    return c.distance == nullptr && c.soft_cap <= 0.0f ? launch<HD, NG, true>(c, p, s) : launch<HD, NG, false>(c, p, s);
 }
 
 }  // namespace
@@ -751,8 +756,8 @@ TilesPlan tiles_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int h
 }
 
 int many_rows(const Call& c, int head_dim, const TilesPlan& p, cudaStream_t s) {
-    if (head_dim == 64) return c.pages.groups == 1 ? launch<64, 1>(c, p, s) : launch<64, 2>(c, p, s);
-    return c.pages.groups == 1 ? launch<128, 1>(c, p, s) : c.pages.groups == 2 ? launch<128, 2>(c, p, s) : launch<128, 4>(c, p, s);
+    if (head_dim == 64) return c.pages.groups == 1 ? launch_for<64, 1>(c, p, s) : launch_for<64, 2>(c, p, s);
+    return c.pages.groups == 1 ? launch_for<128, 1>(c, p, s) : c.pages.groups == 2 ? launch_for<128, 2>(c, p, s) : launch_for<128, 4>(c, p, s);
 }
 
 }  // namespace lb_a4

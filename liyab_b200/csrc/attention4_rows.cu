@@ -565,7 +565,8 @@ int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     if (int rc = lb_tc_status_word(&status)) return rc;
     auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN>;
     const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
-    LB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1)));
+    static std::atomic<uint64_t> asked{0};
+    if (int rc = allow_shared(kernel, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1), asked)) return rc;
     LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.blocks, (c.n_seq + p.per_row - 1) / p.per_row), dim3(kWarps * 32), smem, s, c, p.per_row, p.tiles, status));
     // Blocks of four warps or more, but no warps past the rows.
     int join_warps = p.join_team;

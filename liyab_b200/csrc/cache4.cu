@@ -4,6 +4,7 @@
 // evict4 is two launches.  The first chooses: a block a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  The
 // second copies: a warp a block of sixteen keys of the destination, whose pieces it gathers.  The destination is never a source, so nothing waits for anything.
+#include "attention4.h"
 #include "cache4.cuh"
 #include "linear4.h"
 
@@ -77,30 +78,40 @@ __device__ __forceinline__ __nv_bfloat16 group_scale(uint32_t top) {
     return __float2bfloat16_rn(__fdiv_rn(a, 7.0f));
 }
 
-// Eight values over their scales (the first four over s0), the quotients rounded to 32 bits and then to the nearest even integer, as nibbles n + 8.  VALUES: nibble n is value
-// 4 (n % 4 / 2) + 2 (n % 2) + n / 4, else 2 (n % 4) + n / 4.  The quotient is x r corrected by its rest times r, r the scale's rounded reciprocal (Markstein's division, correctly rounded): six
-// operations a value with the rounding (adding 1.5 2^23) and the place in the word (four numbers -7 .. 7 in base 16).  |x| is at most 7.03 s as long as s is a normal number.
-template <bool VALUES>
-__device__ __forceinline__ uint32_t eight_nibbles(const float* x, float s0, float s1) {
+// A scale and its rounded reciprocal, and whether that is within float32's range.
+struct Divisor {
+    float s, r;
+    __device__ __forceinline__ bool plain() const { return s >= 0x1p-90f; }
+};
+__device__ __forceinline__ Divisor divisor(__nv_bfloat16 scale) {
+    const float s = __bfloat162float(scale);
+    return Divisor{s, __frcp_rn(s)};
+}
+
+// Eight values over their scales (the first four over a), the quotients rounded to 32 bits and then to the nearest even integer, as nibbles n + 8: nibble n is value 2 (n % 4) + n / 4, of keys and of
+// values.  The quotient is x r corrected by its rest times r, r the scale's rounded reciprocal (Markstein's division, correctly rounded): six operations a value with the rounding (adding 1.5 2^23) and the
+// place in the word (four numbers -7 .. 7 in base 16).  |x| is at most 7.03 s as long as s is a normal number.
+__device__ __forceinline__ uint32_t eight_nibbles(const float* x, const Divisor& a, const Divisor& b) {
     constexpr float kMagic = 12582912.0f;
-    auto value_at = [](int n) { return VALUES ? 4 * ((n & 3) >> 1) + 2 * (n & 1) + (n >> 2) : 2 * (n & 3) + (n >> 2); };
-    if (s0 >= 0x1p-90f && s1 >= 0x1p-90f) {
-        const float r0 = __frcp_rn(s0), r1 = __frcp_rn(s1);
+    if (a.plain() && b.plain()) {
         float half[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int n = 7; n >= 0; --n) {
-            const int d = value_at(n);
-            const float s = d < 4 ? s0 : s1, r = d < 4 ? r0 : r1, q = x[d] * r;
+            const int d = 2 * (n & 3) + (n >> 2);
+            const float s = d < 4 ? a.s : b.s, r = d < 4 ? a.r : b.r, q = x[d] * r;
             half[n >> 2] = fmaf(half[n >> 2], 16.0f, fmaf(fmaf(-q, s, x[d]), r, q) + kMagic - kMagic);
         }
         const uint32_t lo = __float_as_uint(half[0] + (kMagic + 34952.0f)), hi = __float_as_uint(half[1] + (kMagic + 34952.0f));         // 8 added to each: 0x8888
         return __byte_perm(lo, hi, 0x5410);
     }
     uint32_t word = 0;                                     // scales of 0, NaN, or with a reciprocal past float32's range
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < 8; ++n) {
-        const int d = value_at(n);
-        const float s = d < 4 ? s0 : s1, q = s > 0.0f ? rintf(__fdiv_rn(x[d], s)) : 0.0f;
+        const int d = 2 * (n & 3) + (n >> 2);
+        float v = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) v = i == d ? x[i] : v;
+        const float s = d < 4 ? a.s : b.s, q = s > 0.0f ? rintf(__fdiv_rn(v, s)) : 0.0f;
         word |= (uint32_t)((int)fminf(fmaxf(q, -8.0f), 7.0f) + 8) << (4 * n);
     }
     return word;
@@ -170,8 +181,8 @@ append4_kernel(const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, in
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         const __nv_bfloat16 sa = group_scale<T>(top[i][0]), sb = group > 32 ? sa : group_scale<T>(top[i][1]);
-        const float fa = __bfloat162float(sa), fb = __bfloat162float(sb);
-        *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, i)) = of == 0 ? eight_nibbles<false>(x[i], fa, fa) : eight_nibbles<true>(x[i], fa, fb);
+        const Divisor a = divisor(sa);
+        *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, i)) = eight_nibbles(x[i], a, group > 32 ? a : divisor(sb));
         const int da = S::dim(of, r, i, 0), db = S::dim(of, r, i, 1);
         if (da % group == 0) scales[da / group] = sa;
         if (of == 1 && group == 32 && db % group == 0) scales[db / group] = sb;
@@ -501,7 +512,8 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
     const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
                       a.n_mass, a.n_dest_mass};
     const int held = a.max_keys < kMostHeld ? a.max_keys : kMostHeld;
-    LB_CHECK_CUDA(cudaFuncSetAttribute(evict4_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostHeld));
+    static std::atomic<uint64_t> asked{0};
+    if (int rc = lb_a4::allow_shared(evict4_choose_kernel, 4 * kMostHeld, asked)) return rc;
     LB_CHECK_CUDA(lb_launch_overlapped(evict4_choose_kernel, dim3(pages.n_kv_head, a.n_seq), dim3(kChoiceThreads), 4 * held, s, c, held));
     const dim3 grid((a.keep + 63) / 64, pages.n_kv_head, a.n_seq);
     LB_CHECK_CUDA(lb_launch_overlapped(a.cache->head_dim == 128 ? evict4_copy_kernel<128> : evict4_copy_kernel<64>, grid, dim3(128), 0, s, pages, a.block_table, a.table_stride,

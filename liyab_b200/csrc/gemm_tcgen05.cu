@@ -436,9 +436,13 @@ int lb_tensor_map_2d_encode(CUtensorMap* out, const void* base, int elem_bytes, 
 }
 
 int lb_tc_status_word(int** out) {
-    static int* addr = nullptr;
-    if (addr == nullptr) LB_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&addr), g_status));
-    *out = addr;
+    constexpr int kDevices = 64;
+    static int* addr[kDevices] = {};               // each device has its own
+    int device = 0;
+    LB_CHECK_CUDA(cudaGetDevice(&device));
+    LB_CHECK_ARG(device >= 0 && device < kDevices, "device %d: up to %d are known", device, kDevices);
+    if (addr[device] == nullptr) LB_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&addr[device]), g_status));
+    *out = addr[device];
     return LB_OK;
 }
 

@@ -1428,7 +1428,7 @@ class Cache4:
     """Pages of keys and values in 4 bits: x[slot, d] = n s[d / group], n in -8 .. 7, s bfloat16, a slot being page * page_size + place.  Heads of 64 or 128 values, groups of 32, 64 or
     128, pages of a power of two keys, 16 or more.  The memory belongs to this object; what no append4 or evict4 has written is undefined, and no attention reads it."""
 
-    __slots__ = ("n_pages", "n_kv_head", "head_dim", "page_size", "group", "device", "index", "memory", "args", "ref")
+    __slots__ = ("n_pages", "n_kv_head", "head_dim", "page_size", "group", "device", "index", "memory", "args", "ref", "scratch")
 
     def __init__(self, n_pages: int, n_kv_head: int, head_dim: int, page_size: int = 16, group: int = 64, device="cuda"):
         size = ctypes.c_int64(0)
@@ -1440,6 +1440,7 @@ class Cache4:
         self.device, self.index = self.memory.device, self.memory.get_device()
         self.args = Cache4Args(self.memory.data_ptr(), n_pages, n_kv_head, head_dim, page_size, group, self.index + 1)
         self.ref = ctypes.addressof(self.args)
+        self.scratch = {}                          # bytes of scratch memory by the sizes of an attention call: the library is asked once
 
     @property
     def nbytes(self) -> int:
@@ -1475,10 +1476,16 @@ def cache4_values(cache: Cache4, slots: torch.Tensor, n: int, k: torch.Tensor, v
     return k, v
 
 
-def _ints4(what: str, name: str, t: torch.Tensor, index: int, shape: tuple) -> int:
-    """An int32 tensor of at least this shape, dense within a row."""
-    if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != len(shape) or any(a < b for a, b in zip(t.shape, shape)) or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        raise invalid_argument(f"{what}: {name} has to be int32 of at least {shape}, dense within a row, on the cache's device; it is {t.dtype} {tuple(t.shape)} on {t.device}")
+def _ints4(what: str, name: str, t: torch.Tensor, index: int, least: int, columns: int = 0) -> int:
+    """An int32 vector of at least `least` numbers, or a matrix of as many rows and at least `columns` columns, dense within a row."""
+    shape = t.shape
+    if columns == 0:
+        good = len(shape) == 1 and shape[0] >= least and (t.stride(0) == 1 or shape[0] < 2)
+    else:
+        good = len(shape) == 2 and shape[0] >= least and shape[1] >= columns and (t.stride(1) == 1 or shape[1] == 1)
+    if not good or t.dtype is not torch.int32 or t.get_device() != index:
+        raise invalid_argument(f"{what}: {name} has to be int32 of at least {least}{f' x {columns}' if columns else ''}, dense within a row, on the cache's device; it is {t.dtype} "
+                               f"{tuple(shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -1492,16 +1499,23 @@ def _weights_of4(what: str, name: str, t: torch.Tensor, cache: Cache4, keys: int
 
 def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[torch.Tensor], last: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, n_seq: int,
                 max_q_len: int, n_head: int, scale: float, window: int, mass: Optional[torch.Tensor], total: Optional[torch.Tensor], mass_rows: Optional[torch.Tensor],
-                distance: Optional[torch.Tensor], sink: Optional[torch.Tensor], soft_cap: float, max_keys: int, plan=None):
+                distance: Optional[torch.Tensor], sink: Optional[torch.Tensor], soft_cap: float, max_keys: int) -> torch.Tensor:
     index, width = cache.index, n_head * cache.head_dim
+    q_shape, out_shape = q.shape, out.shape
     if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or q.get_device() != index or out.get_device() != index:
         raise invalid_argument(f"{what}: q and out are bfloat16 on the cache's device; they are {q.dtype} on {q.device} and {out.dtype} on {out.device}")
-    if q.dim() != 2 or out.dim() != 2 or q.shape[1] != width or out.shape[1] != width or out.shape[0] < q.shape[0] or q.stride(1) != 1 or out.stride(1) != 1:
-        raise invalid_argument(f"{what}: q and out are rows of {width} values, dense within a row; they are {tuple(q.shape)} and {tuple(out.shape)}")
-    last_at = _ints4(what, "positions" if q_start is None else "n_past", last, index, (n_seq,))
-    table_at = _ints4(what, "block_table", block_table, index, (n_seq, 1))
-    start_at = 0 if q_start is None else _ints4(what, "q_start", q_start, index, (n_seq + 1,))
-    keys = min(max_keys, block_table.shape[1] * cache.page_size) if max_keys > 0 else block_table.shape[1] * cache.page_size
+    if len(q_shape) != 2 or len(out_shape) != 2 or q_shape[1] != width or out_shape[1] != width or out_shape[0] < q_shape[0]:
+        raise invalid_argument(f"{what}: q and out are rows of {width} values; they are {tuple(q_shape)} and {tuple(out_shape)}")
+    (ldq, dense_q), (ldo, dense_out) = q.stride(), out.stride()
+    if dense_q != 1 or dense_out != 1:
+        raise invalid_argument(f"{what}: q and out have to be dense within a row")
+    last_at = _ints4(what, "positions" if q_start is None else "n_past", last, index, n_seq)
+    table_at = _ints4(what, "block_table", block_table, index, n_seq, 1)
+    start_at = 0 if q_start is None else _ints4(what, "q_start", q_start, index, n_seq + 1)
+    table_rows, table_columns = block_table.shape
+    keys = table_columns * cache.page_size
+    if 0 < max_keys < keys:
+        keys = max_keys
     mass_at = total_at = rows_at = n_mass = 0
     strides = (0, 0, 0, 0)
     if mass is not None:
@@ -1510,7 +1524,7 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
         n_mass = min(mass.shape[0], total.shape[0])
         strides = (mass.stride(0), mass.stride(1), total.stride(0), total.stride(1))
         if mass_rows is not None:
-            rows_at = _ints4(what, "mass_rows", mass_rows, index, (n_seq,))
+            rows_at = _ints4(what, "mass_rows", mass_rows, index, n_seq)
         elif n_mass < n_seq:
             raise invalid_argument(f"{what}: {n_seq} requests, weights of {n_mass}")
     elif total is not None or mass_rows is not None:
@@ -1520,17 +1534,19 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
             raise invalid_argument(f"{what}: {name} has to be {n} float32 numbers on the cache's device")
     parts = (cache.ref, q.data_ptr(), start_at, last_at, table_at, out.data_ptr(), mass_at, total_at, rows_at, 0 if distance is None else distance.data_ptr(),
              0 if sink is None else sink.data_ptr())
-    rest = (stream_of(index), q.stride(0), out.stride(0), *strides, block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], n_seq, q.shape[0], n_head, max_q_len, keys, n_mass,
-            window, scale, soft_cap)
-    packed = _attention4_args(*parts, 0, *rest)
+    rest = (stream_of(index), ldq, ldo, *strides, block_table.stride(0) if table_rows > 1 else table_columns, n_seq, q_shape[0], n_head, max_q_len, keys, n_mass, window, scale, soft_cap)
     l = lib()
-    if plan is not None:
-        return check(l.lb_attention4_plan(packed, plan), what)
-    size = l.lb_attention4_scratch(packed)
-    if size:
-        scratch = torch.empty(size, dtype=torch.uint8, device=cache.device)
-        packed = _attention4_args(*parts, scratch.data_ptr(), *rest)
-    check(l.lb_attention4(packed), what)
+    sizes = (n_seq, max_q_len, n_head, keys, mass is None, rest[7])
+    size = cache.scratch.get(sizes)
+    known = size is not None
+    if not known:
+        size = l.lb_attention4_scratch(_attention4_args(*parts, 0, *rest))
+    scratch = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
+    check(l.lb_attention4(_attention4_args(*parts, 0 if scratch is None else scratch.data_ptr(), *rest)), what)
+    if not known:
+        if len(cache.scratch) >= 4096:
+            cache.scratch.clear()
+        cache.scratch[sizes] = size
     return out
 
 
@@ -1561,18 +1577,18 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
     the lowest places).  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
     they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (memory of its own, not mass)."""
     index, page = cache.index, cache.page_size
-    table_at, dest_at = _ints4("evict4", "block_table", block_table, index, (n_seq, 1)), _ints4("evict4", "dest_table", dest_table, index, (n_seq, -(-keep // page)))
+    table_at, dest_at = _ints4("evict4", "block_table", block_table, index, n_seq, 1), _ints4("evict4", "dest_table", dest_table, index, n_seq, max(1, -(-keep // page)))
     keys = min(block_table.shape[1] * page, mass.shape[2] if mass.dim() == 3 else 0)
-    mass_at, n_keys_at = _weights_of4("evict4", "mass", mass, cache, 1), _ints4("evict4", "n_keys", n_keys, index, (n_seq,))
-    kept_at = _ints4("evict4", "kept", kept, index, (n_seq, cache.n_kv_head, keep))
-    if tuple(kept.shape[1:]) != (cache.n_kv_head, keep) or not kept.is_contiguous():
-        raise invalid_argument(f"evict4: kept has to be contiguous [requests, {cache.n_kv_head}, {keep}]; it is {tuple(kept.shape)}")
+    mass_at, n_keys_at = _weights_of4("evict4", "mass", mass, cache, 1), _ints4("evict4", "n_keys", n_keys, index, n_seq)
+    kept_at, kept_shape = kept.data_ptr(), kept.shape
+    if kept.dtype is not torch.int32 or kept.get_device() != index or len(kept_shape) != 3 or kept_shape[0] < n_seq or kept_shape[1:] != (cache.n_kv_head, keep) or not kept.is_contiguous():
+        raise invalid_argument(f"evict4: kept has to be contiguous int32 [requests, {cache.n_kv_head}, {keep}] on the cache's device; it is {kept.dtype} {tuple(kept_shape)} on {kept.device}")
     rows_at = dest_mass_at = n_dest = 0
     strides = (0, 0)
     if dest_mass is not None:
         dest_mass_at, n_dest, strides = _weights_of4("evict4", "dest_mass", dest_mass, cache, keep), dest_mass.shape[0], (dest_mass.stride(0), dest_mass.stride(1))
     if mass_rows is not None:
-        rows_at = _ints4("evict4", "mass_rows", mass_rows, index, (n_seq,))
+        rows_at = _ints4("evict4", "mass_rows", mass_rows, index, n_seq)
     elif mass.shape[0] < n_seq or (dest_mass is not None and n_dest < n_seq):
         raise invalid_argument(f"evict4: {n_seq} requests, weights of {mass.shape[0]}{'' if dest_mass is None else f' and {n_dest}'}")
     check(lib().lb_evict4(_evict4_args(cache.ref, mass_at, rows_at, table_at, n_keys_at, dest_at, kept_at, dest_mass_at, stream_of(index), mass.stride(0), mass.stride(1), *strides,
