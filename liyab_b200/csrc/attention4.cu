@@ -63,7 +63,7 @@ bool takes_many(const lb_attention4_args& a, int max_rows, int keys, const RowsP
     const bool wide = a.cache->head_dim == 128;
     const double units = (double)a.n_seq * a.cache->n_kv_head;
     const double tile = few.rows == 4 ? (wide ? 0.00043 : 0.00027) : wide ? 0.00068 : 0.0004;
-    const double few_us = 10.0 + units * few.tiles * ((keys + 15) / 16) * tile;
+    const double few_us = (few.whole ? 7.0 : 10.0) + units * few.tiles * ((keys + 15) / 16) * tile;
     const double blocks = units * ((max_rows + 255) / 256) * many.splits, each = ((keys + 127) / 128 + many.splits - 1) / many.splits;
     const double many_us = (many.splits > 1 ? 12.0 : 9.0) + std::ceil(blocks / n_sm) * each * (max_rows <= 128 ? (wide ? 2.5 : 1.9) : wide ? 2.9 : 2.6);
     return many_us < few_us;
@@ -144,8 +144,8 @@ extern "C" int lb_attention4_plan(const lb_attention4_args* args, int* plan) {
     if (int rc = check(args, &c, &p)) return rc;
     plan[0] = p.many ? 1 : 0;
     plan[1] = p.many ? 256 : p.rows.rows;
-    plan[2] = p.many ? p.tiles.splits : p.rows.blocks;
-    plan[3] = p.many ? 1 : p.rows.per_row;
+    plan[2] = p.many ? p.tiles.splits : p.rows.whole ? 1 : p.rows.blocks;
+    plan[3] = p.many || p.rows.whole ? 1 : p.rows.per_row;
     return LB_OK;
 }
 

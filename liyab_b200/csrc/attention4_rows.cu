@@ -88,7 +88,8 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
 // bfloat16 number i of a run of words.
 __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
 
-constexpr int kWarps = 4;                      // a block's; they share nothing but the list of requests
+constexpr int kWarps = 4, kWholeWarps = 8;     // a block's; four share nothing but the list of requests, eight have a row tile's keys between them
+constexpr int kWholeTiles = 64;                // tiles of keys that eight warps take between them where blocks have row tiles of their own
 constexpr int kMostRequests = 1024;            // of a launch row (grid.y)
 constexpr int kLeastTiles = 4;                 // of a warp
 
@@ -122,21 +123,23 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, lb_tc::mbar_wait(bar, parity, nullptr));
 }
 
-// NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.
-template <int HD, int NG, int NT, bool PLAIN>
-__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(HD, NT))
+// NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.  WHOLE: a block has one request's (blockIdx.y) row tile
+// and key/value head (blockIdx.x), whose keys its warps share out and whose result it makes itself; else the states of the warps' runs meet in another launch.
+template <int HD, int NG, int NT, bool PLAIN, bool WHOLE>
+__global__ void __launch_bounds__((WHOLE ? kWholeWarps : lb_a4::kWarps) * 32, WHOLE ? 1 : blocks_per_sm(HD, NT))
 attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
     constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, two places, the values
     constexpr int JK = HD / 32, JV = HD / 64;             // words of a lane: of a key, of a value row
-    constexpr int kBlock = block_bytes(HD, NG);
+    constexpr int kBlock = block_bytes(HD, NG), kWarps = WHOLE ? kWholeWarps : lb_a4::kWarps;
     // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
     constexpr int VT = NT == 1 ? 1 : NT / 2, VG = NT == 1 ? (NG + 1) / 2 : NG;
-    // The warps' rings, then the list of requests: where their tiles start in the row's order, and in their keys.
+    // The warps' rings, (WHOLE) their states, then the list of requests: where their tiles start in the row's order, and in their keys.
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ int found[kWarps][64];                      // the cache's blocks of the tiles to come; -1: on no page
-    int* starts = reinterpret_cast<int*>(smem + kWarps * kStages * 2 * kBlock);
+    float* states = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * kBlock);
+    int* starts = reinterpret_cast<int*>(states + (WHOLE ? kWarps * kRows * kState : 0));
     int* firsts = starts + per_row + 1;
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -170,12 +173,24 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         if (lane == 0) starts[n_seq] = sum;
     }
     __syncthreads();
+    auto row_tiles_of = [&](const Portion& p) { return c.q_start == nullptr ? tiles : (p.count * c.per + kRows - 1) / kRows; };
     const int total = starts[n_seq], n_warps = gridDim.x * kWarps, me = blockIdx.x * kWarps + warp;
-    const int share = share_of(total, n_warps);
-    if (blockIdx.x == 0)                                    // for the launch that joins the states
-        for (int s = threadIdx.x; s <= n_seq; s += kWarps * 32) c.starts[(int64_t)blockIdx.y * (per_row + 1) + s] = starts[s];
-    const int begin = min((int64_t)me * share, (int64_t)total), end = min((int64_t)(me + 1) * share, (int64_t)total);
-    if (begin >= end) return;
+    int begin, end;
+    if constexpr (WHOLE) {
+        const Portion part = portion_of(c, seq0);
+        const int units = part.count > 0 ? kv * row_tiles_of(part) : 0;
+        if ((int)blockIdx.x >= units) return;
+        const int count = total / units, share = (count + kWarps - 1) / kWarps;
+        begin = blockIdx.x * count + min(warp * share, count);
+        end = blockIdx.x * count + min((warp + 1) * share, count);
+    } else {
+        const int share = share_of(total, n_warps);
+        if (blockIdx.x == 0)                                // for the launch that joins the states
+            for (int s = threadIdx.x; s <= n_seq; s += kWarps * 32) c.starts[(int64_t)blockIdx.y * (per_row + 1) + s] = starts[s];
+        begin = min((int64_t)me * share, (int64_t)total);
+        end = min((int64_t)(me + 1) * share, (int64_t)total);
+        if (begin >= end) return;
+    }
     // The request that tile x of the row belongs to.
     auto request_of = [&](int x) {
         int lo = 0, hi = n_seq - 1;
@@ -186,8 +201,6 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         }
         return lo;
     };
-    auto row_tiles_of = [&](const Portion& p) { return c.q_start == nullptr ? tiles : (p.count * c.per + kRows - 1) / kRows; };
-
     uint8_t* ring = smem + warp * kStages * 2 * kBlock;
     const int n_tiles = end - begin;
     // Tiles come in pairs, counted from the warp's first: a barrier a pair, on which two lanes arrive with a tile each.
@@ -507,8 +520,8 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         }
         if (gave_up) break;
 
-        // The run's state, for the launch that joins them: m + f, the sum and the values of its rows.
-        float* state = c.partial + ((int64_t)blockIdx.y * (n_warps + (int64_t)per_row * kv * tiles) + me + ((int64_t)s * kv + kvh) * tiles + row_tile) * (kRows * kState);
+        // The run's state: m + f, the sum and the values of its rows.
+        float* state = WHOLE ? states + warp * (kRows * kState) : c.partial + ((int64_t)blockIdx.y * (n_warps + (int64_t)per_row * kv * tiles) + me + ((int64_t)s * kv + kvh) * tiles + row_tile) * (kRows * kState);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -530,6 +543,16 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         // The copies still in flight land before the block may leave (bounded as well); the result is wrong and the status word says so.
         if (lane == 0) atomicCAS(status, 0, (0xC << 12) | 1);
         for (int i = done >> 1; i < asked; ++i) lb_tc::mbar_wait(&bars[warp][i % kStages], (uint32_t)(i / kStages) & 1u, nullptr);
+    }
+    if constexpr (WHOLE) {
+        // Every warp's state, also of those without keys (and of one that gave up), then a warp a row.
+        static_assert(kRows <= kWarps, "a warp a row");
+        if (n_tiles <= 0 || gave_up)
+            for (int i = lane; i < kRows * kState; i += 32) states[warp * (kRows * kState) + i] = 0.0f;
+        __syncthreads();
+        const Portion part = portion_of(c, seq0);
+        const int in_row = row_tiles_of(part), kvh = blockIdx.x / in_row, r = ((int)blockIdx.x - kvh * in_row) * kRows + warp;
+        if (warp < kRows && r < part.count * c.per) join_row<HD>(c, part, seq0, kvh, r, states + warp * kState, kRows * kState, kWarps, 0, nullptr);
     }
 }
 
@@ -563,7 +586,15 @@ template <int HD, int NG, int NT, bool PLAIN>
 int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     int* status = nullptr;
     if (int rc = lb_tc_status_word(&status)) return rc;
-    auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN>;
+    if (p.whole) {
+        auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, true>;
+        constexpr int smem = kWholeWarps * (kStages * 2 * block_bytes(HD, NG) + 4 * NT * (HD + 4) * 4) + 16;
+        static std::atomic<uint64_t> asked{0};
+        if (int rc = allow_shared(kernel, smem, asked)) return rc;
+        LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(c.pages.n_kv_head * p.tiles, c.n_seq), dim3(kWholeWarps * 32), smem, s, c, 1, p.tiles, status));
+        return LB_OK;
+    }
+    auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, false>;
     const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
     static std::atomic<uint64_t> asked{0};
     if (int rc = allow_shared(kernel, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1), asked)) return rc;
@@ -590,6 +621,8 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     RowsPlan& p = *plan;
     p.rows = max_rows > 4 ? 8 : 4;
     p.tiles = (max_rows + p.rows - 1) / p.rows;
+    // Where an SM has a row tile at most, and it few keys, a block makes its result (1 request, 25 heads of 64 on 512 keys: DECODE1), the other way the states' launch is as long as the rest.
+    p.whole = (int64_t)n_seq * n_kv_head * p.tiles <= n_sm && (max_keys + kBlockKeys - 1) / kBlockKeys <= kWholeTiles;
     // A launch row numbers its tiles in 32 bits.
     const int64_t units = (int64_t)n_kv_head * p.tiles, most = units * ((max_keys + kBlockKeys - 1) / kBlockKeys);
     LB_CHECK_ARG(most <= 1 << 30, "attention4: a request of %d rows and %d keys is more than one launch takes", max_rows, max_keys);
@@ -603,6 +636,7 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
     p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
+    if (p.whole) p.states = p.starts = 0;
     return LB_OK;
 }
 

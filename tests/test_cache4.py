@@ -118,9 +118,10 @@ def test_how_attention_is_cut():
 
 def test_scratch():
     """States of all runs (a run more than warps and units together has), where requests' tiles start, and the keys' weights."""
-    (_, rows, blocks, per), got = _plan(8, 32, 4, 1024, dim=128)
+    (_, rows, blocks, per), got = _plan(8, 32, 4, 4096, dim=128)
     states, starts = (4 * blocks + 4 * 8) * rows * 132 * 4, 5 * 4
     assert got == states + -(-starts // 16) * 16
+    assert _plan(8, 32, 4, 1024, dim=128) == ((0, 4, 1, 1), 0)          # few keys: a block for each request and key/value head, whose warps' states meet in it
     c, ref = _cache(kv=8, dim=128)
     scratch = ops.lib().lb_attention4_scratch
     assert scratch(_call(ref, n_head=32, mass=AT, total=AT)) - scratch(_call(ref, n_head=32)) == 4 * 32 * 1024 * 4 + 4 * 32 * 4
