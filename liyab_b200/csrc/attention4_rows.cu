@@ -27,7 +27,7 @@ namespace {
 
 using namespace lb_c4;
 
-constexpr int kStages = 3;                     // pairs of tiles in a warp's ring
+constexpr int kStages = 2;                     // pairs of tiles in a warp's ring
 constexpr float kSlack = 8.0f;                 // how far a score may pass its row's reference (base 2)
 constexpr float kLeastScale = -80.0f;          // the exponent of the largest value scale, before any
 constexpr float kRoom = 6.0f;                  // p s reaches 2^(kRoom + kSlack) = 2^14 of float16's 2^16; what lies 2^-30 below the largest scale loses bits
@@ -90,7 +90,7 @@ __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uin
 
 constexpr int kWarps = 4, kWholeWarps = 8;     // a block's; four share nothing but the list of requests, eight have a row tile's keys between them
 constexpr int kWholeTiles = 64;                // tiles of keys that eight warps take between them where blocks have row tiles of their own
-constexpr int kMostRequests = 1024;            // of a launch row (grid.y)
+constexpr int kMostRequests = 256;             // of a launch row (grid.y)
 constexpr int kLeastTiles = 4;                 // of a warp
 
 // Blocks an SM.
@@ -103,6 +103,12 @@ __device__ __forceinline__ void tiles_of(const Call& c, const Portion& p, int* f
     *first = lo < 0 ? 0 : lb_first_visible(lo, c.window) / kBlockKeys;
     *count = hi < 0 ? 0 : hi / kBlockKeys + 1 - *first;
 }
+
+// A request of a launch row: its tokens, its first tile of keys and how many, its row tiles for each key/value head.
+struct Request {
+    Portion part;
+    int first, count, in_row;
+};
 
 // How many tiles a warp takes, of `total` in its launch row.
 __host__ __device__ __forceinline__ int share_of(int total, int n_warps) {
@@ -126,7 +132,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
 // NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.  WHOLE: a block has one request's (blockIdx.y) row tile
 // and key/value head (blockIdx.x), whose keys its warps share out and whose result it makes itself; else the states of the warps' runs meet in another launch.
 template <int HD, int NG, int NT, bool PLAIN, bool WHOLE>
-__global__ void __launch_bounds__((WHOLE ? kWholeWarps : lb_a4::kWarps) * 32, WHOLE ? 1 : blocks_per_sm(HD, NT))
+__global__ void __launch_bounds__((WHOLE ? kWholeWarps : lb_a4::kWarps) * 32, WHOLE ? (NT == 1 ? 2 : 1) : blocks_per_sm(HD, NT))
 attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
     constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, two places, the values
@@ -134,13 +140,13 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     constexpr int kBlock = block_bytes(HD, NG), kWarps = WHOLE ? kWholeWarps : lb_a4::kWarps;
     // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
     constexpr int VT = NT == 1 ? 1 : NT / 2, VG = NT == 1 ? (NG + 1) / 2 : NG;
-    // The warps' rings, (WHOLE) their states, then the list of requests: where their tiles start in the row's order, and in their keys.
+    // The warps' rings, (WHOLE) their states, then the list of requests, behind where their tiles start in the row's order.
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ int found[kWarps][64];                      // the cache's blocks of the tiles to come; -1: on no page
     float* states = reinterpret_cast<float*>(smem + kWarps * kStages * 2 * kBlock);
     int* starts = reinterpret_cast<int*>(states + (WHOLE ? kWarps * kRows * kState : 0));
-    int* firsts = starts + per_row + 1;
+    Request* requests = reinterpret_cast<Request*>(starts + per_row + 1);
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int seq0 = blockIdx.y * per_row, n_seq = min(per_row, c.n_seq - seq0), kv = c.pages.n_kv_head;
@@ -152,11 +158,14 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         int sum = 0;
         for (int s0 = 0; s0 < n_seq; s0 += 32) {
             const int s = s0 + lane;
-            int first = 0, mine = 0;
+            int mine = 0;
             if (s < n_seq) {
-                const Portion p = portion_of(c, seq0 + s);
-                tiles_of(c, p, &first, &mine);
-                mine *= kv * (c.q_start == nullptr ? tiles : p.count > 0 ? (p.count * c.per + kRows - 1) / kRows : 0);
+                Request r;
+                r.part = portion_of(c, seq0 + s);
+                tiles_of(c, r.part, &r.first, &r.count);
+                r.in_row = c.q_start == nullptr ? tiles : r.part.count > 0 ? (r.part.count * c.per + kRows - 1) / kRows : 0;
+                requests[s] = r;
+                mine = kv * r.in_row * r.count;
             }
             int before = mine;
 #pragma unroll
@@ -164,23 +173,17 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                 const int v = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += v;
             }
-            if (s < n_seq) {
-                starts[s] = sum + before - mine;
-                firsts[s] = first;
-            }
+            if (s < n_seq) starts[s] = sum + before - mine;
             sum += __shfl_sync(0xffffffffu, before, 31);
         }
         if (lane == 0) starts[n_seq] = sum;
     }
     __syncthreads();
-    auto row_tiles_of = [&](const Portion& p) { return c.q_start == nullptr ? tiles : (p.count * c.per + kRows - 1) / kRows; };
     const int total = starts[n_seq], n_warps = gridDim.x * kWarps, me = blockIdx.x * kWarps + warp;
     int begin, end;
     if constexpr (WHOLE) {
-        const Portion part = portion_of(c, seq0);
-        const int units = part.count > 0 ? kv * row_tiles_of(part) : 0;
-        if ((int)blockIdx.x >= units) return;
-        const int count = total / units, share = (count + kWarps - 1) / kWarps;
+        if ((int)blockIdx.x >= kv * requests[0].in_row) return;
+        const int count = requests[0].count, share = (count + kWarps - 1) / kWarps;
         begin = blockIdx.x * count + min(warp * share, count);
         end = blockIdx.x * count + min((warp + 1) * share, count);
     } else {
@@ -213,8 +216,8 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             const int x = begin + listed + lane;
             int at = -1;
             if (x < end) {
-                const int s = request_of(x), in_row = row_tiles_of(portion_of(c, seq0 + s)), count = (starts[s + 1] - starts[s]) / (kv * in_row);
-                const int unit = (x - starts[s]) / count, tile = firsts[s] + x - starts[s] - unit * count, kvh = unit / in_row;
+                const int s = request_of(x), count = requests[s].count, in_row = requests[s].in_row;
+                const int unit = (x - starts[s]) / count, tile = requests[s].first + x - starts[s] - unit * count, kvh = in_row == 1 ? unit : unit / in_row;
                 const int page = c.table[(int64_t)(seq0 + s) * c.table_stride + (tile * kBlockKeys >> c.pages.page_shift)];
                 if ((unsigned)page < (unsigned)c.pages.n_pages) at = ((page * kv + kvh) << (c.pages.page_shift - 4)) + (tile & ((1 << (c.pages.page_shift - 4)) - 1));
             }
@@ -247,10 +250,10 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     // A run: the tiles of one request, key/value head and row tile.
     while (done < n_tiles && !gave_up) {
         const int s = request_of(begin + done), seq = seq0 + s;
-        const Portion part = portion_of(c, seq);
-        const int in_row = row_tiles_of(part), count = (starts[s + 1] - starts[s]) / (kv * in_row);
-        const int unit = (begin + done - starts[s]) / count, kvh = unit / in_row, row_tile = unit - kvh * in_row;
-        const int tile0 = firsts[s] + begin + done - starts[s] - unit * count;
+        const Portion part = requests[s].part;
+        const int in_row = requests[s].in_row, count = requests[s].count;
+        const int unit = (begin + done - starts[s]) / count, kvh = in_row == 1 ? unit : unit / in_row, row_tile = unit - kvh * in_row;
+        const int tile0 = requests[s].first + begin + done - starts[s] - unit * count;
         const int run_end = min(n_tiles, starts[s] + (unit + 1) * count - begin), run_begin = done;
         const int n_rows = part.count * c.per, row0 = row_tile * kRows, rows_here = min(kRows, n_rows - row0);
         auto token_of = [&](int row) { return part.count == 1 ? 0 : row / c.per; };
@@ -550,8 +553,8 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         if (n_tiles <= 0 || gave_up)
             for (int i = lane; i < kRows * kState; i += 32) states[warp * (kRows * kState) + i] = 0.0f;
         __syncthreads();
-        const Portion part = portion_of(c, seq0);
-        const int in_row = row_tiles_of(part), kvh = blockIdx.x / in_row, r = ((int)blockIdx.x - kvh * in_row) * kRows + warp;
+        const Portion part = requests[0].part;
+        const int in_row = requests[0].in_row, kvh = blockIdx.x / in_row, r = ((int)blockIdx.x - kvh * in_row) * kRows + warp;
         if (warp < kRows && r < part.count * c.per) join_row<HD>(c, part, seq0, kvh, r, states + warp * kState, kRows * kState, kWarps, 0, nullptr);
     }
 }
@@ -588,16 +591,16 @@ int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     if (int rc = lb_tc_status_word(&status)) return rc;
     if (p.whole) {
         auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, true>;
-        constexpr int smem = kWholeWarps * (kStages * 2 * block_bytes(HD, NG) + 4 * NT * (HD + 4) * 4) + 16;
+        constexpr int smem = kWholeWarps * (kStages * 2 * block_bytes(HD, NG) + 4 * NT * (HD + 4) * 4) + 8 + (int)sizeof(Request);
         static std::atomic<uint64_t> asked{0};
         if (int rc = allow_shared(kernel, smem, asked)) return rc;
         LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(c.pages.n_kv_head * p.tiles, c.n_seq), dim3(kWholeWarps * 32), smem, s, c, 1, p.tiles, status));
         return LB_OK;
     }
     auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, false>;
-    const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * p.per_row + 1);
+    const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (p.per_row + 1) + (int)sizeof(Request) * p.per_row;
     static std::atomic<uint64_t> asked{0};
-    if (int rc = allow_shared(kernel, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (2 * kMostRequests + 1), asked)) return rc;
+    if (int rc = allow_shared(kernel, kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (kMostRequests + 1) + (int)sizeof(Request) * kMostRequests, asked)) return rc;
     LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(p.blocks, (c.n_seq + p.per_row - 1) / p.per_row), dim3(kWarps * 32), smem, s, c, p.per_row, p.tiles, status));
     // Blocks of four warps or more, but no warps past the rows.
     int join_warps = p.join_team;

@@ -109,7 +109,7 @@ def test_how_attention_is_cut():
     """Rows a tile, blocks, and requests that share them, by the requests, heads, tokens and keys alone."""
     assert _plan(25, 25, 64, 1024)[0] == (0, 4, 5 * 148, 64) and _plan(8, 128, 64, 1024, dim=128)[0] == (0, 8, 3 * 148, 64)
     assert _plan(8, 32, 1, 16)[0][2] == 1                      # eight tiles of keys, two warps' work
-    assert _plan(1, 1, 65535, 1024)[0][3] == 1024              # requests in rows of the launch
+    assert _plan(1, 1, 65535, 1024)[0][3] == 256              # requests in rows of the launch
     assert _plan(32, 32, 100, 1 << 27)[0][3] == 4              # a row numbers its tiles in 30 bits
     c, ref = _cache()
     assert ops.lib().lb_attention4_plan(_call(ref), None) != 0
