@@ -60,6 +60,7 @@ int allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
 struct RowsPlan {
     int rows, tiles, per_row, blocks, join_team;
     bool whole;                     // a block for each request's row tiles and key/value heads
+    double us;                      // about how long it takes
     int64_t states, starts;
 };
 int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);

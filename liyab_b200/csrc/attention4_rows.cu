@@ -21,6 +21,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cmath>
 
 namespace lb_a4 {
 namespace {
@@ -88,13 +89,13 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
 // bfloat16 number i of a run of words.
 __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
 
-constexpr int kWarps = 4, kWholeWarps = 8;     // a block's; four share nothing but the list of requests, eight have a row tile's keys between them
-constexpr int kWholeTiles = 64;                // tiles of keys that eight warps take between them where blocks have row tiles of their own
+// A block's warps.
+__host__ __device__ constexpr int warps_of(int nt, bool whole) { return whole || nt == 1 ? 8 : 4; }
 constexpr int kMostRequests = 256;             // of a launch row (grid.y)
 constexpr int kLeastTiles = 4;                 // of a warp
 
-// Blocks an SM.
-__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return nt == 1 ? (hd == 64 ? 5 : 4) : hd == 64 ? 4 : 3; }
+// Blocks an SM.  (Heads of 64 have registers for three with one tile of rows: 64 x 1024 keys 34.8 us against 32.0.)
+__host__ __device__ constexpr int blocks_per_sm(int hd, int nt, bool whole) { return nt == 1 ? 2 : whole ? 1 : hd == 64 ? 4 : 3; }
 
 // The blocks of keys of a request that any of its rows sees: the first and how many.
 __device__ __forceinline__ void tiles_of(const Call& c, const Portion& p, int* first, int* count) {
@@ -132,12 +133,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
 // NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.  WHOLE: a block has one request's (blockIdx.y) row tile
 // and key/value head (blockIdx.x), whose keys its warps share out and whose result it makes itself; else the states of the warps' runs meet in another launch.
 template <int HD, int NG, int NT, bool PLAIN, bool WHOLE>
-__global__ void __launch_bounds__((WHOLE ? kWholeWarps : lb_a4::kWarps) * 32, WHOLE ? (NT == 1 ? 2 : 1) : blocks_per_sm(HD, NT))
+__global__ void __launch_bounds__(warps_of(NT, WHOLE) * 32, blocks_per_sm(HD, NT, WHOLE))
 attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
     constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, two places, the values
     constexpr int JK = HD / 32, JV = HD / 64;             // words of a lane: of a key, of a value row
-    constexpr int kBlock = block_bytes(HD, NG), kWarps = WHOLE ? kWholeWarps : lb_a4::kWarps;
+    constexpr int kBlock = block_bytes(HD, NG), kWarps = warps_of(NT, WHOLE);
     // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
     constexpr int VT = NT == 1 ? 1 : NT / 2, VG = NT == 1 ? (NG + 1) / 2 : NG;
     // The warps' rings, (WHOLE) their states, then the list of requests, behind where their tiles start in the row's order.
@@ -591,12 +592,13 @@ int launch(const Call& c, const RowsPlan& p, cudaStream_t s) {
     if (int rc = lb_tc_status_word(&status)) return rc;
     if (p.whole) {
         auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, true>;
-        constexpr int smem = kWholeWarps * (kStages * 2 * block_bytes(HD, NG) + 4 * NT * (HD + 4) * 4) + 8 + (int)sizeof(Request);
+        constexpr int kWarps = warps_of(NT, true), smem = kWarps * (kStages * 2 * block_bytes(HD, NG) + 4 * NT * (HD + 4) * 4) + 8 + (int)sizeof(Request);
         static std::atomic<uint64_t> asked{0};
         if (int rc = allow_shared(kernel, smem, asked)) return rc;
-        LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(c.pages.n_kv_head * p.tiles, c.n_seq), dim3(kWholeWarps * 32), smem, s, c, 1, p.tiles, status));
+        LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3(c.pages.n_kv_head * p.tiles, c.n_seq), dim3(kWarps * 32), smem, s, c, 1, p.tiles, status));
         return LB_OK;
     }
+    constexpr int kWarps = warps_of(NT, false);
     auto kernel = attention4_rows_kernel<HD, NG, NT, PLAIN, false>;
     const int smem = kWarps * kStages * 2 * block_bytes(HD, NG) + 4 * (p.per_row + 1) + (int)sizeof(Request) * p.per_row;
     static std::atomic<uint64_t> asked{0};
@@ -624,13 +626,12 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     RowsPlan& p = *plan;
     p.rows = max_rows > 4 ? 8 : 4;
     p.tiles = (max_rows + p.rows - 1) / p.rows;
-    // Where an SM has a row tile at most, and it few keys, a block makes its result (1 request, 25 heads of 64 on 512 keys: DECODE1), the other way the states' launch is as long as the rest.
-    p.whole = (int64_t)n_seq * n_kv_head * p.tiles <= n_sm && (max_keys + kBlockKeys - 1) / kBlockKeys <= kWholeTiles;
     // A launch row numbers its tiles in 32 bits.
     const int64_t units = (int64_t)n_kv_head * p.tiles, most = units * ((max_keys + kBlockKeys - 1) / kBlockKeys);
     LB_CHECK_ARG(most <= 1 << 30, "attention4: a request of %d rows and %d keys is more than one launch takes", max_rows, max_keys);
     p.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)std::max(1, n_seq), (int64_t)kMostRequests, ((int64_t)1 << 30) / std::max<int64_t>(1, most)}));
-    const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
+    const int kWarps = warps_of(p.rows / 4, false);
+    const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4, false) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
     p.blocks = (int)std::max<int64_t>(1, (warps + kWarps - 1) / kWarps);
     // Runs that a row has, about; a warp takes some four of them.
     const int64_t runs = p.blocks * kWarps / (units * p.per_row) + 2;
@@ -639,6 +640,20 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
     p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
+    // Which way: by an estimate of both in microseconds, from 150 calls of 1 to 64 requests on 64 to 8,192 keys (25 heads of 64; 32 over 8, and over 4, of 128).  Blocks that have a row tile's keys to
+    // themselves: a start and an end for each wave of them, and the keys, which all SMs' blocks read side by side (1 request, 25 heads, 512 keys 5.9 us, the other way 8.6; 64 requests, 8 heads, 4,096 keys
+    // 68 / 79).  Warps that share all tiles: a start, a join, and the tiles of a warp (1 request, 8 heads, 8,192 keys 39 / 13; 16 requests 42 / 40).
+    const bool wide = head_dim == 128, two = p.rows == 8;
+    const double all = (double)units * n_seq, thousands = max_keys / 1024.0;
+    const double waves = std::ceil(all / (n_sm * blocks_per_sm(head_dim, p.rows / 4, true)));
+    const double one = two ? (wide ? 4.55 : 3.3) : wide ? 4.25 : 2.9, shared = two ? (wide ? 0.0375 : 0.022) : wide ? 0.0286 : 0.0165;
+    const double whole_us = 1.3 + (two ? 5.0 : 4.2) * waves + thousands * std::max(one, shared * all);
+    const double tiles_of_warp = std::max<double>(kLeastTiles, (double)most * n_seq / (n_sm * blocks_per_sm(head_dim, p.rows / 4, false) * kWarps));
+    const double shared_us = 9.0 + tiles_of_warp * (two ? (wide ? 0.85 : 0.6) : wide ? 1.2 : 0.62) + std::min(tiles_of_warp, 10.0) * (wide && !two ? 0.0 : 0.25) + (tiles_of_warp > kLeastTiles ? 2.0 : 0.0);
+    // (The estimates take every request to be as long as the longest.  Where they are not, sharing gains and a block's own keys do not: 16 requests of 2,048 keys on average and 4,096 at most 38 us and
+    // 30.  So a block has its own keys only where that is clearly the shorter.)
+    p.whole = whole_us < 0.8 * shared_us;
+    p.us = std::min(whole_us, shared_us);
     if (p.whole) p.states = p.starts = 0;
     return LB_OK;
 }

@@ -59,15 +59,6 @@ __device__ __forceinline__ void load_values(const T* p, bool wide, float* v) {
     }
 }
 
-// max |v| as an integer that orders like it, a NaN above all.
-template <int N>
-__device__ __forceinline__ uint32_t size_of(const float* v) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    return top;
-}
-
 // The scale of a group whose largest |x| this is, bfloat16(x / 7); the rounding that follows divides by what was stored.
 template <typename T>
 __device__ __forceinline__ __nv_bfloat16 group_scale(uint32_t top) {
@@ -144,14 +135,16 @@ append4_kernel(const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, in
     const int slot = token < n_tokens ? slot_mapping[token] : -1;
     const bool there = slot >= 0 && slot >> pages.page_shift < pages.n_pages;
     float x[W][8] = {};
-    uint32_t top[W][2];                                    // of a word's first, and of its second four values
+    uint32_t top[W][2];                                    // of a word's first, and of its second four values: the bits of the largest |x|
     const T* from = (of == 0 ? k + (int64_t)token * ldk : v + (int64_t)token * ldv) + head * HD;
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (there) load_values<T, 4>(from + S::dim(of, r, i, e), wide, x[i] + 4 * e);
-            top[i][e] = size_of<4>(x[i] + 4 * e);
+            const float* y = x[i] + 4 * e;
+            // A NaN's bits are the largest of all, also among integers: fmaxf would drop it.
+            top[i][e] = max(max(__float_as_uint(y[0]) << 1, __float_as_uint(y[1]) << 1), max(__float_as_uint(y[2]) << 1, __float_as_uint(y[3]) << 1)) >> 1;
         }
     // Keys: a word lies in one group of 32, which four threads share; two words of a thread, or those of the other four, make groups of 64.  Values: a word's halves lie in two groups of 32,
     // which the eight threads share.
@@ -178,29 +171,27 @@ append4_kernel(const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, in
     uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
     const int key = slot & 15;
     __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(block + L::scale(key, NG, of));
+    uint32_t word[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         const __nv_bfloat16 sa = group_scale<T>(top[i][0]), sb = group > 32 ? sa : group_scale<T>(top[i][1]);
         const Divisor a = divisor(sa);
-        *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, i)) = eight_nibbles(x[i], a, group > 32 ? a : divisor(sb));
+        word[i] = eight_nibbles(x[i], a, group > 32 ? a : divisor(sb));
         const int da = S::dim(of, r, i, 0), db = S::dim(of, r, i, 1);
         if (da % group == 0) scales[da / group] = sa;
         if (of == 1 && group == 32 && db % group == 0) scales[db / group] = sb;
     }
+    // A thread's words are neighbours.
+    if constexpr (W == 2) *reinterpret_cast<uint2*>(block + S::place(of, key, r, 0)) = make_uint2(word[0], word[W - 1]);
+    else *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, 0)) = word[0];
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool wide, const float* v) {
+__device__ __forceinline__ void store4(float* p, bool wide, const float* v) {
     if (wide) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-            *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        }
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = lb_from_float<T>(v[i]);
+        for (int i = 0; i < 4; ++i) p[i] = v[i];
     }
 }
 
@@ -222,18 +213,43 @@ cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n
     const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(block + L::scale(key, NG, of));
     T* to = (of == 0 ? k + (int64_t)i * ldk : v + (int64_t)i * ldv) + head * HD;
     uint32_t word[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) word[j] = *reinterpret_cast<const uint32_t*>(block + S::place(of, key, r, j));
+    if constexpr (W == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(block + S::place(of, key, r, 0));
+        word[0] = u.x;
+        word[W - 1] = u.y;
+    } else {
+        word[0] = *reinterpret_cast<const uint32_t*>(block + S::place(of, key, r, 0));
+    }
 #pragma unroll
     for (int j = 0; j < W; ++j) {
         const int da = S::dim(of, r, j, 0), db = S::dim(of, r, j, 1);
-        const float sa = __bfloat162float(scales[da / group]), sb = group > 32 ? sa : __bfloat162float(scales[db / group]);
-        // Value d of a word is nibble d / 2 + 4 (d % 2), of keys and of values.  1.5 2^23 + n + 8, less that and 8.
-        float x[8];
+        const __nv_bfloat16 sa = scales[da / group], sb = group > 32 ? sa : scales[db / group];
+        if constexpr (sizeof(T) == 2) {
+            // 128 + n as bfloat16 less 136, times the scale: one rounding.  Value d of a word is nibble d / 2 + 4 (d % 2).
+            const __nv_bfloat162 offset = __float2bfloat162_rn(-136.0f);
+            uint32_t x[4];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) x[d] = (__uint_as_float((word[j] >> (4 * (d / 2 + 4 * (d % 2))) & 15u) | 0x4b400000u) - 12582920.0f) * (d < 4 ? sa : sb);
-        store4(to + da, wide, x);
-        store4(to + db, wide, x + 4);
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t u = (word[j] >> (4 * d) & 0x000f000fu) | 0x43004300u;
+                const __nv_bfloat162 y = __hmul2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), offset), __bfloat162bfloat162(d < 2 ? sa : sb));
+                x[d] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+            if (wide) {
+                *reinterpret_cast<uint2*>(to + da) = make_uint2(x[0], x[1]);
+                *reinterpret_cast<uint2*>(to + db) = make_uint2(x[2], x[3]);
+            } else {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) to[(d < 4 ? da : db) + d % 4] = __ushort_as_bfloat16((uint16_t)(x[d / 2] >> (16 * (d % 2))));
+            }
+        } else {
+            // 1.5 2^23 + n + 8, less that and 8, times the scale: exact.
+            const float fa = __bfloat162float(sa), fb = __bfloat162float(sb);
+            float x[8];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) x[d] = (__uint_as_float((word[j] >> (4 * (d / 2 + 4 * (d % 2))) & 15u) | 0x4b400000u) - 12582920.0f) * (d < 4 ? fa : fb);
+            store4(to + da, wide, x);
+            store4(to + db, wide, x + 4);
+        }
     }
 }
 

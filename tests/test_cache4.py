@@ -107,7 +107,7 @@ def _plan(kv, heads, n_seq, keys, q_len=1, dim=64):
 
 def test_how_attention_is_cut():
     """Rows a tile, blocks, and requests that share them, by the requests, heads, tokens and keys alone."""
-    assert _plan(25, 25, 64, 1024)[0] == (0, 4, 5 * 148, 64) and _plan(8, 128, 64, 1024, dim=128)[0] == (0, 8, 3 * 148, 64)
+    assert _plan(25, 25, 64, 1024)[0] == (0, 4, 2 * 148, 64) and _plan(8, 128, 64, 1024, dim=128)[0] == (0, 8, 3 * 148, 64)
     assert _plan(8, 32, 1, 16)[0][2] == 1                      # eight tiles of keys, two warps' work
     assert _plan(1, 1, 65535, 1024)[0][3] == 256              # requests in rows of the launch
     assert _plan(32, 32, 100, 1 << 27)[0][3] == 4              # a row numbers its tiles in 30 bits
@@ -119,7 +119,7 @@ def test_how_attention_is_cut():
 def test_scratch():
     """States of all runs (a run more than warps and units together has), where requests' tiles start, and the keys' weights."""
     (_, rows, blocks, per), got = _plan(8, 32, 4, 4096, dim=128)
-    states, starts = (4 * blocks + 4 * 8) * rows * 132 * 4, 5 * 4
+    states, starts = (8 * blocks + 4 * 8) * rows * 132 * 4, 5 * 4
     assert got == states + -(-starts // 16) * 16
     assert _plan(8, 32, 4, 1024, dim=128) == ((0, 4, 1, 1), 0)          # few keys: a block for each request and key/value head, whose warps' states meet in it
     c, ref = _cache(kv=8, dim=128)
