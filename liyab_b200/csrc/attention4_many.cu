@@ -69,13 +69,13 @@ __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uin
 template <int BYTES>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
     if constexpr (BYTES == 16) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
         w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
     } else if constexpr (BYTES == 8) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
         w[0] = u.x; w[1] = u.y;
     } else {
-        w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
 }
 // A word's values times s as four float16 pairs: nibbles (i, i + 4).
@@ -524,9 +524,7 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
         const int place = place_of(row), first = first_of(place);
         const int w_row = row0 + g * kBM + quarter * 32;
         const int place_lo = place_of(w_row), first_hi = first_of(place_of(w_row + 31));            // of the warp's rows
-        const lb_soft_cap capped(PLAIN ? 0.0f : c.soft_cap, 0.25f * c.soft_cap);          // in its series' form
-        const float exact_in = PLAIN ? 0.0f : 2.0f / c.soft_cap;
-        const Two cap_in = two(capped.in, capped.in);
+        const float units_out = !PLAIN && c.soft_cap > 0.0f ? c.soft_cap * kLbLog2e : 1.0f, units_in = 1.0f / units_out;          // (scores are in base 2)
         const bool biased = !PLAIN && c.distance != nullptr;
         const float r1 = biased ? c.distance[head] : 0.0f, r2 = biased ? c.distance[c.n_head + head] : 0.0f;
         const int lo = g == 0 ? g_lo[0] : g_lo[1], hi = g == 0 ? g_hi[0] : g_hi[1];
@@ -548,28 +546,32 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
             tmem_ld_wait32(v);
             if (!PLAIN || masked) {
                 if constexpr (!PLAIN) {
+                    // Scores, or, capped, in units of the cap: z, and what brings them back, f0.
+                    const float g0 = f0 * units_in, g1 = f1 * units_in;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) of_two(mul2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), i < 16 ? two(f0, f0) : two(f1, f1)), v[i], v[i + 1]);
-                    f0 = f1 = 1.0f;
+                    for (int i = 0; i < 32; i += 2) of_two(mul2(two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), i < 16 ? two(g0, g0) : two(g1, g1)), v[i], v[i + 1]);
+                    f0 = f1 = units_out;
                     if (c.soft_cap > 0.0f) {
-                        // Where no score of the warp passes a quarter of the cap, the series of tanh (see lb_soft_cap); else 1 - 2 / (1 + e^2x).
+                        // Where no score of the warp passes a quarter of the cap, tanh z is z times the polynomial in z^2 that is nearest to tanh z / z on 0 .. 1/16 (within 5.1e-7 of it); else
+                        // 1 - 2 / (1 + e^2z).
                         float size = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) size = max3(size, fabsf(__uint_as_float(v[i])), fabsf(__uint_as_float(v[i + 1])));
-                        if (__all_sync(0xffffffffu, size <= 0.25f * capped.out)) {
+                        if (__all_sync(0xffffffffu, size <= 0.25f)) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const Two z = two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), w = mul2(z, cap_in), y = mul2(w, w);
-                                of_two(fma2(mul2(z, y), fma2(y, fma2(y, two(-17.0f / 315.0f, -17.0f / 315.0f), two(2.0f / 15.0f, 2.0f / 15.0f)), two(-1.0f / 3.0f, -1.0f / 3.0f)), z), v[i], v[i + 1]);
+                                const Two z = two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), y = mul2(z, z);
+                                of_two(mul2(z, fma2(y, fma2(y, two(0.128418818f, 0.128418818f), two(-0.333219707f, -0.333219707f)), two(0.999999642f, 0.999999642f))), v[i], v[i + 1]);
                             }
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(-2.0f * capped.out, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[i]) * exact_in)), capped.out));
+                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(-2.0f, __fdividef(1.0f, 1.0f + ex2(__uint_as_float(v[i]) * (2.0f * kLbLog2e))), 1.0f));
                         }
                     }
                     if (biased) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) - lb_distance_penalty_log2(r1, r2, max(place - (key0 + i), 0)));
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), units_out, -lb_distance_penalty_log2(r1, r2, max(place - (key0 + i), 0))));
+                        f0 = f1 = 1.0f;
                     }
                 }
                 if (masked) {
