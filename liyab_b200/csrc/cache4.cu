@@ -1,6 +1,6 @@
 // The 4-bit cache's own work: rows in, values out, and eviction.
 //
-// append4 and cache4_values move each value once; sixteen threads have a row, in the order of cache4.cuh.
+// append4 and cache4_values move each value once; eight threads have a row of keys or of values, in the order of cache4.cuh.
 // evict4 is two launches.  The first chooses: a block a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  The
 // second copies: a warp a block of sixteen keys of the destination, whose pieces it gathers.  The destination is never a source, so nothing waits for anything.
@@ -36,26 +36,37 @@ namespace {
 
 using namespace lb_c4;
 
-// N (4 or 8) neighbouring values of a row.
+// N (4 or 8) neighbouring values of a row as 32-bit numbers, and the bits of the largest |x|.  (Compared as integers, where a NaN is the largest of all: fmaxf would drop it.)
 template <typename T, int N>
-__device__ __forceinline__ void load_values(const T* p, bool wide, float* v) {
-    if (wide) {
-        if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ uint32_t load_values(const T* p, bool wide, float* v) {
+    if constexpr (sizeof(T) == 4) {
+        if (wide) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(p + i);
         } else {
-            uint32_t u[N / 2];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = p[i];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(v[i]) << 1);
+        return top >> 1;
+    } else {
+        uint32_t u[N / 2], top = 0;
+        if (wide) {
             if constexpr (N == 8) *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(p);
             else *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(p);
+        } else {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                v[2 * i] = __uint_as_float(u[i] << 16);
-                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-            }
+            for (int i = 0; i < N / 2; ++i) u[i] = __bfloat16_as_ushort(p[2 * i]) | (uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16;
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = lb_to_float(p[i]);
+        for (int i = 0; i < N / 2; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+            top = __vmaxu2(top, u[i] & 0x7fff7fffu);
+        }
+        return max(top << 16, top & 0xffff0000u);
     }
 }
 
@@ -80,20 +91,30 @@ __device__ __forceinline__ Divisor divisor(__nv_bfloat16 scale) {
 }
 
 // Eight values over their scales (the first four over a), the quotients rounded to 32 bits and then to the nearest even integer, as nibbles n + 8: nibble n is value 2 (n % 4) + n / 4, of keys and of
-// values.  The quotient is x r corrected by its rest times r, r the scale's rounded reciprocal (Markstein's division, correctly rounded): six operations a value with the rounding (adding 1.5 2^23) and the
-// place in the word (four numbers -7 .. 7 in base 16).  |x| is at most 7.03 s as long as s is a normal number.
+// values.  |x| is at most 7.03 s as long as s is a normal number, so the integers are -7 .. 7.  They come out of an addition of 1.5 2^23, whose bits are a number in base 16 as they are: what the
+// eight times 0x4b400000 come to is taken off at the end, modulo 2^32.
+// The quotient of float32 numbers is x r corrected by its rest times r, r the scale's rounded reciprocal (Markstein's division, correctly rounded).  That of bfloat16 numbers (eight bits each) lies on
+// the middle of two integers or 2^-10 away from it at least: (2 a 2^d - (2 k + 1) b) / 2 b for whole a, b < 256, where d >= -2 as a quotient below 1 / 4 rounds to 0.  So x r, off by 2^-21 at
+// most, rounded to a multiple of 2^-11 by adding 6144 lies on the same side of the middle, or on it.
+template <typename T>
 __device__ __forceinline__ uint32_t eight_nibbles(const float* x, const Divisor& a, const Divisor& b) {
-    constexpr float kMagic = 12582912.0f;
+    constexpr float kMagic = 12582912.0f, kCoarse = 6144.0f;
     if (a.plain() && b.plain()) {
-        float half[2] = {0.0f, 0.0f};
+        uint32_t word = 0;
 #pragma unroll
         for (int n = 7; n >= 0; --n) {
             const int d = 2 * (n & 3) + (n >> 2);
-            const float s = d < 4 ? a.s : b.s, r = d < 4 ? a.r : b.r, q = x[d] * r;
-            half[n >> 2] = fmaf(half[n >> 2], 16.0f, fmaf(fmaf(-q, s, x[d]), r, q) + kMagic - kMagic);
+            const float s = d < 4 ? a.s : b.s, r = d < 4 ? a.r : b.r;
+            float whole;
+            if constexpr (sizeof(T) == 2) {
+                whole = fmaf(x[d], r, kCoarse) + (kMagic - kCoarse);
+            } else {
+                const float q = x[d] * r;
+                whole = fmaf(fmaf(-q, s, x[d]), r, q) + kMagic;
+            }
+            word = (word << 4) + __float_as_uint(whole);
         }
-        const uint32_t lo = __float_as_uint(half[0] + (kMagic + 34952.0f)), hi = __float_as_uint(half[1] + (kMagic + 34952.0f));         // 8 added to each: 0x8888
-        return __byte_perm(lo, hi, 0x5410);
+        return word + (8u - 0x4b400000u) * 0x11111111u;
     }
     uint32_t word = 0;                                     // scales of 0, NaN, or with a reciprocal past float32's range
 #pragma unroll 1
@@ -108,82 +129,78 @@ __device__ __forceinline__ uint32_t eight_nibbles(const float* x, const Divisor&
     return word;
 }
 
-// Eight threads have a row of keys, the next eight its values: HD / 64 words each.
-template <int HD>
+// Eight threads have a row of keys (OF 0) or values (1), HD / 64 words each; they are neighbours in a warp, which has four rows of the same kind.  A block has sixteen tokens' rows of one head, keys
+// and values.
+template <int HD, int NG, int OF>
 struct Share {
-    static constexpr int kWords = HD / 64, kRowThreads = 16, kBlockRows = 256 / kRowThreads;
-    // The first dim of word i's first, and of its second four values; r: the thread of the eight.
-    __device__ static int dim(int of, int r, int i, int second) {
-        return of == 0 ? 32 * ((r >> 2) * kWords + i) + 8 * (r & 3) + 4 * second : 64 * i + 32 * second + 4 * r;
-    }
-    __device__ static int place(int of, int key, int r, int i) {
-        return of == 0 ? Layout<HD>::k_word(key, 4 * ((r >> 2) * kWords + i) + (r & 3)) : Layout<HD>::v_word(key, r, i);
-    }
+    static constexpr int kWords = HD / 64, kGroup = HD / NG;
+    // A thread's groups, and that of word i's first (second) four values.  Keys: a word lies in one group of 32, which four threads share.  Values: a word's halves lie in two groups of 32, which
+    // eight threads share.
+    static constexpr int kGroups = OF == 0 ? (kGroup == 32 ? kWords : 1) : kGroup == 32 ? 2 * kWords : kGroup == 64 ? kWords : 1;
+    static constexpr bool kAll = OF == 1 || kGroup == HD;               // whether eight threads share a group
+    __device__ static constexpr int group(int i, int second) { return OF == 0 ? (kGroup == 32 ? i : 0) : kGroup == 32 ? 2 * i + second : kGroup == 64 ? i : 0; }
+    // The first dim of a word's first, and of its second four values; r: the thread of the eight.
+    __device__ static int dim(int r, int i, int second) { return OF == 0 ? 32 * ((r >> 2) * kWords + i) + 8 * (r & 3) + 4 * second : 64 * i + 32 * second + 4 * r; }
+    // Which of the row's scales a thread's is.
+    __device__ static int scale(int r, int gr) { return kGroups == NG ? gr : OF == 0 ? (r >> 2) * kGroups + gr : 0; }
+    __device__ static int place(int key, int r) { return OF == 0 ? Layout<HD>::k_word(key, 4 * (r >> 2) * kWords + (r & 3)) : Layout<HD>::v_word(key, r, 0); }
 };
+constexpr int kBlockRows = 16;
+
+template <typename T, int HD, int NG, int OF>
+__device__ __forceinline__ void append_row(const T* __restrict__ rows, int64_t ld, const int32_t* __restrict__ slot_mapping, const Pages& pages, int n_tokens, bool wide) {
+    using S = Share<HD, NG, OF>;
+    constexpr int W = S::kWords;
+    const int token = blockIdx.x * kBlockRows + ((threadIdx.x & 127) >> 3), head = blockIdx.y, r = threadIdx.x & 7;
+    // Threads past the end and those of skipped rows go along with the shuffles.
+    const int slot = token < n_tokens ? slot_mapping[token] : -1;
+    const bool there = slot >= 0 && slot >> pages.page_shift < pages.n_pages;
+    float x[W][8] = {};
+    uint32_t top[S::kGroups] = {};
+    const T* from = rows + (int64_t)token * ld + head * HD;
+    if (there) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (OF == 0) {
+                top[S::group(i, 0)] = max(top[S::group(i, 0)], load_values<T, 8>(from + S::dim(r, i, 0), wide, x[i]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) top[S::group(i, e)] = max(top[S::group(i, e)], load_values<T, 4>(from + S::dim(r, i, e), wide, x[i] + 4 * e));
+            }
+        }
+    }
+#pragma unroll
+    for (int gr = 0; gr < S::kGroups; ++gr) {
+        top[gr] = max(top[gr], __shfl_xor_sync(0xffffffffu, top[gr], 1));
+        top[gr] = max(top[gr], __shfl_xor_sync(0xffffffffu, top[gr], 2));
+        if (S::kAll) top[gr] = max(top[gr], __shfl_xor_sync(0xffffffffu, top[gr], 4));
+    }
+    if (!there) return;
+    uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
+    const int key = slot & 15;
+    __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(block + Layout<HD>::scale(key, NG, OF));
+    Divisor by[S::kGroups];
+#pragma unroll
+    for (int gr = 0; gr < S::kGroups; ++gr) {
+        const __nv_bfloat16 scale = group_scale<T>(top[gr]);
+        by[gr] = divisor(scale);
+        if ((S::kAll ? r : r & 3) == 0) scales[S::scale(r, gr)] = scale;
+    }
+    uint32_t word[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) word[i] = eight_nibbles<T>(x[i], by[S::group(i, 0)], by[S::group(i, 1)]);
+    // A thread's words are neighbours.
+    if constexpr (W == 2) *reinterpret_cast<uint2*>(block + S::place(key, r)) = make_uint2(word[0], word[W - 1]);
+    else *reinterpret_cast<uint32_t*>(block + S::place(key, r)) = word[0];
+}
 
 template <typename T, int HD, int NG>
 __global__ void __launch_bounds__(256)
 append4_kernel(const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv, const int32_t* __restrict__ slot_mapping, const Pages pages, int n_tokens, int wide) {
-    using L = Layout<HD>;
-    using S = Share<HD>;
-    constexpr int W = S::kWords, group = HD / NG;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int row = blockIdx.x * S::kBlockRows + threadIdx.x / S::kRowThreads, of = threadIdx.x >> 3 & 1, r = threadIdx.x & 7;
-    const int token = row / pages.n_kv_head, head = row - token * pages.n_kv_head;
-    // The threads of a row are neighbours in one warp; those past the end and those of skipped rows go along with the shuffles.
-    const int slot = token < n_tokens ? slot_mapping[token] : -1;
-    const bool there = slot >= 0 && slot >> pages.page_shift < pages.n_pages;
-    float x[W][8] = {};
-    uint32_t top[W][2];                                    // of a word's first, and of its second four values: the bits of the largest |x|
-    const T* from = (of == 0 ? k + (int64_t)token * ldk : v + (int64_t)token * ldv) + head * HD;
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (there) load_values<T, 4>(from + S::dim(of, r, i, e), wide, x[i] + 4 * e);
-            const float* y = x[i] + 4 * e;
-            // A NaN's bits are the largest of all, also among integers: fmaxf would drop it.
-            top[i][e] = max(max(__float_as_uint(y[0]) << 1, __float_as_uint(y[1]) << 1), max(__float_as_uint(y[2]) << 1, __float_as_uint(y[3]) << 1)) >> 1;
-        }
-    // Keys: a word lies in one group of 32, which four threads share; two words of a thread, or those of the other four, make groups of 64.  Values: a word's halves lie in two groups of 32,
-    // which the eight threads share.
-    if (of == 0 || group > 32) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) top[i][0] = top[i][1] = max(top[i][0], top[i][1]);
-    }
-    if (W == 2 && (group == 128 || (group == 64 && of == 0))) top[0][0] = top[0][1] = top[W - 1][0] = top[W - 1][1] = max(top[0][0], top[W - 1][0]);
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            if (group > 32 && e == 1) {
-                top[i][1] = top[i][0];
-                continue;
-            }
-            uint32_t a = top[i][e];
-            a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-            a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-            const uint32_t far = __shfl_xor_sync(0xffffffffu, a, 4);
-            top[i][e] = of == 1 || group == HD ? max(a, far) : a;
-        }
-    if (!there) return;
-    uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
-    const int key = slot & 15;
-    __nv_bfloat16* scales = reinterpret_cast<__nv_bfloat16*>(block + L::scale(key, NG, of));
-    uint32_t word[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const __nv_bfloat16 sa = group_scale<T>(top[i][0]), sb = group > 32 ? sa : group_scale<T>(top[i][1]);
-        const Divisor a = divisor(sa);
-        word[i] = eight_nibbles(x[i], a, group > 32 ? a : divisor(sb));
-        const int da = S::dim(of, r, i, 0), db = S::dim(of, r, i, 1);
-        if (da % group == 0) scales[da / group] = sa;
-        if (of == 1 && group == 32 && db % group == 0) scales[db / group] = sb;
-    }
-    // A thread's words are neighbours.
-    if constexpr (W == 2) *reinterpret_cast<uint2*>(block + S::place(of, key, r, 0)) = make_uint2(word[0], word[W - 1]);
-    else *reinterpret_cast<uint32_t*>(block + S::place(of, key, r, 0)) = word[0];
+    if (threadIdx.x < 128) append_row<T, HD, NG, 0>(k, ldk, slot_mapping, pages, n_tokens, wide != 0);
+    else append_row<T, HD, NG, 1>(v, ldv, slot_mapping, pages, n_tokens, wide != 0);
 }
 
 __device__ __forceinline__ void store4(float* p, bool wide, const float* v) {
@@ -195,35 +212,33 @@ __device__ __forceinline__ void store4(float* p, bool wide, const float* v) {
     }
 }
 
-template <typename T, int HD, int NG>
-__global__ void __launch_bounds__(256)
-cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv, int wide) {
-    using L = Layout<HD>;
-    using S = Share<HD>;
-    constexpr int W = S::kWords, group = HD / NG;
-    lb_wait_for_predecessor();
-    lb_dependents_may_launch();
-    const int row = blockIdx.x * S::kBlockRows + threadIdx.x / S::kRowThreads, of = threadIdx.x >> 3 & 1, r = threadIdx.x & 7;
-    const int i = row / pages.n_kv_head, head = row - i * pages.n_kv_head;
+template <typename T, int HD, int NG, int OF>
+__device__ __forceinline__ void row_values(const Pages& pages, const int32_t* __restrict__ slots, int n, T* __restrict__ rows, int64_t ld, bool wide) {
+    using S = Share<HD, NG, OF>;
+    constexpr int W = S::kWords;
+    const int i = blockIdx.x * kBlockRows + ((threadIdx.x & 127) >> 3), head = blockIdx.y, r = threadIdx.x & 7;
     if (i >= n) return;
     const int slot = slots[i];
     if (slot < 0 || slot >> pages.page_shift >= pages.n_pages) return;
     const uint8_t* block = pages.memory + pages.at(slot >> pages.page_shift, head, slot);
     const int key = slot & 15;
-    const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(block + L::scale(key, NG, of));
-    T* to = (of == 0 ? k + (int64_t)i * ldk : v + (int64_t)i * ldv) + head * HD;
+    const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(block + Layout<HD>::scale(key, NG, OF));
+    T* to = rows + (int64_t)i * ld + head * HD;
     uint32_t word[W];
     if constexpr (W == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(block + S::place(of, key, r, 0));
+        const uint2 u = *reinterpret_cast<const uint2*>(block + S::place(key, r));
         word[0] = u.x;
         word[W - 1] = u.y;
     } else {
-        word[0] = *reinterpret_cast<const uint32_t*>(block + S::place(of, key, r, 0));
+        word[0] = *reinterpret_cast<const uint32_t*>(block + S::place(key, r));
     }
+    __nv_bfloat16 by[S::kGroups];
+#pragma unroll
+    for (int gr = 0; gr < S::kGroups; ++gr) by[gr] = scales[S::scale(r, gr)];
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-        const int da = S::dim(of, r, j, 0), db = S::dim(of, r, j, 1);
-        const __nv_bfloat16 sa = scales[da / group], sb = group > 32 ? sa : scales[db / group];
+        const int da = S::dim(r, j, 0), db = S::dim(r, j, 1);
+        const __nv_bfloat16 sa = by[S::group(j, 0)], sb = by[S::group(j, 1)];
         if constexpr (sizeof(T) == 2) {
             // 128 + n as bfloat16 less 136, times the scale: one rounding.  Value d of a word is nibble d / 2 + 4 (d % 2).
             const __nv_bfloat162 offset = __float2bfloat162_rn(-136.0f);
@@ -234,12 +249,14 @@ cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n
                 const __nv_bfloat162 y = __hmul2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&u), offset), __bfloat162bfloat162(d < 2 ? sa : sb));
                 x[d] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            if (wide) {
-                *reinterpret_cast<uint2*>(to + da) = make_uint2(x[0], x[1]);
-                *reinterpret_cast<uint2*>(to + db) = make_uint2(x[2], x[3]);
-            } else {
+            if (!wide) {
 #pragma unroll
                 for (int d = 0; d < 8; ++d) to[(d < 4 ? da : db) + d % 4] = __ushort_as_bfloat16((uint16_t)(x[d / 2] >> (16 * (d % 2))));
+            } else if constexpr (OF == 0) {
+                *reinterpret_cast<uint4*>(to + da) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
+                *reinterpret_cast<uint2*>(to + da) = make_uint2(x[0], x[1]);
+                *reinterpret_cast<uint2*>(to + db) = make_uint2(x[2], x[3]);
             }
         } else {
             // 1.5 2^23 + n + 8, less that and 8, times the scale: exact.
@@ -251,6 +268,15 @@ cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n
             store4(to + db, wide, x + 4);
         }
     }
+}
+
+template <typename T, int HD, int NG>
+__global__ void __launch_bounds__(256)
+cache4_values_kernel(const Pages pages, const int32_t* __restrict__ slots, int n, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv, int wide) {
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
+    if (threadIdx.x < 128) row_values<T, HD, NG, 0>(pages, slots, n, k, ldk, wide != 0);
+    else row_values<T, HD, NG, 1>(pages, slots, n, v, ldv, wide != 0);
 }
 
 // ---- eviction ----
@@ -451,20 +477,18 @@ bool wide_rows(const void* p, int64_t ld, int bytes) { return reinterpret_cast<u
 template <typename T>
 int append_rows(const T* k, int64_t ldk, const T* v, int64_t ldv, const int32_t* slots, const Pages& pages, int hd, int n, cudaStream_t s) {
     const int wide = wide_rows(k, ldk, sizeof(T)) && wide_rows(v, ldv, sizeof(T));
-    LB_CHECK_ARG((int64_t)n * pages.n_kv_head <= INT32_MAX - 256, "append4: %d tokens are more than one launch takes", n);
-    const int blocks = (n * pages.n_kv_head + 15) / 16;                  // a block has sixteen rows
+    const dim3 blocks((unsigned)((n + (int64_t)kBlockRows - 1) / kBlockRows), (unsigned)pages.n_kv_head);
     LB_CHECK_CUDA(lb_launch_overlapped(hd == 64 ? (pages.groups == 1 ? append4_kernel<T, 64, 1> : append4_kernel<T, 64, 2>)
-                                       : pages.groups == 1 ? append4_kernel<T, 128, 1> : pages.groups == 2 ? append4_kernel<T, 128, 2> : append4_kernel<T, 128, 4>, dim3((unsigned)blocks), dim3(256), 0, s, k, ldk, v, ldv, slots, pages, n, wide));
+                                       : pages.groups == 1 ? append4_kernel<T, 128, 1> : pages.groups == 2 ? append4_kernel<T, 128, 2> : append4_kernel<T, 128, 4>, blocks, dim3(256), 0, s, k, ldk, v, ldv, slots, pages, n, wide));
     return LB_OK;
 }
 
 template <typename T>
 int value_rows(const Pages& pages, const int32_t* slots, int n, T* k, int64_t ldk, T* v, int64_t ldv, int hd, cudaStream_t s) {
     const int wide = wide_rows(k, ldk, sizeof(T)) && wide_rows(v, ldv, sizeof(T));
-    LB_CHECK_ARG((int64_t)n * pages.n_kv_head <= INT32_MAX - 256, "cache4_values: %d rows are more than one launch takes", n);
-    const int blocks = (n * pages.n_kv_head + 15) / 16;                  // a block has sixteen rows
+    const dim3 blocks((unsigned)((n + (int64_t)kBlockRows - 1) / kBlockRows), (unsigned)pages.n_kv_head);
     LB_CHECK_CUDA(lb_launch_overlapped(hd == 64 ? (pages.groups == 1 ? cache4_values_kernel<T, 64, 1> : cache4_values_kernel<T, 64, 2>)
-                                       : pages.groups == 1 ? cache4_values_kernel<T, 128, 1> : pages.groups == 2 ? cache4_values_kernel<T, 128, 2> : cache4_values_kernel<T, 128, 4>, dim3((unsigned)blocks), dim3(256), 0, s, pages, slots, n, k, ldk, v, ldv,
+                                       : pages.groups == 1 ? cache4_values_kernel<T, 128, 1> : pages.groups == 2 ? cache4_values_kernel<T, 128, 2> : cache4_values_kernel<T, 128, 4>, blocks, dim3(256), 0, s, pages, slots, n, k, ldk, v, ldv,
                                        wide));
     return LB_OK;
 }

@@ -45,7 +45,7 @@ struct Pages {
     __device__ __forceinline__ int64_t at(int page, int head, int key) const {
         if ((unsigned)page >= (unsigned)n_pages) return -1;
         const int in_page = key & ((1 << page_shift) - 1);
-        return ((((int64_t)page * n_kv_head + head) << (page_shift - 4)) + (in_page >> 4)) * block;
+        return (int64_t)(((page * n_kv_head + head) << (page_shift - 4)) + (in_page >> 4)) * block;          // (a cache has fewer than 2^31 blocks)
     }
 };
 
