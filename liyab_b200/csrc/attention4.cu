@@ -54,17 +54,6 @@ struct Plan {
     int64_t scores, log_sums, partial, starts, bytes;       // offsets in the scratch memory
 };
 
-// Whether the tcgen05 kernel takes a call: by an estimate of both in microseconds (the other's: rows_plan), from their times on 84 calls of 1 to 128 tokens a request (1 and 8 requests on 256, 2,048 and
-// 16,384 keys, 32 heads over 8 of 128 and 12 over 12 of 64): a start and an end, a join of states, and what a block takes for 128 keys, which is little less where it has 128 rows or fewer.  (8 requests
-// on 2,048 keys, 32 heads over 8: 8 tokens each 34 us on the kernel for few rows, 36 on this; 16 tokens 52 / 36; 1 request on 2,048 keys: 32 tokens 20 / 24, 128 tokens 51 / 32.)
-bool takes_many(const lb_attention4_args& a, int max_rows, int keys, const RowsPlan& few, const TilesPlan& many, int n_sm) {
-    if (a.total != nullptr) return false;
-    const bool wide = a.cache->head_dim == 128;
-    const double blocks = (double)a.n_seq * a.cache->n_kv_head * ((max_rows + 255) / 256) * many.splits, each = ((keys + 127) / 128 + many.splits - 1) / many.splits;
-    const double many_us = (many.splits > 1 ? 12.0 : 9.0) + std::ceil(blocks / n_sm) * each * (max_rows <= 128 ? (wide ? 2.5 : 1.9) : wide ? 2.9 : 2.6);
-    return many_us < few.us;
-}
-
 int check(const lb_attention4_args* args, Call* c, Plan* p) {
     LB_CHECK_ARG(args != nullptr, "attention4: no arguments");
     const lb_attention4_args& a = *args;
@@ -106,8 +95,10 @@ int check(const lb_attention4_args* args, Call* c, Plan* p) {
     auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
     const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
     if (int rc = rows_plan(&p->rows, a.n_seq, a.cache->n_kv_head, (int)rows, keys, a.cache->head_dim, n_sm)) return rc;
-    p->tiles = tiles_plan(a.n_seq, a.cache->n_kv_head, (int)rows, keys, a.cache->head_dim, n_sm);
-    p->many = takes_many(a, (int)rows, keys, p->rows, p->tiles, n_sm);
+    p->tiles = tiles_plan(a.n_seq, a.cache->n_kv_head, c->per, (int)rows, keys, a.window, a.cache->head_dim, n_sm);
+    // The tcgen05 kernel takes a call where the estimates (rows_plan, tiles_plan), which are from both kernels' times on 84 calls of 1 to 128 tokens a request, say so: 8 requests on 2,048 keys, 32 heads
+    // over 8: 8 tokens each 34 us on the kernel for few rows, 36 on this; 16 tokens 52 / 36; 1 request on 2,048 keys: 32 tokens 20 / 24, 128 tokens 51 / 32.
+    p->many = a.total == nullptr && p->tiles.us < p->rows.us;
     p->scores = 0;
     p->log_sums = a.total != nullptr ? up(units * rows * keys * 4) : 0;
     p->partial = p->log_sums + (a.total != nullptr ? up(units * rows * 4) : 0);

@@ -64,12 +64,13 @@ struct RowsPlan {
     int64_t states, starts;
 };
 int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
-// Portions of many rows, on tcgen05: blocks that share a row tile's keys, bytes of their states.
+// Portions of many rows, on tcgen05: blocks that may share a row tile's keys, tiles of 128 keys each has at most, bytes of their states, about how long it takes.
 struct TilesPlan {
-    int splits;
+    int splits, share;
     int64_t states;
+    double us;
 };
-TilesPlan tiles_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+TilesPlan tiles_plan(int n_seq, int n_kv_head, int per, int max_rows, int max_keys, int window, int head_dim, int n_sm);
 int many_rows(const Call& c, int head_dim, const TilesPlan& p, cudaStream_t stream);
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t stream);
 

@@ -45,7 +45,7 @@ struct Control {
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups][2];       // of units in turn: what waits may be a unit behind, and a parity tells no more than two phases apart
     uint32_t tmem_base;
-    int abort_flag;
+    int abort_flag, whole;                                                 // whole: the block has all keys of its rows
     float k_factor[kNotes][kMakers], v_exponent[kNotes][kMakers];          // of a tile's blocks of sixteen keys
     uint8_t gone[kNotes][kMakers], nans[kNotes][kMakers];                  // on no page; values with scales that are NaN
     uint8_t nan_groups[kNotes][kBN];                                       // a bit a group
@@ -214,9 +214,23 @@ __device__ __forceinline__ bool any_of_pair(int barrier, bool mine) {
     return any != 0;
 }
 
+// The keys that a tile of rows sees: the first (the start of a tile of keys), and tiles.
+__device__ __forceinline__ void keys_of_rows(const Call& c, const Portion& part, int row0, int* lo, int* tiles) {
+    const int n_rows = part.count * c.per, limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;
+    auto place_of = [&](int row) { return min(part.place + min(row, n_rows - 1) / c.per, limit); };
+    const int last = place_of(row0 + kTileRows - 1);
+    *lo = 0;
+    if (c.window != 0) {
+        const int first = place_of(row0);
+        *lo = first < 0 ? 0 : lb_first_visible(first, c.window) / kBN * kBN;
+    }
+    *tiles = last >= 0 ? (last - *lo) / kBN + 1 : 0;
+}
+
+// `n_splits` blocks share a row tile's keys, `share` tiles of keys each, the last what is left.
 template <int HD, int NG, bool PLAIN>
 __global__ void __launch_bounds__(kManyThreads, 1)
-attention4_many_kernel(const Call c, int n_splits, int* status) {
+attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
     using L = Layout<HD>;
     constexpr int SUBS = HD / 64, JK = HD / 32, JV = HD / 64;
     extern __shared__ uint8_t smem_raw[];
@@ -232,16 +246,18 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
     lb_dependents_may_launch();
     const int seq = blockIdx.z, kvh = blockIdx.y, kv = c.pages.n_kv_head;
     const Portion part = portion_of(c, seq);
-    // The last tiles first, which see the most keys; `n_splits` blocks share a tile's.
+    // The last tiles first, which see the most keys.
     const int split = (int)blockIdx.x % n_splits;
     const int n_rows = part.count * c.per, row0 = ((n_rows + kTileRows - 1) / kTileRows - 1 - (int)blockIdx.x / n_splits) * kTileRows;
     if (row0 < 0 || n_rows <= 0) return;
     const int limit = min(c.max_keys, c.table_stride << c.pages.page_shift) - 1;          // no key past this place is read
     auto place_of = [&](int row) { return min(part.place + min(row, n_rows - 1) / c.per, limit); };
     auto first_of = [&](int place) { return place < 0 ? 0 : lb_first_visible(place, c.window); };
-    const int last = place_of(row0 + kTileRows - 1), all_lo = first_of(place_of(row0)) / kBN * kBN, all_tiles = last >= 0 ? (last - all_lo) / kBN + 1 : 0;
-    const int share = (all_tiles + n_splits - 1) / n_splits, kv_lo = all_lo + split * share * kBN;
-    const int n_tiles = max(0, min(share, all_tiles - split * share)), p_hi = min(last, kv_lo + n_tiles * kBN - 1);
+    int all_lo, all_tiles;
+    keys_of_rows(c, part, row0, &all_lo, &all_tiles);
+    if (split > 0 && split * share >= all_tiles) return;
+    const int last = place_of(row0 + kTileRows - 1), kv_lo = all_lo + split * share * kBN;
+    const int n_tiles = split == n_splits - 1 ? all_tiles - split * share : min(share, all_tiles - split * share), p_hi = min(last, kv_lo + n_tiles * kBN - 1);
     // Whether rows of group g see keys of unit u.
     int g_lo[kGroups], g_hi[kGroups];                               // units
 #pragma unroll
@@ -267,6 +283,7 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
             mbar_init(&ctl->o_done[i / 2][i % 2], 1);
         }
         ctl->abort_flag = 0;
+        ctl->whole = all_tiles <= share;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kIssuer) {
@@ -509,8 +526,7 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
                 for (int e = 0; e < 4; ++e)
                     w[e] = finite ? h2(__floats2half2_rn(__uint_as_float(u[i][e] << 16) * up * up2, __uint_as_float(u[i][e] & 0xffff0000u) * up * up2)) : 0u;
                 *reinterpret_cast<uint4*>(q_s + ((r >> 7) * SUBS + (chunk >> 3)) * kSub + (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                // (Not 0, so that -inf stays what it is.)
-                if (chunk == 0) ctl->row_scale[r] = !finite ? CUDART_NAN_F : fmaxf(fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2), 1e-37f);
+                if (chunk == 0) ctl->row_scale[r] = !finite ? CUDART_NAN_F : fabsf(c.scale) * kLbLog2e * pow2(-shift / 2) * pow2(-shift - -shift / 2);
             }
             }
             fence_async_shared();
@@ -582,6 +598,9 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
                     if (gone1 != 0) seen &= 0x0000ffffu;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = (seen >> i & 1u) != 0 ? v[i] : 0xff800000u;
+                    // Times a factor that is 0 in 32 bits it would be NaN.  (What the least factor makes of a score is nothing beside 1; a NaN stays.)
+                    f0 = f0 < 1e-37f ? 1e-37f : f0;
+                    f1 = f1 < 1e-37f ? 1e-37f : f1;
                 }
             }
             float h[2][2];
@@ -672,8 +691,8 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
         nan_bits |= ctl->row_nans[g][x ^ 1][quarter * 32 + lane];
         if (ok && w_row < n_rows) {
             tc_fence_after();
-            // A row's result; where blocks share its keys a state, normed so that its sum is 1.
-            const bool none = l == 0.0f, whole = n_splits == 1;                          // no key seen: O may be what the memory held
+            // A row's result; where blocks share its keys a state, normed so that its sum is 1.  (Rows whose keys are one block's share have none.)
+            const bool none = l == 0.0f, whole = ctl->whole != 0;                          // no key seen: O may be what the memory held
             float* state = c.partial + ((((int64_t)seq * kv + kvh) * c.max_rows + row) * n_splits + split) * (HD + 4);
             if (!whole && there && x == 0) *reinterpret_cast<float2*>(state) = make_float2(none ? kLowest : m + log2f(l), none ? 0.0f : 1.0f);
             float factor = 1.0f;
@@ -718,14 +737,17 @@ attention4_many_kernel(const Call c, int n_splits, int* status) {
 // The states of blocks that share a row's keys.
 template <int HD>
 __global__ void __launch_bounds__(128)
-attention4_many_join_kernel(const Call c, int n_splits) {
+attention4_many_join_kernel(const Call c, int n_splits, int share) {
     __shared__ float joined[1][HD + 2];
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
     const int seq = blockIdx.z, kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 5);
     const Portion part = portion_of(c, seq);
     const float* state = r < part.count * c.per ? c.partial + (((int64_t)seq * c.pages.n_kv_head + kvh) * c.max_rows + r) * n_splits * (HD + 4) : nullptr;
-    join_row<HD>(c, part, seq, kvh, r, state, HD + 4, n_splits, 0, joined);
+    int lo, all_tiles;
+    keys_of_rows(c, part, r / kTileRows * kTileRows, &lo, &all_tiles);
+    if (all_tiles <= share) return;                 // (a block had them all.  The rows of a thread block are of one tile, so all its threads leave.)
+    join_row<HD>(c, part, seq, kvh, r, state, HD + 4, min(n_splits, max(1, (all_tiles + share - 1) / share)), 0, joined);
 }
 
 template <int HD, int NG, bool PLAIN>
@@ -736,8 +758,8 @@ int launch(const Call& c, const TilesPlan& p, cudaStream_t s) {
     constexpr int smem = 1024 + (kGroups + 2 * kStages) * (HD / 64) * kSub + (int)sizeof(Control);
     static std::atomic<uint64_t> asked{0};
     if (int rc = allow_shared(kernel, smem, asked)) return rc;
-    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows * p.splits, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, p.splits, status));
-    if (p.splits > 1) LB_CHECK_CUDA(lb_launch_overlapped(attention4_many_join_kernel<HD>, dim3((c.max_rows + 3) / 4, c.pages.n_kv_head, c.n_seq), dim3(128), 0, s, c, p.splits));
+    LB_CHECK_CUDA(lb_launch_overlapped(kernel, dim3((c.max_rows + kTileRows - 1) / kTileRows * p.splits, c.pages.n_kv_head, c.n_seq), dim3(kManyThreads), smem, s, c, p.splits, p.share, status));
+    if (p.splits > 1) LB_CHECK_CUDA(lb_launch_overlapped(attention4_many_join_kernel<HD>, dim3((c.max_rows + 3) / 4, c.pages.n_kv_head, c.n_seq), dim3(128), 0, s, c, p.splits, p.share));
     return LB_OK;
 }
 
@@ -748,12 +770,33 @@ int launch_for(const Call& c, const TilesPlan& p, cudaStream_t s) {
 
 }  // namespace
 
-TilesPlan tiles_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
-    // As many blocks as SMs, with two tiles of keys each at least.
-    const int64_t blocks = (int64_t)std::max(1, n_seq) * n_kv_head * ((max_rows + kTileRows - 1) / kTileRows);
-    TilesPlan p;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({n_sm / blocks, (int64_t)(max_keys + 2 * kBN - 1) / (2 * kBN), 32}));
-    p.states = p.splits > 1 ? (int64_t)std::max(1, n_seq) * n_kv_head * max_rows * p.splits * (head_dim + 4) * 4 : 0;
+TilesPlan tiles_plan(int n_seq, int n_kv_head, int per, int max_rows, int max_keys, int window, int head_dim, int n_sm) {
+    const int64_t units = (int64_t)std::max(1, n_seq) * n_kv_head;
+    const int tiles = (max_rows + kTileRows - 1) / kTileRows;
+    // Tiles of keys that row tile i sees at most, where the rows are those of the last of max_keys tokens.
+    auto keys_of = [&](int i) {
+        const int last = std::max(1, max_keys - (max_rows - std::min((i + 1) * kTileRows, max_rows)) / per), all = (last + kBN - 1) / kBN;
+        return window > 0 ? std::min(all, std::min(window, max_keys) / kBN + (kTileRows / per + 1) / kBN + 3) : all;
+    };
+    const int most = keys_of(tiles - 1);
+    // The time by an estimate, in microseconds: a start and an end, and what a block takes for 128 keys, little less where it has 128 rows or fewer.  Where blocks share a row tile's keys, with two tiles
+    // each at least and all of them on an SM of their own, the states are written, read and joined.  (32 heads over 8 of 128, 64 tokens behind 16,384 keys: 134 us, shared 53.
+    // 2 x 1,024 tokens, 12 heads of 64: 28.5 us; shared by 2, 33.8, as many rows' states take longer than the keys they save.)
+    const double each = max_rows <= kBM ? (head_dim == 128 ? 2.5 : 1.9) : head_dim == 128 ? 2.9 : 2.6;
+    TilesPlan p = {1, most, 0, 9.0 + std::ceil((double)(units * tiles) / n_sm) * most * each};
+    const int first = units * tiles <= n_sm ? (int)std::min<int64_t>({2 * n_sm / (units * tiles) + 1, (most + 1) / 2, 32}) : 1;
+    for (int s = first; s > 1; --s) {
+        const int share = (most + s - 1) / s, splits = (most + share - 1) / share;
+        int64_t blocks = 0, shared = 0;
+        for (int i = 0; i < tiles; ++i) {
+            const int n = (keys_of(i) + share - 1) / share;
+            blocks += n;
+            if (n > 1) shared += (int64_t)n * std::min(kTileRows, max_rows - i * kTileRows);
+        }
+        if (blocks * units > n_sm) continue;
+        const double us = 12.0 + share * each + units * shared * (head_dim + 4) * 4 / 1.25e6;
+        if (us < p.us - 3.0) p = {splits, share, units * max_rows * splits * (head_dim + 4) * 4, us};
+    }
     return p;
 }
 

@@ -1536,7 +1536,7 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
              0 if sink is None else sink.data_ptr())
     rest = (stream_of(index), ldq, ldo, *strides, block_table.stride(0) if table_rows > 1 else table_columns, n_seq, q_shape[0], n_head, max_q_len, keys, n_mass, window, scale, soft_cap)
     l = lib()
-    sizes = (n_seq, max_q_len, n_head, keys, mass is None, rest[7])
+    sizes = (n_seq, max_q_len, n_head, keys, mass is None, rest[7], window)
     size = cache.scratch.get(sizes)
     known = size is not None
     if not known:

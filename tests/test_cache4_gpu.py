@@ -1,11 +1,14 @@
 """The 4-bit cache: its rounding, attention of single tokens and of portions over it, the weights its keys gather, and eviction by them, against plain forms in 64 bits."""
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import pytest
 import torch
 
+from liyab_b200 import ops
+from test_cache4 import AT, _call
 from test_kernels_gpu import dev  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -68,7 +71,7 @@ class Filled:
         self.lengths, self.dev, self.kv, self.dim, self.table = lengths, dev, kv, dim, self.table.to(dev)
 
 
-def _attention(q, k, v, places, scale, window=0, distance=None, sink=None, cap=0.0):
+def _attention(q, k, v, places, scale, window=0, distance=None, sink=None, cap=0.0, many=False):
     """(out [tokens, heads, dim], the weights [tokens, heads, keys], the bound on out's error before its rounding, the relative bound on the weights') in 64 bits.
     q [tokens, heads, dim]; k, v [keys, kv, dim]; places: of the tokens."""
     tokens, heads, dim = q.shape
@@ -87,6 +90,9 @@ def _attention(q, k, v, places, scale, window=0, distance=None, sink=None, cap=0
         if keys:
             large = q[:, h].double().abs().amax(1, keepdim=True)
             error = error + ((q[:, h].double().abs() < large * 2.0 ** -6).double() * large * 2.0 ** -15 @ kh.abs().T * abs(scale)).amax(1)
+        # The kernel for many rows multiplies n s (4 bits by 8) as float16, off by up to 2^-12.
+        if many:
+            error = error + 2.0 ** -12 * size
         if cap > 0:
             z = cap * torch.tanh(z / cap)
             error = error + 16 * 2.0 ** -23 * cap
@@ -374,6 +380,16 @@ def test_keys_that_are_not_finite(dev):
 
 # ---- portions ----------------------------------------------------------------------------------------------
 
+def _way(f, n, heads, most, window=0, mass=False):
+    """How the library runs such a call: (1 for the kernel for many rows, rows a tile, blocks that share keys, ..)."""
+    got = (C.c_int * 4)()
+    width, keys = heads * f.dim, f.table.shape[1] * f.cache.page_size
+    call = _call(f.cache.ref, n_head=heads, n_seq=n, n_tokens=n * most, max_keys=keys, table_stride=f.table.shape[1], q_stride=width, out_stride=width, q_start=AT, max_q_len=most, window=window,
+                 **(dict(mass=AT, total=AT) if mass else {}))
+    assert ops.lib().lb_attention4_plan(call, got) == 0
+    return tuple(got)
+
+
 def _portions(f, new, heads, seed=0, size=1.0, mass=False, max_q=None, **more):
     """prefill_attention4 beside the plain form; new[i] tokens of request i, its last ones."""
     from liyab_b200 import ops
@@ -384,13 +400,14 @@ def _portions(f, new, heads, seed=0, size=1.0, mass=False, max_q=None, **more):
     out = torch.full((sum(new) + 2, heads * f.dim), 7.5, dtype=BF16, device=f.dev)
     before = torch.rand(n, f.kv, f.table.shape[1] * f.cache.page_size, generator=torch.Generator().manual_seed(seed)).to(f.dev) if mass else None
     total = torch.full_like(before, 7.5) if mass else None
-    ops.prefill_attention4(q, f.cache, start, past, f.table, out, n, max(new) if max_q is None else max_q, heads, scale, mass=before, total=total, **more)
+    most = max(new) if max_q is None else max_q
+    ops.prefill_attention4(q, f.cache, start, past, f.table, out, n, most, heads, scale, mass=before, total=total, **more)
     plain = {k: v for k, v in more.items() if k in ("window", "distance", "sink")} | dict(cap=more.get("soft_cap", 0.0))
     token = 0
     for i in range(n):
         places = torch.arange(f.lengths[i] - new[i], f.lengths[i], device=f.dev)
         m = f.lengths[i]
-        want, weights, bound, relative = _attention(q[token:token + new[i]].view(-1, heads, f.dim), f.k[i], f.v[i], places, scale, **plain)
+        want, weights, bound, relative = _attention(q[token:token + new[i]].view(-1, heads, f.dim), f.k[i], f.v[i], places, scale, many=_way(f, n, heads, most, more.get("window", 0), mass)[0] == 1, **plain)
         _close(out[token:token + new[i]].view(-1, heads, f.dim), want, bound)
         if mass and new[i]:
             gained = weights.sum(0).view(f.kv, heads // f.kv, m).sum(1)
@@ -430,6 +447,133 @@ def test_portions_longer_than_named_are_cut(dev):
     want, _, bound, _ = _attention(q[:8].view(8, 2, 64), f.k[0], f.v[0], torch.arange(28, 36, device=dev), 0.125)
     _close(out[:8].view(8, 2, 64), want, bound)
     assert (out[8:] == 7.5).all() and not mass[0, 0, 36:].any() and abs(mass.sum().item() - 16) < 1e-3
+
+
+def _forms_of_many(dev, heads):
+    """Options beside each other, with scores that stay far below the cap and some that pass it."""
+    gen = torch.Generator().manual_seed(heads)
+    sink = torch.randn(heads, generator=gen).to(dev)
+    slopes = torch.rand(heads, generator=gen)
+    line = torch.cat([slopes * 0.1, torch.full((heads,), -1.0)]).to(dev)
+    log = torch.cat([slopes, slopes * 0.3]).to(dev)
+    return [(1.0, dict(sink=sink)), (1.0, dict(soft_cap=50.0)), (4.0, dict(soft_cap=3.0, sink=sink)), (1.0, dict(distance=line)), (1.0, dict(distance=log, sink=sink))]
+
+
+@pytest.mark.parametrize("form", range(5))
+@pytest.mark.parametrize("dim,group,heads,kv,window", [(64, 32, 8, 2, 0), (128, 64, 6, 2, 200), (128, 32, 4, 4, -96), (64, 64, 16, 1, 7)])
+def test_portions_of_many_rows_with_sinks_caps_and_distances(dev, form, dim, group, heads, kv, window):
+    size, more = _forms_of_many(dev, heads)[form]
+    f = Filled(dev, [300, 900, 129], kv, dim, group, 32, seed=form)
+    assert _way(f, 3, heads, 300, window)[0] == 1
+    _portions(f, [300, 260, 128], heads, seed=form, size=size, window=window, **more)
+
+
+@pytest.mark.parametrize("window", [0, 1000, -1024, 100, 1])
+@pytest.mark.parametrize("dim,group,heads,kv,new", [(128, 64, 8, 2, [64, 60, 9]), (64, 64, 4, 4, [150, 1, 129]), (128, 128, 16, 1, [200, 70, 0])])
+def test_portions_of_many_rows_whose_keys_blocks_share(dev, dim, group, heads, kv, new, window):
+    """One request behind many keys, and requests of all lengths beside each other: blocks of the short ones find no keys."""
+    f = Filled(dev, [6000, 90, 2000], kv, dim, group, 64, seed=window % 97)
+    assert window != 0 or (_way(f, 3, heads, max(new))[0] == 1 and _way(f, 3, heads, max(new))[2] > 1)
+    _portions(f, new, heads, window=window)
+    one = Filled(dev, [5000], kv, dim, group, 16, seed=5)
+    _portions(one, [max(new)], heads, window=window, sink=torch.randn(heads, device=dev))
+
+
+def test_portions_of_many_rows_of_any_place(dev):
+    """Rows of q and out that no wide load reaches, in the middle of wider rows; what lies between them is left alone."""
+    f = Filled(dev, [400, 300], 1, 128, 32, 16, seed=3)
+    assert _way(f, 2, 16, 300)[:3] == (1, 256, 1)
+    q = _queries(f, 600, 16, 3)
+    start, past = torch.tensor([0, 300, 600], dtype=torch.int32, device=dev), torch.tensor([100, 0], dtype=torch.int32, device=dev)
+    want = ops.prefill_attention4(q, f.cache, start, past, f.table, torch.empty_like(q), 2, 300, 16, 0.125)
+    for pad in (1, 8):
+        wide = torch.zeros(600, 2048 + 2 * pad + 1, dtype=BF16, device=dev)
+        wide[:, pad:pad + 2048] = q
+        out = torch.full((601, 2048 + 2 * pad), 7.5, dtype=BF16, device=dev)
+        ops.prefill_attention4(wide[:, pad:pad + 2048], f.cache, start, past, f.table, out[:600, pad:pad + 2048], 2, 300, 16, 0.125)
+        assert torch.equal(out[:600, pad:pad + 2048], want) and (out[:, :pad] == 7.5).all() and (out[:, pad + 2048:] == 7.5).all() and (out[600] == 7.5).all()
+
+
+def test_portions_of_many_rows_on_pages_that_are_not_there(dev):
+    """Keys on pages outside the cache are not there; a request without any has rows of zeros; a place of the batch without tokens changes nothing."""
+    f = Filled(dev, [400, 300, 260], 2, 128, 64, 16, seed=4)
+    assert _way(f, 3, 8, 400)[0] == 1
+    table = f.table.clone()
+    table[0, 3], table[0, 20], table[1, :] = -1, 1 << 29, -5
+    q, out = _queries(f, 700, 8, 1), torch.full((702, 1024), 7.5, dtype=BF16, device=dev)
+    start, past = torch.tensor([0, 400, 700, 700], dtype=torch.int32, device=dev), torch.tensor([0, 0, 260], dtype=torch.int32, device=dev)
+    ops.prefill_attention4(q, f.cache, start, past, table, out, 3, 400, 8, 0.1)
+    keys = torch.tensor([k for k in range(400) if k // 16 not in (3, 20)], device=dev)
+    k, v = f.k[0].clone(), f.v[0].clone()
+    # The plain form for each token over the keys that are there: those up to its place.
+    for place in (47, 48, 63, 64, 255, 256, 319, 340, 399):
+        there = keys[keys <= place]
+        want, _, bound, _ = _attention(q[place:place + 1].view(1, 8, 128), k[there], v[there], torch.tensor([1 << 20], device=dev), 0.1, many=True)
+        _close(out[place].view(1, 8, 128), want, bound)
+    assert not out[400:700].any() and (out[700:] == 7.5).all()
+
+
+@pytest.mark.parametrize("past", [0, 4000])
+def test_portions_of_many_rows_and_keys_that_are_not_finite(dev, past):
+    """A key with a NaN, or a value's group: the rows that see it are NaN there, and the others are as they were."""
+    f = Filled(dev, [past + 300], 2, 64, 32, 16, seed=6)
+    assert _way(f, 1, 32, 300)[0] == 1
+    q, start, n_past = _queries(f, 300, 32, 0), torch.tensor([0, 300], dtype=torch.int32, device=dev), torch.tensor([past], dtype=torch.int32, device=dev)
+    run = lambda **more: ops.prefill_attention4(q, f.cache, start, n_past, f.table, torch.empty_like(q), 1, 300, 32, 0.125, **more)  # noqa: E731
+    clean, narrow = run(), run(window=40)
+    place = past + 130
+    for which in range(2):
+        rows = [_values_as_rows(x[0][place:place + 1]) for x in (f.k, f.v)]
+        rows[which][0, 3] = math.nan
+        ops.append4(*rows, _slots(f.table.cpu(), 0, place + 1, 16)[place:].to(dev), f.cache, 1)
+        got, got_narrow = run(), run(window=40)
+        assert torch.equal(got[:130], clean[:130]) and torch.equal(got_narrow[:130], narrow[:130]) and torch.equal(got_narrow[170:], narrow[170:])
+        columns = [c for h in range(16) for c in range(64 * h, 64 * h + (64 if which == 0 else 32))]
+        others = [c for c in range(2048) if c not in columns]
+        assert got[130:, columns].isnan().all() and got_narrow[130:170, columns].isnan().all()
+        assert torch.equal(got[:, others], clean[:, others]) and torch.equal(got_narrow[:, others], narrow[:, others])
+        rows = [_values_as_rows(x[0][place:place + 1]) for x in (f.k, f.v)]
+        ops.append4(*rows, _slots(f.table.cpu(), 0, place + 1, 16)[place:].to(dev), f.cache, 1)
+    q[7] = math.nan
+    got = run()
+    assert got[7].isnan().all() and torch.equal(got[:7], clean[:7]) and torch.equal(got[8:], clean[8:])
+
+
+def _values_as_rows(x):
+    """Rows whose rounding is these values again: n s, its largest |n| being 7 (7 s / 7 is s; a bfloat16 scale of values that float32 holds exactly)."""
+    return x.reshape(1, -1).float().contiguous()
+
+
+@pytest.mark.parametrize("k_size,v_size,q_size", [(1e-3, 1e3, 1e3), (1e4, 1e-6, 1e-4), (1e-15, 1e15, 1e15), (1.0, 1e-20, 1.0), (1.0, 1e30, 1e-30), (1e30, 1.0, 1e-30)])
+def test_portions_of_many_rows_of_all_sizes(dev, k_size, v_size, q_size):
+    f = Filled(dev, [700, 300], 2, 128, 32, seed=9, k_size=k_size, v_size=v_size)
+    assert _way(f, 2, 16, 300)[0] == 1
+    _portions(f, [300, 257], 16, size=q_size)
+
+
+def test_portions_are_the_same_every_time(dev):
+    f = Filled(dev, [3000, 20, 900], 2, 128, 32, seed=4)
+    for new in ([300, 20, 257], [64, 3, 50], [2, 3, 1]):
+        assert torch.equal(_portions(f, new, 8), _portions(f, new, 8))
+
+
+def test_decode_of_more_requests_than_a_launch_row(dev):
+    """Requests of one block each and requests whose keys all warps share give what each gives alone."""
+    f = Filled(dev, [(i * 37) % 90 for i in range(290)], 1, 64, 64, seed=2)
+    ways = set()
+    for most in (0, 96, 1 << 20):
+        table = torch.nn.functional.pad(f.table, (0, 4096 if most > 96 else 0), value=-1)
+        q, positions = _queries(f, 290, 2, 0), torch.tensor([n - 1 for n in f.lengths], dtype=torch.int32, device=dev)
+        out = torch.full((290, 128), 7.5, dtype=BF16, device=dev)
+        ops.decode_attention4(q, f.cache, positions, table, out, 290, 2, 0.125, max_keys=most)
+        got = (C.c_int * 4)()
+        call = _call(f.cache.ref, n_head=2, n_seq=290, n_tokens=290, max_keys=table.shape[1] * 16 if most != 96 else 96, table_stride=table.shape[1], q_stride=128, out_stride=128)
+        assert ops.lib().lb_attention4_plan(call, got) == 0
+        ways.add(got[3] > 1)
+        for i in range(0, 290, 7):
+            want, _, bound, _ = _attention(q[i:i + 1].view(1, 2, 64), f.k[i], f.v[i], torch.tensor([f.lengths[i] - 1], device=dev), 0.125)
+            _close(out[i].view(1, 2, 64), want, bound)
+    assert ways == {False, True}
 
 
 # ---- eviction ----------------------------------------------------------------------------------------------
@@ -505,6 +649,14 @@ def test_evict_rows_of_another_order(dev):
     _evict(f, mass, 50, 10, torch.tensor([4, 1], dtype=torch.int32, device=dev))
 
 
+@pytest.mark.parametrize("keep,recent", [(1000, 10), (50000, 49990), (59999, 0)])
+def test_evict_of_more_keys_than_a_block_holds(dev, keep, recent):
+    f = Filled(dev, [60000], 1, 64, 64, 64, seed=1, extra=-(-keep // 64))
+    mass = torch.rand(1, 1, f.table.shape[1] * 64, generator=torch.Generator().manual_seed(2)).to(dev)
+    _evict(f, mass, keep, recent)
+    _evict(f, (mass * 4).floor(), keep, recent)              # equal weights on both sides of what the block holds
+
+
 # ---- together ----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("captured", [False, True])
@@ -577,3 +729,68 @@ def test_a_run_of_them_together(dev, captured):
         for i in range(2):
             assert torch.allclose(mass[i].double(), gathered[i], rtol=1e-4, atol=1e-6)
     stream.synchronize()
+
+
+def test_two_streams_and_graphs_beside_each_other(dev):
+    """Calls under way on two streams at once, eager ones and graphs' replays, with inputs that change between replays, give what they give alone."""
+    kv, heads, dim = 2, 8, 128
+    f = Filled(dev, [4000, 100, 1500], kv, dim, 64, 16, seed=8, extra=120)
+    mass = torch.rand(3, kv, f.table.shape[1] * 16, generator=torch.Generator().manual_seed(3)).to(dev)
+    n_keys = torch.tensor(f.lengths, dtype=torch.int32, device=dev)
+    dest = f.spare[:60].view(3, 20).to(dev)
+    dest2 = f.spare[60:120].view(3, 20).to(dev)
+    positions = n_keys - 1
+    new = [200, 64, 130]
+    start = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(dev)
+    past = n_keys - torch.tensor(new, dtype=torch.int32, device=dev)
+
+    class Work:
+        def __init__(self, dest):
+            self.q, self.p = torch.empty(3, heads * dim, dtype=BF16, device=dev), torch.empty(sum(new), heads * dim, dtype=BF16, device=dev)
+            self.out, self.outp, self.total = torch.empty_like(self.q), torch.empty_like(self.p), torch.zeros_like(mass)          # (behind the newest key nothing is written)
+            self.kept, self.dest = torch.empty(3, kv, 320, dtype=torch.int32, device=dev), dest
+            self.few = torch.empty(9, heads * dim, dtype=BF16, device=dev)
+
+        def load(self, seed):
+            gen = torch.Generator().manual_seed(seed)
+            for t in (self.q, self.p):
+                t.copy_(torch.randn(t.shape, generator=gen).to(BF16))
+
+        def run(self):
+            ops.decode_attention4(self.q, f.cache, positions, f.table, self.out, 3, heads, 0.09, mass=mass, total=self.total)
+            ops.prefill_attention4(self.p, f.cache, start, past, f.table, self.outp, 3, 200, heads, 0.09)
+            ops.prefill_attention4(self.p[:9], f.cache, self.three, n_keys - 3, f.table, self.few, 3, 3, heads, 0.09)
+            ops.evict4(f.cache, self.total, f.table, n_keys, 3, 320, 20, self.dest, self.kept)
+
+        three = torch.tensor([0, 3, 6, 9], dtype=torch.int32, device=dev)
+
+        def results(self):
+            return [t.clone() for t in (self.out, self.outp, self.total, self.kept, self.few)]
+
+    a, b = Work(dest), Work(dest2)
+    want = {}
+    for seed in range(4):
+        a.load(seed)
+        a.run()
+        want[seed] = a.results()
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for w, s in zip((a, b), streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            w.run()
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for first, second in ((0, 1), (2, 3), (1, 1)):
+        for replayed in (True, False):
+            for w, seed in ((a, first), (b, second)):
+                w.load(seed)
+            torch.cuda.synchronize()
+            for _ in range(5):
+                for w, s, g in zip((a, b), streams, graphs):
+                    with torch.cuda.stream(s):
+                        g.replay() if replayed else w.run()
+            torch.cuda.synchronize()
+            for w, seed in ((a, first), (b, second)):
+                assert all(torch.equal(x, y) for x, y in zip(w.results(), want[seed]))
+    del graphs
