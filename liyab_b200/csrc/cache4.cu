@@ -300,11 +300,13 @@ struct Choice {
     int keep, recent, max_keys, n_mass, n_dest_mass;
 };
 
+// (1,024 threads also for few keys: 1 request of 2,048, 12 heads, 14.9 us in all; with 512 16.6, with 256 23.2, as the passes wait for shared memory.)
 __global__ void __launch_bounds__(kChoiceThreads)
 evict4_choose_kernel(const Choice c, int held) {
+    constexpr int THREADS = kChoiceThreads, kOwn = kBins / THREADS;
     extern __shared__ uint32_t keys_s[];       // the first `held` keys' weights as ordered integers
-    __shared__ uint32_t bins[kBins];
-    __shared__ uint32_t sums[32];
+    __shared__ __align__(16) uint32_t bins[kBins];
+    __shared__ uint32_t sums[THREADS / 32];
     __shared__ uint32_t found[2];              // the bin that holds the last key to stay, and how many of it stay
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
@@ -317,54 +319,75 @@ evict4_choose_kernel(const Choice c, int held) {
     float* dest = c.dest_mass != nullptr && (unsigned)r < (unsigned)c.n_dest_mass ? c.dest_mass + (int64_t)r * c.dest_stride + (int64_t)head * c.dest_head_stride : nullptr;
     const int stay = min(n, c.keep), old = n - min(c.recent, n);
     const int by_weight = stay - (n - old);           // of the `old` first keys; recent <= keep, so never negative
-    for (int i0 = threadIdx.x; i0 < min(old, held); i0 += 4 * kChoiceThreads) {
+    for (int i0 = threadIdx.x; i0 < min(old, held); i0 += 4 * THREADS) {
         float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = weighed && i0 + j * kChoiceThreads < old ? mass[i0 + j * kChoiceThreads] : 0.0f;
+        for (int j = 0; j < 4; ++j) v[j] = weighed && i0 + j * THREADS < old ? mass[i0 + j * THREADS] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i0 + j * kChoiceThreads < min(old, held)) keys_s[i0 + j * kChoiceThreads] = ordered(v[j]);
+            if (i0 + j * THREADS < min(old, held)) keys_s[i0 + j * THREADS] = ordered(v[j]);
     }
     __syncthreads();
     auto key_at = [&](int i) { return i < held ? keys_s[i] : weighed ? ordered(mass[i]) : 0x80000000u; };
     // The sum of what the warps before this one left.
     auto before = [&](const uint32_t* of_warps) { return __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[lane] : 0u); };
-    // The by_weight-th largest key among the first `old`: `above` its prefix so far, `left` how many keys with that prefix stay.
+    // The by_weight-th largest key among the first `old`: `threshold` its prefix so far, `left` how many keys with that prefix stay.
     uint32_t threshold = 0, left = (uint32_t)by_weight;
     if (by_weight < old && by_weight > 0) {
         int low = 32;
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int bits = pass < 2 ? 11 : 10, high = low;
             low -= bits;
-            for (int i = threadIdx.x; i < kBins; i += kChoiceThreads) bins[i] = 0;
+            const uint32_t mask = (1u << bits) - 1u, prefix = pass == 0 ? 0u : threshold >> high;
+            for (int i = 4 * threadIdx.x; i < kBins; i += 4 * THREADS) *reinterpret_cast<uint4*>(bins + i) = make_uint4(0, 0, 0, 0);
             __syncthreads();
-            for (int i0 = 0; i0 < old; i0 += kChoiceThreads) {
-                const int i = i0 + threadIdx.x;
-                const uint32_t key = i < old ? key_at(i) : 0u;
-                const bool counts = i < old && (pass == 0 || key >> high == threshold >> high);
-                // Many weights are 0: the warp's enter with one addition.
-                const uint32_t zeros = __ballot_sync(0xffffffffu, counts && key == 0x80000000u);
-                if (counts && key != 0x80000000u) atomicAdd(&bins[key >> low & ((1u << bits) - 1u)], 1u);
-                if (zeros != 0 && lane == 0) atomicAdd(&bins[0x80000000u >> low & ((1u << bits) - 1u)], (uint32_t)__popc(zeros));
+            // Many weights are 0: they are counted in a register and enter with one addition a warp.
+            uint32_t zeros = 0;
+            auto enter = [&](uint32_t key) {
+                if (pass != 0 && key >> high != prefix) return;
+                if (key == 0x80000000u) ++zeros;
+                else atomicAdd(&bins[key >> low & mask], 1u);
+            };
+            int i = threadIdx.x;
+            const int in_shared = min(old, held);
+            for (; i + 3 * THREADS < in_shared; i += 4 * THREADS) {
+                uint32_t key[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) key[j] = keys_s[i + j * THREADS];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) enter(key[j]);
             }
+            for (; i < old; i += THREADS) enter(key_at(i));
+            zeros = __reduce_add_sync(0xffffffffu, zeros);
+            if (zeros != 0 && lane == 0) atomicAdd(&bins[0x80000000u >> low & mask], zeros);
             __syncthreads();
-            // Two bins a thread, from the largest down: how many keys lie in larger bins.
-            const int top = kBins - 1 - 2 * threadIdx.x;
-            const uint32_t b0 = bins[top], b1 = bins[top - 1];
-            uint32_t sum = b0 + b1;
+            // A few neighbouring bins a thread, from the largest down: how many keys lie in larger bins.
+            const int top = kBins - 1 - kOwn * threadIdx.x;
+            uint32_t own[kOwn], sum = 0;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+                own[j] = bins[top - j];
+                sum += own[j];
+            }
+            uint32_t larger = sum;
+#pragma unroll
             for (int o = 1; o < 32; o *= 2) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += v;
+                const uint32_t v = __shfl_up_sync(0xffffffffu, larger, o);
+                if (lane >= o) larger += v;
             }
-            if (lane == 31) sums[warp] = sum;
+            if (lane == 31) sums[warp] = larger;
             __syncthreads();
-            const uint32_t larger = sum - b0 - b1 + before(sums);
-            if (larger < left && left <= larger + b0) {
-                found[0] = (uint32_t)top;
-                found[1] = left - larger;
-            } else if (larger + b0 < left && left <= larger + b0 + b1) {
-                found[0] = (uint32_t)(top - 1);
-                found[1] = left - larger - b0;
+            larger += before(sums) - sum;
+            if (larger < left && left <= larger + sum) {
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) {
+                    if (larger < left && left <= larger + own[j]) {
+                        found[0] = (uint32_t)(top - j);
+                        found[1] = left - larger;
+                    }
+                    larger += own[j];
+                }
             }
             __syncthreads();
             threshold |= found[0] << low;
@@ -377,7 +400,7 @@ evict4_choose_kernel(const Choice c, int held) {
         left = 0xffffffffu;            // all do
     }
     // A warp has a stretch of the keys: it counts those above the threshold and those at it, the warps' counts meet, and it writes its own.
-    const int stretch = (old + 32 * 32 - 1) / (32 * 32) * 32, from = min(old, warp * stretch), to = min(old, from + stretch);
+    const int stretch = (old + THREADS - 1) / THREADS * 32, from = min(old, warp * stretch), to = min(old, from + stretch);
     uint32_t above = 0, at = 0;
     for (int i = from + lane; i < to; i += 32) {
         const uint32_t key = key_at(i);
@@ -410,7 +433,7 @@ evict4_choose_kernel(const Choice c, int held) {
         place += __popc(mask);
         ties += __popc(tie_mask);
     }
-    for (int i = max(by_weight, 0) + threadIdx.x; i < c.keep; i += kChoiceThreads) {
+    for (int i = max(by_weight, 0) + threadIdx.x; i < c.keep; i += THREADS) {
         const int key = old + i - max(by_weight, 0);
         const bool there = i < stay;
         kept[i] = there ? key : -1;
@@ -448,28 +471,43 @@ evict4_copy_kernel(const Pages pages, const int32_t* __restrict__ table, int tab
         *place = __shfl_sync(0xffffffffu, key_from, key);
         return at < 0 ? nullptr : pages.memory + at;
     };
+    // A lane's pieces: K of the keys g and g + 8, V of every fourth key (eight lanes each), the scales of a key's K or V.  All are on their way before the first is stored.
+    Piece k[2];
+    Half v[4];
+    uint16_t scale[4];
+    bool there[6], scaled;
+    const int of = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {                     // K: a lane's pieces of keys g and g + 8
-        const int key = 8 * i + (lane >> 2);
+    for (int i = 0; i < 2; ++i) {
         int place;
-        const uint8_t* block = source_of(key, &place);
-        if (block != nullptr) *reinterpret_cast<Piece*>(dest + L::k_word(key, lane & 3)) = *reinterpret_cast<const Piece*>(block + L::k_word(place, lane & 3));
+        const uint8_t* block = source_of(8 * i + (lane >> 2), &place);
+        there[i] = block != nullptr;
+        if (there[i]) k[i] = *reinterpret_cast<const Piece*>(block + L::k_word(place, lane & 3));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                     // V: four keys, eight pieces each
-        const int key = 4 * i + (lane >> 3), g = lane & 7;
+    for (int i = 0; i < 4; ++i) {
         int place;
-        const uint8_t* block = source_of(key, &place);
-        if (block != nullptr) *reinterpret_cast<Half*>(dest + L::v_word(key, g, 0)) = *reinterpret_cast<const Half*>(block + L::v_word(place, g, 0));
+        const uint8_t* block = source_of(4 * i + (lane >> 3), &place);
+        there[2 + i] = block != nullptr;
+        if (there[2 + i]) v[i] = *reinterpret_cast<const Half*>(block + L::v_word(place, lane & 7, 0));
     }
     {
-        const int key = lane & 15, of = lane >> 4;
         int place;
-        const uint8_t* block = source_of(key, &place);
-        if (block != nullptr)
-            for (int s = 0; s < pages.groups; ++s)
-                reinterpret_cast<uint16_t*>(dest + L::scale(key, pages.groups, of))[s] = reinterpret_cast<const uint16_t*>(block + L::scale(place, pages.groups, of))[s];
+        const uint8_t* block = source_of(lane & 15, &place);
+        scaled = block != nullptr;
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s)
+            if (scaled && s < pages.groups) scale[s] = reinterpret_cast<const uint16_t*>(block + L::scale(place, pages.groups, of))[s];
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (there[i]) *reinterpret_cast<Piece*>(dest + L::k_word(8 * i + (lane >> 2), lane & 3)) = k[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (there[2 + i]) *reinterpret_cast<Half*>(dest + L::v_word(4 * i + (lane >> 3), lane & 7, 0)) = v[i];
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s)
+        if (scaled && s < pages.groups) reinterpret_cast<uint16_t*>(dest + L::scale(lane & 15, pages.groups, of))[s] = scale[s];
 }
 
 bool wide_rows(const void* p, int64_t ld, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; }
