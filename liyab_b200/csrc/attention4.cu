@@ -94,7 +94,9 @@ int check(const lb_attention4_args* args, Call* c, Plan* p) {
     // What lies in the scratch memory: scores and divisors for the keys' weights, states, where requests' tiles start.
     auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
     const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
-    if (int rc = rows_plan(&p->rows, a.n_seq, a.cache->n_kv_head, (int)rows, keys, a.cache->head_dim, n_sm)) return rc;
+    // (Under a window a request's rows see no more keys than it and the portion have, and what rounds them to tiles.)
+    const int seen = a.window == 0 ? keys : (int)std::min<int64_t>(keys, std::abs((int64_t)a.window) + a.max_q_len + 2 * lb_c4::kBlockKeys);
+    if (int rc = rows_plan(&p->rows, a.n_seq, a.cache->n_kv_head, (int)rows, seen, a.cache->head_dim, n_sm)) return rc;
     p->tiles = tiles_plan(a.n_seq, a.cache->n_kv_head, c->per, (int)rows, keys, a.window, a.cache->head_dim, n_sm);
     // The tcgen05 kernel takes a call where the estimates (rows_plan, tiles_plan), which are from both kernels' times on 84 calls of 1 to 128 tokens a request, say so: 8 requests on 2,048 keys, 32 heads
     // over 8: 8 tokens each 34 us on the kernel for few rows, 36 on this; 16 tokens 52 / 36; 1 request on 2,048 keys: 32 tokens 20 / 24, 128 tokens 51 / 32.

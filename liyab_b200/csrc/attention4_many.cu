@@ -776,7 +776,7 @@ TilesPlan tiles_plan(int n_seq, int n_kv_head, int per, int max_rows, int max_ke
     // Tiles of keys that row tile i sees at most, where the rows are those of the last of max_keys tokens.
     auto keys_of = [&](int i) {
         const int last = std::max(1, max_keys - (max_rows - std::min((i + 1) * kTileRows, max_rows)) / per), all = (last + kBN - 1) / kBN;
-        return window > 0 ? std::min(all, std::min(window, max_keys) / kBN + (kTileRows / per + 1) / kBN + 3) : all;
+        return window != 0 ? std::min(all, (int)std::min<int64_t>(std::abs((int64_t)window), max_keys) / kBN + (kTileRows / per + 1) / kBN + 3) : all;
     };
     const int most = keys_of(tiles - 1);
     // The time by an estimate, in microseconds: a start and an end, and what a block takes for 128 keys, little less where it has 128 rows or fewer.  Where blocks share a row tile's keys, with two tiles
