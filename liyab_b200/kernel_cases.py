@@ -11,6 +11,7 @@
     python -m liyab_b200.kernel_cases norm-join --rows 2048 --width 768 --experts 16
     python -m liyab_b200.kernel_cases streams --rows 2048 --streams 2 --width 768 --experts 20
     python -m liyab_b200.kernel_cases weights4 --rows 1 --width 4096 --inner 10240 [--e4m3]
+    python -m liyab_b200.kernel_cases cache4 --batch 8 --context 8192 --heads 32 --kv 8 --dim 128 --new 512
 
 Each prints one line with the CUDA-event time per repetition and the achieved rate.  The cases are what the
 ncu summaries under profiles/ were captured on (one kernel, a few launches, inputs of a few hundred MB at most).
@@ -362,6 +363,55 @@ def case_weights4(args) -> None:
           f"bfloat16 {us16:.1f} us, {sum(2 * w.numel() for w in plain) / 1e6:.0f} MB; what the sublayers add differs by {100 * apart:.1f} %")
 
 
+def case_cache4(args) -> None:
+    """A 4-bit cache's calls as serving makes them: a step's rows go in, its tokens attend (with and without the keys' weights), a portion of a prompt does, and the keys that gained least
+    are dropped.  Beside them the same tokens and portion over a bfloat16 cache, and how far the tokens' results are apart."""
+    from . import ops
+    dev, B, C, H, KV, D, N = torch.device("cuda:0"), args.batch, args.context, args.heads, args.kv, args.dim, min(args.new, args.context)
+    gen = torch.Generator(device=dev).manual_seed(0)
+    r = lambda *shape: torch.randn(*shape, device=dev, generator=gen).bfloat16()
+    page, scale, keep = 16, D ** -0.5, max(1, C // 2)
+    per, kept_pages = -(-C // page), -(-keep // page)
+    table = torch.randperm(B * per, device=dev, generator=gen).to(torch.int32).view(B, per)
+    cache = ops.Cache4(B * (per + kept_pages), KV, D, page, args.group)
+    dest = torch.arange(B * per, B * (per + kept_pages), dtype=torch.int32, device=dev).view(B, kept_pages)
+    plain = torch.empty(B * per, 2, KV, page, D, dtype=torch.bfloat16, device=dev)
+    key = torch.arange(C, device=dev)
+    for i in range(B):
+        k, v = r(C, KV * D), r(C, KV * D)
+        ops.append4(k, v, (table[i, key // page] * page + key % page).to(torch.int32), cache, C)
+        for of, x in enumerate((k, v)):
+            rows = torch.zeros(per * page, KV, D, dtype=torch.bfloat16, device=dev)
+            rows[:C] = x.view(C, KV, D)
+            plain[table[i].long(), of] = rows.view(per, page, KV, D).transpose(1, 2)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    k1, v1, q1, qn = r(B, KV * D), r(B, KV * D), r(B, H * D), r(B * N, H * D)
+    o1, o16, on = torch.empty_like(q1), torch.empty_like(q1), torch.empty_like(qn)
+    slots, last, n_keys, start, past = table[:, -1] * page + (C - 1) % page, i32([C - 1] * B), i32([C] * B), i32([N * i for i in range(B + 1)]), i32([C - N] * B)
+    mass = torch.zeros(B, KV, per * page, device=dev)
+    total, kept = torch.zeros_like(mass), torch.empty(B, KV, keep, dtype=torch.int32, device=dev)
+    splits = ops.decode_splits(B, KV, C, tensor_cores=True)
+    partial, counters = torch.empty(B * H * splits * (D + 2), device=dev), torch.zeros(B * H, dtype=torch.int32, device=dev)
+
+    def tokens16():
+        ops.decode_attention(q1, plain, last, table, o16, partial, counters, B, H, KV, D, page, scale, 0, splits)
+
+    us = lambda fn: 1e3 * _graph_timed(fn, args.reps)
+    ops.decode_attention4(q1, cache, last, table, o1, B, H, scale, mass=mass, total=total)
+    line = {"tokens": us(lambda: ops.decode_attention4(q1, cache, last, table, o1, B, H, scale)),
+            "with weights": us(lambda: ops.decode_attention4(q1, cache, last, table, o1, B, H, scale, mass=mass, total=total)),
+            f"portions of {N}": us(lambda: ops.prefill_attention4(qn, cache, start, past, table, on, B, N, H, scale)),
+            f"{keep} keys kept": us(lambda: ops.evict4(cache, total, table, n_keys, B, keep, min(keep, 32), dest, kept))}
+    if ops.decode_attention_supports(H, KV, D, page):
+        line["tokens over bfloat16"] = us(tokens16)
+    if ops.prefill_attention_supports(H, KV, D, page):
+        line["portions over bfloat16"] = us(lambda: ops.prefill_attention(qn, plain, start, past, table, on, B, N, H, KV, D, page, scale))
+    apart = f"; tokens' results differ by {100 * ((o1.float() - o16.float()).norm() / o16.float().norm()).item():.1f} %" if "tokens over bfloat16" in line else ""
+    line["rows in"] = us(lambda: ops.append4(k1, v1, slots, cache, B))
+    print(f"cache4 {B} x {C} keys, {H} heads over {KV} of {D}, groups of {args.group}: {', '.join(f'{k} {v:.1f} us' for k, v in line.items())}; "
+          f"{B * per * page * KV * (D + 4 * D // args.group) / 1e6:.0f} MB of keys and values, bfloat16 {2 * plain.numel() / 1e6:.0f}{apart}")
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m liyab_b200.kernel_cases")
     sub = ap.add_subparsers(dest="case", required=True)
@@ -448,6 +498,15 @@ def main(argv=None) -> int:
     w4.add_argument("--group", type=int, default=128, choices=[32, 64, 128])
     w4.add_argument("--e4m3", action="store_true", help="the norms leave e4m3 rows with a scale each")
     w4.add_argument("--reps", type=int, default=200)
+    c4 = sub.add_parser("cache4")
+    c4.add_argument("--batch", type=int, default=8)
+    c4.add_argument("--context", type=int, default=8192)
+    c4.add_argument("--heads", type=int, default=32)
+    c4.add_argument("--kv", type=int, default=8)
+    c4.add_argument("--dim", type=int, default=128, choices=[64, 128])
+    c4.add_argument("--group", type=int, default=64, choices=[32, 64, 128])
+    c4.add_argument("--new", type=int, default=512, help="tokens of a portion")
+    c4.add_argument("--reps", type=int, default=100)
     for name in ("decode-step", "prefill-step"):
         p = sub.add_parser(name)
         p.add_argument("--batch", type=int, default=8)
@@ -463,7 +522,7 @@ def main(argv=None) -> int:
         p.add_argument("--stamps", action="store_true", help="decode-step: per-phase times from inside the one-kernel step")
     args = ap.parse_args(argv)
     {"gemm": case_gemm, "generic-attention": case_generic_attention, "gemm-f32": case_gemm_f32, "decode-attention": case_decode_attention, "prefill-attention": case_prefill_attention, "sample": case_sample, "decode-step": case_decode_step,
-     "prefill-step": case_prefill_step, "channel-memory": case_channel_memory, "streams": case_streams, "norm-join": case_norm_join, "weights4": case_weights4}[args.case](args)
+     "prefill-step": case_prefill_step, "channel-memory": case_channel_memory, "streams": case_streams, "norm-join": case_norm_join, "weights4": case_weights4, "cache4": case_cache4}[args.case](args)
     return 0
 
 
