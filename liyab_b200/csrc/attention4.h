@@ -24,6 +24,7 @@ struct Call {
     int64_t q_stride, out_stride;
     int table_stride, n_seq, n_tokens, n_head, per, max_rows, score_keys, max_keys, window;
     float scale, soft_cap;
+    int withhold;                   // a test's launch, in which what the kernels wait for does not come
 };
 
 // The tokens of request s, [first, first + count), and the place of its first: decode calls have a token a request.

@@ -12,6 +12,11 @@
 // multiplied by again (for p relative to the largest block's so far, F, which O is in units of).  So K, V and p are rounded to float16 (2^-12), and bfloat16's range is kept.
 // A value scale that is NaN would meet p = 0 of rows that do not see its key in the products: such groups are made zeros, and the rows that see them take a note (a bit a group) and end as NaN.
 // Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results.
+// What bounds it.  A block alone on an SM (204 KB) gets through 256 rows by 64 keys in 1.46 us for heads of 128 (838 TFLOP/s over 148 SMs; 0.51 of cuBLAS's burst) and 1.30 for heads of 64 (469): its
+// schedulers issue in 71 % of all cycles, exponentials, conversions and the largest score of a row above all (16 softmax warps), the makers' nibbles after them.  Leaving the makers' work out, or the
+// exponentials, saved less than a tenth, as did turns that keep the groups half a unit apart: no one part is the bound.  A soft cap adds 36 % (4 x 512 tokens behind 8,192 keys, 32 heads over 8 of 128,
+// capped: 514 us; the tangent by its series of four terms in scores of their own scale 583).  With one thread a row and the products of all groups issued by one warp 742, as a row's maximum, exponentials and sum are
+// twice as long a chain.  A block takes 9 us to start (queries, first keys, tensor memory) and end; 2 x 1,024 tokens, 12 heads of 64: 28 us, of which 16 units of keys are 20.
 #include "attention4.h"
 #include "attention4_join.cuh"
 #include "tcgen05.cuh"
@@ -321,7 +326,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
 #pragma unroll
                     for (int i = 0; i < HD / kUmmaK; ++i)
                         umma_bf16(s_at + (u & 1) * kUnit, dq + (uint64_t)(((i / 4) * kSub + i % 4 * 32) >> 4), db + (uint64_t)(((i / 4) * kSub + i % 4 * 32) >> 4), idesc_s, i != 0 ? 1u : 0u);
-                    umma_commit(&ctl->s_full[g][u & 1]);
+                    if (c.withhold == 0) umma_commit(&ctl->s_full[g][u & 1]);
                 }
                 __syncwarp();
             }
@@ -734,7 +739,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
     }
 }
 
-// The states of blocks that share a row's keys.
+// The states of blocks that share a row's keys, a warp a row: bound by their bytes and by two trips to memory.
 template <int HD>
 __global__ void __launch_bounds__(128)
 attention4_many_join_kernel(const Call c, int n_splits, int share) {
@@ -781,7 +786,7 @@ TilesPlan tiles_plan(int n_seq, int n_kv_head, int per, int max_rows, int max_ke
     const int most = keys_of(tiles - 1);
     // The time by an estimate, in microseconds: a start and an end, and what a block takes for 128 keys, little less where it has 128 rows or fewer.  Where blocks share a row tile's keys, with two tiles
     // each at least and all of them on an SM of their own, the states are written, read and joined.  (32 heads over 8 of 128, 64 tokens behind 16,384 keys: 134 us, shared 53.
-    // 2 x 1,024 tokens, 12 heads of 64: 28.5 us; shared by 2, 33.8, as many rows' states take longer than the keys they save.)
+    // 2 x 1,024 tokens, 12 heads of 64: 28.4 us; shared by 2, 33.8, as many rows' states take longer than the keys they save.)
     const double each = max_rows <= kBM ? (head_dim == 128 ? 2.5 : 1.9) : head_dim == 128 ? 2.9 : 2.6;
     TilesPlan p = {1, most, 0, 9.0 + std::ceil((double)(units * tiles) / n_sm) * most * each};
     const int first = units * tiles <= n_sm ? (int)std::min<int64_t>({2 * n_sm / (units * tiles) + 1, (most + 1) / 2, 32}) : 1;

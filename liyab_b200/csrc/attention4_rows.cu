@@ -1,17 +1,27 @@
 // Attention over a 4-bit cache for few query rows: single tokens, drafts of a few, the last tokens of a prompt.
 //
-// The query rows of a request that share a key/value head (its tokens' heads, in the order of the tokens) are cut into tiles of 8 or 16.  A block serves (key range,
-// key/value head and row tile, request); its warps take the range's blocks of sixteen keys in turn, each fetched by one bulk copy into a ring of the warp's own.  A
-// lane finds its values there in the order of the operands (cache4.cuh) and makes float16 numbers of the nibbles: w & 0x000f000f | 0x6400 6400 is 1024 + n of two
-// values, which less 1032 is n - 8, exactly.  Then
-//   S^T = K q^T      mma.sync m16n8k16, rows are keys, columns query rows: sums over a group of the scales, each met by its key's scale in 32 bits;
+// The query rows of a request that share a key/value head (its tokens' heads, in the order of the tokens) are cut into tiles of 4 or 8.  A warp takes blocks of sixteen keys in pairs, each
+// block fetched by one bulk copy into a ring of the warp's own.  A lane finds its values there in the order of the operands (cache4.cuh).  Then
+//   S^T = K q^T      mma.sync m16n8k32 on bytes: the first operand is n + 8 as it lies (a mask, a shift), the second a row of queries as whole numbers of 16 bits in two digits, so a
+//                    column is a row's digit.  The sums start at -8 times the digits' sum and at the bits of a float, so that two subtractions and a multiply-add make the number; each group's
+//                    meets its key's scale in 32 bits;
 //   p = 2^(S - m)    m a row's reference in 32 bits;
-//   O^T += V^T p^T   rows are dims; p times the value's scale, rounded to float16, turned by movmatrix into the second operand, one such for each group.
-// So the numbers that are multiplied are exact but for p s (2^-12, or 2^-31 of the warp's largest value scale) and queries far below their row's largest (below 2^-29 of it).  The queries come as bfloat16 and become float16
-// after a power of two a row that puts their largest at 2^14; the values' scales have any size that bfloat16 has, so m is the row's largest score plus the exponent of the warp's
-// largest value scale f (down to 2^-80), less 6: 2^(S - m) s is at most 2^14.  Everything is relative to m, so f leaves no trace in the result.  m moves when a score passes it by more than
-// 2^8, or a scale f: the warp votes, which costs a few instructions a tile where searching the maximum cost thirty.
-// The warps' states meet in shared memory in their order, the ranges' in the shared memory of a cluster (up to 16), or in memory in another launch.
+//   O^T += V^T p^T   mma.sync m16n8k16 on float16: rows are dims, n - 8 made of the nibbles exactly (w & 0x000f000f | 0x64006400 is 1024 + n of two values, less 1032); p times the value's
+//                    scale, rounded to float16, turned by movmatrix into the second operand.
+// What is rounded: p s to float16 (2^-12, or 2^-31 of the warp's largest value scale), and queries more than 2^6 below their row's largest (to 2^-15 of it); a row's 16 bits hold bfloat16's
+// eight of all others.  A power of two a row puts its largest at 2^14.  The values' scales have any size that bfloat16 has, so what p is relative to is the row's largest score plus the exponent
+// of the warp's largest value scale f (down to 2^-80), less 6: 2^(S - m) s is at most 2^14.  f leaves no trace in the result.  m moves when a score passes it by more than 2^8, or a scale f: the warp
+// votes, which costs a few instructions a pair where searching the maximum cost thirty a tile.
+//
+// Two ways to share the keys out (rows_plan chooses by an estimate of both).  WHOLE: a block has a request's row tile and key/value head, its eight warps a stretch of the keys each, whose states meet
+// in shared memory and become the result: no scratch memory, one launch.  Else all warps of the launch take equal shares of all tiles of all requests (256 at most to a launch row), wherever they
+// begin and end, and another launch joins the states of a row's runs in their order.
+//
+// What bounds it.  A block of sixteen keys takes some 257 instructions for heads of 128 with four rows, most of them on the pipe for integers and halves at two cycles each, so the GPU gets through
+// 5.1 TB/s of cache (heads of 64: 4.3), 0.78 of the copy bandwidth, after a start of 8 us (requests, block tables, first keys, queries: four trips to memory, and the launch)
+// and before a join of 3.  8 requests on 16,384 keys, 32 heads over 8 of 128: 38 us, 3.75 TB/s; 64 on 1,024, 25 heads of 64: 31 us; 1 on 131,072: 39; 1 on 512, 25 heads of 64: 5.3.
+// Float16 products for K as well, a tile at a time, took 67 us for the first, with a block to a range of one request's keys.  Five blocks of four warps an SM for heads of 64, not four: 34.8 us for the
+// second against 32.0; twice the blocks for the third 47 against 38.7; tiles of sixteen rows lose to two of eight, as their registers leave half the warps; a third pair in the ring changes nothing.
 #include "attention4.h"
 #include "attention4_join.cuh"
 #include "tcgen05.cuh"
@@ -227,7 +237,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             listed += 32;
             __syncwarp();
         }
-        if (lane < 2) {
+        if (lane < 2 - c.withhold) {
             const int stage = asked % kStages, at = found[warp][(2 * asked + lane) & 63];
             if (at >= 0) {
                 lb_tc::mbar_expect_tx(&bars[warp][stage], kBlock);
@@ -641,8 +651,8 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
     // Which way: by an estimate of both in microseconds, from 150 calls of 1 to 64 requests on 64 to 8,192 keys (25 heads of 64; 32 over 8, and over 4, of 128).  Blocks that have a row tile's keys to
-    // themselves: a start and an end for each wave of them, and the keys, which all SMs' blocks read side by side (1 request, 25 heads, 512 keys 5.9 us, the other way 8.6; 64 requests, 8 heads, 4,096 keys
-    // 68 / 79).  Warps that share all tiles: a start, a join, and the tiles of a warp (1 request, 8 heads, 8,192 keys 39 / 13; 16 requests 42 / 40).
+    // themselves: a start and an end for each wave of them, and the keys, which all SMs' blocks read side by side (1 request, 25 heads of 64, 512 keys 5.9 us, the other way 8.6; 16 requests, 8 heads,
+    // 2,048 keys 13.5 / 20).  Warps that share all tiles: a start, a join, and the tiles of a warp (1 request, 8 heads, 8,192 keys 39 / 13; 16 requests 42 / 40).
     const bool wide = head_dim == 128, two = p.rows == 8;
     const double all = (double)units * n_seq, thousands = max_keys / 1024.0;
     const double waves = std::ceil(all / (n_sm * blocks_per_sm(head_dim, p.rows / 4, true)));

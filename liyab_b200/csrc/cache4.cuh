@@ -2,9 +2,10 @@
 //
 // A page is, for each key/value head, page_size / 16 blocks of sixteen neighbouring keys.  A block is one run of memory, so that one bulk copy fetches a tile of keys
 // with their values and scales: [K nibbles 8 hd bytes][V nibbles 8 hd][K scales][V scales], scales bfloat16, hd / group a row.  The order inside a block is that of the
-// operands of mma.sync m16n8k16, so that a lane (g = lane / 4, t = lane % 4) finds its values of a tile in 16-byte pieces (8 for heads of 64) without bank conflicts:
-//   K, the first operand of K q^T (rows are keys): lane (g, t) has of the keys g and g + 8 the words t, 4 + t, ..: dims 8 w .. 8 w + 7, so that the dims of one product all
-//      lie in the same 32, one group of the scales.  Dim 8 w + d is nibble d / 2 + 4 (d % 2) of its word: a shift and a mask give two neighbours in the halves of a register.
+// operands of mma.sync (m16n8k32 on bytes for the keys, m16n8k16 on halves for the values), so that a lane (g = lane / 4, t = lane % 4) finds its values of a tile in 16-byte pieces (8 for heads of 64) without bank conflicts:
+//   K, the first operand of K q^T (rows are keys): lane (g, t) has of the keys g and g + 8 the words t, 4 + t, ..: dims 8 w .. 8 w + 7, so that the dims of one product
+//      are the same 32, one group of the scales.  Dim 8 w + d is nibble d / 2 + 4 (d % 2) of its word: a mask gives four of them in the bytes of a register, a shift and a mask two neighbours in
+//      its halves.
 //   V, the first operand of V^T p^T (rows are dims): lane (g, t) has of the keys 2 t, 2 t + 1 (and of those plus 8) the words (g, j): nibble n is dim
 //      64 j + 32 (n % 4 / 2) + 4 g + 2 (n % 2) + n / 4, so that the sixteen dims of one product lie in the same 32 as well; the low (high) halves of two keys' words, put beside each
 //      other, are the operand's row g (g + 8).

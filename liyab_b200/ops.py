@@ -1419,6 +1419,7 @@ for _name, _args in {
     "lb_cache4_values": [_i, _p, _p, _i, _p, _l, _p, _l, _p],
     "lb_attention4": [_c.c_char_p],
     "lb_attention4_plan": [_c.c_char_p, _p],
+    "lb_attention4_withhold_next": [_i],
     "lb_evict4": [_c.c_char_p],
 }.items():
     _SIGNATURES[_name] = _args

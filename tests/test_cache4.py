@@ -96,6 +96,12 @@ def test_eviction_refused(change):
     assert ops.lib().lb_evict4(_evict(ref, **change)) != 0 and ops.lib().lb_last_error()
 
 
+@pytest.mark.parametrize("change", [dict(max_keys=(1 << 30) + 1, table_stride=1 << 27), dict(keep=(1 << 30) + 1, dest_table_stride=1 << 27)])
+def test_evictions_too_long_are_refused(change):
+    c, ref = _cache()
+    assert ops.lib().lb_evict4(_evict(ref, **change)) != 0 and b"more than one launch" in ops.lib().lb_last_error()
+
+
 def _plan(kv, heads, n_seq, keys, q_len=1, dim=64):
     c, ref = _cache(kv=kv, dim=dim)
     got = (C.c_int * 4)()
