@@ -1448,54 +1448,68 @@ class Cache4:
         return self.memory.numel()
 
 
-def _rows_of4(what: str, cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, n: int) -> int:
-    """What append4 and cache4_values check of their rows; their type."""
-    width = cache.n_kv_head * cache.head_dim
-    code = _DT.get(k.dtype, -1)
-    if code < 0 or v.dtype is not k.dtype:
+_I32, _F32 = torch.int32, torch.float32
+
+
+# (A call of the smallest sizes takes the GPU less than the host, so what is asked of a tensor is asked once.)
+def _rows_of4(what: str, cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, n: int) -> tuple:
+    """What append4 and cache4_values check of their rows; their type and row strides."""
+    kind, width, index = k.dtype, cache.n_kv_head * cache.head_dim, cache.index
+    code = _DT.get(kind, -1)
+    if code < 0 or v.dtype is not kind:
         raise invalid_argument(f"{what}: keys and values are both float32 or both bfloat16, not {k.dtype} and {v.dtype}")
-    if k.dim() != 2 or v.dim() != 2 or k.shape[1] != width or v.shape[1] != width or k.stride(1) != 1 or v.stride(1) != 1 or not 0 <= n <= min(k.shape[0], v.shape[0]):
-        raise invalid_argument(f"{what}: {n} rows of {width} values, dense within a row, from {tuple(k.shape)} and {tuple(v.shape)}")
-    if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.shape[0] < n:
+    k_shape, v_shape, k_stride, v_stride, places = k.shape, v.shape, k.stride(), v.stride(), slots.shape
+    if len(k_shape) != 2 or len(v_shape) != 2 or k_shape[1] != width or v_shape[1] != width or k_stride[1] != 1 or v_stride[1] != 1 or not 0 <= n <= k_shape[0] or n > v_shape[0]:
+        raise invalid_argument(f"{what}: {n} rows of {width} values, dense within a row, from {tuple(k_shape)} and {tuple(v_shape)}")
+    if slots.dtype is not _I32 or len(places) != 1 or places[0] < n or not slots.is_contiguous():
         raise invalid_argument(f"{what}: the slots are int32, one a row")
-    if k.get_device() != cache.index or v.get_device() != cache.index or slots.get_device() != cache.index:
+    if k.get_device() != index or v.get_device() != index or slots.get_device() != index:
         raise invalid_argument(f"{what}: keys are on {k.device}, values on {v.device} and slots on {slots.device}, the cache on {cache.device}")
-    return code
+    return code, k_stride[0], v_stride[0]
 
 
 def append4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, cache: Cache4, n_tokens: int) -> None:
     """Rounds the step's key and value rows ([tokens, n_kv_head * head_dim], float32 or bfloat16, any row strides) into the cache's slots (int32, negative: skipped; no slot twice in a call):
     a group's scale is its largest |x| / 7 in bfloat16, each value the nearest multiple of it.  A group that is not finite reads back as NaN."""
-    code = _rows_of4("append4", cache, k, v, slot_mapping, n_tokens)
-    check(lib().lb_append4(code, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot_mapping.data_ptr(), cache.ref, n_tokens, stream_of(cache.index)), "append4")
+    code, ldk, ldv = _rows_of4("append4", cache, k, v, slot_mapping, n_tokens)
+    check(lib().lb_append4(code, k.data_ptr(), ldk, v.data_ptr(), ldv, slot_mapping.data_ptr(), cache.ref, n_tokens, stream_of(cache.index)), "append4")
 
 
 def cache4_values(cache: Cache4, slots: torch.Tensor, n: int, k: torch.Tensor, v: torch.Tensor) -> tuple:
     """The first n slots' keys and values as rows of float32 or bfloat16 (rows of negative slots are left as they were); (k, v)."""
-    code = _rows_of4("cache4_values", cache, k, v, slots, n)
-    check(lib().lb_cache4_values(code, cache.ref, slots.data_ptr(), n, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), stream_of(cache.index)), "cache4_values")
+    code, ldk, ldv = _rows_of4("cache4_values", cache, k, v, slots, n)
+    check(lib().lb_cache4_values(code, cache.ref, slots.data_ptr(), n, k.data_ptr(), ldk, v.data_ptr(), ldv, stream_of(cache.index)), "cache4_values")
     return k, v
 
 
-def _ints4(what: str, name: str, t: torch.Tensor, index: int, least: int, columns: int = 0) -> int:
-    """An int32 vector of at least `least` numbers, or a matrix of as many rows and at least `columns` columns, dense within a row."""
+def _not_ints4(what: str, name: str, t: torch.Tensor, least: int, columns: int) -> Exception:
+    return invalid_argument(f"{what}: {name} has to be int32 of at least {least}{f' x {columns}' if columns else ''}, dense within a row, on the cache's device; it is {t.dtype} "
+                            f"{tuple(t.shape)} on {t.device}")
+
+
+def _ints4(what: str, name: str, t: torch.Tensor, index: int, least: int) -> int:
+    """An int32 vector of at least `least` numbers."""
     shape = t.shape
-    if columns == 0:
-        good = len(shape) == 1 and shape[0] >= least and (t.stride(0) == 1 or shape[0] < 2)
-    else:
-        good = len(shape) == 2 and shape[0] >= least and shape[1] >= columns and (t.stride(1) == 1 or shape[1] == 1)
-    if not good or t.dtype is not torch.int32 or t.get_device() != index:
-        raise invalid_argument(f"{what}: {name} has to be int32 of at least {least}{f' x {columns}' if columns else ''}, dense within a row, on the cache's device; it is {t.dtype} "
-                               f"{tuple(shape)} on {t.device}")
+    if t.dtype is not _I32 or t.get_device() != index or len(shape) != 1 or shape[0] < least or not t.is_contiguous():
+        raise _not_ints4(what, name, t, least, 0)
     return t.data_ptr()
 
 
-def _weights_of4(what: str, name: str, t: torch.Tensor, cache: Cache4, keys: int) -> int:
-    """Accumulated weights [rows, n_kv_head, keys], dense within a row."""
-    if (t.dtype is not torch.float32 or t.get_device() != cache.index or t.dim() != 3 or t.shape[1] != cache.n_kv_head or t.shape[2] < keys or (t.stride(2) != 1 and t.shape[2] > 1)):
-        raise invalid_argument(f"{what}: {name} has to be float32 [rows, {cache.n_kv_head}, at least {keys}], dense within a row, on the cache's device; it is {t.dtype} {tuple(t.shape)} "
+def _table4(what: str, name: str, t: torch.Tensor, index: int, least: int, columns: int) -> tuple:
+    """An int32 matrix of at least `least` rows and `columns` columns, dense within a row: its place, the stride of its rows, and its columns."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _I32 or t.get_device() != index or len(shape) != 2 or shape[0] < least or shape[1] < columns or (stride[1] != 1 and shape[1] != 1):
+        raise _not_ints4(what, name, t, least, columns)
+    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1], shape[1]
+
+
+def _weights_of4(what: str, name: str, t: torch.Tensor, cache: Cache4, keys: int) -> tuple:
+    """Accumulated weights [rows, n_kv_head, keys], dense within a row: their place, rows, keys, and the strides of a row and a head."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _F32 or t.get_device() != cache.index or len(shape) != 3 or shape[1] != cache.n_kv_head or shape[2] < keys or (stride[2] != 1 and shape[2] > 1):
+        raise invalid_argument(f"{what}: {name} has to be float32 [rows, {cache.n_kv_head}, at least {keys}], dense within a row, on the cache's device; it is {t.dtype} {tuple(shape)} "
                                f"on {t.device}")
-    return t.data_ptr()
+    return t.data_ptr(), shape[0], shape[2], stride[0], stride[1]
 
 
 def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[torch.Tensor], last: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor, n_seq: int,
@@ -1511,19 +1525,17 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
     if dense_q != 1 or dense_out != 1:
         raise invalid_argument(f"{what}: q and out have to be dense within a row")
     last_at = _ints4(what, "positions" if q_start is None else "n_past", last, index, n_seq)
-    table_at = _ints4(what, "block_table", block_table, index, n_seq, 1)
+    table_at, table_stride, table_columns = _table4(what, "block_table", block_table, index, n_seq, 1)
     start_at = 0 if q_start is None else _ints4(what, "q_start", q_start, index, n_seq + 1)
-    table_rows, table_columns = block_table.shape
     keys = table_columns * cache.page_size
     if 0 < max_keys < keys:
         keys = max_keys
     mass_at = total_at = rows_at = n_mass = 0
     strides = (0, 0, 0, 0)
     if mass is not None:
-        total = mass if total is None else total
-        mass_at, total_at = _weights_of4(what, "mass", mass, cache, keys), _weights_of4(what, "total", total, cache, keys)
-        n_mass = min(mass.shape[0], total.shape[0])
-        strides = (mass.stride(0), mass.stride(1), total.stride(0), total.stride(1))
+        mass_at, n_mass, _, *of_mass = _weights_of4(what, "mass", mass, cache, keys)
+        total_at, n_total, _, *of_total = (mass_at, n_mass, 0, *of_mass) if total is None else _weights_of4(what, "total", total, cache, keys)
+        n_mass, strides = min(n_mass, n_total), (*of_mass, *of_total)
         if mass_rows is not None:
             rows_at = _ints4(what, "mass_rows", mass_rows, index, n_seq)
         elif n_mass < n_seq:
@@ -1535,7 +1547,7 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
             raise invalid_argument(f"{what}: {name} has to be {n} float32 numbers on the cache's device")
     parts = (cache.ref, q.data_ptr(), start_at, last_at, table_at, out.data_ptr(), mass_at, total_at, rows_at, 0 if distance is None else distance.data_ptr(),
              0 if sink is None else sink.data_ptr())
-    rest = (stream_of(index), ldq, ldo, *strides, block_table.stride(0) if table_rows > 1 else table_columns, n_seq, q_shape[0], n_head, max_q_len, keys, n_mass, window, scale, soft_cap)
+    rest = (stream_of(index), ldq, ldo, *strides, table_stride, n_seq, q_shape[0], n_head, max_q_len, keys, n_mass, window, scale, soft_cap)
     l = lib()
     sizes = (n_seq, max_q_len, n_head, keys, mass is None, rest[7], window)
     size = cache.scratch.get(sizes)
@@ -1578,21 +1590,20 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
     the lowest places).  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
     they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (memory of its own, not mass)."""
     index, page = cache.index, cache.page_size
-    table_at, dest_at = _ints4("evict4", "block_table", block_table, index, n_seq, 1), _ints4("evict4", "dest_table", dest_table, index, n_seq, max(1, -(-keep // page)))
-    keys = min(block_table.shape[1] * page, mass.shape[2] if mass.dim() == 3 else 0)
-    mass_at, n_keys_at = _weights_of4("evict4", "mass", mass, cache, 1), _ints4("evict4", "n_keys", n_keys, index, n_seq)
-    kept_at, kept_shape = kept.data_ptr(), kept.shape
-    if kept.dtype is not torch.int32 or kept.get_device() != index or len(kept_shape) != 3 or kept_shape[0] < n_seq or kept_shape[1:] != (cache.n_kv_head, keep) or not kept.is_contiguous():
+    table_at, table_stride, columns = _table4("evict4", "block_table", block_table, index, n_seq, 1)
+    dest_at, dest_stride, _ = _table4("evict4", "dest_table", dest_table, index, n_seq, max(1, -(-keep // page)))
+    mass_at, n_mass, keys, mass_stride, mass_head = _weights_of4("evict4", "mass", mass, cache, 1)
+    n_keys_at = _ints4("evict4", "n_keys", n_keys, index, n_seq)
+    kept_shape = kept.shape
+    if kept.dtype is not _I32 or kept.get_device() != index or len(kept_shape) != 3 or kept_shape[0] < n_seq or kept_shape[1:] != (cache.n_kv_head, keep) or not kept.is_contiguous():
         raise invalid_argument(f"evict4: kept has to be contiguous int32 [requests, {cache.n_kv_head}, {keep}] on the cache's device; it is {kept.dtype} {tuple(kept_shape)} on {kept.device}")
-    rows_at = dest_mass_at = n_dest = 0
-    strides = (0, 0)
+    rows_at = dest_mass_at = n_dest = dest_mass_stride = dest_head = 0
     if dest_mass is not None:
-        dest_mass_at, n_dest, strides = _weights_of4("evict4", "dest_mass", dest_mass, cache, keep), dest_mass.shape[0], (dest_mass.stride(0), dest_mass.stride(1))
+        dest_mass_at, n_dest, _, dest_mass_stride, dest_head = _weights_of4("evict4", "dest_mass", dest_mass, cache, keep)
     if mass_rows is not None:
         rows_at = _ints4("evict4", "mass_rows", mass_rows, index, n_seq)
-    elif mass.shape[0] < n_seq or (dest_mass is not None and n_dest < n_seq):
-        raise invalid_argument(f"evict4: {n_seq} requests, weights of {mass.shape[0]}{'' if dest_mass is None else f' and {n_dest}'}")
-    check(lib().lb_evict4(_evict4_args(cache.ref, mass_at, rows_at, table_at, n_keys_at, dest_at, kept_at, dest_mass_at, stream_of(index), mass.stride(0), mass.stride(1), *strides,
-                                       block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1], dest_table.stride(0) if dest_table.shape[0] > 1 else dest_table.shape[1],
-                                       n_seq, keep, recent, keys, mass.shape[0], n_dest)), "evict4")
+    elif n_mass < n_seq or (dest_mass is not None and n_dest < n_seq):
+        raise invalid_argument(f"evict4: {n_seq} requests, weights of {n_mass}{'' if dest_mass is None else f' and {n_dest}'}")
+    check(lib().lb_evict4(_evict4_args(cache.ref, mass_at, rows_at, table_at, n_keys_at, dest_at, kept.data_ptr(), dest_mass_at, stream_of(index), mass_stride, mass_head, dest_mass_stride,
+                                       dest_head, table_stride, dest_stride, n_seq, keep, recent, min(columns * page, keys), n_mass, n_dest)), "evict4")
     return kept
