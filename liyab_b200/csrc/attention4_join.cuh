@@ -25,10 +25,27 @@ __device__ __forceinline__ void join_row(const Call& c, const Portion& part, int
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, team = 1 << team_shift, mine = warp & (team - 1);
     float m = kLowest, l = 0.0f, v[V] = {};
     if (state != nullptr) {
-        // Thirty-two at a time: a lane has a state's reference and sum, and its factor once the largest reference is known.
+        // Thirty-two at a time: a lane has a state's reference and sum, and its factor once the largest reference is known.  The values come eight states at a time, the first eight before the factors.
         for (int i0 = mine; i0 < runs; i0 += 32 * team) {
+            constexpr int kAhead = 8;
+            const int n = min(32, (runs - i0 + team - 1) >> team_shift);
+            const float* at = state + i0 * step + 4 + V * lane;
             float2 ml = make_float2(kLowest, 0.0f);
-            if (i0 + lane * team < runs) ml = *reinterpret_cast<const float2*>(state + (i0 + lane * team) * step);
+            if (lane < n) ml = *reinterpret_cast<const float2*>(state + (i0 + lane * team) * step);
+            float o[kAhead][V];
+            auto load = [&](int x0) {
+#pragma unroll
+                for (int x = 0; x < kAhead; ++x) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o[x][e] = 0.0f;
+                    if (x0 + x < n) {
+                        const float* p = at + (x0 + x) * team * step;
+                        if constexpr (V == 4) *reinterpret_cast<float4*>(o[x]) = *reinterpret_cast<const float4*>(p);
+                        else *reinterpret_cast<float2*>(o[x]) = *reinterpret_cast<const float2*>(p);
+                    }
+                }
+            };
+            load(0);
             const bool some = ml.y != 0.0f;                 // (a NaN is some)
             float high = some ? ml.x : kLowest;
 #pragma unroll
@@ -39,16 +56,14 @@ __device__ __forceinline__ void join_row(const Call& c, const Portion& part, int
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] *= keep;
             m = high;
-            const int n = min(32, (runs - i0 + team - 1) >> team_shift);
-            const float* at = state + i0 * step + 4 + V * lane;
-#pragma unroll 4
-            for (int x = 0; x < n; ++x, at += team * step) {
-                const float f = __shfl_sync(0xffffffffu, w, x);
-                float o[V];
-                if constexpr (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(at);
-                else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(at);
+            for (int x0 = 0; x0 < n; x0 += kAhead) {
+                if (x0 > 0) load(x0);
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = fmaf(o[e], f, v[e]);
+                for (int x = 0; x < kAhead; ++x) {
+                    const float f = __shfl_sync(0xffffffffu, w, (x0 + x) & 31);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] = fmaf(o[x][e], f, v[e]);
+                }
             }
         }
     }
@@ -61,12 +76,22 @@ __device__ __forceinline__ void join_row(const Call& c, const Portion& part, int
         }
         __syncthreads();
         if (mine > 0) return;
-        for (int i = 1; i < team; ++i) {
-            const float mi = joined[warp + i][0], li = joined[warp + i][1], high = li == 0.0f ? m : fmaxf(m, mi), w = li == 0.0f ? 0.0f : ex2(mi - high), keep = ex2(m - high);
-            l = fmaf(l, keep, li * w);
+        // A lane has a warp's reference and sum.
+        const float mi = lane < team ? joined[warp + lane][0] : kLowest, li = lane < team ? joined[warp + lane][1] : 0.0f;
+        const bool some = li != 0.0f;
+        float high = some ? mi : kLowest;
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = fmaf(v[e], keep, joined[warp + i][2 + V * lane + e] * w);
-            m = high;
+        for (int x = 16; x > 0; x /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+        const float w = some ? ex2(mi - high) : 0.0f;
+        l = lb_warp_sum(some ? li * w : 0.0f);
+        m = high;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < team; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = fmaf(joined[warp + i][2 + V * lane + e], f, v[e]);
         }
     }
     if (state == nullptr) return;

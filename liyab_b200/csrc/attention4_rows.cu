@@ -576,11 +576,12 @@ __global__ void __launch_bounds__(1024)
 attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int rows_shift, int team_shift) {
     constexpr int kState = HD + 4;
     __shared__ float joined[32][HD + 2];
-    lb_wait_for_predecessor();
-    lb_dependents_may_launch();
     const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row;
     const int r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (threadIdx.x >> 5 >> team_shift);
+    // What the kernel before read as well was written before it began, as its blocks let this one start only behind their own wait.
     const Portion part = portion_of(c, seq);
+    lb_wait_for_predecessor();
+    lb_dependents_may_launch();
     const float* state = nullptr;
     int runs = 0;
     if (r < part.count * c.per) {
@@ -643,10 +644,10 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     const int kWarps = warps_of(p.rows / 4, false);
     const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4, false) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
     p.blocks = (int)std::max<int64_t>(1, (warps + kWarps - 1) / kWarps);
-    // Runs that a row has, about; a warp takes some four of them.
+    // Runs that a row has, about; a warp takes eight of them or fewer, whose values are on their way at once.
     const int64_t runs = p.blocks * kWarps / (units * p.per_row) + 2;
     p.join_team = 1;
-    while (p.join_team < 32 && p.join_team * 4 < runs) p.join_team *= 2;
+    while (p.join_team < 32 && p.join_team * 8 < runs) p.join_team *= 2;
     const int64_t rows = (std::max(1, n_seq) + p.per_row - 1) / p.per_row;
     p.states = rows * (p.blocks * kWarps + p.per_row * units) * p.rows * (head_dim + 4) * 4;
     p.starts = rows * (p.per_row + 1) * 4;
