@@ -5,8 +5,8 @@
 // out in 16 us (85 MB, 5.3 TB/s).
 // evict4 is two launches.  The first chooses: a block a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  It is bound by the passes' chains of
-// barriers and, for long requests, by their instructions on the SMs that have a request and head (from cold memory 12 x 2,048 keys 9.3 us, 64 x 8,192 keys 14; with eleven bits of zeros counted a vote at a
-// time, one key a step, 17).  The second copies: a warp a block of sixteen keys of the
+// barriers and, for long requests, by their instructions on the SMs that have a request and head (from cold memory 12 x 2,048 keys 9.3 us, 64 x 8,192 keys 14; with zeros counted by votes
+// and one key a step 17).  The second copies: a warp a block of sixteen keys of the
 // destination, whose pieces it gathers, all asked for before the first is stored (64 x 2,048 keys of 128 dims, 36 MB read and written, 10.4 us; a piece at a time 12.2).  The destination is never
 // a source, so nothing waits for anything.
 #include "attention4.h"

@@ -576,6 +576,54 @@ def test_decode_of_more_requests_than_a_launch_row(dev):
     assert ways == {False, True}
 
 
+@pytest.mark.parametrize("heads,new,many", [(4, 6, 0), (32, 300, 1)])
+@pytest.mark.parametrize("window", [0, 50, -64])
+def test_portions_read_no_key_past_the_most(dev, heads, new, many, window):
+    """Places past max_keys are taken as the last key there, in the kernel for few rows and the one for many."""
+    f = Filled(dev, [700, 400], 2, 64, 32, 16, seed=5)
+    q = _queries(f, 2 * new, heads, 1)
+    start, past = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=dev), torch.tensor([700 - new, 400 - new], dtype=torch.int32, device=dev)
+    most = 700 - new // 2
+    got = (C.c_int * 4)()
+    call = _call(f.cache.ref, n_head=heads, n_seq=2, n_tokens=2 * new, max_keys=most, table_stride=f.table.shape[1], q_stride=64 * heads, out_stride=64 * heads, q_start=AT, max_q_len=new,
+                 window=window)
+    assert ops.lib().lb_attention4_plan(call, got) == 0 and got[0] == many
+    out = ops.prefill_attention4(q, f.cache, start, past, f.table, torch.empty_like(q), 2, new, heads, 0.125, window=window, max_keys=most)
+    for i, n in enumerate((700, 400)):
+        places = torch.arange(n - new, n, device=dev).clamp(max=most - 1)
+        want, _, bound, _ = _attention(q[i * new:(i + 1) * new].view(new, heads, 64), f.k[i][:most], f.v[i][:most], places, 0.125, window=window, many=many == 1)
+        _close(out[i * new:(i + 1) * new].view(new, heads, 64), want, bound)
+
+
+def test_requests_that_share_pages_and_weights_of_other_rows(dev):
+    """Two requests over the same pages; the keys' weights on rows of any order, others left alone, rows outside skipped."""
+    f = Filled(dev, [300, 100], 2, 64, 64, 16, seed=2)
+    table = torch.stack([f.table[0], f.table[0], f.table[1]])
+    q, places = _queries(f, 3, 4, 0), torch.tensor([299, 120, 99], dtype=torch.int32, device=dev)
+    mass = torch.full((4, 2, table.shape[1] * 16), 0.5, device=dev)
+    rows = torch.tensor([3, 7, 0], dtype=torch.int32, device=dev)
+    out = ops.decode_attention4(q, f.cache, places, table, torch.empty_like(q), 3, 4, 0.125, mass=mass, mass_rows=rows)
+    for i, (of, n, r) in enumerate(((0, 300, 3), (0, 121, None), (1, 100, 0))):
+        want, weights, bound, relative = _attention(q[i:i + 1].view(1, 4, 64), f.k[of][:n], f.v[of][:n], torch.tensor([n - 1], device=dev), 0.125)
+        _close(out[i].view(1, 4, 64), want, bound)
+        if r is not None:
+            gained = weights.view(2, 2, n).sum(1)
+            assert ((mass[r, :, :n].double() - 0.5 - gained).abs() <= gained * (3 * relative.max() + 2.0 ** -21) + (0.5 + gained) * 2.0 ** -23).all() and (mass[r, :, n:] == 0.5).all()
+    assert (mass[1:3] == 0.5).all()
+
+
+def test_calls_of_nothing(dev):
+    f = Filled(dev, [40], 2, 64, 64, seed=1)
+    none, i32 = torch.empty(0, 256, dtype=BF16, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    before = f.cache.memory.clone()
+    ops.append4(none[:, :128], none[:, :128], i32, f.cache, 0)
+    ops.cache4_values(f.cache, i32, 0, none[:, :128], none[:, :128])
+    ops.decode_attention4(none, f.cache, i32[:0], f.table, none, 0, 4, 0.125)
+    ops.prefill_attention4(none, f.cache, i32, i32[:0], f.table, none, 0, 5, 4, 0.125)
+    ops.evict4(f.cache, torch.zeros(1, 2, 48, device=dev), f.table, i32, 0, 4, 2, f.table, torch.empty(0, 2, 4, dtype=torch.int32, device=dev))
+    assert torch.equal(f.cache.memory, before)
+
+
 # ---- eviction ----------------------------------------------------------------------------------------------
 
 def _evict(f, mass, keep, recent, mass_rows=None):
