@@ -579,10 +579,9 @@ attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int ro
     __shared__ float joined[32][HD + 2];
     const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row;
     const int r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (threadIdx.x >> 5 >> team_shift);
-    // What the kernel before read as well was written before it began, as its blocks let this one start only behind their own wait.
-    const Portion part = portion_of(c, seq);
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
+    const Portion part = portion_of(c, seq);
     const float* state = nullptr;
     int runs = 0;
     if (r < part.count * c.per) {

@@ -3,7 +3,7 @@
 // append4 and cache4_values move each value once; eight threads have a row of keys or of values, in the order of cache4.cuh.  They are bound by instructions, 281 a warp of 512 values in and 123 out:
 // 4,096 tokens of 8 heads of 128 go in in 11.2 us by themselves from cold memory (477 instructions a warp, with keys and values in each and a corrected division a value: 16), 16,384 rows of 8 heads come
 // out in 16 us (85 MB, 5.3 TB/s).
-// evict4 is two launches.  The first chooses: a block a request and key/value head finds the weight of the last key that stays by a radix selection over the
+// evict4 is two launches.  The first chooses: a block (a cluster of up to eight for more than 8,192 keys) a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  It is bound by the passes' chains of
 // barriers and, for long requests, by their instructions on the SMs that have a request and head (from cold memory 12 x 2,048 keys 9.3 us, 64 x 8,192 keys 14; with zeros counted by votes
 // and one key a step 17).  The second copies: a warp a block of sixteen keys of the
@@ -14,6 +14,8 @@
 #include "linear4.h"
 
 #include <math_constants.h>
+
+#include <algorithm>
 
 namespace lb_c4 {
 
@@ -305,35 +307,58 @@ struct Choice {
     int keep, recent, max_keys, n_mass, n_dest_mass;
 };
 
+// A barrier of the cluster's threads (`blocks` 1: of the block's), and a pair of numbers in block r's shared memory.
+__device__ __forceinline__ void meet(int blocks) {
+    if (blocks == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+}
+__device__ __forceinline__ uint2 of_block(const uint32_t* here, int r) {
+    uint2 v;
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(here)), "r"(r));
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
+// `blocks` blocks, a cluster, share a request's and head's keys: their counts meet in each other's shared memory.
 // (1,024 threads also for few keys: 1 request of 2,048, 12 heads, 14.9 us in all; with 512 16.6, with 256 23.2, as the passes wait for shared memory.)
+template <bool SHARED>
 __global__ void __launch_bounds__(kChoiceThreads)
-evict4_choose_kernel(const Choice c, int held) {
+evict4_choose_kernel(const Choice c, int held, int n_blocks) {
+    const int blocks = SHARED ? n_blocks : 1;
     constexpr int THREADS = kChoiceThreads, kOwn = kBins / THREADS;
-    extern __shared__ uint32_t keys_s[];       // the first `held` keys' weights as ordered integers
-    __shared__ __align__(16) uint32_t bins[kBins];
+    static_assert(kOwn == 2, "a thread's bins are read as a pair");
+    extern __shared__ uint32_t keys_s[];       // the first `held` of the block's keys' weights as ordered integers
+    __shared__ __align__(16) uint32_t both[2][kBins];         // a pass's counts, in turns: the others of the cluster may be at the last pass's still
+    __shared__ __align__(8) uint32_t kept_here[2];          // keys of this block above the threshold, and at it
     __shared__ uint32_t sums[THREADS / 32];
     __shared__ uint32_t found[2];              // the bin that holds the last key to stay, and how many of it stay
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
-    const int head = blockIdx.x, seq = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int head = blockIdx.x / blocks, rank = blockIdx.x - head * blocks, n_head = gridDim.x / blocks, seq = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = min(max(c.n_keys[seq], 0), c.max_keys);
     const int r = c.mass_rows != nullptr ? c.mass_rows[seq] : seq;
     const bool weighed = (unsigned)r < (unsigned)c.n_mass;
     const float* mass = c.mass + (weighed ? (int64_t)r * c.mass_stride + (int64_t)head * c.mass_head_stride : 0);
-    int32_t* kept = c.kept + ((int64_t)seq * gridDim.x + head) * c.keep;
+    int32_t* kept = c.kept + ((int64_t)seq * n_head + head) * c.keep;
     float* dest = c.dest_mass != nullptr && (unsigned)r < (unsigned)c.n_dest_mass ? c.dest_mass + (int64_t)r * c.dest_stride + (int64_t)head * c.dest_head_stride : nullptr;
     const int stay = min(n, c.keep), old = n - min(c.recent, n);
     const int by_weight = stay - (n - old);           // of the `old` first keys; recent <= keep, so never negative
-    for (int i0 = threadIdx.x; i0 < min(old, held); i0 += 4 * THREADS) {
+    // The block's stretch of the old keys.
+    const int share = ((old + blocks - 1) / blocks + 31) / 32 * 32, lo = min(old, rank * share), mine = min(old, lo + share) - lo, in_shared = min(mine, held);
+    for (int i0 = threadIdx.x; i0 < in_shared; i0 += 4 * THREADS) {
         float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = weighed && i0 + j * THREADS < old ? mass[i0 + j * THREADS] : 0.0f;
+        for (int j = 0; j < 4; ++j) v[j] = weighed && i0 + j * THREADS < mine ? mass[lo + i0 + j * THREADS] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i0 + j * THREADS < min(old, held)) keys_s[i0 + j * THREADS] = ordered(v[j]);
+            if (i0 + j * THREADS < in_shared) keys_s[i0 + j * THREADS] = ordered(v[j]);
     }
     __syncthreads();
-    auto key_at = [&](int i) { return i < held ? keys_s[i] : weighed ? ordered(mass[i]) : 0x80000000u; };
+    auto key_at = [&](int i) { return i < held ? keys_s[i] : weighed ? ordered(mass[lo + i]) : 0x80000000u; };
     // The sum of what the warps before this one left.
     auto before = [&](const uint32_t* of_warps) { return __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[lane] : 0u); };
     // The by_weight-th largest key among the first `old`: `threshold` its prefix so far, `left` how many keys with that prefix stay.
@@ -345,6 +370,7 @@ evict4_choose_kernel(const Choice c, int held) {
             const int bits = pass < 2 ? 11 : 10, high = low;
             low -= bits;
             const uint32_t mask = (1u << bits) - 1u, prefix = pass == 0 ? 0u : threshold >> high;
+            uint32_t* bins = both[pass & 1];
             for (int i = 4 * threadIdx.x; i < kBins; i += 4 * THREADS) *reinterpret_cast<uint4*>(bins + i) = make_uint4(0, 0, 0, 0);
             __syncthreads();
             // Many weights are 0: they are counted in a register and enter with one addition a warp.
@@ -355,7 +381,6 @@ evict4_choose_kernel(const Choice c, int held) {
                 else atomicAdd(&bins[key >> low & mask], 1u);
             };
             int i = threadIdx.x;
-            const int in_shared = min(old, held);
             for (; i + 3 * THREADS < in_shared; i += 4 * THREADS) {
                 uint32_t key[4];
 #pragma unroll
@@ -363,18 +388,19 @@ evict4_choose_kernel(const Choice c, int held) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) enter(key[j]);
             }
-            for (; i < old; i += THREADS) enter(key_at(i));
+            for (; i < mine; i += THREADS) enter(key_at(i));
             zeros = __reduce_add_sync(0xffffffffu, zeros);
             if (zeros != 0 && lane == 0) atomicAdd(&bins[0x80000000u >> low & mask], zeros);
-            __syncthreads();
-            // A few neighbouring bins a thread, from the largest down: how many keys lie in larger bins.
+            meet(blocks);
+            // Two neighbouring bins a thread, from the largest down, of all the cluster's blocks: how many keys lie in larger bins.  Every block does the same sums.
             const int top = kBins - 1 - kOwn * threadIdx.x;
-            uint32_t own[kOwn], sum = 0;
-#pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-                own[j] = bins[top - j];
-                sum += own[j];
+            uint32_t own[kOwn] = {};
+            for (int r = 0; r < blocks; ++r) {
+                const uint2 two = blocks == 1 ? *reinterpret_cast<const uint2*>(bins + top - 1) : of_block(bins + top - 1, r);
+                own[0] += two.y;
+                own[1] += two.x;
             }
+            const uint32_t sum = own[0] + own[1];
             uint32_t larger = sum;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
@@ -405,7 +431,7 @@ evict4_choose_kernel(const Choice c, int held) {
         left = 0xffffffffu;            // all do
     }
     // A warp has a stretch of the keys: it counts those above the threshold and those at it, the warps' counts meet, and it writes its own.
-    const int stretch = (old + THREADS - 1) / THREADS * 32, from = min(old, warp * stretch), to = min(old, from + stretch);
+    const int stretch = (mine + THREADS - 1) / THREADS * 32, from = min(mine, warp * stretch), to = min(mine, from + stretch);
     uint32_t above = 0, at = 0;
     for (int i = from + lane; i < to; i += 32) {
         const uint32_t key = key_at(i);
@@ -414,13 +440,25 @@ evict4_choose_kernel(const Choice c, int held) {
     }
     above = __reduce_add_sync(0xffffffffu, above);
     at = __reduce_add_sync(0xffffffffu, at);
-    __syncthreads();
+    uint32_t* counts = both[1];                // (the last pass's are the other; no block reads these any more)
     if (lane == 0) {
-        bins[warp] = above;
-        bins[32 + warp] = at;
+        counts[warp] = above;
+        counts[32 + warp] = at;
     }
     __syncthreads();
-    uint32_t place = before(bins), ties = before(bins + 32);
+    uint32_t place = before(counts), ties = before(counts + 32);
+    if (blocks > 1) {
+        if (threadIdx.x == THREADS - 1) {
+            kept_here[0] = place + above;
+            kept_here[1] = ties + at;
+        }
+        meet(blocks);
+        for (int r = 0; r < rank; ++r) {
+            const uint2 two = of_block(kept_here, r);
+            place += two.x;
+            ties += two.y;
+        }
+    }
     place += min(ties, left);
     for (int i0 = from; i0 < to; i0 += 32) {
         const int i = i0 + lane;
@@ -432,18 +470,19 @@ evict4_choose_kernel(const Choice c, int held) {
         const uint32_t mask = __ballot_sync(0xffffffffu, stays);
         const uint32_t p = place + __popc(mask & below);
         if (stays && p < (uint32_t)c.keep) {
-            kept[p] = i;
-            if (dest != nullptr) dest[p] = weighed ? mass[i] : 0.0f;
+            kept[p] = lo + i;
+            if (dest != nullptr) dest[p] = weighed ? mass[lo + i] : 0.0f;
         }
         place += __popc(mask);
         ties += __popc(tie_mask);
     }
-    for (int i = max(by_weight, 0) + threadIdx.x; i < c.keep; i += THREADS) {
+    for (int i = max(by_weight, 0) + rank * THREADS + threadIdx.x; i < c.keep; i += blocks * THREADS) {
         const int key = old + i - max(by_weight, 0);
         const bool there = i < stay;
         kept[i] = there ? key : -1;
         if (dest != nullptr) dest[i] = there && weighed ? mass[key] : 0.0f;
     }
+    if (blocks > 1) meet(blocks);              // no block leaves while another reads its counts
 }
 
 template <int HD>
@@ -595,11 +634,16 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
                       a.n_mass, a.n_dest_mass};
-    const int held = a.max_keys < kMostHeld ? a.max_keys : kMostHeld;
-    static std::atomic<uint64_t> asked{0};
-    if (int rc = lb_a4::allow_shared(evict4_choose_kernel, 4 * kMostHeld, asked)) return rc;
-    LB_CHECK_CUDA(lb_launch_overlapped(evict4_choose_kernel, dim3(pages.n_kv_head, a.n_seq), dim3(kChoiceThreads), 4 * held, s, c, held));
-    const dim3 grid((a.keep + 63) / 64, pages.n_kv_head, a.n_seq);
+    // A block a request and head up to 8,192 keys (8 x 8,192 keys, 8 heads: 38.9 us, by two blocks each 39.8, whose barriers cost what they save); for more as many as there are SMs for (1 x 131,072
+    // keys, 8 heads: 57 us by eight blocks each, 230 by one).
+    int blocks = 1;
+    while (blocks < 8 && (int64_t)pages.n_kv_head * a.n_seq * blocks * 2 <= linear4_sm_count() && a.max_keys > 8192 * blocks) blocks *= 2;
+    const int held = std::min(((a.max_keys + blocks - 1) / blocks + 31) / 32 * 32, kMostHeld);
+    auto choose = blocks > 1 ? evict4_choose_kernel<true> : evict4_choose_kernel<false>;
+    static std::atomic<uint64_t> asked[2];
+    if (int rc = lb_a4::allow_shared(choose, 4 * kMostHeld, asked[blocks > 1])) return rc;
+    LB_CHECK_CUDA(lb_launch_overlapped_cluster(0, blocks, choose, dim3(pages.n_kv_head * blocks, a.n_seq), dim3(kChoiceThreads), 4 * held, s, c, held, blocks));
+    const dim3 grid((a.keep - 1) / 64 + 1, pages.n_kv_head, a.n_seq);
     LB_CHECK_CUDA(lb_launch_overlapped(a.cache->head_dim == 128 ? evict4_copy_kernel<128> : evict4_copy_kernel<64>, grid, dim3(128), 0, s, pages, a.block_table, a.table_stride,
                                        a.dest_table, a.dest_table_stride, a.kept, a.keep, a.max_keys));
     return LB_OK;

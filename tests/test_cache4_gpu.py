@@ -705,6 +705,17 @@ def test_evict_of_more_keys_than_a_block_holds(dev, keep, recent):
     _evict(f, (mass * 4).floor(), keep, recent)              # equal weights on both sides of what the block holds
 
 
+@pytest.mark.parametrize("kv,n,keep,recent", [(2, 8193, 100, 3), (1, 20000, 19000, 0), (3, 70001, 333, 40), (40, 9000, 4500, 32), (1, 8200, 8200, 8200)])
+def test_evict_of_keys_that_blocks_share(dev, kv, n, keep, recent):
+    """Two to eight blocks a head, and one where there are many heads; other requests beside them with none and one of their keys to drop."""
+    lengths = [n, 0, keep + 1] if kv < 40 else [n]
+    f = Filled(dev, lengths, kv, 64, 64, 64, seed=1, extra=len(lengths) * -(-keep // 64))
+    mass = torch.rand(len(lengths), kv, f.table.shape[1] * 64, generator=torch.Generator().manual_seed(2)).to(dev)
+    _evict(f, mass, keep, recent)
+    _evict(f, (mass * 3).floor(), keep, recent)
+    _evict(f, torch.zeros_like(mass), keep, recent)
+
+
 # ---- together ----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("captured", [False, True])
