@@ -11,7 +11,8 @@
 // What is rounded: p s to float16 (2^-12, or 2^-31 of the warp's largest value scale), and queries more than 2^6 below their row's largest (to 2^-15 of it); a row's 16 bits hold bfloat16's
 // eight of all others.  A power of two a row puts its largest at 2^14.  The values' scales have any size that bfloat16 has, so what p is relative to is the row's largest score plus the exponent
 // of the warp's largest value scale f (down to 2^-80), less 6: 2^(S - m) s is at most 2^14.  f leaves no trace in the result.  m moves when a score passes it by more than 2^8, or a scale f: the warp
-// votes, which costs a few instructions a pair where searching the maximum cost thirty a tile.
+// votes, which costs a few instructions a pair where searching the maximum cost thirty a tile.  A scale that is NaN (of a group that was not finite) is no f and no factor: it would meet p = 0 of rows
+// that do not see its key.  It passes every f, so it is met where the warp has voted: its products are 0, and the sums of the rows that see it are NaN from there on.
 //
 // Two ways to share the keys out (rows_plan chooses by an estimate of both).  WHOLE: a block has a request's row tile and key/value head, its eight warps a stretch of the keys each, whose states meet
 // in shared memory and become the result: no scratch memory, one launch.  Else all warps of the launch take equal shares of all tiles of all requests (256 at most to a launch row), wherever they
@@ -455,10 +456,36 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) moved = moved || fmaxf(fmaxf(z[n][0][0], z[n][0][1]), fmaxf(z[n][1][0], z[n][1][1])) > passes[n];
             if (__any_sync(0xffffffffu, moved)) {
+                // A scale that is NaN (it passes any f) is 0 in the products, and what the rows that see its key have of the group's dims becomes NaN, which no later factor or sum changes.
+                uint32_t nans = 0;                          // a bit a row and group
+                top = 0;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2 * NG; ++i) {
+                        const uint32_t half_word = i % 2 != 0 ? 0xffff0000u : 0x0000ffffu;
+                        if ((vs[u][i / 2] & half_word & 0x7fff7fffu) >= (0x7f807f80u & half_word)) {
+                            vs[u][i / 2] &= ~half_word;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) nans |= z[n][u][i / NG] != -CUDART_INF_F ? 1u << (n * NG + i % NG) : 0u;
+                        }
+                        if (i % 2 != 0) top = __vmaxu2(top, vs[u][i / 2]);
+                    }
+                if (__any_sync(0xffffffffu, nans != 0)) {
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) nans |= __shfl_xor_sync(0xffffffffu, nans, d);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < JV * 4; ++k) {
+                            const int gr = (64 * (k / 4) + 32 * (k % 4 >> 1)) / (HD / NG), e = NT == 1 ? gr & 1 : n & 1;
+                            if ((nans >> (n * NG + gr) & 1u) != 0) o[n / 2][k][e] = o[n / 2][k][e + 2] = CUDART_NAN_F;
+                        }
+                }
                 top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
                 float f_new = f;
                 if (top > f_bits) {
-                    f_bits = (min(top, 0x7f00u) + 0x7fu) & 0x7f80u;         // the next power of two (2^127 at most; a NaN stays one whatever it is divided by)
+                    f_bits = (min(top, 0x7f00u) + 0x7fu) & 0x7f80u;         // the next power of two (2^127 at most)
                     f_new = (float)((int)(f_bits >> 7) - 127) - kRoom;
                 }
                 float corr[NT];

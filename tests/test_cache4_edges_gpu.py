@@ -1,0 +1,92 @@
+"""The 4-bit cache where single values are not finite or of the largest and smallest sizes, against plain forms in 64 bits."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from liyab_b200 import ops
+from test_cache4 import _call
+from test_cache4_gpu import BF16, FORMS, Filled, _attention, _close, _queries, _slots, _values_as_rows
+from test_kernels_gpu import dev  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _shared(f, n, heads, most, **more):
+    """Whether all warps of a launch share the keys (a launch joins their states), or a block has a request's row tile and key/value head to itself; None: the kernel for many rows."""
+    got = (C.c_int * 4)()
+    width, keys = heads * f.dim, f.table.shape[1] * f.cache.page_size
+    portions = dict(q_start=1 << 20, max_q_len=most) if most > 1 else {}
+    call = _call(f.cache.ref, n_head=heads, n_seq=n, n_tokens=n * most, max_keys=keys, table_stride=f.table.shape[1], q_stride=width, out_stride=width, **portions, **more)
+    assert ops.lib().lb_attention4_plan(call, got) == 0
+    return None if got[0] == 1 else got[2] > 1 or got[3] > 1
+
+
+def _spoil(f, i, place, head, group):
+    """A value of request i's key at `place` becomes NaN: the group of this head's that has it is not finite."""
+    rows = [_values_as_rows(x[i][place:place + 1]) for x in (f.k, f.v)]
+    rows[1][0, head * f.dim + group * f.cache.group + 3] = math.nan
+    ops.append4(*rows, _slots(f.table.cpu(), i, place + 1, f.cache.page_size)[place:].to(f.dev), f.cache, 1)
+    f.v[i][place, head, group * f.cache.group:(group + 1) * f.cache.group] = math.nan
+
+
+def _beside(f, new, heads, seed=0, mass=False, window=0, sink=None):
+    """Attention of the last new[i] tokens of each request beside the plain form, whose values that are NaN are 0: a row that sees such a group is NaN there, all else is within its bound."""
+    n, scale = len(f.lengths), 1 / math.sqrt(f.dim)
+    q, out = _queries(f, sum(new), heads, seed), torch.full((sum(new), heads * f.dim), 7.5, dtype=BF16, device=f.dev)
+    cells = f.table.shape[1] * f.cache.page_size
+    before = torch.rand(n, f.kv, cells, generator=torch.Generator().manual_seed(seed)).to(f.dev) if mass else None
+    total = torch.full_like(before, 7.5) if mass else None
+    more = dict(mass=before, total=total, window=window, sink=sink)
+    past = torch.tensor([a - b for a, b in zip(f.lengths, new)], dtype=torch.int32, device=f.dev)
+    if max(new) == 1:
+        ops.decode_attention4(q, f.cache, past, f.table, out, n, heads, scale, **more)
+    else:
+        ops.prefill_attention4(q, f.cache, torch.tensor([0] + new).cumsum(0).to(torch.int32).to(f.dev), past, f.table, out, n, max(new), heads, scale, **more)
+    token = 0
+    for i, (m, count) in enumerate(zip(f.lengths, new)):
+        places, key = torch.arange(m - count, m, device=f.dev)[:, None], torch.arange(m, device=f.dev)[None, :]
+        want, weights, bound, relative = _attention(q[token:token + count].view(-1, heads, f.dim), f.k[i], f.v[i].nan_to_num(0.0), places[:, 0], scale, window=window, sink=sink)
+        sees = (key <= places) & (key > places - (window if window > 0 else 1 << 30))
+        nan = (sees.double() @ f.v[i].isnan().double().view(m, -1) > 0).view(count, f.kv, 1, f.dim).expand(-1, -1, heads // f.kv, -1).reshape(count, heads, f.dim)
+        got = out[token:token + count].view(-1, heads, f.dim)
+        assert torch.equal(got.isnan(), nan)
+        _close(torch.where(nan, torch.zeros_like(got), got), want.masked_fill(nan, 0.0), bound)
+        if mass:
+            gained = weights.sum(0).view(f.kv, heads // f.kv, m).sum(1)
+            allowed = gained * (3 * relative.max() + (count * heads // f.kv + 2) * 2.0 ** -23) + (before[i, :, :m].double() + gained) * 2.0 ** -23
+            assert ((total[i, :, :m].double() - before[i, :, :m].double() - gained).abs() <= allowed).all()
+        token += count
+
+
+@pytest.mark.parametrize("dim,group", FORMS)
+@pytest.mark.parametrize("heads", [2, 4, 16])
+@pytest.mark.parametrize("lengths,shared", [([200, 90], False), ([9000, 40], True)])
+def test_a_value_that_is_not_finite_changes_nothing_but_its_group(dev, dim, group, heads, lengths, shared):  # noqa: F811
+    """Single tokens: the other groups of the head, the other heads, and the weights that the keys got are what they are without it."""
+    f = Filled(dev, lengths, 2, dim, group, seed=heads)
+    assert _shared(f, 2, heads, 1) == shared
+    _spoil(f, 0, 101, 0, 0)
+    _spoil(f, 0, lengths[0] - 1, 1, dim // group - 1)
+    _spoil(f, 1, 0, 1, 0)
+    for more in (dict(), dict(mass=True), dict(window=120), dict(sink=torch.randn(heads, generator=torch.Generator().manual_seed(1)).to(dev), mass=True)):
+        _beside(f, [1, 1], heads, **more)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (64, 32), (128, 64), (128, 32)])
+@pytest.mark.parametrize("heads", [2, 4, 10])
+@pytest.mark.parametrize("lengths,shared", [([60, 45, 8], False), ([9000, 45, 8], True)])
+def test_a_later_token_that_is_not_finite_does_not_reach_the_ones_before(dev, dim, group, heads, lengths, shared):  # noqa: F811
+    """Drafts: the last token's value is NaN; under a window, that of a key which only the first tokens see."""
+    f = Filled(dev, lengths, 2, dim, group, seed=heads)
+    assert _shared(f, 3, heads, 5) == shared
+    _spoil(f, 0, lengths[0] - 1, 0, 0)
+    _spoil(f, 1, 43, 1, dim // group - 1)
+    for mass in (False, True):
+        _beside(f, [5, 4, 3], heads, mass=mass)
+    _spoil(f, 0, lengths[0] - 23, 1, 0)
+    for mass in (False, True):
+        _beside(f, [5, 4, 3], heads, mass=mass, window=20)
