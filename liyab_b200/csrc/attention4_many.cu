@@ -699,7 +699,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
             // A row's result; where blocks share its keys a state, normed so that its sum is 1.  (Rows whose keys are one block's share have none.)
             const bool none = l == 0.0f, whole = ctl->whole != 0;                          // no key seen: O may be what the memory held
             float* state = c.partial + ((((int64_t)seq * kv + kvh) * c.max_rows + row) * n_splits + split) * (HD + 4);
-            if (!whole && there && x == 0) *reinterpret_cast<float2*>(state) = make_float2(none ? kLowest : m + log2f(l), none ? 0.0f : 1.0f);
+            if (!whole && there && x == 0) *reinterpret_cast<float4*>(state) = make_float4(none ? kLowest : m + log2f(l), none ? 0.0f : 1.0f, 0.0f, 0.0f);
             float factor = 1.0f;
             if (whole && c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
             factor = factor / l * ex2(big * 0.5f);
@@ -743,7 +743,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
 template <int HD>
 __global__ void __launch_bounds__(128)
 attention4_many_join_kernel(const Call c, int n_splits, int share) {
-    __shared__ float joined[1][HD + 2];
+    __shared__ float joined[1][HD + 3];
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
     const int seq = blockIdx.z, kvh = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 5);

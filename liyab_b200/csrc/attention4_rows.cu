@@ -9,10 +9,11 @@
 //   O^T += V^T p^T   mma.sync m16n8k16 on float16: rows are dims, n - 8 made of the nibbles exactly (w & 0x000f000f | 0x64006400 is 1024 + n of two values, less 1032); p times the value's
 //                    scale, rounded to float16, turned by movmatrix into the second operand.
 // What is rounded: p s to float16 (2^-12, or 2^-31 of the warp's largest value scale), and queries more than 2^6 below their row's largest (to 2^-15 of it); a row's 16 bits hold bfloat16's
-// eight of all others.  A power of two a row puts its largest at 2^14.  The values' scales have any size that bfloat16 has, so what p is relative to is the row's largest score plus the exponent
-// of the warp's largest value scale f (down to 2^-80), less 6: 2^(S - m) s is at most 2^14.  f leaves no trace in the result.  m moves when a score passes it by more than 2^8, or a scale f: the warp
-// votes, which costs a few instructions a pair where searching the maximum cost thirty a tile.  A scale that is NaN (of a group that was not finite) is no f and no factor: it would meet p = 0 of rows
-// that do not see its key.  It passes every f, so it is met where the warp has voted: its products are 0, and the sums of the rows that see it are NaN from there on.
+// eight of all others.  A power of two a row puts its largest at 2^14.  The values' scales have any size that bfloat16 has, so they are taken in units of 2^f, f the exponent of the warp's largest
+// (2^-120 at least), less 6: 2^(S - m) s is at most 2^14.  p takes 2^-f along as far as that leaves it and its sum well within float32's range, f in -40 .. 40; what is beyond, the scales are multiplied
+// by.  A state's sum is relative to m alone, and it carries f, which is O's.  m moves when a score passes it by more than 2^8, or a scale f: the warp votes, which costs a few instructions a pair where
+// searching the maximum cost thirty a tile.  A scale that is NaN (of a group that was not finite) is no f and no factor: it would meet p = 0 of rows that do not see its key.  It passes every f, so it
+// is met where the warp has voted: its products are 0, and the sums of the rows that see it are NaN from there on.
 //
 // Two ways to share the keys out (rows_plan chooses by an estimate of both).  WHOLE: a block has a request's row tile and key/value head, its eight warps a stretch of the keys each, whose states meet
 // in shared memory and become the result: no scratch memory, one launch.  Else all warps of the launch take equal shares of all tiles of all requests (256 at most to a launch row), wherever they
@@ -41,8 +42,9 @@ using namespace lb_c4;
 
 constexpr int kStages = 2;                     // pairs of tiles in a warp's ring
 constexpr float kSlack = 8.0f;                 // how far a score may pass its row's reference (base 2)
-constexpr float kLeastScale = -80.0f;          // the exponent of the largest value scale, before any
-constexpr float kRoom = 6.0f;                  // p s reaches 2^(kRoom + kSlack) = 2^14 of float16's 2^16; what lies 2^-30 below the largest scale loses bits
+constexpr int kLeastScale = -120;              // the exponent of the largest value scale, before any
+constexpr int kEven = 40;                      // of f, p has -kEven .. kEven
+constexpr int kRoom = 6;                       // p s reaches 2^(kRoom + kSlack) = 2^14 of float16's 2^16; what lies 2^-30 below the largest scale loses bits
 
 // 2^n, n in -126 .. 127.
 __device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
@@ -97,6 +99,11 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
         w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
 }
+// Two bfloat16 numbers times a power of two, exact but below the smallest normal number.
+__device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t by) {
+    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&by));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
 // bfloat16 number i of a run of words.
 __device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
 
@@ -147,7 +154,7 @@ template <int HD, int NG, int NT, bool PLAIN, bool WHOLE>
 __global__ void __launch_bounds__(warps_of(NT, WHOLE) * 32, blocks_per_sm(HD, NT, WHOLE))
 attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
     using L = Layout<HD>;
-    constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, two places, the values
+    constexpr int kRows = 4 * NT, kState = HD + 4;         // a state is a reference, a sum, the values' unit, a place, the values
     constexpr int JK = HD / 32, JV = HD / 64;             // words of a lane: of a key, of a value row
     constexpr int kBlock = block_bytes(HD, NG), kWarps = warps_of(NT, WHOLE);
     // The columns of V^T p^T: with four rows a pair of columns is a row times the scales of two groups, else two rows, an operand for each group.
@@ -334,7 +341,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             const uint32_t row_top = __shfl_sync(0xffffffffu, top, 8 * t);
             row_scale[n] = row_top >= 0x7f80u ? CUDART_NAN_F : c.scale * kLbLog2e * pow2(-sh / 2) * pow2(-sh - -sh / 2);
         }
-        // m: a row's largest score, or near it; ref: m + f, what scores are taken relative to; passes: m and the slack.
+        // m: a row's largest score, or near it; ref: m and p's share of f, what scores are taken relative to; passes: m and the slack.
         float m[NT], l[NT], ref[NT], passes[NT], o[VT][JV * 4][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) m[n] = ref[n] = passes[n] = kLowest, l[n] = 0.0f;
@@ -344,8 +351,9 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             for (int i = 0; i < JV * 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-        float f = kLeastScale - kRoom;
-        uint32_t f_bits = (uint32_t)(127 + (int)kLeastScale) << 7;              // 2^(f + kRoom) as bfloat16: no scale seen is larger
+        int f = kLeastScale - kRoom;
+        uint32_t most_bits = 0;                                                 // 2^(f + kRoom) as bfloat16: a scale that is larger moves f; 0 where every pair's scales are to be multiplied
+        auto share_of_p = [](int units) { return min(max(units, -kEven), kEven); };
         float r1[NT], r2[NT];
         int place[NT];
 #pragma unroll
@@ -452,26 +460,28 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             uint32_t top = __vmaxu2(vs[0][0], vs[1][0]);
 #pragma unroll
             for (int i = 1; i < NG; ++i) top = __vmaxu2(top, __vmaxu2(vs[0][i], vs[1][i]));
-            bool moved = (top >> 16) > f_bits || (top & 0xffffu) > f_bits;
+            bool moved = (top >> 16) > most_bits || (top & 0xffffu) > most_bits;
 #pragma unroll
             for (int n = 0; n < NT; ++n) moved = moved || fmaxf(fmaxf(z[n][0][0], z[n][0][1]), fmaxf(z[n][1][0], z[n][1][1])) > passes[n];
             if (__any_sync(0xffffffffu, moved)) {
-                // A scale that is NaN (it passes any f) is 0 in the products, and what the rows that see its key have of the group's dims becomes NaN, which no later factor or sum changes.
-                uint32_t nans = 0;                          // a bit a row and group
-                top = 0;
+                top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+                if (top >= 0x7f80u) {
+                    // A scale that is NaN is 0 in the products, and what the rows that see its key have of the group's dims becomes NaN, which no later factor or sum changes.
+                    uint32_t nans = 0;                          // a bit a row and group
+                    top = 0;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < 2 * NG; ++i) {
-                        const uint32_t half_word = i % 2 != 0 ? 0xffff0000u : 0x0000ffffu;
-                        if ((vs[u][i / 2] & half_word & 0x7fff7fffu) >= (0x7f807f80u & half_word)) {
-                            vs[u][i / 2] &= ~half_word;
+                        for (int i = 0; i < 2 * NG; ++i) {
+                            const uint32_t half_word = i % 2 != 0 ? 0xffff0000u : 0x0000ffffu;
+                            if ((vs[u][i / 2] & half_word & 0x7fff7fffu) >= (0x7f807f80u & half_word)) {
+                                vs[u][i / 2] &= ~half_word;
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) nans |= z[n][u][i / NG] != -CUDART_INF_F ? 1u << (n * NG + i % NG) : 0u;
+                                for (int n = 0; n < NT; ++n) nans |= z[n][u][i / NG] != -CUDART_INF_F ? 1u << (n * NG + i % NG) : 0u;
+                            }
+                            if (i % 2 != 0) top = __vmaxu2(top, vs[u][i / 2]);
                         }
-                        if (i % 2 != 0) top = __vmaxu2(top, vs[u][i / 2]);
-                    }
-                if (__any_sync(0xffffffffu, nans != 0)) {
+                    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) nans |= __shfl_xor_sync(0xffffffffu, nans, d);
 #pragma unroll
@@ -482,11 +492,16 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                             if ((nans >> (n * NG + gr) & 1u) != 0) o[n / 2][k][e] = o[n / 2][k][e + 2] = CUDART_NAN_F;
                         }
                 }
-                top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-                float f_new = f;
-                if (top > f_bits) {
-                    f_bits = (min(top, 0x7f00u) + 0x7fu) & 0x7f80u;         // the next power of two (2^127 at most)
-                    f_new = (float)((int)(f_bits >> 7) - 127) - kRoom;
+                const int f_old = f;
+                f = max(f, (int)((min(top, 0x7f00u) + 0x7fu) >> 7) - 127 - kRoom);             // the next power of two (2^127 at most)
+                const int of_p = share_of_p(f);
+                most_bits = f == of_p ? (uint32_t)(127 + kRoom + f) << 7 : 0;
+                if (f != of_p) {
+                    const uint32_t by = (uint32_t)(127 - (f - of_p)) * 0x00800080u;            // a power of two, twice
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) vs[u][i] = scaled(vs[u][i], by);
                 }
                 float corr[NT];
 #pragma unroll
@@ -495,11 +510,11 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
                     high = fmaxf(high, m[n]);
-                    corr[n] = ex2((m[n] - high) + (f - f_new));
+                    corr[n] = ex2((m[n] - high) + (float)(f_old - f));
+                    l[n] *= ex2((m[n] - high) + (float)(share_of_p(f_old) - of_p));
                     m[n] = high;
-                    ref[n] = high + f_new;
+                    ref[n] = high + (float)of_p;
                     passes[n] = high + kSlack;
-                    l[n] *= corr[n];
                 }
 #pragma unroll
                 for (int v = 0; v < VT; ++v)
@@ -507,7 +522,6 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                     for (int k = 0; k < JV * 4; ++k)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[v][k][e] *= NT == 1 ? corr[0] : corr[(2 * v + (e & 1)) % NT];
-                f = f_new;
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -561,7 +575,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         }
         if (gave_up) break;
 
-        // The run's state: m + f, the sum and the values of its rows.
+        // The run's state: m, the sum, f and the values of its rows.
         float* state = WHOLE ? states + warp * (kRows * kState) : c.partial + ((int64_t)blockIdx.y * (n_warps + (int64_t)per_row * kv * tiles) + me + ((int64_t)s * kv + kvh) * tiles + row_tile) * (kRows * kState);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -570,7 +584,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
             const int row = 4 * n + t;
             if (row >= rows_here) continue;
             float* to = state + row * kState;
-            if (g == 0) *reinterpret_cast<float2*>(to) = make_float2(ref[n], l[n]);
+            if (g == 0) *reinterpret_cast<float4*>(to) = make_float4(m[n], l[n] * pow2(share_of_p(f)), (float)f, 0.0f);
 #pragma unroll
             for (int j = 0; j < JV; ++j)
 #pragma unroll
@@ -603,7 +617,7 @@ template <int HD>
 __global__ void __launch_bounds__(1024)
 attention4_join_kernel(const Call c, int per_row, int n_warps, int tiles, int rows_shift, int team_shift) {
     constexpr int kState = HD + 4;
-    __shared__ float joined[32][HD + 2];
+    __shared__ float joined[32][HD + 3];
     const int kv = c.pages.n_kv_head, seq = blockIdx.z, kvh = blockIdx.y, row_of = seq < per_row ? 0 : seq / per_row, s = seq - row_of * per_row;
     const int r = blockIdx.x * (blockDim.x >> 5 >> team_shift) + (threadIdx.x >> 5 >> team_shift);
     lb_wait_for_predecessor();

@@ -9,7 +9,7 @@ import torch
 
 from liyab_b200 import ops
 from test_cache4 import _call
-from test_cache4_gpu import BF16, FORMS, Filled, _attention, _close, _queries, _slots, _values_as_rows
+from test_cache4_gpu import BF16, FORMS, Filled, _attention, _close, _decode, _portions, _queries, _slots, _values_as_rows
 from test_kernels_gpu import dev  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +90,34 @@ def test_a_later_token_that_is_not_finite_does_not_reach_the_ones_before(dev, di
     _spoil(f, 0, lengths[0] - 23, 1, 0)
     for mass in (False, True):
         _beside(f, [5, 4, 3], heads, mass=mass, window=20)
+
+
+@pytest.mark.parametrize("v_size", [3e37, 1e-34])
+@pytest.mark.parametrize("dim,group,heads", [(64, 64, 2), (64, 32, 10), (128, 32, 8), (128, 128, 2)])
+@pytest.mark.parametrize("lengths", [[200, 90], [9000, 40]])
+def test_values_of_the_largest_and_the_smallest_sizes(dev, lengths, dim, group, heads, v_size):  # noqa: F811
+    """The weights and their sums do not depend on the values' size, nor do the results' relative errors."""
+    f = Filled(dev, lengths, 2, dim, group, seed=heads, v_size=v_size)
+    _decode(f, heads, mass=True)
+    _decode(f, heads, window=150, sink=torch.zeros(heads, device=dev))
+    _portions(f, [5, 3], heads, mass=True)
+
+
+def _resize_values(f, i, power):
+    """Request i's values times 2^power[key]."""
+    f.v[i] = f.v[i] * torch.exp2(power.double())[:, None, None]
+    m = f.lengths[i]
+    ops.append4(*(_values_as_rows(x[i].flatten()).view(m, -1) for x in (f.k, f.v)), _slots(f.table.cpu(), i, m, f.cache.page_size).to(f.dev), f.cache, m)
+
+
+@pytest.mark.parametrize("dim,group,heads", [(64, 32, 2), (64, 64, 10), (128, 64, 8), (128, 32, 4)])
+@pytest.mark.parametrize("lengths", [[200, 90], [9000, 40]])
+@pytest.mark.parametrize("low,high", [(0, 122), (-110, 0), (-100, 120)])
+def test_values_of_sizes_far_apart(dev, lengths, dim, group, heads, low, high):  # noqa: F811
+    """Keys whose values are near the ends of float32's range beside others: states of very different units meet, and every key keeps its weight."""
+    f = Filled(dev, lengths, 2, dim, group, seed=heads, k_size=2.0)
+    gen = torch.Generator().manual_seed(heads)
+    for i, m in enumerate(lengths):
+        _resize_values(f, i, torch.where((torch.rand(m // 8 + 1, generator=gen) < 0.3).repeat_interleave(8)[:m], float(high), float(low)).to(dev))
+    _decode(f, heads, mass=True)
+    _portions(f, [5, 3], heads, mass=True)
