@@ -65,9 +65,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Sums of products of bytes, n + 8 by a query's digit.  kMagicBits: the bits of 1.5 2^23, after which integers up to 2^22 either way are the bits of that number plus themselves.
-constexpr int kMagicBits = 0x4b400000;
-constexpr float kMagic = 12582912.0f;
+constexpr float kMagic = 12582912.0f;          // 1.5 2^23
+// Sums of products of bytes, n + 8 by a query's digit.  kSumBits: the bits of 1.5 2^11, after which integers up to 2^22 either way are the bits of that number plus themselves in units of 2^-12: a sum,
+// 2^25 at most, times a key's scale stays within float32's range for scales up to 2^114 (in units of 1 up to 2^102).
+constexpr int kSumBits = 0x45400000, kSumUnit = 12;
+constexpr float kSum = 3072.0f;
 __device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, int c0, int c1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
@@ -282,7 +284,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 
         // The queries as the second operand: columns are (row, digit).  A row times a power of two, so that its largest is in 2^14 .. 2^15, is rounded to 16 bits, 256 high + low, both
         // -128 .. 127; lane (g, t) has digit g % 2 of the dims 32 j + 8 t .. + 7 of row g / 2, in the order of the nibbles of a key's word.  An operand's keys are n + 8, so the sums start
-        // at -8 times the digits' sum, and at the bits of 1.5 2^23: what they come to is a float's bits.
+        // at -8 times the digits' sum, and at the bits of 1.5 2^11: what they come to is a float's bits.
         uint32_t qd[NT][JK][2];
         int base[NT][NG][2];                                   // of columns 2 t and 2 t + 1: high and low digit of row t
         float row_scale[NT];
@@ -335,9 +337,9 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
 #pragma unroll
                 for (int j = gr * JK / NG; j < (gr + 1) * JK / NG; ++j) sum += sums[j];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) base[n][gr][e] = kMagicBits - 8 * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+                for (int e = 0; e < 2; ++e) base[n][gr][e] = kSumBits - 8 * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
             }
-            const int sh = __shfl_sync(0xffffffffu, shift, 8 * t);
+            const int sh = __shfl_sync(0xffffffffu, shift, 8 * t) - kSumUnit;
             const uint32_t row_top = __shfl_sync(0xffffffffu, top, 8 * t);
             row_scale[n] = row_top >= 0x7f80u ? CUDART_NAN_F : c.scale * kLbLog2e * pow2(-sh / 2) * pow2(-sh - -sh / 2);
         }
@@ -405,8 +407,8 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                     const float s0 = number(sc, gr), s1 = number(sc, NG + gr);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float k0 = fmaf(__int_as_float(a[n][0]) - kMagic, 256.0f, __int_as_float(a[n][1]) - kMagic);
-                        const float k1 = fmaf(__int_as_float(a[n][2]) - kMagic, 256.0f, __int_as_float(a[n][3]) - kMagic);
+                        const float k0 = fmaf(__int_as_float(a[n][0]) - kSum, 256.0f, __int_as_float(a[n][1]) - kSum);
+                        const float k1 = fmaf(__int_as_float(a[n][2]) - kSum, 256.0f, __int_as_float(a[n][3]) - kSum);
                         z[n][u][0] = gr == 0 ? k0 * s0 : fmaf(k0, s0, z[n][u][0]);
                         z[n][u][1] = gr == 0 ? k1 * s1 : fmaf(k1, s1, z[n][u][1]);
                     }

@@ -121,3 +121,16 @@ def test_values_of_sizes_far_apart(dev, lengths, dim, group, heads, low, high): 
         _resize_values(f, i, torch.where((torch.rand(m // 8 + 1, generator=gen) < 0.3).repeat_interleave(8)[:m], float(high), float(low)).to(dev))
     _decode(f, heads, mass=True)
     _portions(f, [5, 3], heads, mass=True)
+
+
+@pytest.mark.parametrize("k_size,q_size", [(1e34, 1e-34), (1e-36, 1e36)])
+@pytest.mark.parametrize("dim,group,heads", [(64, 64, 2), (64, 32, 10), (128, 32, 8), (128, 128, 2)])
+def test_keys_of_the_largest_and_the_smallest_sizes(dev, dim, group, heads, k_size, q_size):  # noqa: F811
+    """Keys far from 1 whose scores are ordinary numbers, in the kernel for few rows, both ways, and in the one for many."""
+    for lengths in ([200, 90], [9000, 40]):
+        f = Filled(dev, lengths, 2, dim, group, seed=heads, k_size=k_size)
+        _decode(f, heads, mass=True, size=q_size)
+        _portions(f, [5, 3], heads, size=q_size)
+    f = Filled(dev, [400, 300], 1, dim, group, seed=heads, k_size=k_size)
+    assert _shared(f, 2, 16, 300) is None
+    _portions(f, [300, 257], 16, size=q_size)
