@@ -874,8 +874,8 @@ int64_t lb_attention4_scratch(const lb_attention4_args* args);
 int lb_attention4_plan(const lb_attention4_args* args, int* plan);
 /* Tests: in the next call's attention kernel what it waits for (a pair's second tile; a group's scores) is never announced, so that its bounded waits run out. */
 int lb_attention4_withhold_next(int on);
-/* Eviction: of request s's n_keys[s] keys, key/value head h keeps the `recent` newest and, of the others, those with the largest mass[s][h][key] (equal ones: the lowest
- * places; a NaN counts as the largest), `keep` in all, or all where there are no more.  They are copied, in their order, to the places 0, 1, .. of the pages that
+/* Eviction: of request s's n_keys[s] keys, key/value head h keeps those of the `recent` last places and, of the others, those with the largest mass[s][h][key] (equal ones: the
+ * lowest places; a NaN counts as the largest), `keep` in all, or all where there are no more.  Keys on pages that are not there do not stay.  They are copied, in their order, to the places 0, 1, .. of the pages that
  * dest_table[s] names (pages that no source table of the call names), kept[s][h][i] is the place that the i-th came from (-1 past the last) and
  * dest_mass[s][h][i] its mass (0 past the last), i < keep.  mass and dest_mass have rows r = mass_rows[s], or s. */
 typedef struct {

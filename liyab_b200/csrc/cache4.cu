@@ -303,8 +303,9 @@ struct Choice {
     const int32_t* n_keys;
     int32_t* kept;
     float* dest_mass;
+    const int32_t* table;
     int64_t mass_stride, mass_head_stride, dest_stride, dest_head_stride;
-    int keep, recent, max_keys, n_mass, n_dest_mass;
+    int keep, recent, max_keys, n_mass, n_dest_mass, table_stride, page_shift, n_pages;
 };
 
 // A barrier of the cluster's threads (`blocks` 1: of the block's), and a pair of numbers in block r's shared memory.
@@ -324,6 +325,8 @@ __device__ __forceinline__ uint2 of_block(const uint32_t* here, int r) {
 }
 
 // `blocks` blocks, a cluster, share a request's and head's keys: their counts meet in each other's shared memory.
+// Keys on pages that are not there do not stay: of the old keys their place in the order is 0, below every number's, and no more stay than are there; of the newest they are left out, and as many more
+// of the old ones stay.
 // (1,024 threads also for few keys: 1 request of 2,048, 12 heads, 14.9 us in all; with 512 16.6, with 256 23.2, as the passes wait for shared memory.)
 template <bool SHARED>
 __global__ void __launch_bounds__(kChoiceThreads)
@@ -336,6 +339,8 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
     __shared__ __align__(8) uint32_t kept_here[2];          // keys of this block above the threshold, and at it
     __shared__ uint32_t sums[THREADS / 32];
     __shared__ uint32_t found[2];              // the bin that holds the last key to stay, and how many of it stay
+    __shared__ int gone[2];                    // how many of the old keys, and of the newest, are not there
+    if (threadIdx.x < 2) gone[threadIdx.x] = 0;
     lb_wait_for_predecessor();
     lb_dependents_may_launch();
     const int head = blockIdx.x / blocks, rank = blockIdx.x - head * blocks, n_head = gridDim.x / blocks, seq = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -345,8 +350,11 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
     const float* mass = c.mass + (weighed ? (int64_t)r * c.mass_stride + (int64_t)head * c.mass_head_stride : 0);
     int32_t* kept = c.kept + ((int64_t)seq * n_head + head) * c.keep;
     float* dest = c.dest_mass != nullptr && (unsigned)r < (unsigned)c.n_dest_mass ? c.dest_mass + (int64_t)r * c.dest_stride + (int64_t)head * c.dest_head_stride : nullptr;
-    const int stay = min(n, c.keep), old = n - min(c.recent, n);
-    const int by_weight = stay - (n - old);           // of the `old` first keys; recent <= keep, so never negative
+    const int old = n - min(c.recent, n);
+    const int32_t* table = c.table + (int64_t)seq * c.table_stride;
+    auto absent = [&](int key) { return (unsigned)table[key >> c.page_shift] >= (unsigned)c.n_pages; };
+    const int n_table = (n + (1 << c.page_shift) - 1) >> c.page_shift;
+    int page = (int)threadIdx.x < n_table ? table[threadIdx.x] : 0;               // (asked for ahead of the weights, and looked at behind them)
     // The block's stretch of the old keys.
     const int share = ((old + blocks - 1) / blocks + 31) / 32 * 32, lo = min(old, rank * share), mine = min(old, lo + share) - lo, in_shared = min(mine, held);
     for (int i0 = threadIdx.x; i0 < in_shared; i0 += 4 * THREADS) {
@@ -357,8 +365,22 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
         for (int j = 0; j < 4; ++j)
             if (i0 + j * THREADS < in_shared) keys_s[i0 + j * THREADS] = ordered(v[j]);
     }
+    for (int i = 4 * threadIdx.x; i < kBins; i += 4 * THREADS) *reinterpret_cast<uint4*>(both[0] + i) = make_uint4(0, 0, 0, 0);
+    asm volatile("" : "+r"(page) : : "memory");
     __syncthreads();
-    auto key_at = [&](int i) { return i < held ? keys_s[i] : weighed ? ordered(mass[lo + i]) : 0x80000000u; };
+#pragma unroll 1
+    for (int p = threadIdx.x; p < n_table; p += THREADS) {
+        if (p >= THREADS) page = table[p];
+        if ((unsigned)page >= (unsigned)c.n_pages) {
+            const int first = p << c.page_shift, end = min(first + (1 << c.page_shift), n);
+            for (int i = max(first - lo, 0); i < min(end - lo, in_shared); ++i) keys_s[i] = 0;
+            if (first < old) atomicAdd(&gone[0], min(end, old) - first);
+            if (end > old) atomicAdd(&gone[1], end - max(first, old));
+        }
+    }
+    __syncthreads();
+    const int new_there = n - old - gone[1], by_weight = min(old - gone[0], c.keep - new_there), stay = by_weight + new_there;         // recent <= keep, so by_weight is never negative
+    auto key_at = [&](int i) { return i < held ? keys_s[i] : absent(lo + i) ? 0u : weighed ? ordered(mass[lo + i]) : 0x80000000u; };
     // The sum of what the warps before this one left.
     auto before = [&](const uint32_t* of_warps) { return __reduce_add_sync(0xffffffffu, lane < warp ? of_warps[lane] : 0u); };
     // The by_weight-th largest key among the first `old`: `threshold` its prefix so far, `left` how many keys with that prefix stay.
@@ -371,8 +393,10 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
             low -= bits;
             const uint32_t mask = (1u << bits) - 1u, prefix = pass == 0 ? 0u : threshold >> high;
             uint32_t* bins = both[pass & 1];
-            for (int i = 4 * threadIdx.x; i < kBins; i += 4 * THREADS) *reinterpret_cast<uint4*>(bins + i) = make_uint4(0, 0, 0, 0);
-            __syncthreads();
+            if (pass > 0) {
+                for (int i = 4 * threadIdx.x; i < kBins; i += 4 * THREADS) *reinterpret_cast<uint4*>(bins + i) = make_uint4(0, 0, 0, 0);
+                __syncthreads();
+            }
             // Many weights are 0: they are counted in a register and enter with one addition a warp.
             uint32_t zeros = 0;
             auto enter = [&](uint32_t key) {
@@ -388,6 +412,8 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) enter(key[j]);
             }
+            for (; i < in_shared; i += THREADS) enter(keys_s[i]);
+#pragma unroll 1
             for (; i < mine; i += THREADS) enter(key_at(i));
             zeros = __reduce_add_sync(0xffffffffu, zeros);
             if (zeros != 0 && lane == 0) atomicAdd(&bins[0x80000000u >> low & mask], zeros);
@@ -424,7 +450,7 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
             threshold |= found[0] << low;
             left = found[1];
         }
-    } else if (by_weight <= 0) {
+    } else if (by_weight == 0) {
         threshold = 0xffffffffu;       // none stays by its weight
         left = 0;
     } else {
@@ -432,12 +458,15 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
     }
     // A warp has a stretch of the keys: it counts those above the threshold and those at it, the warps' counts meet, and it writes its own.
     const int stretch = (mine + THREADS - 1) / THREADS * 32, from = min(mine, warp * stretch), to = min(mine, from + stretch);
+    const int to_shared = min(to, held);
     uint32_t above = 0, at = 0;
-    for (int i = from + lane; i < to; i += 32) {
-        const uint32_t key = key_at(i);
+    auto count = [&](uint32_t key) {
         above += key > threshold;
         at += key == threshold;
-    }
+    };
+    for (int i = from + lane; i < to_shared; i += 32) count(keys_s[i]);
+#pragma unroll 1
+    for (int i = max(from, held) + lane; i < to; i += 32) count(key_at(i));
     above = __reduce_add_sync(0xffffffffu, above);
     at = __reduce_add_sync(0xffffffffu, at);
     uint32_t* counts = both[1];                // (the last pass's are the other; no block reads these any more)
@@ -460,9 +489,7 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
         }
     }
     place += min(ties, left);
-    for (int i0 = from; i0 < to; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key = i < to ? key_at(i) : 0;
+    auto write = [&](int i, uint32_t key) {
         const bool tie = i < to && key == threshold;
         const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
         const uint32_t below = (1u << lane) - 1u;
@@ -475,9 +502,27 @@ evict4_choose_kernel(const Choice c, int held, int n_blocks) {
         }
         place += __popc(mask);
         ties += __popc(tie_mask);
+    };
+    for (int i0 = from; i0 < to_shared; i0 += 32) write(i0 + lane, i0 + lane < to ? keys_s[i0 + lane] : 0);
+#pragma unroll 1
+    for (int i0 = max(from, held); i0 < to; i0 += 32) write(i0 + lane, i0 + lane < to ? key_at(i0 + lane) : 0);
+    // The newest, in their order; where some are not there a warp goes through them.
+    if (gone[1] != 0 && rank == 0 && warp == 0) {
+        int p = by_weight;
+        for (int k0 = old; k0 < n; k0 += 32) {
+            const int key = k0 + lane;
+            const bool there = key < n && !absent(key);
+            const uint32_t mask = __ballot_sync(0xffffffffu, there);
+            if (there) {
+                const int i = p + __popc(mask & ((1u << lane) - 1u));
+                kept[i] = key;
+                if (dest != nullptr) dest[i] = weighed ? mass[key] : 0.0f;
+            }
+            p += __popc(mask);
+        }
     }
-    for (int i = max(by_weight, 0) + rank * THREADS + threadIdx.x; i < c.keep; i += blocks * THREADS) {
-        const int key = old + i - max(by_weight, 0);
+    for (int i = (gone[1] != 0 ? stay : by_weight) + rank * THREADS + threadIdx.x; i < c.keep; i += blocks * THREADS) {
+        const int key = old + i - by_weight;
         const bool there = i < stay;
         kept[i] = there ? key : -1;
         if (dest != nullptr) dest[i] = there && weighed ? mass[key] : 0.0f;
@@ -632,8 +677,8 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
     LB_CHECK_ARG(a.dest_mass == nullptr || a.dest_mass != a.mass, "evict4: the kept keys' weights go to memory of their own");
     if (int rc = device_check("evict4", a.cache->device)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
-    const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
-                      a.n_mass, a.n_dest_mass};
+    const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.block_table, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
+                      a.n_mass, a.n_dest_mass, a.table_stride, pages.page_shift, pages.n_pages};
     // A block a request and head up to 8,192 keys (8 x 8,192 keys, 8 heads: 38.9 us, by two blocks each 39.8, whose barriers cost what they save); for more as many as there are SMs for (1 x 131,072
     // keys, 8 heads: 57 us by eight blocks each, 230 by one).
     int blocks = 1;

@@ -1587,7 +1587,7 @@ def prefill_attention4(q: torch.Tensor, cache: Cache4, q_start: torch.Tensor, n_
 def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys: torch.Tensor, n_seq: int, keep: int, recent: int, dest_table: torch.Tensor, kept: torch.Tensor,
            dest_mass: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Leaves each request and key/value head `keep` of its n_keys[s] keys: the `recent` newest and, of the others, those with the largest `mass` (as decode_attention4 adds it up; equal ones:
-    the lowest places).  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
+    the lowest places); none that lies on a page outside the cache.  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
     they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (memory of its own, not mass)."""
     index, page = cache.index, cache.page_size
     table_at, table_stride, columns = _table4("evict4", "block_table", block_table, index, n_seq, 1)

@@ -134,3 +134,62 @@ def test_keys_of_the_largest_and_the_smallest_sizes(dev, dim, group, heads, k_si
     f = Filled(dev, [400, 300], 1, dim, group, seed=heads, k_size=k_size)
     assert _shared(f, 2, 16, 300) is None
     _portions(f, [300, 257], 16, size=q_size)
+
+
+def _evict_with_holes(f, table, mass, keep, recent, mass_rows=None):
+    """evict4 of requests some of whose pages are not in the cache beside what api.h says: of the keys that are there the last `recent` places' and then those with the largest weights; nothing else is
+    named as kept, and nothing else's destination is written."""
+    n, page, dev = len(f.lengths), f.cache.page_size, f.dev  # noqa: F811
+    per = -(-keep // page)
+    dest = f.spare[:n * per].view(n, per).to(dev)
+    kept, dest_mass = torch.full((n, f.kv, keep), 77, dtype=torch.int32, device=dev), torch.full((mass.shape[0], f.kv, keep), 7.5, device=dev)
+    size = f.cache.memory.numel() // f.cache.n_pages
+    f.cache.memory.view(-1, size)[dest.long().view(-1)] = 255                    # scales that are NaN
+    before = f.cache.memory.clone()
+    n_keys = torch.tensor(f.lengths, dtype=torch.int32, device=dev)
+    ops.evict4(f.cache, mass, table, n_keys, n, keep, recent, dest, kept, dest_mass, mass_rows=mass_rows)
+    stays = torch.zeros(n, dtype=torch.int32)
+    for i, m in enumerate(f.lengths):
+        key, r = torch.arange(m, device=dev), i if mass_rows is None else int(mass_rows[i])
+        pages = table[i, key // page]
+        there = (pages >= 0) & (pages < f.cache.n_pages)
+        for h in range(f.kv):
+            new = key[there & (key >= m - recent)]
+            old = key[there & (key < m - recent)]
+            w = mass[r, h][old].double()
+            first = old[torch.sort(w, descending=True, stable=True).indices[:keep - len(new)]]
+            want = torch.cat([first, new]).sort().values
+            stay = len(want)
+            assert torch.equal(kept[i, h, :stay].long(), want) and (kept[i, h, stay:] == -1).all()
+            assert torch.equal(dest_mass[r, h, :stay], mass[r, h][want]) and (dest_mass[r, h, stay:] == 0).all()
+            stays[i] = stay
+            slots = _slots(dest.cpu(), i, keep, page)[:stay].to(dev)
+            k, v = (torch.zeros(stay, f.kv * f.dim, device=dev) for _ in range(2))
+            ops.cache4_values(f.cache, slots, stay, k, v)
+            assert torch.equal(k.view(stay, f.kv, f.dim)[:, h], f.k[i][want, h].float()) and torch.equal(v.view(stay, f.kv, f.dim)[:, h], f.v[i][want, h].float())
+    untouched = torch.ones(f.cache.n_pages, dtype=torch.bool)
+    untouched[dest.cpu().long().view(-1)] = False
+    assert torch.equal(f.cache.memory.view(-1, size)[untouched], before.view(-1, size)[untouched])
+    return dest, stays
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("lengths,keep,recent", [([400, 330, 70], 100, 30), ([500, 64, 0], 64, 64), ([900, 40, 333], 300, 0), ([20000], 300, 100), ([20000, 9000], 12000, 11000), ([70001], 4000, 17)])
+def test_evict_of_requests_with_pages_that_are_not_there(dev, lengths, keep, recent, page):  # noqa: F811
+    """Keys on pages outside the cache do not stay, in what blocks of one and of several share, past what a block holds, among the newest and the others; attention over what stayed is attention over those
+    keys."""
+    n = len(lengths)
+    f = Filled(dev, lengths, 2, 64, 32, page, seed=keep, extra=n * -(-keep // page))
+    gen = torch.Generator().manual_seed(keep)
+    mass = torch.exp(2 * torch.randn(n, 2, f.table.shape[1] * page, generator=gen)).to(dev)
+    for holes in (0.0, 0.1, 0.9, 1.0):
+        table = torch.where(torch.rand(f.table.shape, generator=gen).to(dev) < holes, torch.tensor([-1, 1 << 29, f.pages, -(1 << 31)], dtype=torch.int32)[torch.randint(0, 4, f.table.shape, generator=gen)].to(dev), f.table)
+        dest, stays = _evict_with_holes(f, table, mass, keep, recent)
+        _evict_with_holes(f, table, (mass * 2).floor(), keep, recent)
+        _evict_with_holes(f, table, torch.full_like(mass, -math.inf), keep, recent)
+    for i, m in enumerate(lengths):                       # one page of the newest keys, one of the first
+        if m:
+            table = f.table.clone()
+            table[:, 0] = -1
+            table[i, (m - 1) // page] = f.pages
+            _evict_with_holes(f, table, mass, keep, recent)
