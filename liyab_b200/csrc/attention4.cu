@@ -99,11 +99,14 @@ int check(const lb_attention4_args* args, Call* c, Plan* p) {
     const int64_t units = (int64_t)a.n_seq * a.cache->n_kv_head;
     // (Under a window a request's rows see no more keys than it and the portion have, and what rounds them to tiles.)
     const int seen = a.window == 0 ? keys : (int)std::min<int64_t>(keys, std::abs((int64_t)a.window) + a.max_q_len + 2 * lb_c4::kBlockKeys);
-    if (int rc = rows_plan(&p->rows, a.n_seq, a.cache->n_kv_head, (int)rows, seen, a.cache->head_dim, n_sm)) return rc;
+    p->rows = rows_plan(a.n_seq, a.cache->n_kv_head, (int)rows, seen, a.cache->head_dim, n_sm);
     p->tiles = tiles_plan(a.n_seq, a.cache->n_kv_head, c->per, (int)rows, keys, a.window, a.cache->head_dim, n_sm);
     // The tcgen05 kernel takes a call where the estimates (rows_plan, tiles_plan), which are from both kernels' times on 84 calls of 1 to 128 tokens a request, say so: 8 requests on 2,048 keys, 32 heads
     // over 8: 8 tokens each 34 us on the kernel for few rows, 36 on this; 16 tokens 52 / 36; 1 request on 2,048 keys: 32 tokens 20 / 24, 128 tokens 51 / 32.
     p->many = a.total == nullptr && p->tiles.us < p->rows.us;
+    // (The tcgen05 kernel takes 2^42 pairs of a query row and a key in some three seconds.  Under a window a tile of 256 rows walks that many keys, its rows' own and what rounds them.)
+    const int64_t walked = a.window == 0 ? keys : std::min<int64_t>(keys, std::abs((int64_t)a.window) + 512);
+    LB_CHECK_ARG(p->many ? a.cache->n_kv_head * rows * walked <= (int64_t)1 << 42 : p->rows.fits, "attention4: a request of %d rows and %d keys is more than one launch takes", (int)rows, keys);
     p->scores = 0;
     p->log_sums = a.total != nullptr ? up(units * rows * keys * 4) : 0;
     p->partial = p->log_sums + (a.total != nullptr ? up(units * rows * 4) : 0);

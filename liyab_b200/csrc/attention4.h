@@ -60,11 +60,12 @@ int allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {
 // states, bytes of the states and of the requests' starts.
 struct RowsPlan {
     int rows, tiles, per_row, blocks, join_team;
+    bool fits;                      // whether it can run at all
     bool whole;                     // a block for each request's row tiles and key/value heads
     double us;                      // about how long it takes
     int64_t states, starts;
 };
-int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
+RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm);
 // Portions of many rows, on tcgen05: blocks that may share a row tile's keys, tiles of 128 keys each has at most, bytes of their states, about how long it takes.
 struct TilesPlan {
     int splits, share;

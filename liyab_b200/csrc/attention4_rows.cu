@@ -34,6 +34,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 namespace lb_a4 {
 namespace {
@@ -676,13 +677,17 @@ int launch_for(const Call& c, const RowsPlan& p, cudaStream_t s) {
 
 }  // namespace
 
-int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
-    RowsPlan& p = *plan;
+RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int head_dim, int n_sm) {
+    RowsPlan p = {};
     p.rows = max_rows > 4 ? 8 : 4;
     p.tiles = (max_rows + p.rows - 1) / p.rows;
-    // A launch row numbers its tiles in 32 bits.
+    // A launch row numbers its tiles in 32 bits: a request of more is not this kernel's.
     const int64_t units = (int64_t)n_kv_head * p.tiles, most = units * ((max_keys + kBlockKeys - 1) / kBlockKeys);
-    LB_CHECK_ARG(most <= 1 << 30, "attention4: a request of %d rows and %d keys is more than one launch takes", max_rows, max_keys);
+    p.fits = most <= 1 << 30;
+    if (!p.fits) {
+        p.us = std::numeric_limits<double>::infinity();
+        return p;
+    }
     p.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)std::max(1, n_seq), (int64_t)kMostRequests, ((int64_t)1 << 30) / std::max<int64_t>(1, most)}));
     const int kWarps = warps_of(p.rows / 4, false);
     const int64_t warps = std::min<int64_t>((int64_t)n_sm * blocks_per_sm(head_dim, p.rows / 4, false) * kWarps, (most * p.per_row + kLeastTiles - 1) / kLeastTiles);
@@ -709,7 +714,7 @@ int rows_plan(RowsPlan* plan, int n_seq, int n_kv_head, int max_rows, int max_ke
     p.whole = whole_us < 0.8 * shared_us;
     p.us = std::min(whole_us, shared_us);
     if (p.whole) p.states = p.starts = 0;
-    return LB_OK;
+    return p;
 }
 
 int few_rows(const Call& c, int head_dim, const RowsPlan& p, cudaStream_t s) {

@@ -193,3 +193,16 @@ def test_evict_of_requests_with_pages_that_are_not_there(dev, lengths, keep, rec
             table[:, 0] = -1
             table[i, (m - 1) // page] = f.pages
             _evict_with_holes(f, table, mass, keep, recent)
+
+
+def test_a_whole_prompt_that_the_kernel_for_few_rows_does_not_number(dev):  # noqa: F811
+    n, kv, heads = 131072, 4, 16
+    f = Filled(dev, [n], kv, 64, 64, 128, seed=1)
+    q = _queries(f, n, heads, 0)
+    out = torch.full((n + 1, heads * 64), 7.5, dtype=BF16, device=dev)
+    start, past = torch.tensor([0, n], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    ops.prefill_attention4(q, f.cache, start, past, f.table, out, 1, n, heads, 0.125)
+    tokens = torch.tensor([0, 1, 255, 256, 40000, 65535, 65536, 100001, n - 1], device=dev)
+    want, _, bound, _ = _attention(q[tokens].view(-1, heads, 64), f.k[0], f.v[0], tokens, 0.125, many=True)
+    _close(out[tokens].view(-1, heads, 64), want, bound)
+    assert not out.isnan().any() and (out[n] == 7.5).all()
