@@ -712,7 +712,7 @@ RowsPlan rows_plan(int n_seq, int n_kv_head, int max_rows, int max_keys, int hea
     // (The estimates take every request to be as long as the longest.  Where they are not, sharing gains and a block's own keys do not: 16 requests of 2,048 keys on average and 4,096 at most 38 us and
     // 30.  So a block has its own keys only where that is clearly the shorter.)
     p.whole = whole_us < 0.8 * shared_us;
-    p.us = std::min(whole_us, shared_us);
+    p.us = p.whole ? whole_us : shared_us;
     if (p.whole) p.states = p.starts = 0;
     return p;
 }

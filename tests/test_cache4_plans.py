@@ -25,3 +25,9 @@ def test_long_prompts_are_the_kernel_for_many_rows_s():
     assert _plan(1, 4096, 1, 1 << 20, 64)[0] == 1
     assert _plan(1, 4096, 1, 1 << 20, 64, mass=AT, total=AT) is None and b"more than one launch" in ops.lib().lb_last_error()
     assert _plan(1, 4096, 1, 1 << 18, 64, mass=AT, total=AT)[0] == 0
+
+
+def test_the_kernel_is_chosen_by_the_time_of_the_way_that_runs():
+    """Calls whose keys all warps share out although a block to a row tile is estimated to be a bit shorter: it is the time of what would run that the other kernel's is compared with."""
+    assert _plan(2, 8, 8, 4096, 16, dim=64)[:2] == (1, 256) and _plan(12, 12, 2, 4096, 48)[:2] == (1, 256)
+    assert _plan(2, 8, 8, 4096, 4, dim=64)[0] == 0
