@@ -844,7 +844,8 @@ int lb_cache4_values(int dtype, const lb_cache4* cache, const int32_t* slots, in
  * has the tokens q_start[s] .. q_start[s + 1] - 1, the first at place last[s].  A token sees the keys up to its own place under `window` (as in lb_paged_attention_generic); one that sees
  * none has an output of zeros.  Query head h reads key/value head h / (n_head / n_kv_head).
  * total (or null): total[r][kv head][key] = mass[r][kv head][key] + the sum, over the request's tokens and the heads of the key/value head, of the softmax weights of that key,
- * for the keys up to the newest; r = mass_rows[s], or s.  total may be mass.  Portions of up to 64 tokens. */
+ * for the keys up to the newest; r = mass_rows[s], or s (no row twice).  total's rows of max_keys numbers do not overlap; they are mass's, or share no number with them.  Portions of
+ * up to 64 tokens. */
 typedef struct {
     const lb_cache4* cache;
     const void* q;              /* bfloat16 [tokens, n_head * head_dim] */
@@ -877,7 +878,8 @@ int lb_attention4_withhold_next(int on);
 /* Eviction: of request s's n_keys[s] keys, key/value head h keeps those of the `recent` last places and, of the others, those with the largest mass[s][h][key] (equal ones: the
  * lowest places; a NaN counts as the largest), `keep` in all, or all where there are no more.  Keys on pages that are not there do not stay.  They are copied, in their order, to the places 0, 1, .. of the pages that
  * dest_table[s] names (pages that no source table of the call names), kept[s][h][i] is the place that the i-th came from (-1 past the last) and
- * dest_mass[s][h][i] its mass (0 past the last), i < keep.  mass and dest_mass have rows r = mass_rows[s], or s. */
+ * dest_mass[s][h][i] its mass (0 past the last), i < keep.  mass and dest_mass have rows r = mass_rows[s], or s (no row twice); dest_mass's do not overlap, and share no number with
+ * mass's. */
 typedef struct {
     const lb_cache4* cache;
     const float* mass;

@@ -126,6 +126,38 @@ int check(const lb_attention4_args* args, Call* c, Plan* p) {
 
 }  // namespace
 
+namespace lb_a4 {
+
+bool rows_apart(const WeightRows& a) {
+    if (a.n <= 0) return true;
+    if ((a.heads > 1 && a.head < a.width) || (a.n > 1 && a.row < a.width)) return false;
+    return a.heads <= 1 || a.n <= 1 || a.row >= (a.heads - 1) * a.head + a.width || a.head >= (a.n - 1) * a.row + a.width;
+}
+
+bool rows_disjoint(const WeightRows& a, const WeightRows& b) {
+    if (a.n <= 0 || b.n <= 0 || a.width <= 0 || b.width <= 0) return true;
+    auto stride = [](int64_t s, int64_t n) { return n > 1 ? s : 0; };                       // (that of a single row is any number)
+    auto first = [](const WeightRows& w) { return (int64_t)(reinterpret_cast<uintptr_t>(w.at) / sizeof(float)); };
+    auto last = [&](const WeightRows& w) { return first(w) + stride(w.row, w.n) * (w.n - 1) + stride(w.head, w.heads) * (w.heads - 1) + w.width - 1; };
+    if (last(a) < first(b) || last(b) < first(a)) return true;
+    const int64_t row = std::max(stride(a.row, a.n), stride(b.row, b.n)), head = std::max(stride(a.head, a.heads), stride(b.head, b.heads));
+    if ((a.n > 1 && a.row != row) || (b.n > 1 && b.row != row) || (a.heads > 1 && a.head != head) || (b.heads > 1 && b.head != head)) return false;
+    // A row of b starts at x, counted from one of a's: dr rows and dh heads on.  They overlap where -b.width < x < a.width.
+    for (int64_t dh = 1 - a.heads; dh < b.heads; ++dh) {
+        const int64_t x = first(b) - first(a) + dh * head;
+        if (row == 0) {
+            if (x > -b.width && x < a.width) return false;
+        } else {
+            // The least dr that takes x past -b.width.
+            const int64_t short_of = 1 - b.width - x, dr = std::max(1 - a.n, short_of >= 0 ? (short_of + row - 1) / row : -(-short_of / row));
+            if (dr < b.n && x + dr * row < a.width) return false;
+        }
+    }
+    return true;
+}
+
+}  // namespace lb_a4
+
 extern "C" int64_t lb_attention4_scratch(const lb_attention4_args* args) {
     Call c;
     Plan p;
@@ -155,6 +187,14 @@ extern "C" int lb_attention4(const lb_attention4_args* args) {
     const int64_t width = (int64_t)a.n_head * a.cache->head_dim;
     LB_CHECK_ARG(a.n_tokens < 2 || (a.q_stride >= width && a.out_stride >= width), "attention4: rows overlap");
     LB_CHECK_ARG(p.bytes == 0 || (a.scratch != nullptr && reinterpret_cast<uintptr_t>(a.scratch) % 16 == 0), "attention4: scratch memory is missing or not 16-byte aligned");
+    if (a.total != nullptr) {
+        const int64_t n = a.n_mass, heads = a.cache->n_kv_head, keys = c.score_keys;
+        const WeightRows mass = {a.mass, a.mass_stride, a.mass_head_stride, n, heads, keys}, total = {a.total, a.total_stride, a.total_head_stride, n, heads, keys};
+        LB_CHECK_ARG(rows_apart(total), "attention4: the keys' weights go to rows that overlap (%lld and %lld numbers apart, of %d keys)", (long long)a.total_stride, (long long)a.total_head_stride,
+                     c.score_keys);
+        const bool same = a.total == a.mass && (n <= 1 || a.total_stride == a.mass_stride) && (heads <= 1 || a.total_head_stride == a.mass_head_stride);
+        LB_CHECK_ARG(same || rows_disjoint(mass, total), "attention4: the keys' weights go to memory that overlaps where they come from, and is not the same");
+    }
     if (int rc = device_check("attention4", a.cache->device)) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
     c.withhold = g_withhold_next;

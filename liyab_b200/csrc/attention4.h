@@ -44,6 +44,16 @@ __device__ __forceinline__ Portion portion_of(const Call& c, int s) {
     return p;
 }
 
+// Rows of weights in memory: [n][heads][width] floats, `row` and `head` from one to the next (host).
+struct WeightRows {
+    const float* at;
+    int64_t row, head, n, heads, width;
+};
+// Whether no two of the rows overlap: one of the strides has the rows of the other between two of its own.
+bool rows_apart(const WeightRows& a);
+// Whether no number is in both.  (Rows of the same strides may lie between each other's; of other strides they do not share a stretch of memory.)
+bool rows_disjoint(const WeightRows& a, const WeightRows& b);
+
 // Lets a kernel have this much dynamic shared memory: asked once a device (a question costs as much as half a launch).
 template <typename Kernel>
 int allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& asked) {

@@ -674,7 +674,11 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
                  "evict4: weights of no size");
     if (a.n_seq == 0) return LB_OK;
     LB_CHECK_ARG(a.mass != nullptr && a.block_table != nullptr && a.n_keys != nullptr && a.dest_table != nullptr && a.kept != nullptr, "evict4: a pointer is missing");
-    LB_CHECK_ARG(a.dest_mass == nullptr || a.dest_mass != a.mass, "evict4: the kept keys' weights go to memory of their own");
+    const lb_a4::WeightRows mass = {a.mass, a.mass_stride, a.mass_head_stride, a.n_mass, pages.n_kv_head, a.max_keys};
+    const lb_a4::WeightRows dest_mass = {a.dest_mass, a.dest_stride, a.dest_head_stride, a.n_dest_mass, pages.n_kv_head, a.keep};
+    LB_CHECK_ARG(a.dest_mass == nullptr || (a.dest_mass != a.mass && lb_a4::rows_disjoint(mass, dest_mass)), "evict4: the kept keys' weights go to memory of their own");
+    LB_CHECK_ARG(a.dest_mass == nullptr || lb_a4::rows_apart(dest_mass), "evict4: the kept keys' weights go to rows that overlap (%lld and %lld numbers apart, of %d keys)", (long long)a.dest_stride,
+                 (long long)a.dest_head_stride, a.keep);
     if (int rc = device_check("evict4", a.cache->device)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(a.stream);
     const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.block_table, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,

@@ -1569,7 +1569,7 @@ def decode_attention4(q: torch.Tensor, cache: Cache4, positions: torch.Tensor, b
     """Attention of one new token per request (row i of q is request i's, its newest key at positions[i]; -1: no keys, a row of zeros) over the pages of a 4-bit cache.  `window`,
     `distance`, `sink`, `soft_cap`: as for paged_attention_generic.  `max_keys`: the most keys a request has (0: what the block table holds); none past it is read.
     `mass` (float32 [rows, n_kv_head, keys]): total[r, h, key] = mass[r, h, key] + the softmax weights that the key got from the query heads of h, for the keys up to the newest; r is
-    the request's number or mass_rows[request] (no row twice in a call); `total` None: back into mass."""
+    the request's number or mass_rows[request] (no row twice in a call); `total` None: back into mass.  Rows of total do not overlap each other, nor, if they are not the same, mass's."""
     if q.dim() == 2 and not 0 <= n_seq <= q.shape[0]:
         raise invalid_argument(f"decode_attention4: {n_seq} requests, {q.shape[0]} rows of q")
     return _attention4("decode_attention4", q, cache, None, positions, block_table, out, n_seq, 1, n_head, scale, window, mass, total, mass_rows, distance, sink, soft_cap, max_keys)
@@ -1588,7 +1588,8 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
            dest_mass: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Leaves each request and key/value head `keep` of its n_keys[s] keys: the `recent` newest and, of the others, those with the largest `mass` (as decode_attention4 adds it up; equal ones:
     the lowest places); none that lies on a page outside the cache.  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
-    they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (memory of its own, not mass)."""
+    they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (rows
+    that overlap neither each other nor mass's).  mass and dest_mass have the request's row, or mass_rows[request] (no row twice in a call)."""
     index, page = cache.index, cache.page_size
     table_at, table_stride, columns = _table4("evict4", "block_table", block_table, index, n_seq, 1)
     dest_at, dest_stride, _ = _table4("evict4", "dest_table", dest_table, index, n_seq, max(1, -(-keep // page)))

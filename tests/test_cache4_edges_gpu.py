@@ -206,3 +206,40 @@ def test_a_whole_prompt_that_the_kernel_for_few_rows_does_not_number(dev):  # no
     want, _, bound, _ = _attention(q[tokens].view(-1, heads, 64), f.k[0], f.v[0], tokens, 0.125, many=True)
     _close(out[tokens].view(-1, heads, 64), want, bound)
     assert not out.isnan().any() and (out[n] == 7.5).all()
+
+
+def test_weights_in_memory_that_is_shared(dev):  # noqa: F811
+    """Rows of weights that lie between another tensor's give what rows of their own do; rows that overlap are refused, and nothing is written."""
+    from liyab_b200.status import LiyabError
+    kv, heads, n = 2, 4, 3
+    f = Filled(dev, [100, 40, 77], kv, 64, 64, seed=1, extra=3 * 4)
+    cells, keep, q = f.table.shape[1] * 16, 50, _queries(f, n, heads, 0)
+    places, out = torch.tensor([m - 1 for m in f.lengths], dtype=torch.int32, device=dev), torch.empty(n, heads * 64, dtype=BF16, device=dev)
+    n_keys, dest, kept = places + 1, f.spare[:12].view(3, 4).to(dev), torch.empty(n, kv, keep, dtype=torch.int32, device=dev)
+    mass = torch.rand(n, kv, cells, generator=torch.Generator().manual_seed(2)).to(dev)
+
+    def run(mass, total, dest_mass):
+        ops.decode_attention4(q, f.cache, places, f.table, out, n, heads, 0.125, mass=mass, total=total)
+        ops.evict4(f.cache, mass if total is None else total, f.table, n_keys, n, keep, 5, dest, kept, dest_mass)
+
+    total, dest_mass = torch.zeros_like(mass), torch.zeros(n, kv, keep, device=dev)
+    run(mass, total, dest_mass)
+    for shape, pick in (((2, n, kv, cells), 0), ((n, 2, kv, cells), 1), ((n, kv, 2, cells), 2)):
+        buffer = torch.zeros(shape, device=dev)
+        a, b = buffer.select(pick, 0), buffer.select(pick, 1)
+        a.copy_(mass)
+        run(a, b, dest_mass_2 := torch.zeros(n, kv, keep, device=dev))
+        assert torch.equal(b, total) and torch.equal(a, mass) and torch.equal(dest_mass_2, dest_mass)
+        ops.evict4(f.cache, b, f.table, n_keys, n, keep, 5, dest, kept, a[:, :, :keep])
+        assert torch.equal(a[:, :, :keep], dest_mass)
+    wide = torch.zeros(n, kv, cells + 1, device=dev)
+    wide[:, :, :cells] = mass
+    before = wide.clone()
+    shared = torch.zeros(1, kv, cells, device=dev)
+    for bad in (lambda: run(mass, shared.expand(n, -1, -1), dest_mass), lambda: run(mass, torch.zeros(n, 1, cells, device=dev).expand(-1, kv, -1), dest_mass),
+                lambda: run(shared.expand(n, -1, -1), None, dest_mass), lambda: run(wide[:, :, :cells], wide[:, :, 1:], dest_mass), lambda: run(wide[:, :, 1:], wide[:, :, :cells], dest_mass),
+                lambda: ops.evict4(f.cache, wide, f.table, n_keys, n, keep, 5, dest, kept, wide[:, :, 1:1 + keep]),
+                lambda: ops.evict4(f.cache, wide, f.table, n_keys, n, keep, 5, dest, kept, torch.zeros(1, kv, keep, device=dev).expand(n, -1, -1))):
+        with pytest.raises(LiyabError):
+            bad()
+    assert torch.equal(wide, before) and not shared.any()
