@@ -873,7 +873,7 @@ int64_t lb_attention4_scratch(const lb_attention4_args* args);
 /* How a call is cut: plan[0] 0 by the kernel for few rows, 1 by the one for many; plan[1] query rows a tile; plan[2] blocks, or
  * those that share a tile's keys; plan[3] requests that the blocks share. */
 int lb_attention4_plan(const lb_attention4_args* args, int* plan);
-/* Tests: in the next call's attention kernel what it waits for (a pair's second tile; a group's scores) is never announced, so that its bounded waits run out. */
+/* Tests: in the calling thread's next call's attention kernel what it waits for (a pair's second tile; a group's scores) is never announced, so that its bounded waits run out. */
 int lb_attention4_withhold_next(int on);
 /* Eviction: of request s's n_keys[s] keys, key/value head h keeps those of the `recent` last places and, of the others, those with the largest mass[s][h][key] (equal ones: the
  * lowest places; a NaN counts as the largest), `keep` in all, or all where there are no more.  Keys on pages that are not there do not stay.  They are copied, in their order, to the places 0, 1, .. of the pages that

@@ -46,7 +46,7 @@ attention4_mass_kernel(const Call c, const Mass w) {
 }
 
 constexpr int kMostMassTokens = 64;
-int g_withhold_next = 0;            // the next call's kernels leave barriers unsignalled (tests)
+thread_local int g_withhold_next = 0;            // this thread's next call's kernels leave barriers unsignalled (tests)
 
 // How a call runs.
 struct Plan {
@@ -208,7 +208,7 @@ extern "C" int lb_attention4(const lb_attention4_args* args) {
     return LB_OK;
 }
 
-// Tests: the next call's waits run out.
+// Tests: the waits of this thread's next call run out.
 extern "C" int lb_attention4_withhold_next(int on) {
     g_withhold_next = on;
     return LB_OK;
