@@ -11,7 +11,7 @@
 // Numbers: a row of queries is float16 after a power of two that puts its largest at 2^14; n s after one for the block of sixteen keys that puts its largest scale at 2^8, which the scores, and p, are
 // multiplied by again (for p relative to the largest block's so far, F, which O is in units of).  So K, V and p are rounded to float16 (2^-12), and bfloat16's range is kept.
 // A value scale that is NaN would meet p = 0 of rows that do not see its key in the products: such groups are made zeros, and the rows that see them take a note (a bit a group) and end as NaN.
-// Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results.
+// Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results, once the products that it asked for are through.
 // What bounds it.  A block alone on an SM (204 KB) gets through 256 rows by 64 keys in 1.46 us for heads of 128 (838 TFLOP/s over 148 SMs; 0.51 of cuBLAS's burst) and 1.30 for heads of 64 (469): its
 // schedulers issue in 71 % of all cycles, exponentials, conversions and the largest score of a row above all (16 softmax warps), the makers' nibbles after them.  Leaving the makers' work out, or the
 // exponentials, saved less than a tenth, as did turns that keep the groups half a unit apart: no one part is the bound.  A soft cap adds 36 % (4 x 512 tokens behind 8,192 keys, 32 heads over 8 of 128,
@@ -49,6 +49,7 @@ struct Control {
     uint64_t q_full;
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t s_full[kGroups][2], p_full[kGroups][2], o_done[kGroups][2];       // of units in turn: what waits may be a unit behind, and a parity tells no more than two phases apart
+    uint64_t drained[kGroups];                                             // of a group that gave up: the products under way are through
     uint32_t tmem_base;
     int abort_flag, whole;                                                 // whole: the block has all keys of its rows
     float k_factor[kNotes][kMakers], v_exponent[kNotes][kMakers];          // of a tile's blocks of sixteen keys
@@ -287,6 +288,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
             mbar_init(&ctl->p_full[i / 2][i % 2], kSoftmaxWarps / kGroups);
             mbar_init(&ctl->o_done[i / 2][i % 2], 1);
         }
+        for (int i = 0; i < kGroups; ++i) mbar_init(&ctl->drained[i], 1);
         ctl->abort_flag = 0;
         ctl->whole = all_tiles <= share;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -354,7 +356,13 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
             if (ok && (u & 1) == 1 && elect_one()) umma_commit(&ctl->v_empty[st]);
             __syncwarp();
         }
-        if (!ok) give_up(ctl, status, 3);
+        if (!ok) {
+            // Products that are under way read shared memory and write tensor memory: they end (bounded as well) before the block gives either back.
+            give_up(ctl, status, 3);
+            if (elect_one()) umma_commit(&ctl->drained[g]);
+            __syncwarp();
+            mbar_wait(&ctl->drained[g], 0, nullptr);
+        }
     } else if (warp >= kMaker) {
         // ---- makers
         const int b = warp - kMaker, g = lane >> 2, t = lane & 3;
