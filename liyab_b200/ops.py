@@ -1432,6 +1432,8 @@ class Cache4:
     __slots__ = ("n_pages", "n_kv_head", "head_dim", "page_size", "group", "device", "index", "memory", "args", "ref", "scratch")
 
     def __init__(self, n_pages: int, n_kv_head: int, head_dim: int, page_size: int = 16, group: int = 64, device="cuda"):
+        if not all(0 <= x < 1 << 31 for x in (n_pages, n_kv_head, head_dim, page_size, group)):
+            raise invalid_argument(f"cache4: {n_pages} pages of {page_size} keys, {n_kv_head} heads of {head_dim} values, groups of {group}")
         size = ctypes.c_int64(0)
         check(lib().lb_cache4_bytes(n_pages, n_kv_head, head_dim, page_size, group, ctypes.byref(size)), "cache4")
         self.n_pages, self.n_kv_head, self.head_dim, self.page_size, self.group = n_pages, n_kv_head, head_dim, page_size, group
@@ -1528,6 +1530,8 @@ def _attention4(what: str, q: torch.Tensor, cache: Cache4, q_start: Optional[tor
     table_at, table_stride, table_columns = _table4(what, "block_table", block_table, index, n_seq, 1)
     start_at = 0 if q_start is None else _ints4(what, "q_start", q_start, index, n_seq + 1)
     keys = table_columns * cache.page_size
+    if max_keys < 0 or max(keys, max_q_len, abs(window)) >= 1 << 31:
+        raise invalid_argument(f"{what}: up to {max_keys} keys of {keys}, portions of up to {max_q_len} tokens, a window of {window}")
     if 0 < max_keys < keys:
         keys = max_keys
     mass_at = total_at = rows_at = n_mass = 0
@@ -1591,6 +1595,8 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
     they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (rows
     that overlap neither each other nor mass's).  mass and dest_mass have the request's row, or mass_rows[request] (no row twice in a call)."""
     index, page = cache.index, cache.page_size
+    if not (0 < keep < 1 << 31 and 0 <= recent <= keep):
+        raise invalid_argument(f"evict4: keep {keep} keys, {recent} of them the newest")
     table_at, table_stride, columns = _table4("evict4", "block_table", block_table, index, n_seq, 1)
     dest_at, dest_stride, _ = _table4("evict4", "dest_table", dest_table, index, n_seq, max(1, -(-keep // page)))
     mass_at, n_mass, keys, mass_stride, mass_head = _weights_of4("evict4", "mass", mass, cache, 1)
@@ -1606,5 +1612,5 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
     elif n_mass < n_seq or (dest_mass is not None and n_dest < n_seq):
         raise invalid_argument(f"evict4: {n_seq} requests, weights of {n_mass}{'' if dest_mass is None else f' and {n_dest}'}")
     check(lib().lb_evict4(_evict4_args(cache.ref, mass_at, rows_at, table_at, n_keys_at, dest_at, kept.data_ptr(), dest_mass_at, stream_of(index), mass_stride, mass_head, dest_mass_stride,
-                                       dest_head, table_stride, dest_stride, n_seq, keep, recent, min(columns * page, keys), n_mass, n_dest)), "evict4")
+                                       dest_head, table_stride, dest_stride, n_seq, keep, recent, min(columns * page, keys, (1 << 31) - 1), n_mass, n_dest)), "evict4")
     return kept

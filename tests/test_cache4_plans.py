@@ -4,8 +4,10 @@ from __future__ import annotations
 import ctypes as C
 
 import pytest
+import torch
 
 from liyab_b200 import ops
+from liyab_b200.status import LiyabError
 from test_cache4 import AT, _cache, _call, _evict
 
 
@@ -78,3 +80,24 @@ def test_weights_of_single_rows_have_any_stride():
         weights = dict(mass=AT, mass_stride=1, mass_head=5, total=AT, total_stride=strides[0], total_head=strides[1], n_mass=1)
         rc = ops.lib().lb_attention4(_call(ref, n_head=4, n_seq=1, n_tokens=1, max_keys=64, scratch=AT, **weights))
         assert rc != 0 and b"overlap" not in ops.lib().lb_last_error()
+
+
+def test_numbers_that_no_call_holds_are_refused(monkeypatch):
+    """Sizes past 32 bits and negative ones are refused as the other arguments are, by `ops`, before the library is asked."""
+    class Sizes:
+        n_kv_head, head_dim, page_size, group, index, device, n_pages, ref, scratch = 2, 64, 1 << 20, 64, -1, torch.device("cpu"), 4, 0, {}
+    monkeypatch.setattr(ops, "stream_of", lambda index: 0)
+    monkeypatch.setattr(ops, "lib", lambda: pytest.fail("the library was asked"))
+    cache, i32 = Sizes(), torch.int32
+    rows, places, table = torch.zeros(3, 128, dtype=torch.bfloat16), torch.zeros(4, dtype=i32), torch.zeros(3, 4, dtype=i32)
+    wide = torch.zeros(3, 1, dtype=i32).expand(3, 2048)                                        # 2^31 keys
+    weights, kept = torch.zeros(3, 2, 64), torch.zeros(3, 2, 16, dtype=i32)
+    for call in (lambda: ops.decode_attention4(rows, cache, places, table, rows, 3, 2, 0.1, max_keys=-1), lambda: ops.decode_attention4(rows, cache, places, table, rows, 3, 2, 0.1, window=1 << 40),
+                 lambda: ops.decode_attention4(rows, cache, places, table, rows, 3, 2, 0.1, window=-(1 << 31)),
+                 lambda: ops.decode_attention4(rows, cache, places, wide.contiguous(), rows, 3, 2, 0.1),
+                 lambda: ops.prefill_attention4(rows, cache, places, places, table, rows, 3, 1 << 31, 2, 0.1),
+                 lambda: ops.evict4(cache, weights, table, places, 3, 0, 0, table, kept[:, :, :0]), lambda: ops.evict4(cache, weights, table, places, 3, 16, -1, table, kept),
+                 lambda: ops.evict4(cache, weights, table, places, 3, 16, 17, table, kept), lambda: ops.evict4(cache, weights, table, places, 3, 16, 1 << 32, table, kept),
+                 lambda: ops.Cache4((1 << 32) + 1, 2, 64), lambda: ops.Cache4(4, 2, 64 + (1 << 32)), lambda: ops.Cache4(-1, 2, 64)):
+        with pytest.raises(LiyabError):
+            call()
