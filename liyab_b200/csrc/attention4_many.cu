@@ -19,9 +19,8 @@
 // twice as long a chain.  A block takes 9 us to start (queries, first keys, tensor memory) and end; 2 x 1,024 tokens, 12 heads of 64: 28 us, of which 16 units of keys are 20.
 #include "attention4.h"
 #include "attention4_join.cuh"
-#include "tcgen05.cuh"
+#include "attention4_parts.cuh"
 
-#include <cuda_fp16.h>
 #include <float.h>
 #include <math_constants.h>
 
@@ -68,30 +67,12 @@ template <int N>
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-__device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-__device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
-template <int BYTES>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-    if constexpr (BYTES == 16) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (BYTES == 8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x; w[1] = u.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-}
 // A word's values times s as four float16 pairs: nibbles (i, i + 4).
 __device__ __forceinline__ void scaled_pairs(uint32_t w, __half2 s, uint32_t (&r)[4]) {
-    const __half2 offset = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f), offset16 = __float2half2_rn(-72.0f);
-    const uint32_t hi = w >> 8;
-    r[0] = h2(__hmul2(__hadd2(as_h2((w & 0x000f000fu) | 0x64006400u), offset), s));
-    r[1] = h2(__hmul2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, offset16), s));
-    r[2] = h2(__hmul2(__hadd2(as_h2((hi & 0x000f000fu) | 0x64006400u), offset), s));
-    r[3] = h2(__hmul2(__hfma2(as_h2((hi & 0x00f000f0u) | 0x64006400u), sixteenth, offset16), s));
+    __half2 n[4];
+    pairs_of(w, n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = h2(__hmul2(n[i], s));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
@@ -154,19 +135,6 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
                    "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                  :: "memory");
-}
-
-// A bounded wait, one answer for the warp.  Most find the phase done: one question then (mbar_wait's loop is 90 cycles of a warp that has the SM for itself, this 30).
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "vote.sync.all.pred q, p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok != 0) return true;
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
 // Two multiply-adds, two additions, and the largest of three in one instruction each.

@@ -26,9 +26,8 @@
 // second against 32.0; twice the blocks for the third 47 against 38.7; tiles of sixteen rows lose to two of eight, as their registers leave half the warps; a third pair in the ring changes nothing.
 #include "attention4.h"
 #include "attention4_join.cuh"
-#include "tcgen05.cuh"
+#include "attention4_parts.cuh"
 
-#include <cuda_fp16.h>
 #include <float.h>
 #include <math_constants.h>
 
@@ -47,20 +46,6 @@ constexpr int kLeastScale = -120;              // the exponent of the largest va
 constexpr int kEven = 40;                      // of f, p has -kEven .. kEven
 constexpr int kRoom = 6;                       // p s reaches 2^(kRoom + kSlack) = 2^14 of float16's 2^16; what lies 2^-30 below the largest scale loses bits
 
-// 2^n, n in -126 .. 127.
-__device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-
-// A word's values as four float16 pairs: r[i] = nibbles (i, i + 4) less 8.
-__device__ __forceinline__ void pairs_of(uint32_t w, uint32_t (&r)[4]) {
-    const __half2 offset = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f), offset16 = __float2half2_rn(-72.0f);
-    const uint32_t hi = w >> 8;
-    r[0] = h2(__hadd2(as_h2((w & 0x000f000fu) | 0x64006400u), offset));
-    r[1] = h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, offset16));         // (1024 + 16 n) / 16 - 72
-    r[2] = h2(__hadd2(as_h2((hi & 0x000f000fu) | 0x64006400u), offset));
-    r[3] = h2(__hfma2(as_h2((hi & 0x00f000f0u) | 0x64006400u), sixteenth, offset16));
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -90,26 +75,11 @@ __device__ __forceinline__ void copy_block(void* to, const void* from, uint32_t 
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(lb_tc::smem_u32(to)), "l"(from), "r"(bytes), "r"(lb_tc::smem_u32(bar)) : "memory");
 }
-template <int BYTES>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-    if constexpr (BYTES == 16) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (BYTES == 8) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x; w[1] = u.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-}
 // Two bfloat16 numbers times a power of two, exact but below the smallest normal number.
 __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t by) {
     const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&by));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
-// bfloat16 number i of a run of words.
-__device__ __forceinline__ float number(const uint32_t* w, int i) { return __uint_as_float((i & 1) != 0 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); }
-
 // A block's warps.
 __host__ __device__ constexpr int warps_of(int nt, bool whole) { return whole || nt == 1 ? 8 : 4; }
 constexpr int kMostRequests = 256;             // of a launch row (grid.y)
@@ -136,19 +106,6 @@ struct Request {
 __host__ __device__ __forceinline__ int share_of(int total, int n_warps) {
     const int even = (total + n_warps - 1) / n_warps;
     return even > kLeastTiles ? even : kLeastTiles;
-}
-
-// A bounded wait, one answer for the warp; most find the phase done.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "vote.sync.all.pred q, p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(ok) : "r"(lb_tc::smem_u32(bar)), "r"(parity) : "memory");
-    if (ok != 0) return true;
-    return __all_sync(0xffffffffu, lb_tc::mbar_wait(bar, parity, nullptr));
 }
 
 // NG groups of scales a head, NT tiles of 4 query rows (two digits each).  PLAIN: no soft cap, no penalty by distance, no scores written.  WHOLE: a block has one request's (blockIdx.y) row tile
@@ -377,7 +334,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
         while (done < run_end) {
             // A pair of tiles; where the run begins or ends within one, the other of its two is masked.
             const int pair = done >> 1;
-            if (!wait(&bars[warp][stage], parity)) {               // bounded; one answer for the warp
+            if (!wait(&bars[warp][stage], parity, nullptr)) {               // bounded; one answer for the warp
                 gave_up = true;
                 break;
             }
@@ -555,7 +512,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                 load_words<L::kPiece>(block + u * kBlock + L::kV + 32 * L::kPiece + at, y);
 #pragma unroll
                 for (int j = 0; j < JV; ++j) {
-                    uint32_t a0[4], a1[4], a2[4], a3[4];
+                    __half2 a0[4], a1[4], a2[4], a3[4];
                     pairs_of(__byte_perm(x[j], x[JV + j], 0x5410), a0);
                     pairs_of(__byte_perm(x[j], x[JV + j], 0x7632), a1);
                     pairs_of(__byte_perm(y[j], y[JV + j], 0x5410), a2);
@@ -564,7 +521,7 @@ attention4_rows_kernel(const Call c, int per_row, int tiles, int* status) {
                     for (int k = 0; k < 4; ++k) {
                         const int gr = (64 * j + 32 * (k >> 1)) / (HD / NG), x2 = NT == 1 ? gr / 2 : gr;
 #pragma unroll
-                        for (int v = 0; v < VT; ++v) mma_f16(o[v][j * 4 + k], a0[k], a1[k], a2[k], a3[k], pf[v][x2][0], pf[v][x2][1]);
+                        for (int v = 0; v < VT; ++v) mma_f16(o[v][j * 4 + k], h2(a0[k]), h2(a1[k]), h2(a2[k]), h2(a3[k]), pf[v][x2][0], pf[v][x2][1]);
                     }
                 }
             }
