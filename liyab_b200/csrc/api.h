@@ -842,7 +842,8 @@ int lb_append4(int dtype, const void* k, int64_t ldk, const void* v, int64_t ldv
 int lb_cache4_values(int dtype, const lb_cache4* cache, const int32_t* slots, int n, void* k, int64_t ldk, void* v, int64_t ldv, void* stream);
 /* Attention over a 4-bit cache.  Decode (q_start null): token i is request i's, its newest key at place last[i] (-1: no keys; the output row is zeros).  Portions: request s
  * has the tokens q_start[s] .. q_start[s + 1] - 1, the first at place last[s].  A token sees the keys up to its own place under `window` (as in lb_paged_attention_generic); one that sees
- * none has an output of zeros.  Query head h reads key/value head h / (n_head / n_kv_head).
+ * none has an output of zeros.  Windows and distances go by the places of keys in the table (after an eviction those of the keys that stayed, not their tokens' positions).  Query
+ * head h reads key/value head h / (n_head / n_kv_head).
  * total (or null): total[r][kv head][key] = mass[r][kv head][key] + the sum, over the request's tokens and the heads of the key/value head, of the softmax weights of that key,
  * for the keys up to the newest; r = mass_rows[s], or s (no row twice).  total's rows of max_keys numbers do not overlap; they are mass's, or share no number with them.  Portions of
  * up to 64 tokens. */

@@ -18,7 +18,7 @@ struct Mass {
 };
 
 // total = mass + the sum over a request's rows of 2^(score - log_sum), a thread a key.  The rows come in their order, so the sum does not depend on the launch.  The scores come from the attention
-// kernel by way of memory, a row's 32-bit numbers a key, as a weight needs its row's whole sum: a launch, and 4 bytes a row and key each way (16 requests of 4,096 keys at most, with attention 29.7 us).
+// kernel by way of memory, a row's 32-bit numbers a key, as a weight needs its row's whole sum: a launch, and 4 bytes a row and key each way (16 requests of 4,096 keys at most, with attention 29.8 us).
 __global__ void __launch_bounds__(256)
 attention4_mass_kernel(const Call c, const Mass w) {
     lb_wait_for_predecessor();

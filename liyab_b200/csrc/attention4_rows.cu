@@ -21,7 +21,7 @@
 //
 // What bounds it.  A block of sixteen keys takes some 257 instructions for heads of 128 with four rows, most of them on the pipe for integers and halves at two cycles each, so the GPU gets through
 // 5.1 TB/s of cache (heads of 64: 4.3), 0.78 of the copy bandwidth, after a start of 8 us (requests, block tables, first keys, queries: four trips to memory, and the launch)
-// and before a join of 3 to 6.  8 requests on 16,384 keys, 32 heads over 8 of 128: 37 us, 3.8 TB/s; 64 on 1,024, 25 heads of 64: 31 us; 1 on 131,072: 37; 1 on 512, 25 heads of 64: 5.3.
+// and before a join of 3 to 6.  8 requests on 16,384 keys, 32 heads over 8 of 128: 38 us, 3.8 TB/s; 64 on 1,024, 25 heads of 64: 31.5 us; 1 on 131,072: 38; 1 on 512, 25 heads of 64: 5.5.
 // Float16 products for K as well, a tile at a time, took 67 us for the first, with a block to a range of one request's keys.  Five blocks of four warps an SM for heads of 64, not four: 34.8 us for the
 // second against 32.0; twice the blocks for the third 47 against 38.7; tiles of sixteen rows lose to two of eight, as their registers leave half the warps; a third pair in the ring changes nothing.
 #include "attention4.h"

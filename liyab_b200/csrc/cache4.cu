@@ -5,9 +5,9 @@
 // out in 16 us (85 MB, 5.3 TB/s).
 // evict4 is two launches.  The first chooses: a block (a cluster of up to eight for more than 8,192 keys) a request and key/value head finds the weight of the last key that stays by a radix selection over the
 // weights as ordered integers (three passes over 11, 11 and 10 bits), then every warp counts its stretch of the keys and writes those that stay in their order.  It is bound by the passes' chains of
-// barriers and, for long requests, by their instructions on the SMs that have a request and head (from cold memory 12 x 2,048 keys 9.3 us, 64 x 8,192 keys 14; with zeros counted by votes
-// and one key a step 17).  The second copies: a warp a block of sixteen keys of the
-// destination, whose pieces it gathers, all asked for before the first is stored (64 x 2,048 keys of 128 dims, 36 MB read and written, 10.4 us; a piece at a time 12.2).  The destination is never
+// barriers and, for long requests, by their instructions on the SMs that have a request and head (from cold memory 12 x 2,048 keys 11.0 us, 64 x 8,192 keys 16;
+// without a look at the pages 9.3 and 14; with zeros counted by votes and one key a step 17 then).  The second copies: a warp a block of sixteen keys of the
+// destination, whose pieces it gathers, all asked for before the first is stored (64 x 2,048 keys of 128 dims, 36 MB read and written, 11 us; a piece at a time 12.2).  The destination is never
 // a source, so nothing waits for anything.
 #include "attention4.h"
 #include "cache4.cuh"
@@ -684,7 +684,7 @@ extern "C" int lb_evict4(const lb_evict4_args* args) {
     const Choice c = {a.mass, a.mass_rows, a.n_keys, a.kept, a.dest_mass, a.block_table, a.mass_stride, a.mass_head_stride, a.dest_stride, a.dest_head_stride, a.keep, a.recent, a.max_keys,
                       a.n_mass, a.n_dest_mass, a.table_stride, pages.page_shift, pages.n_pages};
     // A block a request and head up to 8,192 keys (8 x 8,192 keys, 8 heads: 38.9 us, by two blocks each 39.8, whose barriers cost what they save); for more as many as there are SMs for (1 x 131,072
-    // keys, 8 heads: 57 us by eight blocks each, 230 by one).
+    // keys, 8 heads: 56 us by eight blocks each, 230 by one).
     int blocks = 1;
     while (blocks < 8 && (int64_t)pages.n_kv_head * a.n_seq * blocks * 2 <= linear4_sm_count() && a.max_keys > 8192 * blocks) blocks *= 2;
     const int held = std::min(((a.max_keys + blocks - 1) / blocks + 31) / 32 * 32, kMostHeld);

@@ -1571,7 +1571,8 @@ def decode_attention4(q: torch.Tensor, cache: Cache4, positions: torch.Tensor, b
                       mass: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None, distance: Optional[torch.Tensor] = None,
                       sink: Optional[torch.Tensor] = None, soft_cap: float = 0.0, max_keys: int = 0) -> torch.Tensor:
     """Attention of one new token per request (row i of q is request i's, its newest key at positions[i]; -1: no keys, a row of zeros) over the pages of a 4-bit cache.  `window`,
-    `distance`, `sink`, `soft_cap`: as for paged_attention_generic.  `max_keys`: the most keys a request has (0: what the block table holds); none past it is read.
+    `distance`, `sink`, `soft_cap`: as for paged_attention_generic; windows and distances go by the keys' places.
+    `max_keys`: the most keys a request has (0: what the block table holds); none past it is read.
     `mass` (float32 [rows, n_kv_head, keys]): total[r, h, key] = mass[r, h, key] + the softmax weights that the key got from the query heads of h, for the keys up to the newest; r is
     the request's number or mass_rows[request] (no row twice in a call); `total` None: back into mass.  Rows of total do not overlap each other, nor, if they are not the same, mass's."""
     if q.dim() == 2 and not 0 <= n_seq <= q.shape[0]:
@@ -1584,7 +1585,8 @@ def prefill_attention4(q: torch.Tensor, cache: Cache4, q_start: torch.Tensor, n_
                        distance: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None, soft_cap: float = 0.0, max_keys: int = 0) -> torch.Tensor:
     """Causal attention of portions of up to `max_q_len` tokens per request over the pages of a 4-bit cache, which holds the portions' own keys already: request s has the rows
     q_start[s] .. q_start[s + 1] - 1 of q, the first at place n_past[s].  The other arguments as for decode_attention4; with `mass` portions of up to 64 tokens (the weights of all of
-    a portion's tokens are added up)."""
+    a portion's tokens are added up; 4 bytes of scratch memory a query head, token and key).  Tokens are cut as if every request had `max_q_len`: single tokens beside a long portion are a call of
+    decode_attention4."""
     return _attention4("prefill_attention4", q, cache, q_start, n_past, block_table, out, n_seq, max_q_len, n_head, scale, window, mass, total, mass_rows, distance, sink, soft_cap, max_keys)
 
 
@@ -1592,8 +1594,8 @@ def evict4(cache: Cache4, mass: torch.Tensor, block_table: torch.Tensor, n_keys:
            dest_mass: Optional[torch.Tensor] = None, mass_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Leaves each request and key/value head `keep` of its n_keys[s] keys: the `recent` newest and, of the others, those with the largest `mass` (as decode_attention4 adds it up; equal ones:
     the lowest places); none that lies on a page outside the cache.  They are copied in their order to the places 0, 1, .. of the pages of dest_table, which no block table of the call names (the old pages may be shared: they stay as
-    they were).  kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (rows
-    that overlap neither each other nor mass's).  mass and dest_mass have the request's row, or mass_rows[request] (no row twice in a call)."""
+    they were).  There attention's windows and distances go by the new places, not by the positions that the keys had.
+    kept (int32 [n_seq, n_kv_head, keep]): where each came from, -1 past the last; dest_mass: its weight, 0 past the last (rows that overlap neither each other nor mass's).  mass and dest_mass have the request's row, or mass_rows[request] (no row twice in a call)."""
     index, page = cache.index, cache.page_size
     if not (0 < keep < 1 << 31 and 0 <= recent <= keep):
         raise invalid_argument(f"evict4: keep {keep} keys, {recent} of them the newest")
