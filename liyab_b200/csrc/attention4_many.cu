@@ -2,14 +2,15 @@
 //
 // The query rows of a request that share a key/value head (its tokens' heads, in the order of the tokens) are cut into tiles of 256; a block has a tile, as two groups of 128 rows, and walks the
 // keys 128 at a time.  Both groups read the same keys and values, which eight warps make from the cache's nibbles:
-//   warps 0..15   softmax, two threads a row: p = 2^(S - m) as float16 back into tensor memory over the scores it came from, and O rescaled where m moved.
+//   warps 0..15   softmax, two threads a row: p = 2^(S - m + 7) as float16 back into tensor memory over the scores it came from, and O rescaled where m moved.
 //   warps 16..23  makers: a warp has a block of sixteen keys.  The nibbles of the next tile are on their way while this one's become n s as float16, in the 128-byte swizzle that tcgen05 reads.
 //   warps 24, 25  issue tcgen05.mma, one for each group: S = Q K^T (128 x 128), O += P V (64 values at a time, V as it lies, [key][dim]: the "MN-major" form).
 // Tensor memory: the groups' scores (and p, in the first half of their columns), then the groups' O.  A group's next scores are asked for once its update has read p; meanwhile the other group is at
 // its exponentials, so the two take turns at the tensor cores and at the special-function units (a tile's 2 x 16,384 exponentials take those 2,048 cycles, its products for heads of 128 the tensor
 // cores 2,048).
 // Numbers: a row of queries is float16 after a power of two that puts its largest at 2^14; n s after one for the block of sixteen keys that puts its largest scale at 2^8, which the scores, and p, are
-// multiplied by again (for p relative to the largest block's so far, F, which O is in units of).  So K, V and p are rounded to float16 (2^-12), and bfloat16's range is kept.
+// multiplied by again (for p relative to the largest block's so far, F, which O is in units of).  So K, V and p are rounded to float16 (2^-12, p of weights below 2^-21 of
+// the row's largest to 2^-32 of it; without the factor of 2^7 it would be 2^-25, which 131,072 keys beside one that takes most of the weight made 2 % of the rest), and bfloat16's range is kept.
 // A value scale that is NaN would meet p = 0 of rows that do not see its key in the products: such groups are made zeros, and the rows that see them take a note (a bit a group) and end as NaN.
 // Every wait is bounded; one that runs out records a code in the device status word, and the block ends without results, once the products that it asked for are through.
 // What bounds it.  A block alone on an SM (204 KB) gets through 256 rows by 64 keys in 1.46 us for heads of 128 (838 TFLOP/s over 148 SMs; 0.51 of cuBLAS's burst) and 1.30 for heads of 64 (469): its
@@ -43,6 +44,7 @@ constexpr int kSoftmaxRegs = 80, kMakerRegs = 72, kIssuerRegs = 40;
 constexpr int kSub = 128 * 128;                // [128 rows][128 bytes]: 64 values of a tile
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr float kSlack = 8.0f, kLeastExponent = -100.0f;
+constexpr float kUp = 7.0f;                    // p is 2^(S - m + kUp), up to 2^(kUp + kSlack) of float16's 2^16
 
 struct Control {
     uint64_t q_full;
@@ -637,7 +639,7 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
             uint32_t pk[16];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float less = fmaxf((half == 0 ? e0 : e1) - big, -60.0f), from = less - m, factor = half == 0 ? f0 : f1;
+                const float less = fmaxf((half == 0 ? e0 : e1) - big, -60.0f), from = less - m + kUp, factor = half == 0 ? f0 : f1;
                 float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
@@ -675,9 +677,9 @@ attention4_many_kernel(const Call c, int n_splits, int share, int* status) {
             // A row's result; where blocks share its keys a state, normed so that its sum is 1.  (Rows whose keys are one block's share have none.)
             const bool none = l == 0.0f, whole = ctl->whole != 0;                          // no key seen: O may be what the memory held
             float* state = c.partial + ((((int64_t)seq * kv + kvh) * c.max_rows + row) * n_splits + split) * (HD + 4);
-            if (!whole && there && x == 0) *reinterpret_cast<float4*>(state) = make_float4(none ? kLowest : m + log2f(l), none ? 0.0f : 1.0f, 0.0f, 0.0f);
+            if (!whole && there && x == 0) *reinterpret_cast<float4*>(state) = make_float4(none ? kLowest : m - kUp + log2f(l), none ? 0.0f : 1.0f, 0.0f, 0.0f);
             float factor = 1.0f;
-            if (whole && c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m, l);
+            if (whole && c.sink != nullptr) factor = lb_sink_join_exp2(c.sink[head] * kLbLog2e, m - kUp, l);
             factor = factor / l * ex2(big * 0.5f);
             const float factor2 = ex2(big * 0.5f - 8.0f);                 // in two steps: big may be 2^127's exponent
             __nv_bfloat16* out = c.out + (int64_t)(part.first + token) * c.out_stride + (int64_t)head * HD + x * (HD / 2);

@@ -9,7 +9,7 @@ import torch
 
 from liyab_b200 import ops
 from test_cache4 import _call
-from test_cache4_gpu import BF16, FORMS, Filled, _attention, _close, _decode, _portions, _queries, _slots, _values_as_rows
+from test_cache4_gpu import BF16, FORMS, Filled, _attention, _close, _decode, _portions, _queries, _rounded, _slots, _values, _values_as_rows
 from test_kernels_gpu import dev  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -243,3 +243,31 @@ def test_weights_in_memory_that_is_shared(dev):  # noqa: F811
         with pytest.raises(LiyabError):
             bad()
     assert torch.equal(wide, before) and not shared.any()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 32)])
+@pytest.mark.parametrize("requests,new", [(1, 1), (160, 1), (160, 16)])
+def test_a_key_of_little_value_that_takes_most_weight(dev, dim, group, requests, new):  # noqa: F811
+    """The first key takes most of the weight and has values of zero; what comes out is made of 2^17 equal weights of 2^-20.5 of its: they do not lose bits beside it, in the kernels for few rows and for many.
+    (Requests over the same pages, so many that none shares its keys out.)"""
+    n, heads = 1 << 17, 16
+    f = Filled(dev, [16], 1, dim, group, 128, seed=1, extra=n // 128)
+    table = torch.cat([f.table[0], f.spare.to(dev)])[None, :n // 128].expand(requests, -1).contiguous()
+    k, v = torch.zeros(n, dim, device=dev), torch.ones(n, dim, device=dev)
+    k[1:, 0], v[0] = -7.109375, 0.0
+    slot = torch.arange(n, device=dev)
+    ops.append4(k, v, (table[0, slot // 128] * 128 + slot % 128).to(torch.int32), f.cache, n)
+    (kn, ks), (vn, vs) = _rounded(k, 1, dim, group), _rounded(v, 1, dim, group)
+    q = torch.zeros(requests * new, heads * dim, dtype=BF16, device=dev)
+    q.view(-1, heads, dim)[:, :, 0] = 16.0
+    out, past = torch.empty_like(q), torch.full((requests,), n - new, dtype=torch.int32, device=dev)
+    f.table = table
+    if new == 1:
+        ops.decode_attention4(q, f.cache, past, table, out, requests, heads, 0.125)
+    else:
+        assert _shared(f, requests, heads, new) is None
+        ops.prefill_attention4(q, f.cache, torch.arange(0, requests * new + 1, new, dtype=torch.int32, device=dev), past, table, out, requests, new, heads, 0.125)
+    want, _, bound, _ = _attention(q[:1].view(1, heads, dim), _values(kn, ks, group), _values(vn, vs, group), torch.tensor([n - new], device=dev), 0.125)
+    assert 0.05 < want.min() and want.max() < 0.1
+    _close(out[::new][:1].view(1, heads, dim), want, bound)
+    assert torch.equal(out[::new], out[:1].expand(requests, -1))
